@@ -17,6 +17,7 @@ i64 = ctypes.c_int64
 u64 = ctypes.c_uint64
 f32 = ctypes.c_float
 f64 = ctypes.c_double
+sz = ctypes.c_size_t
 vp = ctypes.c_void_p
 P = ctypes.POINTER
 
@@ -107,6 +108,11 @@ STREAM_READ = 0                        # sporder_stream_op_t
 STREAM_WRITE = 1
 STREAM_COPY = 2
 
+TYPE_F32 = 0                           # sporder_type_t
+TYPE_BF16 = 1
+TYPE_F16 = 2
+OK = 0                                 # SPORDER_OK
+
 # Every symbol include/sporder.h declares, with its ctypes signature.
 SIGNATURES = {
     "sporder_context_create": ([], vp),
@@ -132,6 +138,14 @@ SIGNATURES = {
     "sporder_spmm_plan_create": ([vp, i32, i32, vp, vp, P(SpmmPlanInfo)], vp),
     "sporder_spmm_plan_destroy": ([vp], None),
     "sporder_spmm_csr_plan": ([vp, vp, i32, i32, vp, vp, vp, i32, vp, vp, P(f32)], None),
+    "sporder_embedding": ([vp, i32, i64, i64, i64, vp, i64, i32, vp, f32, i64, vp], i32),
+    "sporder_embedding_grad_work_bytes": ([i64, i64, i64], sz),
+    "sporder_embedding_grad": (
+        [vp, i32, i64, i64, i64, vp, i32, vp, f32, i64, i64, i32, i64, vp, vp, sz], i32),
+    "sporder_layer_norm": ([vp, i32, i32, i64, i64, i64, vp, vp, vp, f32, i64, vp, vp, vp], i32),
+    "sporder_layer_norm_grad_work_bytes": ([i64, i64], sz),
+    "sporder_layer_norm_grad": (
+        [vp, i32, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, sz], i32),
     "sporder_hbm_stream": ([vp, i32, i32, vp, vp, ctypes.c_int64, i32, P(f32)], None),
 }
 

@@ -1,0 +1,103 @@
+// dense.hpp -- pieces shared by the training operators (layer_norm.hip,
+// embedding.hip, newton_schulz.hip): element types, vector access, sums over
+// lane groups and the status codes of their C entries.
+//
+// These entries differ from the rest of the library: they run on the caller's
+// stream, return before the work is done, take their scratch from the caller
+// and report errors by a return code, because a training step makes them
+// many times between two products and reads their results on the same stream.
+#pragma once
+
+#include <initializer_list>
+#include <tuple>
+#include <type_traits>
+
+#include "common.hpp"
+
+namespace sporder_hip {
+
+using bf16_t = __bf16;
+using f16_t = _Float16;
+
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack {
+  T v[VEC];
+};
+
+template <int VEC, typename T>
+__device__ __forceinline__ void load_f32(const T *p, float (&out)[VEC]) {
+  const Pack<T, VEC> q = *reinterpret_cast<const Pack<T, VEC> *>(p);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) out[i] = static_cast<float>(q.v[i]);
+}
+
+template <int VEC, typename T>
+__device__ __forceinline__ void store_f32(T *p, const float (&in)[VEC]) {
+  Pack<T, VEC> q;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) q.v[i] = static_cast<T>(in[i]);
+  *reinterpret_cast<Pack<T, VEC> *>(p) = q;
+}
+
+// Element i of a vector whose type is known at run time.
+__device__ __forceinline__ float load_typed(const void *p, int type, int64_t i) {
+  if (type == SPORDER_TYPE_BF16) return static_cast<float>(static_cast<const bf16_t *>(p)[i]);
+  if (type == SPORDER_TYPE_F16) return static_cast<float>(static_cast<const f16_t *>(p)[i]);
+  return static_cast<const float *>(p)[i];
+}
+__device__ __forceinline__ void store_typed(void *p, int type, int64_t i, float v) {
+  if (type == SPORDER_TYPE_BF16)
+    static_cast<bf16_t *>(p)[i] = static_cast<bf16_t>(v);
+  else if (type == SPORDER_TYPE_F16)
+    static_cast<f16_t *>(p)[i] = static_cast<f16_t>(v);
+  else
+    static_cast<float *>(p)[i] = v;
+}
+
+// Sum over aligned groups of L lanes (a power of two up to 64), in every lane.
+template <int L> __device__ __forceinline__ float group_sum(float v) {
+#pragma unroll
+  for (int j = 1; j < L; j <<= 1) v += lane_xor_f32(v, j);
+  return v;
+}
+
+constexpr bool type_known(int32_t t) { return t >= SPORDER_TYPE_F32 && t <= SPORDER_TYPE_F16; }
+constexpr int type_bytes(int32_t t) { return t == SPORDER_TYPE_F32 ? 4 : 2; }
+
+// Queues a kernel and tells its own status: hipGetLastError would also report
+// an error that some earlier call of the caller's left behind.
+template <typename... P, typename... A>
+inline int32_t launch(void (*kernel)(P...), dim3 grid, dim3 block, void *stream, A... args) {
+  std::tuple<P...> held(static_cast<P>(args)...);
+  const hipError_t err = std::apply(
+      [&](P &...a) {
+        void *list[] = {static_cast<void *>(&a)...};
+        return hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, list, 0,
+                               static_cast<hipStream_t>(stream));
+      },
+      held);
+  if (err == hipSuccess) return SPORDER_OK;
+  (void)hipGetLastError(); // reported here, so not left for the caller's next check
+  return SPORDER_LAUNCH_FAILED;
+}
+
+inline bool aligned_to(const void *p, size_t bytes) {
+  return reinterpret_cast<uintptr_t>(p) % bytes == 0;
+}
+
+constexpr int64_t kMostDim = int64_t(1) << 23; // elements of a row
+
+// Elements per access of rows whose wider type has `bytes_each` bytes: 16
+// bytes, or 4 elements, where the length, the strides and the bases allow it,
+// else one element.
+inline int row_vec(int bytes_each, int64_t dim, std::initializer_list<int64_t> strides,
+                   std::initializer_list<const void *> bases) {
+  for (int vec : {16 / bytes_each, 4}) {
+    bool ok = dim % vec == 0;
+    for (int64_t s : strides) ok = ok && s % vec == 0;
+    for (const void *p : bases) ok = ok && aligned_to(p, static_cast<size_t>(vec) * bytes_each);
+    if (ok) return vec;
+  }
+  return 1;
+}
+
+} // namespace sporder_hip

@@ -1,0 +1,240 @@
+"""Operators of a training step around the SpMM: row lookup, layer norm and
+the orthogonalisation of a weight's update, each with what its backward pass
+needs.  They have no counterpart in the reference.
+
+Unlike the rest of the package they run on torch's current stream of the
+input's device and return without waiting, so they follow and precede torch
+operations on that stream and can be captured into a graph.  Outputs and
+scratch come from torch's allocator.  They take no Context.  Inputs are torch
+GPU tensors, or DLPack-capable GPU arrays.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _lib
+from ._sporder import _as_tensor
+
+_TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16,
+          torch.float16: _lib.TYPE_F16}
+_TOKEN_BITS = {torch.int32: 32, torch.int64: 64}
+
+
+def _floats(a, name):
+    t = _as_tensor(a, name)
+    if not t.is_cuda:
+        raise TypeError(f"{name} must be a GPU tensor")
+    if t.dtype not in _TYPES:
+        raise TypeError(f"{name} must be float32, bfloat16 or float16, got {t.dtype}")
+    return t
+
+
+def _token_ids(a, ref):
+    t = _as_tensor(a, "tokens")
+    if not t.is_cuda:
+        raise TypeError("tokens must be a GPU tensor")
+    if t.dtype not in _TOKEN_BITS:
+        raise TypeError(f"tokens must be int32 or int64, got {t.dtype}")
+    _same_device(t, ref, "tokens")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _same_device(t, ref, name):
+    if t.device != ref.device:
+        raise ValueError(f"{name} lives on {t.device}, expected {ref.device}")
+
+
+def _rows(t):
+    """(tensor, rows, stride): `t` as rows of its last dimension a fixed number
+    of elements apart, copied only where its strides allow no such view."""
+    dim = t.shape[-1]
+    if t.is_contiguous():
+        return t, t.numel() // dim, dim
+    if t.dim() == 2 and (t.stride(1) == 1 or dim == 1):
+        return t, t.shape[0], t.stride(0)
+    t = t.contiguous()
+    return t, t.numel() // dim, dim
+
+
+def _out(out, shape, dtype, ref):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=ref.device)
+    if (not isinstance(out, torch.Tensor) or out.shape != torch.Size(shape) or out.dtype != dtype
+            or out.device != ref.device or not out.is_contiguous()):
+        raise ValueError(f"out must be a contiguous {dtype} tensor of shape {tuple(shape)} on "
+                         f"{ref.device}")
+    return out
+
+
+def _call(name, ref, *args):
+    """Queues a C entry on the current stream of ref's device."""
+    device = ref.device
+    fn = getattr(_lib.load(), name)
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device.index == torch.cuda.current_device():
+        rc = fn(stream, *args)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(stream, *args)
+    if rc != _lib.OK:
+        raise RuntimeError(f"{name} returned {rc}")
+
+
+def embedding(table, tokens, *, scale=1.0, out=None):
+    """Rows of a table by token: out[..., :] = scale * table[tokens[...]].
+
+    Arguments:
+        table: (rows, dim) float32, bfloat16 or float16; unit stride along dim
+        tokens: int32 or int64 ids of any shape
+        scale: factor applied in 32 bits before the one rounding to the type
+        out: contiguous tensor of shape tokens.shape + (dim,), or None
+
+    A token outside [0, rows) gives a row of NaN.  Returns out.
+    """
+    table = _floats(table, "table")
+    if table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1:
+        raise ValueError("table must be a (rows, dim) tensor of at least one element")
+    tokens = _token_ids(tokens, table)
+    rows, dim = table.shape
+    out = _out(out, (*tokens.shape, dim), table.dtype, table)
+    table, _, stride = _rows(table)
+    _call("sporder_embedding", table, _TYPES[table.dtype], rows, dim, stride, table.data_ptr(),
+          tokens.numel(), _TOKEN_BITS[tokens.dtype], tokens.data_ptr(), float(scale), dim,
+          out.data_ptr())
+    return out
+
+
+def embedding_grad(grad, tokens, num_rows, *, scale=1.0, padding_idx=None, dtype=None, out=None):
+    """Gradient of :func:`embedding` by its table, dense:
+    out[v] = scale * sum of grad[t] over the tokens equal to v.
+
+    Arguments:
+        grad: tokens.shape + (dim,), float32, bfloat16 or float16
+        tokens: int32 or int64 ids; ids outside [0, num_rows) are left out
+        num_rows: rows of the table
+        padding_idx: a row that gets no gradient, or None
+        dtype: grad's type (default) or float32, the type of the result
+        out: contiguous (num_rows, dim) tensor of that type, or None
+
+    The sums are held in 32 bits, their order depends on the tokens alone (the
+    result is the same bit for bit from run to run), and every row is written.
+    Returns out.
+    """
+    grad = _floats(grad, "grad")
+    tokens = _token_ids(tokens, grad)
+    if grad.dim() < 1 or grad.shape[:-1] != tokens.shape or grad.shape[-1] < 1:
+        raise ValueError("grad must have the tokens' shape and one more dimension")
+    num_rows = int(num_rows)
+    if not 1 <= num_rows <= 2**31 - 2:
+        raise ValueError("num_rows must be in [1, 2^31 - 2]")
+    if dtype is None:
+        dtype = grad.dtype
+    elif dtype not in (grad.dtype, torch.float32):
+        raise ValueError("dtype must be grad's type or float32")
+    dim = grad.shape[-1]
+    count = tokens.numel()
+    out = _out(out, (num_rows, dim), dtype, grad)
+    grad, _, stride = _rows(grad)
+    size = _lib.load().sporder_embedding_grad_work_bytes(count, num_rows, dim)
+    work = torch.empty(size, dtype=torch.uint8, device=grad.device)
+    _call("sporder_embedding_grad", grad, _TYPES[grad.dtype], count, dim, stride, grad.data_ptr(),
+          _TOKEN_BITS[tokens.dtype], tokens.data_ptr(), float(scale),
+          -1 if padding_idx is None else int(padding_idx), num_rows, _TYPES[dtype], dim,
+          out.data_ptr(), work.data_ptr(), size)
+    return out
+
+
+def _norm_vector(a, name, dim, ref):
+    t = _floats(a, name)
+    if t.dtype not in (ref.dtype, torch.float32):
+        raise TypeError(f"{name} must have x's type or float32, got {t.dtype}")
+    if t.dim() != 1 or t.shape[0] != dim:
+        raise ValueError(f"{name} must have shape ({dim},)")
+    _same_device(t, ref, name)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None):
+    """Layer norm over the last dimension:
+    y = (x - mean) * rstd * weight + bias, rstd = (var + eps)^-1/2.
+
+    Arguments:
+        x: (..., dim) float32, bfloat16 or float16; rows a fixed number of
+            elements apart are read in place, other strides are copied
+        weight, bias: (dim,) of x's type or float32 (both of one type), or None
+        eps: >= 0
+        out: contiguous tensor of x's shape and type, or None; may be x
+
+    Returns (y, mean, rstd); mean and rstd are float32 of shape x.shape[:-1],
+    as :func:`layer_norm_grad` takes them.
+    """
+    x = _floats(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have a last dimension of at least one element")
+    if not eps >= 0.0:
+        raise ValueError("eps must be >= 0")
+    dim = x.shape[-1]
+    if weight is not None:
+        weight = _norm_vector(weight, "weight", dim, x)
+    if bias is not None:
+        bias = _norm_vector(bias, "bias", dim, x)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise TypeError("weight and bias must have the same type")
+    y = _out(out, x.shape, x.dtype, x)
+    mean = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    rstd = torch.empty_like(mean)
+    given = weight if weight is not None else bias
+    x, rows, stride = _rows(x)
+    _call("sporder_layer_norm", x, _TYPES[x.dtype],
+          _lib.TYPE_F32 if given is None else _TYPES[given.dtype], rows, dim, stride,
+          x.data_ptr(), 0 if weight is None else weight.data_ptr(),
+          0 if bias is None else bias.data_ptr(), eps, dim, y.data_ptr(), mean.data_ptr(),
+          rstd.data_ptr())
+    return y, mean, rstd
+
+
+def layer_norm_grad(grad, x, mean, rstd, weight=None):
+    """Gradients of :func:`layer_norm`.
+
+    Arguments:
+        grad, x: the gradient by y and the forward call's x, of one shape and
+            type
+        mean, rstd: as the forward call returned them
+        weight: as in the forward call
+
+    Returns (dx, dweight, dbias): dx of x's type; dweight and dbias of
+    weight's type (float32 without a weight), summed over all rows in 32 bits
+    in an order that depends on the sizes alone.
+    """
+    x = _floats(x, "x")
+    grad = _floats(grad, "grad")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have a last dimension of at least one element")
+    if grad.shape != x.shape:
+        raise ValueError("grad must have x's shape")
+    if grad.dtype != x.dtype:
+        raise TypeError("grad must have x's type")
+    _same_device(grad, x, "grad")
+    dim = x.shape[-1]
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 \
+                or t.shape != x.shape[:-1] or t.device != x.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be the contiguous float32 tensor that layer_norm "
+                             f"returned, of shape {tuple(x.shape[:-1])} on {x.device}")
+    dtype = torch.float32
+    if weight is not None:
+        weight = _norm_vector(weight, "weight", dim, x)
+        dtype = weight.dtype
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    dweight = torch.empty(dim, dtype=dtype, device=x.device)
+    dbias = torch.empty(dim, dtype=dtype, device=x.device)
+    x, rows, stride = _rows(x)
+    grad, _, grad_stride = _rows(grad)
+    size = _lib.load().sporder_layer_norm_grad_work_bytes(rows, dim)
+    work = torch.empty(size, dtype=torch.uint8, device=x.device)
+    _call("sporder_layer_norm_grad", x, _TYPES[x.dtype], _TYPES[dtype], rows, dim, grad_stride,
+          grad.data_ptr(), stride, x.data_ptr(), mean.data_ptr(), rstd.data_ptr(),
+          0 if weight is None else weight.data_ptr(), dim, dx.data_ptr(), dweight.data_ptr(),
+          dbias.data_ptr(), work.data_ptr(), size)
+    return dx, dweight, dbias

@@ -11,7 +11,8 @@
  * (nanobind, ctypes, cgo, ...) links against this library unchanged.  Entry
  * points marked "(new)" have no counterpart there.
  *
- * Conventions shared by every entry point (reference sporder.h:13-41):
+ * Conventions shared by every entry point (reference sporder.h:13-41) except
+ * the training operators at the end, which state their own:
  *   - Synchronous: calls return only after device outputs and host
  *     out-parameters are ready.
  *   - d_-prefixed pointers are device memory on the context's device; all
@@ -31,6 +32,7 @@
  */
 
 #include <stdbool.h>
+#include <stddef.h>
 #include <stdint.h>
 
 #define SPORDER_API __attribute__((visibility("default")))
@@ -415,6 +417,87 @@ SPORDER_API int32_t sporder_spmm_csr_noalloc(sporder_context_t ctx, int32_t n,
                                              int32_t nnz, const int32_t *d_ptr,
                                              const int32_t *d_ind, const float *d_val,
                                              int32_t cols, const float *d_b, float *d_c);
+
+/*
+ * (new) Operators of a training step around the SpMM: row lookup, layer norm
+ * and the orthogonalisation of a weight's update.  They have no counterpart in
+ * the reference, whose GCN driver (experiments/e2e_gcn.py:107-133) trains two
+ * linear layers on given features with torch's optimiser.
+ *
+ * Unlike the entries above they are stream-ordered: `stream` is a hipStream_t
+ * of the device current at the call (NULL: its default stream), the work is
+ * queued there and the call returns without waiting, so a step's calls follow
+ * one another and can be recorded into a HIP graph.  They need no context,
+ * allocate nothing (d_work is the caller's, of the size the matching
+ * *_work_bytes function names) and return a code instead of aborting:
+ *   SPORDER_OK             queued (or nothing to do)
+ *   SPORDER_BAD_ARGUMENT   nothing queued
+ *   SPORDER_LAUNCH_FAILED  HIP refused a launch
+ * `type` arguments are sporder_type_t.  Sums are held in 32 bits whatever the
+ * type and results are rounded to it once, at the end; every result is the
+ * same bit for bit from run to run.
+ */
+typedef enum {
+  SPORDER_TYPE_F32 = 0,
+  SPORDER_TYPE_BF16 = 1,
+  SPORDER_TYPE_F16 = 2
+} sporder_type_t;
+#define SPORDER_OK 0
+#define SPORDER_BAD_ARGUMENT 2
+#define SPORDER_LAUNCH_FAILED 3
+
+/*
+ * d_out[t] = scale d_table[d_tokens[t]] for `count` tokens of token_bits (32
+ * or 64, signed) bits; rows of `dim` elements of `type`, table_stride and
+ * out_stride elements apart.  A token outside [0, rows) gives a row of NaN.
+ */
+SPORDER_API int32_t sporder_embedding(void *stream, int32_t type, int64_t rows, int64_t dim,
+                                      int64_t table_stride, const void *d_table, int64_t count,
+                                      int32_t token_bits, const void *d_tokens, float scale,
+                                      int64_t out_stride, void *d_out);
+
+/*
+ * Its gradient by the table: d_out[v] = scale * sum of d_grad[t] over the t
+ * with d_tokens[t] = v, summed in the order of t within groups whose sizes
+ * depend on the tokens alone, for each of `rows` rows (0 where there is no
+ * such t).  Tokens equal to padding_idx and tokens outside [0, rows) are left
+ * out.  out_type is `type` or SPORDER_TYPE_F32.  d_work is 256-byte aligned.
+ */
+SPORDER_API size_t sporder_embedding_grad_work_bytes(int64_t count, int64_t rows, int64_t dim);
+SPORDER_API int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count,
+                                           int64_t dim, int64_t grad_stride,
+                                           const void *d_grad, int32_t token_bits,
+                                           const void *d_tokens, float scale,
+                                           int64_t padding_idx, int64_t rows, int32_t out_type,
+                                           int64_t out_stride, void *d_out, void *d_work,
+                                           size_t work_bytes);
+
+/*
+ * y = weight (x - mean) rstd + bias for each of `rows` rows of `dim` elements,
+ * mean and var = sum (x - mean)^2 / dim over the row, rstd = (var + eps)^-1/2.
+ * Rows of x and y start x_stride and y_stride elements apart; d_weight and
+ * d_bias (dim elements of weight_type) may be NULL (1 and 0); d_mean and
+ * d_rstd receive `rows` floats.  d_y may be d_x.
+ */
+SPORDER_API int32_t sporder_layer_norm(void *stream, int32_t type, int32_t weight_type,
+                                       int64_t rows, int64_t dim, int64_t x_stride,
+                                       const void *d_x, const void *d_weight,
+                                       const void *d_bias, float eps, int64_t y_stride,
+                                       void *d_y, float *d_mean, float *d_rstd);
+
+/*
+ * Its gradients from dy and the forward call's mean and rstd: d_dx (rows of
+ * dim elements, dx_stride apart), and, where not NULL, d_dweight and d_dbias
+ * (dim elements of weight_type, summed over the rows).  d_dx may be d_dy.
+ */
+SPORDER_API size_t sporder_layer_norm_grad_work_bytes(int64_t rows, int64_t dim);
+SPORDER_API int32_t sporder_layer_norm_grad(void *stream, int32_t type, int32_t weight_type,
+                                            int64_t rows, int64_t dim, int64_t dy_stride,
+                                            const void *d_dy, int64_t x_stride,
+                                            const void *d_x, const float *d_mean,
+                                            const float *d_rstd, const void *d_weight,
+                                            int64_t dx_stride, void *d_dx, void *d_dweight,
+                                            void *d_dbias, void *d_work, size_t work_bytes);
 
 #ifdef __cplusplus
 }

@@ -4,20 +4,21 @@
 //   dtable[v] = scale sum of grad[t] over the t with tokens[t] = v
 //
 // Both move memory and compute next to nothing.  The gradient is a sum over
-// equal tokens in the order of t, in 32 bits, written once for every row of
-// the table (zero rows too).  Atomic additions would be one launch, but their
-// order, and with it the result, changes from run to run and a common token
-// serialises them, so the tokens are sorted instead, as far as the sums need
-// it and in two launches:
+// equal tokens in 32 bits, written once for every row of the table (zero rows
+// too).  Atomic additions would be one launch, but their order, and with it
+// the result, changes from run to run and a common token serialises them, so
+// the tokens are sorted instead, as far as the sums need it:
 //
 //   1. each tile of 4096 tokens is sorted in LDS (stable), and the table's
-//      rows, cut into spans, find where their tokens begin in it.  64
-//      neighbours of one token in that order (a common token: a hub, padding
-//      that is not left out) become one entry,
-//   2. whose sum a wave forms;
+//      rows, cut into spans, find where their tokens begin in it.  16 to 64
+//      neighbours of one token in that order (a common token: a hub) become
+//      one entry,
+//   2. whose sum a group of lanes forms;
 //   3. a workgroup per span gathers its entries from every tile, in the
-//      tiles' order, which is the order of t, sorts them by row in LDS and
-//      adds up and writes each row.
+//      tiles' order, sorts them by row in LDS and adds up and writes each row.
+//
+// A few tokens need no tiles: each span picks its own from all of them, in
+// one launch.
 #include <algorithm>
 
 #include "dense.hpp"
@@ -70,11 +71,15 @@ constexpr int kTile = 4096;       // tokens sorted by one workgroup
 constexpr int kTileBlock = 1024;
 constexpr int kTileWaves = kTileBlock / kWave;
 constexpr int kTileRounds = kTile / kTileBlock;
-constexpr int kChunk = kWave;     // sorted neighbours that may become one entry
+constexpr int kChunk = kWave;     // sorted neighbours looked at together
 constexpr int kTileChunks = kTile / kChunk;
-constexpr uint32_t kSummed = 0x80000000u; // an entry that is a chunk's sum
+constexpr int kRun = 16;          // equal tokens of a chunk that become one entry
+constexpr int kChunkRuns = kChunk / kRun;
+constexpr int kTileRuns = kTileChunks * kChunkRuns;
+constexpr uint32_t kSummed = 0x80000000u; // an entry that is a run's sum
 constexpr int kSpanMost = 256;    // table rows per span
-constexpr int kListMost = 4096;   // a span's entries that fit the list in LDS
+constexpr int kListMost = 2048;   // a span's entries that fit the list in LDS
+constexpr int kAlone = 32;        // entries of a row that one group of lanes adds up
 
 struct GradArgs {
   const void *grad, *tokens;
@@ -85,14 +90,20 @@ struct GradArgs {
   int key_bits;
   int span;      // table rows per workgroup of the last launch
   int64_t spans; // ceil(rows / span)
-  int64_t tiles;
+  int64_t tiles; // 0: spans read the tokens themselves
   uint32_t *keys;      // [tiles][kTile] the tiles' entries: row,
-  uint32_t *sources;   // and token index, or chunk index | kSummed
+  uint32_t *sources;   // and token index, or run index | kSummed
   uint16_t *order;     // [tiles][kTile] the sorted order within the tile
-  uint64_t *uniform;   // [tiles] chunks that are one entry
+  uint16_t *runs;      // [tiles][kTileRuns] first place in the chunk and length; 0: none
   uint16_t *starts;    // [tiles][spans + 1] first entry of each span
-  float *sums;         // [tiles * kTileChunks][dim]
+  float *sums;         // [tiles * kTileRuns][dim]
 };
+
+// The table row of token i, or `rows` (none) for padding and ids outside.
+__device__ __forceinline__ uint32_t token_row(const GradArgs &a, int64_t i) {
+  const int64_t t = token_at(a.tokens, a.wide, i);
+  return static_cast<uint32_t>(t >= 0 && t < a.rows && t != a.padding ? t : a.rows);
+}
 
 // Peers of this lane: the lanes whose `bits` low bits of `digit` equal its own.
 __device__ __forceinline__ uint64_t match_lanes(uint32_t digit, int bits) {
@@ -113,20 +124,16 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
   __shared__ uint16_t idx[2][kTile];
   __shared__ uint16_t cnt[kTileWaves][kDigits];
   __shared__ int wave_total[kTileWaves];
-  __shared__ int chunk_size[kTileChunks];
+  __shared__ int chunk_entries[kTileChunks];
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
   const uint64_t below = (uint64_t(1) << lane) - 1;
   const int64_t tile = blockIdx.x, base = tile * kTile;
+  const uint32_t none = static_cast<uint32_t>(a.rows); // sorted last, dropped
 
 #pragma unroll
   for (int r = 0; r < kTileRounds; ++r) {
     const int i = r * kTileBlock + tid;
-    uint32_t k = static_cast<uint32_t>(a.rows); // no row: sorted last, dropped
-    if (base + i < a.count) {
-      const int64_t t = token_at(a.tokens, a.wide, base + i);
-      if (t >= 0 && t < a.rows && t != a.padding) k = static_cast<uint32_t>(t);
-    }
-    key[0][i] = k;
+    key[0][i] = base + i < a.count ? token_row(a, base + i) : none;
     idx[0][i] = static_cast<uint16_t>(i);
   }
   __syncthreads();
@@ -180,37 +187,47 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
     __syncthreads();
   }
 
-  // Entries: a chunk of one row is one, any other chunk its tokens.
-  const uint32_t none = static_cast<uint32_t>(a.rows);
+  // Entries: a run of kRun or more equal rows within a chunk is one, held by
+  // the run's first lane; every other token is its own.
+  uint64_t held[kTileRounds]; // lanes that hold an entry
+  uint64_t heads[kTileRounds]; // of them, those whose entry is a run
 #pragma unroll
   for (int r = 0; r < kTileRounds; ++r) {
     const int chunk = wave * kTileRounds + r;
     const uint32_t k = key[from][chunk * kChunk + lane];
-    const bool one = ballot(k == static_cast<uint32_t>(readlane(k, 0))) == ~uint64_t(0);
-    const int valid = __popcll(ballot(k != none));
-    if (lane == 0) chunk_size[chunk] = one && valid ? -1 : valid;
+    const uint32_t before = __shfl_up(k, 1);
+    const uint64_t first = ballot(lane == 0 || k != before); // of each run
+    const int begin = 63 - __clzll(first & (below | (uint64_t(1) << lane)));
+    const uint64_t above = lane == 63 ? 0 : first >> (lane + 1);
+    const int end = above ? lane + 1 + __builtin_ctzll(above) : kChunk;
+    const bool run = k != none && end - begin >= kRun;
+    heads[r] = ballot(run && lane == begin);
+    held[r] = ballot(k != none && (!run || lane == begin));
+    if (lane == 0) chunk_entries[chunk] = __popcll(held[r]);
     a.order[base + chunk * kChunk + lane] = idx[from][chunk * kChunk + lane];
+    uint16_t *const runs = a.runs + tile * kTileRuns + chunk * kChunkRuns;
+    if (run && lane == begin)
+      runs[__popcll(heads[r] & below)] = static_cast<uint16_t>(begin << 8 | (end - begin));
+    if (lane < kChunkRuns && lane >= __popcll(heads[r])) runs[lane] = 0;
   }
   __syncthreads();
-  const int mine = chunk_size[lane]; // kTileChunks = kWave: every wave holds all of them
-  const int place = wave_incl_scan(mine < 0 ? 1 : mine) - (mine < 0 ? 1 : mine);
-  const int entries = wave_sum(mine < 0 ? 1 : mine);
-  const uint64_t uniform = ballot(mine < 0);
-  if (tid == 0) a.uniform[tile] = uniform;
+  const int mine = chunk_entries[lane]; // kTileChunks = kWave: every wave holds all of them
+  const int place = wave_incl_scan(mine) - mine;
+  const int entries = wave_sum(mine);
   const int to = from ^ 1;
 #pragma unroll
   for (int r = 0; r < kTileRounds; ++r) {
     const int chunk = wave * kTileRounds + r;
-    const uint32_t k = key[from][chunk * kChunk + lane];
-    const uint32_t i = idx[from][chunk * kChunk + lane];
-    const int at = readlane(place, chunk);
-    const bool one = (uniform >> chunk) & 1;
-    if (one ? lane == 0 : k != none) {
-      key[to][at + lane] = k;
-      a.keys[base + at + lane] = k;
-      a.sources[base + at + lane] =
-          one ? kSummed | static_cast<uint32_t>(tile * kTileChunks + chunk)
-              : static_cast<uint32_t>(base + i);
+    if ((held[r] >> lane) & 1) {
+      const uint32_t k = key[from][chunk * kChunk + lane];
+      const int at = readlane(place, chunk) + __popcll(held[r] & below);
+      key[to][at] = k;
+      a.keys[base + at] = k;
+      a.sources[base + at] =
+          (heads[r] >> lane) & 1
+              ? kSummed | static_cast<uint32_t>(tile * kTileRuns + chunk * kChunkRuns +
+                                                __popcll(heads[r] & below))
+              : static_cast<uint32_t>(base + idx[from][chunk * kChunk + lane]);
     }
   }
   __syncthreads();
@@ -228,66 +245,81 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
   }
 }
 
-// The sums of the chunks that are one entry: a workgroup per chunk and slice
-// of columns, four waves over the slice's vectors.
-template <typename T, int VEC>
-__global__ void __launch_bounds__(256) embedding_chunk_kernel(GradArgs a) {
-  const int64_t tile = blockIdx.x / kTileChunks;
-  const int chunk = blockIdx.x % kTileChunks;
-  if (!((a.uniform[tile] >> chunk) & 1)) return;
-  __shared__ uint16_t place[kChunk];
-  if (threadIdx.x < kChunk) place[threadIdx.x] = a.order[tile * kTile + chunk * kChunk + threadIdx.x];
-  __syncthreads();
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * 256 + threadIdx.x) * VEC;
-  if (c >= a.dim) return;
-  const T *const grad = static_cast<const T *>(a.grad) + tile * kTile * a.grad_stride + c;
-  float acc[VEC] = {};
+// The sums of the runs, L lanes each.
+template <typename T, int VEC, int L>
+__global__ void __launch_bounds__(256) embedding_run_kernel(GradArgs a) {
+  const int64_t run = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
+  if (run >= a.tiles * kTileRuns) return;
+  const int what = a.runs[run];
+  if (what == 0) return;
+  const int64_t tile = run / kTileRuns;
+  const int n = what & 0xff;
+  const uint16_t *const order =
+      a.order + tile * kTile + run % kTileRuns / kChunkRuns * kChunk + (what >> 8);
+  const T *const grad = static_cast<const T *>(a.grad) + tile * kTile * a.grad_stride;
+  for (int64_t c = (threadIdx.x % L) * VEC; c < a.dim; c += L * VEC) {
+    float acc[VEC] = {};
 #pragma unroll 8
-  for (int i = 0; i < kChunk; ++i) {
+    for (int i = 0; i < n; ++i) {
+      float v[VEC];
+      load_f32<VEC>(grad + order[i] * a.grad_stride + c, v);
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+    }
+    store_f32<VEC>(a.sums + run * a.dim + c, acc);
+  }
+}
+
+// Adds rows base[at[i] & ~kSummed], i in [i, end), to acc.
+template <typename T, int VEC>
+__device__ __forceinline__ void add_rows(const T *base, int64_t stride, const uint32_t *at, int i,
+                                         int end, float (&acc)[VEC]) {
+#pragma unroll 8
+  for (; i < end; ++i) {
     float v[VEC];
-    load_f32<VEC>(grad + place[i] * a.grad_stride, v);
+    load_f32<VEC>(base + (at[i] & ~kSummed) * stride, v);
 #pragma unroll
     for (int k = 0; k < VEC; ++k) acc[k] += v[k];
   }
-  store_f32<VEC>(a.sums + static_cast<int64_t>(blockIdx.x) * a.dim + c, acc);
 }
 
-template <typename T, int VEC>
-__device__ __forceinline__ void add_entry(const GradArgs &a, uint32_t source, int64_t c,
-                                          float (&acc)[VEC]) {
-  float v[VEC];
-  if (source & kSummed)
-    load_f32<VEC>(a.sums + static_cast<int64_t>(source & ~kSummed) * a.dim + c, v);
-  else
-    load_f32<VEC>(static_cast<const T *>(a.grad) + source * a.grad_stride + c, v);
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] += v[k];
-}
-
-// One span of table rows.  L lanes per row.
+// One span of table rows, L lanes per row.  A row's entries are added in two
+// loops, the sums and the single tokens, so that several loads of each are
+// under way at once; a row of many entries (a hub) is shared by all the
+// groups of the workgroup, each a contiguous part, joined through LDS.
 template <typename T, typename O, int VEC, int L>
 __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
   constexpr int kGroups = 256 / L;
+  constexpr int kBins = 2 * kSpanMost; // sums of row r, tokens of row r
   __shared__ uint32_t source[kListMost];
   __shared__ uint32_t sorted[kListMost];
-  __shared__ uint8_t local[kListMost];
-  __shared__ int first[kSpanMost + 1];
-  __shared__ int next[kSpanMost];
+  __shared__ uint16_t local[kListMost];
+  __shared__ int first[kBins + 1];
+  __shared__ int next[kBins];
   __shared__ int wave_total[256 / kWave];
+  __shared__ float joined[kGroups][L * VEC];
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
+  const uint64_t below = (uint64_t(1) << lane) - 1;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.span;
   const int rows = static_cast<int>(min(static_cast<int64_t>(a.span), a.rows - row0));
   const uint16_t *const starts = a.starts + blockIdx.x;
 
-  // The entries, in the tiles' order.
-  for (int i = tid; i < kSpanMost; i += 256) next[i] = 0;
+  // The entries, in the tiles' order, or the tokens in theirs.
+  for (int i = tid; i < kBins; i += 256) next[i] = 0;
   int total = 0;
-  for (int64_t t0 = 0; t0 < a.tiles; t0 += 256) {
-    const int64_t tile = t0 + tid;
+  const int64_t items = a.tiles ? a.tiles : a.count;
+  for (int64_t i0 = 0; i0 < items; i0 += 256) {
+    const int64_t item = i0 + tid;
     int lo = 0, n = 0;
-    if (tile < a.tiles) {
-      lo = starts[tile * (a.spans + 1)];
-      n = starts[tile * (a.spans + 1) + 1] - lo;
+    uint32_t row = 0;
+    if (item < items) {
+      if (a.tiles) {
+        lo = starts[item * (a.spans + 1)];
+        n = starts[item * (a.spans + 1) + 1] - lo;
+      } else {
+        row = token_row(a, item);
+        n = row >= row0 && row < row0 + rows;
+      }
     }
     const int incl = wave_incl_scan(n);
     __syncthreads(); // the totals of the round before have been read
@@ -299,75 +331,115 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
       total += wave_total[w];
     }
     for (int i = 0; i < n && at + i < kListMost; ++i) {
-      const int64_t e = tile * kTile + lo + i;
-      const int r = static_cast<int>(a.keys[e] - row0);
-      source[at + i] = a.sources[e];
-      local[at + i] = static_cast<uint8_t>(r);
-      atomicAdd(&next[r], 1);
+      uint32_t what = static_cast<uint32_t>(item);
+      if (a.tiles) {
+        row = a.keys[item * kTile + lo + i];
+        what = a.sources[item * kTile + lo + i];
+      }
+      const int bin = 2 * static_cast<int>(row - row0) + ((what & kSummed) == 0);
+      source[at + i] = what;
+      local[at + i] = static_cast<uint16_t>(bin);
+      atomicAdd(&next[bin], 1);
     }
   }
   __syncthreads();
   const bool listed = total <= kListMost;
 
-  if (listed) {
-    // Stable counting sort by row: one wave places the list 64 at a time.
-    if (wave == 0) {
-      int carry = 0;
-      for (int r = lane; r < kSpanMost; r += kWave) {
-        const int n = next[r], incl = wave_incl_scan(n);
-        first[r] = carry + incl - n;
-        next[r] = carry + incl - n;
-        carry += readlane(incl, kWave - 1);
-      }
-      if (lane == 0) first[kSpanMost] = carry;
-      wave_lds_order();
-      const uint64_t below = (uint64_t(1) << lane) - 1;
-      for (int i0 = 0; i0 < total; i0 += kWave) {
-        const bool live = i0 + lane < total;
-        const uint32_t r = live ? local[i0 + lane] : 0;
-        const uint64_t peers = match_lanes(r, 8) & ballot(live);
-        if (live) {
-          const int at = next[r] + __popcll(peers & below);
-          sorted[at] = source[i0 + lane];
-          wave_lds_order();
-          if ((peers & below) == 0) next[r] = at + __popcll(peers);
-        }
-        wave_lds_order();
-      }
+  // Stable counting sort by bin: one wave places the list 64 at a time.
+  if (listed && wave == 0) {
+    int carry = 0;
+    for (int b = lane; b < kBins; b += kWave) {
+      const int n = next[b], incl = wave_incl_scan(n);
+      first[b] = next[b] = carry + incl - n;
+      carry += readlane(incl, kWave - 1);
     }
-    __syncthreads();
+    if (lane == 0) first[kBins] = carry;
+    wave_lds_order();
+    for (int i0 = 0; i0 < total; i0 += kWave) {
+      const bool live = i0 + lane < total;
+      const uint32_t bin = live ? local[i0 + lane] : 0;
+      const uint64_t peers = match_lanes(bin, 9) & ballot(live);
+      const int at = next[bin] + __popcll(peers & below);
+      wave_lds_order();
+      if (live) {
+        sorted[at] = source[i0 + lane];
+        if ((peers & below) == 0) next[bin] = at + __popcll(peers);
+      }
+      wave_lds_order();
+    }
   }
+  __syncthreads();
 
   const int group = tid / L;
-  for (int r = group; r < rows; r += kGroups) {
+  const T *const grad = static_cast<const T *>(a.grad);
+  for (int r = group; listed && r < rows; r += kGroups) {
+    const int sums = first[2 * r], singles = first[2 * r + 1], end = first[2 * r + 2];
+    if (end - sums > kAlone && kGroups > 1) continue;
     O *const out = static_cast<O *>(a.out) + (row0 + r) * a.out_stride;
     for (int64_t c = (tid % L) * VEC; c < a.dim; c += L * VEC) {
       float acc[VEC] = {};
-      if (listed) {
-        const int end = first[r + 1];
-#pragma unroll 4
-        for (int e = first[r]; e < end; ++e) add_entry<T, VEC>(a, sorted[e], c, acc);
-      } else {
-        for (int64_t tile = 0; tile < a.tiles; ++tile) {
-          const uint16_t *const s = starts + tile * (a.spans + 1);
-          const uint32_t *const keys = a.keys + tile * kTile;
-          const uint32_t row = static_cast<uint32_t>(row0 + r);
-          int lo = s[0], hi = s[1];
-          const int end = hi;
-          while (lo < hi) {
-            const int mid = (lo + hi) / 2;
-            if (keys[mid] < row)
-              lo = mid + 1;
-            else
-              hi = mid;
-          }
-          for (; lo < end && keys[lo] == row; ++lo)
-            add_entry<T, VEC>(a, a.sources[tile * kTile + lo], c, acc);
-        }
-      }
+      add_rows<float, VEC>(a.sums + c, a.dim, sorted, sums, singles, acc);
+      add_rows<T, VEC>(grad + c, a.grad_stride, sorted, singles, end, acc);
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[k] *= a.scale;
       store_f32<VEC>(out + c, acc);
+    }
+  }
+  if (listed && kGroups == 1) return;
+
+  // Rows of many entries; every row where the list was too long for LDS.
+  for (int r = 0; r < rows; ++r) {
+    const int sums = listed ? first[2 * r] : 0, singles = listed ? first[2 * r + 1] : 0;
+    const int end = listed ? first[2 * r + 2] : 0;
+    if (listed && end - sums <= kAlone) continue;
+    O *const out = static_cast<O *>(a.out) + (row0 + r) * a.out_stride;
+    for (int64_t c0 = 0; c0 < a.dim; c0 += L * VEC) {
+      const int64_t c = c0 + (tid % L) * VEC;
+      float acc[VEC] = {};
+      if (c < a.dim) {
+        if (listed) {
+          const int part = (end - sums + kGroups - 1) / kGroups;
+          const int from = min(sums + group * part, end), to = min(from + part, end);
+          add_rows<float, VEC>(a.sums + c, a.dim, sorted, from, min(to, singles), acc);
+          add_rows<T, VEC>(grad + c, a.grad_stride, sorted, max(from, singles), to, acc);
+        } else {
+          const int64_t part = ceil_div64(a.tiles, kGroups);
+          const int64_t last = min((group + 1) * part, a.tiles);
+          const uint32_t row = static_cast<uint32_t>(row0 + r);
+          for (int64_t tile = group * part; tile < last; ++tile) {
+            const uint32_t *const keys = a.keys + tile * kTile;
+            const uint32_t *const sources = a.sources + tile * kTile;
+            int lo = starts[tile * (a.spans + 1)];
+            const int stop = starts[tile * (a.spans + 1) + 1];
+            for (int hi = stop; lo < hi;) {
+              const int mid = (lo + hi) / 2;
+              if (keys[mid] < row)
+                lo = mid + 1;
+              else
+                hi = mid;
+            }
+            for (; lo < stop && keys[lo] == row; ++lo) {
+              if (sources[lo] & kSummed)
+                add_rows<float, VEC>(a.sums + c, a.dim, sources, lo, lo + 1, acc);
+              else
+                add_rows<T, VEC>(grad + c, a.grad_stride, sources, lo, lo + 1, acc);
+            }
+          }
+        }
+      }
+      __syncthreads(); // the columns before have been read
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) joined[group][(tid % L) * VEC + k] = acc[k];
+      __syncthreads();
+      if (group == 0 && c < a.dim) {
+        for (int g = 1; g < kGroups; ++g) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += joined[g][(tid % L) * VEC + k];
+        }
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] *= a.scale;
+        store_f32<VEC>(out + c, acc);
+      }
     }
   }
 }
@@ -400,51 +472,54 @@ template <typename T> int32_t lookup_typed(const LookupArgs &a, void *stream) {
 struct GradLayout {
   int span;
   int64_t spans, tiles;
-  size_t keys, sources, order, uniform, starts, sums, bytes;
+  size_t keys, sources, order, runs, starts, sums, bytes;
 };
 
 // Table rows per span: enough spans to fill the card several times over, and
-// at most kSpanMost rows each.
+// at most kSpanMost rows each.  Up to kListMost tokens fit every span's list
+// whole, and need no tiles.
 GradLayout grad_layout(int64_t count, int64_t rows, int64_t dim) {
   GradLayout l{};
   l.span = static_cast<int>(std::clamp<int64_t>(rows / 2048, 1, kSpanMost));
   l.spans = ceil_div64(rows, l.span);
+  if (count <= kListMost) return l;
   l.tiles = ceil_div64(count, kTile);
   size_t at = 0;
-  auto take = [&](size_t bytes) {
+  auto take = [&](size_t elems, size_t size) {
     const size_t here = at;
-    at += Workspace::align(bytes);
+    at += Workspace::align(elems * size);
     return here;
   };
-  l.keys = take(static_cast<size_t>(l.tiles) * kTile * sizeof(uint32_t));
-  l.sources = take(static_cast<size_t>(l.tiles) * kTile * sizeof(uint32_t));
-  l.order = take(static_cast<size_t>(l.tiles) * kTile * sizeof(uint16_t));
-  l.uniform = take(static_cast<size_t>(l.tiles) * sizeof(uint64_t));
-  l.starts = take(static_cast<size_t>(l.tiles) * (l.spans + 1) * sizeof(uint16_t));
-  l.sums = take(static_cast<size_t>(l.tiles) * kTileChunks * dim * sizeof(float));
+  const size_t tiles = static_cast<size_t>(l.tiles);
+  l.keys = take(tiles * kTile, sizeof(uint32_t));
+  l.sources = take(tiles * kTile, sizeof(uint32_t));
+  l.order = take(tiles * kTile, sizeof(uint16_t));
+  l.runs = take(tiles * kTileRuns, sizeof(uint16_t));
+  l.starts = take(tiles * (l.spans + 1), sizeof(uint16_t));
+  l.sums = take(tiles * kTileRuns * dim, sizeof(float));
   l.bytes = at;
   return l;
 }
 
 template <typename T, typename O, int VEC, int L>
-int32_t run_span(const GradArgs &a, void *stream) {
+int32_t run_grad(const GradArgs &a, void *stream) {
+  if (a.tiles > 0) {
+    int32_t rc = launch(embedding_tile_kernel, dim3(a.tiles), dim3(kTileBlock), stream, a);
+    if (rc != SPORDER_OK) return rc;
+    rc = launch(embedding_run_kernel<T, VEC, L>, dim3(ceil_div64(a.tiles * kTileRuns, 256 / L)),
+                dim3(256), stream, a);
+    if (rc != SPORDER_OK) return rc;
+  }
   return launch(embedding_span_kernel<T, O, VEC, L>, dim3(a.spans), dim3(256), stream, a);
 }
 
 template <typename T, typename O, int VEC>
 int32_t grad_vec(const GradArgs &a, void *stream) {
-  if (a.tiles > 0) {
-    int32_t rc = launch(embedding_tile_kernel, dim3(a.tiles), dim3(kTileBlock), stream, a);
-    if (rc != SPORDER_OK) return rc;
-    rc = launch(embedding_chunk_kernel<T, VEC>,
-                dim3(a.tiles * kTileChunks, ceil_div64(a.dim, 256 * VEC)), dim3(256), stream, a);
-    if (rc != SPORDER_OK) return rc;
-  }
   const int64_t vecs = ceil_div64(a.dim, VEC);
-  if (vecs <= 8) return run_span<T, O, VEC, 8>(a, stream);
-  if (vecs <= 32) return run_span<T, O, VEC, 32>(a, stream);
-  if (vecs <= 256) return run_span<T, O, VEC, 64>(a, stream);
-  return run_span<T, O, VEC, 256>(a, stream);
+  if (vecs <= 8) return run_grad<T, O, VEC, 8>(a, stream);
+  if (vecs <= 32) return run_grad<T, O, VEC, 32>(a, stream);
+  if (vecs <= 256) return run_grad<T, O, VEC, 64>(a, stream);
+  return run_grad<T, O, VEC, 256>(a, stream);
 }
 
 template <typename T, typename O> int32_t grad_typed(const GradArgs &a, void *stream) {
@@ -457,9 +532,9 @@ template <typename T, typename O> int32_t grad_typed(const GradArgs &a, void *st
 }
 
 // Rows count in 31 bits with one value over (no row); a launch has fewer than
-// 2^32 threads, and the chunks' launch takes four per token.
+// 2^32 threads, and the runs' launch takes up to 16 per token.
 constexpr int64_t kMostRows = (int64_t(1) << 31) - 2;
-constexpr int64_t kMostTokens = (int64_t(1) << 30) - kTile;
+constexpr int64_t kMostTokens = (int64_t(1) << 28) - kTile;
 
 } // namespace
 
@@ -500,10 +575,10 @@ int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count, int64_
       rows > kMostRows || dim < 1 || dim > kMostDim || count < 0 || count > kMostTokens || grad_stride < 0 ||
       (rows > 1 && out_stride < dim) || (token_bits != 32 && token_bits != 64) || !d_out)
     return SPORDER_BAD_ARGUMENT;
-  if (count > 0 && (!d_grad || !d_tokens || !d_work || !aligned_to(d_work, 256) ||
-                    work_bytes < sporder_embedding_grad_work_bytes(count, rows, dim)))
-    return SPORDER_BAD_ARGUMENT;
+  if (count > 0 && (!d_grad || !d_tokens)) return SPORDER_BAD_ARGUMENT;
   const GradLayout l = grad_layout(count, rows, dim);
+  if (l.bytes > 0 && (!d_work || !aligned_to(d_work, 256) || work_bytes < l.bytes))
+    return SPORDER_BAD_ARGUMENT;
   char *const w = static_cast<char *>(d_work);
   const GradArgs a{d_grad,
                    d_tokens,
@@ -523,7 +598,7 @@ int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count, int64_
                    reinterpret_cast<uint32_t *>(w + l.keys),
                    reinterpret_cast<uint32_t *>(w + l.sources),
                    reinterpret_cast<uint16_t *>(w + l.order),
-                   reinterpret_cast<uint64_t *>(w + l.uniform),
+                   reinterpret_cast<uint16_t *>(w + l.runs),
                    reinterpret_cast<uint16_t *>(w + l.starts),
                    reinterpret_cast<float *>(w + l.sums)};
   if (type == SPORDER_TYPE_F32) return grad_typed<float, float>(a, stream);

@@ -67,16 +67,21 @@ def _out(out, shape, dtype, ref):
     return out
 
 
+# The current stream's handle without a Stream object around it (a call less
+# than a microsecond long instead of a few).
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream",
+                      lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def _call(name, ref, *args):
     """Queues a C entry on the current stream of ref's device."""
-    device = ref.device
+    index = ref.device.index
     fn = getattr(_lib.load(), name)
-    stream = torch.cuda.current_stream(device).cuda_stream
-    if device.index == torch.cuda.current_device():
-        rc = fn(stream, *args)
+    if index == torch.cuda.current_device():
+        rc = fn(_raw_stream(index), *args)
     else:
-        with torch.cuda.device(device):
-            rc = fn(stream, *args)
+        with torch.cuda.device(index):
+            rc = fn(_raw_stream(index), *args)
     if rc != _lib.OK:
         raise RuntimeError(f"{name} returned {rc}")
 
@@ -137,11 +142,11 @@ def embedding_grad(grad, tokens, num_rows, *, scale=1.0, padding_idx=None, dtype
     out = _out(out, (num_rows, dim), dtype, grad)
     grad, _, stride = _rows(grad)
     size = _lib.load().sporder_embedding_grad_work_bytes(count, num_rows, dim)
-    work = torch.empty(size, dtype=torch.uint8, device=grad.device)
+    work = torch.empty(size, dtype=torch.uint8, device=grad.device) if size else None
     _call("sporder_embedding_grad", grad, _TYPES[grad.dtype], count, dim, stride, grad.data_ptr(),
           _TOKEN_BITS[tokens.dtype], tokens.data_ptr(), float(scale),
           -1 if padding_idx is None else int(padding_idx), num_rows, _TYPES[dtype], dim,
-          out.data_ptr(), work.data_ptr(), size)
+          out.data_ptr(), work.data_ptr() if size else 0, size)
     return out
 
 

@@ -458,9 +458,8 @@ SPORDER_API int32_t sporder_embedding(void *stream, int32_t type, int64_t rows, 
 
 /*
  * Its gradient by the table: d_out[v] = scale * sum of d_grad[t] over the t
- * with d_tokens[t] = v, summed in the order of t within groups whose sizes
- * depend on the tokens alone, for each of `rows` rows (0 where there is no
- * such t).  Tokens equal to padding_idx and tokens outside [0, rows) are left
+ * with d_tokens[t] = v, for each of `rows` rows (0 where there is no such t),
+ * summed in an order that depends on the tokens and the sizes alone.  Tokens equal to padding_idx and tokens outside [0, rows) are left
  * out.  out_type is `type` or SPORDER_TYPE_F32.  d_work is 256-byte aligned.
  */
 SPORDER_API size_t sporder_embedding_grad_work_bytes(int64_t count, int64_t rows, int64_t dim);

@@ -112,6 +112,7 @@ TYPE_F32 = 0                           # sporder_type_t
 TYPE_BF16 = 1
 TYPE_F16 = 2
 OK = 0                                 # SPORDER_OK
+BAD_ARGUMENT = 2                       # SPORDER_BAD_ARGUMENT
 
 # Every symbol include/sporder.h declares, with its ctypes signature.
 SIGNATURES = {
@@ -146,6 +147,9 @@ SIGNATURES = {
     "sporder_layer_norm_grad_work_bytes": ([i64, i64], sz),
     "sporder_layer_norm_grad": (
         [vp, i32, i32, i64, i64, i64, vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, sz], i32),
+    "sporder_newton_schulz_work_bytes": ([i64, i64, i64], sz),
+    "sporder_newton_schulz": (
+        [vp, i32, i64, i64, i64, i64, i64, vp, i32, f64, f64, f64, f64, vp, vp, sz], i32),
     "sporder_hbm_stream": ([vp, i32, i32, vp, vp, ctypes.c_int64, i32, P(f32)], None),
 }
 

@@ -9,8 +9,8 @@ as torch tensors on the same device.
 Provided: chunk_similarity_greedy (sporder-csg), chunk_greedy (sporder-cg),
 reorder, count_pillars, similarity_graph, bench_cusparse_spmm, plus spmm_csr
 and chunk_similarity_top_k (new), and the operators of a training step
-around the SpMM (new): embedding, embedding_grad, layer_norm, layer_norm_grad.
-hierarchical_matching and
+around the SpMM (new): embedding, embedding_grad, layer_norm, layer_norm_grad,
+newton_schulz.  hierarchical_matching and
 similarity_graph_exact exist for import compatibility and raise
 NotImplementedError.
 """
@@ -31,7 +31,7 @@ from ._sporder import spmm_csr as _spmm_csr
 from ._sporder import spmm_csr_noalloc as _spmm_csr_noalloc
 from ._sporder import spmm_csr_scaled as _spmm_csr_scaled
 from ._sporder import SpmmPlan
-from ._train import embedding, embedding_grad, layer_norm, layer_norm_grad
+from ._train import embedding, embedding_grad, layer_norm, layer_norm_grad, newton_schulz
 
 __all__ = [
     "bench_cusparse_spmm",
@@ -45,6 +45,7 @@ __all__ = [
     "hierarchical_matching",
     "layer_norm",
     "layer_norm_grad",
+    "newton_schulz",
     "reorder",
     "similarity_graph",
     "similarity_graph_exact",

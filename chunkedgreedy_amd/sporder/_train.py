@@ -21,6 +21,10 @@ _TYPES = {torch.float32: _lib.TYPE_F32, torch.bfloat16: _lib.TYPE_BF16,
 _TOKEN_BITS = {torch.int32: 32, torch.int64: 64}
 
 
+class _BadArgument(ValueError):
+    pass
+
+
 def _floats(a, name):
     t = _as_tensor(a, name)
     if not t.is_cuda:
@@ -82,6 +86,8 @@ def _call(name, ref, *args):
     else:
         with torch.cuda.device(index):
             rc = fn(_raw_stream(index), *args)
+    if rc == _lib.BAD_ARGUMENT:
+        raise _BadArgument(f"{name} refused its arguments")
     if rc != _lib.OK:
         raise RuntimeError(f"{name} returned {rc}")
 
@@ -243,3 +249,55 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None):
           0 if weight is None else weight.data_ptr(), dim, dx.data_ptr(), dweight.data_ptr(),
           dbias.data_ptr(), work.data_ptr(), size)
     return dx, dweight, dbias
+
+
+def newton_schulz(g, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, out=None):
+    """Orthogonalise a matrix by Newton-Schulz products (the Muon optimiser's
+    update): X = g / (|g| + eps) with the Frobenius norm, then ``steps`` times
+    X <- a X + (b A + c A A) X with A = X X^T.
+
+    Every singular value s of g / |g| becomes p(p(...p(s))) with p(s) = a s +
+    b s^3 + c s^5; the default coefficients take most of [0, 1] close to 1 in
+    five steps.  Matrices taller than wide are handled as their transposes.
+
+    Arguments:
+        g: (rows, cols), or a batch (batch, rows, cols), float32, bfloat16 or
+            float16, sides of at most 65536; read in place where its last
+            dimension has unit stride
+        steps: >= 1
+        coefficients: (a, b, c); refused where a singular value in [0, 1], or
+            one of A or b A + c A A, could pass 31 within the steps
+        eps: >= 0
+        out: contiguous tensor of g's shape and type, or None; may be g
+
+    Products have operands of 22 bits and 32-bit sums whatever the type: the
+    result is as close as 32-bit products give it, down to steps of 2^-35 of
+    the norm of the start.  Returns out.
+    """
+    g = _floats(g, "g")
+    if g.dim() not in (2, 3) or g.shape[-1] < 1 or g.shape[-2] < 1 \
+            or max(g.shape[-2:]) > 65536 or (g.dim() == 3 and g.shape[0] > 32768):
+        raise ValueError("g must be (rows, cols) or (batch, rows, cols) with sides of 1 to 65536 "
+                         "and a batch of at most 32768")
+    steps = int(steps)
+    if steps < 1:
+        raise ValueError("steps must be >= 1")
+    if not eps >= 0.0:
+        raise ValueError("eps must be >= 0")
+    a, b, c = (float(v) for v in coefficients)
+    batch = g.shape[0] if g.dim() == 3 else 1
+    rows, cols = g.shape[-2:]
+    out = _out(out, g.shape, g.dtype, g)
+    if g.stride(-1) != 1 and cols > 1:
+        g = g.contiguous()
+    lib = _lib.load()
+    size = lib.sporder_newton_schulz_work_bytes(batch, rows, cols)
+    work = torch.empty(size, dtype=torch.uint8, device=g.device)
+    try:
+        _call("sporder_newton_schulz", g, _TYPES[g.dtype], batch, rows, cols,
+              g.stride(0) if g.dim() == 3 else 0, g.stride(-2), g.data_ptr(), steps, a, b, c,
+              float(eps), out.data_ptr(), work.data_ptr(), size)
+    except _BadArgument:
+        raise ValueError(f"coefficients {(a, b, c)} take singular values past 31 within "
+                         f"{steps} steps") from None
+    return out

@@ -498,6 +498,23 @@ SPORDER_API int32_t sporder_layer_norm_grad(void *stream, int32_t type, int32_t 
                                             int64_t dx_stride, void *d_dx, void *d_dweight,
                                             void *d_dbias, void *d_work, size_t work_bytes);
 
+/*
+ * Newton-Schulz orthogonalisation of each of `batch` matrices G of rows x cols
+ * (rows g_stride, matrices g_batch_stride elements apart): X = G / (|G|_F +
+ * eps), then `steps` (>= 1) times X <- a X + (b A + c A A) X with A = X X^T (of
+ * G^T where rows > cols), written to d_out (contiguous, of G's type).
+ * Products have operands of 22 bits and 32-bit sums.  Coefficients under
+ * which a singular value in [0, 1], or one of A or b A + c A A, could pass 31
+ * within the steps are a bad argument; rows and cols are at most 65536.  d_work is
+ * 256-byte aligned.
+ */
+SPORDER_API size_t sporder_newton_schulz_work_bytes(int64_t batch, int64_t rows, int64_t cols);
+SPORDER_API int32_t sporder_newton_schulz(void *stream, int32_t type, int64_t batch,
+                                          int64_t rows, int64_t cols, int64_t g_batch_stride,
+                                          int64_t g_stride, const void *d_g, int32_t steps,
+                                          double a, double b, double c, double eps, void *d_out,
+                                          void *d_work, size_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

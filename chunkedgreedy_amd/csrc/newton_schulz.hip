@@ -34,13 +34,14 @@ namespace sporder_hip {
 namespace {
 
 using f16x8 = f16_t __attribute__((ext_vector_type(8)));
+using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 using f32x16 = float __attribute__((ext_vector_type(16)));
 
 constexpr float kScale = 2048.0f; // of the stored halves
 constexpr double kMostValue = 31.0;
 constexpr int kBlock = 256;
 constexpr int kPad = 128; // rows and columns are padded to multiples of it
-constexpr int kStageRow = 36; // words per row of a wave's transposing buffer
+constexpr int kStageRow = 40; // halves per row of a wave's transposing buffer
 
 struct OrthoArgs {
   const void *g;
@@ -61,10 +62,6 @@ __host__ __device__ constexpr int64_t packed_units(int64_t rows, int64_t cols) {
   return rows * cols / 4; // two halves of 2 bytes each: 4 bytes per element
 }
 
-// One wave's 32 x 32 block with row i0 and column j0: lane l holds column
-// l % 32, rows 8 q + 4 (l / 32) + e in v[4 q + e], scaled.
-// by_col receives the block with columns as operand rows, by_row (if not
-// null) with its own; k_col and k_row are their numbers of 16-column blocks.
 __device__ __forceinline__ void split_halves(float v, uint32_t &hi, uint32_t &lo) {
   const f16_t h = static_cast<f16_t>(v);
   const f16_t l = static_cast<f16_t>(v - static_cast<float>(h));
@@ -79,41 +76,40 @@ __device__ __forceinline__ uint2 *col_place(uint4 *p, int k_blocks, int i0, int 
   return reinterpret_cast<uint2 *>(unit) + lane / 32;
 }
 
+// Stores one wave's 32 x 32 block with row i0 and column j0, scaled: lane l
+// holds column l % 32, rows 8 q + 4 (l / 32) + e in v[4 q + e].  by_col
+// receives it with columns as operand rows, by_row (if not null) with its own
+// rows, which 8 neighbouring columns of a row take a turn through LDS for;
+// k_col and k_row are their numbers of 16-column blocks.
 __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col, int k_col,
                                             uint4 *by_row, int k_row, int i0, int j0,
-                                            uint32_t *stage) {
+                                            uint16_t *stage) {
   const int lane = lane_id();
+  uint32_t half[2][16];
 #pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    uint32_t hi[4], lo[4];
+  for (int r = 0; r < 16; ++r) split_halves(v[r], half[0][r], half[1][r]);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      split_halves(v[4 * q + e], hi[e], lo[e]);
-      if (by_row) stage[(8 * q + 4 * (lane / 32) + e) * kStageRow + lane % 32] = hi[e] | lo[e] << 16;
+  for (int plane = 0; plane < 2; ++plane) {
+    const uint32_t(&h)[16] = half[plane];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *col_place(by_col, k_col, i0, j0, q, plane, lane) =
+          make_uint2(h[4 * q] | h[4 * q + 1] << 16, h[4 * q + 2] | h[4 * q + 3] << 16);
+    if (!by_row) continue;
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+      stage[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * kStageRow + lane % 32] =
+          static_cast<uint16_t>(h[r]);
+    wave_lds_order();
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int row = lane % 32, part = lane / 32 + 2 * s; // 8 columns from 8 part
+      const int64_t block = static_cast<int64_t>(i0 / 32) * k_row + j0 / 16 + part / 2;
+      by_row[(block * 2 + plane) * kWave + row + 32 * (part % 2)] =
+          *reinterpret_cast<const uint4 *>(stage + row * kStageRow + 8 * part);
     }
-    *col_place(by_col, k_col, i0, j0, q, 0, lane) =
-        make_uint2(hi[0] | hi[1] << 16, hi[2] | hi[3] << 16);
-    *col_place(by_col, k_col, i0, j0, q, 1, lane) =
-        make_uint2(lo[0] | lo[1] << 16, lo[2] | lo[3] << 16);
+    wave_lds_order();
   }
-  if (!by_row) return;
-  wave_lds_order();
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    const int row = lane % 32, part = lane / 32 + 2 * s; // 8 columns from 8 part
-    const uint4 *const from = reinterpret_cast<const uint4 *>(stage + row * kStageRow + 8 * part);
-    const uint4 p = from[0], q = from[1];
-    uint4 hi, lo;
-    hi.x = (p.x & 0xffff) | p.y << 16, lo.x = p.x >> 16 | (p.y & 0xffff0000u);
-    hi.y = (p.z & 0xffff) | p.w << 16, lo.y = p.z >> 16 | (p.w & 0xffff0000u);
-    hi.z = (q.x & 0xffff) | q.y << 16, lo.z = q.x >> 16 | (q.y & 0xffff0000u);
-    hi.w = (q.z & 0xffff) | q.w << 16, lo.w = q.z >> 16 | (q.w & 0xffff0000u);
-    const int64_t block = static_cast<int64_t>(i0 / 32) * k_row + j0 / 16 + part / 2;
-    uint4 *const unit = by_row + block * 2 * kWave + row + 32 * (part % 2);
-    unit[0] = hi;
-    unit[kWave] = lo;
-  }
-  wave_lds_order();
 }
 
 // The values (scaled) that store_block put into by_col.
@@ -136,23 +132,43 @@ __device__ __forceinline__ void load_block(const uint4 *by_col, int k_col, int i
 
 // ---- norm and packing ------------------------------------------------------------
 
-constexpr int kNormBlocks = 256; // partial sums per matrix
+constexpr int kNormBlocks = 256; // partial sums per matrix, at most
+constexpr int kNormThreads = 512;
 
 // Sums of squares in 64 bits: no overflow or underflow at any finite input.
-__global__ void __launch_bounds__(kBlock) ortho_norm_kernel(OrthoArgs a) {
+// The additions go to four sums so that four loads are under way per thread.
+template <typename T, int VEC>
+__global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(OrthoArgs a) {
   const int64_t z = blockIdx.y, rows = a.tall ? a.n : a.m, cols = a.tall ? a.m : a.n;
-  double s = 0.0;
-  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x) {
-    const int64_t base = z * a.g_batch + r * a.g_stride;
-    for (int64_t c = threadIdx.x; c < cols; c += kBlock) {
-      const double v = load_typed(a.g, a.type, base + c);
-      s += v * v;
+  const T *const g = static_cast<const T *>(a.g) + z * a.g_batch;
+  const int64_t vecs = cols / VEC, per = ceil_div64(rows * vecs, gridDim.x);
+  const int64_t first = blockIdx.x * per, last = min(first + per, rows * vecs);
+  double s[4] = {};
+  int64_t at = first + threadIdx.x;
+  int64_t row = at / vecs, col = at % vecs;
+  for (; at < last; at += 4 * kNormThreads) {
+    float v[4][VEC];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (at + k * kNormThreads < last) {
+        load_f32<VEC>(g + row * a.g_stride + col * VEC, v[k]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[k][i] = 0.0f;
+      }
+      col += kNormThreads;
+      if (col >= vecs) row += col / vecs, col %= vecs;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) s[k] += static_cast<double>(v[k][i]) * v[k][i];
     }
   }
-  __shared__ double part[kBlock];
-  part[threadIdx.x] = s;
+  __shared__ double part[kNormThreads];
+  part[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
   __syncthreads();
-  for (int k = kBlock / 2; k > 0; k /= 2) {
+  for (int k = kNormThreads / 2; k > 0; k /= 2) {
     if (threadIdx.x < k) part[threadIdx.x] += part[threadIdx.x + k];
     __syncthreads();
   }
@@ -162,7 +178,7 @@ __global__ void __launch_bounds__(kBlock) ortho_norm_kernel(OrthoArgs a) {
 // Packs X = G / (|G| + eps), 64 x 64 per workgroup, a 32 x 32 block per wave.
 __global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int norm_blocks) {
   __shared__ double part[kBlock];
-  __shared__ __attribute__((aligned(16))) uint32_t stage[4][32 * kStageRow];
+  __shared__ __attribute__((aligned(16))) uint16_t stage[4][32 * kStageRow];
   const int64_t z = blockIdx.y;
   part[threadIdx.x] =
       static_cast<int>(threadIdx.x) < norm_blocks ? a.partial[z * kNormBlocks + threadIdx.x] : 0.0;
@@ -195,6 +211,56 @@ __global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int nor
 
 enum Product { kGram, kPoly, kUpdate, kLast };
 
+// Writes a block of the result, unscaled.
+__device__ __forceinline__ void write_block(const OrthoArgs &a, int64_t z, int i0, int j0,
+                                            const float (&v)[16]) {
+  const int64_t j = j0 + lane_id() % 32;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int64_t i = i0 + 8 * (r / 4) + 4 * (lane_id() / 32) + r % 4;
+    if (i < a.m && j < a.n)
+      store_typed(a.out, a.type, z * a.m * a.n + (a.tall ? j * a.m + i : i * a.n + j),
+                  v[r] * (1.0f / kScale));
+  }
+}
+
+// The epilogue of a product for one wave's block: v holds C, scaled once.
+template <int WHAT>
+__device__ __forceinline__ void finish_block(const OrthoArgs &a, int64_t z, bool mirror, int i0,
+                                             int j0, float (&v)[16], uint16_t *stage) {
+  const int64_t xu = packed_units(a.mp, a.np), mu = packed_units(a.mp, a.mp);
+  const int km = a.mp / 16, kn = a.np / 16;
+  if constexpr (WHAT == kGram) {
+    uint4 *const to = a.gram + z * mu;
+    store_block(v, to, km, mirror ? to : nullptr, km, i0, j0, stage);
+  } else if constexpr (WHAT == kPoly) {
+    float old[16];
+    load_block(a.gram + z * mu, km, i0, j0, old);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = a.b * old[r] + a.c * v[r];
+    uint4 *const to = a.poly + z * mu;
+    store_block(v, to, km, mirror ? to : nullptr, km, i0, j0, stage);
+  } else {
+    float old[16];
+    load_block(a.xt + z * xu, km, i0, j0, old);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[r] = a.a * old[r] + v[r];
+    if constexpr (WHAT == kUpdate)
+      store_block(v, a.xt_next + z * xu, km, a.x + z * xu, kn, i0, j0, stage);
+    else
+      write_block(a, z, i0, j0, v);
+  }
+}
+
+// Tile t of a triangle of `across` rows: row ti holds across - ti tiles.
+__device__ __forceinline__ void triangle_tile(int t, int across, int &ti, int &tj) {
+  const float side = 2 * across + 1;
+  ti = static_cast<int>((side - sqrtf(side * side - 8.0f * t)) / 2);
+  while (ti > 0 && ti * across - ti * (ti - 1) / 2 > t) --ti;
+  while ((ti + 1) * across - (ti + 1) * ti / 2 <= t) ++ti;
+  tj = ti + t - (ti * across - ti * (ti - 1) / 2);
+}
+
 // C = P Q^T of packed operands, one TILE x TILE tile per workgroup of 2 x 2
 // waves, 32 columns of both operands per stage: loaded to registers while the
 // stage before is multiplied, then stored to the other half of LDS.
@@ -218,12 +284,8 @@ __global__ void __launch_bounds__(kBlock) ortho_product_kernel(OrthoArgs a) {
   const int tiles_n = (kSymmetric ? a.mp : a.np) / TILE;
 
   int ti, tj;
-  if (kSymmetric) { // row ti of the triangle holds tiles_n - ti tiles
-    const int t = blockIdx.x;
-    ti = static_cast<int>((2 * tiles_n + 1 - sqrtf(static_cast<float>((2 * tiles_n + 1) * (2 * tiles_n + 1) - 8 * t))) / 2);
-    while (ti > 0 && ti * tiles_n - ti * (ti - 1) / 2 > t) --ti;
-    while ((ti + 1) * tiles_n - (ti + 1) * ti / 2 <= t) ++ti;
-    tj = ti + t - (ti * tiles_n - ti * (ti - 1) / 2);
+  if (kSymmetric) {
+    triangle_tile(blockIdx.x, tiles_n, ti, tj);
   } else {
     ti = blockIdx.x / tiles_n;
     tj = blockIdx.x % tiles_n;
@@ -245,7 +307,6 @@ __global__ void __launch_bounds__(kBlock) ortho_product_kernel(OrthoArgs a) {
     }
   }
 
-  using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
   u32x4 next[2][kRows];
   auto fetch = [&](int stage) {
 #pragma unroll
@@ -295,7 +356,7 @@ __global__ void __launch_bounds__(kBlock) ortho_product_kernel(OrthoArgs a) {
   }
 
   // The accumulators hold products of two scaled values.
-  uint32_t *const stage = reinterpret_cast<uint32_t *>(&lds[0][0][0]) + wave * 32 * kStageRow;
+  uint16_t *const stage = reinterpret_cast<uint16_t *>(&lds[0][0][0]) + wave * 32 * kStageRow;
 #pragma unroll
   for (int bi = 0; bi < kSide; ++bi) {
 #pragma unroll
@@ -304,35 +365,209 @@ __global__ void __launch_bounds__(kBlock) ortho_product_kernel(OrthoArgs a) {
       float v[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) v[r] = acc[bi][bj][r] * (1.0f / kScale);
-      if constexpr (WHAT == kGram) {
-        uint4 *const to = a.gram + z * mu;
-        store_block(v, to, a.mp / 16, ti != tj ? to : nullptr, a.mp / 16, i0, j0, stage);
-      } else if constexpr (WHAT == kPoly) {
-        float old[16];
-        load_block(p, a.mp / 16, i0, j0, old);
+      finish_block<WHAT>(a, z, ti != tj, i0, j0, v, stage);
+    }
+  }
+}
+
+// The same for products of few tiles: 64 x 64 per workgroup, whose four waves
+// each take a quarter of the columns and read their operands straight from
+// memory (in the units' own order, so without LDS); the four sums meet in LDS,
+// a block of 32 x 32 per wave.
+template <int WHAT> __global__ void __launch_bounds__(kBlock) ortho_split_kernel(OrthoArgs a) {
+  constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
+  __shared__ float sums[4][4][16][kWave];
+  const int64_t z = blockIdx.y;
+  const int64_t xu = packed_units(a.mp, a.np), mu = packed_units(a.mp, a.mp);
+  const uint4 *const p = WHAT == kGram ? a.x + z * xu : WHAT == kPoly ? a.gram + z * mu : a.poly + z * mu;
+  const uint4 *const q = kSymmetric ? p : a.xt + z * xu;
+  const int k_blocks = (WHAT == kGram ? a.np : a.mp) / 16;
+  const int across = (kSymmetric ? a.mp : a.np) / 64;
+  int ti, tj;
+  if (kSymmetric) {
+    triangle_tile(blockIdx.x, across, ti, tj);
+  } else {
+    ti = blockIdx.x / across;
+    tj = blockIdx.x % across;
+  }
+  const int wave = threadIdx.x / kWave, lane = lane_id();
+  const int64_t step = static_cast<int64_t>(k_blocks) * 2 * kWave;
+  const int mine = k_blocks / 4; // padded columns: a multiple of 8 blocks
+  const uint4 *const pt = p + ti * 2 * step + static_cast<int64_t>(wave * mine) * 2 * kWave + lane;
+  const uint4 *const qt = q + tj * 2 * step + static_cast<int64_t>(wave * mine) * 2 * kWave + lane;
+
+  f32x16 acc[2][2] = {};
+  struct Operands {
+    u32x4 v[2][2][2]; // operand, block of 32 rows, hi and lo
+  };
+  auto fetch = [&](int k) {
+    Operands o;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = a.b * old[r] + a.c * v[r];
-        uint4 *const to = a.poly + z * mu;
-        store_block(v, to, a.mp / 16, ti != tj ? to : nullptr, a.mp / 16, i0, j0, stage);
-      } else {
-        float old[16];
-        load_block(q, a.mp / 16, i0, j0, old);
+    for (int i = 0; i < 2; ++i) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) v[r] = a.a * old[r] + v[r];
-        if constexpr (WHAT == kUpdate) {
-          store_block(v, a.xt_next + z * xu, a.mp / 16, a.x + z * xu, a.np / 16, i0, j0, stage);
-        } else {
-          const int64_t j = j0 + lane % 32;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) {
-            const int64_t i = i0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
-            if (i < a.m && j < a.n)
-              store_typed(a.out, a.type, z * a.m * a.n + (a.tall ? j * a.m + i : i * a.n + j),
-                          v[r] * (1.0f / kScale));
-          }
-        }
+      for (int h = 0; h < 2; ++h) {
+        o.v[0][i][h] = *reinterpret_cast<const u32x4 *>(pt + i * step + (k * 2 + h) * kWave);
+        o.v[1][i][h] = *reinterpret_cast<const u32x4 *>(qt + i * step + (k * 2 + h) * kWave);
       }
     }
+    return o;
+  };
+  auto multiply = [&](const Operands &o) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const f16x8 ph = __builtin_bit_cast(f16x8, o.v[0][i][0]), pl = __builtin_bit_cast(f16x8, o.v[0][i][1]);
+        const f16x8 qh = __builtin_bit_cast(f16x8, o.v[1][j][0]), ql = __builtin_bit_cast(f16x8, o.v[1][j][1]);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc[i][j], 0, 0, 0);
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc[i][j], 0, 0, 0);
+      }
+    }
+  };
+  // Two steps under way (mine is even).
+  Operands even = fetch(0), odd = fetch(1);
+  for (int k = 0; k < mine; k += 2) {
+    multiply(even);
+    even = fetch(min(k + 2, mine - 1));
+    multiply(odd);
+    odd = fetch(min(k + 3, mine - 1));
+  }
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sums[wave][2 * i + j][r][lane] = acc[i][j][r];
+    }
+  }
+  __syncthreads();
+  float v[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r)
+    v[r] = ((sums[0][wave][r][lane] + sums[1][wave][r][lane]) +
+            (sums[2][wave][r][lane] + sums[3][wave][r][lane])) *
+           (1.0f / kScale);
+  __syncthreads();
+  uint16_t *const stage = reinterpret_cast<uint16_t *>(&sums[wave][0][0][0]);
+  finish_block<WHAT>(a, z, ti != tj, ti * 64 + wave / 2 * 32, tj * 64 + wave % 2 * 32, v, stage);
+}
+
+// A whole matrix in one workgroup, X and X^T in LDS (at most 16 blocks of
+// 32 x 32, padded to 32): its products take less than a launch each.  Eight
+// waves take two blocks of the result each; A, then B, takes X's place until
+// the new X does.
+constexpr int kWholeBlocks = 16;
+constexpr int kWholeWaves = 8;
+constexpr int kWholeUnits = kWholeBlocks * 32 * 32 / 4;
+
+__global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoArgs a, int steps) {
+  __shared__ __attribute__((aligned(16))) uint4 x[kWholeUnits], xt[kWholeUnits];
+  __shared__ __attribute__((aligned(16))) uint16_t stages[kWholeWaves][32 * kStageRow];
+  __shared__ double part[kWholeWaves];
+  const int64_t z = blockIdx.x;
+  const int wave = threadIdx.x / kWave, lane = lane_id();
+  const int mb = a.mp / 32, nb = a.np / 32; // blocks down and across
+  uint16_t *const stage = stages[wave];
+  const int wide = mb * nb, square = mb * (mb + 1) / 2;
+
+  float v[2][16];
+  double s = 0.0;
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int block = wave + t * kWholeWaves;
+    const int i0 = block / nb * 32, j = block % nb * 32 + lane % 32;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+      const int i = i0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+      v[t][r] = 0.0f;
+      if (block < wide && i < a.m && j < a.n)
+        v[t][r] = load_typed(a.g, a.type,
+                             z * a.g_batch + (a.tall ? j * a.g_stride + i : i * a.g_stride + j));
+      s += static_cast<double>(v[t][r]) * v[t][r];
+    }
+  }
+  for (int k = 1; k < kWave; k <<= 1) s += __shfl_xor(s, k);
+  if (lane == 0) part[wave] = s;
+  __syncthreads();
+  s = 0.0;
+  for (int w = 0; w < kWholeWaves; ++w) s += part[w];
+  const double scale = static_cast<double>(kScale) / (sqrt(s) + a.eps);
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    const int block = wave + t * kWholeWaves;
+    if (block >= wide) continue;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) v[t][r] = static_cast<float>(v[t][r] * scale);
+    store_block(v[t], xt, 2 * mb, x, 2 * nb, block / nb * 32, block % nb * 32, stage);
+  }
+  __syncthreads();
+
+  // v[t] = block (bi, bj) of P Q^T, unscaled once; operands with k blocks of 16 columns.
+  auto product = [&](const uint4 *p, const uint4 *q, int k_blocks, int bi, int bj, float (&out)[16]) {
+    f32x16 acc = {};
+    const uint4 *const pt = p + bi * k_blocks * 2 * kWave + lane;
+    const uint4 *const qt = q + bj * k_blocks * 2 * kWave + lane;
+#pragma unroll 2
+    for (int k = 0; k < k_blocks; ++k) {
+      const f16x8 ph = __builtin_bit_cast(f16x8, pt[k * 2 * kWave]);
+      const f16x8 pl = __builtin_bit_cast(f16x8, pt[(k * 2 + 1) * kWave]);
+      const f16x8 qh = __builtin_bit_cast(f16x8, qt[k * 2 * kWave]);
+      const f16x8 ql = __builtin_bit_cast(f16x8, qt[(k * 2 + 1) * kWave]);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
+      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) out[r] = acc[r] * (1.0f / kScale);
+  };
+
+  for (int step = 0; step < steps; ++step) {
+#pragma unroll
+    for (int what = 0; what < 2; ++what) { // A = X X^T, then B = b A + c A A
+      int bi[2], bj[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int block = wave + t * kWholeWaves;
+        if (block >= square) continue;
+        triangle_tile(block, mb, bi[t], bj[t]);
+        product(x, x, what ? 2 * mb : 2 * nb, bi[t], bj[t], v[t]);
+        if (what) {
+          float old[16];
+          load_block(x, 2 * mb, bi[t] * 32, bj[t] * 32, old);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) v[t][r] = a.b * old[r] + a.c * v[t][r];
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (wave + t * kWholeWaves >= square) continue;
+        store_block(v[t], x, 2 * mb, bi[t] != bj[t] ? x : nullptr, 2 * mb, bi[t] * 32, bj[t] * 32, stage);
+      }
+      __syncthreads();
+    }
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int block = wave + t * kWholeWaves;
+      if (block >= wide) continue;
+      product(x, xt, 2 * mb, block / nb, block % nb, v[t]);
+      float old[16];
+      load_block(xt, 2 * mb, block / nb * 32, block % nb * 32, old);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[t][r] = a.a * old[r] + v[t][r];
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int block = wave + t * kWholeWaves;
+      if (block >= wide) continue;
+      if (step + 1 < steps)
+        store_block(v[t], xt, 2 * mb, x, 2 * nb, block / nb * 32, block % nb * 32, stage);
+      else
+        write_block(a, z, block / nb * 32, block % nb * 32, v[t]);
+    }
+    __syncthreads();
   }
 }
 
@@ -340,12 +575,16 @@ __global__ void __launch_bounds__(kBlock) ortho_product_kernel(OrthoArgs a) {
 
 struct OrthoLayout {
   int64_t m, n, mp, np;
+  bool whole; // one workgroup per matrix, no workspace
   size_t partial, x, xt, xt_next, gram, poly, bytes;
 };
 
 OrthoLayout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
   OrthoLayout l{};
   l.m = std::min(rows, cols), l.n = std::max(rows, cols);
+  l.mp = ceil_div64(l.m, 32) * 32, l.np = ceil_div64(l.n, 32) * 32;
+  l.whole = l.mp * l.np <= kWholeBlocks * 32 * 32;
+  if (l.whole) return l;
   l.mp = ceil_div64(l.m, kPad) * kPad, l.np = ceil_div64(l.n, kPad) * kPad;
   size_t at = 0;
   auto take = [&](int64_t elems, size_t size) {
@@ -398,12 +637,24 @@ bool ortho_bounded(double a, double b, double c, int32_t steps) {
   return true;
 }
 
+constexpr int64_t kFewTiles = 256; // a tile of 128 x 128 for each CU
+
+template <typename T> int32_t run_norm(const OrthoArgs &a, int blocks, void *stream) {
+  const int64_t cols = a.tall ? a.m : a.n;
+  const int vec = row_vec(sizeof(T), cols, {a.g_stride, a.g_batch}, {a.g});
+  if (vec > 1) // 4 elements: 16 or 8 bytes
+    return launch(ortho_norm_kernel<T, 4>, dim3(blocks, a.batch), dim3(kNormThreads), stream, a);
+  return launch(ortho_norm_kernel<T, 1>, dim3(blocks, a.batch), dim3(kNormThreads), stream, a);
+}
+
 template <int WHAT> int32_t run_product(const OrthoArgs &a, void *stream) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
   auto tiles = [&](int64_t tile) {
     const int64_t down = a.mp / tile, across = a.np / tile;
     return kSymmetric ? down * (down + 1) / 2 : down * across;
   };
+  if (tiles(128) * a.batch < kFewTiles)
+    return launch(ortho_split_kernel<WHAT>, dim3(tiles(64), a.batch), dim3(kBlock), stream, a);
   return launch(ortho_product_kernel<WHAT, 128>, dim3(tiles(128), a.batch), dim3(kBlock), stream, a);
 }
 
@@ -428,7 +679,8 @@ int32_t sporder_newton_schulz(void *stream, int32_t type, int64_t batch, int64_t
     return SPORDER_BAD_ARGUMENT;
   if (batch == 0) return SPORDER_OK;
   const OrthoLayout l = ortho_layout(batch, rows, cols);
-  if (!d_g || !d_out || !d_work || !aligned_to(d_work, 256) || work_bytes < l.bytes)
+  if (!d_g || !d_out) return SPORDER_BAD_ARGUMENT;
+  if (l.bytes > 0 && (!d_work || !aligned_to(d_work, 256) || work_bytes < l.bytes))
     return SPORDER_BAD_ARGUMENT;
   char *const w = static_cast<char *>(d_work);
   OrthoArgs args{d_g,
@@ -452,8 +704,13 @@ int32_t sporder_newton_schulz(void *stream, int32_t type, int64_t batch, int64_t
                  reinterpret_cast<uint4 *>(w + l.xt_next),
                  reinterpret_cast<uint4 *>(w + l.gram),
                  reinterpret_cast<uint4 *>(w + l.poly)};
-  const int norm_blocks = static_cast<int>(std::min<int64_t>(rows, kNormBlocks));
-  int32_t rc = launch(ortho_norm_kernel, dim3(norm_blocks, batch), dim3(kBlock), stream, args);
+  if (l.whole)
+    return launch(ortho_whole_kernel, dim3(batch), dim3(kWholeWaves * kWave), stream, args, steps);
+  const int norm_blocks = static_cast<int>(
+      std::clamp<int64_t>(rows * cols / (16 * kNormThreads), 1, kNormBlocks));
+  int32_t rc = type == SPORDER_TYPE_BF16  ? run_norm<bf16_t>(args, norm_blocks, stream)
+               : type == SPORDER_TYPE_F16 ? run_norm<f16_t>(args, norm_blocks, stream)
+                                          : run_norm<float>(args, norm_blocks, stream);
   if (rc == SPORDER_OK)
     rc = launch(ortho_pack_kernel, dim3(l.mp / 64 * (l.np / 64), batch), dim3(kBlock), stream, args,
                 norm_blocks);

@@ -292,11 +292,11 @@ def newton_schulz(g, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-
         g = g.contiguous()
     lib = _lib.load()
     size = lib.sporder_newton_schulz_work_bytes(batch, rows, cols)
-    work = torch.empty(size, dtype=torch.uint8, device=g.device)
+    work = torch.empty(size, dtype=torch.uint8, device=g.device) if size else None
     try:
         _call("sporder_newton_schulz", g, _TYPES[g.dtype], batch, rows, cols,
               g.stride(0) if g.dim() == 3 else 0, g.stride(-2), g.data_ptr(), steps, a, b, c,
-              float(eps), out.data_ptr(), work.data_ptr(), size)
+              float(eps), out.data_ptr(), work.data_ptr() if size else 0, size)
     except _BadArgument:
         raise ValueError(f"coefficients {(a, b, c)} take singular values past 31 within "
                          f"{steps} steps") from None

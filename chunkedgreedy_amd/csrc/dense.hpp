@@ -19,7 +19,7 @@ namespace sporder_hip {
 using bf16_t = __bf16;
 using f16_t = _Float16;
 
-template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Pack {
+template <typename T, int VEC> struct alignas(sizeof(T) * VEC < 16 ? sizeof(T) * VEC : 16) Pack {
   T v[VEC];
 };
 
@@ -38,11 +38,16 @@ __device__ __forceinline__ void store_f32(T *p, const float (&in)[VEC]) {
   *reinterpret_cast<Pack<T, VEC> *>(p) = q;
 }
 
-// Element i of a vector whose type is known at run time.
-__device__ __forceinline__ float load_typed(const void *p, int type, int64_t i) {
-  if (type == SPORDER_TYPE_BF16) return static_cast<float>(static_cast<const bf16_t *>(p)[i]);
-  if (type == SPORDER_TYPE_F16) return static_cast<float>(static_cast<const f16_t *>(p)[i]);
-  return static_cast<const float *>(p)[i];
+// Calls f with a pointer of the type known at run time.  The branch goes
+// around whole loops: one around each access would make them wait for one
+// another.
+template <typename F> __device__ __forceinline__ void with_type(const void *p, int type, F &&f) {
+  if (type == SPORDER_TYPE_BF16)
+    f(static_cast<const bf16_t *>(p));
+  else if (type == SPORDER_TYPE_F16)
+    f(static_cast<const f16_t *>(p));
+  else
+    f(static_cast<const float *>(p));
 }
 __device__ __forceinline__ void store_typed(void *p, int type, int64_t i, float v) {
   if (type == SPORDER_TYPE_BF16)
@@ -87,14 +92,14 @@ inline bool aligned_to(const void *p, size_t bytes) {
 constexpr int64_t kMostDim = int64_t(1) << 23; // elements of a row
 
 // Elements per access of rows whose wider type has `bytes_each` bytes: 16
-// bytes, or 4 elements, where the length, the strides and the bases allow it,
-// else one element.
+// bytes, or 4 elements, where the length, the strides and the bases (16-byte
+// aligned) allow it, else one element.
 inline int row_vec(int bytes_each, int64_t dim, std::initializer_list<int64_t> strides,
                    std::initializer_list<const void *> bases) {
   for (int vec : {16 / bytes_each, 4}) {
     bool ok = dim % vec == 0;
     for (int64_t s : strides) ok = ok && s % vec == 0;
-    for (const void *p : bases) ok = ok && aligned_to(p, static_cast<size_t>(vec) * bytes_each);
+    for (const void *p : bases) ok = ok && aligned_to(p, 16);
     if (ok) return vec;
   }
   return 1;

@@ -99,10 +99,23 @@ struct GradArgs {
   float *sums;         // [tiles * kTileRuns][dim]
 };
 
-// The table row of token i, or `rows` (none) for padding and ids outside.
-__device__ __forceinline__ uint32_t token_row(const GradArgs &a, int64_t i) {
-  const int64_t t = token_at(a.tokens, a.wide, i);
-  return static_cast<uint32_t>(t >= 0 && t < a.rows && t != a.padding ? t : a.rows);
+// The table rows of tokens first, first + step, ... before a.count; `rows`
+// (none) for padding, ids outside and places past the end.
+template <int N>
+__device__ __forceinline__ void token_rows(const GradArgs &a, int64_t first, int64_t step,
+                                           uint32_t (&row)[N]) {
+  int64_t t[N];
+  auto load = [&](auto *tokens) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] = first + k * step < a.count ? tokens[first + k * step] : -1;
+  };
+  if (a.wide)
+    load(static_cast<const int64_t *>(a.tokens));
+  else
+    load(static_cast<const int32_t *>(a.tokens));
+#pragma unroll
+  for (int k = 0; k < N; ++k)
+    row[k] = static_cast<uint32_t>(t[k] >= 0 && t[k] < a.rows && t[k] != a.padding ? t[k] : a.rows);
 }
 
 // Peers of this lane: the lanes whose `bits` low bits of `digit` equal its own.
@@ -130,10 +143,12 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
   const int64_t tile = blockIdx.x, base = tile * kTile;
   const uint32_t none = static_cast<uint32_t>(a.rows); // sorted last, dropped
 
+  uint32_t row[kTileRounds];
+  token_rows(a, base + tid, kTileBlock, row);
 #pragma unroll
   for (int r = 0; r < kTileRounds; ++r) {
     const int i = r * kTileBlock + tid;
-    key[0][i] = base + i < a.count ? token_row(a, base + i) : none;
+    key[0][i] = row[r];
     idx[0][i] = static_cast<uint16_t>(i);
   }
   __syncthreads();
@@ -304,57 +319,85 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
   const int rows = static_cast<int>(min(static_cast<int64_t>(a.span), a.rows - row0));
   const uint16_t *const starts = a.starts + blockIdx.x;
 
-  // The entries, in the tiles' order, or the tokens in theirs.
-  for (int i = tid; i < kBins; i += 256) next[i] = 0;
-  int total = 0;
-  const int64_t items = a.tiles ? a.tiles : a.count;
-  for (int64_t i0 = 0; i0 < items; i0 += 256) {
-    const int64_t item = i0 + tid;
-    int lo = 0, n = 0;
-    uint32_t row = 0;
-    if (item < items) {
-      if (a.tiles) {
-        lo = starts[item * (a.spans + 1)];
-        n = starts[item * (a.spans + 1) + 1] - lo;
-      } else {
-        row = token_row(a, item);
-        n = row >= row0 && row < row0 + rows;
-      }
-    }
+  // Exclusive prefix of one count per thread; `total` gets their sum.
+  auto prefix = [&](int n, int &sum) {
     const int incl = wave_incl_scan(n);
-    __syncthreads(); // the totals of the round before have been read
+    __syncthreads(); // the totals of the call before have been read
     if (lane == kWave - 1) wave_total[wave] = incl;
     __syncthreads();
-    int at = total + incl - n;
+    int at = incl - n;
+    sum = 0;
+#pragma unroll
     for (int w = 0; w < 256 / kWave; ++w) {
       if (w < wave) at += wave_total[w];
-      total += wave_total[w];
+      sum += wave_total[w];
     }
-    for (int i = 0; i < n && at + i < kListMost; ++i) {
-      uint32_t what = static_cast<uint32_t>(item);
-      if (a.tiles) {
-        row = a.keys[item * kTile + lo + i];
-        what = a.sources[item * kTile + lo + i];
+    return at;
+  };
+  auto append = [&](int at, uint32_t row, uint32_t what) {
+    if (at >= kListMost) return;
+    const int bin = 2 * static_cast<int>(row - row0) + ((what & kSummed) == 0);
+    source[at] = what;
+    local[at] = static_cast<uint16_t>(bin);
+    atomicAdd(&next[bin], 1);
+  };
+
+  // The entries, in the tiles' order, or the tokens in theirs.
+  next[tid] = next[tid + 256] = 0;
+  int total = 0;
+  if (a.tiles) {
+    for (int64_t t0 = 0; t0 < a.tiles; t0 += 256) {
+      const int64_t tile = t0 + tid;
+      int lo = 0, n = 0, sum;
+      if (tile < a.tiles) {
+        lo = starts[tile * (a.spans + 1)];
+        n = starts[tile * (a.spans + 1) + 1] - lo;
       }
-      const int bin = 2 * static_cast<int>(row - row0) + ((what & kSummed) == 0);
-      source[at + i] = what;
-      local[at + i] = static_cast<uint16_t>(bin);
-      atomicAdd(&next[bin], 1);
+      const int at = total + prefix(n, sum);
+      for (int64_t i = 0, e = tile * kTile + lo; i < n; ++i) append(at + i, a.keys[e + i], a.sources[e + i]);
+      total += sum;
     }
+  } else {
+    constexpr int kEach = kListMost / 256;
+    const int64_t t0 = static_cast<int64_t>(tid) * kEach;
+    uint32_t row[kEach];
+    token_rows(a, t0, 1, row);
+    int n = 0;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) n += row[k] >= row0 && row[k] < row0 + rows;
+    int at = prefix(n, total);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+      if (row[k] >= row0 && row[k] < row0 + rows) append(at++, row[k], static_cast<uint32_t>(t0 + k));
   }
-  __syncthreads();
   const bool listed = total <= kListMost;
 
-  // Stable counting sort by bin: one wave places the list 64 at a time.
-  if (listed && wave == 0) {
-    int carry = 0;
-    for (int b = lane; b < kBins; b += kWave) {
-      const int n = next[b], incl = wave_incl_scan(n);
-      first[b] = next[b] = carry + incl - n;
-      carry += readlane(incl, kWave - 1);
+  if (total == 0) { // rows without a token, the most of a large table
+    const int64_t vecs = a.dim / VEC, all = rows * vecs;
+    O *const out = static_cast<O *>(a.out) + row0 * a.out_stride;
+    float zero[VEC] = {};
+    if (a.out_stride == a.dim) {
+      for (int64_t i = tid; i < all; i += 256) store_f32<VEC>(out + i * VEC, zero);
+    } else {
+      for (int64_t i = tid; i < all; i += 256)
+        store_f32<VEC>(out + i / vecs * a.out_stride + i % vecs * VEC, zero);
     }
-    if (lane == 0) first[kBins] = carry;
-    wave_lds_order();
+    return;
+  }
+
+  if (listed) {
+    // Stable counting sort by bin: two bins per thread, then one wave places
+    // the list 64 at a time.
+    __syncthreads();
+    const int n0 = next[2 * tid], n1 = next[2 * tid + 1];
+    int sum;
+    const int at = prefix(n0 + n1, sum);
+    first[2 * tid] = next[2 * tid] = at;
+    first[2 * tid + 1] = next[2 * tid + 1] = at + n0;
+    if (tid == 255) first[kBins] = sum;
+    __syncthreads();
+  }
+  if (listed && wave == 0) {
     for (int i0 = 0; i0 < total; i0 += kWave) {
       const bool live = i0 + lane < total;
       const uint32_t bin = live ? local[i0 + lane] : 0;

@@ -74,6 +74,25 @@ template <int L, int N> struct RowSum {
   }
 };
 
+// A lane's part of weight or bias, or `value` where there is none.
+template <int VEC, int L, int C>
+__device__ __forceinline__ void load_vector(const void *p, int type, int64_t dim, float value,
+                                            int lane, float (&out)[C][VEC]) {
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) out[c][i] = value;
+  }
+  if (!p) return;
+  with_type(p, type, [&](auto *w) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const int col = (c * L + lane) * VEC;
+      if (col < dim) load_f32<VEC>(w + col, out[c]);
+    }
+  });
+}
+
 template <typename T, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
   constexpr int kGroups = norm_block(L) / L;
@@ -83,15 +102,8 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
   const float dim = static_cast<float>(a.dim);
 
   float w[C][VEC], b[C][VEC];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int64_t col = (c * L + lane) * VEC + i;
-      w[c][i] = a.weight && col < a.dim ? load_typed(a.weight, a.weight_type, col) : 1.0f;
-      b[c][i] = a.bias && col < a.dim ? load_typed(a.bias, a.weight_type, col) : 0.0f;
-    }
-  }
+  load_vector<VEC, L>(a.weight, a.weight_type, a.dim, 1.0f, lane, w);
+  load_vector<VEC, L>(a.bias, a.weight_type, a.dim, 0.0f, lane, b);
 
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < a.rows;
        first += static_cast<int64_t>(gridDim.x) * kGroups) {
@@ -165,8 +177,9 @@ template <typename T> __global__ void __launch_bounds__(1024) layer_norm_long_ke
     row_sum(s);
     const float rstd = 1.0f / sqrtf(s[0] / dim + a.eps);
     for (int64_t i = threadIdx.x; i < a.dim; i += 1024) {
-      const float w = a.weight ? load_typed(a.weight, a.weight_type, i) : 1.0f;
-      const float b = a.bias ? load_typed(a.bias, a.weight_type, i) : 0.0f;
+      float w = 1.0f, b = 0.0f;
+      if (a.weight) with_type(a.weight, a.weight_type, [&](auto *p) { w = static_cast<float>(p[i]); });
+      if (a.bias) with_type(a.bias, a.weight_type, [&](auto *p) { b = static_cast<float>(p[i]); });
       y[i] = static_cast<T>((static_cast<float>(x[i]) - mean) * rstd * w + b);
     }
     if (threadIdx.x == 0) {
@@ -193,16 +206,8 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
   const float dim = static_cast<float>(a.dim);
 
-  float w[C][VEC], dw[C][VEC], db[C][VEC];
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      const int64_t col = (c * L + lane) * VEC + i;
-      w[c][i] = a.weight && col < a.dim ? load_typed(a.weight, a.weight_type, col) : 1.0f;
-      dw[c][i] = db[c][i] = 0.0f;
-    }
-  }
+  float w[C][VEC], dw[C][VEC] = {}, db[C][VEC] = {};
+  load_vector<VEC, L>(a.weight, a.weight_type, a.dim, 1.0f, lane, w);
 
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < a.rows;
        first += static_cast<int64_t>(gridDim.x) * kGroups) {
@@ -306,7 +311,8 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(NormGradArgs
     const float mean = a.mean[row], rstd = a.rstd[row];
     float s[2] = {0.0f, 0.0f};
     for (int64_t i = threadIdx.x; i < a.dim; i += 1024) {
-      const float w = a.weight ? load_typed(a.weight, a.weight_type, i) : 1.0f;
+      float w = 1.0f;
+      if (a.weight) with_type(a.weight, a.weight_type, [&](auto *p) { w = static_cast<float>(p[i]); });
       const float h = (static_cast<float>(x[i]) - mean) * rstd, d = static_cast<float>(dy[i]);
       s[0] += d * w;
       s[1] += d * w * h;
@@ -319,7 +325,8 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(NormGradArgs
     row_sum(s);
     const float m1 = s[0] / dim, m2 = s[1] / dim;
     for (int64_t i = threadIdx.x; i < a.dim; i += 1024) {
-      const float w = a.weight ? load_typed(a.weight, a.weight_type, i) : 1.0f;
+      float w = 1.0f;
+      if (a.weight) with_type(a.weight, a.weight_type, [&](auto *p) { w = static_cast<float>(p[i]); });
       const float h = (static_cast<float>(x[i]) - mean) * rstd, d = static_cast<float>(dy[i]);
       dx[i] = static_cast<T>((d * w - m1 - h * m2) * rstd);
     }
@@ -421,7 +428,8 @@ template <typename T> int32_t norm_typed(const NormArgs &a, void *stream) {
   if (a.dim > kNormMostDim)
     return launch(layer_norm_long_kernel<T>, dim3(std::min(a.rows, kMaxNormBlocks)), dim3(1024),
                   stream, a);
-  const int vec = row_vec(sizeof(T), a.dim, {a.x_stride, a.y_stride}, {a.x, a.y});
+  const int vec = row_vec(sizeof(T), a.dim, {a.x_stride, a.y_stride},
+                          {a.x, a.y, a.weight, a.bias});
   if constexpr (sizeof(T) == 2) {
     if (vec == 8) return pick_norm<T, 8>(a, stream);
   }
@@ -434,7 +442,7 @@ int32_t norm_grad_typed(const NormGradArgs &a, int64_t blocks, void *stream) {
   if (a.dim > kNormGradMostDim)
     return launch(layer_norm_grad_long_kernel<T>, dim3(blocks), dim3(1024), stream, a);
   const int vec = row_vec(sizeof(T), a.dim, {a.x_stride, a.dy_stride, a.dx_stride},
-                          {a.x, a.dy, a.dx});
+                          {a.x, a.dy, a.dx, a.weight});
   if constexpr (sizeof(T) == 2) {
     if (vec == 8) return pick_norm_grad<T, 8>(a, blocks, stream);
   }

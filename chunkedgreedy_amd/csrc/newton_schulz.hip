@@ -50,7 +50,6 @@ struct OrthoArgs {
   int64_t g_batch, g_stride;    // of g, in elements
   int mp, np;                   // padded
   int tall;                     // X = G^T
-  int type;
   double eps;
   float a, b, c;
   double *partial;              // [batch][kNormBlocks]
@@ -79,13 +78,15 @@ __device__ __forceinline__ uint2 *col_place(uint4 *p, int k_blocks, int i0, int 
 // Stores one wave's 32 x 32 block with row i0 and column j0, scaled: lane l
 // holds column l % 32, rows 8 q + 4 (l / 32) + e in v[4 q + e].  by_col
 // receives it with columns as operand rows, by_row (if not null) with its own
-// rows, which 8 neighbouring columns of a row take a turn through LDS for;
-// k_col and k_row are their numbers of 16-column blocks.
+// rows, which 8 neighbouring columns of a row take a turn through LDS for
+// (`stage`, which may be the block's own place in by_row); k_col and k_row
+// are their numbers of 16-column blocks.
 __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col, int k_col,
                                             uint4 *by_row, int k_row, int i0, int j0,
                                             uint16_t *stage) {
   const int lane = lane_id();
   uint32_t half[2][16];
+  u32x4 held[2][2];
 #pragma unroll
   for (int r = 0; r < 16; ++r) split_halves(v[r], half[0][r], half[1][r]);
 #pragma unroll
@@ -102,13 +103,20 @@ __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col,
           static_cast<uint16_t>(h[r]);
     wave_lds_order();
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int row = lane % 32, part = lane / 32 + 2 * s; // 8 columns from 8 part
-      const int64_t block = static_cast<int64_t>(i0 / 32) * k_row + j0 / 16 + part / 2;
-      by_row[(block * 2 + plane) * kWave + row + 32 * (part % 2)] =
-          *reinterpret_cast<const uint4 *>(stage + row * kStageRow + 8 * part);
-    }
+    for (int s = 0; s < 2; ++s)
+      held[plane][s] = *reinterpret_cast<const u32x4 *>(stage + lane % 32 * kStageRow +
+                                                        8 * (lane / 32 + 2 * s));
     wave_lds_order();
+  }
+  if (!by_row) return;
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    const int part = lane / 32 + 2 * s; // 8 columns from 8 part
+    const int64_t block = static_cast<int64_t>(i0 / 32) * k_row + j0 / 16 + part / 2;
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane)
+      *reinterpret_cast<u32x4 *>(by_row + (block * 2 + plane) * kWave + lane % 32 +
+                                 32 * (part % 2)) = held[plane][s];
   }
 }
 
@@ -176,6 +184,7 @@ __global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(OrthoArgs a) {
 }
 
 // Packs X = G / (|G| + eps), 64 x 64 per workgroup, a 32 x 32 block per wave.
+template <typename T>
 __global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int norm_blocks) {
   __shared__ double part[kBlock];
   __shared__ __attribute__((aligned(16))) uint16_t stage[4][32 * kStageRow];
@@ -193,16 +202,17 @@ __global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int nor
   const int i0 = blockIdx.x / across * 64 + wave / 2 * 32;
   const int j0 = blockIdx.x % across * 64 + wave % 2 * 32;
   const int j = j0 + lane % 32;
+  const T *const g = static_cast<const T *>(a.g) + z * a.g_batch;
   float v[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
     const int i = i0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
     v[r] = 0.0f;
-    if (i < a.m && j < a.n) {
-      const int64_t at = a.tall ? j * a.g_stride + i : i * a.g_stride + j;
-      v[r] = static_cast<float>(load_typed(a.g, a.type, z * a.g_batch + at) * scale);
-    }
+    if (i < a.m && j < a.n)
+      v[r] = static_cast<float>(g[a.tall ? j * a.g_stride + i : i * a.g_stride + j]);
   }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) v[r] = static_cast<float>(v[r] * scale);
   const int64_t units = packed_units(a.mp, a.np);
   store_block(v, a.xt + z * units, a.mp / 16, a.x + z * units, a.np / 16, i0, j0, stage[wave]);
 }
@@ -212,6 +222,7 @@ __global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int nor
 enum Product { kGram, kPoly, kUpdate, kLast };
 
 // Writes a block of the result, unscaled.
+template <typename T>
 __device__ __forceinline__ void write_block(const OrthoArgs &a, int64_t z, int i0, int j0,
                                             const float (&v)[16]) {
   const int64_t j = j0 + lane_id() % 32;
@@ -219,13 +230,13 @@ __device__ __forceinline__ void write_block(const OrthoArgs &a, int64_t z, int i
   for (int r = 0; r < 16; ++r) {
     const int64_t i = i0 + 8 * (r / 4) + 4 * (lane_id() / 32) + r % 4;
     if (i < a.m && j < a.n)
-      store_typed(a.out, a.type, z * a.m * a.n + (a.tall ? j * a.m + i : i * a.n + j),
-                  v[r] * (1.0f / kScale));
+      static_cast<T *>(a.out)[z * a.m * a.n + (a.tall ? j * a.m + i : i * a.n + j)] =
+          static_cast<T>(v[r] * (1.0f / kScale));
   }
 }
 
 // The epilogue of a product for one wave's block: v holds C, scaled once.
-template <int WHAT>
+template <int WHAT, typename T>
 __device__ __forceinline__ void finish_block(const OrthoArgs &a, int64_t z, bool mirror, int i0,
                                              int j0, float (&v)[16], uint16_t *stage) {
   const int64_t xu = packed_units(a.mp, a.np), mu = packed_units(a.mp, a.mp);
@@ -248,7 +259,7 @@ __device__ __forceinline__ void finish_block(const OrthoArgs &a, int64_t z, bool
     if constexpr (WHAT == kUpdate)
       store_block(v, a.xt_next + z * xu, km, a.x + z * xu, kn, i0, j0, stage);
     else
-      write_block(a, z, i0, j0, v);
+      write_block<T>(a, z, i0, j0, v);
   }
 }
 
@@ -268,7 +279,7 @@ __device__ __forceinline__ void triangle_tile(int t, int across, int &ti, int &t
 //   kPoly:   P = Q = A;          writes B = b A + c C
 //   kUpdate: P = B, Q = X^T;     writes X = a X + C in both orders
 //   kLast:   the same to out, rounded to its type
-template <int WHAT, int TILE>
+template <int WHAT, int TILE, typename T>
 __global__ void __launch_bounds__(kBlock) ortho_product_kernel(OrthoArgs a) {
   constexpr int kRows = TILE / 32;     // blocks of 32 rows of each operand
   constexpr int kSide = kRows / 2;     // of a wave
@@ -365,18 +376,23 @@ __global__ void __launch_bounds__(kBlock) ortho_product_kernel(OrthoArgs a) {
       float v[16];
 #pragma unroll
       for (int r = 0; r < 16; ++r) v[r] = acc[bi][bj][r] * (1.0f / kScale);
-      finish_block<WHAT>(a, z, ti != tj, i0, j0, v, stage);
+      finish_block<WHAT, T>(a, z, ti != tj, i0, j0, v, stage);
     }
   }
 }
 
-// The same for products of few tiles: 64 x 64 per workgroup, whose four waves
-// each take a quarter of the columns and read their operands straight from
-// memory (in the units' own order, so without LDS); the four sums meet in LDS,
-// a block of 32 x 32 per wave.
-template <int WHAT> __global__ void __launch_bounds__(kBlock) ortho_split_kernel(OrthoArgs a) {
+// The same for products of few tiles: 64 x 64 per workgroup, whose eight waves
+// each take an eighth of the columns and read their operands straight from
+// memory (in the units' own order, so without LDS), four steps ahead; the
+// sums meet in LDS, a block of 32 x 32 for each of four waves.
+constexpr int kSplitWaves = 8;
+constexpr int kAhead = 4;
+
+template <int WHAT, typename T>
+__global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoArgs a) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
-  __shared__ float sums[4][4][16][kWave];
+  constexpr int kHalf = kSplitWaves / 2;
+  __shared__ float sums[kHalf][4][16][kWave];
   const int64_t z = blockIdx.y;
   const int64_t xu = packed_units(a.mp, a.np), mu = packed_units(a.mp, a.mp);
   const uint4 *const p = WHAT == kGram ? a.x + z * xu : WHAT == kPoly ? a.gram + z * mu : a.poly + z * mu;
@@ -392,98 +408,122 @@ template <int WHAT> __global__ void __launch_bounds__(kBlock) ortho_split_kernel
   }
   const int wave = threadIdx.x / kWave, lane = lane_id();
   const int64_t step = static_cast<int64_t>(k_blocks) * 2 * kWave;
-  const int mine = k_blocks / 4; // padded columns: a multiple of 8 blocks
-  const uint4 *const pt = p + ti * 2 * step + static_cast<int64_t>(wave * mine) * 2 * kWave + lane;
-  const uint4 *const qt = q + tj * 2 * step + static_cast<int64_t>(wave * mine) * 2 * kWave + lane;
+  const int mine = k_blocks / kSplitWaves; // padded columns: a multiple of 8 blocks
+  const int64_t first = static_cast<int64_t>(wave * mine) * 2 * kWave + lane;
+  const uint4 *const pt = p + ti * 2 * step + first;
+  const uint4 *const qt = q + tj * 2 * step + first;
 
   f32x16 acc[2][2] = {};
-  struct Operands {
-    u32x4 v[2][2][2]; // operand, block of 32 rows, hi and lo
-  };
-  auto fetch = [&](int k) {
-    Operands o;
+  u32x4 next[kAhead][2][2][2]; // step, operand, block of 32 rows, hi and lo
+  auto fetch = [&](u32x4(&o)[2][2][2], int k) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        o.v[0][i][h] = *reinterpret_cast<const u32x4 *>(pt + i * step + (k * 2 + h) * kWave);
-        o.v[1][i][h] = *reinterpret_cast<const u32x4 *>(qt + i * step + (k * 2 + h) * kWave);
-      }
-    }
-    return o;
-  };
-  auto multiply = [&](const Operands &o) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const f16x8 ph = __builtin_bit_cast(f16x8, o.v[0][i][0]), pl = __builtin_bit_cast(f16x8, o.v[0][i][1]);
-        const f16x8 qh = __builtin_bit_cast(f16x8, o.v[1][j][0]), ql = __builtin_bit_cast(f16x8, o.v[1][j][1]);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc[i][j], 0, 0, 0);
-        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc[i][j], 0, 0, 0);
+        o[0][i][h] = *reinterpret_cast<const u32x4 *>(pt + i * step + (k * 2 + h) * kWave);
+        o[1][i][h] = *reinterpret_cast<const u32x4 *>(qt + i * step + (k * 2 + h) * kWave);
       }
     }
   };
-  // Two steps under way (mine is even).
-  Operands even = fetch(0), odd = fetch(1);
-  for (int k = 0; k < mine; k += 2) {
-    multiply(even);
-    even = fetch(min(k + 2, mine - 1));
-    multiply(odd);
-    odd = fetch(min(k + 3, mine - 1));
+#pragma unroll
+  for (int d = 0; d < kAhead; ++d) fetch(next[d], min(d, mine - 1));
+  for (int k0 = 0; k0 < mine; k0 += kAhead) {
+#pragma unroll
+    for (int d = 0; d < kAhead; ++d) {
+      if (k0 + d < mine) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const f16x8 ph = __builtin_bit_cast(f16x8, next[d][0][i][0]);
+            const f16x8 pl = __builtin_bit_cast(f16x8, next[d][0][i][1]);
+            const f16x8 qh = __builtin_bit_cast(f16x8, next[d][1][j][0]);
+            const f16x8 ql = __builtin_bit_cast(f16x8, next[d][1][j][1]);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc[i][j], 0, 0, 0);
+          }
+        }
+        fetch(next[d], min(k0 + d + kAhead, mine - 1));
+      }
+    }
   }
+  if (wave >= kHalf) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+    for (int b = 0; b < 4; ++b) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) sums[wave][2 * i + j][r][lane] = acc[i][j][r];
+      for (int r = 0; r < 16; ++r) sums[wave - kHalf][b][r][lane] = acc[b / 2][b % 2][r];
     }
   }
   __syncthreads();
+  if (wave < kHalf) {
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sums[wave][b][r][lane] += acc[b / 2][b % 2][r];
+    }
+  }
+  __syncthreads();
+  if (wave >= kHalf) return;
   float v[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r)
     v[r] = ((sums[0][wave][r][lane] + sums[1][wave][r][lane]) +
             (sums[2][wave][r][lane] + sums[3][wave][r][lane])) *
            (1.0f / kScale);
-  __syncthreads();
-  uint16_t *const stage = reinterpret_cast<uint16_t *>(&sums[wave][0][0][0]);
-  finish_block<WHAT>(a, z, ti != tj, ti * 64 + wave / 2 * 32, tj * 64 + wave % 2 * 32, v, stage);
+  // Only this wave reads block `wave` of the sums: one of them becomes its stage.
+  wave_lds_order();
+  uint16_t *const stage = reinterpret_cast<uint16_t *>(&sums[0][wave][0][0]);
+  finish_block<WHAT, T>(a, z, ti != tj, ti * 64 + wave / 2 * 32, tj * 64 + wave % 2 * 32, v, stage);
 }
 
 // A whole matrix in one workgroup, X and X^T in LDS (at most 16 blocks of
 // 32 x 32, padded to 32): its products take less than a launch each.  Eight
-// waves take two blocks of the result each; A, then B, takes X's place until
-// the new X does.
-constexpr int kWholeBlocks = 16;
+// waves take two neighbouring blocks of the result each; A, then B, takes X's
+// place until the new X does.  A and B are computed whole: a wave per two
+// blocks is there anyway, and needs no mirrored store.
 constexpr int kWholeWaves = 8;
+constexpr int kWholeBlocks = 2 * kWholeWaves;
 constexpr int kWholeUnits = kWholeBlocks * 32 * 32 / 4;
 
+// Whether every wave has at most one pair of neighbouring blocks of X (and of
+// the square A, which is no larger).
+constexpr bool ortho_whole(int64_t mp, int64_t np) {
+  return mp / 32 * ((np / 32 + 1) / 2) <= kWholeWaves;
+}
+
+template <typename T>
 __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoArgs a, int steps) {
   __shared__ __attribute__((aligned(16))) uint4 x[kWholeUnits], xt[kWholeUnits];
-  __shared__ __attribute__((aligned(16))) uint16_t stages[kWholeWaves][32 * kStageRow];
   __shared__ double part[kWholeWaves];
   const int64_t z = blockIdx.x;
   const int wave = threadIdx.x / kWave, lane = lane_id();
   const int mb = a.mp / 32, nb = a.np / 32; // blocks down and across
-  uint16_t *const stage = stages[wave];
-  const int wide = mb * nb, square = mb * (mb + 1) / 2;
+  const int km = 2 * mb, kn = 2 * nb;       // blocks of 16 columns
+  // Blocks (bi, bj) and (bi, bj + 1) of X, and of A and B.
+  const int pairs_x = (nb + 1) / 2, pairs_a = (mb + 1) / 2;
+  const int xi = wave / pairs_x, xj = wave % pairs_x * 2;
+  const int ai = wave / pairs_a, aj = wave % pairs_a * 2;
+  const int blocks_x = xi < mb ? min(2, nb - xj) : 0, blocks_a = ai < mb ? min(2, mb - aj) : 0;
 
+  const T *const g = static_cast<const T *>(a.g) + z * a.g_batch;
   float v[2][16];
   double s = 0.0;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int block = wave + t * kWholeWaves;
-    const int i0 = block / nb * 32, j = block % nb * 32 + lane % 32;
+    const int j = (xj + t) * 32 + lane % 32;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int i = i0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+      const int i = xi * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
       v[t][r] = 0.0f;
-      if (block < wide && i < a.m && j < a.n)
-        v[t][r] = load_typed(a.g, a.type,
-                             z * a.g_batch + (a.tall ? j * a.g_stride + i : i * a.g_stride + j));
+      if (t < blocks_x && i < a.m && j < a.n)
+        v[t][r] = static_cast<float>(g[a.tall ? j * a.g_stride + i : i * a.g_stride + j]);
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
       s += static_cast<double>(v[t][r]) * v[t][r];
     }
   }
@@ -493,79 +533,94 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
   s = 0.0;
   for (int w = 0; w < kWholeWaves; ++w) s += part[w];
   const double scale = static_cast<double>(kScale) / (sqrt(s) + a.eps);
+
+  // A block's place in x is its own until the barrier after: its stage.
+  auto store_x = [&](int t) {
+    uint4 *const place = x + (xi * kn + (xj + t) * 2) * 2 * kWave;
+    store_block(v[t], xt, km, x, kn, xi * 32, (xj + t) * 32, reinterpret_cast<uint16_t *>(place));
+  };
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
-    const int block = wave + t * kWholeWaves;
-    if (block >= wide) continue;
+    if (t >= blocks_x) continue;
 #pragma unroll
     for (int r = 0; r < 16; ++r) v[t][r] = static_cast<float>(v[t][r] * scale);
-    store_block(v[t], xt, 2 * mb, x, 2 * nb, block / nb * 32, block % nb * 32, stage);
+    store_x(t);
   }
   __syncthreads();
 
-  // v[t] = block (bi, bj) of P Q^T, unscaled once; operands with k blocks of 16 columns.
-  auto product = [&](const uint4 *p, const uint4 *q, int k_blocks, int bi, int bj, float (&out)[16]) {
-    f32x16 acc = {};
+  // v = blocks (bi, bj) and (bi, bj + more) of P Q^T, operands of k blocks.
+  auto product = [&](const uint4 *p, const uint4 *q, int k_blocks, int bi, int bj, int more) {
+    f32x16 acc[2] = {};
     const uint4 *const pt = p + bi * k_blocks * 2 * kWave + lane;
     const uint4 *const qt = q + bj * k_blocks * 2 * kWave + lane;
-#pragma unroll 2
-    for (int k = 0; k < k_blocks; ++k) {
-      const f16x8 ph = __builtin_bit_cast(f16x8, pt[k * 2 * kWave]);
-      const f16x8 pl = __builtin_bit_cast(f16x8, pt[(k * 2 + 1) * kWave]);
-      const f16x8 qh = __builtin_bit_cast(f16x8, qt[k * 2 * kWave]);
-      const f16x8 ql = __builtin_bit_cast(f16x8, qt[(k * 2 + 1) * kWave]);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl, qh, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, ql, acc, 0, 0, 0);
-      acc = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph, qh, acc, 0, 0, 0);
-    }
+    const uint4 *const rt = qt + more * k_blocks * 2 * kWave;
+    for (int k = 0; k < k_blocks * 2 * kWave; k += 4 * kWave) { // an even number of blocks
+      f16x8 o[2][3][2]; // block, operand, hi and lo
 #pragma unroll
-    for (int r = 0; r < 16; ++r) out[r] = acc[r] * (1.0f / kScale);
-  };
-
-  for (int step = 0; step < steps; ++step) {
+      for (int d = 0; d < 2; ++d) {
 #pragma unroll
-    for (int what = 0; what < 2; ++what) { // A = X X^T, then B = b A + c A A
-      int bi[2], bj[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int block = wave + t * kWholeWaves;
-        if (block >= square) continue;
-        triangle_tile(block, mb, bi[t], bj[t]);
-        product(x, x, what ? 2 * mb : 2 * nb, bi[t], bj[t], v[t]);
-        if (what) {
-          float old[16];
-          load_block(x, 2 * mb, bi[t] * 32, bj[t] * 32, old);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) v[t][r] = a.b * old[r] + a.c * v[t][r];
+        for (int h = 0; h < 2; ++h) {
+          const int at = k + (2 * d + h) * kWave;
+          o[d][0][h] = __builtin_bit_cast(f16x8, pt[at]);
+          o[d][1][h] = __builtin_bit_cast(f16x8, qt[at]);
+          o[d][2][h] = __builtin_bit_cast(f16x8, rt[at]);
         }
       }
-      __syncthreads();
 #pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        if (wave + t * kWholeWaves >= square) continue;
-        store_block(v[t], x, 2 * mb, bi[t] != bj[t] ? x : nullptr, 2 * mb, bi[t] * 32, bj[t] * 32, stage);
+      for (int d = 0; d < 2; ++d) {
+#pragma unroll
+        for (int h = 0; h < 3; ++h) { // lo hi, hi lo, hi hi
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+            acc[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(o[d][0][h == 0], o[d][1 + t][h == 1],
+                                                            acc[t], 0, 0, 0);
+        }
       }
-      __syncthreads();
     }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int block = wave + t * kWholeWaves;
-      if (block >= wide) continue;
-      product(x, xt, 2 * mb, block / nb, block % nb, v[t]);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[t][r] = acc[t][r] * (1.0f / kScale);
+    }
+  };
+  auto store_a = [&]() {
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (t < blocks_a) store_block(v[t], x, km, nullptr, 0, ai * 32, (aj + t) * 32, nullptr);
+    __syncthreads();
+  };
+
+  for (int step = 0; step < steps; ++step) {
+    if (blocks_a) product(x, x, kn, ai, aj, blocks_a - 1);
+    store_a();
+    if (blocks_a) product(x, x, km, ai, aj, blocks_a - 1);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t >= blocks_a) continue;
       float old[16];
-      load_block(xt, 2 * mb, block / nb * 32, block % nb * 32, old);
+      load_block(x, km, ai * 32, (aj + t) * 32, old);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[t][r] = a.b * old[r] + a.c * v[t][r];
+    }
+    store_a();
+    if (blocks_x) product(x, xt, km, xi, xj, blocks_x - 1);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (t >= blocks_x) continue;
+      float old[16];
+      load_block(xt, km, xi * 32, (xj + t) * 32, old);
 #pragma unroll
       for (int r = 0; r < 16; ++r) v[t][r] = a.a * old[r] + v[t][r];
     }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const int block = wave + t * kWholeWaves;
-      if (block >= wide) continue;
+      if (t >= blocks_x) continue;
       if (step + 1 < steps)
-        store_block(v[t], xt, 2 * mb, x, 2 * nb, block / nb * 32, block % nb * 32, stage);
+        store_x(t);
       else
-        write_block(a, z, block / nb * 32, block % nb * 32, v[t]);
+        write_block<T>(a, z, xi * 32, (xj + t) * 32, v[t]);
     }
     __syncthreads();
   }
@@ -583,7 +638,7 @@ OrthoLayout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
   OrthoLayout l{};
   l.m = std::min(rows, cols), l.n = std::max(rows, cols);
   l.mp = ceil_div64(l.m, 32) * 32, l.np = ceil_div64(l.n, 32) * 32;
-  l.whole = l.mp * l.np <= kWholeBlocks * 32 * 32;
+  l.whole = ortho_whole(l.mp, l.np);
   if (l.whole) return l;
   l.mp = ceil_div64(l.m, kPad) * kPad, l.np = ceil_div64(l.n, kPad) * kPad;
   size_t at = 0;
@@ -647,15 +702,37 @@ template <typename T> int32_t run_norm(const OrthoArgs &a, int blocks, void *str
   return launch(ortho_norm_kernel<T, 1>, dim3(blocks, a.batch), dim3(kNormThreads), stream, a);
 }
 
-template <int WHAT> int32_t run_product(const OrthoArgs &a, void *stream) {
+template <int WHAT, typename T = float> int32_t run_product(const OrthoArgs &a, void *stream) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
   auto tiles = [&](int64_t tile) {
     const int64_t down = a.mp / tile, across = a.np / tile;
     return kSymmetric ? down * (down + 1) / 2 : down * across;
   };
   if (tiles(128) * a.batch < kFewTiles)
-    return launch(ortho_split_kernel<WHAT>, dim3(tiles(64), a.batch), dim3(kBlock), stream, a);
-  return launch(ortho_product_kernel<WHAT, 128>, dim3(tiles(128), a.batch), dim3(kBlock), stream, a);
+    return launch(ortho_split_kernel<WHAT, T>, dim3(tiles(64), a.batch), dim3(kSplitWaves * kWave),
+                  stream, a);
+  return launch(ortho_product_kernel<WHAT, 128, T>, dim3(tiles(128), a.batch), dim3(kBlock),
+                stream, a);
+}
+
+template <typename T>
+int32_t ortho_typed(OrthoArgs a, const OrthoLayout &l, int32_t steps, void *stream) {
+  if (l.whole)
+    return launch(ortho_whole_kernel<T>, dim3(a.batch), dim3(kWholeWaves * kWave), stream, a, steps);
+  const int norm_blocks = static_cast<int>(
+      std::clamp<int64_t>(a.m * a.n / (16 * kNormThreads), 1, kNormBlocks));
+  int32_t rc = run_norm<T>(a, norm_blocks, stream);
+  if (rc == SPORDER_OK)
+    rc = launch(ortho_pack_kernel<T>, dim3(l.mp / 64 * (l.np / 64), a.batch), dim3(kBlock), stream,
+                a, norm_blocks);
+  for (int32_t k = 0; k < steps && rc == SPORDER_OK; ++k) {
+    rc = run_product<kGram>(a, stream);
+    if (rc == SPORDER_OK) rc = run_product<kPoly>(a, stream);
+    if (rc == SPORDER_OK)
+      rc = k + 1 < steps ? run_product<kUpdate>(a, stream) : run_product<kLast, T>(a, stream);
+    std::swap(a.xt, a.xt_next);
+  }
+  return rc;
 }
 
 } // namespace
@@ -683,7 +760,7 @@ int32_t sporder_newton_schulz(void *stream, int32_t type, int64_t batch, int64_t
   if (l.bytes > 0 && (!d_work || !aligned_to(d_work, 256) || work_bytes < l.bytes))
     return SPORDER_BAD_ARGUMENT;
   char *const w = static_cast<char *>(d_work);
-  OrthoArgs args{d_g,
+  const OrthoArgs args{d_g,
                  d_out,
                  batch,
                  l.m,
@@ -693,7 +770,6 @@ int32_t sporder_newton_schulz(void *stream, int32_t type, int64_t batch, int64_t
                  static_cast<int>(l.mp),
                  static_cast<int>(l.np),
                  rows > cols,
-                 type,
                  eps,
                  static_cast<float>(a),
                  static_cast<float>(b),
@@ -704,24 +780,9 @@ int32_t sporder_newton_schulz(void *stream, int32_t type, int64_t batch, int64_t
                  reinterpret_cast<uint4 *>(w + l.xt_next),
                  reinterpret_cast<uint4 *>(w + l.gram),
                  reinterpret_cast<uint4 *>(w + l.poly)};
-  if (l.whole)
-    return launch(ortho_whole_kernel, dim3(batch), dim3(kWholeWaves * kWave), stream, args, steps);
-  const int norm_blocks = static_cast<int>(
-      std::clamp<int64_t>(rows * cols / (16 * kNormThreads), 1, kNormBlocks));
-  int32_t rc = type == SPORDER_TYPE_BF16  ? run_norm<bf16_t>(args, norm_blocks, stream)
-               : type == SPORDER_TYPE_F16 ? run_norm<f16_t>(args, norm_blocks, stream)
-                                          : run_norm<float>(args, norm_blocks, stream);
-  if (rc == SPORDER_OK)
-    rc = launch(ortho_pack_kernel, dim3(l.mp / 64 * (l.np / 64), batch), dim3(kBlock), stream, args,
-                norm_blocks);
-  for (int32_t k = 0; k < steps && rc == SPORDER_OK; ++k) {
-    rc = run_product<kGram>(args, stream);
-    if (rc == SPORDER_OK) rc = run_product<kPoly>(args, stream);
-    if (rc == SPORDER_OK)
-      rc = k + 1 < steps ? run_product<kUpdate>(args, stream) : run_product<kLast>(args, stream);
-    std::swap(args.xt, args.xt_next);
-  }
-  return rc;
+  if (type == SPORDER_TYPE_BF16) return ortho_typed<bf16_t>(args, l, steps, stream);
+  if (type == SPORDER_TYPE_F16) return ortho_typed<f16_t>(args, l, steps, stream);
+  return ortho_typed<float>(args, l, steps, stream);
 }
 
 } // extern "C"

@@ -38,6 +38,27 @@ __device__ __forceinline__ void store_f32(T *p, const float (&in)[VEC]) {
   *reinterpret_cast<Pack<T, VEC> *>(p) = q;
 }
 
+// The same past the caches, for output that is not read again soon: it leaves
+// them to what the kernel still reads.
+template <int VEC, typename T>
+__device__ __forceinline__ void stream_f32(T *p, const float (&in)[VEC]) {
+  using words = uint32_t __attribute__((ext_vector_type(4)));
+  Pack<T, VEC> q;
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) q.v[i] = static_cast<T>(in[i]);
+  if constexpr (sizeof(q) % 16 == 0) {
+#pragma unroll
+    for (int i = 0; i < static_cast<int>(sizeof(q) / 16); ++i)
+      __builtin_nontemporal_store(reinterpret_cast<const words *>(&q)[i],
+                                  reinterpret_cast<words *>(p) + i);
+  } else if constexpr (sizeof(q) == 8) {
+    __builtin_nontemporal_store(__builtin_bit_cast(uint64_t, q), reinterpret_cast<uint64_t *>(p));
+  } else {
+    static_assert(VEC == 1);
+    __builtin_nontemporal_store(q.v[0], p);
+  }
+}
+
 // Calls f with a pointer of the type known at run time.  The branch goes
 // around whole loops: one around each access would make them wait for one
 // another.
@@ -91,9 +112,9 @@ inline bool aligned_to(const void *p, size_t bytes) {
 
 constexpr int64_t kMostDim = int64_t(1) << 23; // elements of a row
 
-// Elements per access of rows whose wider type has `bytes_each` bytes: 16
-// bytes, or 4 elements, where the length, the strides and the bases (16-byte
-// aligned) allow it, else one element.
+// Elements per access of rows of `bytes_each` bytes an element: 16 bytes, or 4
+// elements, where the length, the strides and the bases (16-byte aligned)
+// allow it, else one element.
 inline int row_vec(int bytes_each, int64_t dim, std::initializer_list<int64_t> strides,
                    std::initializer_list<const void *> bases) {
   for (int vec : {16 / bytes_each, 4}) {

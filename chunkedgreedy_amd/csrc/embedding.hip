@@ -7,18 +7,21 @@
 // equal tokens in 32 bits, written once for every row of the table (zero rows
 // too).  Atomic additions would be one launch, but their order, and with it
 // the result, changes from run to run and a common token serialises them, so
-// the tokens are sorted instead, as far as the sums need it:
+// the tokens are sorted instead:
 //
 //   1. each tile of 4096 tokens is sorted in LDS (stable), and the table's
 //      rows, cut into spans, find where their tokens begin in it.  16 to 64
 //      neighbours of one token in that order (a common token: a hub) become
 //      one entry,
-//   2. whose sum a group of lanes forms;
+//   2. whose sum a workgroup forms;
 //   3. a workgroup per span gathers its entries from every tile, in the
-//      tiles' order, sorts them by row in LDS and adds up and writes each row.
+//      tiles' order, sorts them by row in LDS and writes them out by row;
+//   4. the table is written front to back, every lane a few vectors of a row
+//      and their sum (this is where the bytes are); a row that still has many
+//      entries is shared by a workgroup.
 //
-// A few tokens need no tiles: each span picks its own from all of them, in
-// one launch.
+// Few tokens need no tiles: each span picks its own from all of them and sums
+// its rows, in one launch.
 #include <algorithm>
 
 #include "dense.hpp"
@@ -79,7 +82,8 @@ constexpr int kTileRuns = kTileChunks * kChunkRuns;
 constexpr uint32_t kSummed = 0x80000000u; // an entry that is a run's sum
 constexpr int kSpanMost = 256;    // table rows per span
 constexpr int kListMost = 2048;   // a span's entries that fit the list in LDS
-constexpr int kAlone = 32;        // entries of a row that one group of lanes adds up
+constexpr int kAlone = 8;         // entries of a row that one lane adds up
+constexpr int kRowsMost = 1024;   // table rows per workgroup of the last launch
 
 struct GradArgs {
   const void *grad, *tokens;
@@ -88,15 +92,19 @@ struct GradArgs {
   float scale;
   int wide;
   int key_bits;
-  int span;      // table rows per workgroup of the last launch
+  int row_block; // table rows per workgroup of the last launch
+  int span;      // and of the one before it
   int64_t spans; // ceil(rows / span)
-  int64_t tiles; // 0: spans read the tokens themselves
+  int64_t tiles;
   uint32_t *keys;      // [tiles][kTile] the tiles' entries: row,
   uint32_t *sources;   // and token index, or run index | kSummed
   uint16_t *order;     // [tiles][kTile] the sorted order within the tile
-  uint16_t *runs;      // [tiles][kTileRuns] first place in the chunk and length; 0: none
+  uint32_t *runs;      // [tiles][kTileRuns] first place in the tile << 8 | length
+  int32_t *run_count;  // [tiles]
   uint16_t *starts;    // [tiles][spans + 1] first entry of each span
   float *sums;         // [tiles * kTileRuns][dim]
+  uint32_t *list;      // [count] the entries' sources by row, sums first
+  int32_t *row_start;  // [rows + 1] first entry in the list
 };
 
 // The table rows of tokens first, first + step, ... before a.count; `rows`
@@ -171,25 +179,23 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
       wave_lds_order();
     }
     __syncthreads();
-    // cnt[w][d] becomes the place of wave w's first item of digit d.
-    int total = 0;
-    if (tid < kDigits) {
+    // cnt[w][d] becomes the place of wave w's first item of digit d: a prefix
+    // over digits, then waves, four waves of a digit per thread.
+    constexpr int kPart = kTileWaves * kDigits / kTileBlock;
+    const int digit = tid / (kTileWaves / kPart), w0 = tid % (kTileWaves / kPart) * kPart;
+    int at[kPart], total = 0;
 #pragma unroll
-      for (int w = 0; w < kTileWaves; ++w) {
-        const int c = cnt[w][tid];
-        cnt[w][tid] = static_cast<uint16_t>(total);
-        total += c;
-      }
-      const int incl = wave_incl_scan(total);
-      if (lane == kWave - 1) wave_total[wave] = incl;
-      total = incl - total;
+    for (int w = 0; w < kPart; ++w) {
+      at[w] = total;
+      total += cnt[w0 + w][digit];
     }
+    const int incl = wave_incl_scan(total);
+    if (lane == kWave - 1) wave_total[wave] = incl;
     __syncthreads();
-    if (tid < kDigits) {
-      for (int w = 0; w < wave; ++w) total += wave_total[w];
+    int before = lane < wave ? wave_total[lane] : 0; // kTileWaves of them
+    before = wave_sum(before) + incl - total;
 #pragma unroll
-      for (int w = 0; w < kTileWaves; ++w) cnt[w][tid] = static_cast<uint16_t>(cnt[w][tid] + total);
-    }
+    for (int w = 0; w < kPart; ++w) cnt[w0 + w][digit] = static_cast<uint16_t>(before + at[w]);
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kTileRounds; ++r) {
@@ -206,6 +212,7 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
   // the run's first lane; every other token is its own.
   uint64_t held[kTileRounds]; // lanes that hold an entry
   uint64_t heads[kTileRounds]; // of them, those whose entry is a run
+  int length[kTileRounds];
 #pragma unroll
   for (int r = 0; r < kTileRounds; ++r) {
     const int chunk = wave * kTileRounds + r;
@@ -218,37 +225,50 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
     const bool run = k != none && end - begin >= kRun;
     heads[r] = ballot(run && lane == begin);
     held[r] = ballot(k != none && (!run || lane == begin));
-    if (lane == 0) chunk_entries[chunk] = __popcll(held[r]);
+    length[r] = end - begin;
+    if (lane == 0) chunk_entries[chunk] = __popcll(held[r]) | __popcll(heads[r]) << 16;
     a.order[base + chunk * kChunk + lane] = idx[from][chunk * kChunk + lane];
-    uint16_t *const runs = a.runs + tile * kTileRuns + chunk * kChunkRuns;
-    if (run && lane == begin)
-      runs[__popcll(heads[r] & below)] = static_cast<uint16_t>(begin << 8 | (end - begin));
-    if (lane < kChunkRuns && lane >= __popcll(heads[r])) runs[lane] = 0;
   }
   __syncthreads();
-  const int mine = chunk_entries[lane]; // kTileChunks = kWave: every wave holds all of them
+  // Entries and runs before each chunk, in the halves of a word; kTileChunks =
+  // kWave, so every wave holds all of them.
+  const int mine = chunk_entries[lane];
   const int place = wave_incl_scan(mine) - mine;
-  const int entries = wave_sum(mine);
+  const int all = wave_sum(mine), entries = all & 0xffff;
+  if (tid == 0) a.run_count[tile] = all >> 16;
   const int to = from ^ 1;
 #pragma unroll
   for (int r = 0; r < kTileRounds; ++r) {
     const int chunk = wave * kTileRounds + r;
     if ((held[r] >> lane) & 1) {
       const uint32_t k = key[from][chunk * kChunk + lane];
-      const int at = readlane(place, chunk) + __popcll(held[r] & below);
+      const int before = readlane(place, chunk);
+      const int at = (before & 0xffff) + __popcll(held[r] & below);
+      uint32_t what = static_cast<uint32_t>(base + idx[from][chunk * kChunk + lane]);
+      if ((heads[r] >> lane) & 1) {
+        const int run = (before >> 16) + __popcll(heads[r] & below);
+        a.runs[tile * kTileRuns + run] = static_cast<uint32_t>((chunk * kChunk + lane) << 8 | length[r]);
+        what = kSummed | static_cast<uint32_t>(tile * kTileRuns + run);
+      }
       key[to][at] = k;
       a.keys[base + at] = k;
-      a.sources[base + at] =
-          (heads[r] >> lane) & 1
-              ? kSummed | static_cast<uint32_t>(tile * kTileRuns + chunk * kChunkRuns +
-                                                __popcll(heads[r] & below))
-              : static_cast<uint32_t>(base + idx[from][chunk * kChunk + lane]);
+      a.sources[base + at] = what;
     }
   }
   __syncthreads();
-  for (int64_t s = tid; s <= a.spans; s += kTileBlock) {
+  // Each thread takes neighbouring spans and searches on from the last start:
+  // by doubling steps, then between the last two.
+  const int64_t per = ceil_div64(a.spans + 1, kTileBlock);
+  const int64_t last = min((tid + 1) * per, a.spans + 1);
+  int lo = 0; // entries before it are below the row
+  for (int64_t s = tid * per; s < last; ++s) {
     const int64_t row = s * a.span;
-    int lo = 0, hi = entries;
+    int width = s == tid * per ? kTile : 1, hi;
+    while ((hi = lo + width) <= entries && key[to][hi - 1] < row) {
+      lo = hi;
+      width *= 2;
+    }
+    hi = min(hi, entries + 1) - 1;
     while (lo < hi) {
       const int mid = (lo + hi) / 2;
       if (key[to][mid] < row)
@@ -260,67 +280,71 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
   }
 }
 
-// The sums of the runs, L lanes each.
+// The sums of the runs: a workgroup per run and slice of L VEC columns, L lanes
+// per token, so that all the loads of a run are under way at once.  A tile's
+// runs are dealt to kRunBlocks workgroups.
+constexpr int kRunBlocks = 32;
+
 template <typename T, int VEC, int L>
 __global__ void __launch_bounds__(256) embedding_run_kernel(GradArgs a) {
-  const int64_t run = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L;
-  if (run >= a.tiles * kTileRuns) return;
-  const int what = a.runs[run];
-  if (what == 0) return;
-  const int64_t tile = run / kTileRuns;
-  const int n = what & 0xff;
-  const uint16_t *const order =
-      a.order + tile * kTile + run % kTileRuns / kChunkRuns * kChunk + (what >> 8);
-  const T *const grad = static_cast<const T *>(a.grad) + tile * kTile * a.grad_stride;
-  for (int64_t c = (threadIdx.x % L) * VEC; c < a.dim; c += L * VEC) {
+  constexpr int kGroups = 256 / L, kWaves = 256 / kWave;
+  constexpr int kEach = kChunk / kGroups > 0 ? kChunk / kGroups : 1;
+  __shared__ float joined[kWaves][L * VEC];
+  const int64_t tile = blockIdx.x / kRunBlocks;
+  const int runs = a.run_count[tile];
+  const int group = threadIdx.x / L, lane = threadIdx.x % L, wave = threadIdx.x / kWave;
+  const int64_t c = (static_cast<int64_t>(blockIdx.y) * L + lane) * VEC;
+  const T *const grad = static_cast<const T *>(a.grad) + tile * kTile * a.grad_stride + c;
+  for (int run = blockIdx.x % kRunBlocks; run < runs; run += kRunBlocks) {
+    const uint32_t what = a.runs[tile * kTileRuns + run];
+    const int n = what & 0xff;
+    const uint16_t *const order = a.order + tile * kTile + (what >> 8);
+    int64_t at[kEach];
+#pragma unroll
+    for (int d = 0; d < kEach; ++d) at[d] = order[min(d * kGroups + group, n - 1)] * a.grad_stride;
+    float v[kEach][VEC] = {};
+#pragma unroll
+    for (int d = 0; d < kEach; ++d)
+      if (c < a.dim && d * kGroups + group < n) load_f32<VEC>(grad + at[d], v[d]);
     float acc[VEC] = {};
-#pragma unroll 8
-    for (int i = 0; i < n; ++i) {
-      float v[VEC];
-      load_f32<VEC>(grad + order[i] * a.grad_stride + c, v);
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+    for (int d = 0; d < kEach; ++d) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += v[d][k];
     }
-    store_f32<VEC>(a.sums + run * a.dim + c, acc);
-  }
-}
-
-// Adds rows base[at[i] & ~kSummed], i in [i, end), to acc.
-template <typename T, int VEC>
-__device__ __forceinline__ void add_rows(const T *base, int64_t stride, const uint32_t *at, int i,
-                                         int end, float (&acc)[VEC]) {
-#pragma unroll 8
-  for (; i < end; ++i) {
-    float v[VEC];
-    load_f32<VEC>(base + (at[i] & ~kSummed) * stride, v);
+    __syncthreads(); // the run before has been read
 #pragma unroll
-    for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+    for (int k = 0; k < VEC; ++k) {
+#pragma unroll
+      for (int j = L; j < kWave; j <<= 1) acc[k] += lane_xor_f32(acc[k], j);
+      if (threadIdx.x % kWave < L) joined[wave][lane * VEC + k] = acc[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < L && c < a.dim) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        acc[k] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWaves; ++w) acc[k] += joined[w][lane * VEC + k];
+      }
+      store_f32<VEC>(a.sums + (tile * kTileRuns + run) * a.dim + c, acc);
+    }
   }
 }
 
-// One span of table rows, L lanes per row.  A row's entries are added in two
-// loops, the sums and the single tokens, so that several loads of each are
-// under way at once; a row of many entries (a hub) is shared by all the
-// groups of the workgroup, each a contiguous part, joined through LDS.
-template <typename T, typename O, int VEC, int L>
-__global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
-  constexpr int kGroups = 256 / L;
-  constexpr int kBins = 2 * kSpanMost; // sums of row r, tokens of row r
-  __shared__ uint32_t source[kListMost];
-  __shared__ uint32_t sorted[kListMost];
-  __shared__ uint16_t local[kListMost];
-  __shared__ int first[kBins + 1];
-  __shared__ int next[kBins];
-  __shared__ int wave_total[256 / kWave];
-  __shared__ float joined[kGroups][L * VEC];
-  const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  const uint64_t below = (uint64_t(1) << lane) - 1;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.span;
-  const int rows = static_cast<int>(min(static_cast<int64_t>(a.span), a.rows - row0));
-  const uint16_t *const starts = a.starts + blockIdx.x;
+// A span's entries in LDS.
+constexpr int kBins = 2 * kSpanMost; // sums of row r, tokens of row r
+constexpr int kSpanWaves = 256 / kWave;
+struct SpanList {
+  uint32_t source[kListMost];
+  uint16_t local[kListMost]; // their bins
+  int first[kBins + 1];
+  int next[kBins];
+  int wave_total[kSpanWaves];
 
-  // Exclusive prefix of one count per thread; `total` gets their sum.
-  auto prefix = [&](int n, int &sum) {
+  // Exclusive prefix of one count per thread; `sum` gets the total.
+  __device__ __forceinline__ int prefix(int n, int &sum) {
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
     const int incl = wave_incl_scan(n);
     __syncthreads(); // the totals of the call before have been read
     if (lane == kWave - 1) wave_total[wave] = incl;
@@ -328,66 +352,21 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
     int at = incl - n;
     sum = 0;
 #pragma unroll
-    for (int w = 0; w < 256 / kWave; ++w) {
+    for (int w = 0; w < kSpanWaves; ++w) {
       if (w < wave) at += wave_total[w];
       sum += wave_total[w];
     }
     return at;
-  };
-  auto append = [&](int at, uint32_t row, uint32_t what) {
-    if (at >= kListMost) return;
-    const int bin = 2 * static_cast<int>(row - row0) + ((what & kSummed) == 0);
-    source[at] = what;
-    local[at] = static_cast<uint16_t>(bin);
-    atomicAdd(&next[bin], 1);
-  };
-
-  // The entries, in the tiles' order, or the tokens in theirs.
-  next[tid] = next[tid + 256] = 0;
-  int total = 0;
-  if (a.tiles) {
-    for (int64_t t0 = 0; t0 < a.tiles; t0 += 256) {
-      const int64_t tile = t0 + tid;
-      int lo = 0, n = 0, sum;
-      if (tile < a.tiles) {
-        lo = starts[tile * (a.spans + 1)];
-        n = starts[tile * (a.spans + 1) + 1] - lo;
-      }
-      const int at = total + prefix(n, sum);
-      for (int64_t i = 0, e = tile * kTile + lo; i < n; ++i) append(at + i, a.keys[e + i], a.sources[e + i]);
-      total += sum;
-    }
-  } else {
-    constexpr int kEach = kListMost / 256;
-    const int64_t t0 = static_cast<int64_t>(tid) * kEach;
-    uint32_t row[kEach];
-    token_rows(a, t0, 1, row);
-    int n = 0;
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) n += row[k] >= row0 && row[k] < row0 + rows;
-    int at = prefix(n, total);
-#pragma unroll
-    for (int k = 0; k < kEach; ++k)
-      if (row[k] >= row0 && row[k] < row0 + rows) append(at++, row[k], static_cast<uint32_t>(t0 + k));
-  }
-  const bool listed = total <= kListMost;
-
-  if (total == 0) { // rows without a token, the most of a large table
-    const int64_t vecs = a.dim / VEC, all = rows * vecs;
-    O *const out = static_cast<O *>(a.out) + row0 * a.out_stride;
-    float zero[VEC] = {};
-    if (a.out_stride == a.dim) {
-      for (int64_t i = tid; i < all; i += 256) store_f32<VEC>(out + i * VEC, zero);
-    } else {
-      for (int64_t i = tid; i < all; i += 256)
-        store_f32<VEC>(out + i / vecs * a.out_stride + i % vecs * VEC, zero);
-    }
-    return;
   }
 
-  if (listed) {
-    // Stable counting sort by bin: two bins per thread, then one wave places
-    // the list 64 at a time.
+  __device__ __forceinline__ void clear() { next[threadIdx.x] = next[threadIdx.x + 256] = 0; }
+  static __device__ __forceinline__ int bin(int row, uint32_t what) {
+    return 2 * row + ((what & kSummed) == 0);
+  }
+
+  // From counts in next to first places, in next and first.
+  __device__ __forceinline__ void open() {
+    const int tid = threadIdx.x;
     __syncthreads();
     const int n0 = next[2 * tid], n1 = next[2 * tid + 1];
     int sum;
@@ -397,94 +376,273 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
     if (tid == 255) first[kBins] = sum;
     __syncthreads();
   }
-  if (listed && wave == 0) {
-    for (int i0 = 0; i0 < total; i0 += kWave) {
-      const bool live = i0 + lane < total;
-      const uint32_t bin = live ? local[i0 + lane] : 0;
-      const uint64_t peers = match_lanes(bin, 9) & ballot(live);
-      const int at = next[bin] + __popcll(peers & below);
-      wave_lds_order();
-      if (live) {
-        sorted[at] = source[i0 + lane];
-        if ((peers & below) == 0) next[bin] = at + __popcll(peers);
-      }
-      wave_lds_order();
-    }
-  }
-  __syncthreads();
 
-  const int group = tid / L;
-  const T *const grad = static_cast<const T *>(a.grad);
-  for (int r = group; listed && r < rows; r += kGroups) {
-    const int sums = first[2 * r], singles = first[2 * r + 1], end = first[2 * r + 2];
-    if (end - sums > kAlone && kGroups > 1) continue;
-    O *const out = static_cast<O *>(a.out) + (row0 + r) * a.out_stride;
-    for (int64_t c = (tid % L) * VEC; c < a.dim; c += L * VEC) {
-      float acc[VEC] = {};
-      add_rows<float, VEC>(a.sums + c, a.dim, sorted, sums, singles, acc);
-      add_rows<T, VEC>(grad + c, a.grad_stride, sorted, singles, end, acc);
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] *= a.scale;
-      store_f32<VEC>(out + c, acc);
-    }
-  }
-  if (listed && kGroups == 1) return;
-
-  // Rows of many entries; every row where the list was too long for LDS.
-  for (int r = 0; r < rows; ++r) {
-    const int sums = listed ? first[2 * r] : 0, singles = listed ? first[2 * r + 1] : 0;
-    const int end = listed ? first[2 * r + 2] : 0;
-    if (listed && end - sums <= kAlone) continue;
-    O *const out = static_cast<O *>(a.out) + (row0 + r) * a.out_stride;
-    for (int64_t c0 = 0; c0 < a.dim; c0 += L * VEC) {
-      const int64_t c = c0 + (tid % L) * VEC;
-      float acc[VEC] = {};
-      if (c < a.dim) {
-        if (listed) {
-          const int part = (end - sums + kGroups - 1) / kGroups;
-          const int from = min(sums + group * part, end), to = min(from + part, end);
-          add_rows<float, VEC>(a.sums + c, a.dim, sorted, from, min(to, singles), acc);
-          add_rows<T, VEC>(grad + c, a.grad_stride, sorted, max(from, singles), to, acc);
-        } else {
-          const int64_t part = ceil_div64(a.tiles, kGroups);
-          const int64_t last = min((group + 1) * part, a.tiles);
-          const uint32_t row = static_cast<uint32_t>(row0 + r);
-          for (int64_t tile = group * part; tile < last; ++tile) {
-            const uint32_t *const keys = a.keys + tile * kTile;
-            const uint32_t *const sources = a.sources + tile * kTile;
-            int lo = starts[tile * (a.spans + 1)];
-            const int stop = starts[tile * (a.spans + 1) + 1];
-            for (int hi = stop; lo < hi;) {
-              const int mid = (lo + hi) / 2;
-              if (keys[mid] < row)
-                lo = mid + 1;
-              else
-                hi = mid;
-            }
-            for (; lo < stop && keys[lo] == row; ++lo) {
-              if (sources[lo] & kSummed)
-                add_rows<float, VEC>(a.sums + c, a.dim, sources, lo, lo + 1, acc);
-              else
-                add_rows<T, VEC>(grad + c, a.grad_stride, sources, lo, lo + 1, acc);
-            }
-          }
+  // Puts the first n entries of the list to their places, in order: one wave,
+  // 64 at a time.
+  template <typename PUT> __device__ __forceinline__ void place(int n, PUT &&put) {
+    const int lane = threadIdx.x;
+    if (lane < kWave) {
+      const uint64_t below = (uint64_t(1) << lane) - 1;
+      for (int i0 = 0; i0 < n; i0 += kWave) {
+        const bool live = i0 + lane < n;
+        const uint32_t b = live ? local[i0 + lane] : 0;
+        const uint64_t peers = match_lanes(b, 9) & ballot(live);
+        const int to = next[b] + __popcll(peers & below);
+        wave_lds_order();
+        if (live) {
+          put(to, source[i0 + lane]);
+          if ((peers & below) == 0) next[b] = to + __popcll(peers);
         }
+        wave_lds_order();
       }
-      __syncthreads(); // the columns before have been read
-#pragma unroll
-      for (int k = 0; k < VEC; ++k) joined[group][(tid % L) * VEC + k] = acc[k];
+    }
+    __syncthreads();
+  }
+};
+
+// Step 3.
+__global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
+  __shared__ SpanList list;
+  const int tid = threadIdx.x;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.span;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(a.span), a.rows - row0));
+  const uint16_t *const starts = a.starts + blockIdx.x;
+
+  // f(tile, first entry in it, number, their place in the tiles' order) for
+  // every tile, one per thread; their total and the entries of lower rows.
+  int total = 0, before = 0;
+  auto each_tile = [&](auto &&f) {
+    total = before = 0;
+    for (int64_t t0 = 0; t0 < a.tiles; t0 += 256) {
+      const int64_t tile = t0 + tid;
+      int lo = 0, n = 0, sum;
+      if (tile < a.tiles) {
+        lo = starts[tile * (a.spans + 1)];
+        n = starts[tile * (a.spans + 1) + 1] - lo;
+      }
+      before += lo;
+      const int at = total + list.prefix(n, sum);
+      f(tile * kTile + lo, n, at);
+      total += sum;
+    }
+  };
+  auto entry_bin = [&](int64_t e) {
+    return SpanList::bin(static_cast<int>(a.keys[e] - row0), a.sources[e]);
+  };
+  // The entries at places [from, from + kListMost) to the list.
+  auto gather = [&](int from, bool count) {
+    each_tile([&](int64_t e, int n, int at) {
+      const int lo = max(from - at, 0), hi = min(n, from + kListMost - at);
+      for (int i = lo; i < hi; ++i) {
+        const int b = entry_bin(e + i);
+        list.source[at + i - from] = a.sources[e + i];
+        list.local[at + i - from] = static_cast<uint16_t>(b);
+        if (count) atomicAdd(&list.next[b], 1);
+      }
+    });
+  };
+  list.clear();
+  gather(0, true);
+  int base;
+  list.prefix(before, base);
+  if (blockIdx.x == gridDim.x - 1 && tid == 0) a.row_start[a.rows] = base + total;
+  if (total == 0) {
+    if (tid < rows) a.row_start[row0 + tid] = base;
+    return;
+  }
+  const int all = total;
+  if (all > kListMost) { // the rest is counted where it lies
+    each_tile([&](int64_t e, int n, int at) {
+      for (int i = max(kListMost - at, 0); i < n; ++i) atomicAdd(&list.next[entry_bin(e + i)], 1);
+    });
+  }
+  list.open();
+  if (tid < rows) a.row_start[row0 + tid] = base + list.first[2 * tid];
+  for (int from = 0; from < all; from += kListMost) {
+    if (from > 0) {
+      gather(from, false);
       __syncthreads();
-      if (group == 0 && c < a.dim) {
-        for (int g = 1; g < kGroups; ++g) {
+    }
+    list.place(min(all - from, kListMost), [&](int to, uint32_t what) { a.list[base + to] = what; });
+  }
+}
+
+// Adds vector c of entry `what` to acc.
+template <typename T, int VEC>
+__device__ __forceinline__ void add_entry(const GradArgs &a, uint32_t what, int64_t c,
+                                          float (&acc)[VEC]) {
+  float v[VEC];
+  if (what & kSummed)
+    load_f32<VEC>(a.sums + (what & ~kSummed) * a.dim + c, v);
+  else
+    load_f32<VEC>(static_cast<const T *>(a.grad) + what * a.grad_stride + c, v);
 #pragma unroll
-          for (int k = 0; k < VEC; ++k) acc[k] += joined[g][(tid % L) * VEC + k];
-        }
+  for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+}
+
+// A row of many entries, [first, end), by the whole workgroup: a contiguous
+// part of them per group of `wide` lanes (a power of two up to a wave), joined
+// across lanes and then through LDS.
+template <typename T, typename O, int VEC, typename ENTRY>
+__device__ __forceinline__ void sum_hub(const GradArgs &a, float (&joined)[kSpanWaves][kWave * VEC],
+                                        int wide, int64_t row, ENTRY &&entry, int first, int end) {
+  const int tid = threadIdx.x, part = tid / wide, column = tid % wide * VEC;
+  const int each = (end - first + 256 / wide - 1) / (256 / wide);
+  const int from = min(first + part * each, end), to = min(from + each, end);
+  for (int64_t c = column; c - column < a.dim; c += wide * VEC) {
+    float acc[VEC] = {};
+    if (c < a.dim) {
+      int i = from;
+      for (; i < to && (entry(i) & kSummed); ++i) add_entry<T, VEC>(a, entry(i), c, acc);
+      const T *const grad = static_cast<const T *>(a.grad) + c;
+#pragma unroll 8
+      for (; i < to; ++i) { // sums come first: these are tokens
+        float v[VEC];
+        load_f32<VEC>(grad + (entry(i) & ~kSummed) * a.grad_stride, v);
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] *= a.scale;
-        store_f32<VEC>(out + c, acc);
+        for (int k = 0; k < VEC; ++k) acc[k] += v[k];
       }
     }
+    for (int j = wide; j < kWave; j <<= 1) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[k] += __shfl_xor(acc[k], j);
+    }
+    __syncthreads(); // what was here before has been read
+    if (tid % kWave < wide) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) joined[tid / kWave][column + k] = acc[k];
+    }
+    __syncthreads();
+    if (tid < wide && c < a.dim) {
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) {
+        acc[k] = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kSpanWaves; ++w) acc[k] += joined[w][column + k];
+        acc[k] *= a.scale;
+      }
+      stream_f32<VEC>(static_cast<O *>(a.out) + row * a.out_stride + c, acc);
+    }
   }
+}
+
+// Rows [row0, row0 + rows), of which r's entries are [first(r), first(r + 1)).
+// The rows' vectors lie in a row before the workgroup's lanes, kItems of them
+// 256 apart per lane and turn, so that stores fill whole lines and a lane has
+// kItems loads under way; the entries after these are fetched meanwhile.
+template <typename T, typename O, int VEC, typename FIRST, typename ENTRY>
+__device__ __forceinline__ void sum_rows(const GradArgs &a, float (&joined)[kSpanWaves][kWave * VEC],
+                                         int64_t row0, int rows, FIRST &&first, ENTRY &&entry) {
+  constexpr int kItems = VEC == 8 ? 2 : 4;
+  const uint32_t vecs = static_cast<uint32_t>(a.dim / VEC);
+  const uint64_t all = static_cast<uint64_t>(rows) * vecs;
+  bool hubs = false;
+  for (uint64_t q0 = threadIdx.x; q0 < all; q0 += 256 * kItems) {
+    float acc[kItems][VEC] = {};
+    int r[kItems], at[kItems], left[kItems], longest = 0;
+    int64_t c[kItems];
+    uint32_t what[kItems];
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      const uint64_t q = q0 + 256 * u;
+      r[u] = q < all ? static_cast<int>(rows == 1 ? 0 : static_cast<uint32_t>(q) / vecs) : -1;
+      c[u] = static_cast<int64_t>(q - static_cast<uint64_t>(max(r[u], 0)) * vecs) * VEC;
+      at[u] = r[u] < 0 ? 0 : first(r[u]);
+      left[u] = r[u] < 0 ? 0 : first(r[u] + 1) - at[u];
+      if (left[u] > kAlone) hubs = true, left[u] = 0, r[u] = -1;
+      longest = max(longest, left[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) what[u] = left[u] > 0 ? entry(at[u]) : 0;
+    for (int i = 0; i < longest; ++i) {
+      float v[kItems][VEC] = {};
+      bool sums = false;
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) {
+        if (i < left[u] && !(what[u] & kSummed))
+          load_f32<VEC>(static_cast<const T *>(a.grad) + what[u] * a.grad_stride + c[u], v[u]);
+        sums = sums || (i < left[u] && (what[u] & kSummed));
+      }
+      if (sums) {
+#pragma unroll
+        for (int u = 0; u < kItems; ++u)
+          if (i < left[u] && (what[u] & kSummed))
+            load_f32<VEC>(a.sums + (what[u] & ~kSummed) * a.dim + c[u], v[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) what[u] = i + 1 < left[u] ? entry(at[u] + i + 1) : 0;
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[u][k] += v[u][k];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < kItems; ++u) {
+      if (r[u] < 0) continue;
+#pragma unroll
+      for (int k = 0; k < VEC; ++k) acc[u][k] *= a.scale;
+      stream_f32<VEC>(static_cast<O *>(a.out) + (row0 + r[u]) * a.out_stride + c[u], acc[u]);
+    }
+  }
+  if (!__syncthreads_or(hubs)) return;
+  const int wide = vecs <= 8 ? 8 : vecs <= 32 ? 32 : 64;
+  for (int n = 0; n < rows; ++n) {
+    const int from = first(n), to = first(n + 1);
+    if (to - from > kAlone) sum_hub<T, O, VEC>(a, joined, wide, row0 + n, entry, from, to);
+  }
+}
+
+// Step 4: a.row_block rows per workgroup.
+template <typename T, typename O, int VEC>
+__global__ void __launch_bounds__(256) embedding_row_kernel(GradArgs a) {
+  __shared__ float joined[kSpanWaves][kWave * VEC];
+  __shared__ int start[kRowsMost + 1];
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.row_block; row0 < a.rows;
+       row0 += static_cast<int64_t>(gridDim.x) * a.row_block) {
+    const int rows = static_cast<int>(min(static_cast<int64_t>(a.row_block), a.rows - row0));
+    for (int i = threadIdx.x; i <= rows; i += 256) start[i] = a.row_start[row0 + i];
+    __syncthreads();
+    sum_rows<T, O, VEC>(
+        a, joined, row0, rows, [&](int r) { return start[r]; }, [&](int i) { return a.list[i]; });
+    __syncthreads(); // `start` has been read
+  }
+}
+
+// At most kListMost tokens: a span per workgroup, from tokens to rows.
+template <typename T, typename O, int VEC>
+__global__ void __launch_bounds__(256) embedding_few_kernel(GradArgs a) {
+  __shared__ SpanList list;
+  __shared__ uint16_t sorted[kListMost]; // token indices by row
+  __shared__ float joined[kSpanWaves][kWave * VEC];
+  const int tid = threadIdx.x;
+  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.span;
+  const int rows = static_cast<int>(min(static_cast<int64_t>(a.span), a.rows - row0));
+  list.clear();
+
+  constexpr int kEach = kListMost / 256;
+  uint32_t row[kEach];
+  token_rows(a, static_cast<int64_t>(tid) * kEach, 1, row);
+  int n = 0, total;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) n += row[k] >= row0 && row[k] < row0 + rows;
+  int at = list.prefix(n, total);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    if (row[k] < row0 || row[k] >= row0 + rows) continue;
+    const uint32_t token = static_cast<uint32_t>(tid * kEach + k);
+    const int b = SpanList::bin(static_cast<int>(row[k] - row0), token);
+    list.source[at] = token;
+    list.local[at++] = static_cast<uint16_t>(b);
+    atomicAdd(&list.next[b], 1);
+  }
+  if (total > 0) {
+    list.open();
+    list.place(total, [&](int to, uint32_t what) { sorted[to] = static_cast<uint16_t>(what); });
+  }
+  sum_rows<T, O, VEC>(
+      a, joined, row0, rows, [&](int r) { return total > 0 ? list.first[2 * r] : 0; },
+      [&](int i) { return static_cast<uint32_t>(sorted[i]); });
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -515,7 +673,7 @@ template <typename T> int32_t lookup_typed(const LookupArgs &a, void *stream) {
 struct GradLayout {
   int span;
   int64_t spans, tiles;
-  size_t keys, sources, order, runs, starts, sums, bytes;
+  size_t keys, sources, order, runs, run_count, starts, sums, list, row_start, bytes;
 };
 
 // Table rows per span: enough spans to fill the card several times over, and
@@ -537,32 +695,38 @@ GradLayout grad_layout(int64_t count, int64_t rows, int64_t dim) {
   l.keys = take(tiles * kTile, sizeof(uint32_t));
   l.sources = take(tiles * kTile, sizeof(uint32_t));
   l.order = take(tiles * kTile, sizeof(uint16_t));
-  l.runs = take(tiles * kTileRuns, sizeof(uint16_t));
+  l.runs = take(tiles * kTileRuns, sizeof(uint32_t));
+  l.run_count = take(tiles, sizeof(int32_t));
   l.starts = take(tiles * (l.spans + 1), sizeof(uint16_t));
   l.sums = take(tiles * kTileRuns * dim, sizeof(float));
+  l.list = take(count, sizeof(uint32_t));
+  l.row_start = take(rows + 1, sizeof(int32_t));
   l.bytes = at;
   return l;
 }
 
-template <typename T, typename O, int VEC, int L>
-int32_t run_grad(const GradArgs &a, void *stream) {
-  if (a.tiles > 0) {
-    int32_t rc = launch(embedding_tile_kernel, dim3(a.tiles), dim3(kTileBlock), stream, a);
-    if (rc != SPORDER_OK) return rc;
-    rc = launch(embedding_run_kernel<T, VEC, L>, dim3(ceil_div64(a.tiles * kTileRuns, 256 / L)),
-                dim3(256), stream, a);
-    if (rc != SPORDER_OK) return rc;
-  }
-  return launch(embedding_span_kernel<T, O, VEC, L>, dim3(a.spans), dim3(256), stream, a);
+template <typename T, int VEC> int32_t run_runs(const GradArgs &a, void *stream) {
+  const int64_t vecs = ceil_div64(a.dim, VEC);
+  auto go = [&](auto kernel, int lanes) {
+    return launch(kernel, dim3(a.tiles * kRunBlocks, ceil_div64(vecs, lanes)), dim3(256), stream, a);
+  };
+  if (vecs <= 8) return go(embedding_run_kernel<T, VEC, 8>, 8);
+  if (vecs <= 32) return go(embedding_run_kernel<T, VEC, 32>, 32);
+  return go(embedding_run_kernel<T, VEC, 64>, 64);
 }
 
-template <typename T, typename O, int VEC>
-int32_t grad_vec(const GradArgs &a, void *stream) {
-  const int64_t vecs = ceil_div64(a.dim, VEC);
-  if (vecs <= 8) return run_grad<T, O, VEC, 8>(a, stream);
-  if (vecs <= 32) return run_grad<T, O, VEC, 32>(a, stream);
-  if (vecs <= 256) return run_grad<T, O, VEC, 64>(a, stream);
-  return run_grad<T, O, VEC, 256>(a, stream);
+template <typename T, typename O, int VEC> int32_t grad_vec(GradArgs a, void *stream) {
+  if (a.tiles == 0)
+    return launch(embedding_few_kernel<T, O, VEC>, dim3(a.spans), dim3(256), stream, a);
+  int32_t rc = launch(embedding_tile_kernel, dim3(a.tiles), dim3(kTileBlock), stream, a);
+  if (rc == SPORDER_OK) rc = run_runs<T, VEC>(a, stream);
+  if (rc == SPORDER_OK) rc = launch(embedding_span_kernel, dim3(a.spans), dim3(256), stream, a);
+  if (rc != SPORDER_OK) return rc;
+  // About one turn of sum_rows per workgroup.
+  const int64_t vecs = a.dim / VEC, turn = 256 * (VEC == 8 ? 2 : 4);
+  a.row_block = static_cast<int>(std::clamp<int64_t>(turn / vecs, 1, kRowsMost));
+  return launch(embedding_row_kernel<T, O, VEC>,
+                dim3(std::min(ceil_div64(a.rows, a.row_block), kMostBlocks)), dim3(256), stream, a);
 }
 
 template <typename T, typename O> int32_t grad_typed(const GradArgs &a, void *stream) {
@@ -635,15 +799,19 @@ int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count, int64_
                    scale,
                    token_bits == 64,
                    bits_for(rows),
+                   0,
                    l.span,
                    l.spans,
                    l.tiles,
                    reinterpret_cast<uint32_t *>(w + l.keys),
                    reinterpret_cast<uint32_t *>(w + l.sources),
                    reinterpret_cast<uint16_t *>(w + l.order),
-                   reinterpret_cast<uint16_t *>(w + l.runs),
+                   reinterpret_cast<uint32_t *>(w + l.runs),
+                   reinterpret_cast<int32_t *>(w + l.run_count),
                    reinterpret_cast<uint16_t *>(w + l.starts),
-                   reinterpret_cast<float *>(w + l.sums)};
+                   reinterpret_cast<float *>(w + l.sums),
+                   reinterpret_cast<uint32_t *>(w + l.list),
+                   reinterpret_cast<int32_t *>(w + l.row_start)};
   if (type == SPORDER_TYPE_F32) return grad_typed<float, float>(a, stream);
   if (type == SPORDER_TYPE_BF16)
     return out_type == type ? grad_typed<bf16_t, bf16_t>(a, stream)

@@ -17,8 +17,9 @@
 //   3. a workgroup per span gathers its entries from every tile, in the
 //      tiles' order, sorts them by row in LDS and writes them out by row;
 //   4. the table is written front to back, every lane a few vectors of a row
-//      and their sum (this is where the bytes are); a row that still has many
-//      entries is shared by a workgroup.
+//      and their sum (this is where the bytes are); rows that still have many
+//      entries are shared by a workgroup for each slice of their columns, in
+//      the launch's first workgroups.
 //
 // Few tokens need no tiles: each span picks its own from all of them and sums
 // its rows, in one launch.
@@ -82,7 +83,10 @@ constexpr int kTileRuns = kTileChunks * kChunkRuns;
 constexpr uint32_t kSummed = 0x80000000u; // an entry that is a run's sum
 constexpr int kSpanMost = 256;    // table rows per span
 constexpr int kListMost = 2048;   // a span's entries that fit the list in LDS
+constexpr int kSparse = 4;        // turns' worth of rows per workgroup, at most
 constexpr int kAlone = 8;         // entries of a row that one lane adds up
+constexpr int kHubLists = 16;
+constexpr int kHubBlocks = 512;   // workgroups of the last launch for rows of more entries
 constexpr int kRowsMost = 1024;   // table rows per workgroup of the last launch
 
 struct GradArgs {
@@ -105,6 +109,11 @@ struct GradArgs {
   float *sums;         // [tiles * kTileRuns][dim]
   uint32_t *list;      // [count] the entries' sources by row, sums first
   int32_t *row_start;  // [rows + 1] first entry in the list
+  // Rows of more than kAlone entries: kHubLists lists, each its length and
+  // then the rows (one counter for all would have every span's atomic wait for
+  // the others': 37 us of 67 with 4,250 such rows).
+  int32_t *hubs;       // [kHubLists][hub_stride]
+  int64_t hub_stride;
 };
 
 // The table rows of tokens first, first + step, ... before a.count; `rows`
@@ -236,6 +245,7 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
   const int place = wave_incl_scan(mine) - mine;
   const int all = wave_sum(mine), entries = all & 0xffff;
   if (tid == 0) a.run_count[tile] = all >> 16;
+  if (tile == 0 && tid < kHubLists) a.hubs[tid * a.hub_stride] = 0;
   const int to = from ^ 1;
 #pragma unroll
   for (int r = 0; r < kTileRounds; ++r) {
@@ -457,7 +467,13 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
     });
   }
   list.open();
-  if (tid < rows) a.row_start[row0 + tid] = base + list.first[2 * tid];
+  if (tid < rows) {
+    const int at = list.first[2 * tid], n = list.first[2 * tid + 2] - at;
+    a.row_start[row0 + tid] = base + at;
+    // Their order changes from run to run; each row's sum does not depend on it.
+    int32_t *const hubs = a.hubs + blockIdx.x % kHubLists * a.hub_stride;
+    if (n > kAlone) hubs[1 + atomicAdd(hubs, 1)] = static_cast<int32_t>(row0 + tid);
+  }
   for (int from = 0; from < all; from += kListMost) {
     if (from > 0) {
       gather(from, false);
@@ -467,40 +483,46 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
   }
 }
 
-// Adds vector c of entry `what` to acc.
-template <typename T, int VEC>
-__device__ __forceinline__ void add_entry(const GradArgs &a, uint32_t what, int64_t c,
-                                          float (&acc)[VEC]) {
-  float v[VEC];
-  if (what & kSummed)
-    load_f32<VEC>(a.sums + (what & ~kSummed) * a.dim + c, v);
-  else
-    load_f32<VEC>(static_cast<const T *>(a.grad) + what * a.grad_stride + c, v);
-#pragma unroll
-  for (int k = 0; k < VEC; ++k) acc[k] += v[k];
-}
-
-// A row of many entries, [first, end), by the whole workgroup: a contiguous
-// part of them per group of `wide` lanes (a power of two up to a wave), joined
-// across lanes and then through LDS.
+// Columns [begin, stop) of a row of many entries, [first, end), by the whole
+// workgroup: a contiguous part of the entries per group of `wide` lanes (a
+// power of two up to a wave), joined across lanes and then through LDS.
 template <typename T, typename O, int VEC, typename ENTRY>
 __device__ __forceinline__ void sum_hub(const GradArgs &a, float (&joined)[kSpanWaves][kWave * VEC],
-                                        int wide, int64_t row, ENTRY &&entry, int first, int end) {
+                                        int wide, int64_t row, ENTRY &&entry, int first, int end,
+                                        int64_t begin, int64_t stop) {
   const int tid = threadIdx.x, part = tid / wide, column = tid % wide * VEC;
   const int each = (end - first + 256 / wide - 1) / (256 / wide);
   const int from = min(first + part * each, end), to = min(from + each, end);
-  for (int64_t c = column; c - column < a.dim; c += wide * VEC) {
+  for (int64_t c = begin + column; c - column < stop; c += wide * VEC) {
     float acc[VEC] = {};
-    if (c < a.dim) {
-      int i = from;
-      for (; i < to && (entry(i) & kSummed); ++i) add_entry<T, VEC>(a, entry(i), c, acc);
+    if (c < stop) {
       const T *const grad = static_cast<const T *>(a.grad) + c;
-#pragma unroll 8
-      for (; i < to; ++i) { // sums come first: these are tokens
-        float v[VEC];
-        load_f32<VEC>(grad + (entry(i) & ~kSummed) * a.grad_stride, v);
+      const float *const sums = a.sums + c;
+      for (int i = from; i < to; i += 8) {
+        uint32_t what[8];
+        float v[8][VEC] = {};
+        int summed = 0; // sums come first: mostly all or none of the eight
 #pragma unroll
-        for (int k = 0; k < VEC; ++k) acc[k] += v[k];
+        for (int d = 0; d < 8; ++d) what[d] = entry(min(i + d, to - 1));
+#pragma unroll
+        for (int d = 0; d < 8; ++d) summed += what[d] >> 31;
+        if (summed < 8) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+            if (i + d < to && !(what[d] & kSummed))
+              load_f32<VEC>(grad + what[d] * a.grad_stride, v[d]);
+        }
+        if (summed > 0) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+            if (i + d < to && (what[d] & kSummed))
+              load_f32<VEC>(sums + (what[d] & ~kSummed) * a.dim, v[d]);
+        }
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+#pragma unroll
+          for (int k = 0; k < VEC; ++k) acc[k] += v[d][k];
+        }
       }
     }
     for (int j = wide; j < kWave; j <<= 1) {
@@ -513,7 +535,7 @@ __device__ __forceinline__ void sum_hub(const GradArgs &a, float (&joined)[kSpan
       for (int k = 0; k < VEC; ++k) joined[tid / kWave][column + k] = acc[k];
     }
     __syncthreads();
-    if (tid < wide && c < a.dim) {
+    if (tid < wide && c < stop) {
 #pragma unroll
       for (int k = 0; k < VEC; ++k) {
         acc[k] = 0.0f;
@@ -526,30 +548,60 @@ __device__ __forceinline__ void sum_hub(const GradArgs &a, float (&joined)[kSpan
   }
 }
 
+// Rows of a workgroup with entries that its lanes add up alone.
+struct BusyRows {
+  uint16_t row[kRowsMost];
+  int count;
+};
+
 // Rows [row0, row0 + rows), of which r's entries are [first(r), first(r + 1)).
-// The rows' vectors lie in a row before the workgroup's lanes, kItems of them
-// 256 apart per lane and turn, so that stores fill whole lines and a lane has
-// kItems loads under way; the entries after these are fetched meanwhile.
+// Empty rows are written first, front to back.  The vectors of the rows with
+// few entries then lie in a row before the workgroup's lanes, kItems of them 256
+// apart per lane and turn, so that stores fill whole lines and every lane has
+// kItems loads under way (with the empty rows among them, most lanes would
+// have none); the entries after these are fetched meanwhile.
 template <typename T, typename O, int VEC, typename FIRST, typename ENTRY>
-__device__ __forceinline__ void sum_rows(const GradArgs &a, float (&joined)[kSpanWaves][kWave * VEC],
-                                         int64_t row0, int rows, FIRST &&first, ENTRY &&entry) {
-  constexpr int kItems = VEC == 8 ? 2 : 4;
+__device__ __forceinline__ void sum_rows(const GradArgs &a, BusyRows &busy, int64_t row0, int rows,
+                                         FIRST &&first, ENTRY &&entry) {
+  constexpr int kItems = 2;
   const uint32_t vecs = static_cast<uint32_t>(a.dim / VEC);
-  const uint64_t all = static_cast<uint64_t>(rows) * vecs;
-  bool hubs = false;
-  for (uint64_t q0 = threadIdx.x; q0 < all; q0 += 256 * kItems) {
+  O *const out = static_cast<O *>(a.out) + row0 * a.out_stride;
+  if (threadIdx.x == 0) busy.count = 0;
+  __syncthreads();
+  for (int r = threadIdx.x; r < rows; r += 256) {
+    const int n = first(r + 1) - first(r);
+    if (n > 0 && n <= kAlone) busy.row[atomicAdd(&busy.count, 1)] = static_cast<uint16_t>(r);
+  }
+  __syncthreads();
+  const int count = busy.count;
+  if (count < rows) {
+    float zero[VEC] = {};
+    if (vecs >= 256) { // a row per turn or more
+      for (int r = 0; r < rows; ++r) {
+        if (first(r + 1) != first(r)) continue;
+        for (uint32_t c = threadIdx.x; c < vecs; c += 256)
+          stream_f32<VEC>(out + r * a.out_stride + static_cast<int64_t>(c) * VEC, zero);
+      }
+    } else {
+      for (uint32_t q = threadIdx.x; q < rows * vecs; q += 256) {
+        const int r = q / vecs;
+        if (first(r + 1) == first(r))
+          stream_f32<VEC>(out + r * a.out_stride + static_cast<int64_t>(q - r * vecs) * VEC, zero);
+      }
+    }
+  }
+  const uint32_t all = count * vecs; // at most 2^31: kMostDim, kSpanMost
+  for (uint32_t q0 = threadIdx.x; q0 < all; q0 += 256 * kItems) {
     float acc[kItems][VEC] = {};
-    int r[kItems], at[kItems], left[kItems], longest = 0;
-    int64_t c[kItems];
-    uint32_t what[kItems];
+    int left[kItems], longest = 0;
+    uint32_t r[kItems], c[kItems], at[kItems], what[kItems];
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
-      const uint64_t q = q0 + 256 * u;
-      r[u] = q < all ? static_cast<int>(rows == 1 ? 0 : static_cast<uint32_t>(q) / vecs) : -1;
-      c[u] = static_cast<int64_t>(q - static_cast<uint64_t>(max(r[u], 0)) * vecs) * VEC;
-      at[u] = r[u] < 0 ? 0 : first(r[u]);
-      left[u] = r[u] < 0 ? 0 : first(r[u] + 1) - at[u];
-      if (left[u] > kAlone) hubs = true, left[u] = 0, r[u] = -1;
+      const uint32_t q = q0 + 256 * u, n = min(q, all - 1) / vecs;
+      c[u] = (q - n * vecs) * VEC;
+      r[u] = busy.row[n];
+      at[u] = first(r[u]);
+      left[u] = q < all ? first(r[u] + 1) - at[u] : 0;
       longest = max(longest, left[u]);
     }
 #pragma unroll
@@ -579,33 +631,44 @@ __device__ __forceinline__ void sum_rows(const GradArgs &a, float (&joined)[kSpa
     }
 #pragma unroll
     for (int u = 0; u < kItems; ++u) {
-      if (r[u] < 0) continue;
+      if (left[u] == 0) continue;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[u][k] *= a.scale;
-      stream_f32<VEC>(static_cast<O *>(a.out) + (row0 + r[u]) * a.out_stride + c[u], acc[u]);
+      stream_f32<VEC>(out + r[u] * a.out_stride + c[u], acc[u]);
     }
-  }
-  if (!__syncthreads_or(hubs)) return;
-  const int wide = vecs <= 8 ? 8 : vecs <= 32 ? 32 : 64;
-  for (int n = 0; n < rows; ++n) {
-    const int from = first(n), to = first(n + 1);
-    if (to - from > kAlone) sum_hub<T, O, VEC>(a, joined, wide, row0 + n, entry, from, to);
   }
 }
 
-// Step 4: a.row_block rows per workgroup.
+__device__ __forceinline__ int hub_lanes(uint32_t vecs) { return vecs <= 8 ? 8 : vecs <= 32 ? 32 : 64; }
+
+// Step 4: a.row_block rows per workgroup, after kHubBlocks workgroups for the
+// hubs, which take longest and so begin first.
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(256) embedding_row_kernel(GradArgs a) {
   __shared__ float joined[kSpanWaves][kWave * VEC];
   __shared__ int start[kRowsMost + 1];
-  for (int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.row_block; row0 < a.rows;
-       row0 += static_cast<int64_t>(gridDim.x) * a.row_block) {
+  __shared__ BusyRows busy;
+  auto entry = [&](uint32_t i) { return a.list[i]; };
+  if (blockIdx.x < kHubBlocks) {
+    const uint32_t vecs = static_cast<uint32_t>(a.dim / VEC);
+    const int wide = hub_lanes(vecs), slices = (vecs + wide - 1) / wide;
+    const int32_t *const hubs = a.hubs + blockIdx.x % kHubLists * a.hub_stride;
+    const int64_t all = static_cast<int64_t>(*hubs) * slices;
+    for (int64_t i = blockIdx.x / kHubLists; i < all; i += kHubBlocks / kHubLists) {
+      const int64_t row = hubs[1 + i / slices], begin = i % slices * wide * VEC;
+      sum_hub<T, O, VEC>(a, joined, wide, row, entry, a.row_start[row], a.row_start[row + 1], begin,
+                         min(begin + wide * VEC, a.dim));
+    }
+    return;
+  }
+  for (int64_t row0 = static_cast<int64_t>(blockIdx.x - kHubBlocks) * a.row_block; row0 < a.rows;
+       row0 += static_cast<int64_t>(gridDim.x - kHubBlocks) * a.row_block) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(a.row_block), a.rows - row0));
     for (int i = threadIdx.x; i <= rows; i += 256) start[i] = a.row_start[row0 + i];
     __syncthreads();
     sum_rows<T, O, VEC>(
-        a, joined, row0, rows, [&](int r) { return start[r]; }, [&](int i) { return a.list[i]; });
-    __syncthreads(); // `start` has been read
+        a, busy, row0, rows, [&](int r) { return start[r]; }, entry);
+    __syncthreads(); // `start` and `busy` have been read
   }
 }
 
@@ -614,6 +677,7 @@ template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(256) embedding_few_kernel(GradArgs a) {
   __shared__ SpanList list;
   __shared__ uint16_t sorted[kListMost]; // token indices by row
+  __shared__ BusyRows busy;
   __shared__ float joined[kSpanWaves][kWave * VEC];
   const int tid = threadIdx.x;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.span;
@@ -640,9 +704,16 @@ __global__ void __launch_bounds__(256) embedding_few_kernel(GradArgs a) {
     list.open();
     list.place(total, [&](int to, uint32_t what) { sorted[to] = static_cast<uint16_t>(what); });
   }
-  sum_rows<T, O, VEC>(
-      a, joined, row0, rows, [&](int r) { return total > 0 ? list.first[2 * r] : 0; },
-      [&](int i) { return static_cast<uint32_t>(sorted[i]); });
+  auto first = [&](int r) { return total > 0 ? list.first[2 * r] : 0; };
+  auto entry = [&](int i) { return static_cast<uint32_t>(sorted[i]); };
+  sum_rows<T, O, VEC>(a, busy, row0, rows, first, entry);
+  if (total <= kAlone) return;
+  const int wide = hub_lanes(static_cast<uint32_t>(a.dim / VEC));
+  for (int r = 0; r < rows; ++r) {
+    const int from = first(r), to = first(r + 1);
+    if (to - from > kAlone)
+      sum_hub<T, O, VEC>(a, joined, wide, row0 + r, entry, from, to, 0, a.dim);
+  }
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -673,7 +744,8 @@ template <typename T> int32_t lookup_typed(const LookupArgs &a, void *stream) {
 struct GradLayout {
   int span;
   int64_t spans, tiles;
-  size_t keys, sources, order, runs, run_count, starts, sums, list, row_start, bytes;
+  size_t keys, sources, order, runs, run_count, starts, sums, list, row_start, hubs, bytes;
+  int64_t hub_stride;
 };
 
 // Table rows per span: enough spans to fill the card several times over, and
@@ -701,6 +773,8 @@ GradLayout grad_layout(int64_t count, int64_t rows, int64_t dim) {
   l.sums = take(tiles * kTileRuns * dim, sizeof(float));
   l.list = take(count, sizeof(uint32_t));
   l.row_start = take(rows + 1, sizeof(int32_t));
+  l.hub_stride = ceil_div64(1 + count / (kAlone + 1), 64) * 64; // lines of their own
+  l.hubs = take(kHubLists * l.hub_stride, sizeof(int32_t));
   l.bytes = at;
   return l;
 }
@@ -722,11 +796,14 @@ template <typename T, typename O, int VEC> int32_t grad_vec(GradArgs a, void *st
   if (rc == SPORDER_OK) rc = run_runs<T, VEC>(a, stream);
   if (rc == SPORDER_OK) rc = launch(embedding_span_kernel, dim3(a.spans), dim3(256), stream, a);
   if (rc != SPORDER_OK) return rc;
-  // About one turn of sum_rows per workgroup.
-  const int64_t vecs = a.dim / VEC, turn = 256 * (VEC == 8 ? 2 : 4);
-  a.row_block = static_cast<int>(std::clamp<int64_t>(turn / vecs, 1, kRowsMost));
+  // About one turn of sum_rows per workgroup, with one row in rows / count
+  // taken to have entries.
+  const int64_t vecs = a.dim / VEC, turn = 512;
+  const int64_t sparse = std::clamp<int64_t>(a.rows / a.count, 1, kSparse);
+  a.row_block = static_cast<int>(std::clamp<int64_t>(turn * sparse / vecs, 1, kRowsMost));
   return launch(embedding_row_kernel<T, O, VEC>,
-                dim3(std::min(ceil_div64(a.rows, a.row_block), kMostBlocks)), dim3(256), stream, a);
+                dim3(kHubBlocks + std::min(ceil_div64(a.rows, a.row_block), kMostBlocks)), dim3(256),
+                stream, a);
 }
 
 template <typename T, typename O> int32_t grad_typed(const GradArgs &a, void *stream) {
@@ -811,7 +888,9 @@ int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count, int64_
                    reinterpret_cast<uint16_t *>(w + l.starts),
                    reinterpret_cast<float *>(w + l.sums),
                    reinterpret_cast<uint32_t *>(w + l.list),
-                   reinterpret_cast<int32_t *>(w + l.row_start)};
+                   reinterpret_cast<int32_t *>(w + l.row_start),
+                   reinterpret_cast<int32_t *>(w + l.hubs),
+                   l.hub_stride};
   if (type == SPORDER_TYPE_F32) return grad_typed<float, float>(a, stream);
   if (type == SPORDER_TYPE_BF16)
     return out_type == type ? grad_typed<bf16_t, bf16_t>(a, stream)

@@ -38,8 +38,8 @@ __device__ __forceinline__ void store_f32(T *p, const float (&in)[VEC]) {
   *reinterpret_cast<Pack<T, VEC> *>(p) = q;
 }
 
-// The same past the caches, for output that is not read again soon: it leaves
-// them to what the kernel still reads.
+// The same past the caches, for output too large to be found there by its
+// reader: it leaves them to what the kernel still reads.
 template <int VEC, typename T>
 __device__ __forceinline__ void stream_f32(T *p, const float (&in)[VEC]) {
   using words = uint32_t __attribute__((ext_vector_type(4)));
@@ -57,6 +57,18 @@ __device__ __forceinline__ void stream_f32(T *p, const float (&in)[VEC]) {
     static_assert(VEC == 1);
     __builtin_nontemporal_store(q.v[0], p);
   }
+}
+
+// Output from which on stores go past the caches (the last level holds 256 MB,
+// and what was read is in it too).
+constexpr int64_t kStreamBytes = int64_t(64) << 20;
+
+template <int VEC, typename T>
+__device__ __forceinline__ void put_f32(bool stream, T *p, const float (&in)[VEC]) {
+  if (stream)
+    stream_f32<VEC>(p, in);
+  else
+    store_f32<VEC>(p, in);
 }
 
 // Calls f with a pointer of the type known at run time.  The branch goes

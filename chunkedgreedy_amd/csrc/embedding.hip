@@ -45,26 +45,54 @@ struct LookupArgs {
   int64_t count, rows, dim, table_stride, out_stride;
   float scale;
   int wide;
+  bool stream;
+  int64_t row_block; // tokens per workgroup and turn
 };
 
-// L lanes per token.  A token outside the table gives a row of NaN (row 0 is
-// read in its place), so that a wrong id cannot pass for a vector.
-template <typename T, int VEC, int L>
-__global__ void __launch_bounds__(256) embedding_kernel(LookupArgs a) {
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * (256 / L) + threadIdx.x / L; t < a.count;
-       t += static_cast<int64_t>(gridDim.x) * (256 / L)) {
-    const int64_t id = token_at(a.tokens, a.wide, t);
-    const bool known = id >= 0 && id < a.rows;
-    const T *const from = static_cast<const T *>(a.table) + (known ? id : 0) * a.table_stride;
-    T *const to = static_cast<T *>(a.out) + t * a.out_stride;
-    const float scale = known ? a.scale : __builtin_nanf("");
-#pragma unroll 4
-    for (int64_t c = (threadIdx.x % L) * VEC; c < a.dim; c += L * VEC) {
-      float v[VEC];
-      load_f32<VEC>(from + c, v);
+// The vectors of a.row_block rows lie in a row before the workgroup's lanes,
+// kItems of them 256 apart per lane and turn: stores fill whole lines whatever
+// the row's length, and a lane has kItems rows under way.  A token outside the
+// table gives a row of NaN (row 0 is read in its place), so that a wrong id
+// cannot pass for a vector.
+constexpr int lookup_items(int vec) { return vec == 1 ? 8 : 4; }
+
+template <typename T, int VEC> __global__ void __launch_bounds__(256) embedding_kernel(LookupArgs a) {
+  constexpr int kItems = lookup_items(VEC);
+  const uint32_t vecs = static_cast<uint32_t>(a.dim / VEC);
+  const T *const table = static_cast<const T *>(a.table);
+  for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * a.row_block; t0 < a.count;
+       t0 += static_cast<int64_t>(gridDim.x) * a.row_block) {
+    const uint32_t rows = static_cast<uint32_t>(min(static_cast<int64_t>(a.row_block), a.count - t0));
+    const uint32_t all = rows * vecs; // at most kMostDim, or a few thousand
+    T *const out = static_cast<T *>(a.out) + t0 * a.out_stride;
+    for (uint32_t q0 = threadIdx.x; q0 < all; q0 += 256 * kItems) {
+      uint32_t t[kItems], c[kItems];
+      int64_t id[kItems];
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) v[i] *= scale;
-      store_f32<VEC>(to + c, v);
+      for (int u = 0; u < kItems; ++u) {
+        const uint32_t q = min(q0 + 256 * u, all - 1);
+        t[u] = q / vecs;
+        c[u] = (q - t[u] * vecs) * VEC;
+      }
+      auto fetch = [&](auto *tokens) {
+#pragma unroll
+        for (int u = 0; u < kItems; ++u) id[u] = tokens[t0 + t[u]];
+      };
+      if (a.wide)
+        fetch(static_cast<const int64_t *>(a.tokens));
+      else
+        fetch(static_cast<const int32_t *>(a.tokens));
+      float v[kItems][VEC];
+#pragma unroll
+      for (int u = 0; u < kItems; ++u)
+        load_f32<VEC>(table + (id[u] >= 0 && id[u] < a.rows ? id[u] : 0) * a.table_stride + c[u], v[u]);
+#pragma unroll
+      for (int u = 0; u < kItems; ++u) {
+        const float scale = id[u] >= 0 && id[u] < a.rows ? a.scale : __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[u][i] *= scale;
+        if (q0 + 256 * u < all) put_f32<VEC>(a.stream, out + t[u] * a.out_stride + c[u], v[u]);
+      }
     }
   }
 }
@@ -95,6 +123,7 @@ struct GradArgs {
   int64_t count, rows, dim, grad_stride, out_stride, padding;
   float scale;
   int wide;
+  bool stream;
   int key_bits;
   int row_block; // table rows per workgroup of the last launch
   int span;      // and of the one before it
@@ -543,7 +572,7 @@ __device__ __forceinline__ void sum_hub(const GradArgs &a, float (&joined)[kSpan
         for (int w = 0; w < kSpanWaves; ++w) acc[k] += joined[w][column + k];
         acc[k] *= a.scale;
       }
-      stream_f32<VEC>(static_cast<O *>(a.out) + row * a.out_stride + c, acc);
+      put_f32<VEC>(a.stream, static_cast<O *>(a.out) + row * a.out_stride + c, acc);
     }
   }
 }
@@ -580,13 +609,13 @@ __device__ __forceinline__ void sum_rows(const GradArgs &a, BusyRows &busy, int6
       for (int r = 0; r < rows; ++r) {
         if (first(r + 1) != first(r)) continue;
         for (uint32_t c = threadIdx.x; c < vecs; c += 256)
-          stream_f32<VEC>(out + r * a.out_stride + static_cast<int64_t>(c) * VEC, zero);
+          put_f32<VEC>(a.stream, out + r * a.out_stride + static_cast<int64_t>(c) * VEC, zero);
       }
     } else {
       for (uint32_t q = threadIdx.x; q < rows * vecs; q += 256) {
         const int r = q / vecs;
         if (first(r + 1) == first(r))
-          stream_f32<VEC>(out + r * a.out_stride + static_cast<int64_t>(q - r * vecs) * VEC, zero);
+          put_f32<VEC>(a.stream, out + r * a.out_stride + static_cast<int64_t>(q - r * vecs) * VEC, zero);
       }
     }
   }
@@ -634,7 +663,7 @@ __device__ __forceinline__ void sum_rows(const GradArgs &a, BusyRows &busy, int6
       if (left[u] == 0) continue;
 #pragma unroll
       for (int k = 0; k < VEC; ++k) acc[u][k] *= a.scale;
-      stream_f32<VEC>(out + r[u] * a.out_stride + c[u], acc[u]);
+      put_f32<VEC>(a.stream, out + r[u] * a.out_stride + c[u], acc[u]);
     }
   }
 }
@@ -718,27 +747,20 @@ __global__ void __launch_bounds__(256) embedding_few_kernel(GradArgs a) {
 
 // ---- host ----------------------------------------------------------------------
 
-template <typename T, int VEC, int L> int32_t run_lookup(const LookupArgs &a, void *stream) {
-  return launch(embedding_kernel<T, VEC, L>, dim3(std::min(ceil_div64(a.count, 256 / L), kMostBlocks)),
-                dim3(256), stream, a);
-}
-
-// Lanes per row: a row of a few vectors leaves the rest of the wave to others.
-template <typename T, int VEC> int32_t pick_lookup(const LookupArgs &a, void *stream) {
-  const int64_t vecs = ceil_div64(a.dim, VEC);
-  if (vecs <= 8) return run_lookup<T, VEC, 8>(a, stream);
-  if (vecs <= 32) return run_lookup<T, VEC, 32>(a, stream);
-  if (vecs <= 256) return run_lookup<T, VEC, 64>(a, stream);
-  return run_lookup<T, VEC, 256>(a, stream);
+// Rows per workgroup: about one turn.
+template <typename T, int VEC> int32_t run_lookup(LookupArgs a, void *stream) {
+  a.row_block = std::max<int64_t>(1, 256 * lookup_items(VEC) * VEC / a.dim);
+  return launch(embedding_kernel<T, VEC>,
+                dim3(std::min(ceil_div64(a.count, a.row_block), kMostBlocks)), dim3(256), stream, a);
 }
 
 template <typename T> int32_t lookup_typed(const LookupArgs &a, void *stream) {
   const int vec = row_vec(sizeof(T), a.dim, {a.table_stride, a.out_stride}, {a.table, a.out});
   if constexpr (sizeof(T) == 2) {
-    if (vec == 8) return pick_lookup<T, 8>(a, stream);
+    if (vec == 8) return run_lookup<T, 8>(a, stream);
   }
-  if (vec == 4) return pick_lookup<T, 4>(a, stream);
-  return pick_lookup<T, 1>(a, stream);
+  if (vec == 4) return run_lookup<T, 4>(a, stream);
+  return run_lookup<T, 1>(a, stream);
 }
 
 struct GradLayout {
@@ -839,7 +861,8 @@ int32_t sporder_embedding(void *stream, int32_t type, int64_t rows, int64_t dim,
   if (count == 0) return SPORDER_OK;
   if (!d_table || !d_tokens || !d_out) return SPORDER_BAD_ARGUMENT;
   const LookupArgs a{d_table, d_tokens,     d_out,      count, rows,
-                     dim,     table_stride, out_stride, scale, token_bits == 64};
+                     dim,     table_stride, out_stride, scale, token_bits == 64,
+                     count * dim * type_bytes(type) >= kStreamBytes, 0};
   if (type == SPORDER_TYPE_BF16) return lookup_typed<bf16_t>(a, stream);
   if (type == SPORDER_TYPE_F16) return lookup_typed<f16_t>(a, stream);
   return lookup_typed<float>(a, stream);
@@ -875,6 +898,7 @@ int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count, int64_
                    padding_idx,
                    scale,
                    token_bits == 64,
+                   rows * dim * type_bytes(out_type) >= kStreamBytes,
                    bits_for(rows),
                    0,
                    l.span,

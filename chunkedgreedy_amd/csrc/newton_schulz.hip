@@ -263,6 +263,22 @@ __device__ __forceinline__ void finish_block(const OrthoArgs &a, int64_t z, bool
   }
 }
 
+// Tile t of `down` x `across` tiles of kTileRows x kTileCols, four rows of
+// tiles at a time, so that the tiles in flight on an XCD share operands; or of
+// those on and above the diagonal, whose row ti begins at tile 2 ti.
+template <bool SYMMETRIC>
+__device__ __forceinline__ void product_tile(int t, int down, int across, int &ti, int &tj) {
+  if constexpr (SYMMETRIC) {
+    for (ti = 0; t >= across - 2 * ti; ++ti) t -= across - 2 * ti;
+    tj = 2 * ti + t;
+  } else {
+    const int group = t / (4 * across), rows = min(4, down - 4 * group);
+    t -= group * 4 * across;
+    ti = 4 * group + t % rows;
+    tj = t / rows;
+  }
+}
+
 // Tile t of a triangle of `across` rows: row ti holds across - ti tiles.
 __device__ __forceinline__ void triangle_tile(int t, int across, int &ti, int &tj) {
   const float side = 2 * across + 1;
@@ -272,111 +288,115 @@ __device__ __forceinline__ void triangle_tile(int t, int across, int &ti, int &t
   tj = ti + t - (ti * across - ti * (ti - 1) / 2);
 }
 
-// C = P Q^T of packed operands, one TILE x TILE tile per workgroup of 2 x 2
-// waves, 32 columns of both operands per stage: loaded to registers while the
-// stage before is multiplied, then stored to the other half of LDS.
+// C = P Q^T of packed operands, 256 x 128 per workgroup, 64 rows for each of
+// four waves, 32 columns of the operands per stage.  A wave reads its own rows
+// of P straight into registers, a stage ahead (no other wave of the workgroup
+// needs them); Q goes through LDS, which then has 80 KB to move per 1,536
+// cycles of products, where two operands in LDS would need twice that and
+// would bound the kernel.
 //   kGram:   P = Q = X;          writes A = C
 //   kPoly:   P = Q = A;          writes B = b A + c C
 //   kUpdate: P = B, Q = X^T;     writes X = a X + C in both orders
 //   kLast:   the same to out, rounded to its type
-template <int WHAT, int TILE, typename T>
-__global__ void __launch_bounds__(kBlock) ortho_product_kernel(OrthoArgs a) {
-  constexpr int kRows = TILE / 32;     // blocks of 32 rows of each operand
-  constexpr int kSide = kRows / 2;     // of a wave
-  constexpr int kStage = 4 * kWave;    // units of 32 rows and 32 columns: 2 blocks, hi and lo
-  __shared__ __attribute__((aligned(16))) uint4 lds[2][2][kRows * kStage];
+constexpr int kTileRows = 256, kTileCols = 128;
+
+template <int WHAT, typename T>
+__global__ void __launch_bounds__(kBlock, 2) ortho_product_kernel(OrthoArgs a) {
+  constexpr int kP = 2, kQ = kTileCols / 32; // blocks of 32 rows of P per wave, and of Q
+  constexpr int kStage = 4 * kWave;          // units of 32 rows and 32 columns: 2 blocks, hi and lo
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
+  __shared__ __attribute__((aligned(16))) u32x4 lds[2][kQ * kStage];
 
   const int64_t z = blockIdx.y;
   const int64_t xu = packed_units(a.mp, a.np), mu = packed_units(a.mp, a.mp);
   const uint4 *const p = WHAT == kGram ? a.x + z * xu : WHAT == kPoly ? a.gram + z * mu : a.poly + z * mu;
   const uint4 *const q = kSymmetric ? p : a.xt + z * xu;
   const int k_blocks = (WHAT == kGram ? a.np : a.mp) / 16; // both operands'
-  const int tiles_n = (kSymmetric ? a.mp : a.np) / TILE;
-
+  const int across = (kSymmetric ? a.mp : a.np) / kTileCols;
+  const int down = (a.mp + kTileRows - 1) / kTileRows;
   int ti, tj;
-  if (kSymmetric) {
-    triangle_tile(blockIdx.x, tiles_n, ti, tj);
-  } else {
-    ti = blockIdx.x / tiles_n;
-    tj = blockIdx.x % tiles_n;
-  }
+  product_tile<kSymmetric>(static_cast<int>(xcd_block()), down, across, ti, tj);
 
   const int tid = threadIdx.x, lane = lane_id(), wave = tid / kWave;
-  const int wy = wave / 2, wx = wave % 2;
   const int64_t step = static_cast<int64_t>(k_blocks) * 2 * kWave; // units of 32 operand rows
-  const uint4 *const pt = p + ti * kRows * step + tid;
-  const uint4 *const qt = q + tj * kRows * step + tid;
+  const int rb = ti * (kTileRows / 32) + wave * kP;                // first block of rows
+  const bool live = rb * 32 < a.mp; // the last tile may hold 128 rows; mp is a multiple of those
+  const u32x4 *const pt = reinterpret_cast<const u32x4 *>(p) + (live ? rb : 0) * step + lane;
+  const u32x4 *const qt = reinterpret_cast<const u32x4 *>(q) + tj * kQ * step + tid;
 
-  f32x16 acc[kSide][kSide];
-#pragma unroll
-  for (int i = 0; i < kSide; ++i) {
-#pragma unroll
-    for (int j = 0; j < kSide; ++j) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    }
-  }
-
-  u32x4 next[2][kRows];
-  auto fetch = [&](int stage) {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      next[0][r] = *reinterpret_cast<const u32x4 *>(pt + r * step + stage * kStage);
-      next[1][r] = *reinterpret_cast<const u32x4 *>(qt + r * step + stage * kStage);
-    }
-  };
-  auto put = [&](int half) {
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-      *reinterpret_cast<u32x4 *>(&lds[half][0][r * kStage + tid]) = next[0][r];
-      *reinterpret_cast<u32x4 *>(&lds[half][1][r * kStage + tid]) = next[1][r];
-    }
-  };
-  const int stages = k_blocks / 2;
-  fetch(0);
-  put(0);
-  __syncthreads();
-  for (int s = 0; s < stages; ++s) {
-    if (s + 1 < stages) fetch(s + 1);
-    const uint4 *const lp = lds[s & 1][0], *const lq = lds[s & 1][1];
+  f32x16 acc[kP][kQ] = {};
+  u32x4 pv[2][2][kP][2], qv[kQ]; // P: parity of the stage, block of columns, of rows, hi and lo
+  auto fetch_p = [&](u32x4(&v)[2][kP][2], int s) {
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      f16x8 ph[kSide], pl[kSide], qh[kSide], ql[kSide];
 #pragma unroll
-      for (int i = 0; i < kSide; ++i) {
-        const uint4 *const u = lp + (wy * kSide + i) * kStage + k * 2 * kWave + lane;
-        ph[i] = __builtin_bit_cast(f16x8, u[0]);
-        pl[i] = __builtin_bit_cast(f16x8, u[kWave]);
-        const uint4 *const w = lq + (wx * kSide + i) * kStage + k * 2 * kWave + lane;
-        qh[i] = __builtin_bit_cast(f16x8, w[0]);
-        ql[i] = __builtin_bit_cast(f16x8, w[kWave]);
-      }
+      for (int i = 0; i < kP; ++i) {
 #pragma unroll
-      for (int i = 0; i < kSide; ++i) {
-#pragma unroll
-        for (int j = 0; j < kSide; ++j) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(pl[i], qh[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], ql[j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ph[i], qh[j], acc[i][j], 0, 0, 0);
-        }
+        for (int h = 0; h < 2; ++h) v[k][i][h] = pt[i * step + s * kStage + (k * 2 + h) * kWave];
       }
     }
-    if (s + 1 < stages) put((s + 1) & 1);
-    __syncthreads();
+  };
+  auto fetch_q = [&](int s) {
+#pragma unroll
+    for (int r = 0; r < kQ; ++r) qv[r] = qt[r * step + s * kStage];
+  };
+  auto put_q = [&](int half) {
+#pragma unroll
+    for (int r = 0; r < kQ; ++r) lds[half][r * kStage + tid] = qv[r];
+  };
+  auto multiply = [&](const u32x4(&v)[2][kP][2], const u32x4 *lq) {
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+#pragma unroll
+      for (int j = 0; j < kQ; ++j) {
+        const f16x8 qh = __builtin_bit_cast(f16x8, lq[j * kStage + k * 2 * kWave + lane]);
+        const f16x8 ql = __builtin_bit_cast(f16x8, lq[j * kStage + (k * 2 + 1) * kWave + lane]);
+#pragma unroll
+        for (int i = 0; i < kP; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[k][i][1]), qh,
+                                                             acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kP; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[k][i][0]), ql,
+                                                             acc[i][j], 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < kP; ++i)
+          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, v[k][i][0]), qh,
+                                                             acc[i][j], 0, 0, 0);
+      }
+    }
+  };
+
+  const int stages = k_blocks / 2; // a multiple of 4
+  fetch_q(0);
+  fetch_p(pv[0], 0);
+  put_q(0);
+  __syncthreads();
+  for (int s = 0; s < stages; s += 2) {
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const int next = min(s + odd + 1, stages - 1);
+      fetch_q(next);
+      fetch_p(pv[odd ^ 1], next);
+      multiply(pv[odd], lds[odd]);
+      put_q(odd ^ 1);
+      __syncthreads();
+    }
   }
 
   // The accumulators hold products of two scaled values.
-  uint16_t *const stage = reinterpret_cast<uint16_t *>(&lds[0][0][0]) + wave * 32 * kStageRow;
+  uint16_t *const stage = reinterpret_cast<uint16_t *>(&lds[0][0]) + wave * 32 * kStageRow;
+  if (!live) return;
 #pragma unroll
-  for (int bi = 0; bi < kSide; ++bi) {
+  for (int i = 0; i < kP; ++i) {
 #pragma unroll
-    for (int bj = 0; bj < kSide; ++bj) {
-      const int i0 = ti * TILE + (wy * kSide + bi) * 32, j0 = tj * TILE + (wx * kSide + bj) * 32;
+    for (int j = 0; j < kQ; ++j) {
+      const int i0 = (rb + i) * 32, j0 = tj * kTileCols + j * 32;
+      if (kSymmetric && i0 > j0) continue; // the mirror image of another block
       float v[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = acc[bi][bj][r] * (1.0f / kScale);
-      finish_block<WHAT, T>(a, z, ti != tj, i0, j0, v, stage);
+      for (int r = 0; r < 16; ++r) v[r] = acc[i][j][r] * (1.0f / kScale);
+      finish_block<WHAT, T>(a, z, i0 != j0, i0, j0, v, stage);
     }
   }
 }
@@ -692,7 +712,7 @@ bool ortho_bounded(double a, double b, double c, int32_t steps) {
   return true;
 }
 
-constexpr int64_t kFewTiles = 256; // a tile of 128 x 128 for each CU
+constexpr int64_t kFewTiles = 128;
 
 template <typename T> int32_t run_norm(const OrthoArgs &a, int blocks, void *stream) {
   const int64_t cols = a.tall ? a.m : a.n;
@@ -704,15 +724,15 @@ template <typename T> int32_t run_norm(const OrthoArgs &a, int blocks, void *str
 
 template <int WHAT, typename T = float> int32_t run_product(const OrthoArgs &a, void *stream) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
-  auto tiles = [&](int64_t tile) {
-    const int64_t down = a.mp / tile, across = a.np / tile;
-    return kSymmetric ? down * (down + 1) / 2 : down * across;
-  };
-  if (tiles(128) * a.batch < kFewTiles)
-    return launch(ortho_split_kernel<WHAT, T>, dim3(tiles(64), a.batch), dim3(kSplitWaves * kWave),
-                  stream, a);
-  return launch(ortho_product_kernel<WHAT, 128, T>, dim3(tiles(128), a.batch), dim3(kBlock),
-                stream, a);
+  const int64_t down = ceil_div64(a.mp, kTileRows), across = (kSymmetric ? a.mp : a.np) / kTileCols;
+  const int64_t tiles = kSymmetric ? down * across - down * (down - 1) : down * across;
+  if (tiles * a.batch < kFewTiles) {
+    const int64_t m64 = a.mp / 64, n64 = a.np / 64;
+    return launch(ortho_split_kernel<WHAT, T>,
+                  dim3(kSymmetric ? m64 * (m64 + 1) / 2 : m64 * n64, a.batch),
+                  dim3(kSplitWaves * kWave), stream, a);
+  }
+  return launch(ortho_product_kernel<WHAT, T>, dim3(tiles, a.batch), dim3(kBlock), stream, a);
 }
 
 template <typename T>

@@ -61,11 +61,15 @@ __host__ __device__ constexpr int64_t packed_units(int64_t rows, int64_t cols) {
   return rows * cols / 4; // two halves of 2 bytes each: 4 bytes per element
 }
 
-__device__ __forceinline__ void split_halves(float v, uint32_t &hi, uint32_t &lo) {
-  const f16_t h = static_cast<f16_t>(v);
-  const f16_t l = static_cast<f16_t>(v - static_cast<float>(h));
-  hi = __builtin_bit_cast(uint16_t, h);
-  lo = __builtin_bit_cast(uint16_t, l);
+// The halves of two scaled values, hi and lo each packed in a word.
+__device__ __forceinline__ void split_halves(float x, float y, uint32_t &hi, uint32_t &lo) {
+  using f16x2 = f16_t __attribute__((ext_vector_type(2)));
+  using f32x2 = float __attribute__((ext_vector_type(2)));
+  const f32x2 v = {x, y};
+  const f16x2 h = __builtin_convertvector(v, f16x2);
+  const f16x2 l = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), f16x2);
+  hi = __builtin_bit_cast(uint32_t, h);
+  lo = __builtin_bit_cast(uint32_t, l);
 }
 
 __device__ __forceinline__ uint2 *col_place(uint4 *p, int k_blocks, int i0, int j0, int q,
@@ -85,22 +89,21 @@ __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col,
                                             uint4 *by_row, int k_row, int i0, int j0,
                                             uint16_t *stage) {
   const int lane = lane_id();
-  uint32_t half[2][16];
+  uint32_t half[2][8];
   u32x4 held[2][2];
 #pragma unroll
-  for (int r = 0; r < 16; ++r) split_halves(v[r], half[0][r], half[1][r]);
+  for (int r = 0; r < 8; ++r) split_halves(v[2 * r], v[2 * r + 1], half[0][r], half[1][r]);
 #pragma unroll
   for (int plane = 0; plane < 2; ++plane) {
-    const uint32_t(&h)[16] = half[plane];
+    const uint32_t(&h)[8] = half[plane];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      *col_place(by_col, k_col, i0, j0, q, plane, lane) =
-          make_uint2(h[4 * q] | h[4 * q + 1] << 16, h[4 * q + 2] | h[4 * q + 3] << 16);
+      *col_place(by_col, k_col, i0, j0, q, plane, lane) = make_uint2(h[2 * q], h[2 * q + 1]);
     if (!by_row) continue;
 #pragma unroll
     for (int r = 0; r < 16; ++r)
       stage[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * kStageRow + lane % 32] =
-          static_cast<uint16_t>(h[r]);
+          static_cast<uint16_t>(h[r / 2] >> 16 * (r % 2));
     wave_lds_order();
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -120,21 +123,30 @@ __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col,
   }
 }
 
-// The values (scaled) that store_block put into by_col.
-__device__ __forceinline__ void load_block(const uint4 *by_col, int k_col, int i0, int j0,
-                                           float (&v)[16]) {
-  const int lane = lane_id();
+// A block as store_block put it into by_col, to be fetched early.
+struct HeldBlock {
+  uint2 word[2][4]; // hi and lo
+};
+__device__ __forceinline__ HeldBlock fetch_block(const uint4 *by_col, int k_col, int i0, int j0) {
+  HeldBlock b;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      b.word[h][q] = *col_place(const_cast<uint4 *>(by_col), k_col, i0, j0, q, h, lane_id());
+  }
+  return b;
+}
+// v <- x (its scaled values) + y v.
+__device__ __forceinline__ void combine_block(const HeldBlock &b, float x, float y, float (&v)[16]) {
+  using f16x4 = f16_t __attribute__((ext_vector_type(4)));
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const uint2 h = *col_place(const_cast<uint4 *>(by_col), k_col, i0, j0, q, 0, lane);
-    const uint2 l = *col_place(const_cast<uint4 *>(by_col), k_col, i0, j0, q, 1, lane);
-    const uint32_t hs[4] = {h.x & 0xffff, h.x >> 16, h.y & 0xffff, h.y >> 16};
-    const uint32_t ls[4] = {l.x & 0xffff, l.x >> 16, l.y & 0xffff, l.y >> 16};
+    const f16x4 hi = __builtin_bit_cast(f16x4, b.word[0][q]);
+    const f16x4 lo = __builtin_bit_cast(f16x4, b.word[1][q]);
 #pragma unroll
     for (int e = 0; e < 4; ++e)
-      v[4 * q + e] =
-          static_cast<float>(__builtin_bit_cast(f16_t, static_cast<uint16_t>(hs[e]))) +
-          static_cast<float>(__builtin_bit_cast(f16_t, static_cast<uint16_t>(ls[e])));
+      v[4 * q + e] = x * (static_cast<float>(hi[e]) + static_cast<float>(lo[e])) + y * v[4 * q + e];
   }
 }
 
@@ -235,31 +247,35 @@ __device__ __forceinline__ void write_block(const OrthoArgs &a, int64_t z, int i
   }
 }
 
-// The epilogue of a product for one wave's block: v holds C, scaled once.
+// What a product's block (i0, j0) is combined with, where it is.
+template <int WHAT>
+__device__ __forceinline__ HeldBlock fetch_old(const OrthoArgs &a, int64_t z, int i0, int j0) {
+  if constexpr (WHAT == kGram) return {};
+  const uint4 *const from = WHAT == kPoly ? a.gram + z * packed_units(a.mp, a.mp)
+                                          : a.xt + z * packed_units(a.mp, a.np);
+  return fetch_block(from, a.mp / 16, i0, j0);
+}
+
+// The epilogue of a product for one wave's block: v holds C scaled twice.
 template <int WHAT, typename T>
 __device__ __forceinline__ void finish_block(const OrthoArgs &a, int64_t z, bool mirror, int i0,
-                                             int j0, float (&v)[16], uint16_t *stage) {
+                                             int j0, float (&v)[16], const HeldBlock &old,
+                                             uint16_t *stage) {
   const int64_t xu = packed_units(a.mp, a.np), mu = packed_units(a.mp, a.mp);
   const int km = a.mp / 16, kn = a.np / 16;
   if constexpr (WHAT == kGram) {
-    uint4 *const to = a.gram + z * mu;
-    store_block(v, to, km, mirror ? to : nullptr, km, i0, j0, stage);
-  } else if constexpr (WHAT == kPoly) {
-    float old[16];
-    load_block(a.gram + z * mu, km, i0, j0, old);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) v[r] = a.b * old[r] + a.c * v[r];
-    uint4 *const to = a.poly + z * mu;
-    store_block(v, to, km, mirror ? to : nullptr, km, i0, j0, stage);
+    for (int r = 0; r < 16; ++r) v[r] *= 1.0f / kScale;
   } else {
-    float old[16];
-    load_block(a.xt + z * xu, km, i0, j0, old);
-#pragma unroll
-    for (int r = 0; r < 16; ++r) v[r] = a.a * old[r] + v[r];
-    if constexpr (WHAT == kUpdate)
-      store_block(v, a.xt_next + z * xu, km, a.x + z * xu, kn, i0, j0, stage);
-    else
-      write_block<T>(a, z, i0, j0, v);
+    combine_block(old, WHAT == kPoly ? a.b : a.a, (WHAT == kPoly ? a.c : 1.0f) / kScale, v);
+  }
+  if constexpr (WHAT == kGram || WHAT == kPoly) {
+    uint4 *const to = (WHAT == kGram ? a.gram : a.poly) + z * mu;
+    store_block(v, to, km, mirror ? to : nullptr, km, i0, j0, stage);
+  } else if constexpr (WHAT == kUpdate) {
+    store_block(v, a.xt_next + z * xu, km, a.x + z * xu, kn, i0, j0, stage);
+  } else {
+    write_block<T>(a, z, i0, j0, v);
   }
 }
 
@@ -395,8 +411,8 @@ __global__ void __launch_bounds__(kBlock, 2) ortho_product_kernel(OrthoArgs a) {
       if (kSymmetric && i0 > j0) continue; // the mirror image of another block
       float v[16];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[r] = acc[i][j][r] * (1.0f / kScale);
-      finish_block<WHAT, T>(a, z, i0 != j0, i0, j0, v, stage);
+      for (int r = 0; r < 16; ++r) v[r] = acc[i][j][r];
+      finish_block<WHAT, T>(a, z, i0 != j0, i0, j0, v, fetch_old<WHAT>(a, z, i0, j0), stage);
     }
   }
 }
@@ -408,8 +424,10 @@ __global__ void __launch_bounds__(kBlock, 2) ortho_product_kernel(OrthoArgs a) {
 constexpr int kSplitWaves = 8;
 constexpr int kAhead = 4;
 
+// With first >= 0 they are the tiles of ortho_product_kernel from that one on,
+// each as eight of these.
 template <int WHAT, typename T>
-__global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoArgs a) {
+__global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoArgs a, int first_tile) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
   constexpr int kHalf = kSplitWaves / 2;
   __shared__ float sums[kHalf][4][16][kWave];
@@ -420,7 +438,13 @@ __global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoAr
   const int k_blocks = (WHAT == kGram ? a.np : a.mp) / 16;
   const int across = (kSymmetric ? a.mp : a.np) / 64;
   int ti, tj;
-  if (kSymmetric) {
+  if (first_tile >= 0) {
+    product_tile<kSymmetric>(first_tile + blockIdx.x / 8, (a.mp + kTileRows - 1) / kTileRows,
+                             across / 2, ti, tj);
+    ti = ti * 4 + blockIdx.x % 8 / 2;
+    tj = tj * 2 + blockIdx.x % 2;
+    if (ti * 64 >= a.mp || (kSymmetric && ti > tj)) return;
+  } else if (kSymmetric) {
     triangle_tile(blockIdx.x, across, ti, tj);
   } else {
     ti = blockIdx.x / across;
@@ -433,6 +457,9 @@ __global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoAr
   const uint4 *const pt = p + ti * 2 * step + first;
   const uint4 *const qt = q + tj * 2 * step + first;
 
+  const int i0 = ti * 64 + wave % 4 / 2 * 32, j0 = tj * 64 + wave % 2 * 32; // finished by this wave
+  HeldBlock old;
+  if (wave < kHalf) old = fetch_old<WHAT>(a, z, i0, j0);
   f32x16 acc[2][2] = {};
   u32x4 next[kAhead][2][2][2]; // step, operand, block of 32 rows, hi and lo
   auto fetch = [&](u32x4(&o)[2][2][2], int k) {
@@ -488,13 +515,12 @@ __global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoAr
   float v[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r)
-    v[r] = ((sums[0][wave][r][lane] + sums[1][wave][r][lane]) +
-            (sums[2][wave][r][lane] + sums[3][wave][r][lane])) *
-           (1.0f / kScale);
+    v[r] = (sums[0][wave][r][lane] + sums[1][wave][r][lane]) +
+           (sums[2][wave][r][lane] + sums[3][wave][r][lane]);
   // Only this wave reads block `wave` of the sums: one of them becomes its stage.
   wave_lds_order();
   uint16_t *const stage = reinterpret_cast<uint16_t *>(&sums[0][wave][0][0]);
-  finish_block<WHAT, T>(a, z, ti != tj, ti * 64 + wave / 2 * 32, tj * 64 + wave % 2 * 32, v, stage);
+  finish_block<WHAT, T>(a, z, ti != tj, i0, j0, v, old, stage);
 }
 
 // A whole matrix in one workgroup, X and X^T in LDS (at most 16 blocks of
@@ -568,7 +594,8 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
   }
   __syncthreads();
 
-  // v = blocks (bi, bj) and (bi, bj + more) of P Q^T, operands of k blocks.
+  // v = blocks (bi, bj) and (bi, bj + more) of P Q^T, scaled twice, operands of
+  // k blocks.
   auto product = [&](const uint4 *p, const uint4 *q, int k_blocks, int bi, int bj, int more) {
     f32x16 acc[2] = {};
     const uint4 *const pt = p + bi * k_blocks * 2 * kWave + lane;
@@ -600,7 +627,7 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[t][r] = acc[t][r] * (1.0f / kScale);
+      for (int r = 0; r < 16; ++r) v[t][r] = acc[t][r];
     }
   };
   auto store_a = [&]() {
@@ -613,26 +640,28 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
 
   for (int step = 0; step < steps; ++step) {
     if (blocks_a) product(x, x, kn, ai, aj, blocks_a - 1);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) v[t][r] *= 1.0f / kScale;
+    }
     store_a();
+    HeldBlock old[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (t < blocks_a) old[t] = fetch_block(x, km, ai * 32, (aj + t) * 32);
     if (blocks_a) product(x, x, km, ai, aj, blocks_a - 1);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t >= blocks_a) continue;
-      float old[16];
-      load_block(x, km, ai * 32, (aj + t) * 32, old);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) v[t][r] = a.b * old[r] + a.c * v[t][r];
-    }
+    for (int t = 0; t < 2; ++t)
+      if (t < blocks_a) combine_block(old[t], a.b, a.c / kScale, v[t]);
     store_a();
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+      if (t < blocks_x) old[t] = fetch_block(xt, km, xi * 32, (xj + t) * 32);
     if (blocks_x) product(x, xt, km, xi, xj, blocks_x - 1);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (t >= blocks_x) continue;
-      float old[16];
-      load_block(xt, km, xi * 32, (xj + t) * 32, old);
-#pragma unroll
-      for (int r = 0; r < 16; ++r) v[t][r] = a.a * old[r] + v[t][r];
-    }
+    for (int t = 0; t < 2; ++t)
+      if (t < blocks_x) combine_block(old[t], a.a, 1.0f / kScale, v[t]);
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -712,7 +741,9 @@ bool ortho_bounded(double a, double b, double c, int32_t steps) {
   return true;
 }
 
+constexpr int64_t kCus = 256;     // of an MI355X
 constexpr int64_t kFewTiles = 128;
+constexpr int64_t kMostOver = 96;
 
 template <typename T> int32_t run_norm(const OrthoArgs &a, int blocks, void *stream) {
   const int64_t cols = a.tall ? a.m : a.n;
@@ -730,9 +761,17 @@ template <int WHAT, typename T = float> int32_t run_product(const OrthoArgs &a, 
     const int64_t m64 = a.mp / 64, n64 = a.np / 64;
     return launch(ortho_split_kernel<WHAT, T>,
                   dim3(kSymmetric ? m64 * (m64 + 1) / 2 : m64 * n64, a.batch),
-                  dim3(kSplitWaves * kWave), stream, a);
+                  dim3(kSplitWaves * kWave), stream, a, -1);
   }
-  return launch(ortho_product_kernel<WHAT, T>, dim3(tiles, a.batch), dim3(kBlock), stream, a);
+  // A CU's tiles take turns: with few tiles past a multiple of the CUs, some CUs
+  // would have one more and the rest would wait, so those few are split.
+  const int64_t over = a.batch == 1 && tiles > kCus && tiles % kCus <= kMostOver ? tiles % kCus : 0;
+  int32_t rc = launch(ortho_product_kernel<WHAT, T>, dim3(tiles - over, a.batch), dim3(kBlock),
+                      stream, a);
+  if (rc == SPORDER_OK && over > 0)
+    rc = launch(ortho_split_kernel<WHAT, T>, dim3(8 * over), dim3(kSplitWaves * kWave), stream, a,
+                static_cast<int>(tiles - over));
+  return rc;
 }
 
 template <typename T>

@@ -198,17 +198,8 @@ __global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(OrthoArgs a) {
 // Packs X = G / (|G| + eps), 64 x 64 per workgroup, a 32 x 32 block per wave.
 template <typename T>
 __global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int norm_blocks) {
-  __shared__ double part[kBlock];
   __shared__ __attribute__((aligned(16))) uint16_t stage[4][32 * kStageRow];
   const int64_t z = blockIdx.y;
-  part[threadIdx.x] =
-      static_cast<int>(threadIdx.x) < norm_blocks ? a.partial[z * kNormBlocks + threadIdx.x] : 0.0;
-  __syncthreads();
-  for (int k = kBlock / 2; k > 0; k /= 2) {
-    if (threadIdx.x < k) part[threadIdx.x] += part[threadIdx.x + k];
-    __syncthreads();
-  }
-  const double scale = static_cast<double>(kScale) / (sqrt(part[0]) + a.eps);
   const int wave = threadIdx.x / kWave, lane = lane_id();
   const int across = a.np / 64;
   const int i0 = blockIdx.x / across * 64 + wave / 2 * 32;
@@ -223,6 +214,13 @@ __global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int nor
     if (i < a.m && j < a.n)
       v[r] = static_cast<float>(g[a.tall ? j * a.g_stride + i : i * a.g_stride + j]);
   }
+  double square = 0.0;
+#pragma unroll
+  for (int k = 0; k < kNormBlocks / kWave; ++k)
+    if (lane + k * kWave < norm_blocks) square += a.partial[z * kNormBlocks + lane + k * kWave];
+#pragma unroll
+  for (int k = 1; k < kWave; k <<= 1) square += __shfl_xor(square, k);
+  const double scale = static_cast<double>(kScale) / (sqrt(square) + a.eps);
 #pragma unroll
   for (int r = 0; r < 16; ++r) v[r] = static_cast<float>(v[r] * scale);
   const int64_t units = packed_units(a.mp, a.np);
@@ -279,29 +277,33 @@ __device__ __forceinline__ void finish_block(const OrthoArgs &a, int64_t z, bool
   }
 }
 
-// Tile t of `down` x `across` tiles of kTileRows x kTileCols, four rows of
-// tiles at a time, so that the tiles in flight on an XCD share operands; or of
-// those on and above the diagonal, whose row ti begins at tile 2 ti.
-template <bool SYMMETRIC>
-__device__ __forceinline__ void product_tile(int t, int down, int across, int &ti, int &tj) {
-  if constexpr (SYMMETRIC) {
-    for (ti = 0; t >= across - 2 * ti; ++ti) t -= across - 2 * ti;
-    tj = 2 * ti + t;
-  } else {
-    const int group = t / (4 * across), rows = min(4, down - 4 * group);
-    t -= group * 4 * across;
-    ti = 4 * group + t % rows;
-    tj = t / rows;
+// Tile t of `down` x `across` tiles, `group` rows of tiles at a time and down
+// each column of them, so that neighbouring tiles share operands on both
+// sides; with `ratio` > 0, of those on and above the diagonal, where row ti
+// begins at tile ratio ti.
+__device__ __forceinline__ void place_tile(int t, int down, int across, int ratio, int group,
+                                           int &ti, int &tj) {
+  for (int g = 0;; g += group) {
+    const int rows = min(group, down - g), left = across - ratio * g;
+    const int corner = ratio ? min(rows * ratio, left) : 0; // columns not all rows reach
+    const int cut = ratio * rows * (rows - 1) / 2;
+    const int all = rows * left - cut;
+    if (t >= all) {
+      t -= all;
+      continue;
+    }
+    const int in_corner = rows * corner - cut;
+    if (t >= in_corner) {
+      t -= in_corner;
+      ti = g + t % rows;
+      tj = ratio * g + corner + t / rows;
+      return;
+    }
+    for (ti = 0; t >= corner - ratio * ti; ++ti) t -= corner - ratio * ti;
+    tj = ratio * (g + ti) + t;
+    ti += g;
+    return;
   }
-}
-
-// Tile t of a triangle of `across` rows: row ti holds across - ti tiles.
-__device__ __forceinline__ void triangle_tile(int t, int across, int &ti, int &tj) {
-  const float side = 2 * across + 1;
-  ti = static_cast<int>((side - sqrtf(side * side - 8.0f * t)) / 2);
-  while (ti > 0 && ti * across - ti * (ti - 1) / 2 > t) --ti;
-  while ((ti + 1) * across - (ti + 1) * ti / 2 <= t) ++ti;
-  tj = ti + t - (ti * across - ti * (ti - 1) / 2);
 }
 
 // C = P Q^T of packed operands, 256 x 128 per workgroup, 64 rows for each of
@@ -331,7 +333,7 @@ __global__ void __launch_bounds__(kBlock, 2) ortho_product_kernel(OrthoArgs a) {
   const int across = (kSymmetric ? a.mp : a.np) / kTileCols;
   const int down = (a.mp + kTileRows - 1) / kTileRows;
   int ti, tj;
-  product_tile<kSymmetric>(static_cast<int>(xcd_block()), down, across, ti, tj);
+  place_tile(static_cast<int>(xcd_block()), down, across, kSymmetric ? 2 : 0, 4, ti, tj);
 
   const int tid = threadIdx.x, lane = lane_id(), wave = tid / kWave;
   const int64_t step = static_cast<int64_t>(k_blocks) * 2 * kWave; // units of 32 operand rows
@@ -417,19 +419,20 @@ __global__ void __launch_bounds__(kBlock, 2) ortho_product_kernel(OrthoArgs a) {
   }
 }
 
-// The same for products of few tiles: 64 x 64 per workgroup, whose eight waves
-// each take an eighth of the columns and read their operands straight from
-// memory (in the units' own order, so without LDS), four steps ahead; the
-// sums meet in LDS, a block of 32 x 32 for each of four waves.
-constexpr int kSplitWaves = 8;
+// The same for products of few tiles: 64 x 64 per workgroup, whose four or
+// eight waves each take a part of the columns and read their operands straight
+// from memory (in the units' own order, so without LDS), four steps ahead; the
+// sums meet in LDS, a block of 32 x 32 for each of four waves.  A CU holds
+// eight such waves: eight per tile while there is a CU for each tile, else
+// four (1024 x 1536 in 1024: 24 us with eight, 20 with four).
 constexpr int kAhead = 4;
 
 // With first >= 0 they are the tiles of ortho_product_kernel from that one on,
 // each as eight of these.
-template <int WHAT, typename T>
-__global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoArgs a, int first_tile) {
+template <int WHAT, typename T, int WAVES>
+__global__ void __launch_bounds__(WAVES *kWave) ortho_split_kernel(OrthoArgs a, int first_tile) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
-  constexpr int kHalf = kSplitWaves / 2;
+  constexpr int kHalf = WAVES / 2;
   __shared__ float sums[kHalf][4][16][kWave];
   const int64_t z = blockIdx.y;
   const int64_t xu = packed_units(a.mp, a.np), mu = packed_units(a.mp, a.mp);
@@ -438,28 +441,26 @@ __global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoAr
   const int k_blocks = (WHAT == kGram ? a.np : a.mp) / 16;
   const int across = (kSymmetric ? a.mp : a.np) / 64;
   int ti, tj;
+  const int t = static_cast<int>(xcd_block());
   if (first_tile >= 0) {
-    product_tile<kSymmetric>(first_tile + blockIdx.x / 8, (a.mp + kTileRows - 1) / kTileRows,
-                             across / 2, ti, tj);
-    ti = ti * 4 + blockIdx.x % 8 / 2;
-    tj = tj * 2 + blockIdx.x % 2;
+    place_tile(first_tile + t / 8, (a.mp + kTileRows - 1) / kTileRows, across / 2,
+               kSymmetric ? 2 : 0, 4, ti, tj);
+    ti = ti * 4 + t % 8 / 2;
+    tj = tj * 2 + t % 2;
     if (ti * 64 >= a.mp || (kSymmetric && ti > tj)) return;
-  } else if (kSymmetric) {
-    triangle_tile(blockIdx.x, across, ti, tj);
   } else {
-    ti = blockIdx.x / across;
-    tj = blockIdx.x % across;
+    place_tile(t, a.mp / 64, across, kSymmetric ? 1 : 0, kSymmetric ? 4 : 8, ti, tj);
   }
   const int wave = threadIdx.x / kWave, lane = lane_id();
   const int64_t step = static_cast<int64_t>(k_blocks) * 2 * kWave;
-  const int mine = k_blocks / kSplitWaves; // padded columns: a multiple of 8 blocks
+  const int mine = k_blocks / WAVES; // padded columns: a multiple of 8 blocks
   const int64_t first = static_cast<int64_t>(wave * mine) * 2 * kWave + lane;
   const uint4 *const pt = p + ti * 2 * step + first;
   const uint4 *const qt = q + tj * 2 * step + first;
 
   const int i0 = ti * 64 + wave % 4 / 2 * 32, j0 = tj * 64 + wave % 2 * 32; // finished by this wave
   HeldBlock old;
-  if (wave < kHalf) old = fetch_old<WHAT>(a, z, i0, j0);
+  if (wave < 4) old = fetch_old<WHAT>(a, z, i0, j0);
   f32x16 acc[2][2] = {};
   u32x4 next[kAhead][2][2][2]; // step, operand, block of 32 rows, hi and lo
   auto fetch = [&](u32x4(&o)[2][2][2], int k) {
@@ -511,12 +512,13 @@ __global__ void __launch_bounds__(kSplitWaves *kWave) ortho_split_kernel(OrthoAr
     }
   }
   __syncthreads();
-  if (wave >= kHalf) return;
+  if (wave >= 4) return;
   float v[16];
 #pragma unroll
-  for (int r = 0; r < 16; ++r)
-    v[r] = (sums[0][wave][r][lane] + sums[1][wave][r][lane]) +
-           (sums[2][wave][r][lane] + sums[3][wave][r][lane]);
+  for (int r = 0; r < 16; ++r) {
+    v[r] = sums[0][wave][r][lane] + sums[1][wave][r][lane];
+    if constexpr (WAVES == 8) v[r] += sums[2][wave][r][lane] + sums[3][wave][r][lane];
+  }
   // Only this wave reads block `wave` of the sums: one of them becomes its stage.
   wave_lds_order();
   uint16_t *const stage = reinterpret_cast<uint16_t *>(&sums[0][wave][0][0]);
@@ -753,15 +755,22 @@ template <typename T> int32_t run_norm(const OrthoArgs &a, int blocks, void *str
   return launch(ortho_norm_kernel<T, 1>, dim3(blocks, a.batch), dim3(kNormThreads), stream, a);
 }
 
+template <int WHAT, typename T>
+int32_t run_split(const OrthoArgs &a, int64_t tiles, int first, void *stream) {
+  if (tiles * a.batch <= kCus)
+    return launch(ortho_split_kernel<WHAT, T, 8>, dim3(tiles, a.batch), dim3(8 * kWave), stream, a,
+                  first);
+  return launch(ortho_split_kernel<WHAT, T, 4>, dim3(tiles, a.batch), dim3(4 * kWave), stream, a,
+                first);
+}
+
 template <int WHAT, typename T = float> int32_t run_product(const OrthoArgs &a, void *stream) {
   constexpr bool kSymmetric = WHAT == kGram || WHAT == kPoly;
   const int64_t down = ceil_div64(a.mp, kTileRows), across = (kSymmetric ? a.mp : a.np) / kTileCols;
   const int64_t tiles = kSymmetric ? down * across - down * (down - 1) : down * across;
   if (tiles * a.batch < kFewTiles) {
     const int64_t m64 = a.mp / 64, n64 = a.np / 64;
-    return launch(ortho_split_kernel<WHAT, T>,
-                  dim3(kSymmetric ? m64 * (m64 + 1) / 2 : m64 * n64, a.batch),
-                  dim3(kSplitWaves * kWave), stream, a, -1);
+    return run_split<WHAT, T>(a, kSymmetric ? m64 * (m64 + 1) / 2 : m64 * n64, -1, stream);
   }
   // A CU's tiles take turns: with few tiles past a multiple of the CUs, some CUs
   // would have one more and the rest would wait, so those few are split.
@@ -769,8 +778,7 @@ template <int WHAT, typename T = float> int32_t run_product(const OrthoArgs &a, 
   int32_t rc = launch(ortho_product_kernel<WHAT, T>, dim3(tiles - over, a.batch), dim3(kBlock),
                       stream, a);
   if (rc == SPORDER_OK && over > 0)
-    rc = launch(ortho_split_kernel<WHAT, T>, dim3(8 * over), dim3(kSplitWaves * kWave), stream, a,
-                static_cast<int>(tiles - over));
+    rc = run_split<WHAT, T>(a, 8 * over, static_cast<int>(tiles - over), stream);
   return rc;
 }
 

@@ -67,7 +67,10 @@ __device__ __forceinline__ void split_halves(float x, float y, uint32_t &hi, uin
   using f32x2 = float __attribute__((ext_vector_type(2)));
   const f32x2 v = {x, y};
   const f16x2 h = __builtin_convertvector(v, f16x2);
-  const f16x2 l = __builtin_convertvector(v - __builtin_convertvector(h, f32x2), f16x2);
+  // As products with -1: one mixed-precision instruction each, and exact.
+  const f32x2 rest = {__builtin_fmaf(static_cast<float>(h.x), -1.0f, x),
+                      __builtin_fmaf(static_cast<float>(h.y), -1.0f, y)};
+  const f16x2 l = __builtin_convertvector(rest, f16x2);
   hi = __builtin_bit_cast(uint32_t, h);
   lo = __builtin_bit_cast(uint32_t, l);
 }
@@ -100,10 +103,15 @@ __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col,
     for (int q = 0; q < 4; ++q)
       *col_place(by_col, k_col, i0, j0, q, plane, lane) = make_uint2(h[2 * q], h[2 * q + 1]);
     if (!by_row) continue;
+    // A word holds rows r and r + 1 of a column; with the neighbouring
+    // column's, an even lane makes row r's word of both and an odd one r + 1's.
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-      stage[(8 * (r / 4) + 4 * (lane / 32) + r % 4) * kStageRow + lane % 32] =
-          static_cast<uint16_t>(h[r / 2] >> 16 * (r % 2));
+    for (int r = 0; r < 16; r += 2) {
+      const uint32_t word = __builtin_amdgcn_perm(lane_xor_u32(h[r / 2], 1), h[r / 2],
+                                                  lane & 1 ? 0x03020706 : 0x05040100);
+      const int row = 8 * (r / 4) + 4 * (lane / 32) + r % 4 + (lane & 1);
+      *reinterpret_cast<uint32_t *>(stage + row * kStageRow + (lane % 32 & ~1)) = word;
+    }
     wave_lds_order();
 #pragma unroll
     for (int s = 0; s < 2; ++s)
@@ -555,7 +563,7 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
   const int blocks_x = xi < mb ? min(2, nb - xj) : 0, blocks_a = ai < mb ? min(2, mb - aj) : 0;
 
   const T *const g = static_cast<const T *>(a.g) + z * a.g_batch;
-  float v[2][16];
+  float va[2][16], vx[2][16]; // this wave's blocks of A or B, and of X, scaled
   double s = 0.0;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
@@ -563,16 +571,16 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
       const int i = xi * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
-      v[t][r] = 0.0f;
+      vx[t][r] = 0.0f;
       if (t < blocks_x && i < a.m && j < a.n)
-        v[t][r] = static_cast<float>(g[a.tall ? j * a.g_stride + i : i * a.g_stride + j]);
+        vx[t][r] = static_cast<float>(g[a.tall ? j * a.g_stride + i : i * a.g_stride + j]);
     }
   }
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      s += static_cast<double>(v[t][r]) * v[t][r];
+      s += static_cast<double>(vx[t][r]) * vx[t][r];
     }
   }
   for (int k = 1; k < kWave; k <<= 1) s += __shfl_xor(s, k);
@@ -585,21 +593,26 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
   // A block's place in x is its own until the barrier after: its stage.
   auto store_x = [&](int t) {
     uint4 *const place = x + (xi * kn + (xj + t) * 2) * 2 * kWave;
-    store_block(v[t], xt, km, x, kn, xi * 32, (xj + t) * 32, reinterpret_cast<uint16_t *>(place));
+    store_block(vx[t], xt, km, x, kn, xi * 32, (xj + t) * 32, reinterpret_cast<uint16_t *>(place));
   };
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     if (t >= blocks_x) continue;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) v[t][r] = static_cast<float>(v[t][r] * scale);
+    for (int r = 0; r < 16; ++r) vx[t][r] = static_cast<float>(vx[t][r] * scale);
     store_x(t);
   }
   __syncthreads();
 
-  // v = blocks (bi, bj) and (bi, bj + more) of P Q^T, scaled twice, operands of
-  // k blocks.
+  // acc = blocks (bi, bj) and (bi, bj + more) of P Q^T, scaled twice, operands
+  // of k blocks.
+  f32x16 acc[2];
   auto product = [&](const uint4 *p, const uint4 *q, int k_blocks, int bi, int bj, int more) {
-    f32x16 acc[2] = {};
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[t][r] = 0.0f;
+    }
     const uint4 *const pt = p + bi * k_blocks * 2 * kWave + lane;
     const uint4 *const qt = q + bj * k_blocks * 2 * kWave + lane;
     const uint4 *const rt = qt + more * k_blocks * 2 * kWave;
@@ -626,17 +639,12 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
         }
       }
     }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) v[t][r] = acc[t][r];
-    }
   };
   auto store_a = [&]() {
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < 2; ++t)
-      if (t < blocks_a) store_block(v[t], x, km, nullptr, 0, ai * 32, (aj + t) * 32, nullptr);
+      if (t < blocks_a) store_block(va[t], x, km, nullptr, 0, ai * 32, (aj + t) * 32, nullptr);
     __syncthreads();
   };
 
@@ -645,25 +653,22 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) v[t][r] *= 1.0f / kScale;
+      for (int r = 0; r < 16; ++r) va[t][r] = acc[t][r] * (1.0f / kScale);
     }
     store_a();
-    HeldBlock old[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (t < blocks_a) old[t] = fetch_block(x, km, ai * 32, (aj + t) * 32);
     if (blocks_a) product(x, x, km, ai, aj, blocks_a - 1);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (t < blocks_a) combine_block(old[t], a.b, a.c / kScale, v[t]);
-    store_a();
+    for (int t = 0; t < 2; ++t) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (t < blocks_x) old[t] = fetch_block(xt, km, xi * 32, (xj + t) * 32);
+      for (int r = 0; r < 16; ++r) va[t][r] = a.b * va[t][r] + a.c / kScale * acc[t][r];
+    }
+    store_a();
     if (blocks_x) product(x, xt, km, xi, xj, blocks_x - 1);
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (t < blocks_x) combine_block(old[t], a.a, 1.0f / kScale, v[t]);
+    for (int t = 0; t < 2; ++t) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) vx[t][r] = a.a * vx[t][r] + 1.0f / kScale * acc[t][r];
+    }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
@@ -671,7 +676,7 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
       if (step + 1 < steps)
         store_x(t);
       else
-        write_block<T>(a, z, xi * 32, (xj + t) * 32, v[t]);
+        write_block<T>(a, z, xi * 32, (xj + t) * 32, vx[t]);
     }
     __syncthreads();
   }

@@ -25,6 +25,17 @@ With --fused-scaling the operator is one call of
 SpMM: the same values bit for bit, without the two elementwise passes); the
 default keeps the reference driver's three steps.
 
+Three more options train a richer model with this library's training operators
+(``chunkedgreedy_amd.nn``), which the reference driver has none of; without
+them the model and its results are the reference's:
+
+  --embed       the node features are learned: X is a table of node vectors
+                (started from the same values), looked up by node id, so that a
+                reordering permutes the ids and not the features
+  --layer-norm  a layer norm on the hidden layer, before its relu
+  --muon        the two weight matrices are updated along their orthogonalised
+                momentum; biases, norm and table stay with Adam
+
 Usage:  python -m chunkedgreedy_amd.e2e_gcn [--nodes N] [--epochs E] ...
 prints one JSON record per ordering (ORIGIN and sporder-csg by default;
 sporder-cg on request).
@@ -97,11 +108,17 @@ def _spmm_fn():
 
 
 def train(ptr, ind, X, y, *, hidden: int, classes: int, epochs: int, warmup: int = 3,
-          seed: int = 0, ctx=None, fused: bool = False) -> dict:
+          seed: int = 0, ctx=None, fused: bool = False, tokens=None, norm: bool = False,
+          muon: bool = False) -> dict:
     """Train the 2-layer GCN for `epochs` timed epochs after `warmup` untimed
-    ones; returns per-epoch times, SpMM time per epoch and the losses."""
+    ones; returns per-epoch times, SpMM time per epoch and the losses.  With
+    `tokens` (a node id per row) X is the start of a learned table of node
+    vectors; `norm` puts a layer norm on the hidden layer; `muon` updates the
+    weight matrices along their orthogonalised momentum."""
     import torch
     import torch.nn.functional as F
+
+    from chunkedgreedy_amd import nn
 
     t0 = time.perf_counter()
     op = GraphOp(ptr, ind, ctx=ctx, fused=fused)
@@ -110,15 +127,32 @@ def train(ptr, ind, X, y, *, hidden: int, classes: int, epochs: int, warmup: int
     torch.manual_seed(seed)
     W1 = torch.nn.Linear(X.shape[1], hidden).to(X.device)
     W2 = torch.nn.Linear(hidden, classes).to(X.device)
-    opt = torch.optim.Adam(list(W1.parameters()) + list(W2.parameters()), lr=0.01)
+    params = list(W1.parameters()) + list(W2.parameters())
+    opts = []
+    if muon:
+        opts.append(nn.Muon([p for p in params if p.dim() == 2]))
+        params = [p for p in params if p.dim() != 2]
+    if norm:
+        scale = torch.nn.Parameter(torch.ones(hidden, device=X.device))
+        shift = torch.nn.Parameter(torch.zeros(hidden, device=X.device))
+        params += [scale, shift]
+    if tokens is not None:
+        table = torch.nn.Parameter(X.clone())
+        params.append(table)
+    opts.append(torch.optim.Adam(params, lr=0.01))
 
     def epoch():
-        opt.zero_grad()
-        h1 = F.relu(SpMMFn.apply(W1(X), op))
-        z = W2(SpMMFn.apply(h1, op))
+        for opt in opts:
+            opt.zero_grad()
+        h0 = X if tokens is None else nn.embedding(table, tokens)
+        h1 = SpMMFn.apply(W1(h0), op)
+        if norm:
+            h1 = nn.layer_norm(h1, scale, shift)
+        z = W2(SpMMFn.apply(F.relu(h1), op))
         loss = -F.log_softmax(z, 1).gather(1, y[:, None]).mean()
         loss.backward()
-        opt.step()
+        for opt in opts:
+            opt.step()
         return loss
 
     losses = []
@@ -148,7 +182,8 @@ def permute_graph(ptr, ind, X, y, order, ctx=None):
 
 
 def run(ptr_h, ind_h, *, features: int, hidden: int, classes: int, epochs: int,
-        orders=("ORIGIN", "sporder-csg"), seed: int = 0, fused: bool = False) -> list[dict]:
+        orders=("ORIGIN", "sporder-csg"), seed: int = 0, fused: bool = False,
+        embed: bool = False, norm: bool = False, muon: bool = False) -> list[dict]:
     import torch
 
     from chunkedgreedy_amd import sporder
@@ -171,6 +206,7 @@ def run(ptr_h, ind_h, *, features: int, hidden: int, classes: int, epochs: int,
         if name == "ORIGIN":
             reorder_ms, perm_ms = 0.0, 0.0
             ptr_u, ind_u, X, y = ptr, ind, X0, y0
+            order = torch.arange(n, dtype=torch.int32, device=dev) if embed else None
         else:
             entry = entries[name]
             entry(ptr, ind, is_symmetric=True, ctx=ctx)  # warmup
@@ -181,10 +217,14 @@ def run(ptr_h, ind_h, *, features: int, hidden: int, classes: int, epochs: int,
             t0 = time.perf_counter()
             ptr_u, ind_u, X, y = permute_graph(ptr, ind, X0, y0, order, ctx=ctx)
             perm_ms = _sync_ms(torch, t0)
-        r = train(ptr_u, ind_u, X, y, hidden=hidden, classes=classes, epochs=epochs, seed=seed,
-                  ctx=ctx, fused=fused)
+        r = train(ptr_u, ind_u, X0 if embed else X, y, hidden=hidden, classes=classes,
+                  epochs=epochs, seed=seed, ctx=ctx, fused=fused,
+                  tokens=order if embed else None, norm=norm, muon=muon)
         total = reorder_ms + perm_ms + r["prep_ms"] + epochs * r["epoch_ms"]
-        rows.append({"order": name, "fused_scaling": fused, "n": n, "nnz": int(ind_h.shape[0]),
+        extras = {k: True for k, on in (("embed", embed), ("layer_norm", norm), ("muon", muon))
+                  if on}
+        rows.append({"order": name, "fused_scaling": fused, **extras, "n": n,
+                     "nnz": int(ind_h.shape[0]),
                      "features": features,
                      "hidden": hidden, "classes": classes, "epochs": epochs,
                      "reorder_ms": round(reorder_ms, 3), "perm_ms": round(perm_ms, 3),
@@ -223,6 +263,10 @@ def main(argv=None) -> int:
     ap.add_argument("--fused-scaling", action="store_true",
                     help="apply d^-1/2 on both sides inside the SpMM (spmm_csr_scaled) "
                     "instead of as two elementwise products around it")
+    ap.add_argument("--embed", action="store_true", help="learn the node vectors")
+    ap.add_argument("--layer-norm", action="store_true", help="a layer norm on the hidden layer")
+    ap.add_argument("--muon", action="store_true",
+                    help="update the weight matrices along their orthogonalised momentum")
     args = ap.parse_args(argv)
 
     import torch
@@ -241,7 +285,8 @@ def main(argv=None) -> int:
     for row in run(ptr_h, ind_h, features=args.features, hidden=args.hidden,
                    classes=args.classes, epochs=args.epochs,
                    orders=tuple(args.orders.split(",")), seed=args.seed,
-                   fused=args.fused_scaling):
+                   fused=args.fused_scaling, embed=args.embed, norm=args.layer_norm,
+                   muon=args.muon):
         print(json.dumps(row), flush=True)
     return 0
 

@@ -38,6 +38,45 @@ __device__ __forceinline__ void store_f32(T *p, const float (&in)[VEC]) {
   *reinterpret_cast<Pack<T, VEC> *>(p) = q;
 }
 
+// The same for rows of any length and alignment: whole vectors at an address
+// aligned to elements only (the memory pipe takes them), and the end of the
+// row, whose length from p on is `left`, by elements.
+template <typename T, int VEC> struct __attribute__((packed, aligned(sizeof(T)))) LoosePack {
+  T v[VEC];
+};
+
+template <bool LOOSE, int VEC, typename T>
+__device__ __forceinline__ Pack<T, VEC> fetch(const T *p, int64_t left) {
+  Pack<T, VEC> q;
+  if constexpr (!LOOSE) {
+    q = *reinterpret_cast<const Pack<T, VEC> *>(p);
+  } else if (left >= VEC) {
+    const LoosePack<T, VEC> r = *reinterpret_cast<const LoosePack<T, VEC> *>(p);
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) q.v[i] = r.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) q.v[i] = i < left ? p[i] : static_cast<T>(0.0f);
+  }
+  return q;
+}
+
+template <bool LOOSE, int VEC, typename T>
+__device__ __forceinline__ void put(T *p, int64_t left, const float (&in)[VEC]) {
+  if constexpr (!LOOSE) {
+    store_f32<VEC>(p, in);
+  } else if (left >= VEC) {
+    LoosePack<T, VEC> q;
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) q.v[i] = static_cast<T>(in[i]);
+    *reinterpret_cast<LoosePack<T, VEC> *>(p) = q;
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+      if (i < left) p[i] = static_cast<T>(in[i]);
+  }
+}
+
 // The same past the caches, for output too large to be found there by its
 // reader: it leaves them to what the kernel still reads.
 template <int VEC, typename T>

@@ -75,7 +75,7 @@ template <int L, int N> struct RowSum {
 };
 
 // A lane's part of weight or bias, or `value` where there is none.
-template <int VEC, int L, int C>
+template <bool LOOSE, int VEC, int L, int C>
 __device__ __forceinline__ void load_vector(const void *p, int type, int64_t dim, float value,
                                             int lane, float (&out)[C][VEC]) {
 #pragma unroll
@@ -88,12 +88,15 @@ __device__ __forceinline__ void load_vector(const void *p, int type, int64_t dim
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * L + lane) * VEC;
-      if (col < dim) load_f32<VEC>(w + col, out[c]);
+      if (col >= dim) continue;
+      const auto q = fetch<LOOSE, VEC>(w + col, dim - col);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) out[c][i] = static_cast<float>(q.v[i]);
     }
   });
 }
 
-template <typename T, int VEC, int L, int C>
+template <typename T, bool LOOSE, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
   constexpr int kGroups = norm_block(L) / L;
   __shared__ float shared[2][1][norm_block(L) / kWave];
@@ -102,21 +105,23 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
   const float dim = static_cast<float>(a.dim);
 
   float w[C][VEC], b[C][VEC];
-  load_vector<VEC, L>(a.weight, a.weight_type, a.dim, 1.0f, lane, w);
-  load_vector<VEC, L>(a.bias, a.weight_type, a.dim, 0.0f, lane, b);
+  load_vector<LOOSE, VEC, L>(a.weight, a.weight_type, a.dim, 1.0f, lane, w);
+  load_vector<LOOSE, VEC, L>(a.bias, a.weight_type, a.dim, 0.0f, lane, b);
 
   for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < a.rows;
        first += static_cast<int64_t>(gridDim.x) * kGroups) {
     const int64_t row = first + group;
     const bool live = row < a.rows;
-    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
+    const T *const x = static_cast<const T *>(a.x) + row * a.x_stride;
     float v[C][VEC];
     float s[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * L + lane) * VEC;
       if (live && col < a.dim) {
-        load_f32<VEC>(x + col, v[c]);
+        const Pack<T, VEC> q = fetch<LOOSE, VEC>(x + col, a.dim - col);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) v[c][i] = static_cast<float>(q.v[i]);
       } else {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) v[c][i] = 0.0f;
@@ -132,11 +137,10 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
     s[0] = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const bool in = (c * L + lane) * VEC < a.dim;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         v[c][i] -= mean;
-        s[0] += in ? v[c][i] * v[c][i] : 0.0f;
+        s[0] += (c * L + lane) * VEC + (LOOSE ? i : 0) < a.dim ? v[c][i] * v[c][i] : 0.0f;
       }
     }
     row_sum(s);
@@ -148,7 +152,7 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
       const int col = (c * L + lane) * VEC;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) v[c][i] = v[c][i] * rstd * w[c][i] + b[c][i];
-      if (col < a.dim) store_f32<VEC>(y + col, v[c]);
+      if (col < a.dim) put<LOOSE, VEC>(y + col, a.dim - col, v[c]);
     }
     if (lane == 0) {
       a.mean[row] = mean;
@@ -192,8 +196,9 @@ template <typename T> __global__ void __launch_bounds__(1024) layer_norm_long_ke
 // dx, and the workgroup's sums of dy h and dy by column: each lane keeps its
 // columns' sums in registers over all the rows that it takes, the groups of a
 // workgroup are added up at the end and the workgroup writes one row of
-// partial sums.  No atomics: the order of every sum is fixed by the grid.
-template <typename T, int VEC, int L, int C>
+// partial sums.  No atomics: the order of every sum is fixed by the grid.  The
+// next row is on its way while a row is worked on, where registers allow.
+template <typename T, bool LOOSE, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGradArgs a) {
   constexpr int kGroups = norm_block(L) / L;
   constexpr int kSpan = L * C * VEC; // columns that a group holds
@@ -207,33 +212,79 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
   const float dim = static_cast<float>(a.dim);
 
   float w[C][VEC], dw[C][VEC] = {}, db[C][VEC] = {};
-  load_vector<VEC, L>(a.weight, a.weight_type, a.dim, 1.0f, lane, w);
+  load_vector<LOOSE, VEC, L>(a.weight, a.weight_type, a.dim, 1.0f, lane, w);
 
-  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < a.rows;
-       first += static_cast<int64_t>(gridDim.x) * kGroups) {
-    const int64_t row = first + group;
+  Pack<T, VEC> next_x[C], next_dy[C];
+  float next_mean = 0.0f, next_rstd = 0.0f;
+  auto fetch_next = [&](int64_t row) {
     const bool live = row < a.rows;
-    const T *x = static_cast<const T *>(a.x) + row * a.x_stride;
-    const T *dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
-    const float mean = live ? a.mean[row] : 0.0f, rstd = live ? a.rstd[row] : 0.0f;
+    const T *const x = static_cast<const T *>(a.x) + row * a.x_stride;
+    const T *const dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
+    auto part = [&](const T *p, int c, Pack<T, VEC> &to) {
+      const int col = (c * L + lane) * VEC;
+      if (live && col < a.dim) {
+        to = fetch<LOOSE, VEC>(p + col, a.dim - col);
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) to.v[i] = static_cast<T>(0.0f);
+      }
+    };
+    auto stats = [&]() {
+      next_mean = live ? a.mean[row] : 0.0f;
+      next_rstd = live ? a.rstd[row] : 0.0f;
+    };
+    // The order of the loads.  16-bit rows at whole accesses, and any at 8 bytes
+    // an access, are faster alternating between x and dy (100 million elements
+    // in rows of 300: 133 us, 196 one row after the other; of 64: 120, 128);
+    // wider rows of floats that end inside a line one after the other (in rows
+    // of 100: 241 us, 332 alternating), and so rows that are fetched ahead.
+    if constexpr ((sizeof(T) == 2 && !LOOSE && L < 512) || VEC * sizeof(T) == 8) {
+      stats();
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int col = (c * L + lane) * VEC;
+        if (live && col < a.dim) { // one branch for both loads
+          next_x[c] = fetch<LOOSE, VEC>(x + col, a.dim - col);
+          next_dy[c] = fetch<LOOSE, VEC>(dy + col, a.dim - col);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) next_x[c].v[i] = next_dy[c].v[i] = static_cast<T>(0.0f);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < C; ++c) part(x, c, next_x[c]);
+#pragma unroll
+      for (int c = 0; c < C; ++c) part(dy, c, next_dy[c]);
+      stats();
+    }
+  };
+  // Measured with rows of 8192 16-bit elements: 144 us for 100 million, 176
+  // without; shorter rows have more waves to hide behind and lose 6 to 12 %,
+  // and 32 elements per lane would spill.
+  constexpr bool kAhead = L == 512 && C * VEC <= 16;
+  const int64_t stride = static_cast<int64_t>(gridDim.x) * kGroups;
+  if (kAhead) fetch_next(static_cast<int64_t>(blockIdx.x) * kGroups + group);
+  for (int64_t first = static_cast<int64_t>(blockIdx.x) * kGroups; first < a.rows; first += stride) {
+    const int64_t row = first + group;
+    if (!kAhead) fetch_next(row);
+    const float mean = next_mean, rstd = next_rstd;
     float h[C][VEC], g[C][VEC];
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int col = (c * L + lane) * VEC;
-      if (live && col < a.dim) {
-        load_f32<VEC>(x + col, h[c]);
-        load_f32<VEC>(dy + col, g[c]);
-      } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) h[c][i] = mean, g[c][i] = 0.0f;
+      for (int i = 0; i < VEC; ++i) {
+        h[c][i] = static_cast<float>(next_x[c].v[i]);
+        g[c][i] = static_cast<float>(next_dy[c].v[i]);
       }
     }
+    if (kAhead) fetch_next(row + stride);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        h[c][i] = (h[c][i] - mean) * rstd;
+        h[c][i] = (h[c][i] - mean) * rstd; // past the row's end meets a dy of 0 only
         dw[c][i] += g[c][i] * h[c][i];
         db[c][i] += g[c][i];
         g[c][i] *= w[c][i];
@@ -243,14 +294,14 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
     }
     row_sum(s);
     const float m1 = s[0] / dim, m2 = s[1] / dim;
-    if (!live) continue;
+    if (row >= a.rows) continue;
     T *dx = static_cast<T *>(a.dx) + row * a.dx_stride;
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * L + lane) * VEC;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) g[c][i] = (g[c][i] - m1 - h[c][i] * m2) * rstd;
-      if (col < a.dim) store_f32<VEC>(dx + col, g[c]);
+      if (col < a.dim) put<LOOSE, VEC>(dx + col, a.dim - col, g[c]);
     }
   }
 
@@ -369,72 +420,84 @@ constexpr int64_t kMaxNormBlocks = 256 * 8;
 constexpr int64_t kNormMostDim = 512 * 64;     // forward, in registers
 constexpr int64_t kNormGradMostDim = 512 * 32; // backward: dw and db are held too
 
-template <typename T, int VEC, int L, int E> int32_t run_norm(const NormArgs &a, void *stream) {
-  constexpr int kGroups = norm_block(L) / L;
-  const int64_t blocks = std::min(ceil_div64(a.rows, kGroups), kMaxNormBlocks);
-  return launch(layer_norm_kernel<T, VEC, L, E / VEC>, dim3(blocks), dim3(norm_block(L)), stream,
-                a);
+// f with a row's lanes and the elements of each, as types: the smallest group
+// that holds the row at 8 elements per lane up to 64, at 16 past them, and
+// past 8192 a workgroup of 512 with as many as `most` elements need.
+template <int N> using Const = std::integral_constant<int, N>;
+template <int MOST, typename F> int32_t with_lanes(int64_t dim, F &&f) {
+  if (dim <= 16) return f(Const<2>{}, Const<8>{});
+  if (dim <= 32) return f(Const<4>{}, Const<8>{});
+  if (dim <= 64) return f(Const<8>{}, Const<8>{});
+  if (dim <= 128) return f(Const<8>{}, Const<16>{});
+  if (dim <= 256) return f(Const<16>{}, Const<16>{});
+  if (dim <= 512) return f(Const<32>{}, Const<16>{});
+  if (dim <= 1024) return f(Const<64>{}, Const<16>{});
+  if (dim <= 2048) return f(Const<128>{}, Const<16>{});
+  if (dim <= 4096) return f(Const<256>{}, Const<16>{});
+  if (dim <= 8192) return f(Const<512>{}, Const<16>{});
+  if (MOST == 32 || dim <= 16384) return f(Const<512>{}, Const<32>{});
+  return f(Const<512>{}, Const<MOST>{});
 }
 
-template <typename T, int VEC> int32_t pick_norm(const NormArgs &a, void *stream) {
-  const int64_t d = a.dim;
-  if constexpr (VEC == 1) { // single elements: whole waves on a row, for contiguous accesses
-    if (d <= 32) return run_norm<T, 1, 32, 1>(a, stream);
-    if (d <= 128) return run_norm<T, 1, 64, 2>(a, stream);
-    if (d <= 256) return run_norm<T, 1, 64, 4>(a, stream);
-    if (d <= 512) return run_norm<T, 1, 64, 8>(a, stream);
-  } else {
-    if (d <= 64) return run_norm<T, VEC, 8, 8>(a, stream);
-    if (d <= 128) return run_norm<T, VEC, 8, 16>(a, stream);
-    if (d <= 256) return run_norm<T, VEC, 16, 16>(a, stream);
-    if (d <= 512) return run_norm<T, VEC, 32, 16>(a, stream);
-  }
-  if (d <= 1024) return run_norm<T, VEC, 64, 16>(a, stream);
-  if (d <= 2048) return run_norm<T, VEC, 128, 16>(a, stream);
-  if (d <= 4096) return run_norm<T, VEC, 256, 16>(a, stream);
-  if (d <= 8192) return run_norm<T, VEC, 512, 16>(a, stream);
-  if (d <= 16384) return run_norm<T, VEC, 512, 32>(a, stream);
-  return run_norm<T, VEC, 512, 64>(a, stream);
+// Lanes and rows at a time of a workgroup of the gradient, by the same rule.
+int64_t norm_groups(int64_t dim) {
+  int lanes = dim <= 16 ? 2 : dim <= 32 ? 4 : 8;
+  while (lanes < 512 && lanes * 16 < dim) lanes *= 2;
+  return norm_block(lanes) / lanes;
 }
 
-template <typename T, int VEC, int L, int E>
-int32_t run_norm_grad(const NormGradArgs &a, int64_t blocks, void *stream) {
-  return launch(layer_norm_grad_kernel<T, VEC, L, E / VEC>, dim3(blocks), dim3(norm_block(L)),
-                stream, a);
+// The same for accesses of a few bytes: whole waves on a row, for contiguous
+// accesses.
+template <int MOST, typename F> int32_t with_waves(int64_t dim, F &&f) {
+  if (dim <= 128) return f(Const<64>{}, Const<2>{});
+  if (dim <= 256) return f(Const<64>{}, Const<4>{});
+  if (dim <= 512) return f(Const<64>{}, Const<8>{});
+  return with_lanes<MOST>(dim, f);
 }
 
-template <typename T, int VEC>
-int32_t pick_norm_grad(const NormGradArgs &a, int64_t blocks, void *stream) {
-  const int64_t d = a.dim;
-  if constexpr (VEC == 1) {
-    if (d <= 32) return run_norm_grad<T, 1, 32, 1>(a, blocks, stream);
-    if (d <= 128) return run_norm_grad<T, 1, 64, 2>(a, blocks, stream);
-    if (d <= 256) return run_norm_grad<T, 1, 64, 4>(a, blocks, stream);
-    if (d <= 512) return run_norm_grad<T, 1, 64, 8>(a, blocks, stream);
-  } else {
-    if (d <= 64) return run_norm_grad<T, VEC, 8, 8>(a, blocks, stream);
-    if (d <= 128) return run_norm_grad<T, VEC, 8, 16>(a, blocks, stream);
-    if (d <= 256) return run_norm_grad<T, VEC, 16, 16>(a, blocks, stream);
-    if (d <= 512) return run_norm_grad<T, VEC, 32, 16>(a, blocks, stream);
-  }
-  if (d <= 1024) return run_norm_grad<T, VEC, 64, 16>(a, blocks, stream);
-  if (d <= 2048) return run_norm_grad<T, VEC, 128, 16>(a, blocks, stream);
-  if (d <= 4096) return run_norm_grad<T, VEC, 256, 16>(a, blocks, stream);
-  if (d <= 8192) return run_norm_grad<T, VEC, 512, 16>(a, blocks, stream);
-  return run_norm_grad<T, VEC, 512, 32>(a, blocks, stream);
+template <typename T, bool LOOSE, int VEC> int32_t norm_lanes(const NormArgs &a, void *stream) {
+  auto go = [&](auto lanes, auto elements) {
+    constexpr int L = decltype(lanes)::value;
+    if constexpr (decltype(elements)::value < VEC) {
+      return static_cast<int32_t>(SPORDER_BAD_ARGUMENT); // not reached
+    } else {
+      const int64_t blocks = std::min(ceil_div64(a.rows, norm_block(L) / L), kMaxNormBlocks);
+      return launch(layer_norm_kernel<T, LOOSE, VEC, L, decltype(elements)::value / VEC>,
+                    dim3(blocks), dim3(norm_block(L)), stream, a);
+    }
+  };
+  if constexpr (VEC >= 4)
+    return with_lanes<64>(a.dim, go);
+  else
+    return with_waves<64>(a.dim, go);
+}
+
+template <typename T, bool LOOSE, int VEC>
+int32_t norm_grad_lanes(const NormGradArgs &a, int64_t blocks, void *stream) {
+  auto go = [&](auto lanes, auto elements) {
+    constexpr int L = decltype(lanes)::value;
+    return launch(layer_norm_grad_kernel<T, LOOSE, VEC, L, decltype(elements)::value / VEC>,
+                  dim3(blocks), dim3(norm_block(L)), stream, a);
+  };
+  if constexpr (VEC >= 4)
+    return with_lanes<32>(a.dim, go);
+  else
+    return with_waves<32>(a.dim, go);
 }
 
 template <typename T> int32_t norm_typed(const NormArgs &a, void *stream) {
   if (a.dim > kNormMostDim)
     return launch(layer_norm_long_kernel<T>, dim3(std::min(a.rows, kMaxNormBlocks)), dim3(1024),
                   stream, a);
-  const int vec = row_vec(sizeof(T), a.dim, {a.x_stride, a.y_stride},
-                          {a.x, a.y, a.weight, a.bias});
+  const int vec = row_vec(sizeof(T), a.dim, {a.x_stride, a.y_stride}, {a.x, a.y, a.weight, a.bias});
   if constexpr (sizeof(T) == 2) {
-    if (vec == 8) return pick_norm<T, 8>(a, stream);
+    if (vec == 8) return norm_lanes<T, false, 8>(a, stream);
+    if (vec == 4) return norm_lanes<T, false, 4>(a, stream);
+    return norm_lanes<T, true, 8>(a, stream);
+  } else {
+    if (vec == 4) return norm_lanes<T, false, 4>(a, stream);
+    return a.dim <= 64 ? norm_lanes<T, true, 4>(a, stream) : norm_lanes<T, false, 1>(a, stream);
   }
-  if (vec == 4) return pick_norm<T, 4>(a, stream);
-  return pick_norm<T, 1>(a, stream);
 }
 
 template <typename T>
@@ -444,21 +507,23 @@ int32_t norm_grad_typed(const NormGradArgs &a, int64_t blocks, void *stream) {
   const int vec = row_vec(sizeof(T), a.dim, {a.x_stride, a.dy_stride, a.dx_stride},
                           {a.x, a.dy, a.dx, a.weight});
   if constexpr (sizeof(T) == 2) {
-    if (vec == 8) return pick_norm_grad<T, 8>(a, blocks, stream);
+    if (vec == 8) return norm_grad_lanes<T, false, 8>(a, blocks, stream);
+    if (vec == 4) return norm_grad_lanes<T, false, 4>(a, blocks, stream);
+    return a.dim <= 4096 ? norm_grad_lanes<T, true, 4>(a, blocks, stream)
+                         : norm_grad_lanes<T, true, 8>(a, blocks, stream);
+  } else {
+    if (vec == 4) return norm_grad_lanes<T, false, 4>(a, blocks, stream);
+    return a.dim <= 64 ? norm_grad_lanes<T, true, 4>(a, blocks, stream)
+                       : norm_grad_lanes<T, false, 1>(a, blocks, stream);
   }
-  if (vec == 4) return pick_norm_grad<T, 4>(a, blocks, stream);
-  return pick_norm_grad<T, 1>(a, blocks, stream);
 }
 
 // Workgroups of the gradient, each with a partial row of 2 dim floats: enough
 // to fill the card, and few enough that the partial rows stay small beside
 // the rows themselves (at least 8 rows per workgroup).
 int64_t norm_grad_blocks(int64_t rows, int64_t dim) {
-  int lanes = 8;
-  while (lanes < 512 && lanes * 16 < dim) lanes *= 2;
-  const int64_t groups = norm_block(lanes) / lanes;
-  const int64_t most = std::max<int64_t>(256, kMaxNormBlocks * 256 / norm_block(lanes) / 2);
-  return std::max<int64_t>(1, std::min(ceil_div64(rows, 8 * groups), most));
+  const int64_t most = dim > 4096 ? 512 : 1024;
+  return std::max<int64_t>(1, std::min(ceil_div64(rows, 8 * norm_groups(dim)), most));
 }
 
 } // namespace

@@ -9,14 +9,14 @@
 // the result, changes from run to run and a common token serialises them, so
 // the tokens are sorted instead:
 //
-//   1. each tile of 4096 tokens is sorted in LDS (stable), and the table's
-//      rows, cut into spans, find where their tokens begin in it.  16 to 64
-//      neighbours of one token in that order (a common token: a hub) become
-//      one entry,
-//   2. whose sum a workgroup forms;
-//   3. a workgroup per span gathers its entries from every tile, in the
-//      tiles' order, sorts them by row in LDS and writes them out by row;
-//   4. the table is written front to back, every lane a few vectors of a row
+//   1. each tile of 1024 or 4096 tokens is sorted in LDS (stable), and the
+//      table's rows, cut into spans, find where their tokens begin in it.  16
+//      to 64 neighbours of one token in that order (a common token: a hub)
+//      become one entry,
+//   2. whose sum a workgroup forms; in the same launch a workgroup per span
+//      gathers its entries from every tile, in the tiles' order, sorts them by
+//      row in LDS and writes them out by row;
+//   3. the table is written front to back, every lane a few vectors of a row
 //      and their sum (this is where the bytes are); rows that still have many
 //      entries are shared by a workgroup for each slice of their columns, in
 //      the launch's first workgroups.
@@ -99,18 +99,24 @@ template <typename T, int VEC> __global__ void __launch_bounds__(256) embedding_
 
 // ---- gradient ------------------------------------------------------------------
 
-constexpr int kTile = 4096;       // tokens sorted by one workgroup
-constexpr int kTileBlock = 1024;
-constexpr int kTileWaves = kTileBlock / kWave;
-constexpr int kTileRounds = kTile / kTileBlock;
+// Tokens sorted by one workgroup: small tiles sort in half the time, but every
+// span has to ask each of them.
+constexpr int kSmallTile = 1024, kLargeTile = 4096;
+constexpr int kMostSmallTiles = 64;
+constexpr int kTileRounds = 4;    // tokens per thread of a tile
 constexpr int kChunk = kWave;     // sorted neighbours looked at together
-constexpr int kTileChunks = kTile / kChunk;
 constexpr int kRun = 16;          // equal tokens of a chunk that become one entry
-constexpr int kChunkRuns = kChunk / kRun;
-constexpr int kTileRuns = kTileChunks * kChunkRuns;
 constexpr uint32_t kSummed = 0x80000000u; // an entry that is a run's sum
 constexpr int kSpanMost = 256;    // table rows per span
-constexpr int kListMost = 2048;   // a span's entries that fit the list in LDS
+constexpr int kListMost = 2048;   // a span's entries in LDS at a time
+// Few tokens need no tiles: every span looks through them by itself, in one
+// launch, or a workgroup per token does where the table is large.  They are few
+// by their number, by what the spans read of them, and by their elements, which
+// one workgroup may have to add up alone (2 MB at most, some 25 us).
+constexpr int kFewMost = 8192;
+constexpr int64_t kFewReads = int64_t(1) << 24, kFewElements = int64_t(1) << 19;
+constexpr int64_t kFewBlocks = 1024;
+constexpr int64_t kLarge = int64_t(1) << 24; // elements of a large table
 constexpr int kSparse = 4;        // turns' worth of rows per workgroup, at most
 constexpr int kAlone = 8;         // entries of a row that one lane adds up
 constexpr int kHubLists = 16;
@@ -123,19 +129,20 @@ struct GradArgs {
   int64_t count, rows, dim, grad_stride, out_stride, padding;
   float scale;
   int wide;
-  bool stream;
+  bool stream, large;
   int key_bits;
   int row_block; // table rows per workgroup of the last launch
   int span;      // and of the one before it
   int64_t spans; // ceil(rows / span)
+  int tile;      // tokens per tile
   int64_t tiles;
-  uint32_t *keys;      // [tiles][kTile] the tiles' entries: row,
+  uint32_t *keys;      // [tiles][tile] the tiles' entries: row,
   uint32_t *sources;   // and token index, or run index | kSummed
-  uint16_t *order;     // [tiles][kTile] the sorted order within the tile
-  uint32_t *runs;      // [tiles][kTileRuns] first place in the tile << 8 | length
+  uint16_t *order;     // [tiles][tile] the sorted order within the tile
+  uint32_t *runs;      // [tiles][tile / kRun] first place in the tile << 8 | length
   int32_t *run_count;  // [tiles]
   uint16_t *starts;    // [tiles][spans + 1] first entry of each span
-  float *sums;         // [tiles * kTileRuns][dim]
+  float *sums;         // [tiles * tile / kRun][dim]
   uint32_t *list;      // [count] the entries' sources by row, sums first
   int32_t *row_start;  // [rows + 1] first entry in the list
   // Rows of more than kAlone entries: kHubLists lists, each its length and
@@ -166,18 +173,22 @@ __device__ __forceinline__ void token_rows(const GradArgs &a, int64_t first, int
 
 // Peers of this lane: the lanes whose `bits` low bits of `digit` equal its own.
 __device__ __forceinline__ uint64_t match_lanes(uint32_t digit, int bits) {
-  uint64_t peers = ~uint64_t(0);
+  uint32_t low = ~0u, high = ~0u;
   for (int b = 0; b < bits; ++b) {
-    const bool bit = (digit >> b) & 1;
-    const uint64_t m = ballot(bit);
-    peers &= bit ? m : ~m;
+    const uint32_t set = static_cast<uint32_t>(static_cast<int32_t>(digit << (31 - b)) >> 31);
+    const uint64_t m = ballot(set != 0); // lanes with the bit; peers agree with this lane's
+    low &= ~(static_cast<uint32_t>(m) ^ set);
+    high &= ~(static_cast<uint32_t>(m >> 32) ^ set);
   }
-  return peers;
+  return static_cast<uint64_t>(high) << 32 | low;
 }
 
 // Sorts one tile by row (LSD, 8 bits per pass; each wave ranks its own 256
 // consecutive items) and writes its entries and the spans' starts.
-__global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) {
+template <int TILE>
+__global__ void __launch_bounds__(TILE / kTileRounds) embedding_tile_kernel(GradArgs a) {
+  constexpr int kTile = TILE, kTileBlock = TILE / kTileRounds, kTileWaves = kTileBlock / kWave;
+  constexpr int kTileChunks = kTile / kChunk, kTileRuns = kTile / kRun;
   constexpr int kDigits = 256;
   __shared__ uint32_t key[2][kTile];
   __shared__ uint16_t idx[2][kTile];
@@ -268,9 +279,9 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
     a.order[base + chunk * kChunk + lane] = idx[from][chunk * kChunk + lane];
   }
   __syncthreads();
-  // Entries and runs before each chunk, in the halves of a word; kTileChunks =
-  // kWave, so every wave holds all of them.
-  const int mine = chunk_entries[lane];
+  // Entries and runs before each chunk, in the halves of a word: every wave
+  // holds all of the chunks, at most one per lane.
+  const int mine = lane < kTileChunks ? chunk_entries[lane] : 0;
   const int place = wave_incl_scan(mine) - mine;
   const int all = wave_sum(mine), entries = all & 0xffff;
   if (tid == 0) a.run_count[tile] = all >> 16;
@@ -319,37 +330,40 @@ __global__ void __launch_bounds__(kTileBlock) embedding_tile_kernel(GradArgs a) 
   }
 }
 
-// The sums of the runs: a workgroup per run and slice of L VEC columns, L lanes
-// per token, so that all the loads of a run are under way at once.  A tile's
-// runs are dealt to kRunBlocks workgroups.
-constexpr int kRunBlocks = 32;
+// The sum of run blocks: `block` of kRunBlocks(tile) for each tile and slice
+// of L VEC columns, L lanes per token, 32 / VEC tokens of a lane under way at
+// once.
+constexpr int run_blocks(int tile) { return tile / 128; }
 
 template <typename T, int VEC, int L>
-__global__ void __launch_bounds__(256) embedding_run_kernel(GradArgs a) {
+__device__ __forceinline__ void sum_runs(const GradArgs &a, float (&joined)[4][L * VEC], int64_t block) {
   constexpr int kGroups = 256 / L, kWaves = 256 / kWave;
-  constexpr int kEach = kChunk / kGroups > 0 ? kChunk / kGroups : 1;
-  __shared__ float joined[kWaves][L * VEC];
-  const int64_t tile = blockIdx.x / kRunBlocks;
-  const int runs = a.run_count[tile];
+  constexpr int kMost = kChunk / kGroups, kEach = kMost > 32 / VEC ? 32 / VEC : kMost > 0 ? kMost : 1;
+  const int per_tile = run_blocks(a.tile), slices = static_cast<int>(ceil_div64(a.dim, L * VEC));
+  const int64_t tile = block / (per_tile * slices);
+  const int within = static_cast<int>(block % (per_tile * slices));
+  const int runs = a.run_count[tile], tile_runs = a.tile / kRun;
   const int group = threadIdx.x / L, lane = threadIdx.x % L, wave = threadIdx.x / kWave;
-  const int64_t c = (static_cast<int64_t>(blockIdx.y) * L + lane) * VEC;
-  const T *const grad = static_cast<const T *>(a.grad) + tile * kTile * a.grad_stride + c;
-  for (int run = blockIdx.x % kRunBlocks; run < runs; run += kRunBlocks) {
-    const uint32_t what = a.runs[tile * kTileRuns + run];
+  const int64_t c = (static_cast<int64_t>(within / per_tile) * L + lane) * VEC;
+  const T *const grad = static_cast<const T *>(a.grad) + tile * a.tile * a.grad_stride + c;
+  for (int run = within % per_tile; run < runs; run += per_tile) {
+    const uint32_t what = a.runs[tile * tile_runs + run];
     const int n = what & 0xff;
-    const uint16_t *const order = a.order + tile * kTile + (what >> 8);
-    int64_t at[kEach];
-#pragma unroll
-    for (int d = 0; d < kEach; ++d) at[d] = order[min(d * kGroups + group, n - 1)] * a.grad_stride;
-    float v[kEach][VEC] = {};
-#pragma unroll
-    for (int d = 0; d < kEach; ++d)
-      if (c < a.dim && d * kGroups + group < n) load_f32<VEC>(grad + at[d], v[d]);
+    const uint16_t *const order = a.order + tile * a.tile + (what >> 8);
     float acc[VEC] = {};
+    for (int i0 = group; i0 < n; i0 += kEach * kGroups) {
+      int64_t at[kEach];
 #pragma unroll
-    for (int d = 0; d < kEach; ++d) {
+      for (int d = 0; d < kEach; ++d) at[d] = order[min(i0 + d * kGroups, n - 1)] * a.grad_stride;
+      float v[kEach][VEC] = {};
 #pragma unroll
-      for (int k = 0; k < VEC; ++k) acc[k] += v[d][k];
+      for (int d = 0; d < kEach; ++d)
+        if (c < a.dim && i0 + d * kGroups < n) load_f32<VEC>(grad + at[d], v[d]);
+#pragma unroll
+      for (int d = 0; d < kEach; ++d) {
+#pragma unroll
+        for (int k = 0; k < VEC; ++k) acc[k] += v[d][k];
+      }
     }
     __syncthreads(); // the run before has been read
 #pragma unroll
@@ -366,17 +380,20 @@ __global__ void __launch_bounds__(256) embedding_run_kernel(GradArgs a) {
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) acc[k] += joined[w][lane * VEC + k];
       }
-      store_f32<VEC>(a.sums + (tile * kTileRuns + run) * a.dim + c, acc);
+      store_f32<VEC>(a.sums + (tile * tile_runs + run) * a.dim + c, acc);
     }
   }
 }
 
 // A span's entries in LDS.
 constexpr int kBins = 2 * kSpanMost; // sums of row r, tokens of row r
+__device__ __forceinline__ int entry_bin(int row, uint32_t what) {
+  return 2 * row + ((what & kSummed) == 0);
+}
 constexpr int kSpanWaves = 256 / kWave;
-struct SpanList {
-  uint32_t source[kListMost];
-  uint16_t local[kListMost]; // their bins
+template <typename SOURCE, int MOST> struct SpanList {
+  SOURCE source[MOST];
+  uint16_t local[MOST]; // their bins
   int first[kBins + 1];
   int next[kBins];
   int wave_total[kSpanWaves];
@@ -399,9 +416,6 @@ struct SpanList {
   }
 
   __device__ __forceinline__ void clear() { next[threadIdx.x] = next[threadIdx.x + 256] = 0; }
-  static __device__ __forceinline__ int bin(int row, uint32_t what) {
-    return 2 * row + ((what & kSummed) == 0);
-  }
 
   // From counts in next to first places, in next and first.
   __device__ __forceinline__ void open() {
@@ -429,7 +443,7 @@ struct SpanList {
         const int to = next[b] + __popcll(peers & below);
         wave_lds_order();
         if (live) {
-          put(to, source[i0 + lane]);
+          put(to, static_cast<uint32_t>(source[i0 + lane]));
           if ((peers & below) == 0) next[b] = to + __popcll(peers);
         }
         wave_lds_order();
@@ -439,13 +453,23 @@ struct SpanList {
   }
 };
 
-// Step 3.
-__global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
-  __shared__ SpanList list;
+// Step 2: `run_grid` workgroups for the runs, then one per span.
+template <typename T, int VEC, int L>
+__global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a, int64_t run_grid) {
+  __shared__ union {
+    SpanList<uint32_t, kListMost> list;
+    float joined[4][L * VEC];
+  } shared;
+  if (blockIdx.x < run_grid) {
+    sum_runs<T, VEC, L>(a, shared.joined, blockIdx.x);
+    return;
+  }
+  auto &list = shared.list;
   const int tid = threadIdx.x;
-  const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.span;
+  const int64_t span = blockIdx.x - run_grid;
+  const int64_t row0 = span * a.span;
   const int rows = static_cast<int>(min(static_cast<int64_t>(a.span), a.rows - row0));
-  const uint16_t *const starts = a.starts + blockIdx.x;
+  const uint16_t *const starts = a.starts + span;
 
   // f(tile, first entry in it, number, their place in the tiles' order) for
   // every tile, one per thread; their total and the entries of lower rows.
@@ -461,19 +485,19 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
       }
       before += lo;
       const int at = total + list.prefix(n, sum);
-      f(tile * kTile + lo, n, at);
+      f(tile * a.tile + lo, n, at);
       total += sum;
     }
   };
-  auto entry_bin = [&](int64_t e) {
-    return SpanList::bin(static_cast<int>(a.keys[e] - row0), a.sources[e]);
+  auto bin_at = [&](int64_t e) {
+    return entry_bin(static_cast<int>(a.keys[e] - row0), a.sources[e]);
   };
   // The entries at places [from, from + kListMost) to the list.
   auto gather = [&](int from, bool count) {
     each_tile([&](int64_t e, int n, int at) {
       const int lo = max(from - at, 0), hi = min(n, from + kListMost - at);
       for (int i = lo; i < hi; ++i) {
-        const int b = entry_bin(e + i);
+        const int b = bin_at(e + i);
         list.source[at + i - from] = a.sources[e + i];
         list.local[at + i - from] = static_cast<uint16_t>(b);
         if (count) atomicAdd(&list.next[b], 1);
@@ -484,7 +508,7 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
   gather(0, true);
   int base;
   list.prefix(before, base);
-  if (blockIdx.x == gridDim.x - 1 && tid == 0) a.row_start[a.rows] = base + total;
+  if (span == a.spans - 1 && tid == 0) a.row_start[a.rows] = base + total;
   if (total == 0) {
     if (tid < rows) a.row_start[row0 + tid] = base;
     return;
@@ -492,7 +516,7 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
   const int all = total;
   if (all > kListMost) { // the rest is counted where it lies
     each_tile([&](int64_t e, int n, int at) {
-      for (int i = max(kListMost - at, 0); i < n; ++i) atomicAdd(&list.next[entry_bin(e + i)], 1);
+      for (int i = max(kListMost - at, 0); i < n; ++i) atomicAdd(&list.next[bin_at(e + i)], 1);
     });
   }
   list.open();
@@ -500,7 +524,7 @@ __global__ void __launch_bounds__(256) embedding_span_kernel(GradArgs a) {
     const int at = list.first[2 * tid], n = list.first[2 * tid + 2] - at;
     a.row_start[row0 + tid] = base + at;
     // Their order changes from run to run; each row's sum does not depend on it.
-    int32_t *const hubs = a.hubs + blockIdx.x % kHubLists * a.hub_stride;
+    int32_t *const hubs = a.hubs + span % kHubLists * a.hub_stride;
     if (n > kAlone) hubs[1 + atomicAdd(hubs, 1)] = static_cast<int32_t>(row0 + tid);
   }
   for (int from = 0; from < all; from += kListMost) {
@@ -584,12 +608,12 @@ struct BusyRows {
 };
 
 // Rows [row0, row0 + rows), of which r's entries are [first(r), first(r + 1)).
-// Empty rows are written first, front to back.  The vectors of the rows with
-// few entries then lie in a row before the workgroup's lanes, kItems of them 256
+// Empty rows are written first, front to back (with ZERO).  The vectors of the
+// rows with few entries then lie in a row before the workgroup's lanes, kItems of them 256
 // apart per lane and turn, so that stores fill whole lines and every lane has
 // kItems loads under way (with the empty rows among them, most lanes would
 // have none); the entries after these are fetched meanwhile.
-template <typename T, typename O, int VEC, typename FIRST, typename ENTRY>
+template <typename T, typename O, int VEC, bool ZERO, typename FIRST, typename ENTRY>
 __device__ __forceinline__ void sum_rows(const GradArgs &a, BusyRows &busy, int64_t row0, int rows,
                                          FIRST &&first, ENTRY &&entry) {
   constexpr int kItems = 2;
@@ -603,7 +627,7 @@ __device__ __forceinline__ void sum_rows(const GradArgs &a, BusyRows &busy, int6
   }
   __syncthreads();
   const int count = busy.count;
-  if (count < rows) {
+  if (ZERO && count < rows) {
     float zero[VEC] = {};
     if (vecs >= 256) { // a row per turn or more
       for (int r = 0; r < rows; ++r) {
@@ -670,7 +694,7 @@ __device__ __forceinline__ void sum_rows(const GradArgs &a, BusyRows &busy, int6
 
 __device__ __forceinline__ int hub_lanes(uint32_t vecs) { return vecs <= 8 ? 8 : vecs <= 32 ? 32 : 64; }
 
-// Step 4: a.row_block rows per workgroup, after kHubBlocks workgroups for the
+// Step 3: a.row_block rows per workgroup, after kHubBlocks workgroups for the
 // hubs, which take longest and so begin first.
 template <typename T, typename O, int VEC>
 __global__ void __launch_bounds__(256) embedding_row_kernel(GradArgs a) {
@@ -695,53 +719,144 @@ __global__ void __launch_bounds__(256) embedding_row_kernel(GradArgs a) {
     const int rows = static_cast<int>(min(static_cast<int64_t>(a.row_block), a.rows - row0));
     for (int i = threadIdx.x; i <= rows; i += 256) start[i] = a.row_start[row0 + i];
     __syncthreads();
-    sum_rows<T, O, VEC>(
+    sum_rows<T, O, VEC, true>(
         a, busy, row0, rows, [&](int r) { return start[r]; }, entry);
     __syncthreads(); // `start` and `busy` have been read
   }
 }
 
-// At most kListMost tokens: a span per workgroup, from tokens to rows.
-template <typename T, typename O, int VEC>
+// Zeros for a whole table, 4 vectors per thread.  A large table that few tokens
+// touch is zeroed by a launch of its own, whose waves end with their stores:
+// 6.8 TB/s, where spans that zero themselves reach 5.1 (614 MB: 92 and 125 us).
+constexpr int kZeroItems = 4;
+template <typename O, int VEC> __global__ void __launch_bounds__(256) embedding_zero_kernel(GradArgs a) {
+  const int64_t vecs = a.dim / VEC, all = a.rows * vecs;
+  const int64_t turn = static_cast<int64_t>(gridDim.x) * 256 * kZeroItems;
+  O *const out = static_cast<O *>(a.out);
+  float zero[VEC] = {};
+  for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 * kZeroItems + threadIdx.x; i0 < all;
+       i0 += turn) {
+#pragma unroll
+    for (int u = 0; u < kZeroItems; ++u) {
+      const int64_t i = i0 + 256 * u;
+      if (i < all)
+        store_f32<VEC>(out + (a.out_stride == a.dim ? i * VEC
+                                                    : i / vecs * a.out_stride + i % vecs * VEC),
+                       zero);
+    }
+  }
+}
+
+// Places in order for the tokens of a workgroup that `here` marks, the k-th 64
+// of each wave in here[k]: f(k, place) for each, on its lane.  All threads call
+// it; the marks' number.
+template <int EACH, typename F>
+__device__ __forceinline__ int place_marked(int (&counts)[EACH * kSpanWaves],
+                                            const uint64_t (&here)[EACH], F &&f) {
+  static_assert(EACH * kSpanWaves <= 2 * kWave);
+  const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+#pragma unroll
+  for (int k = 0; k < EACH; ++k)
+    if (lane == 0) counts[k * kSpanWaves + wave] = __popcll(here[k]);
+  __syncthreads();
+  const int c0 = lane < EACH * kSpanWaves ? counts[lane] : 0;
+  const int c1 = lane + kWave < EACH * kSpanWaves ? counts[lane + kWave] : 0;
+  const int in0 = wave_incl_scan(c0), in1 = wave_incl_scan(c1) + readlane(in0, kWave - 1);
+  const uint64_t below = (uint64_t(1) << lane) - 1;
+#pragma unroll
+  for (int k = 0; k < EACH; ++k) {
+    const int c = k * kSpanWaves + wave;
+    const int before = c < kWave ? readlane(in0 - c0, c) : readlane(in1 - c1, c - kWave);
+    if ((here[k] >> lane) & 1) f(k, before + __popcll(here[k] & below));
+  }
+  return readlane(in1, kWave - 1);
+}
+
+// At most MOST tokens and a table that is not large: a span per workgroup,
+// zeroed while the tokens are on their way, and its rows that have some written
+// again.
+template <typename T, typename O, int VEC, int MOST>
 __global__ void __launch_bounds__(256) embedding_few_kernel(GradArgs a) {
-  __shared__ SpanList list;
-  __shared__ uint16_t sorted[kListMost]; // token indices by row
+  constexpr int kEach = MOST / 256;
+  __shared__ SpanList<uint16_t, MOST> list;
+  __shared__ uint16_t sorted[MOST]; // token indices by row
   __shared__ BusyRows busy;
   __shared__ float joined[kSpanWaves][kWave * VEC];
+  __shared__ int counts[kEach * kSpanWaves];
   const int tid = threadIdx.x;
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * a.span;
   const int rows = static_cast<int>(min(static_cast<int64_t>(a.span), a.rows - row0));
   list.clear();
-
-  constexpr int kEach = kListMost / 256;
   uint32_t row[kEach];
-  token_rows(a, static_cast<int64_t>(tid) * kEach, 1, row);
-  int n = 0, total;
+  token_rows(a, tid, 256, row);
+  const int64_t vecs = a.dim / VEC, all = rows * vecs;
+  O *const out = static_cast<O *>(a.out) + row0 * a.out_stride;
+  float zero[VEC] = {};
+  for (int64_t i = tid; i < all; i += 256)
+    store_f32<VEC>(out + (a.out_stride == a.dim ? i * VEC
+                                                : i / vecs * a.out_stride + i % vecs * VEC),
+                   zero);
+  uint64_t here[kEach];
 #pragma unroll
-  for (int k = 0; k < kEach; ++k) n += row[k] >= row0 && row[k] < row0 + rows;
-  int at = list.prefix(n, total);
-#pragma unroll
-  for (int k = 0; k < kEach; ++k) {
-    if (row[k] < row0 || row[k] >= row0 + rows) continue;
-    const uint32_t token = static_cast<uint32_t>(tid * kEach + k);
-    const int b = SpanList::bin(static_cast<int>(row[k] - row0), token);
-    list.source[at] = token;
-    list.local[at++] = static_cast<uint16_t>(b);
+  for (int k = 0; k < kEach; ++k) here[k] = ballot(row[k] >= row0 && row[k] < row0 + rows);
+  const int total = place_marked<kEach>(counts, here, [&](int k, int at) { // after the zeros
+    const uint32_t token = static_cast<uint32_t>(k * 256 + tid);
+    const int b = entry_bin(static_cast<int>(row[k] - row0), token);
+    list.source[at] = static_cast<uint16_t>(token);
+    list.local[at] = static_cast<uint16_t>(b);
     atomicAdd(&list.next[b], 1);
-  }
-  if (total > 0) {
-    list.open();
-    list.place(total, [&](int to, uint32_t what) { sorted[to] = static_cast<uint16_t>(what); });
-  }
-  auto first = [&](int r) { return total > 0 ? list.first[2 * r] : 0; };
+  });
+  if (total == 0) return;
+  list.open();
+  list.place(total, [&](int to, uint32_t what) { sorted[to] = static_cast<uint16_t>(what); });
+  auto first = [&](int r) { return list.first[2 * r]; };
   auto entry = [&](int i) { return static_cast<uint32_t>(sorted[i]); };
-  sum_rows<T, O, VEC>(a, busy, row0, rows, first, entry);
+  sum_rows<T, O, VEC, false>(a, busy, row0, rows, first, entry);
   if (total <= kAlone) return;
-  const int wide = hub_lanes(static_cast<uint32_t>(a.dim / VEC));
+  const int wide = hub_lanes(static_cast<uint32_t>(vecs));
   for (int r = 0; r < rows; ++r) {
     const int from = first(r), to = first(r + 1);
     if (to - from > kAlone)
       sum_hub<T, O, VEC>(a, joined, wide, row0 + r, entry, from, to, 0, a.dim);
+  }
+}
+
+// At most MOST tokens and a large table, zeroed before: a workgroup per token,
+// which goes on if no earlier token is the same, lists those that are and sums
+// their row.  All tokens stay in its registers while it takes its tokens in
+// turn.
+template <typename T, typename O, int VEC, int MOST>
+__global__ void __launch_bounds__(256) embedding_token_kernel(GradArgs a) {
+  constexpr int kEach = MOST / 256;
+  __shared__ uint32_t all[MOST];
+  __shared__ uint16_t same[MOST];
+  __shared__ float joined[kSpanWaves][kWave * VEC];
+  __shared__ int counts[kEach * kSpanWaves];
+  const int tid = threadIdx.x, wave_first = tid / kWave * kWave;
+  uint32_t row[kEach];
+  token_rows(a, tid, 256, row);
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) all[k * 256 + tid] = row[k];
+  __syncthreads();
+  const int wide = hub_lanes(static_cast<uint32_t>(a.dim / VEC));
+  for (int t = blockIdx.x; t < a.count; t += gridDim.x) {
+    const uint32_t mine = all[t];
+    if (mine == static_cast<uint32_t>(a.rows)) continue;
+    uint64_t here[kEach];
+    bool before = false;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+      here[k] = ballot(row[k] == mine);
+      const int ahead = t - (k * 256 + wave_first); // of these 64, how many come before t
+      before = before || (ahead >= kWave ? here[k] != 0
+                                         : ahead > 0 && (here[k] & ((uint64_t(1) << ahead) - 1)) != 0);
+    }
+    if (__syncthreads_or(before)) continue; // also: the row before has been summed
+    const int n = place_marked<kEach>(
+        counts, here, [&](int k, int at) { same[at] = static_cast<uint16_t>(k * 256 + tid); });
+    __syncthreads();
+    sum_hub<T, O, VEC>(
+        a, joined, wide, mine, [&](int i) { return static_cast<uint32_t>(same[i]); }, 0, n, 0, a.dim);
   }
 }
 
@@ -764,21 +879,29 @@ template <typename T> int32_t lookup_typed(const LookupArgs &a, void *stream) {
 }
 
 struct GradLayout {
-  int span;
+  bool large;
+  int span, tile;
   int64_t spans, tiles;
   size_t keys, sources, order, runs, run_count, starts, sums, list, row_start, hubs, bytes;
   int64_t hub_stride;
 };
 
 // Table rows per span: enough spans to fill the card several times over, and
-// at most kSpanMost rows each.  Up to kListMost tokens fit every span's list
-// whole, and need no tiles.
+// at most kSpanMost rows each.  Few tokens need no tiles.
 GradLayout grad_layout(int64_t count, int64_t rows, int64_t dim) {
   GradLayout l{};
-  l.span = static_cast<int>(std::clamp<int64_t>(rows / 2048, 1, kSpanMost));
-  l.spans = ceil_div64(rows, l.span);
-  if (count <= kListMost) return l;
-  l.tiles = ceil_div64(count, kTile);
+  l.large = rows * dim >= kLarge;
+  auto cut = [&](int64_t spans) {
+    l.span = static_cast<int>(std::clamp<int64_t>(rows / spans, 1, kSpanMost));
+    l.spans = ceil_div64(rows, l.span);
+  };
+  cut(1024);
+  if (count <= kFewMost && count * dim <= kFewElements &&
+      (l.large || count * l.spans <= kFewReads))
+    return l;
+  cut(2048);
+  l.tile = count <= int64_t(kSmallTile) * kMostSmallTiles ? kSmallTile : kLargeTile;
+  l.tiles = ceil_div64(count, l.tile);
   size_t at = 0;
   auto take = [&](size_t elems, size_t size) {
     const size_t here = at;
@@ -786,13 +909,13 @@ GradLayout grad_layout(int64_t count, int64_t rows, int64_t dim) {
     return here;
   };
   const size_t tiles = static_cast<size_t>(l.tiles);
-  l.keys = take(tiles * kTile, sizeof(uint32_t));
-  l.sources = take(tiles * kTile, sizeof(uint32_t));
-  l.order = take(tiles * kTile, sizeof(uint16_t));
-  l.runs = take(tiles * kTileRuns, sizeof(uint32_t));
+  l.keys = take(tiles * l.tile, sizeof(uint32_t));
+  l.sources = take(tiles * l.tile, sizeof(uint32_t));
+  l.order = take(tiles * l.tile, sizeof(uint16_t));
+  l.runs = take(tiles * l.tile / kRun, sizeof(uint32_t));
   l.run_count = take(tiles, sizeof(int32_t));
   l.starts = take(tiles * (l.spans + 1), sizeof(uint16_t));
-  l.sums = take(tiles * kTileRuns * dim, sizeof(float));
+  l.sums = take(tiles * l.tile / kRun * dim, sizeof(float));
   l.list = take(count, sizeof(uint32_t));
   l.row_start = take(rows + 1, sizeof(int32_t));
   l.hub_stride = ceil_div64(1 + count / (kAlone + 1), 64) * 64; // lines of their own
@@ -801,22 +924,40 @@ GradLayout grad_layout(int64_t count, int64_t rows, int64_t dim) {
   return l;
 }
 
-template <typename T, int VEC> int32_t run_runs(const GradArgs &a, void *stream) {
+template <typename T, int VEC> int32_t run_spans(const GradArgs &a, void *stream) {
   const int64_t vecs = ceil_div64(a.dim, VEC);
   auto go = [&](auto kernel, int lanes) {
-    return launch(kernel, dim3(a.tiles * kRunBlocks, ceil_div64(vecs, lanes)), dim3(256), stream, a);
+    const int64_t run_grid = a.tiles * run_blocks(a.tile) * ceil_div64(vecs, lanes);
+    return launch(kernel, dim3(run_grid + a.spans), dim3(256), stream, a, run_grid);
   };
-  if (vecs <= 8) return go(embedding_run_kernel<T, VEC, 8>, 8);
-  if (vecs <= 32) return go(embedding_run_kernel<T, VEC, 32>, 32);
-  return go(embedding_run_kernel<T, VEC, 64>, 64);
+  if (vecs <= 8) return go(embedding_span_kernel<T, VEC, 8>, 8);
+  if (vecs <= 32) return go(embedding_span_kernel<T, VEC, 32>, 32);
+  return go(embedding_span_kernel<T, VEC, 64>, 64);
 }
 
 template <typename T, typename O, int VEC> int32_t grad_vec(GradArgs a, void *stream) {
-  if (a.tiles == 0)
-    return launch(embedding_few_kernel<T, O, VEC>, dim3(a.spans), dim3(256), stream, a);
-  int32_t rc = launch(embedding_tile_kernel, dim3(a.tiles), dim3(kTileBlock), stream, a);
-  if (rc == SPORDER_OK) rc = run_runs<T, VEC>(a, stream);
-  if (rc == SPORDER_OK) rc = launch(embedding_span_kernel, dim3(a.spans), dim3(256), stream, a);
+  if (a.tiles == 0) {
+    auto go = [&](auto kernel, int64_t blocks) {
+      return launch(kernel, dim3(blocks), dim3(256), stream, a);
+    };
+    if (!a.large)
+      return a.count <= 1024   ? go(embedding_few_kernel<T, O, VEC, 1024>, a.spans)
+             : a.count <= 4096 ? go(embedding_few_kernel<T, O, VEC, 4096>, a.spans)
+                               : go(embedding_few_kernel<T, O, VEC, kFewMost>, a.spans);
+    const int64_t blocks = ceil_div64(a.rows * (a.dim / VEC), 256 * kZeroItems);
+    const int32_t rc = go(embedding_zero_kernel<O, VEC>, std::min(blocks, kMostBlocks));
+    if (rc != SPORDER_OK || a.count == 0) return rc;
+    const int64_t turns = std::min(a.count, kFewBlocks);
+    return a.count <= 1024   ? go(embedding_token_kernel<T, O, VEC, 1024>, turns)
+           : a.count <= 4096 ? go(embedding_token_kernel<T, O, VEC, 4096>, turns)
+                             : go(embedding_token_kernel<T, O, VEC, kFewMost>, turns);
+  }
+  int32_t rc = a.tile == kSmallTile
+                   ? launch(embedding_tile_kernel<kSmallTile>, dim3(a.tiles),
+                            dim3(kSmallTile / kTileRounds), stream, a)
+                   : launch(embedding_tile_kernel<kLargeTile>, dim3(a.tiles),
+                            dim3(kLargeTile / kTileRounds), stream, a);
+  if (rc == SPORDER_OK) rc = run_spans<T, VEC>(a, stream);
   if (rc != SPORDER_OK) return rc;
   // About one turn of sum_rows per workgroup, with one row in rows / count
   // taken to have entries.
@@ -838,9 +979,9 @@ template <typename T, typename O> int32_t grad_typed(const GradArgs &a, void *st
 }
 
 // Rows count in 31 bits with one value over (no row); a launch has fewer than
-// 2^32 threads, and the runs' launch takes up to 16 per token.
+// 2^32 threads, and the runs' launch takes 2 per token and slice.
 constexpr int64_t kMostRows = (int64_t(1) << 31) - 2;
-constexpr int64_t kMostTokens = (int64_t(1) << 28) - kTile;
+constexpr int64_t kMostTokens = (int64_t(1) << 28) - kLargeTile;
 
 } // namespace
 
@@ -899,10 +1040,12 @@ int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count, int64_
                    scale,
                    token_bits == 64,
                    rows * dim * type_bytes(out_type) >= kStreamBytes,
+                   l.large,
                    bits_for(rows),
                    0,
                    l.span,
                    l.spans,
+                   l.tile,
                    l.tiles,
                    reinterpret_cast<uint32_t *>(w + l.keys),
                    reinterpret_cast<uint32_t *>(w + l.sources),

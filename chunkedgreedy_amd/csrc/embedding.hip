@@ -22,7 +22,8 @@
 //      the launch's first workgroups.
 //
 // Few tokens need no tiles: each span picks its own from all of them and sums
-// its rows, in one launch.
+// its rows, in one launch.  A large table of few tokens is zeroed at the speed
+// of a fill, then a workgroup per token finds its equals and sums their row.
 #include <algorithm>
 
 #include "dense.hpp"

@@ -214,20 +214,23 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
   float w[C][VEC], dw[C][VEC] = {}, db[C][VEC] = {};
   load_vector<LOOSE, VEC, L>(a.weight, a.weight_type, a.dim, 1.0f, lane, w);
 
-  Pack<T, VEC> next_x[C], next_dy[C];
+  // Words until they are used: elements of 16 bits that meet the zeros past a
+  // row's end one by one go through scratch memory.
+  struct Words {
+    uint32_t v[VEC * sizeof(T) / 4];
+  };
+  Words next_x[C], next_dy[C];
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto fetch_next = [&](int64_t row) {
     const bool live = row < a.rows;
     const T *const x = static_cast<const T *>(a.x) + row * a.x_stride;
     const T *const dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
-    auto part = [&](const T *p, int c, Pack<T, VEC> &to) {
+    auto words = [&](const T *p, int col) {
+      return __builtin_bit_cast(Words, fetch<LOOSE, VEC>(p + col, a.dim - col));
+    };
+    auto part = [&](const T *p, int c) {
       const int col = (c * L + lane) * VEC;
-      if (live && col < a.dim) {
-        to = fetch<LOOSE, VEC>(p + col, a.dim - col);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) to.v[i] = static_cast<T>(0.0f);
-      }
+      return live && col < a.dim ? words(p, col) : Words{};
     };
     auto stats = [&]() {
       next_mean = live ? a.mean[row] : 0.0f;
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
     };
     // The order of the loads.  16-bit rows at whole accesses, and any at 8 bytes
     // an access, are faster alternating between x and dy (100 million elements
-    // in rows of 300: 133 us, 196 one row after the other; of 64: 120, 128);
+    // in rows of 300: 127 us, 196 one row after the other; of 64: 120, 128);
     // wider rows of floats that end inside a line one after the other (in rows
     // of 100: 241 us, 332 alternating), and so rows that are fetched ahead.
     if constexpr ((sizeof(T) == 2 && !LOOSE && L < 512) || VEC * sizeof(T) == 8) {
@@ -243,19 +246,17 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int col = (c * L + lane) * VEC;
+        next_x[c] = next_dy[c] = Words{};
         if (live && col < a.dim) { // one branch for both loads
-          next_x[c] = fetch<LOOSE, VEC>(x + col, a.dim - col);
-          next_dy[c] = fetch<LOOSE, VEC>(dy + col, a.dim - col);
-        } else {
-#pragma unroll
-          for (int i = 0; i < VEC; ++i) next_x[c].v[i] = next_dy[c].v[i] = static_cast<T>(0.0f);
+          next_x[c] = words(x, col);
+          next_dy[c] = words(dy, col);
         }
       }
     } else {
 #pragma unroll
-      for (int c = 0; c < C; ++c) part(x, c, next_x[c]);
+      for (int c = 0; c < C; ++c) next_x[c] = part(x, c);
 #pragma unroll
-      for (int c = 0; c < C; ++c) part(dy, c, next_dy[c]);
+      for (int c = 0; c < C; ++c) next_dy[c] = part(dy, c);
       stats();
     }
   };
@@ -273,10 +274,12 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      const auto x = __builtin_bit_cast(Pack<T, VEC>, next_x[c]);
+      const auto dy = __builtin_bit_cast(Pack<T, VEC>, next_dy[c]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        h[c][i] = static_cast<float>(next_x[c].v[i]);
-        g[c][i] = static_cast<float>(next_dy[c].v[i]);
+        h[c][i] = static_cast<float>(x.v[i]);
+        g[c][i] = static_cast<float>(dy.v[i]);
       }
     }
     if (kAhead) fetch_next(row + stride);
@@ -455,15 +458,28 @@ template <int MOST, typename F> int32_t with_waves(int64_t dim, F &&f) {
   return with_lanes<MOST>(dim, f);
 }
 
+// Rows of 32-bit elements that no vector fits are read by elements where a wave
+// has many of a row side by side, by vectors at any alignment where it has few
+// and where a lane would hold 64 elements apart (100 million elements, forward
+// and backward, by elements and by vectors: rows of 101 224 + 288 and 284 + 339
+// us, of 8191 148 + 231 and 202 + 264, of 24001 488 and 279 forward).  Rows of
+// 16-bit elements are always read by vectors; the gradient takes 4 elements at
+// a time up to 4096 and 8 past it.
+constexpr bool norm_loose(int64_t dim) { return dim <= 64 || dim > 16384; }
+constexpr bool norm_grad_loose(int64_t dim) { return dim <= 64; }
+constexpr int norm_grad_loose_vec(int64_t dim) { return dim <= 4096 ? 4 : 8; }
+
+// Kernels are built for what the rules above pick at some dim that their lanes
+// and elements hold.
 template <typename T, bool LOOSE, int VEC> int32_t norm_lanes(const NormArgs &a, void *stream) {
   auto go = [&](auto lanes, auto elements) {
-    constexpr int L = decltype(lanes)::value;
-    if constexpr (decltype(elements)::value < VEC) {
+    constexpr int L = decltype(lanes)::value, E = decltype(elements)::value;
+    if constexpr (sizeof(T) == 4 && (LOOSE || VEC == 1) && norm_loose(L * E) != LOOSE) {
       return static_cast<int32_t>(SPORDER_BAD_ARGUMENT); // not reached
     } else {
       const int64_t blocks = std::min(ceil_div64(a.rows, norm_block(L) / L), kMaxNormBlocks);
-      return launch(layer_norm_kernel<T, LOOSE, VEC, L, decltype(elements)::value / VEC>,
-                    dim3(blocks), dim3(norm_block(L)), stream, a);
+      return launch(layer_norm_kernel<T, LOOSE, VEC, L, E / VEC>, dim3(blocks), dim3(norm_block(L)),
+                    stream, a);
     }
   };
   if constexpr (VEC >= 4)
@@ -475,9 +491,14 @@ template <typename T, bool LOOSE, int VEC> int32_t norm_lanes(const NormArgs &a,
 template <typename T, bool LOOSE, int VEC>
 int32_t norm_grad_lanes(const NormGradArgs &a, int64_t blocks, void *stream) {
   auto go = [&](auto lanes, auto elements) {
-    constexpr int L = decltype(lanes)::value;
-    return launch(layer_norm_grad_kernel<T, LOOSE, VEC, L, decltype(elements)::value / VEC>,
-                  dim3(blocks), dim3(norm_block(L)), stream, a);
+    constexpr int L = decltype(lanes)::value, E = decltype(elements)::value;
+    if constexpr ((sizeof(T) == 4 && (LOOSE || VEC == 1) && norm_grad_loose(L * E) != LOOSE) ||
+                  (sizeof(T) == 2 && LOOSE && norm_grad_loose_vec(L * E) != VEC)) {
+      return static_cast<int32_t>(SPORDER_BAD_ARGUMENT); // not reached
+    } else {
+      return launch(layer_norm_grad_kernel<T, LOOSE, VEC, L, E / VEC>, dim3(blocks),
+                    dim3(norm_block(L)), stream, a);
+    }
   };
   if constexpr (VEC >= 4)
     return with_lanes<32>(a.dim, go);
@@ -496,7 +517,7 @@ template <typename T> int32_t norm_typed(const NormArgs &a, void *stream) {
     return norm_lanes<T, true, 8>(a, stream);
   } else {
     if (vec == 4) return norm_lanes<T, false, 4>(a, stream);
-    return a.dim <= 64 ? norm_lanes<T, true, 4>(a, stream) : norm_lanes<T, false, 1>(a, stream);
+    return norm_loose(a.dim) ? norm_lanes<T, true, 4>(a, stream) : norm_lanes<T, false, 1>(a, stream);
   }
 }
 
@@ -509,12 +530,12 @@ int32_t norm_grad_typed(const NormGradArgs &a, int64_t blocks, void *stream) {
   if constexpr (sizeof(T) == 2) {
     if (vec == 8) return norm_grad_lanes<T, false, 8>(a, blocks, stream);
     if (vec == 4) return norm_grad_lanes<T, false, 4>(a, blocks, stream);
-    return a.dim <= 4096 ? norm_grad_lanes<T, true, 4>(a, blocks, stream)
-                         : norm_grad_lanes<T, true, 8>(a, blocks, stream);
+    return norm_grad_loose_vec(a.dim) == 4 ? norm_grad_lanes<T, true, 4>(a, blocks, stream)
+                                           : norm_grad_lanes<T, true, 8>(a, blocks, stream);
   } else {
     if (vec == 4) return norm_grad_lanes<T, false, 4>(a, blocks, stream);
-    return a.dim <= 64 ? norm_grad_lanes<T, true, 4>(a, blocks, stream)
-                       : norm_grad_lanes<T, false, 1>(a, blocks, stream);
+    return norm_grad_loose(a.dim) ? norm_grad_lanes<T, true, 4>(a, blocks, stream)
+                                  : norm_grad_lanes<T, false, 1>(a, blocks, stream);
   }
 }
 
@@ -575,7 +596,7 @@ int32_t sporder_layer_norm_grad(void *stream, int32_t type, int32_t weight_type,
   if (!d_dy || !d_x || !d_mean || !d_rstd || !d_dx) return SPORDER_BAD_ARGUMENT;
   const int64_t blocks = norm_grad_blocks(rows, dim);
   if (columns &&
-      (!d_work || !aligned_to(d_work, 4) || work_bytes < sporder_layer_norm_grad_work_bytes(rows, dim)))
+      (!d_work || !aligned_to(d_work, 256) || work_bytes < sporder_layer_norm_grad_work_bytes(rows, dim)))
     return SPORDER_BAD_ARGUMENT;
   float *const partial = columns ? static_cast<float *>(d_work) : nullptr;
   const NormGradArgs a{rows, dim,      dy_stride, x_stride, dx_stride, d_dy,

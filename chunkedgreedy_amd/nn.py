@@ -4,13 +4,14 @@ the orthogonalisation.
 ``embedding`` and ``layer_norm`` are ``sporder.embedding`` and
 ``sporder.layer_norm`` with their gradients behind torch's autograd; ``Muon``
 updates weight matrices along the orthogonalised momentum
-(``sporder.newton_schulz``).  The end-to-end GCN (``e2e_gcn``) trains with them
-on request.  They have no counterpart in the reference.
+(``sporder.newton_schulz``).  Their backward passes are not differentiable in
+turn.  The end-to-end GCN (``e2e_gcn``) trains with them on request.  They have no counterpart in the reference.
 """
 
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import sporder
 
@@ -23,6 +24,7 @@ class _Embedding(torch.autograd.Function):
         return sporder.embedding(table, tokens, scale=scale)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         (tokens,) = ctx.saved_tensors
         return sporder.embedding_grad(grad, tokens, ctx.rows, scale=ctx.scale,
@@ -44,6 +46,7 @@ class _LayerNorm(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         x, mean, rstd, weight = ctx.saved_tensors
         dx, dweight, dbias = sporder.layer_norm_grad(grad, x, mean, rstd, weight)
@@ -87,7 +90,10 @@ class Muon(torch.optim.Optimizer):
             for p in group["params"]:
                 if p.grad is None:
                     continue
-                m = self.state[p].setdefault("momentum", torch.zeros_like(p))
+                state = self.state[p]
+                if "momentum" not in state:
+                    state["momentum"] = torch.zeros_like(p)
+                m = state["momentum"]
                 m.mul_(group["momentum"]).add_(p.grad)
                 update = sporder.newton_schulz(p.grad.add(m, alpha=group["momentum"]),
                                                steps=group["steps"])

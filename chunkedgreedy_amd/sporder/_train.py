@@ -131,7 +131,7 @@ def embedding_grad(grad, tokens, num_rows, *, scale=1.0, padding_idx=None, dtype
         grad: tokens.shape + (dim,), float32, bfloat16 or float16
         tokens: int32 or int64 ids; ids outside [0, num_rows) are left out
         num_rows: rows of the table
-        padding_idx: a row that gets no gradient, or None
+        padding_idx: a row in [0, num_rows) that gets no gradient, or None
         dtype: grad's type (default) or float32, the type of the result
         out: contiguous (num_rows, dim) tensor of that type, or None
 
@@ -146,6 +146,8 @@ def embedding_grad(grad, tokens, num_rows, *, scale=1.0, padding_idx=None, dtype
     num_rows = int(num_rows)
     if not 1 <= num_rows <= 2**31 - 2:
         raise ValueError("num_rows must be in [1, 2^31 - 2]")
+    if padding_idx is not None and not 0 <= padding_idx < num_rows:
+        raise ValueError("padding_idx must be a row of the table")
     if dtype is None:
         dtype = grad.dtype
     elif dtype not in (grad.dtype, torch.float32):
@@ -287,8 +289,8 @@ def newton_schulz(g, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-
         raise ValueError("g must be (rows, cols) or (batch, rows, cols) with sides of 1 to 65536 "
                          "and a batch of at most 32768")
     steps = int(steps)
-    if steps < 1:
-        raise ValueError("steps must be >= 1")
+    if not 1 <= steps < 2**31:
+        raise ValueError("steps must be >= 1 and below 2^31")
     if not eps >= 0.0:
         raise ValueError("eps must be >= 0")
     a, b, c = (float(v) for v in coefficients)

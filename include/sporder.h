@@ -459,8 +459,9 @@ SPORDER_API int32_t sporder_embedding(void *stream, int32_t type, int64_t rows, 
 /*
  * Its gradient by the table: d_out[v] = scale * sum of d_grad[t] over the t
  * with d_tokens[t] = v, for each of `rows` rows (0 where there is no such t),
- * summed in an order that depends on the tokens and the sizes alone.  Tokens equal to padding_idx and tokens outside [0, rows) are left
- * out.  out_type is `type` or SPORDER_TYPE_F32.  d_work is 256-byte aligned.
+ * summed in an order that depends on the tokens and the sizes alone.  Tokens
+ * equal to padding_idx and tokens outside [0, rows) are left out.  out_type is
+ * `type` or SPORDER_TYPE_F32.  d_work is 256-byte aligned.
  */
 SPORDER_API size_t sporder_embedding_grad_work_bytes(int64_t count, int64_t rows, int64_t dim);
 SPORDER_API int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count,
@@ -488,6 +489,7 @@ SPORDER_API int32_t sporder_layer_norm(void *stream, int32_t type, int32_t weigh
  * Its gradients from dy and the forward call's mean and rstd: d_dx (rows of
  * dim elements, dx_stride apart), and, where not NULL, d_dweight and d_dbias
  * (dim elements of weight_type, summed over the rows).  d_dx may be d_dy.
+ * d_work, needed for those two, is 256-byte aligned.
  */
 SPORDER_API size_t sporder_layer_norm_grad_work_bytes(int64_t rows, int64_t dim);
 SPORDER_API int32_t sporder_layer_norm_grad(void *stream, int32_t type, int32_t weight_type,

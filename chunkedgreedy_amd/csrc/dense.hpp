@@ -61,6 +61,18 @@ __device__ __forceinline__ Pack<T, VEC> fetch(const T *p, int64_t left) {
   return q;
 }
 
+// The same as words, for rows fetched in a branch: elements converted there make
+// each access wait for the one before, and elements of 16 bits that meet the
+// zeros past a row's end one by one go through scratch memory.
+template <typename T, int VEC> struct Words {
+  uint32_t v[VEC * sizeof(T) / 4];
+};
+
+template <bool LOOSE, int VEC, typename T>
+__device__ __forceinline__ Words<T, VEC> fetch_words(const T *p, int64_t left) {
+  return __builtin_bit_cast(Words<T, VEC>, fetch<LOOSE, VEC>(p, left));
+}
+
 template <bool LOOSE, int VEC, typename T>
 __device__ __forceinline__ void put(T *p, int64_t left, const float (&in)[VEC]) {
   if constexpr (!LOOSE) {

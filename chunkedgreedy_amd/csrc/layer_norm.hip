@@ -113,24 +113,22 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
     const int64_t row = first + group;
     const bool live = row < a.rows;
     const T *const x = static_cast<const T *>(a.x) + row * a.x_stride;
+    Words<T, VEC> raw[C];
     float v[C][VEC];
     float s[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
       const int col = (c * L + lane) * VEC;
-      if (live && col < a.dim) {
-        const Pack<T, VEC> q = fetch<LOOSE, VEC>(x + col, a.dim - col);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[c][i] = static_cast<float>(q.v[i]);
-      } else {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) v[c][i] = 0.0f;
-      }
+      raw[c] = live && col < a.dim ? fetch_words<LOOSE, VEC>(x + col, a.dim - col) : Words<T, VEC>{};
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      const auto q = __builtin_bit_cast(Pack<T, VEC>, raw[c]);
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s[0] += v[c][i];
+      for (int i = 0; i < VEC; ++i) {
+        v[c][i] = static_cast<float>(q.v[i]);
+        s[0] += v[c][i];
+      }
     }
     row_sum(s);
     const float mean = s[0] / dim;
@@ -214,23 +212,16 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
   float w[C][VEC], dw[C][VEC] = {}, db[C][VEC] = {};
   load_vector<LOOSE, VEC, L>(a.weight, a.weight_type, a.dim, 1.0f, lane, w);
 
-  // Words until they are used: elements of 16 bits that meet the zeros past a
-  // row's end one by one go through scratch memory.
-  struct Words {
-    uint32_t v[VEC * sizeof(T) / 4];
-  };
-  Words next_x[C], next_dy[C];
+  Words<T, VEC> next_x[C], next_dy[C];
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto fetch_next = [&](int64_t row) {
     const bool live = row < a.rows;
     const T *const x = static_cast<const T *>(a.x) + row * a.x_stride;
     const T *const dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
-    auto words = [&](const T *p, int col) {
-      return __builtin_bit_cast(Words, fetch<LOOSE, VEC>(p + col, a.dim - col));
-    };
+    auto words = [&](const T *p, int col) { return fetch_words<LOOSE, VEC>(p + col, a.dim - col); };
     auto part = [&](const T *p, int c) {
       const int col = (c * L + lane) * VEC;
-      return live && col < a.dim ? words(p, col) : Words{};
+      return live && col < a.dim ? words(p, col) : Words<T, VEC>{};
     };
     auto stats = [&]() {
       next_mean = live ? a.mean[row] : 0.0f;
@@ -246,7 +237,7 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
 #pragma unroll
       for (int c = 0; c < C; ++c) {
         const int col = (c * L + lane) * VEC;
-        next_x[c] = next_dy[c] = Words{};
+        next_x[c] = next_dy[c] = Words<T, VEC>{};
         if (live && col < a.dim) { // one branch for both loads
           next_x[c] = words(x, col);
           next_dy[c] = words(dy, col);

@@ -61,16 +61,39 @@ __device__ __forceinline__ Pack<T, VEC> fetch(const T *p, int64_t left) {
   return q;
 }
 
-// The same as words, for rows fetched in a branch: elements converted there make
-// each access wait for the one before, and elements of 16 bits that meet the
-// zeros past a row's end one by one go through scratch memory.
+// A row's VEC elements from `col` on in two halves, for rows of which many
+// accesses are to be on their way at once: the words, then the elements, zeros
+// past the row's end and where the row is not `live`.  Elements converted
+// between accesses would make each wait for the one before.  A loose row that
+// holds a vector can be read by vectors alone (CLAMP), the last one ending with
+// the row and moved into place afterwards: `row` is then a row's address whether
+// it is live or not.
 template <typename T, int VEC> struct Words {
   uint32_t v[VEC * sizeof(T) / 4];
 };
 
-template <bool LOOSE, int VEC, typename T>
-__device__ __forceinline__ Words<T, VEC> fetch_words(const T *p, int64_t left) {
-  return __builtin_bit_cast(Words<T, VEC>, fetch<LOOSE, VEC>(p, left));
+template <bool LOOSE, bool CLAMP, int VEC, typename T>
+__device__ __forceinline__ Words<T, VEC> fetch_words(const T *row, int col, int64_t dim, bool live) {
+  if constexpr (CLAMP) {
+    if (dim >= VEC)
+      return __builtin_bit_cast(Words<T, VEC>,
+                                *reinterpret_cast<const LoosePack<T, VEC> *>(
+                                    row + min(col, static_cast<int>(dim) - VEC)));
+  }
+  return live && col < dim ? __builtin_bit_cast(Words<T, VEC>, fetch<LOOSE, VEC>(row + col, dim - col))
+                           : Words<T, VEC>{};
+}
+
+template <bool CLAMP, int VEC, typename T>
+__device__ __forceinline__ Pack<T, VEC> elements(Words<T, VEC> w, int col, int64_t dim, bool live) {
+  if constexpr (CLAMP) {
+    using Bits = std::conditional_t<sizeof(w) == 16, unsigned __int128, uint64_t>;
+    const int past = live ? col + VEC - static_cast<int>(dim) : VEC;
+    if (dim >= VEC && past > 0)
+      w = past < VEC ? __builtin_bit_cast(Words<T, VEC>, __builtin_bit_cast(Bits, w) >> past * 8 * sizeof(T))
+                     : Words<T, VEC>{};
+  }
+  return __builtin_bit_cast(Pack<T, VEC>, w);
 }
 
 template <bool LOOSE, int VEC, typename T>

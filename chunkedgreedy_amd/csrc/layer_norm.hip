@@ -99,6 +99,8 @@ __device__ __forceinline__ void load_vector(const void *p, int type, int64_t dim
 template <typename T, bool LOOSE, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
   constexpr int kGroups = norm_block(L) / L;
+  // 100 million elements in rows of 101 143 us, 159 without; of 8195 205, 146.
+  constexpr bool kClamp = LOOSE && sizeof(T) == 2 && L < 512;
   __shared__ float shared[2][1][norm_block(L) / kWave];
   RowSum<L, 1> row_sum{shared};
   const int lane = threadIdx.x % L, group = threadIdx.x / L;
@@ -112,18 +114,17 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
        first += static_cast<int64_t>(gridDim.x) * kGroups) {
     const int64_t row = first + group;
     const bool live = row < a.rows;
-    const T *const x = static_cast<const T *>(a.x) + row * a.x_stride;
+    const T *const x = static_cast<const T *>(a.x) + (kClamp && !live ? first : row) * a.x_stride;
     Words<T, VEC> raw[C];
     float v[C][VEC];
     float s[1] = {0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const int col = (c * L + lane) * VEC;
-      raw[c] = live && col < a.dim ? fetch_words<LOOSE, VEC>(x + col, a.dim - col) : Words<T, VEC>{};
+      raw[c] = fetch_words<LOOSE, kClamp, VEC>(x, (c * L + lane) * VEC, a.dim, live);
     }
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const auto q = __builtin_bit_cast(Pack<T, VEC>, raw[c]);
+      const auto q = elements<kClamp, VEC, T>(raw[c], (c * L + lane) * VEC, a.dim, live);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         v[c][i] = static_cast<float>(q.v[i]);
@@ -199,6 +200,7 @@ template <typename T> __global__ void __launch_bounds__(1024) layer_norm_long_ke
 template <typename T, bool LOOSE, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGradArgs a) {
   constexpr int kGroups = norm_block(L) / L;
+  constexpr bool kClamp = LOOSE && sizeof(T) == 2; // rows of 101 170 us, 208 without
   constexpr int kSpan = L * C * VEC; // columns that a group holds
   constexpr int kBlockWaves = norm_block(L) / kWave;
   constexpr int kRowWaves = L > kWave ? L / kWave : 1;
@@ -216,12 +218,11 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
   float next_mean = 0.0f, next_rstd = 0.0f;
   auto fetch_next = [&](int64_t row) {
     const bool live = row < a.rows;
-    const T *const x = static_cast<const T *>(a.x) + row * a.x_stride;
-    const T *const dy = static_cast<const T *>(a.dy) + row * a.dy_stride;
-    auto words = [&](const T *p, int col) { return fetch_words<LOOSE, VEC>(p + col, a.dim - col); };
+    const int64_t from = kClamp && !live ? a.rows - 1 : row;
+    const T *const x = static_cast<const T *>(a.x) + from * a.x_stride;
+    const T *const dy = static_cast<const T *>(a.dy) + from * a.dy_stride;
     auto part = [&](const T *p, int c) {
-      const int col = (c * L + lane) * VEC;
-      return live && col < a.dim ? words(p, col) : Words<T, VEC>{};
+      return fetch_words<LOOSE, kClamp, VEC>(p, (c * L + lane) * VEC, a.dim, live);
     };
     auto stats = [&]() {
       next_mean = live ? a.mean[row] : 0.0f;
@@ -238,9 +239,9 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
       for (int c = 0; c < C; ++c) {
         const int col = (c * L + lane) * VEC;
         next_x[c] = next_dy[c] = Words<T, VEC>{};
-        if (live && col < a.dim) { // one branch for both loads
-          next_x[c] = words(x, col);
-          next_dy[c] = words(dy, col);
+        if (kClamp || (live && col < a.dim)) { // one branch for both loads
+          next_x[c] = part(x, c);
+          next_dy[c] = part(dy, c);
         }
       }
     } else {
@@ -265,8 +266,9 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
     float s[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int c = 0; c < C; ++c) {
-      const auto x = __builtin_bit_cast(Pack<T, VEC>, next_x[c]);
-      const auto dy = __builtin_bit_cast(Pack<T, VEC>, next_dy[c]);
+      const int col = (c * L + lane) * VEC;
+      const auto x = elements<kClamp, VEC, T>(next_x[c], col, a.dim, row < a.rows);
+      const auto dy = elements<kClamp, VEC, T>(next_dy[c], col, a.dim, row < a.rows);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
         h[c][i] = static_cast<float>(x.v[i]);
@@ -451,13 +453,13 @@ template <int MOST, typename F> int32_t with_waves(int64_t dim, F &&f) {
 
 // Rows of 32-bit elements that no vector fits are read by elements where a wave
 // has many of a row side by side, by vectors at any alignment where it has few
-// and where a lane would hold 64 elements apart (100 million elements, forward
-// and backward, by elements and by vectors: rows of 101 224 + 288 and 284 + 339
-// us, of 8191 148 + 231 and 202 + 264, of 24001 488 and 279 forward).  Rows of
+// and where a lane would hold many elements apart (100 million elements, by
+// elements and by vectors: rows of 101 forward 224 and 284 us, backward 288 and
+// 339; of 24001 forward 488 and 280; of 12003 backward 371 and 314).  Rows of
 // 16-bit elements are always read by vectors; the gradient takes 4 elements at
-// a time up to 4096 and 8 past it.
+// a time up to 4096 (rows of 259: 168 us, 214 with 8) and 8 past it.
 constexpr bool norm_loose(int64_t dim) { return dim <= 64 || dim > 16384; }
-constexpr bool norm_grad_loose(int64_t dim) { return dim <= 64; }
+constexpr bool norm_grad_loose(int64_t dim) { return dim <= 64 || dim > 8192; }
 constexpr int norm_grad_loose_vec(int64_t dim) { return dim <= 4096 ? 4 : 8; }
 
 // Kernels are built for what the rules above pick at some dim that their lanes

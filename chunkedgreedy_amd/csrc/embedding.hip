@@ -116,7 +116,8 @@ constexpr int kListMost = 2048;   // a span's entries in LDS at a time
 // one workgroup may have to add up alone (2 MB at most, some 25 us).
 constexpr int kFewMost = 8192;
 constexpr int64_t kFewReads = int64_t(1) << 24, kFewElements = int64_t(1) << 19;
-constexpr int64_t kFewBlocks = 1024;
+constexpr int kLargeFewMost = 2048; // past it the spans are faster
+constexpr int64_t kTokenSlices = 32;
 constexpr int64_t kLarge = int64_t(1) << 24; // elements of a large table
 constexpr int kSparse = 4;        // turns' worth of rows per workgroup, at most
 constexpr int kAlone = 8;         // entries of a row that one lane adds up
@@ -693,7 +694,7 @@ __device__ __forceinline__ void sum_rows(const GradArgs &a, BusyRows &busy, int6
   }
 }
 
-__device__ __forceinline__ int hub_lanes(uint32_t vecs) { return vecs <= 8 ? 8 : vecs <= 32 ? 32 : 64; }
+__host__ __device__ __forceinline__ int hub_lanes(uint32_t vecs) { return vecs <= 8 ? 8 : vecs <= 32 ? 32 : 64; }
 
 // Step 3: a.row_block rows per workgroup, after kHubBlocks workgroups for the
 // hubs, which take longest and so begin first.
@@ -726,26 +727,27 @@ __global__ void __launch_bounds__(256) embedding_row_kernel(GradArgs a) {
   }
 }
 
-// Zeros for a whole table, 4 vectors per thread.  A large table that few tokens
-// touch is zeroed by a launch of its own, whose waves end with their stores:
-// 6.8 TB/s, where spans that zero themselves reach 5.1 (614 MB: 92 and 125 us).
+// Zeros for `rows` rows of `dim` elements, 4 vectors per thread; a contiguous
+// table is one row of any length.  A large table that few tokens touch is
+// zeroed by a launch of its own, whose waves end with their stores: 6.8 TB/s,
+// where spans that zero themselves reach 5.1 (614 MB: 92 and 125 us).
 constexpr int kZeroItems = 4;
-template <typename O, int VEC> __global__ void __launch_bounds__(256) embedding_zero_kernel(GradArgs a) {
-  const int64_t vecs = a.dim / VEC, all = a.rows * vecs;
+template <typename O, int VEC>
+__global__ void __launch_bounds__(256) embedding_zero_kernel(O *out, int64_t rows, int64_t dim,
+                                                             int64_t stride) {
+  const int64_t vecs = dim / VEC, all = rows * vecs;
   const int64_t turn = static_cast<int64_t>(gridDim.x) * 256 * kZeroItems;
-  O *const out = static_cast<O *>(a.out);
   float zero[VEC] = {};
   for (int64_t i0 = static_cast<int64_t>(blockIdx.x) * 256 * kZeroItems + threadIdx.x; i0 < all;
        i0 += turn) {
 #pragma unroll
     for (int u = 0; u < kZeroItems; ++u) {
       const int64_t i = i0 + 256 * u;
-      if (i < all)
-        store_f32<VEC>(out + (a.out_stride == a.dim ? i * VEC
-                                                    : i / vecs * a.out_stride + i % vecs * VEC),
-                       zero);
+      if (i < all) store_f32<VEC>(out + (rows == 1 ? i * VEC : i / vecs * stride + i % vecs * VEC), zero);
     }
   }
+  const int64_t end = vecs * VEC + threadIdx.x; // of a row that is no whole vectors
+  if (rows == 1 && blockIdx.x == 0 && end < dim) out[end] = static_cast<O>(0.0f);
 }
 
 // Places in order for the tokens of a workgroup that `here` marks, the k-th 64
@@ -822,43 +824,42 @@ __global__ void __launch_bounds__(256) embedding_few_kernel(GradArgs a) {
   }
 }
 
-// At most MOST tokens and a large table, zeroed before: a workgroup per token,
-// which goes on if no earlier token is the same, lists those that are and sums
-// their row.  All tokens stay in its registers while it takes its tokens in
-// turn.
+// At most MOST tokens and a large table, zeroed before: a workgroup per token
+// and slice of the columns, which ends if an earlier token is the same, or else
+// lists those that are and sums its slice of their row.
 template <typename T, typename O, int VEC, int MOST>
-__global__ void __launch_bounds__(256) embedding_token_kernel(GradArgs a) {
+__global__ void __launch_bounds__(256) embedding_token_kernel(GradArgs a, int64_t slice) {
   constexpr int kEach = MOST / 256;
-  __shared__ uint32_t all[MOST];
+  __shared__ uint32_t token_row;
   __shared__ uint16_t same[MOST];
   __shared__ float joined[kSpanWaves][kWave * VEC];
   __shared__ int counts[kEach * kSpanWaves];
-  const int tid = threadIdx.x, wave_first = tid / kWave * kWave;
+  const int tid = threadIdx.x, wave_first = tid / kWave * kWave, t = blockIdx.x;
   uint32_t row[kEach];
   token_rows(a, tid, 256, row);
 #pragma unroll
-  for (int k = 0; k < kEach; ++k) all[k * 256 + tid] = row[k];
+  for (int k = 0; k < kEach; ++k)
+    if (k * 256 + tid == t) token_row = row[k];
   __syncthreads();
-  const int wide = hub_lanes(static_cast<uint32_t>(a.dim / VEC));
-  for (int t = blockIdx.x; t < a.count; t += gridDim.x) {
-    const uint32_t mine = all[t];
-    if (mine == static_cast<uint32_t>(a.rows)) continue;
-    uint64_t here[kEach];
-    bool before = false;
+  const uint32_t mine = token_row;
+  if (mine == static_cast<uint32_t>(a.rows)) return;
+  uint64_t here[kEach];
+  bool before = false;
 #pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-      here[k] = ballot(row[k] == mine);
-      const int ahead = t - (k * 256 + wave_first); // of these 64, how many come before t
-      before = before || (ahead >= kWave ? here[k] != 0
-                                         : ahead > 0 && (here[k] & ((uint64_t(1) << ahead) - 1)) != 0);
-    }
-    if (__syncthreads_or(before)) continue; // also: the row before has been summed
-    const int n = place_marked<kEach>(
-        counts, here, [&](int k, int at) { same[at] = static_cast<uint16_t>(k * 256 + tid); });
-    __syncthreads();
-    sum_hub<T, O, VEC>(
-        a, joined, wide, mine, [&](int i) { return static_cast<uint32_t>(same[i]); }, 0, n, 0, a.dim);
+  for (int k = 0; k < kEach; ++k) {
+    here[k] = ballot(row[k] == mine);
+    const int ahead = t - (k * 256 + wave_first); // of these 64, how many come before t
+    before = before || (ahead >= kWave ? here[k] != 0
+                                       : ahead > 0 && (here[k] & ((uint64_t(1) << ahead) - 1)) != 0);
   }
+  if (__syncthreads_or(before)) return;
+  const int n = place_marked<kEach>(
+      counts, here, [&](int k, int at) { same[at] = static_cast<uint16_t>(k * 256 + tid); });
+  __syncthreads();
+  const int64_t begin = blockIdx.y * slice;
+  sum_hub<T, O, VEC>(
+      a, joined, hub_lanes(static_cast<uint32_t>(a.dim / VEC)), mine,
+      [&](int i) { return static_cast<uint32_t>(same[i]); }, 0, n, begin, min(begin + slice, a.dim));
 }
 
 // ---- host ----------------------------------------------------------------------
@@ -897,8 +898,8 @@ GradLayout grad_layout(int64_t count, int64_t rows, int64_t dim) {
     l.spans = ceil_div64(rows, l.span);
   };
   cut(1024);
-  if (count <= kFewMost && count * dim <= kFewElements &&
-      (l.large || count * l.spans <= kFewReads))
+  if (count * dim <= kFewElements && (l.large ? count <= kLargeFewMost
+                                              : count <= kFewMost && count * l.spans <= kFewReads))
     return l;
   cut(2048);
   l.tile = count <= int64_t(kSmallTile) * kMostSmallTiles ? kSmallTile : kLargeTile;
@@ -936,6 +937,18 @@ template <typename T, int VEC> int32_t run_spans(const GradArgs &a, void *stream
   return go(embedding_span_kernel<T, VEC, 64>, 64);
 }
 
+template <typename O, int VEC> int32_t zero_table(const GradArgs &a, void *stream) {
+  auto go = [&](auto kernel, int64_t rows, int64_t vecs, int64_t dim) {
+    const int64_t blocks = std::max<int64_t>(1, ceil_div64(rows * vecs, 256 * kZeroItems));
+    return launch(kernel, dim3(std::min(blocks, kMostBlocks)), dim3(256), stream,
+                  static_cast<O *>(a.out), rows, dim, a.out_stride);
+  };
+  constexpr int kWhole = 16 / sizeof(O);
+  if ((a.out_stride == a.dim || a.rows == 1) && aligned_to(a.out, 16))
+    return go(embedding_zero_kernel<O, kWhole>, 1, a.rows * a.dim / kWhole, a.rows * a.dim);
+  return go(embedding_zero_kernel<O, VEC>, a.rows, a.dim / VEC, a.dim);
+}
+
 template <typename T, typename O, int VEC> int32_t grad_vec(GradArgs a, void *stream) {
   if (a.tiles == 0) {
     auto go = [&](auto kernel, int64_t blocks) {
@@ -945,13 +958,16 @@ template <typename T, typename O, int VEC> int32_t grad_vec(GradArgs a, void *st
       return a.count <= 1024   ? go(embedding_few_kernel<T, O, VEC, 1024>, a.spans)
              : a.count <= 4096 ? go(embedding_few_kernel<T, O, VEC, 4096>, a.spans)
                                : go(embedding_few_kernel<T, O, VEC, kFewMost>, a.spans);
-    const int64_t blocks = ceil_div64(a.rows * (a.dim / VEC), 256 * kZeroItems);
-    const int32_t rc = go(embedding_zero_kernel<O, VEC>, std::min(blocks, kMostBlocks));
+    const int32_t rc = zero_table<O, VEC>(a, stream);
     if (rc != SPORDER_OK || a.count == 0) return rc;
-    const int64_t turns = std::min(a.count, kFewBlocks);
-    return a.count <= 1024   ? go(embedding_token_kernel<T, O, VEC, 1024>, turns)
-           : a.count <= 4096 ? go(embedding_token_kernel<T, O, VEC, 4096>, turns)
-                             : go(embedding_token_kernel<T, O, VEC, kFewMost>, turns);
+    const int64_t vecs = a.dim / VEC, wide = hub_lanes(static_cast<uint32_t>(vecs));
+    const int64_t pieces = ceil_div64(vecs, wide);
+    const int64_t slice = ceil_div64(pieces, std::min(pieces, kTokenSlices)) * wide * VEC;
+    auto sum = [&](auto kernel) {
+      return launch(kernel, dim3(a.count, ceil_div64(a.dim, slice)), dim3(256), stream, a, slice);
+    };
+    return a.count <= 512 ? sum(embedding_token_kernel<T, O, VEC, 512>)
+                          : sum(embedding_token_kernel<T, O, VEC, kLargeFewMost>);
   }
   int32_t rc = a.tile == kSmallTile
                    ? launch(embedding_tile_kernel<kSmallTile>, dim3(a.tiles),

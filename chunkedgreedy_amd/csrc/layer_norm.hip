@@ -96,6 +96,10 @@ __device__ __forceinline__ void load_vector(const void *p, int type, int64_t dim
   });
 }
 
+// A row stays in the registers of its L lanes from its one read to its one
+// write; the variance is a second sum over the registers, so that a large mean
+// cancels nothing.  Bound by memory: 2.4 million rows of 128 floats in 485 us,
+// 2.53 GB at 5.2 TB/s; 64 rows of 512 16-bit elements take 3.6 us.
 template <typename T, bool LOOSE, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
   constexpr int kGroups = norm_block(L) / L;
@@ -160,7 +164,8 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_kernel(NormArgs a) {
   }
 }
 
-// Rows that no workgroup's registers hold: three passes over each.
+// Rows that no workgroup's registers hold: three passes over each.  Bound by
+// the passes, which L2 does not always hold: no figure here is near a copy's.
 template <typename T> __global__ void __launch_bounds__(1024) layer_norm_long_kernel(NormArgs a) {
   __shared__ float shared[2][1][1024 / kWave];
   RowSum<1024, 1> row_sum{shared};
@@ -197,6 +202,8 @@ template <typename T> __global__ void __launch_bounds__(1024) layer_norm_long_ke
 // workgroup are added up at the end and the workgroup writes one row of
 // partial sums.  No atomics: the order of every sum is fixed by the grid.  The
 // next row is on its way while a row is worked on, where registers allow.
+// Bound by memory: 16,384 rows of 4096 16-bit elements in 90 us, 403 MB at 4.5
+// TB/s; 1,000,003 of 100 floats in 238 us, 5.0 TB/s.
 template <typename T, bool LOOSE, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGradArgs a) {
   constexpr int kGroups = norm_block(L) / L;
@@ -344,7 +351,8 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
 }
 
 // Rows that no workgroup's registers hold: two passes over each, the column
-// sums kept in the workgroup's partial row (each thread its own columns).
+// sums kept in the workgroup's partial row (each thread its own columns):
+// 100 million elements in rows of 24,001 take 560 us with 16 bits, 710 with 32.
 template <typename T>
 __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(NormGradArgs a) {
   __shared__ float shared[2][2][1024 / kWave];
@@ -381,7 +389,7 @@ __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(NormGradArgs
 }
 
 // Column sums of the partial rows: 64 columns per workgroup, 16 threads per
-// column over interleaved rows, added up in LDS.
+// column over interleaved rows, added up in LDS: 6 us for 1,024 rows of 8,192.
 constexpr int kSumRows = 16;
 __global__ void __launch_bounds__(kWave *kSumRows)
     norm_column_sum_kernel(const float *partial, int64_t count, int64_t dim, void *dweight,

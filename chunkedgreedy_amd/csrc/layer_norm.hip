@@ -286,9 +286,12 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
     if (kAhead) fetch_next(row + stride);
 #pragma unroll
     for (int c = 0; c < C; ++c) {
+      const int col = (c * L + lane) * VEC;
 #pragma unroll
       for (int i = 0; i < VEC; ++i) {
-        h[c][i] = (h[c][i] - mean) * rstd; // past the row's end meets a dy of 0 only
+        // Past the row's end h is 0: -mean rstd may pass 32 bits where no h of
+        // the row does, and a dy of 0 times infinity is not 0.
+        h[c][i] = (h[c][i] - mean) * (col + (LOOSE ? i : 0) < a.dim ? rstd : 0.0f);
         dw[c][i] += g[c][i] * h[c][i];
         db[c][i] += g[c][i];
         g[c][i] *= w[c][i];

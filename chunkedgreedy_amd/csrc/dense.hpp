@@ -172,6 +172,13 @@ template <int L> __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
+// The largest of theirs (of NaN and a number, the number).
+template <int L> __device__ __forceinline__ float group_max(float v) {
+#pragma unroll
+  for (int j = 1; j < L; j <<= 1) v = fmaxf(v, lane_xor_f32(v, j));
+  return v;
+}
+
 constexpr bool type_known(int32_t t) { return t >= SPORDER_TYPE_F32 && t <= SPORDER_TYPE_F16; }
 constexpr int type_bytes(int32_t t) { return t == SPORDER_TYPE_F32 ? 4 : 2; }
 

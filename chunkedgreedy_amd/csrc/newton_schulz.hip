@@ -7,14 +7,23 @@
 // c s^5, and the singular vectors stay.
 //
 // Products.  The matrix units multiply 32-bit floats at a sixteenth of the rate of
-// 16-bit ones, so every operand x is kept as two 16-bit halves of x 2^11:
-// hi = fl16(x 2^11) and lo = fl16(x 2^11 - hi), together 22 bits and a sign,
-// and a product is hi hi + hi lo + lo hi with 32-bit accumulation: three
-// matrix products, and lo lo (2^-22 of the result) left out.  All values are
-// at most 31 in magnitude (singular values start at most 1 and the entry
-// refuses coefficients that take X's, A's or B's past 31), so hi does not
-// overflow, and lo keeps absolute steps of 2^-35 where the largest singular
-// value starts at most 1.
+// 16-bit ones, so an operand x is two 16-bit halves, hi = fl16(x / u) and lo =
+// fl16(x / u - hi), together 22 bits and a sign, and a product is hi hi + hi lo +
+// lo hi with 32-bit accumulation: three matrix products, and lo lo (2^-22 of the
+// result) left out.  X itself is held in 32 bits: only B X is made of halves.
+//
+// Units.  Small singular values grow by |a| a step, and a small row or column
+// keeps its own size beside large ones, so steps that are absolute, or relative
+// to the whole matrix, would grow into the result.  Every operand row has a unit
+// u of its own, a power of two with 2^14 <= bound / u < 2^15 for a bound on the
+// row's norm: nothing passes 2^16, and lo is exact down to 2^-39 of the bound.
+// With q(t) = a + b t + c t^2 the update is q(A) X = X q(X^T X), so a step
+// multiplies the norm of a row or column of X by at most the maximum g of |q(t)|,
+// t = s^2, over the singular values s in [0, S] that occur, and leaves it at most
+// S; A = X X^T has rows of at most S times X's, B = X (X^T (b + c A)) of at most h
+// times, the maximum of |s (b + c s^2)|.  S, g and h follow from the coefficients
+// and the number of steps, the first bounds from the largest elements of X's rows
+// and columns.
 //
 // Layout.  Operands are stored as the matrix units read them: blocks of 32
 // rows by 16 columns, each 64 lanes of 8 halves (lane l holds row l % 32,
@@ -37,8 +46,7 @@ using f16x8 = f16_t __attribute__((ext_vector_type(8)));
 using u32x4 = uint32_t __attribute__((ext_vector_type(4)));
 using f32x16 = float __attribute__((ext_vector_type(16)));
 
-constexpr float kScale = 2048.0f; // of the stored halves
-constexpr double kMostValue = 31.0;
+constexpr double kMostValue = 31.0; // of singular values, A's and B's: past it nothing converges
 constexpr int kBlock = 256;
 constexpr int kPad = 128; // rows and columns are padded to multiples of it
 constexpr int kStageRow = 40; // halves per row of a wave's transposing buffer
@@ -52,7 +60,15 @@ struct OrthoArgs {
   int tall;                     // X = G^T
   double eps;
   float a, b, c;
+  float root_m, root_n;         // a little more than the roots of m and n
+  float most, growth;           // S and g
+  float now, next;              // growth of the norms up to this step, and past it
+  float gram_unit, poly_unit;   // powers of two, at least S and h: units of A and B beside X's
+  int row_strips, col_strips;   // of g, for its norm
   double *partial;              // [batch][kNormBlocks]
+  float *row_part, *col_part;   // [batch][col_strips][g's rows], [batch][row_strips][g's columns]
+  float *row_bound, *col_bound; // [batch][mp], [batch][np] of the first X
+  float4 *state;                // X by blocks of 32 x 32, in the order of a wave's results
   uint4 *x, *xt, *xt_next, *gram, *poly; // packed operands, one after another per matrix
 };
 
@@ -61,7 +77,22 @@ __host__ __device__ constexpr int64_t packed_units(int64_t rows, int64_t cols) {
   return rows * cols / 4; // two halves of 2 bytes each: 4 bytes per element
 }
 
-// The halves of two scaled values, hi and lo each packed in a word.
+// The unit of a row whose norm is at most `bound`; the least, of bounds up to
+// 2^-99, is 2^-114.
+__device__ __forceinline__ float unit_above(float bound) {
+  return __builtin_bit_cast(float, (max(__builtin_bit_cast(uint32_t, bound) >> 23, 27u) - 14) << 23);
+}
+// 1 / u for a power of two.
+__device__ __forceinline__ float inverse(float u) {
+  return __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, u));
+}
+// The bound on a row or column of the first X from its largest element before
+// the scaling and its length's root.
+__device__ __forceinline__ float first_bound(float most, double scale, float root) {
+  return fminf(1.0f, static_cast<float>(most * scale) * root); // NaN: 1
+}
+
+// The halves of two values in their units, hi and lo each packed in a word.
 __device__ __forceinline__ void split_halves(float x, float y, uint32_t &hi, uint32_t &lo) {
   using f16x2 = f16_t __attribute__((ext_vector_type(2)));
   using f32x2 = float __attribute__((ext_vector_type(2)));
@@ -75,6 +106,22 @@ __device__ __forceinline__ void split_halves(float x, float y, uint32_t &hi, uin
   lo = __builtin_bit_cast(uint32_t, l);
 }
 
+// A wave's 32 x 32 block with row i0 and column j0: lane l holds column l % 32,
+// rows 8 q + 4 (l / 32) + e in v[4 q + e].
+__device__ __forceinline__ int block_row(int r) { return 8 * (r / 4) + 4 * (lane_id() / 32) + r % 4; }
+
+// The units of a lane's rows, from their bounds.
+__device__ __forceinline__ void row_units(const float4 (&bounds)[4], float growth, float most,
+                                          float (&u)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    u[4 * q] = unit_above(fminf(most, bounds[q].x * growth));
+    u[4 * q + 1] = unit_above(fminf(most, bounds[q].y * growth));
+    u[4 * q + 2] = unit_above(fminf(most, bounds[q].z * growth));
+    u[4 * q + 3] = unit_above(fminf(most, bounds[q].w * growth));
+  }
+}
+
 __device__ __forceinline__ uint2 *col_place(uint4 *p, int k_blocks, int i0, int j0, int q,
                                             int plane, int lane) {
   const int64_t block = static_cast<int64_t>(j0 / 32) * k_blocks + i0 / 16 + q / 2;
@@ -82,15 +129,25 @@ __device__ __forceinline__ uint2 *col_place(uint4 *p, int k_blocks, int i0, int 
   return reinterpret_cast<uint2 *>(unit) + lane / 32;
 }
 
-// Stores one wave's 32 x 32 block with row i0 and column j0, scaled: lane l
-// holds column l % 32, rows 8 q + 4 (l / 32) + e in v[4 q + e].  by_col
-// receives it with columns as operand rows, by_row (if not null) with its own
-// rows, which 8 neighbouring columns of a row take a turn through LDS for
-// (`stage`, which may be the block's own place in by_row); k_col and k_row
-// are their numbers of 16-column blocks.
-__device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col, int k_col,
-                                            uint4 *by_row, int k_row, int i0, int j0,
-                                            uint16_t *stage) {
+// Stores a block, in units of its columns, with columns as operand rows; k_col
+// is the operand's number of 16-column blocks.
+__device__ __forceinline__ void store_by_col(const float (&v)[16], uint4 *by_col, int k_col, int i0,
+                                             int j0) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint2 hi, lo;
+    split_halves(v[4 * q], v[4 * q + 1], hi.x, lo.x);
+    split_halves(v[4 * q + 2], v[4 * q + 3], hi.y, lo.y);
+    *col_place(by_col, k_col, i0, j0, q, 0, lane_id()) = hi;
+    *col_place(by_col, k_col, i0, j0, q, 1, lane_id()) = lo;
+  }
+}
+
+// The same in units of its rows, with its own rows as operand rows: 8
+// neighbouring columns of a row take a turn through LDS (`stage`, which may be
+// the block's own place in by_row).
+__device__ __forceinline__ void store_by_row(const float (&v)[16], uint4 *by_row, int k_row, int i0,
+                                             int j0, uint16_t *stage) {
   const int lane = lane_id();
   uint32_t half[2][8];
   u32x4 held[2][2];
@@ -99,17 +156,13 @@ __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col,
 #pragma unroll
   for (int plane = 0; plane < 2; ++plane) {
     const uint32_t(&h)[8] = half[plane];
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      *col_place(by_col, k_col, i0, j0, q, plane, lane) = make_uint2(h[2 * q], h[2 * q + 1]);
-    if (!by_row) continue;
     // A word holds rows r and r + 1 of a column; with the neighbouring
     // column's, an even lane makes row r's word of both and an odd one r + 1's.
 #pragma unroll
     for (int r = 0; r < 16; r += 2) {
       const uint32_t word = __builtin_amdgcn_perm(lane_xor_u32(h[r / 2], 1), h[r / 2],
                                                   lane & 1 ? 0x03020706 : 0x05040100);
-      const int row = 8 * (r / 4) + 4 * (lane / 32) + r % 4 + (lane & 1);
+      const int row = block_row(r) + (lane & 1);
       *reinterpret_cast<uint32_t *>(stage + row * kStageRow + (lane % 32 & ~1)) = word;
     }
     wave_lds_order();
@@ -119,7 +172,6 @@ __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col,
                                                         8 * (lane / 32 + 2 * s));
     wave_lds_order();
   }
-  if (!by_row) return;
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     const int part = lane / 32 + 2 * s; // 8 columns from 8 part
@@ -131,72 +183,91 @@ __device__ __forceinline__ void store_block(const float (&v)[16], uint4 *by_col,
   }
 }
 
-// A block as store_block put it into by_col, to be fetched early.
+// X's block in the state, float4 q of lane l.
+__device__ __forceinline__ float4 *state_place(const OrthoArgs &a, int64_t z, int i0, int j0, int q) {
+  const int64_t block = static_cast<int64_t>(i0 / 32) * (a.np / 32) + j0 / 32;
+  return a.state + z * (static_cast<int64_t>(a.mp) * a.np / 4) + (block * 4 + q) * kWave + lane_id();
+}
+
+// What a product's block is combined with, to be fetched early: hi and lo as
+// store_by_col put them, or the state, and the bounds of its rows and column.
 struct HeldBlock {
-  uint2 word[2][4]; // hi and lo
+  uint4 word[4];
+  float4 rows[4];
+  float column;
 };
-__device__ __forceinline__ HeldBlock fetch_block(const uint4 *by_col, int k_col, int i0, int j0) {
-  HeldBlock b;
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-      b.word[h][q] = *col_place(const_cast<uint4 *>(by_col), k_col, i0, j0, q, h, lane_id());
-  }
-  return b;
-}
-// v <- x (its scaled values) + y v.
-__device__ __forceinline__ void combine_block(const HeldBlock &b, float x, float y, float (&v)[16]) {
-  using f16x4 = f16_t __attribute__((ext_vector_type(4)));
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const f16x4 hi = __builtin_bit_cast(f16x4, b.word[0][q]);
-    const f16x4 lo = __builtin_bit_cast(f16x4, b.word[1][q]);
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      v[4 * q + e] = x * (static_cast<float>(hi[e]) + static_cast<float>(lo[e])) + y * v[4 * q + e];
-  }
-}
 
 // ---- norm and packing ------------------------------------------------------------
 
 constexpr int kNormBlocks = 256; // partial sums per matrix, at most
 constexpr int kNormThreads = 512;
 
-// Sums of squares in 64 bits: no overflow or underflow at any finite input.
-// The additions go to four sums so that four loads are under way per thread:
-// 4096 x 4096 floats in 24 us, 2.8 TB/s.
+constexpr int kStripCols = 512; // columns of a workgroup's strip: 8 per lane
+constexpr int kStripRows = 32;  // and its rows, at least
+
+// Sums of squares in 64 bits (no overflow or underflow at any finite input) and
+// the largest elements of rows and columns, for a strip of rows and columns per
+// workgroup: a row per wave, four of them under way.  4096 x 4096 floats in 18
+// us, 3.8 TB/s.
 template <typename T, int VEC>
 __global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(OrthoArgs a) {
+  constexpr int kParts = kStripCols / kWave / VEC, kWaves = kNormThreads / kWave, kRows = 4;
   const int64_t z = blockIdx.y, rows = a.tall ? a.n : a.m, cols = a.tall ? a.m : a.n;
+  const int col_strip = blockIdx.x % a.col_strips, row_strip = blockIdx.x / a.col_strips;
+  const int64_t per = ceil_div64(rows, a.row_strips);
+  const int64_t first = row_strip * per, last = min(first + per, rows);
+  const int64_t col0 = static_cast<int64_t>(col_strip) * kStripCols;
+  const int lane = lane_id(), wave = threadIdx.x / kWave;
   const T *const g = static_cast<const T *>(a.g) + z * a.g_batch;
-  const int64_t vecs = cols / VEC, per = ceil_div64(rows * vecs, gridDim.x);
-  const int64_t first = blockIdx.x * per, last = min(first + per, rows * vecs);
-  double s[4] = {};
-  int64_t at = first + threadIdx.x;
-  int64_t row = at / vecs, col = at % vecs;
-  for (; at < last; at += 4 * kNormThreads) {
-    float v[4][VEC];
+  float *const row_part = a.row_part + (z * a.col_strips + col_strip) * rows;
+  float col_most[kParts][VEC] = {};
+  double s[kRows] = {};
+  for (int64_t row = first + wave; row < last; row += kRows * kWaves) {
+    float v[kRows][kParts][VEC];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (at + k * kNormThreads < last) {
-        load_f32<VEC>(g + row * a.g_stride + col * VEC, v[k]);
-      } else {
+    for (int u = 0; u < kRows; ++u) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[k][i] = 0.0f;
+      for (int p = 0; p < kParts; ++p) {
+        const int64_t col = col0 + (p * kWave + lane) * VEC;
+        if (row + u * kWaves < last && col < cols) {
+          load_f32<VEC>(g + (row + u * kWaves) * a.g_stride + col, v[u][p]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) v[u][p][i] = 0.0f;
+        }
       }
-      col += kNormThreads;
-      if (col >= vecs) row += col / vecs, col %= vecs;
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
+    for (int u = 0; u < kRows; ++u) {
+      float most = 0.0f;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) s[k] += static_cast<double>(v[k][i]) * v[k][i];
+      for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          s[u] += static_cast<double>(v[u][p][i]) * v[u][p][i];
+          most = fmaxf(most, fabsf(v[u][p][i]));
+          col_most[p][i] = fmaxf(col_most[p][i], fabsf(v[u][p][i]));
+        }
+      }
+      most = group_max<kWave>(most);
+      if (lane == 0 && row + u * kWaves < last) row_part[row + u * kWaves] = most;
     }
   }
   __shared__ double part[kNormThreads];
+  __shared__ float most[kWaves][kStripCols];
   part[threadIdx.x] = (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+  for (int p = 0; p < kParts; ++p) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) most[wave][(p * kWave + lane) * VEC + i] = col_most[p][i];
+  }
   __syncthreads();
+  static_assert(kNormThreads == kStripCols);
+  float m = 0.0f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) m = fmaxf(m, most[w][threadIdx.x]);
+  if (col0 + threadIdx.x < cols)
+    a.col_part[(z * a.row_strips + row_strip) * cols + col0 + threadIdx.x] = m;
   for (int k = kNormThreads / 2; k > 0; k /= 2) {
     if (threadIdx.x < k) part[threadIdx.x] += part[threadIdx.x + k];
     __syncthreads();
@@ -204,25 +275,42 @@ __global__ void __launch_bounds__(kNormThreads) ortho_norm_kernel(OrthoArgs a) {
   if (threadIdx.x == 0) a.partial[z * kNormBlocks + blockIdx.x] = part[0];
 }
 
-// Packs X = G / (|G| + eps), 64 x 64 per workgroup, a 32 x 32 block per wave:
-// 4096 x 4096 floats in 34 us, 201 MB at 5.9 TB/s.
+// Packs X = G / (|G| + eps), 64 x 64 per workgroup, a 32 x 32 block per wave,
+// after the bounds of the rows and columns that it meets: 4096 x 4096 floats in
+// 57 us, 268 MB at 4.7 TB/s.
 template <typename T>
-__global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int norm_blocks) {
+__global__ void __launch_bounds__(kBlock, 6) ortho_pack_kernel(OrthoArgs a, int norm_blocks) {
   __shared__ __attribute__((aligned(16))) uint16_t stage[4][32 * kStageRow];
+  __shared__ float most[2][128];
+  __shared__ __attribute__((aligned(16))) float bound[128]; // 64 rows, then 64 columns
   const int64_t z = blockIdx.y;
-  const int wave = threadIdx.x / kWave, lane = lane_id();
+  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   const int across = a.np / 64;
-  const int i0 = blockIdx.x / across * 64 + wave / 2 * 32;
-  const int j0 = blockIdx.x % across * 64 + wave % 2 * 32;
+  const int tile_i = blockIdx.x / across * 64, tile_j = blockIdx.x % across * 64;
+  const int i0 = tile_i + wave / 2 * 32, j0 = tile_j + wave % 2 * 32;
   const int j = j0 + lane % 32;
   const T *const g = static_cast<const T *>(a.g) + z * a.g_batch;
   float v[16];
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int i = i0 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+    const int i = i0 + block_row(r);
     v[r] = 0.0f;
     if (i < a.m && j < a.n)
       v[r] = static_cast<float>(g[a.tall ? j * a.g_stride + i : i * a.g_stride + j]);
+  }
+  // Two threads for each of the tile's rows and columns.
+  const int item = tid % 128;
+  const bool column = item >= 64, g_column = column != static_cast<bool>(a.tall);
+  const int64_t at = column ? tile_j + item - 64 : tile_i + item, all = column ? a.n : a.m;
+  if (at < all) {
+    const int strips = g_column ? a.row_strips : a.col_strips;
+    const float *const from = (g_column ? a.col_part : a.row_part) + z * strips * all + at;
+    float m = 0.0f;
+#pragma unroll 8
+    for (int k = tid / 128; k < strips; k += 2) m = fmaxf(m, from[k * all]);
+    most[tid / 128][item] = m;
+  } else {
+    most[tid / 128][item] = 0.0f;
   }
   double square = 0.0;
 #pragma unroll
@@ -230,60 +318,139 @@ __global__ void __launch_bounds__(kBlock) ortho_pack_kernel(OrthoArgs a, int nor
     if (lane + k * kWave < norm_blocks) square += a.partial[z * kNormBlocks + lane + k * kWave];
 #pragma unroll
   for (int k = 1; k < kWave; k <<= 1) square += __shfl_xor(square, k);
-  const double scale = static_cast<double>(kScale) / (sqrt(square) + a.eps);
+  const double scale = 1.0 / (sqrt(square) + a.eps);
+  __syncthreads();
+  if (tid < 128) {
+    bound[item] = first_bound(fmaxf(most[0][item], most[1][item]), scale, column ? a.root_m : a.root_n);
+    if (!column && tile_j == 0) a.row_bound[z * a.mp + tile_i + item] = bound[item];
+    if (column && tile_i == 0) a.col_bound[z * a.np + tile_j + item - 64] = bound[item];
+  }
+  __syncthreads();
 #pragma unroll
   for (int r = 0; r < 16; ++r) v[r] = static_cast<float>(v[r] * scale);
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *state_place(a, z, i0, j0, q) = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
   const int64_t units = packed_units(a.mp, a.np);
-  store_block(v, a.xt + z * units, a.mp / 16, a.x + z * units, a.np / 16, i0, j0, stage[wave]);
+  float u[16], w[16];
+  const float col = inverse(unit_above(bound[64 + j0 - tile_j + lane % 32]));
+#pragma unroll
+  for (int r = 0; r < 16; ++r) w[r] = v[r] * col;
+  store_by_col(w, a.xt + z * units, a.mp / 16, i0, j0);
+  float4 rows[4];
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    rows[q] = *reinterpret_cast<const float4 *>(bound + i0 - tile_i + block_row(4 * q));
+  row_units(rows, 1.0f, 1.0f, u);
+#pragma unroll
+  for (int r = 0; r < 16; ++r) w[r] = v[r] * inverse(u[r]);
+  store_by_row(w, a.x + z * units, a.np / 16, i0, j0, stage[wave]);
 }
 
 // ---- products ----------------------------------------------------------------------
 
 enum Product { kGram, kPoly, kUpdate, kLast };
 
-// Writes a block of the result, unscaled.
+// Writes a block of the result.
 template <typename T>
 __device__ __forceinline__ void write_block(const OrthoArgs &a, int64_t z, int i0, int j0,
                                             const float (&v)[16]) {
   const int64_t j = j0 + lane_id() % 32;
 #pragma unroll
   for (int r = 0; r < 16; ++r) {
-    const int64_t i = i0 + 8 * (r / 4) + 4 * (lane_id() / 32) + r % 4;
+    const int64_t i = i0 + block_row(r);
     if (i < a.m && j < a.n)
       static_cast<T *>(a.out)[z * a.m * a.n + (a.tall ? j * a.m + i : i * a.n + j)] =
-          static_cast<T>(v[r] * (1.0f / kScale));
+          static_cast<T>(v[r]);
   }
 }
 
 // What a product's block (i0, j0) is combined with, where it is.
 template <int WHAT>
 __device__ __forceinline__ HeldBlock fetch_old(const OrthoArgs &a, int64_t z, int i0, int j0) {
-  if constexpr (WHAT == kGram) return {};
-  const uint4 *const from = WHAT == kPoly ? a.gram + z * packed_units(a.mp, a.mp)
-                                          : a.xt + z * packed_units(a.mp, a.np);
-  return fetch_block(from, a.mp / 16, i0, j0);
+  HeldBlock old{};
+  const float *const rows = a.row_bound + z * a.mp;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) old.rows[q] = *reinterpret_cast<const float4 *>(rows + i0 + block_row(4 * q));
+  old.column = (WHAT == kGram || WHAT == kPoly ? rows : a.col_bound + z * a.np)[j0 + lane_id() % 32];
+  if constexpr (WHAT == kPoly) {
+    uint4 *const from = a.gram + z * packed_units(a.mp, a.mp);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint2 hi = *col_place(from, a.mp / 16, i0, j0, q, 0, lane_id());
+      const uint2 lo = *col_place(from, a.mp / 16, i0, j0, q, 1, lane_id());
+      old.word[q] = make_uint4(hi.x, hi.y, lo.x, lo.y);
+    }
+  } else if constexpr (WHAT == kUpdate || WHAT == kLast) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      old.word[q] = *reinterpret_cast<const uint4 *>(state_place(a, z, i0, j0, q));
+  }
+  return old;
 }
 
-// The epilogue of a product for one wave's block: v holds C scaled twice.
+// The epilogue of a product for one wave's block: v holds P Q^T in their units,
+// so that row i's unit times column j's makes it whole.
 template <int WHAT, typename T>
 __device__ __forceinline__ void finish_block(const OrthoArgs &a, int64_t z, bool mirror, int i0,
-                                             int j0, float (&v)[16], const HeldBlock &old,
+                                             int j0, const float (&v)[16], const HeldBlock &old,
                                              uint16_t *stage) {
   const int64_t xu = packed_units(a.mp, a.np), mu = packed_units(a.mp, a.mp);
   const int km = a.mp / 16, kn = a.np / 16;
-  if constexpr (WHAT == kGram) {
-#pragma unroll
-    for (int r = 0; r < 16; ++r) v[r] *= 1.0f / kScale;
-  } else {
-    combine_block(old, WHAT == kPoly ? a.b : a.a, (WHAT == kPoly ? a.c : 1.0f) / kScale, v);
-  }
+  const float uj = unit_above(fminf(a.most, old.column * a.now));
+  float u[16], w[16];
+  row_units(old.rows, a.now, a.most, u);
   if constexpr (WHAT == kGram || WHAT == kPoly) {
     uint4 *const to = (WHAT == kGram ? a.gram : a.poly) + z * mu;
-    store_block(v, to, km, mirror ? to : nullptr, km, i0, j0, stage);
-  } else if constexpr (WHAT == kUpdate) {
-    store_block(v, a.xt_next + z * xu, km, a.x + z * xu, kn, i0, j0, stage);
+    if constexpr (WHAT == kGram) { // A = v u uj, and the unit of A's row j is uj gram_unit
+      const float scale = 1.0f / a.gram_unit;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w[r] = v[r] * (u[r] * scale);
+    } else { // A = held uj gram_unit, A A = v u uj gram_unit^2, B's unit uj poly_unit
+      using f16x4 = f16_t __attribute__((ext_vector_type(4)));
+      const float unit = a.gram_unit / a.poly_unit;
+      const float b = a.b * unit, c = a.c * unit * a.gram_unit;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f16x4 hi = __builtin_bit_cast(f16x4, make_uint2(old.word[q].x, old.word[q].y));
+        const f16x4 lo = __builtin_bit_cast(f16x4, make_uint2(old.word[q].z, old.word[q].w));
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          w[4 * q + e] = b * (static_cast<float>(hi[e]) + static_cast<float>(lo[e])) +
+                         c * (v[4 * q + e] * u[4 * q + e]);
+      }
+    }
+    store_by_col(w, to, km, i0, j0);
+    if (!mirror) return;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] *= uj * inverse(u[r]);
+    store_by_row(w, to, km, i0, j0, stage);
   } else {
-    write_block<T>(a, z, i0, j0, v);
+    float x[16];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t held[4] = {old.word[q].x, old.word[q].y, old.word[q].z, old.word[q].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int r = 4 * q + e;
+        x[r] = a.a * __builtin_bit_cast(float, held[e]) + v[r] * (u[r] * a.poly_unit) * uj;
+      }
+    }
+    if constexpr (WHAT == kLast) {
+      write_block<T>(a, z, i0, j0, x);
+      return;
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      *state_place(a, z, i0, j0, q) = make_float4(x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]);
+    const float next = inverse(unit_above(fminf(a.most, old.column * a.next)));
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] = x[r] * next;
+    store_by_col(w, a.xt_next + z * xu, km, i0, j0);
+    row_units(old.rows, a.next, a.most, u);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] = x[r] * inverse(u[r]);
+    store_by_row(w, a.x + z * xu, kn, i0, j0, stage);
   }
 }
 
@@ -326,8 +493,9 @@ __device__ __forceinline__ void place_tile(int t, int down, int across, int rati
 //   kPoly:   P = Q = A;          writes B = b A + c C
 //   kUpdate: P = B, Q = X^T;     writes X = a X + C in both orders
 //   kLast:   the same to out, rounded to its type
-// Bound by the matrix units: an update of 4096 x 4096 in 359 us, 1.15 PFLOP/s of
-// 16-bit products, as a library's product of that size and type reaches.
+// Bound by the matrix units: an update of 4096 x 4096 in 376 us, 1.10 PFLOP/s of
+// 16-bit products, a library's product of that size and type 1.15; some 20 us are
+// the 134 MB of X in 32 bits, read and written.
 constexpr int kTileRows = 256, kTileCols = 128;
 
 template <int WHAT, typename T>
@@ -414,7 +582,6 @@ __global__ void __launch_bounds__(kBlock, 2) ortho_product_kernel(OrthoArgs a) {
     }
   }
 
-  // The accumulators hold products of two scaled values.
   uint16_t *const stage = reinterpret_cast<uint16_t *>(&lds[0][0]) + wave * 32 * kStageRow;
   if (!live) return;
 #pragma unroll
@@ -436,8 +603,10 @@ __global__ void __launch_bounds__(kBlock, 2) ortho_product_kernel(OrthoArgs a) {
 // from memory (in the units' own order, so without LDS), four steps ahead; the
 // sums meet in LDS, a block of 32 x 32 for each of four waves.  A CU holds
 // eight such waves: eight per tile while there is a CU for each tile, else
-// four (1024 x 1536 in 1024: 24 us with eight, 19 with four).  Bound by latency:
-// products of 1024 x 1024 x 1536 take 12 to 19 us, some 6 of them to begin and end.
+// four (1024 x 1536 in 1024: 27 us with eight, 21 with four).  Products of 1024 x
+// 1024 x 1536 take 13 to 21 us.  An update of them is 384 tiles, one and a half
+// turns of the CUs, that read 240 MB out of L2 at 12 TB/s (39 MB past it), with
+// the matrix units busy in 28 % of the cycles.
 constexpr int kAhead = 4;
 
 // With first >= 0 they are the tiles of ortho_product_kernel from that one on,
@@ -546,6 +715,7 @@ __global__ void __launch_bounds__(WAVES *kWave) ortho_split_kernel(OrthoArgs a, 
 constexpr int kWholeWaves = 8;
 constexpr int kWholeBlocks = 2 * kWholeWaves;
 constexpr int kWholeUnits = kWholeBlocks * 32 * 32 / 4;
+constexpr int kWholeRows = 128, kWholeSides = kWholeRows + 512; // X's rows, and its columns after them
 
 // Whether every wave has at most one pair of neighbouring blocks of X (and of
 // the square A, which is no larger).
@@ -557,6 +727,7 @@ template <typename T>
 __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoArgs a, int steps) {
   __shared__ __attribute__((aligned(16))) uint4 x[kWholeUnits], xt[kWholeUnits];
   __shared__ double part[kWholeWaves];
+  __shared__ __attribute__((aligned(16))) float bound[kWholeSides], unit[2][kWholeSides];
   const int64_t z = blockIdx.x;
   const int wave = threadIdx.x / kWave, lane = lane_id();
   const int mb = a.mp / 32, nb = a.np / 32; // blocks down and across
@@ -568,19 +739,20 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
   const int blocks_x = xi < mb ? min(2, nb - xj) : 0, blocks_a = ai < mb ? min(2, mb - aj) : 0;
 
   const T *const g = static_cast<const T *>(a.g) + z * a.g_batch;
-  float va[2][16], vx[2][16]; // this wave's blocks of A or B, and of X, scaled
+  float va[2][16], vx[2][16]; // this wave's blocks of A or B, beside X's units, and of X
   double s = 0.0;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     const int j = (xj + t) * 32 + lane % 32;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-      const int i = xi * 32 + 8 * (r / 4) + 4 * (lane / 32) + r % 4;
+      const int i = xi * 32 + block_row(r);
       vx[t][r] = 0.0f;
       if (t < blocks_x && i < a.m && j < a.n)
         vx[t][r] = static_cast<float>(g[a.tall ? j * a.g_stride + i : i * a.g_stride + j]);
     }
   }
+  for (int i = threadIdx.x; i < kWholeSides; i += kWholeWaves * kWave) bound[i] = 0.0f;
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
 #pragma unroll
@@ -593,23 +765,71 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
   __syncthreads();
   s = 0.0;
   for (int w = 0; w < kWholeWaves; ++w) s += part[w];
-  const double scale = static_cast<double>(kScale) / (sqrt(s) + a.eps);
+  const double scale = 1.0 / (sqrt(s) + a.eps);
+
+  // The largest elements of rows and columns, as integers: positive floats order
+  // alike, and NaN is past them all.
+  auto largest = [&](int at, uint32_t v) { atomicMax(reinterpret_cast<uint32_t *>(bound) + at, v); };
+  auto magnitude = [&](int t, int r) { return __builtin_bit_cast(uint32_t, vx[t][r]) & 0x7fffffffu; };
+  if (blocks_x) {
+    // Rows: each exchange halves the registers, until one row is left per lane.
+    uint32_t most[16];
+    int row = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most[r] = max(magnitude(0, r), magnitude(1, r));
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int half = 8 >> k;
+      const bool upper = lane >> k & 1;
+      row += upper ? half : 0;
+#pragma unroll
+      for (int r = 0; r < half; ++r) {
+        const uint32_t low = most[r], high = most[r + half];
+        most[r] = max(upper ? high : low, lane_xor_u32(upper ? low : high, 1 << k));
+      }
+    }
+    largest(xi * 32 + block_row(row), max(most[0], lane_xor_u32(most[0], 16)));
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      uint32_t column = 0;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) column = max(column, magnitude(t, r));
+      if (t < blocks_x) largest(kWholeRows + (xj + t) * 32 + lane % 32, column);
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < kWholeSides; i += kWholeWaves * kWave) {
+    bound[i] = first_bound(bound[i], scale, i < kWholeRows ? a.root_n : a.root_m);
+    unit[0][i] = unit_above(bound[i]);
+  }
+  __syncthreads();
 
   // A block's place in x is its own until the barrier after: its stage.
-  auto store_x = [&](int t) {
+  auto store_x = [&](int t, const float *units) {
     uint4 *const place = x + (xi * kn + (xj + t) * 2) * 2 * kWave;
-    store_block(vx[t], xt, km, x, kn, xi * 32, (xj + t) * 32, reinterpret_cast<uint16_t *>(place));
+    const float column = inverse(units[kWholeRows + (xj + t) * 32 + lane % 32]);
+    float w[16];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) w[r] = vx[t][r] * column;
+    store_by_col(w, xt, km, xi * 32, (xj + t) * 32);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4 u = *reinterpret_cast<const float4 *>(units + xi * 32 + block_row(4 * q));
+      w[4 * q] = vx[t][4 * q] * inverse(u.x), w[4 * q + 1] = vx[t][4 * q + 1] * inverse(u.y);
+      w[4 * q + 2] = vx[t][4 * q + 2] * inverse(u.z), w[4 * q + 3] = vx[t][4 * q + 3] * inverse(u.w);
+    }
+    store_by_row(w, x, kn, xi * 32, (xj + t) * 32, reinterpret_cast<uint16_t *>(place));
   };
 #pragma unroll
   for (int t = 0; t < 2; ++t) {
     if (t >= blocks_x) continue;
 #pragma unroll
     for (int r = 0; r < 16; ++r) vx[t][r] = static_cast<float>(vx[t][r] * scale);
-    store_x(t);
+    store_x(t, unit[0]);
   }
   __syncthreads();
 
-  // acc = blocks (bi, bj) and (bi, bj + more) of P Q^T, scaled twice, operands
+  // acc = blocks (bi, bj) and (bi, bj + more) of P Q^T in their units, operands
   // of k blocks.
   f32x16 acc[2];
   auto product = [&](const uint4 *p, const uint4 *q, int k_blocks, int bi, int bj, int more) {
@@ -645,41 +865,72 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
       }
     }
   };
-  auto store_a = [&]() {
+  // A or B, whose rows have X's units times `unit`.
+  auto store_a = [&](float unit) {
     __syncthreads();
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-      if (t < blocks_a) store_block(va[t], x, km, nullptr, 0, ai * 32, (aj + t) * 32, nullptr);
+    for (int t = 0; t < 2; ++t) {
+      if (t >= blocks_a) continue;
+      float w[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) w[r] = va[t][r] * (1.0f / unit);
+      store_by_col(w, x, km, ai * 32, (aj + t) * 32);
+    }
     __syncthreads();
   };
 
+  float growth = 1.0f;
   for (int step = 0; step < steps; ++step) {
-    if (blocks_a) product(x, x, kn, ai, aj, blocks_a - 1);
+    const float *const now = unit[step & 1];
+    float *const next = unit[~step & 1];
+    growth = fminf(growth * a.growth, 0x1p100f);
+    // f(block, register, product times its row's unit) for the products of two
+    // blocks; their columns' units are left to f.
+    auto each = [&](const float4(&rows)[4], auto &&f) {
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
+      for (int t = 0; t < 2; ++t) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) va[t][r] = acc[t][r] * (1.0f / kScale);
+        for (int q = 0; q < 4; ++q) {
+          const float u[4] = {rows[q].x, rows[q].y, rows[q].z, rows[q].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) f(t, 4 * q + e, acc[t][4 * q + e] * u[e]);
+        }
+      }
+    };
+    auto fetch_units = [&](int row0, float4(&rows)[4]) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        rows[q] = *reinterpret_cast<const float4 *>(now + row0 + block_row(4 * q));
+    };
+    float4 units[4];
+    if (blocks_a) {
+      fetch_units(ai * 32, units);
+      product(x, x, kn, ai, aj, blocks_a - 1);
+      each(units, [&](int t, int r, float v) { va[t][r] = v; });
     }
-    store_a();
-    if (blocks_a) product(x, x, km, ai, aj, blocks_a - 1);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) va[t][r] = a.b * va[t][r] + a.c / kScale * acc[t][r];
+    // The next units' place was last read before the step.
+    for (int i = threadIdx.x; i < kWholeSides; i += kWholeWaves * kWave)
+      next[i] = unit_above(fminf(a.most, bound[i] * growth));
+    store_a(a.gram_unit);
+    if (blocks_a) {
+      product(x, x, km, ai, aj, blocks_a - 1);
+      const float c = a.c * a.gram_unit * a.gram_unit;
+      each(units, [&](int t, int r, float v) { va[t][r] = a.b * va[t][r] + c * v; });
     }
-    store_a();
-    if (blocks_x) product(x, xt, km, xi, xj, blocks_x - 1);
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-#pragma unroll
-      for (int r = 0; r < 16; ++r) vx[t][r] = a.a * vx[t][r] + 1.0f / kScale * acc[t][r];
+    store_a(a.poly_unit);
+    if (blocks_x) {
+      fetch_units(xi * 32, units);
+      product(x, xt, km, xi, xj, blocks_x - 1);
+      const float *const columns = now + kWholeRows + xj * 32 + lane % 32;
+      const float column[2] = {columns[0] * a.poly_unit, columns[(blocks_x - 1) * 32] * a.poly_unit};
+      each(units, [&](int t, int r, float v) { vx[t][r] = a.a * vx[t][r] + v * column[t]; });
     }
     __syncthreads();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       if (t >= blocks_x) continue;
       if (step + 1 < steps)
-        store_x(t);
+        store_x(t, next);
       else
         write_block<T>(a, z, xi * 32, (xj + t) * 32, vx[t]);
     }
@@ -692,8 +943,19 @@ __global__ void __launch_bounds__(kWholeWaves *kWave) ortho_whole_kernel(OrthoAr
 struct OrthoLayout {
   int64_t m, n, mp, np;
   bool whole; // one workgroup per matrix, no workspace
-  size_t partial, x, xt, xt_next, gram, poly, bytes;
+  size_t partial, row_part, col_part, row_bound, col_bound, state;
+  size_t x, xt, xt_next, gram, poly, bytes;
 };
+
+// How the norm's workgroups cut G: strips of kStripCols columns, and of at least
+// kStripRows rows, at most kNormBlocks together.
+struct OrthoStrips {
+  int64_t rows, cols;
+};
+OrthoStrips ortho_strips(int64_t rows, int64_t cols) {
+  const int64_t across = ceil_div64(cols, kStripCols);
+  return {std::clamp<int64_t>(ceil_div64(rows, kStripRows), 1, kNormBlocks / across), across};
+}
 
 OrthoLayout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
   OrthoLayout l{};
@@ -709,6 +971,13 @@ OrthoLayout ortho_layout(int64_t batch, int64_t rows, int64_t cols) {
     return here;
   };
   l.partial = take(kNormBlocks, sizeof(double));
+  // Room for G of either orientation.
+  const OrthoStrips wide = ortho_strips(l.m, l.n), tall = ortho_strips(l.n, l.m);
+  l.row_part = take(std::max(wide.cols * l.m, tall.cols * l.n), sizeof(float));
+  l.col_part = take(std::max(wide.rows * l.n, tall.rows * l.m), sizeof(float));
+  l.row_bound = take(l.mp, sizeof(float));
+  l.col_bound = take(l.np, sizeof(float));
+  l.state = take(l.mp * l.np, sizeof(float));
   l.x = take(packed_units(l.mp, l.np), sizeof(uint4));
   l.xt = take(packed_units(l.mp, l.np), sizeof(uint4));
   l.xt_next = take(packed_units(l.mp, l.np), sizeof(uint4));
@@ -726,13 +995,18 @@ bool ortho_sizes(int64_t batch, int64_t rows, int64_t cols) {
          cols <= kMostSide;
 }
 
-// Whether every value of the iteration stays in the halves' range: the largest
-// singular value starts at most 1, and after a step is at most the maximum of
-// |p| up to the largest before, at its end or where p' = a + 3 b t + 5 c t^2
-// (t = s^2) is 0.  A's are its square and B's the maximum of |b t + c t^2|.
-bool ortho_bounded(double a, double b, double c, int32_t steps) {
-  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return false;
-  double s = 1.0;
+// The maxima over the steps, found from the largest singular value: it starts at
+// most 1, and after a step is at most the maximum of |p| up to the largest
+// before, at its end or where p' = a + 3 b t + 5 c t^2 (t = s^2) is 0.  A's are
+// its square and B's the maximum of |b t + c t^2|.
+struct OrthoRange {
+  bool bounded; // none passes kMostValue
+  double most;  // S: of X's singular values
+  double growth, poly; // g and h: maxima of |a + b t + c t^2| and |s (b + c t)| up to S
+};
+OrthoRange ortho_range(double a, double b, double c, int32_t steps) {
+  if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c)) return {};
+  double s = 1.0, most = 1.0;
   for (int32_t k = 0; k < steps; ++k) {
     const double t = s * s;
     double poly = std::abs(b * t + c * t * t);
@@ -747,15 +1021,27 @@ bool ortho_bounded(double a, double b, double c, int32_t steps) {
     if (c == 0.0 && b != 0.0) roots[2] = -a / (3 * b);
     for (double r : roots)
       if (r > 0.0 && r < t) next = std::max(next, std::abs(std::sqrt(r) * (a + r * (b + r * c))));
-    if (!(t <= kMostValue && poly <= kMostValue && next <= kMostValue)) return false;
+    if (!(t <= kMostValue && poly <= kMostValue && next <= kMostValue)) return {};
     s = next;
+    most = std::max(most, s);
   }
-  return true;
+  OrthoRange range{true, most, std::abs(a), 0.0};
+  const double end = most * most;
+  for (double t : {end, c != 0.0 ? -b / (2 * c) : -1.0})
+    if (t > 0.0 && t <= end) range.growth = std::max(range.growth, std::abs(a + t * (b + t * c)));
+  for (double t : {end, c != 0.0 ? -b / (3 * c) : -1.0})
+    if (t > 0.0 && t <= end) range.poly = std::max(range.poly, std::sqrt(t) * std::abs(b + t * c));
+  return range;
 }
 
 constexpr int64_t kCus = 256;     // of an MI355X
 constexpr int64_t kFewTiles = 128;
 constexpr int64_t kMostOver = 96;
+
+// The least power of two that is not below v, from 2^-60 on.
+float power_above(double v) {
+  return static_cast<float>(std::exp2(std::ceil(std::log2(std::max(v, 0x1p-60)))));
+}
 
 template <typename T> int32_t run_norm(const OrthoArgs &a, int blocks, void *stream) {
   const int64_t cols = a.tall ? a.m : a.n;
@@ -796,13 +1082,14 @@ template <typename T>
 int32_t ortho_typed(OrthoArgs a, const OrthoLayout &l, int32_t steps, void *stream) {
   if (l.whole)
     return launch(ortho_whole_kernel<T>, dim3(a.batch), dim3(kWholeWaves * kWave), stream, a, steps);
-  const int norm_blocks = static_cast<int>(
-      std::clamp<int64_t>(a.m * a.n / (16 * kNormThreads), 1, kNormBlocks));
+  const int norm_blocks = a.row_strips * a.col_strips;
   int32_t rc = run_norm<T>(a, norm_blocks, stream);
   if (rc == SPORDER_OK)
     rc = launch(ortho_pack_kernel<T>, dim3(l.mp / 64 * (l.np / 64), a.batch), dim3(kBlock), stream,
                 a, norm_blocks);
   for (int32_t k = 0; k < steps && rc == SPORDER_OK; ++k) {
+    a.now = k > 0 ? a.next : 1.0f;
+    a.next = std::min(a.now * a.growth, 0x1p100f);
     rc = run_product<kGram>(a, stream);
     if (rc == SPORDER_OK) rc = run_product<kPoly>(a, stream);
     if (rc == SPORDER_OK)
@@ -829,34 +1116,41 @@ int32_t sporder_newton_schulz(void *stream, int32_t type, int64_t batch, int64_t
                               const void *d_g, int32_t steps, double a, double b, double c,
                               double eps, void *d_out, void *d_work, size_t work_bytes) {
   if (!type_known(type) || !ortho_sizes(batch, rows, cols) || g_stride < 0 || g_batch_stride < 0 ||
-      steps < 1 || !(eps >= 0.0) || !ortho_bounded(a, b, c, steps))
+      steps < 1 || !(eps >= 0.0))
     return SPORDER_BAD_ARGUMENT;
+  const OrthoRange range = ortho_range(a, b, c, steps);
+  if (!range.bounded) return SPORDER_BAD_ARGUMENT;
   if (batch == 0) return SPORDER_OK;
   const OrthoLayout l = ortho_layout(batch, rows, cols);
   if (!d_g || !d_out) return SPORDER_BAD_ARGUMENT;
   if (l.bytes > 0 && (!d_work || !aligned_to(d_work, 256) || work_bytes < l.bytes))
     return SPORDER_BAD_ARGUMENT;
   char *const w = static_cast<char *>(d_work);
-  const OrthoArgs args{d_g,
-                 d_out,
-                 batch,
-                 l.m,
-                 l.n,
-                 g_batch_stride,
-                 g_stride,
-                 static_cast<int>(l.mp),
-                 static_cast<int>(l.np),
-                 rows > cols,
-                 eps,
-                 static_cast<float>(a),
-                 static_cast<float>(b),
-                 static_cast<float>(c),
-                 reinterpret_cast<double *>(w + l.partial),
-                 reinterpret_cast<uint4 *>(w + l.x),
-                 reinterpret_cast<uint4 *>(w + l.xt),
-                 reinterpret_cast<uint4 *>(w + l.xt_next),
-                 reinterpret_cast<uint4 *>(w + l.gram),
-                 reinterpret_cast<uint4 *>(w + l.poly)};
+  const bool tall = rows > cols;
+  const OrthoStrips strips = ortho_strips(rows, cols);
+  OrthoArgs args{};
+  args.g = d_g, args.out = d_out;
+  args.batch = batch, args.m = l.m, args.n = l.n;
+  args.g_batch = g_batch_stride, args.g_stride = g_stride;
+  args.mp = static_cast<int>(l.mp), args.np = static_cast<int>(l.np);
+  args.tall = tall, args.eps = eps;
+  args.a = static_cast<float>(a), args.b = static_cast<float>(b), args.c = static_cast<float>(c);
+  args.root_m = static_cast<float>(std::sqrt(l.m) * 1.001);
+  args.root_n = static_cast<float>(std::sqrt(l.n) * 1.001);
+  args.most = static_cast<float>(range.most), args.growth = static_cast<float>(range.growth);
+  args.gram_unit = power_above(range.most), args.poly_unit = power_above(range.poly);
+  args.row_strips = static_cast<int>(strips.rows), args.col_strips = static_cast<int>(strips.cols);
+  args.partial = reinterpret_cast<double *>(w + l.partial);
+  args.row_part = reinterpret_cast<float *>(w + l.row_part);
+  args.col_part = reinterpret_cast<float *>(w + l.col_part);
+  args.row_bound = reinterpret_cast<float *>(w + l.row_bound);
+  args.col_bound = reinterpret_cast<float *>(w + l.col_bound);
+  args.state = reinterpret_cast<float4 *>(w + l.state);
+  args.x = reinterpret_cast<uint4 *>(w + l.x);
+  args.xt = reinterpret_cast<uint4 *>(w + l.xt);
+  args.xt_next = reinterpret_cast<uint4 *>(w + l.xt_next);
+  args.gram = reinterpret_cast<uint4 *>(w + l.gram);
+  args.poly = reinterpret_cast<uint4 *>(w + l.poly);
   if (type == SPORDER_TYPE_BF16) return ortho_typed<bf16_t>(args, l, steps, stream);
   if (type == SPORDER_TYPE_F16) return ortho_typed<f16_t>(args, l, steps, stream);
   return ortho_typed<float>(args, l, steps, stream);

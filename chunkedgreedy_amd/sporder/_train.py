@@ -279,9 +279,12 @@ def newton_schulz(g, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-
         eps: >= 0
         out: contiguous tensor of g's shape and type, or None; may be g
 
-    Products have operands of 22 bits and 32-bit sums whatever the type: the
-    result is as close as 32-bit products give it, down to steps of 2^-35 of
-    the norm of the start.  Returns out.
+    X is held in 32 bits whatever the type.  Products have operands of 22 bits
+    and 32-bit sums: a term is within 2^-21 of itself, and within some 2^-37 of
+    the bounds on the norms of its row and column, so small rows, columns and
+    matrices keep their own accuracy.  The result is about as close as 32-bit
+    products give it, or up to some 8 times as far where those have single
+    terms and round once (a diagonal matrix).  Returns out.
     """
     g = _floats(g, "g")
     if g.dim() not in (2, 3) or g.shape[-1] < 1 or g.shape[-2] < 1 \

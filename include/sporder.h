@@ -505,7 +505,8 @@ SPORDER_API int32_t sporder_layer_norm_grad(void *stream, int32_t type, int32_t 
  * (rows g_stride, matrices g_batch_stride elements apart): X = G / (|G|_F +
  * eps), then `steps` (>= 1) times X <- a X + (b A + c A A) X with A = X X^T (of
  * G^T where rows > cols), written to d_out (contiguous, of G's type).
- * Products have operands of 22 bits and 32-bit sums.  Coefficients under
+ * X is held in 32 bits; products have operands of 22 bits, each row of an
+ * operand in a unit of its own, and 32-bit sums.  Coefficients under
  * which a singular value in [0, 1], or one of A or b A + c A A, could pass 31
  * within the steps are a bad argument; rows and cols are at most 65536.  d_work is
  * 256-byte aligned.

@@ -68,6 +68,9 @@ class Muon(torch.optim.Optimizer):
 
     Each singular direction of the update moves the weight by about the same
     amount; the root keeps the update's mean square the same for tall matrices.
+    The momentum and the update are float32 whatever the parameter's type, in
+    whose 16 bits a sum of small gradients would be lost or pass the range; the
+    parameter is rounded once a step.
     """
 
     def __init__(self, params, lr=0.02, momentum=0.95, steps=5):
@@ -92,10 +95,21 @@ class Muon(torch.optim.Optimizer):
                     continue
                 state = self.state[p]
                 if "momentum" not in state:
-                    state["momentum"] = torch.zeros_like(p)
+                    state["momentum"] = torch.zeros_like(p, dtype=torch.float32)
                 m = state["momentum"]
                 m.mul_(group["momentum"]).add_(p.grad)
-                update = sporder.newton_schulz(p.grad.add(m, alpha=group["momentum"]),
+                update = sporder.newton_schulz(p.grad.float().add(m, alpha=group["momentum"]),
                                                steps=group["steps"])
                 p.add_(update, alpha=-group["lr"] * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5)
         return loss
+
+    def load_state_dict(self, state_dict):
+        """As torch's, which rounds the state to the parameters' types: the
+        momentum is taken from ``state_dict`` in float32."""
+        super().load_state_dict(state_dict)
+        ids = (i for group in state_dict["param_groups"] for i in group["params"])
+        params = (p for group in self.param_groups for p in group["params"])
+        for i, p in zip(ids, params):
+            held = state_dict["state"].get(i, {}).get("momentum")
+            if held is not None:
+                self.state[p]["momentum"] = held.to(device=p.device, dtype=torch.float32)

@@ -14,6 +14,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import sporder
+from .sporder import _train
 
 
 class _Embedding(torch.autograd.Function):
@@ -70,7 +71,9 @@ class Muon(torch.optim.Optimizer):
     amount; the root keeps the update's mean square the same for tall matrices.
     The momentum and the update are float32 whatever the parameter's type, in
     whose 16 bits a sum of small gradients would be lost or pass the range; the
-    parameter is rounded once a step.
+    parameter is rounded once a step.  Parameters without a gradient or without
+    elements are passed over; a parameter that newton_schulz refuses ends the
+    step (ValueError or TypeError) before any of them changes.
     """
 
     def __init__(self, params, lr=0.02, momentum=0.95, steps=5):
@@ -89,18 +92,23 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
-            for p in group["params"]:
-                if p.grad is None:
-                    continue
-                state = self.state[p]
-                if "momentum" not in state:
-                    state["momentum"] = torch.zeros_like(p, dtype=torch.float32)
-                m = state["momentum"]
-                m.mul_(group["momentum"]).add_(p.grad)
-                update = sporder.newton_schulz(p.grad.float().add(m, alpha=group["momentum"]),
-                                               steps=group["steps"])
-                p.add_(update, alpha=-group["lr"] * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5)
+        # What can be refused is refused before any parameter or state changes.
+        todo = [(p, group) for group in self.param_groups for p in group["params"]
+                if p.grad is not None and p.numel() > 0]
+        for p, group in todo:
+            _train._step_count(group["steps"])
+            if p.grad.layout != torch.strided:
+                raise ValueError("Muon takes dense gradients")
+            _train._matrices(p.grad, "a parameter's gradient")
+        for p, group in todo:
+            state = self.state[p]
+            if "momentum" not in state:
+                state["momentum"] = torch.zeros_like(p, dtype=torch.float32)
+            m = state["momentum"]
+            m.mul_(group["momentum"]).add_(p.grad)
+            update = sporder.newton_schulz(p.grad.float().add(m, alpha=group["momentum"]),
+                                           steps=group["steps"])
+            p.add_(update, alpha=-group["lr"] * max(1.0, p.shape[-2] / p.shape[-1]) ** 0.5)
         return loss
 
     def load_state_dict(self, state_dict):

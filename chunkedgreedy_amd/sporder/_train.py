@@ -260,6 +260,23 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None):
     return dx, dweight, dbias
 
 
+def _matrices(g, name):
+    """`g` if newton_schulz takes it."""
+    g = _floats(g, name)
+    if g.dim() not in (2, 3) or g.shape[-1] < 1 or g.shape[-2] < 1 \
+            or max(g.shape[-2:]) > 65536 or (g.dim() == 3 and g.shape[0] > 32768):
+        raise ValueError(f"{name} must be (rows, cols) or (batch, rows, cols) with sides of 1 to "
+                         "65536 and a batch of at most 32768")
+    return g
+
+
+def _step_count(steps):
+    steps = int(steps)
+    if not 1 <= steps < 2**31:
+        raise ValueError("steps must be >= 1 and below 2^31")
+    return steps
+
+
 def newton_schulz(g, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-7, out=None):
     """Orthogonalise a matrix by Newton-Schulz products (the Muon optimiser's
     update): X = g / (|g| + eps) with the Frobenius norm, then ``steps`` times
@@ -286,14 +303,8 @@ def newton_schulz(g, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-
     products give it, or up to some 8 times as far where those have single
     terms and round once (a diagonal matrix).  Returns out.
     """
-    g = _floats(g, "g")
-    if g.dim() not in (2, 3) or g.shape[-1] < 1 or g.shape[-2] < 1 \
-            or max(g.shape[-2:]) > 65536 or (g.dim() == 3 and g.shape[0] > 32768):
-        raise ValueError("g must be (rows, cols) or (batch, rows, cols) with sides of 1 to 65536 "
-                         "and a batch of at most 32768")
-    steps = int(steps)
-    if not 1 <= steps < 2**31:
-        raise ValueError("steps must be >= 1 and below 2^31")
+    g = _matrices(g, "g")
+    steps = _step_count(steps)
     if not eps >= 0.0:
         raise ValueError("eps must be >= 0")
     a, b, c = (float(v) for v in coefficients)

@@ -72,3 +72,53 @@ def test_checkpoint_keeps_the_momentum(sporder, dtype):
     opt.step()
     again.step()
     assert torch.equal(first, a) and torch.equal(second, b)
+
+
+def bad_parameters():
+    sparse = torch.zeros(4, 4, device="cuda").requires_grad_()
+    sparse.grad = torch.sparse_coo_tensor([[0], [1]], [1.0], (4, 4)).cuda()
+    plain = [torch.zeros(4, 4), torch.zeros(4, 4, device="cuda", dtype=torch.float64),
+             torch.zeros(65537, 1, device="cuda"), torch.zeros(32769, 1, 1, device="cuda")]
+    for p in plain:
+        p.requires_grad_().grad = torch.zeros_like(p)
+    return plain + [sparse]
+
+
+def test_a_step_that_refuses_changes_nothing(sporder):
+    for bad in bad_parameters():
+        w = weight((5, 6), torch.float32)
+        w.grad = torch.ones_like(w)
+        before, rest = w.detach().clone(), bad.detach().clone()
+        opt = nn.Muon([w, bad])
+        with pytest.raises((TypeError, ValueError)):
+            opt.step()
+        assert torch.equal(w, before) and torch.equal(bad, rest) and not opt.state
+        bad.grad = None
+        opt.step()
+        assert not torch.equal(w, before)
+    w = weight((5, 6), torch.float32)
+    w.grad = torch.ones_like(w)
+    other = weight((6, 5), torch.float32)
+    other.grad = torch.ones_like(other)
+    before = w.detach().clone()
+    opt = nn.Muon([{"params": [w]}, {"params": [other]}])
+    opt.param_groups[1]["steps"] = 0
+    with pytest.raises(ValueError):
+        opt.step()
+    opt.param_groups[1]["steps"] = 5
+    opt.add_param_group({"params": [weight((3,), torch.float32)]})
+    opt.param_groups[2]["params"][0].grad = torch.ones(3, device="cuda")
+    with pytest.raises(ValueError):
+        opt.step()
+    assert torch.equal(w, before) and not opt.state
+
+
+def test_parameters_without_elements_are_passed_over(sporder):
+    w = weight((5, 6), torch.float32)
+    empty = [torch.zeros(s, device="cuda", requires_grad=True) for s in ((0, 5), (3, 0), (0, 2, 2))]
+    for p in [w, *empty]:
+        p.grad = torch.ones_like(p)
+    before = w.detach().clone()
+    nn.Muon([empty[0], w, *empty[1:]]).step()
+    assert not torch.equal(w, before)
+

@@ -21,8 +21,10 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, table, tokens, scale, padding_idx):
         ctx.save_for_backward(tokens)
+        out = sporder.embedding(table, tokens, scale=scale)
+        _train._padding_row(padding_idx, table.shape[0])  # the table has passed its own checks
         ctx.rows, ctx.scale, ctx.padding_idx = table.shape[0], scale, padding_idx
-        return sporder.embedding(table, tokens, scale=scale)
+        return out
 
     @staticmethod
     @once_differentiable

@@ -123,6 +123,11 @@ def embedding(table, tokens, *, scale=1.0, out=None):
     return out
 
 
+def _padding_row(padding_idx, num_rows):
+    if padding_idx is not None and not 0 <= padding_idx < num_rows:
+        raise ValueError("padding_idx must be a row of the table")
+
+
 def embedding_grad(grad, tokens, num_rows, *, scale=1.0, padding_idx=None, dtype=None, out=None):
     """Gradient of :func:`embedding` by its table, dense:
     out[v] = scale * sum of grad[t] over the tokens equal to v.
@@ -146,8 +151,7 @@ def embedding_grad(grad, tokens, num_rows, *, scale=1.0, padding_idx=None, dtype
     num_rows = int(num_rows)
     if not 1 <= num_rows <= 2**31 - 2:
         raise ValueError("num_rows must be in [1, 2^31 - 2]")
-    if padding_idx is not None and not 0 <= padding_idx < num_rows:
-        raise ValueError("padding_idx must be a row of the table")
+    _padding_row(padding_idx, num_rows)
     if dtype is None:
         dtype = grad.dtype
     elif dtype not in (grad.dtype, torch.float32):

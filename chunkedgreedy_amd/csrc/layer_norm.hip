@@ -203,8 +203,8 @@ template <typename T> __global__ void __launch_bounds__(1024) layer_norm_long_ke
 // workgroup are added up at the end and the workgroup writes one row of
 // partial sums.  No atomics: the order of every sum is fixed by the grid.  The
 // next row is on its way while a row is worked on, where registers allow.
-// Bound by memory: 16,384 rows of 4096 16-bit elements in 90 us, 403 MB at 4.5
-// TB/s; 1,000,003 of 100 floats in 238 us, 5.0 TB/s.
+// Bound by memory: 16,384 rows of 4096 16-bit elements in 90 us, 403 MB and 34
+// of partial rows at 4.9 TB/s; 1,000,003 of 100 floats in 239 us, 5.0 TB/s.
 template <typename T, bool LOOSE, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGradArgs a) {
   constexpr int kGroups = norm_block(L) / L;
@@ -357,7 +357,8 @@ __global__ void __launch_bounds__(norm_block(L)) layer_norm_grad_kernel(NormGrad
 // Rows that no workgroup's registers hold: two passes over each, the column
 // sums kept in the workgroup's partial row (each thread its own columns):
 // 100 million elements in rows of 24,001 take 560 us with 16 bits and 710 with
-// 32, of 100,001 1,312 and 1,745 (the partial row is read and written for each).
+// 32, of 100,001 1,312 and 1,745: the partial row is read and written for each,
+// and 1,000 rows are 125 workgroups, half a card, of 8 rows in turn.
 template <typename T>
 __global__ void __launch_bounds__(1024) layer_norm_grad_long_kernel(NormGradArgs a) {
   __shared__ float shared[2][2][1024 / kWave];
@@ -448,7 +449,9 @@ template <int MOST, typename F> int32_t with_lanes(int64_t dim, F &&f) {
   return f(Const<512>{}, Const<MOST>{});
 }
 
-// Lanes and rows at a time of a workgroup of the gradient, by the same rule.
+// Rows at a time of a workgroup of the gradient, by with_lanes.  Rows of 65 to
+// 512 elements read one at a time (with_waves) are fewer at a time than this,
+// 4, so that their workgroups take more turns than the grid is made for.
 int64_t norm_groups(int64_t dim) {
   int lanes = dim <= 16 ? 2 : dim <= 32 ? 4 : 8;
   while (lanes < 512 && lanes * 16 < dim) lanes *= 2;
@@ -545,9 +548,10 @@ int32_t norm_grad_typed(const NormGradArgs &a, int64_t blocks, void *stream) {
   }
 }
 
-// Workgroups of the gradient, each with a partial row of 2 dim floats: enough
-// to fill the card, and few enough that the partial rows stay small beside
-// the rows themselves (at least 8 rows per workgroup).
+// Workgroups of the gradient, each with a partial row of 2 dim floats: at most
+// enough to fill the card, and few enough that the partial rows stay small
+// beside the rows themselves (8 turns of rows per workgroup, so that few rows
+// leave CUs without work).
 int64_t norm_grad_blocks(int64_t rows, int64_t dim) {
   const int64_t most = dim > 4096 ? 512 : 1024;
   return std::max<int64_t>(1, std::min(ceil_div64(rows, 8 * norm_groups(dim)), most));

@@ -493,9 +493,9 @@ __device__ __forceinline__ void place_tile(int t, int down, int across, int rati
 //   kPoly:   P = Q = A;          writes B = b A + c C
 //   kUpdate: P = B, Q = X^T;     writes X = a X + C in both orders
 //   kLast:   the same to out, rounded to its type
-// Bound by the matrix units: an update of 4096 x 4096 in 376 us, 1.10 PFLOP/s of
-// 16-bit products, a library's product of that size and type 1.15; some 20 us are
-// the 134 MB of X in 32 bits, read and written.
+// Bound by the matrix units: an update of 4096 x 4096 in 373 to 384 us, 1.07 to
+// 1.11 PFLOP/s of 16-bit products, a library's product of that size and type
+// 1.15; some 20 us are the 134 MB of X in 32 bits, read and written.
 constexpr int kTileRows = 256, kTileCols = 128;
 
 template <int WHAT, typename T>
@@ -711,7 +711,8 @@ __global__ void __launch_bounds__(WAVES *kWave) ortho_split_kernel(OrthoArgs a, 
 // 32 x 32, padded to 32): its products take less than a launch each.  Eight
 // waves take two neighbouring blocks of the result each; A, then B, takes X's
 // place until the new X does.  A and B are computed whole: a wave per two
-// blocks is there anyway, and needs no mirrored store.
+// blocks is there anyway, and needs no mirrored store.  100 x 128 in 52 us, 19 of
+// them the CU's matrix units, the rest 15 products' waits and epilogues.
 constexpr int kWholeWaves = 8;
 constexpr int kWholeBlocks = 2 * kWholeWaves;
 constexpr int kWholeUnits = kWholeBlocks * 32 * 32 / 4;

@@ -5,7 +5,9 @@ the orthogonalisation.
 ``sporder.layer_norm`` with their gradients behind torch's autograd; ``Muon``
 updates weight matrices along the orthogonalised momentum
 (``sporder.newton_schulz``).  Their backward passes are not differentiable in
-turn.  The end-to-end GCN (``e2e_gcn``) trains with them on request.  They have no counterpart in the reference.
+turn, and they take neither forward-mode derivatives nor ``torch.func``'s
+transforms (RuntimeError).  The end-to-end GCN (``e2e_gcn``) trains with them
+on request.  They have no counterpart in the reference.
 """
 
 from __future__ import annotations

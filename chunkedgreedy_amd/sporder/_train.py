@@ -134,15 +134,17 @@ def embedding_grad(grad, tokens, num_rows, *, scale=1.0, padding_idx=None, dtype
 
     Arguments:
         grad: tokens.shape + (dim,), float32, bfloat16 or float16
-        tokens: int32 or int64 ids; ids outside [0, num_rows) are left out
+        tokens: int32 or int64 ids, at most 2^28 - 4096 of them; ids outside
+            [0, num_rows) are left out
         num_rows: rows of the table
         padding_idx: a row in [0, num_rows) that gets no gradient, or None
         dtype: grad's type (default) or float32, the type of the result
         out: contiguous (num_rows, dim) tensor of that type, or None
 
-    The sums are held in 32 bits, their order depends on the tokens alone (the
-    result is the same bit for bit from run to run), and every row is written.
-    Returns out.
+    The sums are held in 32 bits.  Their order depends on the tokens, the sizes
+    and grad's type, strides and alignment: the same call gives the same bits
+    from run to run, the same values laid out otherwise may differ in the last
+    ones.  Every row is written.  Returns out.
     """
     grad = _floats(grad, "grad")
     tokens = _token_ids(tokens, grad)
@@ -229,7 +231,8 @@ def layer_norm_grad(grad, x, mean, rstd, weight=None):
 
     Returns (dx, dweight, dbias): dx of x's type; dweight and dbias of
     weight's type (float32 without a weight), summed over all rows in 32 bits
-    in an order that depends on the sizes alone.
+    in an order that depends on the sizes and the inputs' types, strides and
+    alignment: the same call gives the same bits from run to run.
     """
     x = _floats(x, "x")
     grad = _floats(grad, "grad")

@@ -433,9 +433,12 @@ SPORDER_API int32_t sporder_spmm_csr_noalloc(sporder_context_t ctx, int32_t n,
  *   SPORDER_OK             queued (or nothing to do)
  *   SPORDER_BAD_ARGUMENT   nothing queued
  *   SPORDER_LAUNCH_FAILED  HIP refused a launch
- * `type` arguments are sporder_type_t.  Sums are held in 32 bits whatever the
- * type and results are rounded to it once, at the end; every result is the
- * same bit for bit from run to run.
+ * `type` arguments are sporder_type_t and `dim` is at most 2^23.  Sums are held
+ * in 32 bits whatever the type and results are rounded to it once, at the end.
+ * The order of every sum follows from the arguments alone (tokens, sizes, types,
+ * strides and the alignment of the pointers): the same call gives the same bits
+ * from run to run, and the same values laid out otherwise may differ in the
+ * last ones.
  */
 typedef enum {
   SPORDER_TYPE_F32 = 0,
@@ -458,10 +461,10 @@ SPORDER_API int32_t sporder_embedding(void *stream, int32_t type, int64_t rows, 
 
 /*
  * Its gradient by the table: d_out[v] = scale * sum of d_grad[t] over the t
- * with d_tokens[t] = v, for each of `rows` rows (0 where there is no such t),
- * summed in an order that depends on the tokens and the sizes alone.  Tokens
- * equal to padding_idx and tokens outside [0, rows) are left out.  out_type is
- * `type` or SPORDER_TYPE_F32.  d_work is 256-byte aligned.
+ * with d_tokens[t] = v, for each of `rows` rows (0 where there is no such t).
+ * Tokens equal to padding_idx and tokens outside [0, rows) are left out.
+ * out_type is `type` or SPORDER_TYPE_F32; count is at most 2^28 - 4096, rows
+ * at most 2^31 - 2.  d_work is 256-byte aligned.
  */
 SPORDER_API size_t sporder_embedding_grad_work_bytes(int64_t count, int64_t rows, int64_t dim);
 SPORDER_API int32_t sporder_embedding_grad(void *stream, int32_t type, int64_t count,

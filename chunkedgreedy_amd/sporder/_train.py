@@ -194,6 +194,8 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5, out=None):
 
     Returns (y, mean, rstd); mean and rstd are float32 of shape x.shape[:-1],
     as :func:`layer_norm_grad` takes them.
+    Sums and squares are held in 32 bits: a row whose deviations from its mean
+    pass some 1e19 has an infinite variance, and y is its bias.
     """
     x = _floats(x, "x")
     if x.dim() < 1 or x.shape[-1] < 1:

@@ -150,6 +150,22 @@ SIGNATURES = {
     "sporder_newton_schulz_work_bytes": ([i64, i64, i64], sz),
     "sporder_newton_schulz": (
         [vp, i32, i64, i64, i64, i64, i64, vp, i32, f64, f64, f64, f64, vp, vp, sz], i32),
+    "sporder_dropout": (
+        [vp, i32, i64, i64, i64, vp, i64, vp, f64, u64, u64, vp, i64, vp], i32),
+    "sporder_residual_norm": (
+        [vp, i32, i32, i64, i64, i64, vp, i64, vp, i32, i64, vp, vp, vp, f32, f32, i32, i64, vp,
+         i64, vp, vp, vp], i32),
+    "sporder_residual_norm_grad_work_bytes": ([i64, i64], sz),
+    "sporder_residual_norm_grad": (
+        [vp, i32, i32, i64, i64, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, i32, i64, vp, vp, vp,
+         f32, i32, i64, vp, i64, vp, i64, vp, vp, vp, vp, sz], i32),
+    "sporder_linear_cross_entropy_work_bytes": ([i32, i64, i64, i64, i64, vp, i64, vp], sz),
+    "sporder_linear_cross_entropy": (
+        [vp, i32, i64, i64, i64, i64, vp, i64, vp, i32, vp, i32, vp, i64, vp, vp, vp, vp, sz], i32),
+    "sporder_linear_cross_entropy_grad_work_bytes": ([i32, i64, i64, i64, i64, vp, i64, vp], sz),
+    "sporder_linear_cross_entropy_grad": (
+        [vp, i32, i64, i64, i64, i64, vp, i64, vp, i64, vp, i32, vp, i32, vp, i64, vp, i64, vp, i32,
+         i64, vp, vp, vp, sz], i32),
     "sporder_hbm_stream": ([vp, i32, i32, vp, vp, ctypes.c_int64, i32, P(f32)], None),
 }
 

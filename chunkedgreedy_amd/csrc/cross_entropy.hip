@@ -1,0 +1,1048 @@
+// cross_entropy.hip -- softmax cross entropy of linear logits that are never
+// kept, and its gradients.
+//
+//   z[t][v] = x[t] . w[v] + b[v],  lse[t] = log sum_v exp z,  loss = lse - z[t][target]
+//   g[t][v] = s[t] (exp(z - lse) - [v = target]),  dx = g w,  dw = g^T x,  db = sum_t g
+//
+// Rows.  Rows whose target is ignored cost nothing: the others are listed first
+// and every product runs over the list.
+//
+// Forward.  A tile of z stays in the accumulators of its workgroup: each wave
+// writes its tokens' largest logit and sum of exponentials over its classes, and
+// the target's logit where it meets it; a second kernel joins the pieces.
+//
+// Backward.  For a piece of the classes at a time the logits are made again and
+// become g, in 16 bits and in both orders, since both products that follow sum
+// along another side of it; the piece's rows of dw are then final and dx is
+// summed over the pieces in 32 bits.  The pieces' size bounds the scratch.
+//
+// 16-bit types.  g is rounded to the type before its products (a relative 2^-9 or
+// 2^-12 of each term, as its factors in w and x are already rounded): the matrix
+// units take 16 bits.  A token's scale s = m 2^e enters as m, with 1 <= |m| < 2,
+// times 2^13, so that float16 keeps 11 bits down to g = 2^-27; 2^e goes to dx in
+// 32 bits and to dw with x's rows, where it is exact.
+// 32-bit types.  Operands are two 16-bit halves (22 bits) in units of their row, a
+// power of two by its largest element, and products are three.
+#include <algorithm>
+
+#include "mfma_product.hpp"
+
+namespace sporder_hip {
+
+namespace {
+
+constexpr int kShift = 13; // g is held 2^13 times as large
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kListBlock = 1024; // rows of a block of the list
+constexpr int64_t kListDirect = 65536; // rows up to which a block counts those before it
+
+struct CeMeta {
+  int32_t count; // rows listed
+  int32_t most;  // largest exponent of their scales
+};
+
+struct CeArgs {
+  int64_t rows, dim, classes;
+  int64_t x_stride, w_stride; // elements
+  const void *x, *w, *bias, *targets;
+  int64_t ignore;
+  int type, bias_type, target_bits;
+  // forward
+  float *loss, *lse, *sums;
+  // backward
+  const float *grad, *given_lse;
+  int64_t grad_stride;
+  void *dx, *dw, *db;
+  int64_t dx_stride, dw_stride;
+  int dw_type;
+  // scratch
+  CeMeta *meta;
+  int32_t *counts;       // of the list's blocks, past kListDirect rows
+  int32_t *list, *target; // of the listed rows
+  int32_t *exponent;
+  float *mantissa, *row_lse;
+  float *bias32;      // [classes_pad], -inf past the classes
+  float *hit;         // the target's logit
+  float2 *partial;    // [chunks][rows_pad] largest and sum
+  double *sum_parts;
+  char *xp, *wp;      // operands of z: packed rows, or x and w themselves
+  int64_t xp_stride, wp_stride, xp_plane, wp_plane; // bytes
+  bool x_packed;      // by list position
+  float *x_unit, *w_unit; // of their rows (32-bit types)
+  char *xt, *wt;      // transposed operands, [dim][rows_pad] and [dim][piece]
+  float *x_most, *w_most; // [dim]: largest of each column, as bits
+  char *g, *gt;       // [rows_pad][piece] and [piece][rows_pad]
+  float *dx32;        // [rows_pad][dim_pad]
+  float *db_part;     // [token chunks][piece]
+  int64_t rows_pad, dim_pad, classes_pad, chunks, piece;
+};
+
+__device__ __forceinline__ int64_t target_of(const CeArgs &a, int64_t row) {
+  return a.target_bits == 64 ? static_cast<const int64_t *>(a.targets)[row]
+                             : static_cast<const int32_t *>(a.targets)[row];
+}
+__device__ __forceinline__ bool counted(const CeArgs &a, int64_t target) {
+  return target != a.ignore && target >= 0 && target < a.classes;
+}
+
+// ---- the list of rows, and what else comes first -----------------------------------
+
+__global__ void __launch_bounds__(256) ce_prepare_kernel(CeArgs a, bool backward) {
+  const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
+  if (i == 0) *a.meta = {0, -1000};
+  if (i < a.classes_pad) {
+    float b = -INFINITY;
+    if (i < a.classes) {
+      b = 0.0f;
+      if (a.bias) with_type(a.bias, a.bias_type, [&](auto *p) { b = static_cast<float>(p[i]); });
+    }
+    a.bias32[i] = b;
+  }
+  if (a.w_unit && i >= a.classes && i < a.classes_pad) a.w_unit[i] = 1.0f;
+  if (backward && i < a.dim && a.x_most) {
+    a.x_most[i] = 0.0f;
+    a.w_most[i] = 0.0f;
+  }
+}
+
+__global__ void __launch_bounds__(256) ce_count_kernel(CeArgs a) {
+  __shared__ int32_t part[4];
+  int n = 0;
+#pragma unroll
+  for (int k = 0; k < kListBlock / 256; ++k) {
+    const int64_t row = blockIdx.x * int64_t(kListBlock) + k * 256 + threadIdx.x;
+    n += __popcll(__ballot(row < a.rows && counted(a, target_of(a, row))));
+  }
+  if (lane_id() == 0) part[threadIdx.x / kWave] = n;
+  __syncthreads();
+  if (threadIdx.x == 0) a.counts[blockIdx.x] = part[0] + part[1] + part[2] + part[3];
+}
+
+// Sum over the workgroup, of one int per wave in `part` (uniform in each wave).
+__device__ __forceinline__ int block_total(int mine, int32_t *part) {
+  __syncthreads();
+  if (lane_id() == 0) part[threadIdx.x / kWave] = mine;
+  __syncthreads();
+  return part[0] + part[1] + part[2] + part[3];
+}
+
+__device__ __forceinline__ int wave_total(int v) {
+#pragma unroll
+  for (int j = 1; j < kWave; j <<= 1) v += __shfl_xor(v, j);
+  return v;
+}
+
+// The rows' places in the list: those counted before the block, then before the
+// thread in it.
+__global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward) {
+  __shared__ int32_t part[4], most;
+  const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
+  const int64_t first = blockIdx.x * int64_t(kListBlock);
+  if (tid == 0) most = -1000;
+  int before = 0;
+  if (a.rows <= kListDirect) {
+#pragma unroll 4
+    for (int64_t row = tid; row < first; row += 256)
+      before += counted(a, target_of(a, row)) ? 1 : 0;
+  } else {
+#pragma unroll 4
+    for (int64_t b = tid; b < blockIdx.x; b += 256) before += a.counts[b];
+  }
+  before = block_total(wave_total(before), part);
+#pragma unroll
+  for (int k = 0; k < kListBlock / 256; ++k) {
+    const int64_t row = first + k * 256 + tid;
+    const bool inside = row < a.rows;
+    const int64_t target = inside ? target_of(a, row) : -1;
+    const bool on = inside && counted(a, target);
+    const uint64_t mask = __ballot(on);
+    __syncthreads();
+    if (lane == 0) part[wave] = __popcll(mask);
+    __syncthreads();
+    int at = before + __popcll(mask & ((uint64_t(1) << lane) - 1));
+    for (int w = 0; w < wave; ++w) at += part[w];
+    if (on) {
+      a.list[at] = static_cast<int32_t>(row);
+      a.target[at] = static_cast<int32_t>(target);
+      if (backward) {
+        const float s = a.grad[row * a.grad_stride];
+        // |s| = m 2^e with 1 <= m < 2 (a scale below 2^-126 keeps its place in m).
+        const int e = max(static_cast<int>(__builtin_bit_cast(uint32_t, s) >> 23 & 255), 1) - 127;
+        a.exponent[at] = e;
+        a.mantissa[at] = ldexpf(s, -e);
+        a.row_lse[at] = a.given_lse[row];
+        if (s != 0.0f) atomicMax(&most, e);
+      }
+    } else if (inside && !backward) {
+      const float none = target == a.ignore ? 0.0f : NAN;
+      a.loss[row] = none;
+      a.lse[row] = none;
+    }
+    before += part[0] + part[1] + part[2] + part[3];
+  }
+  __syncthreads();
+  if (backward && tid == 0) atomicMax(&a.meta->most, most);
+  if (blockIdx.x != gridDim.x - 1) return;
+  if (tid == 0) a.meta->count = before;
+  // What the last tile reads past the list.
+  const int64_t at = before + tid;
+  if (at < a.rows_pad) {
+    a.list[at] = 0;
+    a.target[at] = -1;
+    if (backward) {
+      a.exponent[at] = 0;
+      a.mantissa[at] = 0.0f;
+      a.row_lse[at] = 0.0f;
+    }
+  }
+}
+
+// ---- packing -------------------------------------------------------------------------
+
+template <typename U> __device__ __forceinline__ void split(float v, U &hi, U &lo) {
+  hi = static_cast<U>(v);
+  lo = static_cast<U>(v - static_cast<float>(hi));
+}
+
+// Rows of x (listed) or w, zeros up to a multiple of 64 elements: a wave per row,
+// 8 elements a lane.
+template <typename T, typename U, int PLANES>
+__global__ void __launch_bounds__(256)
+    ce_pack_rows_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
+                        const int32_t *list, char *out, int64_t out_stride, int64_t plane, float *unit) {
+  const int64_t row = blockIdx.x * int64_t(4) + threadIdx.x / kWave;
+  if (row >= (list ? meta->count : rows)) return;
+  const T *const from = src + (list ? list[row] : row) * stride;
+  const int lane = lane_id();
+  float scale = 1.0f;
+  if constexpr (PLANES == 2) {
+    float most = 0.0f;
+    for (int64_t c = lane * 4; c < dim; c += kWave * 4) {
+      const auto q = fetch<true, 4>(from + c, dim - c);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) most = fmaxf(most, fabsf(static_cast<float>(q.v[i])));
+    }
+    const float u = unit_of(group_max<kWave>(most));
+    scale = unit_inverse(u);
+    if (lane == 0) unit[row] = u;
+  }
+  const int64_t width = ceil_div64(dim, kStageK) * kStageK;
+  for (int64_t c = lane * 8; c < width; c += kWave * 8) {
+    Pack<T, 8> q{};
+    if (c < dim) q = fetch<true, 8>(from + c, dim - c);
+    Pack<U, 8> hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (PLANES == 2)
+        split(static_cast<float>(q.v[i]) * scale, hi.v[i], lo.v[i]);
+      else
+        hi.v[i] = static_cast<U>(q.v[i]);
+    }
+    U *const to = reinterpret_cast<U *>(out + row * out_stride) + c;
+    *reinterpret_cast<Pack<U, 8> *>(to) = hi;
+    if constexpr (PLANES == 2)
+      *reinterpret_cast<Pack<U, 8> *>(reinterpret_cast<char *>(to) + plane) = lo;
+  }
+}
+
+// The largest element of each column of rows of x (listed) or w, as the bits of a
+// non-negative float: their order is the floats'.  64 columns and a strip of rows
+// per workgroup.
+template <typename T>
+__global__ void __launch_bounds__(256)
+    ce_column_most_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
+                          const int32_t *list, float *most) {
+  const int64_t all = list ? meta->count : rows;
+  const int64_t col = blockIdx.x * int64_t(64) + threadIdx.x % 64;
+  if (col >= dim) return;
+  float m = 0.0f;
+#pragma unroll 4
+  for (int64_t r = blockIdx.y * int64_t(4) + threadIdx.x / 64; r < all; r += gridDim.y * int64_t(4))
+    m = fmaxf(m, fabsf(static_cast<float>(src[(list ? list[r] : r) * stride + col])));
+  atomicMax(reinterpret_cast<uint32_t *>(most) + col, __builtin_bit_cast(uint32_t, m));
+}
+
+// Columns of rows of x (listed) or w as operand rows: out[j][k] of k-th row,
+// zeros for k past the rows up to a multiple of 64.  64 x 64 per workgroup,
+// turned in LDS.  Listed rows come with 2^(their exponent - the largest).
+template <typename T, typename U, int PLANES>
+__global__ void __launch_bounds__(256)
+    ce_pack_columns_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
+                           const int32_t *list, const int32_t *exponent, const float *most, char *out,
+                           int64_t out_stride, int64_t plane) {
+  __shared__ float tile[64][65];
+  const int64_t all = list ? meta->count : rows;
+  const int64_t k0 = blockIdx.y * int64_t(64), j0 = blockIdx.x * int64_t(64);
+  if (k0 >= all) return;
+  const int x = threadIdx.x % 64, y = threadIdx.x / 64;
+  const int top = list ? meta->most : 0;
+  const bool in = j0 + x < dim;
+  float scale = 1.0f;
+  if constexpr (PLANES == 2) scale = in ? unit_inverse(unit_of(most[j0 + x])) : 0.0f;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int64_t k = k0 + y + 4 * i;
+    float v = 0.0f;
+    if (in && k < all) {
+      v = static_cast<float>(src[(list ? list[k] : k) * stride + j0 + x]) * scale;
+      if (list) v = ldexpf(v, min(exponent[k] - top, 0)); // no row has a scale: top is below all
+    }
+    tile[y + 4 * i][x] = v;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int j = threadIdx.x / 8 + 32 * i, c = threadIdx.x % 8 * 8;
+    if (j0 + j >= dim) continue;
+    Pack<U, 8> hi, lo;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if constexpr (PLANES == 2)
+        split(tile[c + e][j], hi.v[e], lo.v[e]);
+      else
+        hi.v[e] = static_cast<U>(tile[c + e][j]);
+    }
+    U *const to = reinterpret_cast<U *>(out + (j0 + j) * out_stride) + k0 + c;
+    *reinterpret_cast<Pack<U, 8> *>(to) = hi;
+    if constexpr (PLANES == 2)
+      *reinterpret_cast<Pack<U, 8> *>(reinterpret_cast<char *>(to) + plane) = lo;
+  }
+}
+
+// ---- logits ----------------------------------------------------------------------------
+
+using Large = TileShape<2, 4, 4, 2>; // 256 classes x 256 tokens
+using Middle = TileShape<2, 2, 2, 2>; // 128 x 128
+using Narrow = TileShape<4, 1, 1, 1>; // 128 x 32
+
+template <typename S> constexpr int logit_lds(bool backward) {
+  const int a = S::kN * (S::kM * 2 + 16), b = S::kM * (S::kN * 2 + 16), c = 2 * S::kStage;
+  return backward ? std::max(std::max(a, b), c) : c;
+}
+
+// z of a tile: classes (from v0 on) down, listed rows across.
+template <typename U, int PLANES, typename S>
+__device__ __forceinline__ void logit_tile(const CeArgs &a, char *lds, int wave, int64_t m0, int64_t n0,
+                                           int64_t v0, int count, f32x16 (&acc)[S::MB][S::NB]) {
+  uint32_t a_off[S::kFetchA], b_off[S::kFetchB];
+  fetch_offsets<S::kWaves>(wave, a_off, [&](int r) {
+    return static_cast<uint32_t>(min(static_cast<int64_t>(r), a.classes - 1 - v0 - m0) * a.wp_stride);
+  });
+  fetch_offsets<S::kWaves>(wave, b_off, [&](int r) {
+    const int64_t n = min(n0 + r, int64_t(count) - 1);
+    return static_cast<uint32_t>((a.x_packed ? n - n0 : a.list[n]) * a.xp_stride);
+  });
+  tile_product<U, PLANES, S>(lds, wave, a.wp + (v0 + m0) * a.wp_stride, a.wp_plane, a_off,
+                             a.xp + (a.x_packed ? n0 * a.xp_stride : 0), a.xp_plane, b_off,
+                             static_cast<int>(ceil_div64(a.dim, kStageK)), acc);
+  // Units and bias.
+  const int lane = lane_id(), wm = wave / S::WN, wn = wave % S::WN;
+  float x_unit[S::NB];
+  if constexpr (PLANES == 2) {
+#pragma unroll
+    for (int j = 0; j < S::NB; ++j) x_unit[j] = a.x_unit[n0 + (wn * S::NB + j) * 32 + lane % 32];
+  }
+#pragma unroll
+  for (int i = 0; i < S::MB; ++i) {
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int64_t m = v0 + m0 + (wm * S::MB + i) * 32 + result_row(4 * q);
+      const float4 b = *reinterpret_cast<const float4 *>(a.bias32 + m);
+      const float bias[4] = {b.x, b.y, b.z, b.w};
+      float unit[4] = {1.0f, 1.0f, 1.0f, 1.0f};
+      if constexpr (PLANES == 2) {
+        const float4 u = *reinterpret_cast<const float4 *>(a.w_unit + m);
+        unit[0] = u.x, unit[1] = u.y, unit[2] = u.z, unit[3] = u.w;
+      }
+#pragma unroll
+      for (int j = 0; j < S::NB; ++j) {
+        const float un = PLANES == 2 ? x_unit[j] : 1.0f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float z = acc[i][j][4 * q + e];
+          acc[i][j][4 * q + e] = (PLANES == 2 ? z * unit[e] * un : z) + bias[e];
+        }
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0); // all blocks' vectors at once would not fit the registers
+  }
+}
+
+template <typename U, int PLANES, typename S>
+__global__ void __launch_bounds__(S::kThreads) ce_loss_kernel(CeArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[logit_lds<S>(false)];
+  const int count = a.meta->count;
+  int64_t ti, tj;
+  place_tile(xcd_block(), ceil_div64(a.classes, S::kM), ceil_div64(a.rows, S::kN), 8, ti, tj);
+  const int64_t m0 = ti * S::kM, n0 = tj * S::kN;
+  if (n0 >= count) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  f32x16 acc[S::MB][S::NB] = {};
+  logit_tile<U, PLANES, S>(a, lds, wave, m0, n0, 0, count, acc);
+#pragma unroll
+  for (int j = 0; j < S::NB; ++j) {
+    const int64_t n = n0 + (wn * S::NB + j) * 32 + lane % 32;
+    const int target = (n < count ? a.target[n] : -1) - static_cast<int>(m0);
+    float most = -INFINITY, hit = 0.0f;
+    bool met = false;
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        most = fmaxf(most, acc[i][j][r]);
+        const bool here = (wm * S::MB + i) * 32 + result_row(r) == target;
+        hit = here ? acc[i][j][r] : hit;
+        met = met || here;
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (met) a.hit[n] = hit;
+    most = fmaxf(most, lane_xor_f32(most, 32));
+    const float base = most == -INFINITY ? 0.0f : most;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2e);
+    }
+    sum += lane_xor_f32(sum, 32);
+    if (lane < 32 && n < count)
+      a.partial[(ti * S::WM + wm) * a.rows_pad + n] = make_float2(most, sum);
+  }
+}
+
+// Joins the pieces of 16 rows, 16 threads each.
+__global__ void __launch_bounds__(256) ce_join_kernel(CeArgs a) {
+  __shared__ float2 part[16][17];
+  const int x = threadIdx.x % 16, y = threadIdx.x / 16;
+  const int64_t n = blockIdx.x * int64_t(16) + x;
+  const int count = a.meta->count;
+  if (blockIdx.x * int64_t(16) >= count) return;
+  float most = -INFINITY, sum = 0.0f;
+  if (n < count) {
+#pragma unroll 4
+    for (int64_t c = y; c < a.chunks; c += 16) {
+      const float2 p = a.partial[c * a.rows_pad + n];
+      const float m = fmaxf(most, p.x), base = m == -INFINITY ? 0.0f : m;
+      sum = sum * __builtin_amdgcn_exp2f((most - base) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - base) * kLog2e);
+      most = m;
+    }
+  }
+  part[y][x] = make_float2(most, sum);
+  __syncthreads();
+  if (y != 0 || n >= count) return;
+  for (int k = 1; k < 16; ++k) most = fmaxf(most, part[k][x].x);
+  const float base = most == -INFINITY ? 0.0f : most;
+  sum = 0.0f;
+  for (int k = 0; k < 16; ++k) sum += part[k][x].y * __builtin_amdgcn_exp2f((part[k][x].x - base) * kLog2e);
+  const float lse = base + logf(sum);
+  a.lse[a.list[n]] = lse;
+  a.loss[a.list[n]] = lse - a.hit[n];
+}
+
+// The losses' sum and the number of rows not ignored, in 64 bits and a fixed
+// order: workgroup by workgroup, then their parts.
+constexpr int64_t kSumRows = 8192; // of a workgroup, or more
+constexpr int64_t kSumBlocks = 256;
+
+__device__ __forceinline__ void block_sums(double s, double n, double (&part)[2][4]) {
+#pragma unroll
+  for (int j = 1; j < kWave; j <<= 1) {
+    s += __shfl_xor(s, j);
+    n += __shfl_xor(n, j);
+  }
+  if (lane_id() == 0) {
+    part[0][threadIdx.x / kWave] = s;
+    part[1][threadIdx.x / kWave] = n;
+  }
+  __syncthreads();
+}
+
+__global__ void __launch_bounds__(256) ce_sums_kernel(CeArgs a, int64_t per) {
+  __shared__ double part[2][4];
+  const int64_t first = blockIdx.x * per, last = min(first + per, a.rows);
+  double s = 0.0, n = 0.0;
+#pragma unroll 4
+  for (int64_t row = first + threadIdx.x; row < last; row += 256) {
+    s += a.loss[row];
+    n += target_of(a, row) != a.ignore ? 1.0 : 0.0;
+  }
+  block_sums(s, n, part);
+  if (threadIdx.x >= 2) return;
+  const double *const p = part[threadIdx.x];
+  const double v = (p[0] + p[1]) + (p[2] + p[3]);
+  if (gridDim.x == 1)
+    a.sums[threadIdx.x] = static_cast<float>(v);
+  else
+    a.sum_parts[2 * blockIdx.x + threadIdx.x] = v;
+}
+
+__global__ void __launch_bounds__(256) ce_total_kernel(CeArgs a, int blocks) {
+  __shared__ double part[2][4];
+  double s = 0.0, n = 0.0;
+  if (static_cast<int>(threadIdx.x) < blocks) {
+    s = a.sum_parts[2 * threadIdx.x];
+    n = a.sum_parts[2 * threadIdx.x + 1];
+  }
+  block_sums(s, n, part);
+  if (threadIdx.x >= 2) return;
+  const double *const p = part[threadIdx.x];
+  a.sums[threadIdx.x] = static_cast<float>((p[0] + p[1]) + (p[2] + p[3]));
+}
+
+// ---- gradients ---------------------------------------------------------------------------
+
+// g of a tile in both orders.
+template <typename U, int PLANES, typename S>
+__global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0) {
+  __shared__ __attribute__((aligned(16))) char lds[logit_lds<S>(true)];
+  const int count = a.meta->count;
+  int64_t ti, tj;
+  place_tile(xcd_block(), ceil_div64(min(a.piece, a.classes - v0), S::kM), ceil_div64(a.rows, S::kN), 8,
+             ti, tj);
+  const int64_t m0 = ti * S::kM, n0 = tj * S::kN;
+  if (n0 >= count) return;
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / kWave), lane = lane_id();
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  f32x16 acc[S::MB][S::NB] = {};
+  logit_tile<U, PLANES, S>(a, lds, wave, m0, n0, v0, count, acc);
+  float lse[S::NB], m[S::NB], grad[S::NB];
+  int target[S::NB];
+#pragma unroll
+  for (int j = 0; j < S::NB; ++j) {
+    const int64_t n = n0 + (wn * S::NB + j) * 32 + lane % 32;
+    const bool on = n < count;
+    target[j] = on ? a.target[n] - static_cast<int>(v0 + m0) : -1;
+    lse[j] = on ? a.row_lse[n] : 0.0f;
+    m[j] = on ? a.mantissa[n] * (1 << kShift) : 0.0f;
+    grad[j] = on ? ldexpf(a.mantissa[n], a.exponent[n]) : 0.0f;
+  }
+#pragma unroll
+  for (int i = 0; i < S::MB; ++i) {
+    float total[16] = {}; // of the classes over this wave's tokens
+#pragma unroll
+    for (int j = 0; j < S::NB; ++j) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int row = (wm * S::MB + i) * 32 + result_row(r);
+        float g = __builtin_amdgcn_exp2f((acc[i][j][r] - lse[j]) * kLog2e) - (row == target[j] ? 1.0f : 0.0f);
+        g = n0 + (wn * S::NB + j) * 32 + lane % 32 < count ? g : 0.0f; // the product is of another row
+        total[r] += g * grad[j];
+        acc[i][j][r] = g * m[j];
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (a.db) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const float v = group_sum<32>(total[r]);
+        if (lane % 32 == 0)
+          a.db_part[(tj * S::WN + wn) * a.piece + m0 + (wm * S::MB + i) * 32 + result_row(r)] = v;
+      }
+    }
+  }
+  constexpr int kDown = S::kM * 2 + 16, kAcross = S::kN * 2 + 16; // bytes of a row in LDS
+#pragma unroll
+  for (int plane = 0; plane < PLANES; ++plane) {
+    // A plane's halves, two classes of a token in a word.
+    uint32_t half[S::MB][S::NB][8];
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i) {
+#pragma unroll
+      for (int j = 0; j < S::NB; ++j) {
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          Pack<U, 2> p;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float v = acc[i][j][2 * r + e];
+            p.v[e] = static_cast<U>(v);
+            if constexpr (PLANES == 2) acc[i][j][2 * r + e] = v - static_cast<float>(p.v[e]);
+          }
+          half[i][j][r] = __builtin_bit_cast(uint32_t, p);
+        }
+      }
+    }
+    if (plane) __syncthreads();
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i) {
+#pragma unroll
+      for (int j = 0; j < S::NB; ++j) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<uint2 *>(lds + ((wn * S::NB + j) * 32 + lane % 32) * kDown +
+                                     ((wm * S::MB + i) * 32 + result_row(4 * q)) * 2) =
+              make_uint2(half[i][j][2 * q], half[i][j][2 * q + 1]);
+      }
+    }
+    __syncthreads();
+    char *const g = a.g + plane * (a.rows_pad * a.piece * 2) + (n0 * a.piece + m0) * 2;
+    for (int c = tid; c < S::kN * (S::kM / 8); c += S::kThreads) {
+      const int row = c / (S::kM / 8), part = c % (S::kM / 8);
+      *reinterpret_cast<uint4 *>(g + row * a.piece * 2 + part * 16) =
+          *reinterpret_cast<const uint4 *>(lds + row * kDown + part * 16);
+    }
+    __syncthreads();
+    // A word holds classes r and r + 1 of a token; with the neighbouring token's,
+    // an even lane makes class r's word of both and an odd one r + 1's.
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i) {
+#pragma unroll
+      for (int j = 0; j < S::NB; ++j) {
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const uint32_t mine = half[i][j][r / 2];
+          const uint32_t word = __builtin_amdgcn_perm(lane_xor_u32(mine, 1), mine,
+                                                      lane & 1 ? 0x03020706 : 0x05040100);
+          const int row = (wm * S::MB + i) * 32 + result_row(r) + (lane & 1);
+          *reinterpret_cast<uint32_t *>(lds + row * kAcross +
+                                        ((wn * S::NB + j) * 32 + (lane % 32 & ~1)) * 2) = word;
+        }
+      }
+    }
+    __syncthreads();
+    char *const gt = a.gt + plane * (a.rows_pad * a.piece * 2) + (m0 * a.rows_pad + n0) * 2;
+    for (int c = tid; c < S::kM * (S::kN / 8); c += S::kThreads) {
+      const int row = c / (S::kN / 8), part = c % (S::kN / 8);
+      *reinterpret_cast<uint4 *>(gt + row * a.rows_pad * 2 + part * 16) =
+          *reinterpret_cast<const uint4 *>(lds + row * kAcross + part * 16);
+    }
+  }
+}
+
+// Four neighbouring elements of an output row.
+template <typename O>
+__device__ __forceinline__ void put_four(O *row, int64_t j, int64_t dim, bool whole, const float (&v)[4]) {
+  if (whole && j + 4 <= dim) {
+    store_f32<4>(row + j, v);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (j + e < dim) row[j + e] = static_cast<O>(v[e]);
+}
+
+// dx (DX) or the piece's rows of dw: features down, listed rows or classes across.
+// dx is summed over the pieces: `add` to what is there, and to its type at the `last`.
+template <typename U, int PLANES, typename S, typename O, bool DX>
+__global__ void __launch_bounds__(S::kThreads)
+    ce_gradient_kernel(CeArgs a, int64_t v0, bool add, bool last) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::kStage];
+  const int count = a.meta->count;
+  const int64_t across = DX ? a.rows : min(a.piece, a.classes - v0);
+  int64_t ti, tj;
+  place_tile(xcd_block(), ceil_div64(a.dim, S::kM), ceil_div64(across, S::kN), 8, ti, tj);
+  const int64_t m0 = ti * S::kM, n0 = tj * S::kN;
+  const int64_t limit = DX ? count : across;
+  if (n0 >= limit) return;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  const int64_t a_stride = (DX ? a.piece : a.rows_pad) * 2;
+  uint32_t a_off[S::kFetchA], b_off[S::kFetchB];
+  fetch_offsets<S::kWaves>(wave, a_off, [&](int r) {
+    return static_cast<uint32_t>(min(static_cast<int64_t>(r), a.dim - 1 - m0) * a_stride);
+  });
+  fetch_offsets<S::kWaves>(wave, b_off, [&](int r) {
+    return static_cast<uint32_t>(min(static_cast<int64_t>(r), limit - 1 - n0) * a_stride);
+  });
+  f32x16 acc[S::MB][S::NB] = {};
+  const int64_t g_plane = a.rows_pad * a.piece * 2;
+  tile_product<U, PLANES, S>(lds, wave, (DX ? a.wt : a.xt) + m0 * a_stride, a.dim * a_stride, a_off,
+                             (DX ? a.g : a.gt) + n0 * a_stride, g_plane, b_off,
+                             static_cast<int>(ceil_div64(DX ? min(a.piece, a.classes - v0) : count, kStageK)), acc);
+  O *const out = static_cast<O *>(DX ? a.dx : a.dw);
+  const int64_t stride = DX ? a.dx_stride : a.dw_stride;
+  const bool whole = stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(O)) == 0;
+#pragma unroll
+  for (int j = 0; j < S::NB; ++j) {
+    const int64_t n = n0 + (wn * S::NB + j) * 32 + lane % 32;
+    if (n >= limit) continue;
+    const int power = (DX ? a.exponent[n] : a.meta->most) - kShift;
+    O *const row = out + (DX ? a.list[n] : v0 + n) * stride;
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int64_t m = m0 + (wm * S::MB + i) * 32 + result_row(4 * q);
+        if (m >= a.dim) continue;
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+        if (DX && (add || !last)) {
+          float4 *const held = reinterpret_cast<float4 *>(a.dx32 + n * a.dim_pad + m);
+          if (add) {
+            const float4 old = *held;
+            v[0] += old.x, v[1] += old.y, v[2] += old.z, v[3] += old.w;
+          }
+          if (!last) {
+            *held = make_float4(v[0], v[1], v[2], v[3]);
+            continue;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if constexpr (PLANES == 2)
+            v[e] *= unit_of((DX ? a.w_most : a.x_most)[min(m + e, a.dim - 1)]);
+          v[e] = ldexpf(v[e], power);
+        }
+        put_four(row, m, a.dim, whole, v);
+      }
+    }
+  }
+}
+
+// dx of the rows that are not listed.
+template <typename T> __global__ void __launch_bounds__(256) ce_zero_kernel(CeArgs a) {
+  const int64_t row = blockIdx.x * int64_t(4) + threadIdx.x / kWave;
+  if (row >= a.rows || counted(a, target_of(a, row))) return;
+  T *const out = static_cast<T *>(a.dx) + row * a.dx_stride;
+  for (int64_t c = lane_id(); c < a.dim; c += kWave) out[c] = static_cast<T>(0.0f);
+}
+
+// db of a piece: 64 classes per workgroup, four threads each.
+__global__ void __launch_bounds__(256) ce_bias_kernel(CeArgs a, int64_t v0, int tile) {
+  __shared__ float part[4][kWave];
+  const int x = threadIdx.x % kWave, y = threadIdx.x / kWave;
+  const int64_t v = blockIdx.x * int64_t(kWave) + x;
+  const int64_t chunks = ceil_div64(a.meta->count, tile) * (tile / 64);
+  float s = 0.0f;
+#pragma unroll 4
+  for (int64_t c = y; c < chunks; c += 4) s += a.db_part[c * a.piece + v];
+  part[y][x] = s;
+  __syncthreads();
+  if (y == 0 && v0 + v < a.classes && v < a.piece)
+    store_typed(a.db, a.bias_type, v0 + v, (part[0][x] + part[1][x]) + (part[2][x] + part[3][x]));
+}
+
+// ---- host --------------------------------------------------------------------------------
+
+constexpr int64_t kPieceBytes = int64_t(512) << 20; // of g in one order, about
+constexpr int64_t kMostRows = (int64_t(1) << 23) - 256; // 256 rows of xt in 32 bits
+constexpr int64_t kMostClasses = int64_t(1) << 25;
+constexpr int64_t kMostLogits = int64_t(1) << 37; // a launch's threads in 32 bits
+constexpr int64_t kMostFeatures = 65536;
+
+struct CePlan {
+  bool x_direct, w_direct;
+  int planes, half;
+  int shape; // 0 narrow, 1 middle, 2 large
+  size_t bytes;
+};
+
+bool direct_rows(int type, int64_t dim, int64_t stride, const void *p, int64_t span_rows) {
+  return type != SPORDER_TYPE_F32 && dim % kStageK == 0 && stride % 8 == 0 && aligned_to(p, 16) &&
+         span_rows * stride * 2 < (int64_t(1) << 32);
+}
+
+// Large tiles where they fill the card, else smaller ones; a few rows have tiles
+// of their own.
+int tile_shape(int64_t down, int64_t across, bool narrow) {
+  if (ceil_div64(down, 256) * ceil_div64(across, 256) >= 256) return 2;
+  return narrow && across <= 64 ? 0 : 1;
+}
+
+CePlan lay_out(CeArgs &a, bool backward, void *work) {
+  CePlan p{};
+  p.planes = a.type == SPORDER_TYPE_F32 ? 2 : 1;
+  p.x_direct = direct_rows(a.type, a.dim, a.x_stride, a.x, a.rows);
+  p.w_direct = direct_rows(a.type, a.dim, a.w_stride, a.w, 256);
+  p.shape = tile_shape(a.classes, a.rows, !backward);
+  a.rows_pad = ceil_div64(a.rows, 256) * 256;
+  a.dim_pad = ceil_div64(a.dim, kStageK) * kStageK;
+  a.piece = ceil_div64(a.classes, 256) * 256;
+  if (backward) {
+    const int64_t most = std::max<int64_t>(1024, kPieceBytes / (a.rows_pad * 2 * p.planes) / 256 * 256);
+    if (a.piece > most) { // pieces of one size
+      const int64_t pieces = ceil_div64(a.piece, most);
+      a.piece = ceil_div64(ceil_div64(a.classes, pieces), 256) * 256;
+    }
+  }
+  a.classes_pad = ceil_div64(a.classes, a.piece) * a.piece;
+  const int span = p.shape == 2 ? 128 : p.shape == 1 ? 64 : 32; // classes of a wave
+  a.chunks = ceil_div64(ceil_div64(a.classes, span), p.shape == 0 ? 4 : 2) * (p.shape == 0 ? 4 : 2);
+  size_t at = 0;
+  auto take = [&](auto *&q, int64_t count) {
+    using P = std::remove_reference_t<decltype(*q)>;
+    q = reinterpret_cast<P *>(static_cast<char *>(work) + at);
+    at += Workspace::align(static_cast<size_t>(count) * sizeof(P));
+  };
+  take(a.meta, 1);
+  if (a.rows > kListDirect) take(a.counts, ceil_div64(a.rows, kListBlock));
+  take(a.list, a.rows_pad);
+  take(a.target, a.rows_pad);
+  take(a.bias32, a.classes_pad);
+  if (p.planes == 2) {
+    take(a.x_unit, a.rows_pad);
+    take(a.w_unit, a.classes_pad);
+  }
+  const int64_t row_bytes = a.dim_pad * 2;
+  a.x_packed = !p.x_direct;
+  if (p.x_direct) {
+    a.xp = static_cast<char *>(const_cast<void *>(a.x));
+    a.xp_stride = a.x_stride * 2;
+  } else {
+    a.xp_stride = row_bytes;
+    a.xp_plane = a.rows * row_bytes;
+    take(a.xp, a.xp_plane * p.planes);
+  }
+  if (p.w_direct) {
+    a.wp = static_cast<char *>(const_cast<void *>(a.w));
+    a.wp_stride = a.w_stride * 2;
+  } else {
+    a.wp_stride = row_bytes;
+    a.wp_plane = a.classes * row_bytes;
+    take(a.wp, a.wp_plane * p.planes);
+  }
+  if (!backward) {
+    take(a.hit, a.rows_pad);
+    take(a.partial, a.chunks * a.rows_pad);
+    take(a.sum_parts, 2 * kSumBlocks);
+  } else {
+    take(a.exponent, a.rows_pad);
+    take(a.mantissa, a.rows_pad);
+    take(a.row_lse, a.rows_pad);
+    if (p.planes == 2) {
+      take(a.x_most, a.dim);
+      take(a.w_most, a.dim);
+    }
+    take(a.xt, a.dim * a.rows_pad * 2 * p.planes);
+    take(a.wt, a.dim * a.piece * 2 * p.planes);
+    take(a.g, a.rows_pad * a.piece * 2 * p.planes);
+    take(a.gt, a.rows_pad * a.piece * 2 * p.planes);
+    if (a.piece < a.classes) take(a.dx32, a.rows_pad * a.dim_pad);
+    if (a.db) take(a.db_part, a.rows_pad / 64 * a.piece);
+  }
+  p.bytes = at;
+  return p;
+}
+
+// Runs steps until one fails.
+struct Steps {
+  int32_t rc = SPORDER_OK;
+  template <typename F> Steps &operator()(F &&f) {
+    if (rc == SPORDER_OK) rc = f();
+    return *this;
+  }
+};
+
+template <typename T, typename U, int PLANES> int32_t pack_operands(const CeArgs &a, const CePlan &p, void *stream) {
+  const T *const x = static_cast<const T *>(a.x), *const w = static_cast<const T *>(a.w);
+  Steps steps;
+  if (!p.x_direct)
+    steps([&] {
+      return launch(ce_pack_rows_kernel<T, U, PLANES>, dim3(ceil_div64(a.rows, 4)), dim3(256), stream, x,
+                    a.x_stride, a.rows, a.dim, a.meta, a.list, a.xp, a.xp_stride, a.xp_plane, a.x_unit);
+    });
+  if (!p.w_direct)
+    steps([&] {
+      return launch(ce_pack_rows_kernel<T, U, PLANES>, dim3(ceil_div64(a.classes, 4)), dim3(256), stream,
+                    w, a.w_stride, a.classes, a.dim, a.meta, static_cast<const int32_t *>(nullptr), a.wp,
+                    a.wp_stride, a.wp_plane, a.w_unit);
+    });
+  return steps.rc;
+}
+
+int32_t list_rows(const CeArgs &a, bool backward, void *stream) {
+  const int64_t first = std::max(a.classes_pad, backward ? a.dim : 1);
+  Steps steps;
+  steps([&] { return launch(ce_prepare_kernel, dim3(ceil_div64(first, 256)), dim3(256), stream, a, backward); });
+  const dim3 blocks(ceil_div64(a.rows, kListBlock));
+  if (a.rows > kListDirect)
+    steps([&] { return launch(ce_count_kernel, blocks, dim3(256), stream, a); });
+  steps([&] { return launch(ce_list_kernel, blocks, dim3(256), stream, a, backward); });
+  return steps.rc;
+}
+
+template <typename T, typename U, int PLANES> int32_t forward(const CeArgs &a, const CePlan &p, void *stream) {
+  Steps steps;
+  steps([&] { return list_rows(a, false, stream); });
+  steps([&] { return pack_operands<T, U, PLANES>(a, p, stream); });
+  auto go = [&](auto shape) {
+    using S = decltype(shape);
+    return launch(ce_loss_kernel<U, PLANES, S>,
+                  dim3(ceil_div64(a.classes, S::kM) * ceil_div64(a.rows, S::kN)), dim3(S::kThreads),
+                  stream, a);
+  };
+  steps([&] { return p.shape == 2 ? go(Large{}) : p.shape == 1 ? go(Middle{}) : go(Narrow{}); });
+  steps([&] { return launch(ce_join_kernel, dim3(ceil_div64(a.rows, 16)), dim3(256), stream, a); });
+  const int64_t blocks = std::min(ceil_div64(a.rows, kSumRows), kSumBlocks);
+  const int64_t per = ceil_div64(a.rows, blocks);
+  steps([&] { return launch(ce_sums_kernel, dim3(blocks), dim3(256), stream, a, per); });
+  if (blocks > 1)
+    steps([&] { return launch(ce_total_kernel, dim3(1), dim3(256), stream, a, static_cast<int>(blocks)); });
+  return steps.rc;
+}
+
+template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, const CePlan &p, void *stream) {
+  const T *const x = static_cast<const T *>(a.x), *const w = static_cast<const T *>(a.w);
+  const int32_t *const no_list = nullptr;
+  const float *const no_most = nullptr;
+  const float *const x_most = a.x_most, *const w_most = a.w_most;
+  Steps steps;
+  steps([&] { return list_rows(a, true, stream); });
+  steps([&] { return pack_operands<T, U, PLANES>(a, p, stream); });
+  if constexpr (PLANES == 2) {
+    steps([&] {
+      return launch(ce_column_most_kernel<T>, dim3(ceil_div64(a.dim, 64), std::min<int64_t>(ceil_div64(a.rows, 64), 256)),
+                    dim3(256), stream, x, a.x_stride, a.rows, a.dim, a.meta, a.list, a.x_most);
+    });
+    steps([&] {
+      return launch(ce_column_most_kernel<T>, dim3(ceil_div64(a.dim, 64), std::min<int64_t>(ceil_div64(a.classes, 64), 256)),
+                    dim3(256), stream, w, a.w_stride, a.classes, a.dim, a.meta, no_list, a.w_most);
+    });
+  }
+  steps([&] {
+    return launch(ce_pack_columns_kernel<T, U, PLANES>, dim3(ceil_div64(a.dim, 64), ceil_div64(a.rows, 64)),
+                  dim3(256), stream, x, a.x_stride, a.rows, a.dim, a.meta, a.list, a.exponent,
+                  PLANES == 2 ? x_most : no_most, a.xt, a.rows_pad * 2, a.dim * a.rows_pad * 2);
+  });
+  steps([&] { return launch(ce_zero_kernel<T>, dim3(ceil_div64(a.rows, 4)), dim3(256), stream, a); });
+  for (int64_t v0 = 0; v0 < a.classes; v0 += a.piece) {
+    const bool last = v0 + a.piece >= a.classes;
+    const int64_t here = std::min(a.piece, a.classes - v0);
+    steps([&] {
+      return launch(ce_pack_columns_kernel<T, U, PLANES>, dim3(ceil_div64(a.dim, 64), a.piece / 64),
+                    dim3(256), stream, w + v0 * a.w_stride, a.w_stride, here, a.dim, a.meta, no_list,
+                    no_list, PLANES == 2 ? w_most : no_most, a.wt, a.piece * 2, a.dim * a.piece * 2);
+    });
+    auto tiles = [&](auto shape) {
+      using S = decltype(shape);
+      return launch(ce_g_kernel<U, PLANES, S>, dim3(ceil_div64(here, S::kM) * ceil_div64(a.rows, S::kN)),
+                    dim3(S::kThreads), stream, a, v0);
+    };
+    const int shape = tile_shape(here, a.rows, false);
+    steps([&] { return shape == 2 ? tiles(Large{}) : tiles(Middle{}); });
+    if (a.db)
+      steps([&] {
+        return launch(ce_bias_kernel, dim3(a.piece / 64), dim3(256), stream, a, v0, shape == 2 ? 256 : 128);
+      });
+    auto dx = [&](auto shape) {
+      using S = decltype(shape);
+      return launch(ce_gradient_kernel<U, PLANES, S, T, true>,
+                    dim3(ceil_div64(a.dim, S::kM) * ceil_div64(a.rows, S::kN)), dim3(S::kThreads), stream,
+                    a, v0, v0 > 0, last);
+    };
+    steps([&] { return tile_shape(a.dim, a.rows, false) == 2 ? dx(Large{}) : dx(Middle{}); });
+    auto dw = [&](auto shape) {
+      using S = decltype(shape);
+      const dim3 grid(ceil_div64(a.dim, S::kM) * ceil_div64(here, S::kN));
+      if constexpr (sizeof(T) == 2) {
+        if (a.dw_type != SPORDER_TYPE_F32)
+          return launch(ce_gradient_kernel<U, PLANES, S, T, false>, grid, dim3(S::kThreads), stream, a, v0,
+                        false, true);
+      }
+      return launch(ce_gradient_kernel<U, PLANES, S, float, false>, grid, dim3(S::kThreads), stream, a, v0,
+                    false, true);
+    };
+    steps([&] { return tile_shape(a.dim, here, false) == 2 ? dw(Large{}) : dw(Middle{}); });
+  }
+  return steps.rc;
+}
+
+bool bad_sizes(const CeArgs &a) {
+  return !type_known(a.type) || !type_known(a.bias_type) || (a.target_bits != 32 && a.target_bits != 64) ||
+         a.rows < 0 || a.rows > kMostRows || a.dim < 1 || a.dim > kMostFeatures || a.classes < 1 ||
+         a.classes > kMostClasses || a.rows > kMostLogits / a.classes || a.x_stride < 0 || a.w_stride < 0;
+}
+
+template <typename T> __global__ void ce_nothing_kernel(CeArgs a) {
+  const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
+  const int64_t step = gridDim.x * int64_t(256);
+  for (int64_t k = i; k < a.classes * a.dim; k += step)
+    static_cast<T *>(a.dw)[k / a.dim * a.dw_stride + k % a.dim] = static_cast<T>(0.0f);
+  for (int64_t k = i; k < a.classes && a.db; k += step) store_typed(a.db, a.bias_type, k, 0.0f);
+}
+
+__global__ void ce_no_rows_kernel(CeArgs a) {
+  if (threadIdx.x < 2) a.sums[threadIdx.x] = 0.0f;
+}
+
+} // namespace
+
+} // namespace sporder_hip
+
+using namespace sporder_hip;
+
+extern "C" {
+
+size_t sporder_linear_cross_entropy_work_bytes(int32_t type, int64_t rows, int64_t dim, int64_t classes,
+                                               int64_t x_stride, const void *d_x,
+                                               int64_t weight_stride, const void *d_weight) {
+  CeArgs a{};
+  a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = 64;
+  a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
+  if (bad_sizes(a) || rows == 0) return 0;
+  return lay_out(a, false, nullptr).bytes;
+}
+
+int32_t sporder_linear_cross_entropy(void *stream, int32_t type, int64_t rows, int64_t dim,
+                                     int64_t classes, int64_t x_stride, const void *d_x,
+                                     int64_t weight_stride, const void *d_weight, int32_t bias_type,
+                                     const void *d_bias, int32_t target_bits, const void *d_targets,
+                                     int64_t ignore_index, float *d_loss, float *d_lse,
+                                     float *d_sums, void *d_work, size_t work_bytes) {
+  CeArgs a{};
+  a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = target_bits;
+  a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
+  a.bias_type = bias_type, a.bias = d_bias, a.targets = d_targets, a.ignore = ignore_index;
+  a.loss = d_loss, a.lse = d_lse, a.sums = d_sums;
+  if (bad_sizes(a) || !d_sums) return SPORDER_BAD_ARGUMENT;
+  if (rows == 0) return launch(ce_no_rows_kernel, dim3(1), dim3(kWave), stream, a);
+  if (!d_x || !d_weight || !d_targets || !d_loss || !d_lse || !d_work || !aligned_to(d_work, 256))
+    return SPORDER_BAD_ARGUMENT;
+  const CePlan p = lay_out(a, false, d_work);
+  if (work_bytes < p.bytes) return SPORDER_BAD_ARGUMENT;
+  if (type == SPORDER_TYPE_BF16) return forward<bf16_t, bf16_t, 1>(a, p, stream);
+  if (type == SPORDER_TYPE_F16) return forward<f16_t, f16_t, 1>(a, p, stream);
+  return forward<float, f16_t, 2>(a, p, stream);
+}
+
+size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows, int64_t dim,
+                                                    int64_t classes, int64_t x_stride,
+                                                    const void *d_x, int64_t weight_stride,
+                                                    const void *d_weight) {
+  CeArgs a{};
+  a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = 64;
+  a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
+  a.db = &a; // the scratch of a bias whether there is one or not
+  if (bad_sizes(a) || rows == 0) return 0;
+  return lay_out(a, true, nullptr).bytes;
+}
+
+int32_t sporder_linear_cross_entropy_grad(void *stream, int32_t type, int64_t rows, int64_t dim,
+                                          int64_t classes, int64_t grad_stride, const float *d_grad,
+                                          int64_t x_stride, const void *d_x, int64_t weight_stride,
+                                          const void *d_weight, int32_t bias_type,
+                                          const void *d_bias, int32_t target_bits,
+                                          const void *d_targets, int64_t ignore_index,
+                                          const float *d_lse, int64_t dx_stride, void *d_dx,
+                                          int32_t dweight_type, int64_t dweight_stride,
+                                          void *d_dweight, void *d_dbias, void *d_work,
+                                          size_t work_bytes) {
+  CeArgs a{};
+  a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = target_bits;
+  a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
+  a.bias_type = bias_type, a.bias = d_bias, a.targets = d_targets, a.ignore = ignore_index;
+  a.grad = d_grad, a.grad_stride = grad_stride, a.given_lse = d_lse;
+  a.dx = d_dx, a.dx_stride = dx_stride, a.dw = d_dweight, a.dw_stride = dweight_stride;
+  a.dw_type = dweight_type, a.db = d_dbias;
+  if (bad_sizes(a) || (dweight_type != type && dweight_type != SPORDER_TYPE_F32) || grad_stride < 0 ||
+      dx_stride < 0 || (rows > 1 && dx_stride < dim) || dweight_stride < 0 ||
+      (classes > 1 && dweight_stride < dim) || !d_dweight)
+    return SPORDER_BAD_ARGUMENT;
+  if (rows == 0) {
+    const dim3 grid(std::min<int64_t>(ceil_div64(classes * dim, 256), 1 << 16));
+    return dweight_type == SPORDER_TYPE_F32 ? launch(ce_nothing_kernel<float>, grid, dim3(256), stream, a)
+                                            : launch(ce_nothing_kernel<f16_t>, grid, dim3(256), stream, a);
+  }
+  if (!d_grad || !d_x || !d_weight || !d_targets || !d_lse || !d_dx || !d_work || !aligned_to(d_work, 256))
+    return SPORDER_BAD_ARGUMENT;
+  const CePlan p = lay_out(a, true, d_work);
+  if (work_bytes < p.bytes) return SPORDER_BAD_ARGUMENT;
+  if (type == SPORDER_TYPE_BF16) return backward<bf16_t, bf16_t, 1>(a, p, stream);
+  if (type == SPORDER_TYPE_F16) return backward<f16_t, f16_t, 1>(a, p, stream);
+  return backward<float, f16_t, 2>(a, p, stream);
+}
+
+} // extern "C"

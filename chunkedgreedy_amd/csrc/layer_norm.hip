@@ -15,7 +15,7 @@
 // backward) are read more than once.
 #include <algorithm>
 
-#include "dense.hpp"
+#include "norm.hpp"
 
 namespace sporder_hip {
 
@@ -38,63 +38,6 @@ struct NormGradArgs {
   float *partial; // [grid][2][dim] sums of dy h and dy, or null
   int weight_type;
 };
-
-// Sums of N values over the L lanes that hold a row, in each of them.  Past a
-// wave the waves' sums meet in `shared`; calls alternate between its halves
-// (`turn`), so that one barrier per call is enough: a wave writes a half again
-// only after the barrier of the call between.
-constexpr int norm_block(int lanes) { return lanes > 256 ? lanes : 256; }
-
-template <int L, int N> struct RowSum {
-  static constexpr int kWaves = L > kWave ? L / kWave : 1; // of a row
-  static constexpr int kBlockWaves = norm_block(L) / kWave;
-  float (*shared)[N][kBlockWaves];
-  int turn = 0;
-
-  __device__ __forceinline__ void operator()(float (&v)[N]) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = group_sum<(L < kWave ? L : kWave)>(v[i]);
-    if constexpr (L > kWave) {
-      const int wave = threadIdx.x / kWave;
-      if (threadIdx.x % kWave == 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) shared[turn][i][wave] = v[i];
-      }
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float *const row = shared[turn][i] + wave / kWaves * kWaves;
-        float s = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) s += row[w];
-        v[i] = s;
-      }
-      turn ^= 1;
-    }
-  }
-};
-
-// A lane's part of weight or bias, or `value` where there is none.
-template <bool LOOSE, int VEC, int L, int C>
-__device__ __forceinline__ void load_vector(const void *p, int type, int64_t dim, float value,
-                                            int lane, float (&out)[C][VEC]) {
-#pragma unroll
-  for (int c = 0; c < C; ++c) {
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) out[c][i] = value;
-  }
-  if (!p) return;
-  with_type(p, type, [&](auto *w) {
-#pragma unroll
-    for (int c = 0; c < C; ++c) {
-      const int col = (c * L + lane) * VEC;
-      if (col >= dim) continue;
-      const auto q = fetch<LOOSE, VEC>(w + col, dim - col);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) out[c][i] = static_cast<float>(q.v[i]);
-    }
-  });
-}
 
 // A row stays in the registers of its L lanes from its one read to its one
 // write; the variance is a second sum over the registers, so that a large mean
@@ -433,7 +376,6 @@ constexpr int64_t kNormGradMostDim = 512 * 32; // backward: dw and db are held t
 // f with a row's lanes and the elements of each, as types: the smallest group
 // that holds the row at 8 elements per lane up to 64, at 16 past them, and
 // past 8192 a workgroup of 512 with as many as `most` elements need.
-template <int N> using Const = std::integral_constant<int, N>;
 template <int MOST, typename F> int32_t with_lanes(int64_t dim, F &&f) {
   if (dim <= 16) return f(Const<2>{}, Const<8>{});
   if (dim <= 32) return f(Const<4>{}, Const<8>{});

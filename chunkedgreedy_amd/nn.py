@@ -64,6 +64,80 @@ def layer_norm(x, weight=None, bias=None, *, eps=1e-5):
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
+class _Dropout(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, p, seed, offset):
+        if isinstance(seed, torch.Tensor):
+            seed = seed.clone()  # the backward pass needs what this call reads
+            ctx.save_for_backward(seed)
+        ctx.p, ctx.seed, ctx.offset = p, seed, offset
+        return sporder.dropout(x, p, seed, offset=offset, residual=residual)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        (seed,) = ctx.saved_tensors or (ctx.seed,)
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = sporder.dropout(grad, ctx.p, seed, offset=ctx.offset)
+        return dx, grad if ctx.needs_input_grad[1] else None, None, None, None
+
+
+def dropout(x, p, seed, *, offset=0, residual=None, training=True):
+    """residual + dropout of x, whose mask follows from seed and offset
+    (``sporder.dropout``) and is made again for the gradient; x (plus residual)
+    itself where not ``training``."""
+    if not training:
+        return x if residual is None else x + residual
+    return _Dropout.apply(x, residual, p, seed, offset)
+
+
+class Dropout(torch.nn.Module):
+    """Dropout with its own seed and a count of its calls, held on the GPU so that
+    each replay of a captured step drops other elements."""
+
+    def __init__(self, p=0.5, seed=0):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise ValueError("p must be in [0, 1]")
+        self.p = p
+        self.register_buffer("state", torch.tensor([seed, 0], dtype=torch.int64))
+
+    def forward(self, x, residual=None):
+        out = dropout(x, self.p, self.state, residual=residual, training=self.training)
+        if self.training:
+            self.state[1] += 1
+        return out
+
+
+class _ResidualNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, residual, gate, post_weight, weight, scale, eps, post_norm):
+        ctx.set_materialize_grads(False)
+        y, h, post_rstd, rstd = sporder.residual_norm(x, residual, gate, post_weight, weight,
+                                                      scale=scale, eps=eps, post_norm=post_norm)
+        ctx.save_for_backward(x, y, post_rstd, rstd, gate, post_weight, weight)
+        ctx.scale, ctx.post_norm = scale, post_norm
+        return y, h
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y, grad_h):
+        x, y, post_rstd, rstd, gate, post_weight, weight = ctx.saved_tensors
+        dx, dresidual, dgate, dpost, dweight = sporder.residual_norm_grad(
+            grad_y, grad_h, x, y, post_rstd, rstd, gate, post_weight, weight, scale=ctx.scale,
+            post_norm=ctx.post_norm)
+        return (dx, dresidual if ctx.needs_input_grad[1] else None, dgate, dpost, dweight,
+                None, None, None)
+
+
+def residual_norm(x, residual=None, gate=None, post_weight=None, weight=None, *, scale=1.0,
+                  eps=1e-5, post_norm=True):
+    """(y, h): the residual stream after a block and the next block's input
+    (``sporder.residual_norm``), differentiable by all five tensors."""
+    return _ResidualNorm.apply(x, residual, gate, post_weight, weight, scale, eps, post_norm)
+
+
 class Muon(torch.optim.Optimizer):
     """Momentum whose update is orthogonalised, for parameters of two (or, as a
     batch of matrices, three) dimensions:

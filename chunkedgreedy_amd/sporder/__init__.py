@@ -10,7 +10,8 @@ Provided: chunk_similarity_greedy (sporder-csg), chunk_greedy (sporder-cg),
 reorder, count_pillars, similarity_graph, bench_cusparse_spmm, plus spmm_csr
 and chunk_similarity_top_k (new), and the operators of a training step
 around the SpMM (new): embedding, embedding_grad, layer_norm, layer_norm_grad,
-newton_schulz.  hierarchical_matching and
+newton_schulz, dropout, residual_norm, residual_norm_grad, linear_cross_entropy,
+linear_cross_entropy_grad.  hierarchical_matching and
 similarity_graph_exact exist for import compatibility and raise
 NotImplementedError.
 """
@@ -31,7 +32,9 @@ from ._sporder import spmm_csr as _spmm_csr
 from ._sporder import spmm_csr_noalloc as _spmm_csr_noalloc
 from ._sporder import spmm_csr_scaled as _spmm_csr_scaled
 from ._sporder import SpmmPlan
-from ._train import embedding, embedding_grad, layer_norm, layer_norm_grad, newton_schulz
+from ._train import (dropout, embedding, embedding_grad, layer_norm, layer_norm_grad,
+                     linear_cross_entropy, linear_cross_entropy_grad, newton_schulz,
+                     residual_norm, residual_norm_grad)
 
 __all__ = [
     "bench_cusparse_spmm",
@@ -40,13 +43,18 @@ __all__ = [
     "chunk_similarity_greedy",
     "chunk_similarity_top_k",
     "count_pillars",
+    "dropout",
     "embedding",
     "embedding_grad",
     "hierarchical_matching",
     "layer_norm",
     "layer_norm_grad",
+    "linear_cross_entropy",
+    "linear_cross_entropy_grad",
     "newton_schulz",
     "reorder",
+    "residual_norm",
+    "residual_norm_grad",
     "similarity_graph",
     "similarity_graph_exact",
     "spmm_csr",

@@ -333,3 +333,350 @@ def newton_schulz(g, *, steps=5, coefficients=(3.4445, -4.7750, 2.0315), eps=1e-
         raise ValueError(f"coefficients {(a, b, c)} take singular values past 31 within "
                          f"{steps} steps") from None
     return out
+
+
+def _seed_words(seed, offset):
+    """(seed, offset, state): host words, and a GPU tensor of two more or None."""
+    offset = int(offset)
+    if not 0 <= offset < 2**63:
+        raise ValueError("offset must be in [0, 2^63)")
+    if isinstance(seed, torch.Tensor):
+        if seed.dtype != torch.int64 or seed.shape != (2,) or not seed.is_cuda \
+                or not seed.is_contiguous():
+            raise ValueError("a seed on the GPU must be a contiguous int64 tensor (seed, offset)")
+        return 0, offset, seed
+    seed = int(seed)
+    if not 0 <= seed < 2**64:
+        raise ValueError("seed must be in [0, 2^64)")
+    return seed, offset, None
+
+
+def dropout(x, p, seed, *, offset=0, residual=None, out=None):
+    """Dropout whose mask follows from a counter and is never stored:
+    out = residual + (kept ? x / (1 - p) : 0).
+
+    Arguments:
+        x: float32, bfloat16 or float16 of any shape
+        p: probability of being dropped, in [0, 1] (in steps of 2^-32)
+        seed: int in [0, 2^64), or an int64 GPU tensor (seed, offset) that is
+            read when the work runs, so that a captured graph's replays can
+            each have another
+        offset: int in [0, 2^63), added to the tensor's; calls that are to drop
+            different elements under one seed have different offsets
+        residual: tensor of x's shape and type, or None
+        out: contiguous tensor of x's shape and type, or None; may be x or
+            residual
+
+    An element is kept by its index in x's shape alone (not by its type or
+    strides), so the gradient by x is ``dropout(grad, p, seed, offset=offset)``.
+    Dropped elements are 0 whatever x is there.  Returns out.
+    """
+    x = _floats(x, "x")
+    p = float(p)
+    if not 0.0 <= p <= 1.0:
+        raise ValueError("p must be in [0, 1]")
+    seed, offset, state = _seed_words(seed, offset)
+    if state is not None:
+        _same_device(state, x, "seed")
+    if residual is not None:
+        residual = _floats(residual, "residual")
+        if residual.shape != x.shape:
+            raise ValueError("residual must have x's shape")
+        if residual.dtype != x.dtype:
+            raise TypeError("residual must have x's type")
+        _same_device(residual, x, "residual")
+    out = _out(out, x.shape, x.dtype, x)
+    if x.numel() == 0:
+        return out
+    if x.dim() == 0:
+        x, residual = x[None], None if residual is None else residual[None]
+    dim = x.shape[-1]
+    x, rows, stride = _rows(x)
+    residual_stride = 0
+    if residual is not None:
+        residual, _, residual_stride = _rows(residual)
+    _call("sporder_dropout", x, _TYPES[x.dtype], rows, dim, stride, x.data_ptr(), residual_stride,
+          0 if residual is None else residual.data_ptr(), p, seed, offset,
+          0 if state is None else state.data_ptr(), dim, out.data_ptr())
+    return out
+
+
+def _block_inputs(x, gate, post_weight, weight, post_norm):
+    """(gate, post_weight, weight, their type, whether the gate has rows)."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x must have a last dimension of at least one element")
+    dim = x.shape[-1]
+    by_row = gate is not None and getattr(gate, "ndim", 1) == x.dim() > 1
+    if by_row:
+        gate = _like(gate, "gate", x)
+    elif gate is not None:
+        gate = _norm_vector(gate, "gate", dim, x)
+    if post_weight is not None:
+        if not post_norm:
+            raise ValueError("post_weight is the weight of the norm that post_norm=False leaves out")
+        post_weight = _norm_vector(post_weight, "post_weight", dim, x)
+    if weight is not None:
+        weight = _norm_vector(weight, "weight", dim, x)
+    kinds = {t.dtype for t in (None if by_row else gate, post_weight, weight) if t is not None}
+    if len(kinds) > 1:
+        raise TypeError("weights and a gate of shape (dim,) must have the same type")
+    return gate, post_weight, weight, kinds.pop() if kinds else torch.float32, by_row
+
+
+def _like(a, name, x):
+    t = _floats(a, name)
+    if t.shape != x.shape:
+        raise ValueError(f"{name} must have x's shape")
+    if t.dtype != x.dtype:
+        raise TypeError(f"{name} must have x's type")
+    _same_device(t, x, name)
+    return t
+
+
+def _row_args(t):
+    """(tensor to keep, stride, address) of an optional tensor of rows."""
+    if t is None:
+        return None, 0, 0
+    t, _, stride = _rows(t)
+    return t, stride, t.data_ptr()
+
+
+def _address(t):
+    return 0 if t is None else t.data_ptr()
+
+
+def residual_norm(x, residual=None, gate=None, post_weight=None, weight=None, *, scale=1.0,
+                  eps=1e-5, post_norm=True):
+    """The norms after a block and before the next one, with the block's gate
+    and residual scale:
+
+        y = residual + scale * gate * post_weight * x * post_rstd
+        h = weight * y * rstd
+
+    with post_rstd = (mean x^2 + eps)^-1/2 and rstd = (mean y^2 + eps)^-1/2 of
+    each row (root mean square norms).
+
+    Arguments:
+        x: (..., dim) float32, bfloat16 or float16, the block's output; rows a
+            fixed number of elements apart are read in place, other strides
+            are copied
+        residual: the residual stream, of x's shape and type, or None (0)
+        gate: (dim,) like the weights, or of x's shape and type, or None (1)
+        post_weight, weight: (dim,) of x's type or float32, or None (1); they
+            and a gate of (dim,) have one type
+        scale: factor of the block's part
+        eps: >= 0
+        post_norm: whether x is normalised; if not, post_rstd is 1
+
+    Returns (y, h, post_rstd, rstd): y, the new residual stream, and h, the next
+    block's input, of x's shape and type; post_rstd and rstd are float32 of
+    shape x.shape[:-1], as :func:`residual_norm_grad` takes them.  Sums are held
+    in 32 bits, and h is made of y before its rounding.
+    """
+    x = _floats(x, "x")
+    gate, post_weight, weight, kind, by_row = _block_inputs(x, gate, post_weight, weight, post_norm)
+    if not eps >= 0.0:
+        raise ValueError("eps must be >= 0")
+    if residual is not None:
+        residual = _like(residual, "residual", x)
+    y = _out(None, x.shape, x.dtype, x)
+    h = torch.empty_like(y)
+    post_rstd = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    rstd = torch.empty_like(post_rstd)
+    dim = x.shape[-1]
+    x, rows, stride = _rows(x)
+    residual, residual_stride, residual_at = _row_args(residual)
+    gate, gate_stride, gate_at = _row_args(gate) if by_row else (gate, 0, _address(gate))
+    _call("sporder_residual_norm", x, _TYPES[x.dtype], _TYPES[kind], rows, dim, stride,
+          x.data_ptr(), residual_stride, residual_at, int(by_row), gate_stride, gate_at,
+          _address(post_weight), _address(weight), float(scale), float(eps), int(bool(post_norm)),
+          dim, y.data_ptr(), dim, h.data_ptr(), post_rstd.data_ptr(), rstd.data_ptr())
+    return y, h, post_rstd, rstd
+
+
+def residual_norm_grad(grad_y, grad_h, x, y, post_rstd, rstd, gate=None, post_weight=None,
+                       weight=None, *, scale=1.0, post_norm=True):
+    """Gradients of :func:`residual_norm`.
+
+    Arguments:
+        grad_y, grad_h: the gradients by y and h, of x's shape and type; either
+            may be None (0)
+        x, gate, post_weight, weight, scale, post_norm: as in the forward call
+        y, post_rstd, rstd: as it returned them
+
+    Returns (dx, dresidual, dgate, dpost_weight, dweight), None for what was
+    not given (dresidual is returned always); each has its tensor's type.  Sums over the
+    rows are held in 32 bits in an order that depends on the sizes and the
+    inputs' types, strides and alignment: the same call gives the same bits
+    from run to run.
+    """
+    x = _floats(x, "x")
+    gate, post_weight, weight, kind, by_row = _block_inputs(x, gate, post_weight, weight, post_norm)
+    y = _like(y, "y", x)
+    if grad_y is not None:
+        grad_y = _like(grad_y, "grad_y", x)
+    if grad_h is not None:
+        grad_h = _like(grad_h, "grad_h", x)
+    for t, name in ((post_rstd, "post_rstd"), (rstd, "rstd")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 \
+                or t.shape != x.shape[:-1] or t.device != x.device or not t.is_contiguous():
+            raise ValueError(f"{name} must be the contiguous float32 tensor that residual_norm "
+                             f"returned, of shape {tuple(x.shape[:-1])} on {x.device}")
+    dx = _out(None, x.shape, x.dtype, x)
+    dresidual = torch.empty_like(dx)
+    dgate = None
+    if gate is not None:
+        dgate = torch.empty_like(dx) if by_row else torch.empty_like(gate)
+    dpost = None if post_weight is None else torch.empty_like(post_weight)
+    dweight = None if weight is None else torch.empty_like(weight)
+    dim = x.shape[-1]
+    x, rows, stride = _rows(x)
+    y, _, y_stride = _rows(y)
+    grad_y, dy_stride, dy_at = _row_args(grad_y)
+    grad_h, dh_stride, dh_at = _row_args(grad_h)
+    gate, gate_stride, gate_at = _row_args(gate) if by_row else (gate, 0, _address(gate))
+    size = 0
+    if not by_row and gate is not None or dpost is not None or dweight is not None:
+        size = _lib.load().sporder_residual_norm_grad_work_bytes(rows, dim)
+    work = x.new_empty(size, dtype=torch.uint8) if size else None
+    _call("sporder_residual_norm_grad", x, _TYPES[x.dtype], _TYPES[kind], rows, dim, dy_stride,
+          dy_at, dh_stride, dh_at, stride, x.data_ptr(), y_stride, y.data_ptr(),
+          post_rstd.data_ptr(), rstd.data_ptr(), int(by_row), gate_stride, gate_at,
+          _address(post_weight), _address(weight), float(scale), int(bool(post_norm)), dim,
+          dx.data_ptr(), dim, dresidual.data_ptr(), dim, _address(dgate), _address(dpost),
+          _address(dweight), _address(work), size)
+    return dx, dresidual, dgate, dpost, dweight
+
+
+def _loss_inputs(x, weight, targets, bias):
+    """(x of two dimensions, its stride, weight, its stride, targets, bias)."""
+    x = _floats(x, "x")
+    weight = _floats(weight, "weight")
+    if x.dim() < 1 or x.shape[-1] < 1 or x.shape[-1] > 65536:
+        raise ValueError("x must have a last dimension of 1 to 65536 elements")
+    if weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] != x.shape[-1]:
+        raise ValueError(f"weight must be a (classes, {x.shape[-1]}) tensor")
+    if weight.dtype != x.dtype:
+        raise TypeError("weight must have x's type")
+    _same_device(weight, x, "weight")
+    targets = _as_tensor(targets, "targets")
+    if not targets.is_cuda:
+        raise TypeError("targets must be a GPU tensor")
+    if targets.dtype not in _TOKEN_BITS:
+        raise TypeError(f"targets must be int32 or int64, got {targets.dtype}")
+    _same_device(targets, x, "targets")
+    if targets.shape != x.shape[:-1]:
+        raise ValueError("targets must have the shape of x without its last dimension")
+    if bias is not None:
+        bias = _floats(bias, "bias")
+        if bias.dtype not in (x.dtype, torch.float32):
+            raise TypeError(f"bias must have x's type or float32, got {bias.dtype}")
+        if bias.shape != weight.shape[:1]:
+            raise ValueError(f"bias must have shape ({weight.shape[0]},)")
+        _same_device(bias, x, "bias")
+        bias = bias if bias.is_contiguous() else bias.contiguous()
+    classes, rows = weight.shape[0], targets.numel()
+    if rows >= 2**23 - 255 or classes > 2**25 or rows * classes > 2**37:
+        raise ValueError("at most 2^23 - 256 rows, 2^25 classes and 2^37 logits")
+    x, _, x_stride = _rows(x)
+    weight, _, weight_stride = _rows(weight)
+    targets = targets if targets.is_contiguous() else targets.contiguous()
+    return x, x_stride, weight, weight_stride, targets, bias
+
+
+def _ignored(ignore_index):
+    ignore_index = int(ignore_index)
+    if not -(2**63) <= ignore_index < 2**63:
+        raise ValueError("ignore_index must fit 64 bits")
+    return ignore_index
+
+
+def linear_cross_entropy(x, weight, targets, bias=None, *, ignore_index=-100):
+    """Softmax cross entropy of the logits z = x weight^T + bias, which are
+    never kept: lse = log sum exp z, loss = lse - z[target], by row.
+
+    Arguments:
+        x: (..., dim) float32, bfloat16 or float16; rows a fixed number of
+            elements apart are read in place, other strides are copied
+        weight: (classes, dim) of x's type
+        targets: int32 or int64 of shape x.shape[:-1]
+        bias: (classes,) of x's type or float32, or None; -inf leaves a class out
+        ignore_index: rows with this target have loss and lse 0 and are not read
+
+    Returns (loss, lse, sums): loss and lse float32 of the targets' shape (NaN
+    for a target that is neither a class nor ignored), sums float32 (2,) of the
+    losses' sum and the number of rows that are not ignored.  At most 2^23 - 256
+    rows, 2^25 classes and 65536 elements a row.
+
+    Sums are held in 32 bits.  float32 products have operands of 22 bits: a term
+    is within 2^-21 of itself, and within some 2^-38 of the product of its rows'
+    largest elements; a row that holds an infinity gives NaN.
+    """
+    x, x_stride, weight, weight_stride, targets, bias = _loss_inputs(x, weight, targets, bias)
+    ignore_index = _ignored(ignore_index)
+    rows, (classes, dim) = targets.numel(), weight.shape
+    loss = torch.empty(targets.shape, dtype=torch.float32, device=x.device)
+    lse = torch.empty_like(loss)
+    sums = x.new_empty(2, dtype=torch.float32)
+    sizes = (_TYPES[x.dtype], rows, dim, classes, x_stride, x.data_ptr(), weight_stride,
+             weight.data_ptr())
+    size = _lib.load().sporder_linear_cross_entropy_work_bytes(*sizes)
+    work = x.new_empty(size, dtype=torch.uint8) if size else None
+    _call("sporder_linear_cross_entropy", x, *sizes, _TYPES[x.dtype if bias is None else bias.dtype],
+          _address(bias), _TOKEN_BITS[targets.dtype], targets.data_ptr(), ignore_index,
+          loss.data_ptr(), lse.data_ptr(), sums.data_ptr(), _address(work), size)
+    return loss, lse, sums
+
+
+def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignore_index=-100,
+                              dtype=None):
+    """Gradients of :func:`linear_cross_entropy` by x, weight and bias.
+
+    Arguments:
+        grad: the gradient by the losses, float32 of the targets' shape or of
+            one element for all rows
+        x, weight, targets, bias, ignore_index: as in the forward call
+        lse: as it returned it
+        dtype: weight's type (default) or float32, the type of weight's gradient
+
+    Returns (dx, dweight, dbias), dbias None without a bias.  The logits are
+    made again, a piece of the classes at a time; rows that are ignored, or
+    whose target is no class, have no gradient.  g = grad (exp(z - lse) -
+    [target]) is rounded to x's type before its products with weight and x
+    (22 bits for float32), whose sums are held in 32 bits.  The same call gives
+    the same bits from run to run.
+    """
+    x_shape = x.shape
+    x, x_stride, weight, weight_stride, targets, bias = _loss_inputs(x, weight, targets, bias)
+    ignore_index = _ignored(ignore_index)
+    rows, (classes, dim) = targets.numel(), weight.shape
+    for t, name in ((grad, "grad"), (lse, "lse")):
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or not t.is_cuda:
+            raise TypeError(f"{name} must be a float32 GPU tensor")
+        _same_device(t, x, name)
+    if lse.shape != targets.shape:
+        raise ValueError("lse must have the targets' shape")
+    if grad.shape != targets.shape and grad.numel() != 1:
+        raise ValueError("grad must have the targets' shape or one element")
+    if dtype is None:
+        dtype = weight.dtype
+    elif dtype not in (weight.dtype, torch.float32):
+        raise ValueError("dtype must be weight's type or float32")
+    lse = lse if lse.is_contiguous() else lse.contiguous()
+    one = grad.numel() == 1 or all(s == 0 for s in grad.stride())
+    if not one and not grad.is_contiguous():
+        grad = grad.contiguous()
+    dx = x.new_empty(x_shape)
+    dweight = weight.new_empty(weight.shape, dtype=dtype)
+    dbias = None if bias is None else torch.empty_like(bias)
+    sizes = (x_stride, x.data_ptr(), weight_stride, weight.data_ptr())
+    size = _lib.load().sporder_linear_cross_entropy_grad_work_bytes(_TYPES[x.dtype], rows, dim,
+                                                                    classes, *sizes)
+    work = x.new_empty(size, dtype=torch.uint8) if size else None
+    _call("sporder_linear_cross_entropy_grad", x, _TYPES[x.dtype], rows, dim, classes,
+          0 if one else 1, grad.data_ptr(), *sizes,
+          _TYPES[x.dtype if bias is None else bias.dtype], _address(bias),
+          _TOKEN_BITS[targets.dtype], targets.data_ptr(), ignore_index, lse.data_ptr(), dim,
+          dx.data_ptr(), _TYPES[dtype], dim, dweight.data_ptr(), _address(dbias), _address(work),
+          size)
+    return dx, dweight, dbias

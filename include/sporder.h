@@ -521,6 +521,101 @@ SPORDER_API int32_t sporder_newton_schulz(void *stream, int32_t type, int64_t ba
                                           double a, double b, double c, double eps, void *d_out,
                                           void *d_work, size_t work_bytes);
 
+/*
+ * Dropout from a counter: d_out = residual + (u >= round(p 2^32) ? x / (1 - p) : 0) for
+ * each of rows x dim elements (rows x_stride, residual_stride and out_stride elements
+ * apart; d_residual may be NULL: 0), p in [0, 1].  u are 32 bits that follow from the
+ * element's index i = row dim + column, `seed` and `offset` (below 2^63) alone, so the
+ * gradient by x is the same call on the gradient, without a residual:
+ * u = 2^16 H + L, where H is half i % 2 (0: low, 1: high) of word i / 2 % 4 of the
+ * Philox4x32-10 block with key `seed` and the 128-bit counter i / 8 + 2^64 offset, and L
+ * the same of the one with counter i / 8 + 2^64 (offset + 2^63).  d_state, where not NULL,
+ * is two words on the device, read when the work runs and added to seed and offset (modulo
+ * 2^64 and 2^63).  d_out may be d_x or d_residual.
+ */
+SPORDER_API int32_t sporder_dropout(void *stream, int32_t type, int64_t rows, int64_t dim,
+                                    int64_t x_stride, const void *d_x, int64_t residual_stride,
+                                    const void *d_residual, double p, uint64_t seed,
+                                    uint64_t offset, const uint64_t *d_state,
+                                    int64_t out_stride, void *d_out);
+
+/*
+ * The norms after a block and before the next one:
+ *   y = residual + scale gate post_weight x post_rstd,  post_rstd = (mean x^2 + eps)^-1/2
+ *   h = weight y rstd,  rstd = (mean y^2 + eps)^-1/2
+ * for each of `rows` rows of `dim` elements of `type`; without post_norm, post_rstd is 1
+ * (and there is no post_weight).  d_residual (0), d_gate, d_post_weight and d_weight (1) may
+ * be NULL; the weights have dim elements of vector_type, and so has the gate, or it is of
+ * `type` with rows of its own (gate_by_row).  h is made of y before its rounding.  Outputs
+ * do not overlap inputs.
+ */
+SPORDER_API int32_t sporder_residual_norm(
+    void *stream, int32_t type, int32_t vector_type, int64_t rows, int64_t dim, int64_t x_stride,
+    const void *d_x, int64_t residual_stride, const void *d_residual, int32_t gate_by_row,
+    int64_t gate_stride, const void *d_gate, const void *d_post_weight, const void *d_weight,
+    float scale, float eps, int32_t post_norm, int64_t y_stride, void *d_y, int64_t h_stride,
+    void *d_h, float *d_post_rstd, float *d_rstd);
+
+/*
+ * Its gradients from dy and dh (either may be NULL: 0), the call's x, y, post_rstd and rstd:
+ * d_dx and d_dresidual by row; d_dgate by row where the gate is, else of dim elements of
+ * vector_type like d_dpost_weight and d_dweight, which may be NULL.  d_work, needed where
+ * there is one of those three, is 256-byte aligned.
+ */
+SPORDER_API size_t sporder_residual_norm_grad_work_bytes(int64_t rows, int64_t dim);
+SPORDER_API int32_t sporder_residual_norm_grad(
+    void *stream, int32_t type, int32_t vector_type, int64_t rows, int64_t dim, int64_t dy_stride,
+    const void *d_dy, int64_t dh_stride, const void *d_dh, int64_t x_stride, const void *d_x,
+    int64_t y_stride, const void *d_y, const float *d_post_rstd, const float *d_rstd,
+    int32_t gate_by_row, int64_t gate_stride, const void *d_gate, const void *d_post_weight,
+    const void *d_weight, float scale, int32_t post_norm, int64_t dx_stride, void *d_dx,
+    int64_t dresidual_stride, void *d_dresidual, int64_t dgate_stride, void *d_dgate,
+    void *d_dpost_weight, void *d_dweight, void *d_work, size_t work_bytes);
+
+/*
+ * Softmax cross entropy of the logits z = x w^T + bias, which are not kept:
+ *   d_lse[t] = log sum_v exp z[t][v],  d_loss[t] = d_lse[t] - z[t][target]
+ * for `rows` rows of x and `classes` rows of w, of dim elements of `type` (rows x_stride and
+ * weight_stride elements apart), a bias of `classes` elements of bias_type or NULL, and
+ * targets of target_bits (32 or 64, signed).  A row whose target is ignore_index has loss
+ * and lse 0 and is not read; one whose target is no class otherwise has NaN.  d_sums
+ * receives the sum of the losses and the number of rows whose target is not ignore_index.
+ * dim is at most 65536, classes 2^25, rows 2^23 - 256, rows times classes 2^37.  d_work is
+ * 256-byte aligned and of the size that *_work_bytes gives for the same sizes, strides
+ * and alignments.
+ */
+SPORDER_API size_t sporder_linear_cross_entropy_work_bytes(int32_t type, int64_t rows,
+                                                           int64_t dim, int64_t classes,
+                                                           int64_t x_stride, const void *d_x,
+                                                           int64_t weight_stride,
+                                                           const void *d_weight);
+SPORDER_API int32_t sporder_linear_cross_entropy(
+    void *stream, int32_t type, int64_t rows, int64_t dim, int64_t classes, int64_t x_stride,
+    const void *d_x, int64_t weight_stride, const void *d_weight, int32_t bias_type,
+    const void *d_bias, int32_t target_bits, const void *d_targets, int64_t ignore_index,
+    float *d_loss, float *d_lse, float *d_sums, void *d_work, size_t work_bytes);
+
+/*
+ * Its gradients, with g[t][v] = grad[t] (exp(z[t][v] - lse[t]) - [v = target]) for rows whose
+ * target is a class and 0 for the others: d_dx = g w (of `type`), d_dweight = g^T x (of
+ * dweight_type: `type` or SPORDER_TYPE_F32) and, where not NULL, d_dbias = sum_t g (of
+ * bias_type).  d_grad has elements grad_stride apart (0: one for all rows); d_lse is the
+ * forward call's.  g is rounded to `type` before the products of 16-bit types.
+ */
+SPORDER_API size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows,
+                                                                int64_t dim, int64_t classes,
+                                                                int64_t x_stride,
+                                                                const void *d_x,
+                                                                int64_t weight_stride,
+                                                                const void *d_weight);
+SPORDER_API int32_t sporder_linear_cross_entropy_grad(
+    void *stream, int32_t type, int64_t rows, int64_t dim, int64_t classes, int64_t grad_stride,
+    const float *d_grad, int64_t x_stride, const void *d_x, int64_t weight_stride,
+    const void *d_weight, int32_t bias_type, const void *d_bias, int32_t target_bits,
+    const void *d_targets, int64_t ignore_index, const float *d_lse, int64_t dx_stride, void *d_dx,
+    int32_t dweight_type, int64_t dweight_stride, void *d_dweight, void *d_dbias, void *d_work,
+    size_t work_bytes);
+
 #ifdef __cplusplus
 }
 #endif

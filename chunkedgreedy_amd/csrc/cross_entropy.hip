@@ -16,15 +16,20 @@
 // along another side of it; the piece's rows of dw are then final and dx is
 // summed over the pieces in 32 bits.  The pieces' size bounds the scratch.
 //
-// 16-bit types.  g is rounded to the type before its products (a relative 2^-9 or
-// 2^-12 of each term, as its factors in w and x are already rounded): the matrix
-// units take 16 bits.  A token's scale s = m 2^e enters as m, with 1 <= |m| < 2,
-// times 2^13, so that float16 keeps 11 bits down to g = 2^-27; 2^e goes to dx in
-// 32 bits and to dw with x's rows, where it is exact.
-// 32-bit types.  Operands are two 16-bit halves (22 bits) in units of their row, a
-// power of two by its largest element, and products are three.
+// Types.  The matrix units take 16 bits.  The logits' operands are x and w themselves
+// where those are 16 bits wide.  g is rounded to float16 before its products whatever
+// the type (to bfloat16, one term with the target's class would bring an error of up
+// to 2^-9 into a whole row: dx and dw 3.1e-3 off instead of 1.7e-3, which is the
+// rounding of the results), and so w and x are float16 there, in units of their
+// columns, powers of two by the largest element: bfloat16 values are exact down to
+// 2^-29 of it, smaller ones within 2^-40 of it.  A token's scale s = m 2^e enters g as
+// m, with 1 <= |m| < 2, times 2^13, so that 11 bits are kept down to g = 2^-27; 2^e goes
+// to dx in 32 bits and to dw with x's rows.
+// 32-bit operands are two 16-bit halves (22 bits) in units of their row, a power of two
+// by its largest element, and products are three.
 #include <algorithm>
 
+#include "cross_entropy.hpp"
 #include "mfma_product.hpp"
 
 namespace sporder_hip {
@@ -32,7 +37,6 @@ namespace sporder_hip {
 namespace {
 
 constexpr int kShift = 13; // g is held 2^13 times as large
-constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kListBlock = 1024; // rows of a block of the list
 constexpr int64_t kListDirect = 65536; // rows up to which a block counts those before it
 
@@ -41,20 +45,7 @@ struct CeMeta {
   int32_t most;  // largest exponent of their scales
 };
 
-struct CeArgs {
-  int64_t rows, dim, classes;
-  int64_t x_stride, w_stride; // elements
-  const void *x, *w, *bias, *targets;
-  int64_t ignore;
-  int type, bias_type, target_bits;
-  // forward
-  float *loss, *lse, *sums;
-  // backward
-  const float *grad, *given_lse;
-  int64_t grad_stride;
-  void *dx, *dw, *db;
-  int64_t dx_stride, dw_stride;
-  int dw_type;
+struct CeArgs : CeCall {
   // scratch
   CeMeta *meta;
   int32_t *counts;       // of the list's blocks, past kListDirect rows
@@ -70,20 +61,13 @@ struct CeArgs {
   bool x_packed;      // by list position
   float *x_unit, *w_unit; // of their rows (32-bit types)
   char *xt, *wt;      // transposed operands, [dim][rows_pad] and [dim][piece]
-  float *x_most, *w_most; // [dim]: largest of each column, as bits
+  float *x_most, *w_most; // [dim]: largest of each column
   char *g, *gt;       // [rows_pad][piece] and [piece][rows_pad]
-  float *dx32;        // [rows_pad][dim_pad]
+  float *dx_part;     // [splits][rows_pad][dim_pad]
+  float *dw_part;     // [splits][piece][dim_pad]
   float *db_part;     // [token chunks][piece]
   int64_t rows_pad, dim_pad, classes_pad, chunks, piece;
 };
-
-__device__ __forceinline__ int64_t target_of(const CeArgs &a, int64_t row) {
-  return a.target_bits == 64 ? static_cast<const int64_t *>(a.targets)[row]
-                             : static_cast<const int32_t *>(a.targets)[row];
-}
-__device__ __forceinline__ bool counted(const CeArgs &a, int64_t target) {
-  return target != a.ignore && target >= 0 && target < a.classes;
-}
 
 // ---- the list of rows, and what else comes first -----------------------------------
 
@@ -99,7 +83,7 @@ __global__ void __launch_bounds__(256) ce_prepare_kernel(CeArgs a, bool backward
     a.bias32[i] = b;
   }
   if (a.w_unit && i >= a.classes && i < a.classes_pad) a.w_unit[i] = 1.0f;
-  if (backward && i < a.dim && a.x_most) {
+  if (backward && i < a.dim) {
     a.x_most[i] = 0.0f;
     a.w_most[i] = 0.0f;
   }
@@ -246,39 +230,44 @@ __global__ void __launch_bounds__(256)
 }
 
 // The largest element of each column of rows of x (listed) or w, as the bits of a
-// non-negative float: their order is the floats'.  64 columns and a strip of rows
-// per workgroup.
+// non-negative float: their order is the floats'.  A strip of rows and 64 accesses'
+// columns per workgroup.
 template <typename T>
 __global__ void __launch_bounds__(256)
     ce_column_most_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
                           const int32_t *list, float *most) {
+  constexpr int kVec = 16 / sizeof(T);
   const int64_t all = list ? meta->count : rows;
-  const int64_t col = blockIdx.x * int64_t(64) + threadIdx.x % 64;
+  const int64_t col = (blockIdx.x * int64_t(64) + threadIdx.x % 64) * kVec;
   if (col >= dim) return;
-  float m = 0.0f;
+  float m[kVec] = {};
 #pragma unroll 4
-  for (int64_t r = blockIdx.y * int64_t(4) + threadIdx.x / 64; r < all; r += gridDim.y * int64_t(4))
-    m = fmaxf(m, fabsf(static_cast<float>(src[(list ? list[r] : r) * stride + col])));
-  atomicMax(reinterpret_cast<uint32_t *>(most) + col, __builtin_bit_cast(uint32_t, m));
+  for (int64_t r = blockIdx.y * int64_t(4) + threadIdx.x / 64; r < all; r += gridDim.y * int64_t(4)) {
+    const auto q = fetch<true, kVec>(src + (list ? list[r] : r) * stride + col, dim - col);
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) m[e] = fmaxf(m[e], fabsf(static_cast<float>(q.v[e])));
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; ++e)
+    if (col + e < dim) atomicMax(reinterpret_cast<uint32_t *>(most) + col + e, __builtin_bit_cast(uint32_t, m[e]));
 }
 
 // Columns of rows of x (listed) or w as operand rows: out[j][k] of k-th row,
 // zeros for k past the rows up to a multiple of 64.  64 x 64 per workgroup,
 // turned in LDS.  Listed rows come with 2^(their exponent - the largest).
-template <typename T, typename U, int PLANES>
+template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
     ce_pack_columns_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
                            const int32_t *list, const int32_t *exponent, const float *most, char *out,
                            int64_t out_stride, int64_t plane) {
   __shared__ float tile[64][65];
   const int64_t all = list ? meta->count : rows;
-  const int64_t k0 = blockIdx.y * int64_t(64), j0 = blockIdx.x * int64_t(64);
+  const int64_t k0 = blockIdx.x * int64_t(64), j0 = blockIdx.y * int64_t(64);
   if (k0 >= all) return;
   const int x = threadIdx.x % 64, y = threadIdx.x / 64;
   const int top = list ? meta->most : 0;
   const bool in = j0 + x < dim;
-  float scale = 1.0f;
-  if constexpr (PLANES == 2) scale = in ? unit_inverse(unit_of(most[j0 + x])) : 0.0f;
+  const float scale = in ? unit_inverse(unit_of(most[j0 + x])) : 0.0f;
 #pragma unroll
   for (int i = 0; i < 16; ++i) {
     const int64_t k = k0 + y + 4 * i;
@@ -294,18 +283,13 @@ __global__ void __launch_bounds__(256)
   for (int i = 0; i < 2; ++i) {
     const int j = threadIdx.x / 8 + 32 * i, c = threadIdx.x % 8 * 8;
     if (j0 + j >= dim) continue;
-    Pack<U, 8> hi, lo;
+    Pack<f16_t, 8> hi, lo;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (PLANES == 2)
-        split(tile[c + e][j], hi.v[e], lo.v[e]);
-      else
-        hi.v[e] = static_cast<U>(tile[c + e][j]);
-    }
-    U *const to = reinterpret_cast<U *>(out + (j0 + j) * out_stride) + k0 + c;
-    *reinterpret_cast<Pack<U, 8> *>(to) = hi;
+    for (int e = 0; e < 8; ++e) split(tile[c + e][j], hi.v[e], lo.v[e]);
+    f16_t *const to = reinterpret_cast<f16_t *>(out + (j0 + j) * out_stride) + k0 + c;
+    *reinterpret_cast<Pack<f16_t, 8> *>(to) = hi;
     if constexpr (PLANES == 2)
-      *reinterpret_cast<Pack<U, 8> *>(reinterpret_cast<char *>(to) + plane) = lo;
+      *reinterpret_cast<Pack<f16_t, 8> *>(reinterpret_cast<char *>(to) + plane) = lo;
   }
 }
 
@@ -404,7 +388,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_loss_kernel(CeArgs a) {
 #pragma unroll
     for (int i = 0; i < S::MB; ++i) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2e);
+      for (int r = 0; r < 16; ++r) sum += exp_of(acc[i][j][r] - base);
     }
     sum += lane_xor_f32(sum, 32);
     if (lane < 32 && n < count)
@@ -425,7 +409,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeArgs a) {
     for (int64_t c = y; c < a.chunks; c += 16) {
       const float2 p = a.partial[c * a.rows_pad + n];
       const float m = fmaxf(most, p.x), base = m == -INFINITY ? 0.0f : m;
-      sum = sum * __builtin_amdgcn_exp2f((most - base) * kLog2e) + p.y * __builtin_amdgcn_exp2f((p.x - base) * kLog2e);
+      sum = sum * exp_of(most - base) + p.y * exp_of(p.x - base);
       most = m;
     }
   }
@@ -435,7 +419,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeArgs a) {
   for (int k = 1; k < 16; ++k) most = fmaxf(most, part[k][x].x);
   const float base = most == -INFINITY ? 0.0f : most;
   sum = 0.0f;
-  for (int k = 0; k < 16; ++k) sum += part[k][x].y * __builtin_amdgcn_exp2f((part[k][x].x - base) * kLog2e);
+  for (int k = 0; k < 16; ++k) sum += part[k][x].y * exp_of(part[k][x].x - base);
   const float lse = base + logf(sum);
   a.lse[a.list[n]] = lse;
   a.loss[a.list[n]] = lse - a.hit[n];
@@ -446,19 +430,6 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeArgs a) {
 constexpr int64_t kSumRows = 8192; // of a workgroup, or more
 constexpr int64_t kSumBlocks = 256;
 
-__device__ __forceinline__ void block_sums(double s, double n, double (&part)[2][4]) {
-#pragma unroll
-  for (int j = 1; j < kWave; j <<= 1) {
-    s += __shfl_xor(s, j);
-    n += __shfl_xor(n, j);
-  }
-  if (lane_id() == 0) {
-    part[0][threadIdx.x / kWave] = s;
-    part[1][threadIdx.x / kWave] = n;
-  }
-  __syncthreads();
-}
-
 __global__ void __launch_bounds__(256) ce_sums_kernel(CeArgs a, int64_t per) {
   __shared__ double part[2][4];
   const int64_t first = blockIdx.x * per, last = min(first + per, a.rows);
@@ -468,10 +439,8 @@ __global__ void __launch_bounds__(256) ce_sums_kernel(CeArgs a, int64_t per) {
     s += a.loss[row];
     n += target_of(a, row) != a.ignore ? 1.0 : 0.0;
   }
-  block_sums(s, n, part);
+  const double v = block_sums(s, n, part);
   if (threadIdx.x >= 2) return;
-  const double *const p = part[threadIdx.x];
-  const double v = (p[0] + p[1]) + (p[2] + p[3]);
   if (gridDim.x == 1)
     a.sums[threadIdx.x] = static_cast<float>(v);
   else
@@ -485,10 +454,8 @@ __global__ void __launch_bounds__(256) ce_total_kernel(CeArgs a, int blocks) {
     s = a.sum_parts[2 * threadIdx.x];
     n = a.sum_parts[2 * threadIdx.x + 1];
   }
-  block_sums(s, n, part);
-  if (threadIdx.x >= 2) return;
-  const double *const p = part[threadIdx.x];
-  a.sums[threadIdx.x] = static_cast<float>((p[0] + p[1]) + (p[2] + p[3]));
+  const double v = block_sums(s, n, part);
+  if (threadIdx.x < 2) a.sums[threadIdx.x] = static_cast<float>(v);
 }
 
 // ---- gradients ---------------------------------------------------------------------------
@@ -526,7 +493,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int row = (wm * S::MB + i) * 32 + result_row(r);
-        float g = __builtin_amdgcn_exp2f((acc[i][j][r] - lse[j]) * kLog2e) - (row == target[j] ? 1.0f : 0.0f);
+        float g = exp_of(acc[i][j][r] - lse[j]) - (row == target[j] ? 1.0f : 0.0f);
         g = n0 + (wn * S::NB + j) * 32 + lane % 32 < count ? g : 0.0f; // the product is of another row
         total[r] += g * grad[j];
         acc[i][j][r] = g * m[j];
@@ -553,11 +520,11 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
       for (int j = 0; j < S::NB; ++j) {
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-          Pack<U, 2> p;
+          Pack<f16_t, 2> p;
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const float v = acc[i][j][2 * r + e];
-            p.v[e] = static_cast<U>(v);
+            p.v[e] = static_cast<f16_t>(v);
             if constexpr (PLANES == 2) acc[i][j][2 * r + e] = v - static_cast<float>(p.v[e]);
           }
           half[i][j][r] = __builtin_bit_cast(uint32_t, p);
@@ -623,43 +590,48 @@ __device__ __forceinline__ void put_four(O *row, int64_t j, int64_t dim, bool wh
     if (j + e < dim) row[j + e] = static_cast<O>(v[e]);
 }
 
-// dx (DX) or the piece's rows of dw: features down, listed rows or classes across.
-// dx is summed over the pieces: `add` to what is there, and to its type at the `last`.
-template <typename U, int PLANES, typename S, typename O, bool DX>
+// dx (DX) or the piece's rows of dw: features down, listed rows or classes across, over
+// one of gridDim.y parts of the sum.  A sum in one part, over one piece, goes straight
+// to the output; else to the part's place in 32 bits, added to what is there past the
+// first piece.
+template <int PLANES, typename S, typename O, bool DX>
 __global__ void __launch_bounds__(S::kThreads)
-    ce_gradient_kernel(CeArgs a, int64_t v0, bool add, bool last) {
+    ce_gradient_kernel(CeArgs a, int64_t v0, bool direct, bool add) {
   __shared__ __attribute__((aligned(16))) char lds[2 * S::kStage];
   const int count = a.meta->count;
-  const int64_t across = DX ? a.rows : min(a.piece, a.classes - v0);
+  const int64_t here = min(a.piece, a.classes - v0), across = DX ? a.rows : here;
   int64_t ti, tj;
   place_tile(xcd_block(), ceil_div64(a.dim, S::kM), ceil_div64(across, S::kN), 8, ti, tj);
   const int64_t m0 = ti * S::kM, n0 = tj * S::kN;
-  const int64_t limit = DX ? count : across;
+  const int64_t limit = DX ? count : here;
   if (n0 >= limit) return;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), lane = lane_id();
   const int wm = wave / S::WN, wn = wave % S::WN;
-  const int64_t a_stride = (DX ? a.piece : a.rows_pad) * 2;
+  const int64_t stride = (DX ? a.piece : a.rows_pad) * 2;
   uint32_t a_off[S::kFetchA], b_off[S::kFetchB];
   fetch_offsets<S::kWaves>(wave, a_off, [&](int r) {
-    return static_cast<uint32_t>(min(static_cast<int64_t>(r), a.dim - 1 - m0) * a_stride);
+    return static_cast<uint32_t>(min(static_cast<int64_t>(r), a.dim - 1 - m0) * stride);
   });
   fetch_offsets<S::kWaves>(wave, b_off, [&](int r) {
-    return static_cast<uint32_t>(min(static_cast<int64_t>(r), limit - 1 - n0) * a_stride);
+    return static_cast<uint32_t>(min(static_cast<int64_t>(r), limit - 1 - n0) * stride);
   });
   f32x16 acc[S::MB][S::NB] = {};
-  const int64_t g_plane = a.rows_pad * a.piece * 2;
-  tile_product<U, PLANES, S>(lds, wave, (DX ? a.wt : a.xt) + m0 * a_stride, a.dim * a_stride, a_off,
-                             (DX ? a.g : a.gt) + n0 * a_stride, g_plane, b_off,
-                             static_cast<int>(ceil_div64(DX ? min(a.piece, a.classes - v0) : count, kStageK)), acc);
+  const int64_t stages = ceil_div64(DX ? here : count, kStageK), each = ceil_div64(stages, gridDim.y);
+  const int64_t first = min(blockIdx.y * each, stages), mine = min(each, stages - first);
+  tile_product<f16_t, PLANES, S>(lds, wave, (DX ? a.wt : a.xt) + m0 * stride + first * kStageBytes,
+                                 a.dim * stride, a_off,
+                                 (DX ? a.g : a.gt) + n0 * stride + first * kStageBytes,
+                                 a.rows_pad * a.piece * 2, b_off, static_cast<int>(mine), acc);
   O *const out = static_cast<O *>(DX ? a.dx : a.dw);
-  const int64_t stride = DX ? a.dx_stride : a.dw_stride;
-  const bool whole = stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(O)) == 0;
+  const int64_t out_stride = DX ? a.dx_stride : a.dw_stride;
+  const bool whole = out_stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(O)) == 0;
+  float *const part = (DX ? a.dx_part : a.dw_part) + blockIdx.y * ((DX ? a.rows_pad : a.piece) * a.dim_pad);
 #pragma unroll
   for (int j = 0; j < S::NB; ++j) {
     const int64_t n = n0 + (wn * S::NB + j) * 32 + lane % 32;
     if (n >= limit) continue;
     const int power = (DX ? a.exponent[n] : a.meta->most) - kShift;
-    O *const row = out + (DX ? a.list[n] : v0 + n) * stride;
+    O *const row = out + (DX ? a.list[n] : v0 + n) * out_stride;
 #pragma unroll
     for (int i = 0; i < S::MB; ++i) {
 #pragma unroll
@@ -669,27 +641,45 @@ __global__ void __launch_bounds__(S::kThreads)
         float v[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
-        if (DX && (add || !last)) {
-          float4 *const held = reinterpret_cast<float4 *>(a.dx32 + n * a.dim_pad + m);
-          if (add) {
-            const float4 old = *held;
-            v[0] += old.x, v[1] += old.y, v[2] += old.z, v[3] += old.w;
-          }
-          if (!last) {
-            *held = make_float4(v[0], v[1], v[2], v[3]);
-            continue;
-          }
-        }
+        if (direct) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if constexpr (PLANES == 2)
-            v[e] *= unit_of((DX ? a.w_most : a.x_most)[min(m + e, a.dim - 1)]);
-          v[e] = ldexpf(v[e], power);
+          for (int e = 0; e < 4; ++e)
+            v[e] = ldexpf(v[e] * unit_of((DX ? a.w_most : a.x_most)[min(m + e, a.dim - 1)]), power);
+          put_four(row, m, a.dim, whole, v);
+          continue;
         }
-        put_four(row, m, a.dim, whole, v);
+        float4 *const held = reinterpret_cast<float4 *>(part + n * a.dim_pad + m);
+        if (add) {
+          const float4 old = *held;
+          v[0] += old.x, v[1] += old.y, v[2] += old.z, v[3] += old.w;
+        }
+        *held = make_float4(v[0], v[1], v[2], v[3]);
       }
     }
   }
+}
+
+// The parts' sum, four elements of a row per thread.
+template <typename O, bool DX>
+__global__ void __launch_bounds__(256) ce_finish_kernel(CeArgs a, int64_t v0, int splits) {
+  const int64_t n = blockIdx.z * int64_t(gridDim.y) + blockIdx.y, m = (blockIdx.x * int64_t(256) + threadIdx.x) * 4;
+  const int64_t limit = DX ? a.meta->count : min(a.piece, a.classes - v0);
+  if (n >= limit || m >= a.dim) return;
+  const int64_t part = (DX ? a.rows_pad : a.piece) * a.dim_pad;
+  const float *const from = (DX ? a.dx_part : a.dw_part) + n * a.dim_pad + m;
+  float v[4] = {};
+  for (int s = 0; s < splits; ++s) {
+    const float4 p = *reinterpret_cast<const float4 *>(from + s * part);
+    v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+  }
+  const int power = (DX ? a.exponent[n] : a.meta->most) - kShift;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    v[e] = ldexpf(v[e] * unit_of((DX ? a.w_most : a.x_most)[min(m + e, a.dim - 1)]), power);
+  O *const out = static_cast<O *>(DX ? a.dx : a.dw);
+  const int64_t stride = DX ? a.dx_stride : a.dw_stride;
+  const bool whole = stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(O)) == 0;
+  put_four(out + (DX ? a.list[n] : v0 + n) * stride, m, a.dim, whole, v);
 }
 
 // dx of the rows that are not listed.
@@ -723,10 +713,16 @@ constexpr int64_t kMostClasses = int64_t(1) << 25;
 constexpr int64_t kMostLogits = int64_t(1) << 37; // a launch's threads in 32 bits
 constexpr int64_t kMostFeatures = 65536;
 
+// How a product is cut: tiles of which shape (0 narrow, 1 middle, 2 large), and the sum
+// into how many parts.
+struct Cut {
+  int shape, splits;
+};
+
 struct CePlan {
   bool x_direct, w_direct;
-  int planes, half;
-  int shape; // 0 narrow, 1 middle, 2 large
+  int planes;
+  Cut z, dx, dw;
   size_t bytes;
 };
 
@@ -735,11 +731,27 @@ bool direct_rows(int type, int64_t dim, int64_t stride, const void *p, int64_t s
          span_rows * stride * 2 < (int64_t(1) << 32);
 }
 
-// Large tiles where they fill the card, else smaller ones; a few rows have tiles
-// of their own.
-int tile_shape(int64_t down, int64_t across, bool narrow) {
-  if (ceil_div64(down, 256) * ceil_div64(across, 256) >= 256) return 2;
-  return narrow && across <= 64 ? 0 : 1;
+// Turns of the card's tiles (256 large ones or 512 middle ones at a time, the latter at
+// some 0.65 of a large one's time) times the length of a part, and what a part in 32
+// bits costs besides, as a length: written and read, 900 elements' products.
+Cut cut_product(int64_t down, int64_t across, int64_t length, bool may_split) {
+  Cut best{1, 1};
+  double least = 0.0;
+  const int64_t fewest = may_split ? ceil_div64(length, 65536) : 1; // shorter 32-bit sums
+  for (int shape : {1, 2}) {
+    const int64_t side = shape == 2 ? 256 : 128, slots = shape == 2 ? 256 : 512;
+    const int64_t tiles = ceil_div64(down, side) * ceil_div64(across, side);
+    const int64_t most = may_split ? std::max(fewest, std::min<int64_t>(length / 512, 32)) : 1;
+    for (int64_t s = fewest; s <= most; ++s) {
+      const double turns = static_cast<double>(ceil_div64(tiles * s, slots));
+      const double cost = turns * (static_cast<double>(length) / s + (s > 1 ? 900.0 : 0.0)) * (shape == 2 ? 1.0 : 0.65);
+      if (least == 0.0 || cost < least) {
+        least = cost;
+        best = {shape, static_cast<int>(s)};
+      }
+    }
+  }
+  return best;
 }
 
 CePlan lay_out(CeArgs &a, bool backward, void *work) {
@@ -747,7 +759,6 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
   p.planes = a.type == SPORDER_TYPE_F32 ? 2 : 1;
   p.x_direct = direct_rows(a.type, a.dim, a.x_stride, a.x, a.rows);
   p.w_direct = direct_rows(a.type, a.dim, a.w_stride, a.w, 256);
-  p.shape = tile_shape(a.classes, a.rows, !backward);
   a.rows_pad = ceil_div64(a.rows, 256) * 256;
   a.dim_pad = ceil_div64(a.dim, kStageK) * kStageK;
   a.piece = ceil_div64(a.classes, 256) * 256;
@@ -759,8 +770,10 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     }
   }
   a.classes_pad = ceil_div64(a.classes, a.piece) * a.piece;
-  const int span = p.shape == 2 ? 128 : p.shape == 1 ? 64 : 32; // classes of a wave
-  a.chunks = ceil_div64(ceil_div64(a.classes, span), p.shape == 0 ? 4 : 2) * (p.shape == 0 ? 4 : 2);
+  p.z = cut_product(a.piece, a.rows, a.dim, false);
+  if (!backward && a.rows <= 64) p.z.shape = 0;
+  const int down = p.z.shape == 2 ? Large::kM : Middle::kM; // classes of a tile
+  a.chunks = ceil_div64(a.classes, down) * (p.z.shape == 0 ? Narrow::WM : 2);
   size_t at = 0;
   auto take = [&](auto *&q, int64_t count) {
     using P = std::remove_reference_t<decltype(*q)>;
@@ -802,15 +815,16 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     take(a.exponent, a.rows_pad);
     take(a.mantissa, a.rows_pad);
     take(a.row_lse, a.rows_pad);
-    if (p.planes == 2) {
-      take(a.x_most, a.dim);
-      take(a.w_most, a.dim);
-    }
+    p.dx = cut_product(a.dim, a.rows, a.piece, true);
+    p.dw = cut_product(a.dim, a.piece, a.rows, true);
+    take(a.x_most, a.dim);
+    take(a.w_most, a.dim);
     take(a.xt, a.dim * a.rows_pad * 2 * p.planes);
     take(a.wt, a.dim * a.piece * 2 * p.planes);
     take(a.g, a.rows_pad * a.piece * 2 * p.planes);
     take(a.gt, a.rows_pad * a.piece * 2 * p.planes);
-    if (a.piece < a.classes) take(a.dx32, a.rows_pad * a.dim_pad);
+    if (a.piece < a.classes || p.dx.splits > 1) take(a.dx_part, p.dx.splits * a.rows_pad * a.dim_pad);
+    if (p.dw.splits > 1) take(a.dw_part, p.dw.splits * a.piece * a.dim_pad);
     if (a.db) take(a.db_part, a.rows_pad / 64 * a.piece);
   }
   p.bytes = at;
@@ -864,7 +878,7 @@ template <typename T, typename U, int PLANES> int32_t forward(const CeArgs &a, c
                   dim3(ceil_div64(a.classes, S::kM) * ceil_div64(a.rows, S::kN)), dim3(S::kThreads),
                   stream, a);
   };
-  steps([&] { return p.shape == 2 ? go(Large{}) : p.shape == 1 ? go(Middle{}) : go(Narrow{}); });
+  steps([&] { return p.z.shape == 2 ? go(Large{}) : p.z.shape == 1 ? go(Middle{}) : go(Narrow{}); });
   steps([&] { return launch(ce_join_kernel, dim3(ceil_div64(a.rows, 16)), dim3(256), stream, a); });
   const int64_t blocks = std::min(ceil_div64(a.rows, kSumRows), kSumBlocks);
   const int64_t per = ceil_div64(a.rows, blocks);
@@ -874,76 +888,82 @@ template <typename T, typename U, int PLANES> int32_t forward(const CeArgs &a, c
   return steps.rc;
 }
 
+template <typename O, bool DX>
+int32_t finish(const CeArgs &a, int64_t v0, int64_t rows, int splits, void *stream) {
+  const int64_t deep = std::min<int64_t>(rows, 32768);
+  return launch(ce_finish_kernel<O, DX>, dim3(ceil_div64(a.dim, 1024), ceil_div64(rows, ceil_div64(rows, deep)), ceil_div64(rows, deep)),
+                dim3(256), stream, a, v0, splits);
+}
+
 template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, const CePlan &p, void *stream) {
   const T *const x = static_cast<const T *>(a.x), *const w = static_cast<const T *>(a.w);
   const int32_t *const no_list = nullptr;
-  const float *const no_most = nullptr;
-  const float *const x_most = a.x_most, *const w_most = a.w_most;
   Steps steps;
   steps([&] { return list_rows(a, true, stream); });
   steps([&] { return pack_operands<T, U, PLANES>(a, p, stream); });
-  if constexpr (PLANES == 2) {
-    steps([&] {
-      return launch(ce_column_most_kernel<T>, dim3(ceil_div64(a.dim, 64), std::min<int64_t>(ceil_div64(a.rows, 64), 256)),
-                    dim3(256), stream, x, a.x_stride, a.rows, a.dim, a.meta, a.list, a.x_most);
-    });
-    steps([&] {
-      return launch(ce_column_most_kernel<T>, dim3(ceil_div64(a.dim, 64), std::min<int64_t>(ceil_div64(a.classes, 64), 256)),
-                    dim3(256), stream, w, a.w_stride, a.classes, a.dim, a.meta, no_list, a.w_most);
-    });
-  }
-  steps([&] {
-    return launch(ce_pack_columns_kernel<T, U, PLANES>, dim3(ceil_div64(a.dim, 64), ceil_div64(a.rows, 64)),
-                  dim3(256), stream, x, a.x_stride, a.rows, a.dim, a.meta, a.list, a.exponent,
-                  PLANES == 2 ? x_most : no_most, a.xt, a.rows_pad * 2, a.dim * a.rows_pad * 2);
-  });
+  auto columns_most = [&](const T *src, int64_t stride, int64_t rows, const int32_t *list, float *most) {
+    const dim3 grid(ceil_div64(a.dim, 64 * (16 / sizeof(T))), std::min<int64_t>(ceil_div64(rows, 64), 256));
+    return launch(ce_column_most_kernel<T>, grid, dim3(256), stream, src, stride, rows, a.dim, a.meta, list, most);
+  };
+  steps([&] { return columns_most(x, a.x_stride, a.rows, a.list, a.x_most); });
+  steps([&] { return columns_most(w, a.w_stride, a.classes, no_list, a.w_most); });
+  auto pack_columns = [&](const T *src, int64_t stride, int64_t rows, const int32_t *list, const float *most,
+                          char *out, int64_t out_rows) {
+    return launch(ce_pack_columns_kernel<T, PLANES>, dim3(ceil_div64(rows, 64), ceil_div64(a.dim, 64)), dim3(256),
+                  stream, src, stride, rows, a.dim, a.meta, list, a.exponent, most, out, out_rows * 2,
+                  a.dim * out_rows * 2);
+  };
+  steps([&] { return pack_columns(x, a.x_stride, a.rows, a.list, a.x_most, a.xt, a.rows_pad); });
   steps([&] { return launch(ce_zero_kernel<T>, dim3(ceil_div64(a.rows, 4)), dim3(256), stream, a); });
+  const bool one_piece = a.piece >= a.classes, dx_direct = one_piece && p.dx.splits == 1;
   for (int64_t v0 = 0; v0 < a.classes; v0 += a.piece) {
-    const bool last = v0 + a.piece >= a.classes;
     const int64_t here = std::min(a.piece, a.classes - v0);
-    steps([&] {
-      return launch(ce_pack_columns_kernel<T, U, PLANES>, dim3(ceil_div64(a.dim, 64), a.piece / 64),
-                    dim3(256), stream, w + v0 * a.w_stride, a.w_stride, here, a.dim, a.meta, no_list,
-                    no_list, PLANES == 2 ? w_most : no_most, a.wt, a.piece * 2, a.dim * a.piece * 2);
-    });
+    steps([&] { return pack_columns(w + v0 * a.w_stride, a.w_stride, here, no_list, a.w_most, a.wt, a.piece); });
     auto tiles = [&](auto shape) {
       using S = decltype(shape);
       return launch(ce_g_kernel<U, PLANES, S>, dim3(ceil_div64(here, S::kM) * ceil_div64(a.rows, S::kN)),
                     dim3(S::kThreads), stream, a, v0);
     };
-    const int shape = tile_shape(here, a.rows, false);
-    steps([&] { return shape == 2 ? tiles(Large{}) : tiles(Middle{}); });
+    steps([&] { return p.z.shape == 2 ? tiles(Large{}) : tiles(Middle{}); });
     if (a.db)
       steps([&] {
-        return launch(ce_bias_kernel, dim3(a.piece / 64), dim3(256), stream, a, v0, shape == 2 ? 256 : 128);
+        return launch(ce_bias_kernel, dim3(a.piece / 64), dim3(256), stream, a, v0,
+                      p.z.shape == 2 ? Large::kN : Middle::kN);
       });
     auto dx = [&](auto shape) {
       using S = decltype(shape);
-      return launch(ce_gradient_kernel<U, PLANES, S, T, true>,
-                    dim3(ceil_div64(a.dim, S::kM) * ceil_div64(a.rows, S::kN)), dim3(S::kThreads), stream,
-                    a, v0, v0 > 0, last);
+      return launch(ce_gradient_kernel<PLANES, S, T, true>,
+                    dim3(ceil_div64(a.dim, S::kM) * ceil_div64(a.rows, S::kN), p.dx.splits), dim3(S::kThreads),
+                    stream, a, v0, dx_direct, v0 > 0);
     };
-    steps([&] { return tile_shape(a.dim, a.rows, false) == 2 ? dx(Large{}) : dx(Middle{}); });
-    auto dw = [&](auto shape) {
+    steps([&] { return p.dx.shape == 2 ? dx(Large{}) : dx(Middle{}); });
+    auto dw = [&](auto shape, auto kind) {
       using S = decltype(shape);
-      const dim3 grid(ceil_div64(a.dim, S::kM) * ceil_div64(here, S::kN));
-      if constexpr (sizeof(T) == 2) {
-        if (a.dw_type != SPORDER_TYPE_F32)
-          return launch(ce_gradient_kernel<U, PLANES, S, T, false>, grid, dim3(S::kThreads), stream, a, v0,
-                        false, true);
-      }
-      return launch(ce_gradient_kernel<U, PLANES, S, float, false>, grid, dim3(S::kThreads), stream, a, v0,
-                    false, true);
+      using O = decltype(kind);
+      return launch(ce_gradient_kernel<PLANES, S, O, false>,
+                    dim3(ceil_div64(a.dim, S::kM) * ceil_div64(here, S::kN), p.dw.splits), dim3(S::kThreads),
+                    stream, a, v0, p.dw.splits == 1, false);
     };
-    steps([&] { return tile_shape(a.dim, here, false) == 2 ? dw(Large{}) : dw(Middle{}); });
+    auto finish_dw = [&](auto kind) {
+      return finish<decltype(kind), false>(a, v0, here, p.dw.splits, stream);
+    };
+    const bool wide = sizeof(T) == 2 && a.dw_type == SPORDER_TYPE_F32;
+    steps([&] {
+      if (wide) return p.dw.shape == 2 ? dw(Large{}, float{}) : dw(Middle{}, float{});
+      return p.dw.shape == 2 ? dw(Large{}, T{}) : dw(Middle{}, T{});
+    });
+    if (p.dw.splits > 1) steps([&] { return wide ? finish_dw(float{}) : finish_dw(T{}); });
   }
+  if (!dx_direct) steps([&] { return finish<T, true>(a, 0, a.rows, p.dx.splits, stream); });
   return steps.rc;
 }
 
-bool bad_sizes(const CeArgs &a) {
+bool bad_sizes(const CeArgs &a, bool backward) {
   return !type_known(a.type) || !type_known(a.bias_type) || (a.target_bits != 32 && a.target_bits != 64) ||
-         a.rows < 0 || a.rows > kMostRows || a.dim < 1 || a.dim > kMostFeatures || a.classes < 1 ||
-         a.classes > kMostClasses || a.rows > kMostLogits / a.classes || a.x_stride < 0 || a.w_stride < 0;
+         a.rows < 0 || a.dim < 1 || a.dim > kMostFeatures || a.classes < 1 || a.classes > kMostClasses ||
+         a.rows > (few_takes(a.dim, a.classes, backward) ? kMostLogits
+                                                         : std::min(kMostRows, kMostLogits / a.classes)) ||
+         a.x_stride < 0 || a.w_stride < 0;
 }
 
 template <typename T> __global__ void ce_nothing_kernel(CeArgs a) {
@@ -972,7 +992,8 @@ size_t sporder_linear_cross_entropy_work_bytes(int32_t type, int64_t rows, int64
   CeArgs a{};
   a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = 64;
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
-  if (bad_sizes(a) || rows == 0) return 0;
+  if (bad_sizes(a, false) || rows == 0) return 0;
+  if (few_takes(dim, classes, false)) return few_work_bytes(rows, dim, classes, false);
   return lay_out(a, false, nullptr).bytes;
 }
 
@@ -987,10 +1008,13 @@ int32_t sporder_linear_cross_entropy(void *stream, int32_t type, int64_t rows, i
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
   a.bias_type = bias_type, a.bias = d_bias, a.targets = d_targets, a.ignore = ignore_index;
   a.loss = d_loss, a.lse = d_lse, a.sums = d_sums;
-  if (bad_sizes(a) || !d_sums) return SPORDER_BAD_ARGUMENT;
+  if (bad_sizes(a, false) || !d_sums) return SPORDER_BAD_ARGUMENT;
   if (rows == 0) return launch(ce_no_rows_kernel, dim3(1), dim3(kWave), stream, a);
   if (!d_x || !d_weight || !d_targets || !d_loss || !d_lse || !d_work || !aligned_to(d_work, 256))
     return SPORDER_BAD_ARGUMENT;
+  if (few_takes(dim, classes, false))
+    return work_bytes < few_work_bytes(rows, dim, classes, false) ? SPORDER_BAD_ARGUMENT
+                                                                   : few_forward(a, d_work, stream);
   const CePlan p = lay_out(a, false, d_work);
   if (work_bytes < p.bytes) return SPORDER_BAD_ARGUMENT;
   if (type == SPORDER_TYPE_BF16) return forward<bf16_t, bf16_t, 1>(a, p, stream);
@@ -1006,7 +1030,8 @@ size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows, 
   a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = 64;
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
   a.db = &a; // the scratch of a bias whether there is one or not
-  if (bad_sizes(a) || rows == 0) return 0;
+  if (bad_sizes(a, true) || rows == 0) return 0;
+  if (few_takes(dim, classes, true)) return few_work_bytes(rows, dim, classes, true);
   return lay_out(a, true, nullptr).bytes;
 }
 
@@ -1027,7 +1052,7 @@ int32_t sporder_linear_cross_entropy_grad(void *stream, int32_t type, int64_t ro
   a.grad = d_grad, a.grad_stride = grad_stride, a.given_lse = d_lse;
   a.dx = d_dx, a.dx_stride = dx_stride, a.dw = d_dweight, a.dw_stride = dweight_stride;
   a.dw_type = dweight_type, a.db = d_dbias;
-  if (bad_sizes(a) || (dweight_type != type && dweight_type != SPORDER_TYPE_F32) || grad_stride < 0 ||
+  if (bad_sizes(a, true) || (dweight_type != type && dweight_type != SPORDER_TYPE_F32) || grad_stride < 0 ||
       dx_stride < 0 || (rows > 1 && dx_stride < dim) || dweight_stride < 0 ||
       (classes > 1 && dweight_stride < dim) || !d_dweight)
     return SPORDER_BAD_ARGUMENT;
@@ -1038,6 +1063,9 @@ int32_t sporder_linear_cross_entropy_grad(void *stream, int32_t type, int64_t ro
   }
   if (!d_grad || !d_x || !d_weight || !d_targets || !d_lse || !d_dx || !d_work || !aligned_to(d_work, 256))
     return SPORDER_BAD_ARGUMENT;
+  if (few_takes(dim, classes, true))
+    return work_bytes < few_work_bytes(rows, dim, classes, true) ? SPORDER_BAD_ARGUMENT
+                                                                  : few_backward(a, d_work, stream);
   const CePlan p = lay_out(a, true, d_work);
   if (work_bytes < p.bytes) return SPORDER_BAD_ARGUMENT;
   if (type == SPORDER_TYPE_BF16) return backward<bf16_t, bf16_t, 1>(a, p, stream);

@@ -1,0 +1,62 @@
+// cross_entropy.hpp -- the two forms of the linear cross entropy: tiles of
+// 16-bit products over any number of classes (cross_entropy.hip), and one pass
+// over the rows where the classes' weights fit a workgroup's LDS
+// (cross_entropy_few.hip).
+#pragma once
+
+#include "dense.hpp"
+
+namespace sporder_hip {
+
+// What a call passes, for either form.
+struct CeCall {
+  int64_t rows, dim, classes;
+  int64_t x_stride, w_stride; // elements
+  const void *x, *w, *bias, *targets;
+  int64_t ignore;
+  int type, bias_type, target_bits;
+  // forward
+  float *loss, *lse, *sums;
+  // backward
+  const float *grad, *given_lse;
+  int64_t grad_stride;
+  void *dx, *dw, *db;
+  int64_t dx_stride, dw_stride;
+  int dw_type;
+};
+
+__device__ __forceinline__ int64_t target_of(const CeCall &a, int64_t row) {
+  return a.target_bits == 64 ? static_cast<const int64_t *>(a.targets)[row]
+                             : static_cast<const int32_t *>(a.targets)[row];
+}
+__device__ __forceinline__ bool counted(const CeCall &a, int64_t target) {
+  return target != a.ignore && target >= 0 && target < a.classes;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f;
+__device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
+
+// Sums of two values over a workgroup of 256, in 64 bits and a fixed order, in its
+// first two threads (the first value in thread 0).
+__device__ __forceinline__ double block_sums(double s, double n, double (&part)[2][4]) {
+#pragma unroll
+  for (int j = 1; j < kWave; j <<= 1) {
+    s += __shfl_xor(s, j);
+    n += __shfl_xor(n, j);
+  }
+  if (lane_id() == 0) {
+    part[0][threadIdx.x / kWave] = s;
+    part[1][threadIdx.x / kWave] = n;
+  }
+  __syncthreads();
+  const double *const p = part[threadIdx.x & 1];
+  return (p[0] + p[1]) + (p[2] + p[3]);
+}
+
+// The one-pass form.
+bool few_takes(int64_t dim, int64_t classes, bool backward);
+size_t few_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward);
+int32_t few_forward(const CeCall &a, void *work, void *stream);
+int32_t few_backward(const CeCall &a, void *work, void *stream);
+
+} // namespace sporder_hip

@@ -138,6 +138,37 @@ def residual_norm(x, residual=None, gate=None, post_weight=None, weight=None, *,
     return _ResidualNorm.apply(x, residual, gate, post_weight, weight, scale, eps, post_norm)
 
 
+class _LinearCrossEntropy(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, targets, bias, ignore_index, reduction):
+        loss, lse, sums = sporder.linear_cross_entropy(x, weight, targets, bias,
+                                                       ignore_index=ignore_index)
+        ctx.save_for_backward(x, weight, targets, bias, lse, sums)
+        ctx.ignore_index, ctx.reduction = ignore_index, reduction
+        if reduction == "none":
+            return loss
+        return sums[0] / sums[1] if reduction == "mean" else sums[0].clone()
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        x, weight, targets, bias, lse, sums = ctx.saved_tensors
+        if ctx.reduction == "mean":
+            grad = grad / sums[1]
+        dx, dweight, dbias = sporder.linear_cross_entropy_grad(
+            grad, x, weight, targets, lse, bias, ignore_index=ctx.ignore_index)
+        return dx, dweight, None, dbias, None, None
+
+
+def linear_cross_entropy(x, weight, targets, bias=None, *, ignore_index=-100, reduction="mean"):
+    """Softmax cross entropy of the logits x weight^T + bias, which are never kept
+    (``sporder.linear_cross_entropy``), differentiable by x, weight and bias: the
+    mean over the rows that are not ignored, their sum, or the losses by row."""
+    if reduction not in ("mean", "sum", "none"):
+        raise ValueError("reduction must be mean, sum or none")
+    return _LinearCrossEntropy.apply(x, weight, targets, bias, ignore_index, reduction)
+
+
 class Muon(torch.optim.Optimizer):
     """Momentum whose update is orthogonalised, for parameters of two (or, as a
     batch of matrices, three) dimensions:

@@ -576,8 +576,8 @@ def _loss_inputs(x, weight, targets, bias):
         _same_device(bias, x, "bias")
         bias = bias if bias.is_contiguous() else bias.contiguous()
     classes, rows = weight.shape[0], targets.numel()
-    if rows >= 2**23 - 255 or classes > 2**25 or rows * classes > 2**37:
-        raise ValueError("at most 2^23 - 256 rows, 2^25 classes and 2^37 logits")
+    if classes > 2**25 or (classes > 192 and (rows > 2**23 - 256 or rows * classes > 2**37)):
+        raise ValueError("at most 2^25 classes, and past 192 of them 2^23 - 256 rows and 2^37 logits")
     x, _, x_stride = _rows(x)
     weight, _, weight_stride = _rows(weight)
     targets = targets if targets.is_contiguous() else targets.contiguous()

@@ -21,7 +21,7 @@ namespace {
 
 using f32x4 = float __attribute__((ext_vector_type(4)));
 
-constexpr int kThreads = 256;
+constexpr int kLossThreads = 256, kGradThreads = 512;
 constexpr int kLds = 160 * 1024;
 
 struct FewArgs {
@@ -36,73 +36,134 @@ __device__ __forceinline__ f32x4 mfma_16x16(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// Four elements of a row from `col` on as floats, zeros past its end.
-template <typename T>
-__device__ __forceinline__ f32x4 four(const T *row, int col, int dim) {
-  f32x4 v = {};
-  if (col < dim) {
-    const auto q = fetch<true, 4>(row + col, dim - col);
+// Four elements of a row from `col` on, or its last four where it ends before (a row has
+// four at least).
+template <typename T> __device__ __forceinline__ Words<T, 4> four(const T *row, int col, int dim) {
+  return __builtin_bit_cast(Words<T, 4>, *reinterpret_cast<const LoosePack<T, 4> *>(row + min(col, dim - 4)));
+}
+
+// As floats, zeros past the row's end.
+template <typename T> __device__ __forceinline__ f32x4 floats(const Words<T, 4> &words, int col, int dim) {
+  const auto q = __builtin_bit_cast(Pack<T, 4>, words);
+  f32x4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(q.v[e]);
+  for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(q.v[e]);
+  if (dim % 4 != 0) { // move the row's last elements to their places
+    const int past = col + 4 - dim;
+    if (past > 0)
+      v = past == 1   ? f32x4{v[1], v[2], v[3], 0.0f}
+          : past == 2 ? f32x4{v[2], v[3], 0.0f, 0.0f}
+          : past == 3 ? f32x4{v[3], 0.0f, 0.0f, 0.0f}
+                      : f32x4{};
+  } else if (col >= dim) {
+    v = f32x4{};
   }
   return v;
 }
 
-// w and the bias (-inf past the classes) to LDS, rows of `stride` floats.
-template <typename T, int VB, int DB>
-__device__ __forceinline__ void hold_weights(const CeCall &c, float *w, float *bias, int stride) {
-  const int part = threadIdx.x % 16 * 4;
-  for (int v = threadIdx.x / 16; v < VB * 16; v += kThreads / 16) {
+// Floats of a row of x or w in LDS: whole blocks of 64 features, so that rows' places are
+// constants (a stride known at run time cost 36 registers of addresses).
+constexpr int few_stride(int feature_blocks) { return feature_blocks * 64 + 4; }
+
+// w and the bias (-inf past the classes) to LDS.
+template <typename T, int VB, int DB, int THREADS>
+__device__ __forceinline__ void hold_weights(const CeCall &c, float *w, float *bias) {
+  constexpr int stride = few_stride(DB);
+  const int part = threadIdx.x % 16 * 4, dim = static_cast<int>(c.dim);
+  for (int v = threadIdx.x / 16; v < VB * 16; v += THREADS / 16) {
     const T *const row = static_cast<const T *>(c.w) + v * c.w_stride;
 #pragma unroll
     for (int k = 0; k < DB; ++k)
-      if (k * 64 + part < stride - 4)
-        *reinterpret_cast<f32x4 *>(w + v * stride + k * 64 + part) =
-            v < c.classes ? four<T>(row, k * 64 + part, static_cast<int>(c.dim)) : f32x4{};
+      *reinterpret_cast<f32x4 *>(w + v * stride + k * 64 + part) =
+          v < c.classes ? floats<T>(four<T>(row, k * 64 + part, dim), k * 64 + part, dim) : f32x4{};
   }
-  for (int v = threadIdx.x; v < VB * 16; v += kThreads) {
+  for (int v = threadIdx.x; v < VB * 16; v += THREADS) {
     float b = v < c.classes ? 0.0f : -INFINITY;
     if (c.bias && v < c.classes) with_type(c.bias, c.bias_type, [&](auto *p) { b = static_cast<float>(p[v]); });
     bias[v] = b;
   }
 }
 
-// A tile's rows on their way: 16 threads a row, zeros for rows that count nothing.
-template <typename T, int TB, int DB>
-__device__ __forceinline__ void fetch_tile(const CeCall &c, int64_t first, f32x4 (&v)[TB][DB]) {
+// A row's target as it lies in memory, loaded a tile before it is looked at: without a
+// branch (past the rows the last one's), for a branch's end would wait for it and for
+// every load before it.
+struct RawTarget {
+  int32_t low, high;
+};
+__device__ __forceinline__ RawTarget fetch_target(const CeCall &c, int64_t row) {
+  const int words = c.target_bits / 32;
+  const int32_t *const p = static_cast<const int32_t *>(c.targets) + min(row, c.rows - 1) * words;
+  return {p[0], p[words - 1]};
+}
+
+// As a class, -1 where it counts nothing, -2 where it is no class, -3 past the rows.
+__device__ __forceinline__ int class_of(const CeCall &c, int64_t row, const RawTarget &raw) {
+  const int64_t t = c.target_bits == 64
+                        ? static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(raw.high)) << 32 |
+                                               static_cast<uint32_t>(raw.low))
+                        : raw.low;
+  const int k = t == c.ignore ? -1 : t >= 0 && t < c.classes ? static_cast<int>(t) : -2;
+  return row < c.rows ? k : -3;
+}
+
+// The targets of the rows that a thread fetches of a tile: 16 threads a row, STEP rows
+// at a time.
+template <int STEP, int N>
+__device__ __forceinline__ void fetch_targets(const CeCall &c, int64_t first, RawTarget (&t)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) t[i] = fetch_target(c, first + i * STEP + threadIdx.x / 16);
+}
+template <int STEP, int N>
+__device__ __forceinline__ void classes_of(const CeCall &c, int64_t first, const RawTarget (&t)[N], int (&k)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) k[i] = class_of(c, first + i * STEP + threadIdx.x / 16, t[i]);
+}
+
+// The rows' words on their way.  Rows that count nothing are read as the first one, which
+// the caches hold: a branch around the loads would make each wait for its target.
+template <typename T, int STEP, int N, int DB>
+__device__ __forceinline__ void fetch_tile(const CeCall &c, int64_t first, const int (&t)[N],
+                                           Words<T, 4> (&v)[N][DB]) {
   const int part = threadIdx.x % 16 * 4;
 #pragma unroll
-  for (int i = 0; i < TB; ++i) {
-    const int64_t row = first + i * 16 + threadIdx.x / 16;
-    const bool on = row < c.rows && counted(c, target_of(c, row));
+  for (int i = 0; i < N; ++i) {
+    const int64_t row = t[i] >= 0 ? first + i * STEP + threadIdx.x / 16 : 0;
     const T *const x = static_cast<const T *>(c.x) + row * c.x_stride;
 #pragma unroll
-    for (int k = 0; k < DB; ++k)
-      v[i][k] = on ? four<T>(x, k * 64 + part, static_cast<int>(c.dim)) : f32x4{};
+    for (int k = 0; k < DB; ++k) v[i][k] = four<T>(x, k * 64 + part, static_cast<int>(c.dim));
   }
 }
 
-template <int TB, int DB>
-__device__ __forceinline__ void put_tile(float *x, int stride, const f32x4 (&v)[TB][DB]) {
+// And in LDS, zeros for those that count nothing and past their ends.
+template <typename T, int STEP, int N, int DB>
+__device__ __forceinline__ void put_tile(const CeCall &c, float *x, const int (&t)[N],
+                                         const Words<T, 4> (&v)[N][DB]) {
   const int part = threadIdx.x % 16 * 4;
 #pragma unroll
-  for (int i = 0; i < TB; ++i) {
+  for (int i = 0; i < N; ++i) {
 #pragma unroll
-    for (int k = 0; k < DB; ++k)
-      if (k * 64 + part < stride - 4)
-        *reinterpret_cast<f32x4 *>(x + (i * 16 + threadIdx.x / 16) * stride + k * 64 + part) = v[i][k];
+    for (int k = 0; k < DB; ++k) {
+      const int col = k * 64 + part;
+      *reinterpret_cast<f32x4 *>(x + (i * STEP + threadIdx.x / 16) * few_stride(DB) + col) =
+          t[i] >= 0 ? floats<T>(v[i][k], col, static_cast<int>(c.dim)) : f32x4{};
+    }
   }
 }
 
-// z of 16 rows (of x, from `rows` on) and every STEP-th block of 16 classes.
-template <int BLOCKS, int STEP>
-__device__ __forceinline__ void logits(const float *w, const float *rows, int stride, f32x4 (&z)[BLOCKS]) {
+// z of 16 rows (of x, from `rows` on) and every STEP-th block of 16 classes, `blocks` of
+// them.
+template <int BLOCKS, int STEP, int DB>
+__device__ __forceinline__ void logits(const float *w, const float *rows, int dim16, int blocks,
+                                       f32x4 (&z)[BLOCKS]) {
+  constexpr int stride = few_stride(DB);
   const int lane = lane_id(), at = lane % 16 * stride + lane / 16 * 4;
-  for (int k = 0; k < stride - 4; k += 16) {
-    const f32x4 b = *reinterpret_cast<const f32x4 *>(rows + at + k);
+#pragma unroll 2
+  for (int k = 0; k < dim16; ++k) {
+    const f32x4 b = *reinterpret_cast<const f32x4 *>(rows + at + k * 16);
 #pragma unroll
     for (int v = 0; v < BLOCKS; ++v) {
-      const f32x4 a = *reinterpret_cast<const f32x4 *>(w + v * STEP * 16 * stride + at + k);
+      if (v >= blocks) continue;
+      const f32x4 a = *reinterpret_cast<const f32x4 *>(w + v * STEP * 16 * stride + at + k * 16);
 #pragma unroll
       for (int e = 0; e < 4; ++e) z[v] = mfma_16x16(a[e], b[e], z[v]);
     }
@@ -112,26 +173,37 @@ __device__ __forceinline__ void logits(const float *w, const float *rows, int st
 // ---- forward: 64 rows a tile, 16 a wave ------------------------------------------------
 
 template <typename T, int VB, int DB>
-__global__ void __launch_bounds__(kThreads) few_loss_kernel(FewArgs a) {
+__global__ void __launch_bounds__(kLossThreads) few_loss_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   const CeCall &c = a.c;
-  const int stride = static_cast<int>(ceil_div64(c.dim, 16)) * 16 + 4;
+  constexpr int stride = few_stride(DB);
+  const int dim16 = static_cast<int>(ceil_div64(c.dim, 16));
   float *const w = lds, *const x = w + VB * 16 * stride, *const bias = x + 64 * stride;
   const int lane = lane_id(), wave = threadIdx.x / kWave;
-  hold_weights<T, VB, DB>(c, w, bias, stride);
+  hold_weights<T, VB, DB, kLossThreads>(c, w, bias);
   double sum = 0.0, n = 0.0;
-  f32x4 next[4][DB];
-  fetch_tile<T>(c, blockIdx.x * int64_t(64), next);
+  const int64_t step = gridDim.x * int64_t(64);
+  int target[4];            // of the rows on their way
+  RawTarget next_target[4]; // of those after them
+  Words<T, 4> next[4][DB];
+  int64_t row = blockIdx.x * int64_t(64) + wave * 16 + lane % 16; // of this lane
+  fetch_targets<16>(c, blockIdx.x * int64_t(64), next_target);
+  classes_of<16>(c, blockIdx.x * int64_t(64), next_target, target);
+  fetch_tile<T, 16>(c, blockIdx.x * int64_t(64), target, next);
+  __builtin_amdgcn_sched_barrier(0); // loads in the loop's order, so that it waits for no later ones
+  fetch_targets<16>(c, blockIdx.x * int64_t(64) + step, next_target);
+  RawTarget next_class = fetch_target(c, row);
   for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
     __syncthreads(); // the tile before is done with
-    put_tile(x, stride, next);
+    put_tile<T, 16>(c, x, target, next);
     __syncthreads();
-    fetch_tile<T>(c, (tile + gridDim.x) * 64, next);
+    const int at = class_of(c, row, next_class);
+    classes_of<16>(c, tile * 64 + step, next_target, target);
+    fetch_tile<T, 16>(c, tile * 64 + step, target, next);
+    fetch_targets<16>(c, tile * 64 + 2 * step, next_target);
+    next_class = fetch_target(c, row + step);
     f32x4 z[VB] = {};
-    logits<VB, 1>(w, x + wave * 16 * stride, stride, z);
-    const int64_t row = tile * 64 + wave * 16 + lane % 16;
-    const int64_t target = row < c.rows ? target_of(c, row) : c.ignore;
-    const int at = counted(c, target) ? static_cast<int>(target) : -1;
+    logits<VB, 1, DB>(w, x + wave * 16 * stride, dim16, VB, z);
     float most = -INFINITY, hit = 0.0f;
 #pragma unroll
     for (int v = 0; v < VB; ++v) {
@@ -156,14 +228,15 @@ __global__ void __launch_bounds__(kThreads) few_loss_kernel(FewArgs a) {
     hit += lane_xor_f32(hit, 16);
     total += lane_xor_f32(total, 32);
     hit += lane_xor_f32(hit, 32);
-    if (lane < 16 && row < c.rows) {
+    if (lane < 16 && at > -3) {
       float lse = base + logf(total), loss = lse - hit;
-      if (!counted(c, target)) loss = lse = target == c.ignore ? 0.0f : NAN;
+      if (at < 0) loss = lse = at == -1 ? 0.0f : NAN;
       c.lse[row] = lse;
       c.loss[row] = loss;
       sum += loss;
-      n += target == c.ignore ? 0.0 : 1.0;
+      n += at == -1 ? 0.0 : 1.0;
     }
+    row += step;
   }
   __shared__ double part[2][4];
   const double v = block_sums(sum, n, part);
@@ -174,10 +247,10 @@ __global__ void __launch_bounds__(kThreads) few_loss_kernel(FewArgs a) {
     a.sums[2 * blockIdx.x + threadIdx.x] = v;
 }
 
-__global__ void __launch_bounds__(kThreads) few_total_kernel(FewArgs a, int blocks) {
+__global__ void __launch_bounds__(kLossThreads) few_total_kernel(FewArgs a, int blocks) {
   __shared__ double part[2][4];
   double s = 0.0, n = 0.0;
-  for (int i = threadIdx.x; i < blocks; i += kThreads) {
+  for (int i = threadIdx.x; i < blocks; i += kLossThreads) {
     s += a.sums[2 * i];
     n += a.sums[2 * i + 1];
   }
@@ -185,42 +258,80 @@ __global__ void __launch_bounds__(kThreads) few_total_kernel(FewArgs a, int bloc
   if (threadIdx.x < 2) a.c.sums[threadIdx.x] = static_cast<float>(v);
 }
 
-// ---- backward: TB * 16 rows a tile -----------------------------------------------------
+// ---- backward: 32 rows a tile, eight waves -----------------------------------------------
 
-template <typename T, int VB, int DB, int TB>
-__global__ void __launch_bounds__(kThreads) few_grad_kernel(FewArgs a) {
+constexpr int kRows = 32, kSplit = 4; // waves that share a block of 16 rows
+
+// dx of a tile goes out a tile later, by whole rows through LDS.  (Stored from the
+// accumulators, 64 bytes of 16 rows at a time, it took a third of the kernel's time; stored at
+// the tile's end, the next tile's loads waited for it.)
+template <typename T, int VB, int DB>
+__global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 ? 4 : 2) few_grad_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
-  constexpr int kRows = TB * 16, kSplit = 4 / TB; // waves that share a block of rows
   constexpr int kMine = (VB + kSplit - 1) / kSplit;
-  constexpr int kG = VB * 16 + 4; // floats of a row of g
+  constexpr int kG = VB * 16 + 4;  // floats of a row of g
+  constexpr int kD = (DB + 1) / 2; // blocks of 128 features
+  constexpr int stride = few_stride(DB);
   const CeCall &c = a.c;
-  const int dim16 = static_cast<int>(ceil_div64(c.dim, 16)), stride = dim16 * 16 + 4;
-  float *const w = lds, *const x = w + VB * 16 * stride, *const g = x + kRows * stride;
-  float *const bias = g + kRows * kG;
-  const int lane = lane_id(), wave = threadIdx.x / kWave, q = lane / 16, l = lane % 16;
-  const int tb = wave % TB, part = wave / TB;
-  hold_weights<T, VB, DB>(c, w, bias, stride);
-  f32x4 dw[VB][DB] = {};
+  const int dim16 = static_cast<int>(ceil_div64(c.dim, 16));
+  float *const w = lds, *const x = w + VB * 16 * stride, *const dx = x + kRows * stride;
+  float *const g = dx + kRows * stride, *const bias = g + kRows * kG;
+  const int lane = lane_id(), q = lane / 16, l = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int tb = wave % 2, part = wave / 2;
+  hold_weights<T, VB, DB, kGradThreads>(c, w, bias);
+  f32x4 dw[VB][kD] = {};
   float db[VB] = {};
-  f32x4 next[TB][DB];
-  fetch_tile<T>(c, blockIdx.x * int64_t(kRows), next);
-  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
+  const int64_t step = gridDim.x * int64_t(kRows), first = blockIdx.x * int64_t(kRows);
+  int target[1];            // of the rows on their way
+  RawTarget next_target[1]; // of those after them
+  Words<T, 4> next[1][DB];
+  fetch_targets<32>(c, first, next_target);
+  classes_of<32>(c, first, next_target, target);
+  fetch_tile<T, 32>(c, first, target, next);
+  __builtin_amdgcn_sched_barrier(0); // loads in the loop's order, so that it waits for no later ones
+  fetch_targets<32>(c, first + step, next_target);
+  // This lane's row: its class, scale and lse, a tile ahead too.
+  int64_t row = first + tb * 16 + l;
+  RawTarget next_class;
+  float next_lse, next_scale;
+  auto fetch_row = [&](int64_t r) {
+    next_class = fetch_target(c, r);
+    const int64_t in = min(r, c.rows - 1);
+    next_lse = c.given_lse[in];
+    next_scale = c.grad[in * c.grad_stride];
+  };
+  fetch_row(row);
+  auto put_dx = [&](int64_t tile) {
+    const int64_t r = tile * kRows + threadIdx.x / 16;
+    if (r >= c.rows) return;
+    T *const out = static_cast<T *>(c.dx) + r * c.dx_stride;
+#pragma unroll
+    for (int k = 0; k < DB; ++k) {
+      const int col = k * 64 + threadIdx.x % 16 * 4;
+      if (col >= c.dim) continue;
+      const f32x4 f = *reinterpret_cast<const f32x4 *>(dx + threadIdx.x / 16 * stride + col);
+      const float v[4] = {f[0], f[1], f[2], f[3]};
+      put<true, 4>(out + col, c.dim - col, v);
+    }
+  };
+  int64_t tile = blockIdx.x;
+  for (; tile < a.tiles; tile += gridDim.x) {
+    __syncthreads(); // x is read no more, the last tile's dx is there
+    put_tile<T, 32>(c, x, target, next);
     __syncthreads();
-    put_tile(x, stride, next);
-    __syncthreads();
-    fetch_tile<T>(c, (tile + gridDim.x) * kRows, next);
+    classes_of<32>(c, tile * kRows + step, next_target, target);
+    fetch_tile<T, 32>(c, tile * kRows + step, target, next);
+    fetch_targets<32>(c, tile * kRows + 2 * step, next_target);
+    const int at = class_of(c, row, next_class);
+    const float lse = at >= 0 ? next_lse : 0.0f, s = next_scale;
+    fetch_row(row + step);
+    if (tile != blockIdx.x) put_dx(tile - gridDim.x);
 
     // g of this wave's rows and classes.
-    const int64_t row = tile * kRows + tb * 16 + l;
-    const int64_t target = row < c.rows ? target_of(c, row) : -1;
-    const bool on = row < c.rows && counted(c, target);
-    const int at = on ? static_cast<int>(target) : -1;
-    const float lse = on ? c.given_lse[row] : 0.0f;
-    const float s = on ? c.grad[row * c.grad_stride] : 0.0f;
     f32x4 z[kMine] = {};
-    // With an odd number of blocks the last wave multiplies some of x for its last one
-    // (x lies behind w) and leaves it.
-    logits<kMine, kSplit>(w + part * 16 * stride, x + tb * 16 * stride, stride, z);
+    logits<kMine, kSplit, DB>(w + part * 16 * stride, x + tb * 16 * stride, dim16,
+                              (VB - part + kSplit - 1) / kSplit, z);
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int v = (i * kSplit + part) * 16 + q * 4;
@@ -229,13 +340,14 @@ __global__ void __launch_bounds__(kThreads) few_grad_kernel(FewArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float p = exp_of(z[i][e] + b[e] - lse) - (v + e == at ? 1.0f : 0.0f);
-        z[i][e] = on ? p * s : 0.0f;
+        z[i][e] = at >= 0 ? p * s : 0.0f;
       }
       *reinterpret_cast<f32x4 *>(g + (tb * 16 + l) * kG + v) = z[i];
     }
     __syncthreads();
 
     // dx: this wave's rows and every kSplit-th block of features.
+#pragma unroll 1
     for (int j = part; j < dim16; j += kSplit) {
       f32x4 d = {};
 #pragma unroll
@@ -245,15 +357,11 @@ __global__ void __launch_bounds__(kThreads) few_grad_kernel(FewArgs a) {
         for (int e = 0; e < 4; ++e)
           d = mfma_16x16(w[(v * 16 + q * 4 + e) * stride + j * 16 + l], gv[e], d);
       }
-      const int col = j * 16 + q * 4;
-      if (row < c.rows && col < c.dim) {
-        const float out[4] = {d[0], d[1], d[2], d[3]};
-        put<true, 4>(static_cast<T *>(c.dx) + row * c.dx_stride + col, c.dim - col, out);
-      }
+      *reinterpret_cast<f32x4 *>(dx + (tb * 16 + l) * stride + j * 16 + q * 4) = d;
     }
-    // dw: all classes and every fourth block of features.
-#pragma unroll
-    for (int t = 0; t < TB; ++t) {
+    // dw: all classes and every eighth block of features.
+#pragma unroll 1
+    for (int t = 0; t < kRows / 16; ++t) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int r = t * 16 + q * 4 + e;
@@ -264,24 +372,27 @@ __global__ void __launch_bounds__(kThreads) few_grad_kernel(FewArgs a) {
           db[v] += gv[v];
         }
 #pragma unroll
-        for (int k = 0; k < DB; ++k) {
-          if (k * 4 + wave >= dim16) continue;
-          const float xv = x[r * stride + (k * 4 + wave) * 16 + l];
+        for (int k = 0; k < kD; ++k) {
+          if (k * 8 + wave >= dim16) continue;
+          const float xv = x[r * stride + (k * 8 + wave) * 16 + l];
 #pragma unroll
           for (int v = 0; v < VB; ++v) dw[v][k] = mfma_16x16(gv[v], xv, dw[v][k]);
         }
       }
     }
+    row += step;
   }
+  __syncthreads();
+  put_dx(tile - gridDim.x);
   float *const out = a.dw_part + blockIdx.x * int64_t(VB * 16) * (dim16 * 16);
 #pragma unroll
   for (int v = 0; v < VB; ++v) {
 #pragma unroll
-    for (int k = 0; k < DB; ++k) {
-      if (k * 4 + wave >= dim16) continue;
+    for (int k = 0; k < kD; ++k) {
+      if (k * 8 + wave >= dim16) continue;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
-        out[(v * 16 + q * 4 + e) * (dim16 * 16) + (k * 4 + wave) * 16 + l] = dw[v][k][e];
+        out[(v * 16 + q * 4 + e) * (dim16 * 16) + (k * 8 + wave) * 16 + l] = dw[v][k][e];
     }
     db[v] += lane_xor_f32(db[v], 16);
     db[v] += lane_xor_f32(db[v], 32);
@@ -326,27 +437,25 @@ int class_blocks(int64_t classes) {
   return 0;
 }
 // Blocks of 64 features.
-int feature_blocks(int64_t dim) { return dim <= 64 ? 1 : dim <= 128 ? 2 : dim <= 256 ? 4 : dim <= 512 ? 8 : 0; }
-
-int64_t floats_of(int64_t dim, int blocks, int rows, bool backward) {
-  const int64_t stride = ceil_div64(dim, 16) * 16 + 4;
-  return (blocks * 16 + rows) * stride + (backward ? rows * (blocks * 16 + 4) : 0) + blocks * 16;
-}
-bool fits(int64_t dim, int blocks, int rows, bool backward) {
-  return floats_of(dim, blocks, rows, backward) * 4 + 256 <= kLds;
-}
-// 64 rows a tile where they fit LDS and, beside dw, the registers.
-constexpr bool whole_tile(int vb, int db) { return vb * db < 24 && db < 8; }
-int tile_rows(int64_t dim, int64_t classes) {
-  const int b = class_blocks(classes);
-  return whole_tile(b, feature_blocks(dim)) && fits(dim, b, 64, true) ? 64 : 32;
+int feature_blocks(int64_t dim) {
+  for (int b : {1, 2, 3, 4, 6, 8})
+    if (dim <= b * 64) return b;
+  return 0;
 }
 
-// Workgroups: two per CU where their LDS allows it.
+int64_t floats_of(int64_t dim, int blocks, bool backward) {
+  const int64_t stride = few_stride(feature_blocks(dim));
+  return backward ? (blocks * 16 + 2 * kRows) * stride + kRows * (blocks * 16 + 4) + blocks * 16
+                  : (blocks * 16 + 64) * stride + blocks * 16;
+}
+int64_t lds_of(int64_t dim, int64_t classes, bool backward) {
+  return floats_of(dim, class_blocks(classes), backward) * 4 + 256;
+}
+
+// Workgroups: as many per CU as fit, up to two (sixteen waves) or three of the forward pass's.
 int64_t grid_of(int64_t rows, int64_t dim, int64_t classes, bool backward) {
-  const int tile = backward ? tile_rows(dim, classes) : 64;
-  const int64_t each = floats_of(dim, class_blocks(classes), tile, backward) * 4 + 256;
-  return std::min(ceil_div64(rows, tile), 256 * std::min<int64_t>(kLds / each, 2));
+  const int64_t fit = kLds / lds_of(dim, classes, backward);
+  return std::min(ceil_div64(rows, backward ? kRows : 64), 256 * std::min<int64_t>(fit, backward ? 2 : 3));
 }
 
 template <typename F> int32_t with_blocks(int64_t dim, int64_t classes, F &&f) {
@@ -372,14 +481,16 @@ template <typename F> int32_t with_blocks(int64_t dim, int64_t classes, F &&f) {
   switch (feature_blocks(dim)) {
   case 1: return classes_of(std::integral_constant<int, 1>{});
   case 2: return classes_of(std::integral_constant<int, 2>{});
+  case 3: return classes_of(std::integral_constant<int, 3>{});
   case 4: return classes_of(std::integral_constant<int, 4>{});
+  case 6: return classes_of(std::integral_constant<int, 6>{});
   default: return classes_of(std::integral_constant<int, 8>{});
   }
 }
 
 // LDS past 64 KB has to be asked for.
 template <typename... P, typename... A>
-int32_t launch_lds(void (*kernel)(P...), int64_t grid, int64_t lds, void *stream, A... args) {
+int32_t launch_lds(void (*kernel)(P...), int64_t grid, int threads, int64_t lds, void *stream, A... args) {
   if (lds > 65536 && hipFuncSetAttribute(reinterpret_cast<const void *>(kernel),
                                          hipFuncAttributeMaxDynamicSharedMemorySize,
                                          static_cast<int>(lds)) != hipSuccess) {
@@ -390,7 +501,7 @@ int32_t launch_lds(void (*kernel)(P...), int64_t grid, int64_t lds, void *stream
   const hipError_t err = std::apply(
       [&](P &...p) {
         void *list[] = {static_cast<void *>(&p)...};
-        return hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(grid), dim3(kThreads), list,
+        return hipLaunchKernel(reinterpret_cast<const void *>(kernel), dim3(grid), dim3(threads), list,
                                lds, static_cast<hipStream_t>(stream));
       },
       held);
@@ -426,19 +537,14 @@ FewLayout few_layout(int64_t rows, int64_t dim, int64_t classes, bool backward) 
 template <typename T> int32_t few_loss(const FewArgs &a, int64_t grid, void *stream) {
   return with_blocks(a.c.dim, a.c.classes, [&](auto vb, auto db) {
     constexpr int VB = decltype(vb)::value, DB = decltype(db)::value;
-    return launch_lds(few_loss_kernel<T, VB, DB>, grid, floats_of(a.c.dim, VB, 64, false) * 4, stream, a);
+    return launch_lds(few_loss_kernel<T, VB, DB>, grid, kLossThreads, floats_of(a.c.dim, VB, false) * 4, stream, a);
   });
 }
 
 template <typename T> int32_t few_grad(const FewArgs &a, int64_t grid, void *stream) {
-  const int rows = tile_rows(a.c.dim, a.c.classes);
   return with_blocks(a.c.dim, a.c.classes, [&](auto vb, auto db) {
     constexpr int VB = decltype(vb)::value, DB = decltype(db)::value;
-    const int64_t lds = floats_of(a.c.dim, VB, rows, true) * 4;
-    if constexpr (whole_tile(VB, DB)) {
-      if (rows == 64) return launch_lds(few_grad_kernel<T, VB, DB, 4>, grid, lds, stream, a);
-    }
-    return launch_lds(few_grad_kernel<T, VB, DB, 2>, grid, lds, stream, a);
+    return launch_lds(few_grad_kernel<T, VB, DB>, grid, kGradThreads, floats_of(a.c.dim, VB, true) * 4, stream, a);
   });
 }
 
@@ -446,7 +552,7 @@ template <typename T> int32_t few_grad(const FewArgs &a, int64_t grid, void *str
 
 bool few_takes(int64_t dim, int64_t classes, bool backward) {
   const int b = class_blocks(classes), f = feature_blocks(dim);
-  return b && f && b * f <= 24 && fits(dim, b, backward ? 32 : 64, backward);
+  return dim >= 4 && b && f && b * f <= 24 && lds_of(dim, classes, backward) <= kLds;
 }
 
 size_t few_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward) {
@@ -461,13 +567,13 @@ int32_t few_forward(const CeCall &c, void *work, void *stream) {
                      : c.type == SPORDER_TYPE_F16 ? few_loss<f16_t>(a, l.grid, stream)
                                                   : few_loss<float>(a, l.grid, stream);
   if (rc != SPORDER_OK || l.grid == 1) return rc;
-  return launch(few_total_kernel, dim3(1), dim3(kThreads), stream, a, static_cast<int>(l.grid));
+  return launch(few_total_kernel, dim3(1), dim3(kLossThreads), stream, a, static_cast<int>(l.grid));
 }
 
 int32_t few_backward(const CeCall &c, void *work, void *stream) {
   const FewLayout l = few_layout(c.rows, c.dim, c.classes, true);
   char *const base = static_cast<char *>(work);
-  FewArgs a{c, ceil_div64(c.rows, tile_rows(c.dim, c.classes)), nullptr,
+  FewArgs a{c, ceil_div64(c.rows, kRows), nullptr,
             reinterpret_cast<float *>(base + l.dw), reinterpret_cast<float *>(base + l.db)};
   const int32_t rc = c.type == SPORDER_TYPE_BF16  ? few_grad<bf16_t>(a, l.grid, stream)
                      : c.type == SPORDER_TYPE_F16 ? few_grad<f16_t>(a, l.grid, stream)

@@ -116,7 +116,7 @@ __device__ __forceinline__ int wave_total(int v) {
 // The rows' places in the list: those counted before the block, then before the
 // thread in it.
 __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward) {
-  __shared__ int32_t part[4], most;
+  __shared__ int32_t part[4], placed[kListBlock / 256][4], most;
   const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   const int64_t first = blockIdx.x * int64_t(kListBlock);
   if (tid == 0) most = -1000;
@@ -130,37 +130,50 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward) {
     for (int64_t b = tid; b < blockIdx.x; b += 256) before += a.counts[b];
   }
   before = block_total(wave_total(before), part);
+  constexpr int kEach = kListBlock / 256;
+  int64_t target[kEach];
+  float scale[kEach] = {}, row_lse[kEach] = {};
 #pragma unroll
-  for (int k = 0; k < kListBlock / 256; ++k) {
+  for (int k = 0; k < kEach; ++k) { // past the rows the last one
+    const int64_t row = min(first + k * 256 + tid, a.rows - 1);
+    target[k] = target_of(a, row);
+    if (backward) {
+      scale[k] = a.grad[row * a.grad_stride];
+      row_lse[k] = a.given_lse[row];
+    }
+  }
+  uint64_t mask[kEach];
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
+    mask[k] = __ballot(first + k * 256 + tid < a.rows && counted(a, target[k]));
+    if (lane == 0) placed[k][wave] = __popcll(mask[k]);
+  }
+  __syncthreads();
+  int top = -1000;
+#pragma unroll
+  for (int k = 0; k < kEach; ++k) {
     const int64_t row = first + k * 256 + tid;
-    const bool inside = row < a.rows;
-    const int64_t target = inside ? target_of(a, row) : -1;
-    const bool on = inside && counted(a, target);
-    const uint64_t mask = __ballot(on);
-    __syncthreads();
-    if (lane == 0) part[wave] = __popcll(mask);
-    __syncthreads();
-    int at = before + __popcll(mask & ((uint64_t(1) << lane) - 1));
-    for (int w = 0; w < wave; ++w) at += part[w];
-    if (on) {
+    int at = before + __popcll(mask[k] & ((uint64_t(1) << lane) - 1));
+    for (int w = 0; w < wave; ++w) at += placed[k][w];
+    if (mask[k] >> lane & 1) {
       a.list[at] = static_cast<int32_t>(row);
-      a.target[at] = static_cast<int32_t>(target);
+      a.target[at] = static_cast<int32_t>(target[k]);
       if (backward) {
-        const float s = a.grad[row * a.grad_stride];
         // |s| = m 2^e with 1 <= m < 2 (a scale below 2^-126 keeps its place in m).
-        const int e = max(static_cast<int>(__builtin_bit_cast(uint32_t, s) >> 23 & 255), 1) - 127;
+        const int e = max(static_cast<int>(__builtin_bit_cast(uint32_t, scale[k]) >> 23 & 255), 1) - 127;
         a.exponent[at] = e;
-        a.mantissa[at] = ldexpf(s, -e);
-        a.row_lse[at] = a.given_lse[row];
-        if (s != 0.0f) atomicMax(&most, e);
+        a.mantissa[at] = ldexpf(scale[k], -e);
+        a.row_lse[at] = row_lse[k];
+        if (scale[k] != 0.0f) top = max(top, e);
       }
-    } else if (inside && !backward) {
-      const float none = target == a.ignore ? 0.0f : NAN;
+    } else if (row < a.rows && !backward) {
+      const float none = target[k] == a.ignore ? 0.0f : NAN;
       a.loss[row] = none;
       a.lse[row] = none;
     }
-    before += part[0] + part[1] + part[2] + part[3];
+    before += placed[k][0] + placed[k][1] + placed[k][2] + placed[k][3];
   }
+  if (backward) atomicMax(&most, top);
   __syncthreads();
   if (backward && tid == 0) atomicMax(&a.meta->most, most);
   if (blockIdx.x != gridDim.x - 1) return;
@@ -294,19 +307,31 @@ __global__ void __launch_bounds__(256)
   const int64_t all = list ? meta->count : rows;
   const int64_t k0 = blockIdx.x * int64_t(64), j0 = blockIdx.y * int64_t(64);
   if (k0 >= all) return;
-  const int x = threadIdx.x % 64, y = threadIdx.x / 64;
+  constexpr int kVec = 16 / sizeof(T), kAcross = 64 / kVec, kRound = 256 / kAcross, kRounds = 64 / kRound;
+  const int x = threadIdx.x % kAcross * kVec, y = threadIdx.x / kAcross;
   const int top = list ? meta->most : 0;
-  const bool in = j0 + x < dim;
-  const float scale = in ? unit_inverse(unit_of(most[j0 + x])) : 0.0f;
+  const int64_t col = j0 + x;
+  Pack<T, kVec> q[kRounds];
+  int power[kRounds] = {};
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int64_t k = k0 + y + 4 * i;
-    float v = 0.0f;
-    if (in && k < all) {
-      v = static_cast<float>(src[(list ? list[k] : k) * stride + j0 + x]) * scale;
-      if (list) v = ldexpf(v, min(exponent[k] - top, 0)); // no row has a scale: top is below all
+  for (int i = 0; i < kRounds; ++i) {
+    const int64_t k = min(k0 + y + i * kRound, all - 1);
+    q[i] = {};
+    if (col < dim) q[i] = fetch<true, kVec>(src + (list ? list[k] : k) * stride + col, dim - col);
+    if (list) power[i] = min(exponent[k] - top, 0); // no row has a scale: top is below all
+  }
+  float scale[kVec];
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) scale[e] = unit_inverse(unit_of(most[min(col + e, dim - 1)]));
+#pragma unroll
+  for (int i = 0; i < kRounds; ++i) {
+    const int r = y + i * kRound;
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) {
+      float v = static_cast<float>(q[i].v[e]) * scale[e];
+      if (list) v = ldexpf(v, power[i]);
+      tile[r][x + e] = k0 + r < all ? v : 0.0f;
     }
-    tile[y + 4 * i][x] = v;
   }
   __syncthreads();
 #pragma unroll
@@ -334,21 +359,37 @@ template <typename S> constexpr int logit_lds(bool backward) {
   return backward ? std::max(std::max(a, b), c) : c;
 }
 
+// Where a lane holds row `row` of a wave's MB blocks: i * 16 + r of its register, or -1.
+template <int MB> __device__ __forceinline__ int register_of(int row) {
+  return row >= 0 && row < MB * 32 && (row >> 2 & 1) == lane_id() / 32
+             ? (row >> 5) * 16 + (row >> 3 & 3) * 4 + (row & 3)
+             : -1;
+}
+
 // z of a tile: classes (from v0 on) down, listed rows across.
 template <typename U, int PLANES, typename S>
 __device__ __forceinline__ void logit_tile(const CeArgs &a, char *lds, int wave, int64_t m0, int64_t n0,
                                            int64_t v0, int count, f32x16 (&acc)[S::MB][S::NB]) {
-  uint32_t a_off[S::kFetchA], b_off[S::kFetchB];
-  fetch_offsets<S::kWaves>(wave, a_off, [&](int r) {
+  auto a_row = [&](int r) {
     return static_cast<uint32_t>(min(static_cast<int64_t>(r), a.classes - 1 - v0 - m0) * a.wp_stride);
-  });
-  fetch_offsets<S::kWaves>(wave, b_off, [&](int r) {
+  };
+  auto b_row = [&](int r) {
     const int64_t n = min(n0 + r, int64_t(count) - 1);
     return static_cast<uint32_t>((a.x_packed ? n - n0 : a.list[n]) * a.xp_stride);
-  });
-  tile_product<U, PLANES, S>(lds, wave, a.wp + (v0 + m0) * a.wp_stride, a.wp_plane, a_off,
-                             a.xp + (a.x_packed ? n0 * a.xp_stride : 0), a.xp_plane, b_off,
-                             static_cast<int>(ceil_div64(a.dim, kStageK)), acc);
+  };
+  const char *const pa = a.wp + (v0 + m0) * a.wp_stride, *const pb = a.xp + (a.x_packed ? n0 * a.xp_stride : 0);
+  const int stages = static_cast<int>(ceil_div64(a.dim, kStageK));
+  if constexpr (S::kThreads == 512) {
+    uint32_t a_off[S::kM / 16 / S::kWaves], b_off[S::kN / 16 / S::kWaves];
+    ring_offsets(wave, a_off, a_row);
+    ring_offsets(wave, b_off, b_row);
+    ring_product<U, PLANES, S>(lds, wave, pa, a.wp_plane, a_off, pb, a.xp_plane, b_off, stages, acc);
+  } else {
+    uint32_t a_off[S::kFetchA], b_off[S::kFetchB];
+    fetch_offsets<S::kWaves>(wave, a_off, a_row);
+    fetch_offsets<S::kWaves>(wave, b_off, b_row);
+    tile_product<U, PLANES, S>(lds, wave, pa, a.wp_plane, a_off, pb, a.xp_plane, b_off, stages, acc);
+  }
   // Units and bias.
   const int lane = lane_id(), wm = wave / S::WN, wn = wave % S::WN;
   float x_unit[S::NB];
@@ -377,8 +418,8 @@ __device__ __forceinline__ void logit_tile(const CeArgs &a, char *lds, int wave,
           acc[i][j][4 * q + e] = (PLANES == 2 ? z * unit[e] * un : z) + bias[e];
         }
       }
+      __builtin_amdgcn_sched_barrier(0); // all vectors at once would not fit the registers
     }
-    __builtin_amdgcn_sched_barrier(0); // all blocks' vectors at once would not fit the registers
   }
 }
 
@@ -397,21 +438,18 @@ __global__ void __launch_bounds__(S::kThreads) ce_loss_kernel(CeArgs a) {
 #pragma unroll
   for (int j = 0; j < S::NB; ++j) {
     const int64_t n = n0 + (wn * S::NB + j) * 32 + lane % 32;
-    const int target = (n < count ? a.target[n] : -1) - static_cast<int>(m0);
+    const int met = register_of<S::MB>(n < count ? a.target[n] - static_cast<int>(m0) - wm * S::MB * 32 : -1);
     float most = -INFINITY, hit = 0.0f;
-    bool met = false;
 #pragma unroll
     for (int i = 0; i < S::MB; ++i) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         most = fmaxf(most, acc[i][j][r]);
-        const bool here = (wm * S::MB + i) * 32 + result_row(r) == target;
-        hit = here ? acc[i][j][r] : hit;
-        met = met || here;
+        hit = met == i * 16 + r ? acc[i][j][r] : hit;
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if (met) a.hit[n] = hit;
+    if (met >= 0) a.hit[n] = hit;
     most = fmaxf(most, lane_xor_f32(most, 32));
     const float base = most == -INFINITY ? 0.0f : most;
     float sum = 0.0f;
@@ -419,6 +457,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_loss_kernel(CeArgs a) {
     for (int i = 0; i < S::MB; ++i) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) sum += exp_of(acc[i][j][r] - base);
+      __builtin_amdgcn_sched_barrier(0);
     }
     sum += lane_xor_f32(sum, 32);
     if (lane < 32 && n < count)
@@ -510,7 +549,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
   for (int j = 0; j < S::NB; ++j) {
     const int64_t n = n0 + (wn * S::NB + j) * 32 + lane % 32;
     const bool on = n < count;
-    target[j] = on ? a.target[n] - static_cast<int>(v0 + m0) : -1;
+    target[j] = register_of<S::MB>(on ? a.target[n] - static_cast<int>(v0 + m0) - wm * S::MB * 32 : -1);
     lse[j] = on ? a.row_lse[n] : 0.0f;
     m[j] = on ? a.mantissa[n] * (1 << kShift) : 0.0f;
     grad[j] = on ? ldexpf(a.mantissa[n], a.exponent[n]) : 0.0f;
@@ -522,8 +561,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
     for (int j = 0; j < S::NB; ++j) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int row = (wm * S::MB + i) * 32 + result_row(r);
-        float g = exp_of(acc[i][j][r] - lse[j]) - (row == target[j] ? 1.0f : 0.0f);
+        float g = exp_of(acc[i][j][r] - lse[j]) - (target[j] == i * 16 + r ? 1.0f : 0.0f);
         g = n0 + (wn * S::NB + j) * 32 + lane % 32 < count ? g : 0.0f; // the product is of another row
         total[r] += g * grad[j];
         acc[i][j][r] = g * m[j];
@@ -542,25 +580,29 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
   constexpr int kDown = S::kM * 2 + 16, kAcross = S::kN * 2 + 16; // bytes of a row in LDS
 #pragma unroll
   for (int plane = 0; plane < PLANES; ++plane) {
-    // A plane's halves, two classes of a token in a word.
-    uint32_t half[S::MB][S::NB][8];
+    // A plane's halves of classes 2 r and 2 r + 1 of a token.
+    auto half = [&](int i, int j, int r) {
+      Pack<f16_t, 2> p;
 #pragma unroll
-    for (int i = 0; i < S::MB; ++i) {
+      for (int e = 0; e < 2; ++e) {
+        const float v = acc[i][j][2 * r + e];
+        p.v[e] = static_cast<f16_t>(v);
+        if (plane) p.v[e] = static_cast<f16_t>(v - static_cast<float>(p.v[e]));
+      }
+      return __builtin_bit_cast(uint32_t, p);
+    };
+    // Not to keep the halves from one use to the next: with the sums they are more than
+    // the registers.
+    auto forget = [&] {
+      if constexpr (PLANES == 2) {
 #pragma unroll
-      for (int j = 0; j < S::NB; ++j) {
+        for (int i = 0; i < S::MB; ++i) {
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          Pack<f16_t, 2> p;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float v = acc[i][j][2 * r + e];
-            p.v[e] = static_cast<f16_t>(v);
-            if constexpr (PLANES == 2) acc[i][j][2 * r + e] = v - static_cast<float>(p.v[e]);
-          }
-          half[i][j][r] = __builtin_bit_cast(uint32_t, p);
+          for (int j = 0; j < S::NB; ++j) asm volatile("" : "+v"(acc[i][j]));
         }
       }
-    }
+    };
+    forget();
     if (plane) __syncthreads();
 #pragma unroll
     for (int i = 0; i < S::MB; ++i) {
@@ -570,17 +612,19 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
         for (int q = 0; q < 4; ++q)
           *reinterpret_cast<uint2 *>(lds + ((wn * S::NB + j) * 32 + lane % 32) * kDown +
                                      ((wm * S::MB + i) * 32 + result_row(4 * q)) * 2) =
-              make_uint2(half[i][j][2 * q], half[i][j][2 * q + 1]);
+              make_uint2(half(i, j, 2 * q), half(i, j, 2 * q + 1));
       }
     }
     __syncthreads();
     char *const g = a.g + plane * (a.rows_pad * a.piece * 2) + (n0 * a.piece + m0) * 2;
+#pragma unroll 4
     for (int c = tid; c < S::kN * (S::kM / 8); c += S::kThreads) {
       const int row = c / (S::kM / 8), part = c % (S::kM / 8);
       *reinterpret_cast<uint4 *>(g + row * a.piece * 2 + part * 16) =
           *reinterpret_cast<const uint4 *>(lds + row * kDown + part * 16);
     }
     __syncthreads();
+    forget();
     // A word holds classes r and r + 1 of a token; with the neighbouring token's,
     // an even lane makes class r's word of both and an odd one r + 1's.
 #pragma unroll
@@ -589,7 +633,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
       for (int j = 0; j < S::NB; ++j) {
 #pragma unroll
         for (int r = 0; r < 16; r += 2) {
-          const uint32_t mine = half[i][j][r / 2];
+          const uint32_t mine = half(i, j, r / 2);
           const uint32_t word = __builtin_amdgcn_perm(lane_xor_u32(mine, 1), mine,
                                                       lane & 1 ? 0x03020706 : 0x05040100);
           const int row = (wm * S::MB + i) * 32 + result_row(r) + (lane & 1);
@@ -600,6 +644,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
     }
     __syncthreads();
     char *const gt = a.gt + plane * (a.rows_pad * a.piece * 2) + (m0 * a.rows_pad + n0) * 2;
+#pragma unroll 4
     for (int c = tid; c < S::kM * (S::kN / 8); c += S::kThreads) {
       const int row = c / (S::kN / 8), part = c % (S::kN / 8);
       *reinterpret_cast<uint4 *>(gt + row * a.rows_pad * 2 + part * 16) =
@@ -620,18 +665,29 @@ __device__ __forceinline__ void put_four(O *row, int64_t j, int64_t dim, bool wh
     if (j + e < dim) row[j + e] = static_cast<O>(v[e]);
 }
 
+// A product's workgroups in a launch: `tiles` of them for each of `splits` parts of the sum,
+// from workgroup `first` (a multiple of the XCDs) on.
+struct CeShare {
+  int64_t first, tiles;
+  int splits;
+};
+
 // dx (DX) or the piece's rows of dw: features down, listed rows or classes across, over
-// one of gridDim.y parts of the sum.  A sum in one part, over one piece, goes straight
-// to the output; else to the part's place in 32 bits, added to what is there past the
-// first piece.
+// part `split` of the sum.  A sum in one part, over one piece, goes straight to the
+// output (`direct`); else to the part's place in 32 bits, added to what is there past the
+// first piece (`add`).
 template <int PLANES, typename S, typename O, bool DX>
-__global__ void __launch_bounds__(S::kThreads)
-    ce_gradient_kernel(CeArgs a, int64_t v0, bool direct, bool add) {
-  __shared__ __attribute__((aligned(16))) char lds[2 * S::kStage];
+__device__ __forceinline__ void gradient_tile(const CeArgs &a, char *lds, int64_t v0, const CeShare &share,
+                                              bool direct, bool add) {
   const int count = a.meta->count;
   const int64_t here = min(a.piece, a.classes - v0), across = DX ? a.rows : here;
+  const int64_t at = blockIdx.x - share.first, all = share.tiles * share.splits;
+  if (at >= all) return; // between two shares
+  const int64_t each_xcd = all / kXcds, more = all % kXcds, xcd = at % kXcds;
+  const int64_t t = xcd * each_xcd + min(xcd, more) + at / kXcds; // as xcd_block
+  const int split = static_cast<int>(t / share.tiles);
   int64_t ti, tj;
-  place_tile(xcd_block(), ceil_div64(a.dim, S::kM), ceil_div64(across, S::kN), 8, ti, tj);
+  place_tile(t % share.tiles, ceil_div64(a.dim, S::kM), ceil_div64(across, S::kN), 8, ti, tj);
   const int64_t m0 = ti * S::kM, n0 = tj * S::kN;
   const int64_t limit = DX ? count : here;
   if (n0 >= limit) return;
@@ -646,8 +702,8 @@ __global__ void __launch_bounds__(S::kThreads)
     return static_cast<uint32_t>(min(static_cast<int64_t>(r), limit - 1 - n0) * stride);
   });
   f32x16 acc[S::MB][S::NB] = {};
-  const int64_t stages = ceil_div64(DX ? here : count, kStageK), each = ceil_div64(stages, gridDim.y);
-  const int64_t first = min(blockIdx.y * each, stages), mine = min(each, stages - first);
+  const int64_t stages = ceil_div64(DX ? here : count, kStageK), each = ceil_div64(stages, share.splits);
+  const int64_t first = min(split * each, stages), mine = min(each, stages - first);
   tile_product<f16_t, PLANES, S>(lds, wave, (DX ? a.wt : a.xt) + m0 * stride + first * kStageBytes,
                                  a.dim * stride, a_off,
                                  (DX ? a.g : a.gt) + n0 * stride + first * kStageBytes,
@@ -655,7 +711,7 @@ __global__ void __launch_bounds__(S::kThreads)
   O *const out = static_cast<O *>(DX ? a.dx : a.dw);
   const int64_t out_stride = DX ? a.dx_stride : a.dw_stride;
   const bool whole = out_stride % 4 == 0 && reinterpret_cast<uintptr_t>(out) % (4 * sizeof(O)) == 0;
-  float *const part = (DX ? a.dx_part : a.dw_part) + blockIdx.y * ((DX ? a.rows_pad : a.piece) * a.dim_pad);
+  float *const part = (DX ? a.dx_part : a.dw_part) + split * ((DX ? a.rows_pad : a.piece) * a.dim_pad);
 #pragma unroll
   for (int j = 0; j < S::NB; ++j) {
     const int64_t n = n0 + (wn * S::NB + j) * 32 + lane % 32;
@@ -687,6 +743,19 @@ __global__ void __launch_bounds__(S::kThreads)
       }
     }
   }
+}
+
+// Both gradients of a piece in one launch, the longer sums first, so that the last ones
+// fill what a launch of their own would leave idle.
+template <int PLANES, typename S, typename T, typename O>
+__global__ void __launch_bounds__(S::kThreads)
+    ce_gradients_kernel(CeArgs a, int64_t v0, CeShare dx, CeShare dw, bool dx_direct, bool add, bool dw_direct) {
+  __shared__ __attribute__((aligned(16))) char lds[2 * S::kStage];
+  const bool first_dx = dx.first < dw.first;
+  if (first_dx == (blockIdx.x < max(dx.first, dw.first)))
+    gradient_tile<PLANES, S, T, true>(a, lds, v0, dx, dx_direct, add);
+  else
+    gradient_tile<PLANES, S, O, false>(a, lds, v0, dw, dw_direct, false);
 }
 
 // The parts' sum, four elements of a row per thread.
@@ -761,27 +830,42 @@ bool direct_rows(int type, int64_t dim, int64_t stride, const void *p, int64_t s
          span_rows * stride * 2 < (int64_t(1) << 32);
 }
 
-// Turns of the card's tiles (256 large ones or 512 middle ones at a time, the latter at
-// some 0.65 of a large one's time) times the length of a part, and what a part in 32
-// bits costs besides, as a length: written and read, 900 elements' products.
-Cut cut_product(int64_t down, int64_t across, int64_t length, bool may_split) {
-  Cut best{1, 1};
-  double least = 0.0;
-  const int64_t fewest = may_split ? ceil_div64(length, 65536) : 1; // shorter 32-bit sums
+// A large tile (256 x 256, one to a CU) does 1.3 times the products in its time that the
+// four middle ones of its place (two to a CU) do: 8,192 x 50,000 x 2,048 1.09 and 0.83 PFLOP/s,
+// short sums nearer.
+constexpr double kMiddleTime = 0.65; // of a middle tile, two at a time, beside a large one's
+
+Cut cut_logits(int64_t classes, int64_t rows) {
+  const double large = static_cast<double>(ceil_div64(ceil_div64(classes, 256) * ceil_div64(rows, 256), 256));
+  const double middle = static_cast<double>(ceil_div64(ceil_div64(classes, 128) * ceil_div64(rows, 128), 512));
+  return {large <= middle * kMiddleTime ? 2 : 1, 1};
+}
+
+// The shape of both gradients' tiles and the parts of their sums: least time for all tiles
+// over the card, the last ones half idle on average.  A part in 32 bits costs what 900
+// elements of the sum do (written and read), and 32-bit sums stay below 65,536 terms.
+void cut_gradients(int64_t dim, int64_t rows, int64_t classes, Cut &dx, Cut &dw) {
+  double least = -1.0;
+  auto parts = [](int64_t length) { return ceil_div64(length, 65536); };
   for (int shape : {1, 2}) {
-    const int64_t side = shape == 2 ? 256 : 128, slots = shape == 2 ? 256 : 512;
-    const int64_t tiles = ceil_div64(down, side) * ceil_div64(across, side);
-    const int64_t most = may_split ? std::max(fewest, std::min<int64_t>(length / 512, 32)) : 1;
-    for (int64_t s = fewest; s <= most; ++s) {
-      const double turns = static_cast<double>(ceil_div64(tiles * s, slots));
-      const double cost = turns * (static_cast<double>(length) / s + (s > 1 ? 900.0 : 0.0)) * (shape == 2 ? 1.0 : 0.65);
-      if (least == 0.0 || cost < least) {
-        least = cost;
-        best = {shape, static_cast<int>(s)};
+    const int64_t side = shape == 2 ? 256 : 128;
+    const double slots = shape == 2 ? 256 : 512, unit = shape == 2 ? 1.0 : kMiddleTime;
+    const int64_t down = ceil_div64(dim, side);
+    const int64_t nx = down * ceil_div64(rows, side), nw = down * ceil_div64(classes, side);
+    for (int64_t sx = parts(classes); sx <= std::max<int64_t>(parts(classes), std::min<int64_t>(classes / 512, 32)); ++sx) {
+      for (int64_t sw = parts(rows); sw <= std::max<int64_t>(parts(rows), std::min<int64_t>(rows / 512, 32)); ++sw) {
+        const double x = static_cast<double>(classes) / sx + (sx > 1 ? 900.0 : 0.0) + 200.0;
+        const double w = static_cast<double>(rows) / sw + (sw > 1 ? 900.0 : 0.0) + 200.0;
+        const double all = x * (nx * sx) + w * (nw * sw);
+        const double time = std::max(std::max(x, w), all / slots + 0.5 * std::min(x, w)) * unit;
+        if (least < 0.0 || time < least) {
+          least = time;
+          dx = {shape, static_cast<int>(sx)};
+          dw = {shape, static_cast<int>(sw)};
+        }
       }
     }
   }
-  return best;
 }
 
 CePlan lay_out(CeArgs &a, bool backward, void *work) {
@@ -800,7 +884,7 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     }
   }
   a.classes_pad = ceil_div64(a.classes, a.piece) * a.piece;
-  p.z = cut_product(a.piece, a.rows, a.dim, false);
+  p.z = cut_logits(std::min(a.piece, a.classes), a.rows);
   if (!backward && a.rows <= 64) p.z.shape = 0;
   const int down = p.z.shape == 2 ? Large::kM : Middle::kM; // classes of a tile
   a.chunks = ceil_div64(a.classes, down) * (p.z.shape == 0 ? Narrow::WM : 2);
@@ -845,8 +929,7 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     take(a.exponent, a.rows_pad);
     take(a.mantissa, a.rows_pad);
     take(a.row_lse, a.rows_pad);
-    p.dx = cut_product(a.dim, a.rows, a.piece, true);
-    p.dw = cut_product(a.dim, a.piece, a.rows, true);
+    cut_gradients(a.dim, a.rows, std::min(a.piece, a.classes), p.dx, p.dw);
     take(a.x_most, a.dim);
     take(a.w_most, a.dim);
     take(a.most_part, kStrips * a.dim);
@@ -964,27 +1047,25 @@ template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, 
         return launch(ce_bias_kernel, dim3(a.piece / 64), dim3(256), stream, a, v0,
                       p.z.shape == 2 ? Large::kN : Middle::kN);
       });
-    auto dx = [&](auto shape) {
-      using S = decltype(shape);
-      return launch(ce_gradient_kernel<PLANES, S, T, true>,
-                    dim3(ceil_div64(a.dim, S::kM) * ceil_div64(a.rows, S::kN), p.dx.splits), dim3(S::kThreads),
-                    stream, a, v0, dx_direct, v0 > 0);
-    };
-    steps([&] { return p.dx.shape == 2 ? dx(Large{}) : dx(Middle{}); });
-    auto dw = [&](auto shape, auto kind) {
+    auto gradients = [&](auto shape, auto kind) {
       using S = decltype(shape);
       using O = decltype(kind);
-      return launch(ce_gradient_kernel<PLANES, S, O, false>,
-                    dim3(ceil_div64(a.dim, S::kM) * ceil_div64(here, S::kN), p.dw.splits), dim3(S::kThreads),
-                    stream, a, v0, p.dw.splits == 1, false);
+      const int64_t down = ceil_div64(a.dim, S::kM);
+      CeShare dx{0, down * ceil_div64(a.rows, S::kN), p.dx.splits};
+      CeShare dw{0, down * ceil_div64(here, S::kN), p.dw.splits};
+      const bool dx_first = here / dx.splits >= a.rows / dw.splits;
+      CeShare &one = dx_first ? dx : dw, &two = dx_first ? dw : dx;
+      two.first = ceil_div64(one.tiles * one.splits, kXcds) * kXcds;
+      return launch(ce_gradients_kernel<PLANES, S, T, O>, dim3(two.first + two.tiles * two.splits),
+                    dim3(S::kThreads), stream, a, v0, dx, dw, dx_direct, v0 > 0, p.dw.splits == 1);
     };
     auto finish_dw = [&](auto kind) {
       return finish<decltype(kind), false>(a, v0, here, p.dw.splits, stream);
     };
     const bool wide = sizeof(T) == 2 && a.dw_type == SPORDER_TYPE_F32;
     steps([&] {
-      if (wide) return p.dw.shape == 2 ? dw(Large{}, float{}) : dw(Middle{}, float{});
-      return p.dw.shape == 2 ? dw(Large{}, T{}) : dw(Middle{}, T{});
+      if (wide) return p.dx.shape == 2 ? gradients(Large{}, float{}) : gradients(Middle{}, float{});
+      return p.dx.shape == 2 ? gradients(Large{}, T{}) : gradients(Middle{}, T{});
     });
     if (p.dw.splits > 1) steps([&] { return wide ? finish_dw(float{}) : finish_dw(T{}); });
   }

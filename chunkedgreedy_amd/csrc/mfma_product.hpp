@@ -136,6 +136,90 @@ __device__ __forceinline__ void tile_product(char *lds, int wave, const char *a,
   stage_barrier();
 }
 
+// The same for short sums: LDS as a ring of four slots of 32 elements, three of them on
+// their way or read from, so that a sum begins with three fetches in flight and its
+// matrix instructions go on over the barriers: the first half of a slot's operands is
+// read before the barrier that ends the slot before.  2,048 elements of 256 x 256 tiles:
+// 1.09 PFLOP/s, 0.98 with two stages; 7,424 elements 0.92, 0.95 with two stages.
+template <typename U, int PLANES, typename S>
+__device__ __forceinline__ void ring_product(char *lds, int wave, const char *a, int64_t a_plane,
+                                             const uint32_t (&a_off)[S::kM / 16 / S::kWaves], const char *b,
+                                             int64_t b_plane, const uint32_t (&b_off)[S::kN / 16 / S::kWaves],
+                                             int stages, f32x16 (&acc)[S::MB][S::NB]) {
+  using Vec = typename HalfVector<U>::type;
+  constexpr int kFetchA = S::kM / 16 / S::kWaves, kFetchB = S::kN / 16 / S::kWaves; // 16 rows each
+  constexpr int kRing = 4, kHalf = kStageBytes / 2, kSlot = (S::kM + S::kN) * kHalf;
+  static_assert(kFetchA + kFetchB == 4); // the waits below leave the last two slots' fetches
+  const int lane = lane_id(), wm = wave / S::WN, wn = wave % S::WN, row = lane % 32;
+  const uint32_t to = lds_address(lds);
+  const int slots = 2 * (PLANES == 2 ? 3 * stages : stages);
+  auto issue = [&](int s, int slot) {
+    int64_t at = int64_t(s) * kHalf;
+    const char *pa = a, *pb = b;
+    if constexpr (PLANES == 2) { // hi hi, hi lo, lo hi
+      const int part = s % 3;
+      at = int64_t(s / 3) * kHalf;
+      pa += part == 2 ? a_plane : 0;
+      pb += part == 1 ? b_plane : 0;
+    }
+    const uint32_t base = to + slot * kSlot;
+#pragma unroll
+    for (int i = 0; i < kFetchA; ++i) fetch_to_lds(pa + at, a_off[i], base + (wave * kFetchA + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < kFetchB; ++i)
+      fetch_to_lds(pb + at, b_off[i], base + S::kM * kHalf + (wave * kFetchB + i) * 1024);
+  };
+  Vec va[2][S::MB], vb[2][S::NB];
+  auto load = [&](int slot, int k) {
+    const char *const p = lds + slot * kSlot + row * kHalf + ((2 * k + lane / 32) ^ (row / 2 % 4)) * 16;
+#pragma unroll
+    for (int j = 0; j < S::NB; ++j)
+      vb[k][j] = *reinterpret_cast<const Vec *>(p + (S::kM + (wn * S::NB + j) * 32) * kHalf);
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i)
+      va[k][i] = *reinterpret_cast<const Vec *>(p + (wm * S::MB + i) * 32 * kHalf);
+  };
+  auto multiply = [&](int k) {
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int i = 0; i < S::MB; ++i) {
+#pragma unroll
+      for (int j = 0; j < S::NB; ++j) acc[i][j] = mfma_32x32(va[k][i], vb[k][j], acc[i][j]);
+    }
+    __builtin_amdgcn_s_setprio(0);
+  };
+  // The slot after the one in use has arrived for every wave, and every wave's reads
+  // of the one before are done.
+  auto next_slot = [&] {
+    asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kRing - 1; ++s) issue(min(s, slots - 1), s);
+  next_slot();
+  load(0, 0);
+  for (int s = 0; s < slots; ++s) {
+    issue(min(s + kRing - 1, slots - 1), (s + kRing - 1) % kRing); // past the end the last one again
+    load(s % kRing, 1);
+    multiply(0);
+    next_slot();
+    load((s + 1) % kRing, 0);
+    multiply(1);
+  }
+  stage_barrier();
+}
+
+// Offsets for ring_product: sixteen rows an access, a row's four parts in the order
+// part ^ (row / 2 % 4).
+template <int COUNT, typename F>
+__device__ __forceinline__ void ring_offsets(int wave, uint32_t (&out)[COUNT], F &&row_offset) {
+  const int lane = lane_id();
+#pragma unroll
+  for (int i = 0; i < COUNT; ++i)
+    out[i] = row_offset((wave * COUNT + i) * 16 + lane / 4) + (lane % 4 ^ lane / 8 % 4) * 16;
+}
+
 // Tile t of `down` x `across`, `group` rows of tiles at a time and down each
 // column of them, so that neighbouring tiles share operands on both sides.
 __device__ __forceinline__ void place_tile(int64_t t, int64_t down, int64_t across, int group,

@@ -14,6 +14,7 @@
 #include <algorithm>
 
 #include "cross_entropy.hpp"
+#include "mfma_product.hpp"
 
 namespace sporder_hip {
 
@@ -98,11 +99,10 @@ __device__ __forceinline__ RawTarget fetch_target(const CeCall &c, int64_t row) 
 
 // As a class, -1 where it counts nothing, -2 where it is no class, -3 past the rows.
 __device__ __forceinline__ int class_of(const CeCall &c, int64_t row, const RawTarget &raw) {
-  const int64_t t = c.target_bits == 64
-                        ? static_cast<int64_t>(static_cast<uint64_t>(static_cast<uint32_t>(raw.high)) << 32 |
-                                               static_cast<uint32_t>(raw.low))
-                        : raw.low;
-  const int k = t == c.ignore ? -1 : t >= 0 && t < c.classes ? static_cast<int>(t) : -2;
+  const int high = c.target_bits == 64 ? raw.high : raw.low >> 31;
+  const bool ignored = raw.low == static_cast<int>(c.ignore) && high == static_cast<int>(c.ignore >> 32);
+  const bool in = high == 0 && static_cast<uint32_t>(raw.low) < static_cast<uint32_t>(c.classes);
+  const int k = ignored ? -1 : in ? raw.low : -2;
   return row < c.rows ? k : -3;
 }
 
@@ -266,7 +266,7 @@ constexpr int kRows = 32, kSplit = 4; // waves that share a block of 16 rows
 // accumulators, 64 bytes of 16 rows at a time, it took a third of the kernel's time; stored at
 // the tile's end, the next tile's loads waited for it.)
 template <typename T, int VB, int DB>
-__global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 ? 4 : 2) few_grad_kernel(FewArgs a) {
+__global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB < 8 ? 4 : 2) few_grad_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   constexpr int kMine = (VB + kSplit - 1) / kSplit;
   constexpr int kG = VB * 16 + 4;  // floats of a row of g
@@ -400,6 +400,320 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 ? 4 : 2
   }
 }
 
+// ---- backward, a wave to itself: 16 rows a tile -------------------------------------------
+
+// Where w is small enough for LDS to hold besides it a tile for each of eight waves,
+// every wave takes tiles of its own and keeps a dw of its own, so that nothing waits at
+// barriers and one wave's loads and stores run beside another's products (rows of 128, 47
+// classes: with tiles shared by eight waves the products' 750 us and memory's 420 came one
+// after the other).  z and dx are products of 16-bit halves here, three for each (22 bits,
+// in units of x's and w's rows and w's columns, as in the tiled form), at a fifth of the
+// 32-bit products' time; dw, which sums over rows of any scale, stays with those.  Rows are
+// of whole accesses of four elements, and dx's at such addresses.
+__device__ __forceinline__ f32x4 mfma_halves(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void split_eight(const float (&v)[8], f16x8 &hi, f16x8 &lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const f16_t h = static_cast<f16_t>(v[e]);
+    hi[e] = h;
+    lo[e] = static_cast<f16_t>(v[e] - static_cast<float>(h));
+  }
+}
+
+template <int VB, int DB> struct WaveShape {
+  static constexpr int kV = VB * 16, kV32 = (VB + 1) / 2 * 32, kD = DB * 64;
+  static constexpr int kW = kD + 8, kT = kV32 + 8;   // halves of a row of w and of w^T
+  static constexpr int kX = kD + 4, kG = kV + 4;     // floats of a row of x and g
+  static constexpr int kWaves = kGradThreads / kWave;
+  static constexpr int kTile = 16 * (kX + kG) + 16;  // floats of a wave
+  static constexpr int kHalves = 2 * (kV * kW + kD * kT);
+  static constexpr int kFloats = kHalves / 2 + 2 * kV + kD + kWaves * kTile;
+  static constexpr int kJoin = kV * kX + kV;         // dw and db of the workgroup, over it all
+  static constexpr bool kFits = VB * DB <= 6 && VB < 6 && kFloats * 4 <= kLds && kJoin <= kFloats;
+};
+
+template <typename T, int VB, int DB>
+__global__ void __launch_bounds__(kGradThreads, 2) few_grad_wave_kernel(FewArgs a) {
+  extern __shared__ __attribute__((aligned(16))) float lds[];
+  using S = WaveShape<VB, DB>;
+  const CeCall &c = a.c;
+  const int dim = static_cast<int>(c.dim), dim16 = (dim + 15) / 16;
+  f16_t *const w = reinterpret_cast<f16_t *>(lds), *const wt = w + 2 * S::kV * S::kW; // hi, then lo
+  float *const w_unit = lds + S::kHalves / 2, *const bias = w_unit + S::kV, *const t_unit = bias + S::kV;
+  const int tid = threadIdx.x, lane = lane_id(), q = lane / 16, l = lane % 16;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  float *const x = t_unit + S::kD + wave * S::kTile, *const g = x + 16 * S::kX, *const x_unit = g + 16 * S::kG;
+
+  // w's rows in their units, 16 threads a row.
+  const int part = tid % 16 * 4;
+  for (int v = tid / 16; v < S::kV; v += kGradThreads / 16) {
+    const T *const row = static_cast<const T *>(c.w) + min(static_cast<int64_t>(v), c.classes - 1) * c.w_stride;
+    f32x4 f[DB];
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DB; ++k) {
+      f[k] = floats<T>(four<T>(row, k * 64 + part, dim), k * 64 + part, dim);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) most = fmaxf(most, fabsf(f[k][e]));
+    }
+    const float u = unit_of(group_max<16>(most)), scale = unit_inverse(u);
+    if (part == 0) w_unit[v] = u;
+#pragma unroll
+    for (int k = 0; k < DB; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float s = v < c.classes ? f[k][e] * scale : 0.0f;
+        const f16_t h = static_cast<f16_t>(s);
+        w[v * S::kW + k * 64 + part + e] = h;
+        w[(S::kV + v) * S::kW + k * 64 + part + e] = static_cast<f16_t>(s - static_cast<float>(h));
+      }
+    }
+  }
+  // w's columns in theirs: of 32 classes 16 (e / 4) + 4 q + e % 4 is a lane group's half e.
+  for (int j = tid; j < S::kD; j += kGradThreads) {
+    const T *const col = static_cast<const T *>(c.w) + min(j, dim - 1);
+    float most = 0.0f;
+    for (int v = 0; v < static_cast<int>(c.classes); ++v) most = fmaxf(most, fabsf(static_cast<float>(col[v * c.w_stride])));
+    const float u = unit_of(most), scale = unit_inverse(u);
+    t_unit[j] = u;
+    for (int i = 0; i < S::kV32; ++i) {
+      const int v = i / 32 * 32 + i % 8 / 4 * 16 + i % 32 / 8 * 4 + i % 4;
+      const float s = v < c.classes && j < dim ? static_cast<float>(col[v * c.w_stride]) * scale : 0.0f;
+      const f16_t h = static_cast<f16_t>(s);
+      wt[j * S::kT + i] = h;
+      wt[(S::kD + j) * S::kT + i] = static_cast<f16_t>(s - static_cast<float>(h));
+    }
+  }
+  for (int v = tid; v < S::kV; v += kGradThreads) {
+    float b = v < c.classes ? 0.0f : -INFINITY;
+    if (c.bias && v < c.classes) with_type(c.bias, c.bias_type, [&](auto *p) { b = static_cast<float>(p[v]); });
+    bias[v] = b;
+  }
+  __syncthreads();
+
+  f32x4 dw[VB][DB * 4] = {};
+  float db[VB] = {};
+  const int64_t step = gridDim.x * int64_t(S::kWaves * 16), first = (blockIdx.x * int64_t(S::kWaves) + wave) * 16;
+  // Rows on their way: 16 lanes a row, four at a time.
+  int target[4];
+  RawTarget next_target[4];
+  Words<T, 4> next[4][DB];
+  auto targets_from = [&](int64_t r) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) next_target[i] = fetch_target(c, r + i * 4 + q);
+  };
+  // A tile's rows from a base that the wave shares, in bytes: registers are short.
+  const uint32_t x_step = static_cast<uint32_t>(c.x_stride * sizeof(T));
+  const uint32_t dx_step = static_cast<uint32_t>(c.dx_stride * sizeof(T));
+  auto rows_from = [&](int64_t r) {
+    const char *const base = static_cast<const char *>(c.x) + min(r, c.rows - 1) * (c.x_stride * sizeof(T));
+    uint32_t mine = q * x_step;
+    asm volatile("" : "+v"(mine)); // as below
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      target[i] = class_of(c, r + i * 4 + q, next_target[i]);
+      const uint32_t row = target[i] >= 0 ? mine + i * 4 * x_step : 0;
+#pragma unroll
+      for (int k = 0; k < DB; ++k) {
+        const uint32_t col = static_cast<uint32_t>(min(k * 64 + l * 4, dim - 4) * sizeof(T));
+        next[i][k] = __builtin_bit_cast(Words<T, 4>, *reinterpret_cast<const LoosePack<T, 4> *>(base + (row + col)));
+      }
+    }
+  };
+  RawTarget next_class;
+  float next_lse, next_scale;
+  auto fetch_row = [&](int64_t r) {
+    next_class = fetch_target(c, r);
+    const int64_t in = min(r, c.rows - 1);
+    next_lse = c.given_lse[in];
+    next_scale = c.grad[in * c.grad_stride];
+  };
+  targets_from(first);
+  rows_from(first);
+  __builtin_amdgcn_sched_barrier(0); // loads in the loop's order, so that it waits for no later ones
+  targets_from(first + step);
+  fetch_row(first + l);
+
+  for (int64_t r0 = first; r0 < c.rows; r0 += step) {
+    wave_lds_order(); // the last tile's rows are out
+    const bool every = __all(min(min(target[0], target[1]), min(target[2], target[3])) >= 0);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float most = 0.0f;
+#pragma unroll
+      for (int k = 0; k < DB; ++k) {
+        const auto p = __builtin_bit_cast(Pack<T, 4>, next[i][k]);
+        f32x4 f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f[e] = static_cast<float>(p.v[e]);
+        if (k == DB - 1 && k * 64 + l * 4 >= dim) f = f32x4{};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (!every) f[e] = target[i] >= 0 ? f[e] : 0.0f;
+          most = fmaxf(most, fabsf(f[e]));
+        }
+        *reinterpret_cast<f32x4 *>(x + (i * 4 + q) * S::kX + k * 64 + l * 4) = f;
+      }
+      most = group_max<16>(most);
+      if (l == 0) x_unit[i * 4 + q] = unit_of(most);
+    }
+    wave_lds_order();
+    rows_from(r0 + step);
+    targets_from(r0 + 2 * step);
+    const int at = class_of(c, r0 + l, next_class);
+    const float lse = at >= 0 ? next_lse : 0.0f, scale = next_scale;
+    fetch_row(r0 + step + l);
+
+    // z, and g of them.
+    const float unit = x_unit[l], inverse = unit_inverse(unit);
+    f32x4 z[VB] = {};
+#pragma unroll
+    for (int k = 0; k < DB * 2; ++k) {
+      const f32x4 one = *reinterpret_cast<const f32x4 *>(x + l * S::kX + k * 32 + q * 8);
+      const f32x4 two = *reinterpret_cast<const f32x4 *>(x + l * S::kX + k * 32 + q * 8 + 4);
+      float v[8];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        v[e] = one[e] * inverse;
+        v[4 + e] = two[e] * inverse;
+      }
+      f16x8 hi, lo;
+      split_eight(v, hi, lo);
+      f16x8 wh[VB], wl[VB];
+#pragma unroll
+      for (int b = 0; b < VB; ++b) {
+        const f16_t *const from = w + (b * 16 + l) * S::kW + k * 32 + q * 8;
+        wh[b] = *reinterpret_cast<const f16x8 *>(from);
+        wl[b] = *reinterpret_cast<const f16x8 *>(from + S::kV * S::kW);
+      }
+#pragma unroll
+      for (int b = 0; b < VB; ++b) z[b] = mfma_halves(wl[b], hi, z[b]);
+#pragma unroll
+      for (int b = 0; b < VB; ++b) z[b] = mfma_halves(wh[b], lo, z[b]);
+#pragma unroll
+      for (int b = 0; b < VB; ++b) z[b] = mfma_halves(wh[b], hi, z[b]);
+    }
+    f16x8 gh[S::kV32 / 32], gl[S::kV32 / 32];
+#pragma unroll
+    for (int b = 0; b < VB; ++b) {
+      const int v = b * 16 + q * 4;
+      const f32x4 add = *reinterpret_cast<const f32x4 *>(bias + v), u = *reinterpret_cast<const f32x4 *>(w_unit + v);
+      f32x4 out;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float p = exp_of(z[b][e] * (unit * u[e]) + add[e] - lse) - (v + e == at ? 1.0f : 0.0f);
+        const float held = at >= 0 ? p : 0.0f, much = held * 8192.0f;
+        out[e] = at >= 0 ? held * scale : 0.0f;
+        const f16_t h = static_cast<f16_t>(much);
+        gh[b / 2][b % 2 * 4 + e] = h;
+        gl[b / 2][b % 2 * 4 + e] = static_cast<f16_t>(much - static_cast<float>(h));
+      }
+      *reinterpret_cast<f32x4 *>(g + l * S::kG + v) = out;
+    }
+    if constexpr (VB % 2 == 1) { // no classes there
+#pragma unroll
+      for (int e = 4; e < 8; ++e) gh[VB / 2][e] = gl[VB / 2][e] = static_cast<f16_t>(0.0f);
+    }
+
+    wave_lds_order();
+    // dw.
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      float gv[VB];
+#pragma unroll
+      for (int b = 0; b < VB; ++b) {
+        gv[b] = g[(q * 4 + e) * S::kG + b * 16 + l];
+        db[b] += gv[b];
+      }
+#pragma unroll
+      for (int j = 0; j < DB * 4; ++j) {
+        const float xv = x[(q * 4 + e) * S::kX + j * 16 + l];
+#pragma unroll
+        for (int b = 0; b < VB; ++b) dw[b][j] = mfma_16x16(gv[b], xv, dw[b][j]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // dx.
+    const float down = scale * (1.0f / 8192.0f);
+    const bool all_count = __all(at >= 0); // else rows of zeros, whatever w and the scale hold
+    constexpr int kSide = 2; // side by side: one after another would wait for its sum
+    f32x4 d[DB * 4] = {};
+#pragma unroll
+    for (int j0 = 0; j0 < DB * 4; j0 += kSide) {
+#pragma unroll
+      for (int b = 0; b < S::kV32 / 32; ++b) {
+        f16x8 th[kSide], tl[kSide];
+#pragma unroll
+        for (int j = 0; j < kSide; ++j) {
+          const f16_t *const from = wt + ((j0 + j) * 16 + l) * S::kT + b * 32 + q * 8;
+          th[j] = *reinterpret_cast<const f16x8 *>(from);
+          tl[j] = *reinterpret_cast<const f16x8 *>(from + S::kD * S::kT);
+        }
+#pragma unroll
+        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_halves(tl[j], gh[b], d[j0 + j]);
+#pragma unroll
+        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_halves(th[j], gl[b], d[j0 + j]);
+#pragma unroll
+        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_halves(th[j], gh[b], d[j0 + j]);
+        __builtin_amdgcn_sched_barrier(0); // the next ones' operands would not fit the registers
+      }
+    }
+    // dx in place of x, and out by whole rows.
+    wave_lds_order();
+#pragma unroll
+    for (int j = 0; j < DB * 4; ++j) {
+      const f32x4 u = *reinterpret_cast<const f32x4 *>(t_unit + j * 16 + q * 4);
+      d[j] = d[j] * u * down;
+      if (!all_count) d[j] = at >= 0 ? d[j] : f32x4{};
+      *reinterpret_cast<f32x4 *>(x + l * S::kX + j * 16 + q * 4) = d[j];
+    }
+    wave_lds_order();
+    char *const to = static_cast<char *>(c.dx) + r0 * (c.dx_stride * sizeof(T));
+    uint32_t place = q * dx_step + l * static_cast<uint32_t>(4 * sizeof(T));
+    asm volatile("" : "+v"(place)); // else eight places are made before the loop, as 64-bit addresses
+    const int left = static_cast<int>(min(c.rows - r0, int64_t(16)));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (i * 4 + q >= left) continue;
+#pragma unroll
+      for (int k = 0; k < DB; ++k) {
+        const f32x4 f = *reinterpret_cast<const f32x4 *>(x + (i * 4 + q) * S::kX + k * 64 + l * 4);
+        const float v[4] = {f[0], f[1], f[2], f[3]};
+        if (k < DB - 1 || k * 64 + l * 4 < dim)
+          store_f32<4>(reinterpret_cast<T *>(to + (place + i * 4 * dx_step)) + k * 64, v);
+      }
+    }
+  }
+
+  // The waves' sums, one after another.
+  float *const join = lds, *const join_db = lds + S::kV * S::kX;
+  for (int turn = 0; turn < S::kWaves; ++turn) {
+    __syncthreads();
+    if (wave != turn) continue;
+#pragma unroll
+    for (int b = 0; b < VB; ++b) {
+#pragma unroll
+      for (int j = 0; j < DB * 4; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          float &to = join[(b * 16 + q * 4 + e) * S::kX + j * 16 + l];
+          to = (turn ? to : 0.0f) + dw[b][j][e];
+        }
+      }
+      db[b] += lane_xor_f32(db[b], 16);
+      db[b] += lane_xor_f32(db[b], 32);
+      if (q == 0) join_db[b * 16 + l] = (turn ? join_db[b * 16 + l] : 0.0f) + db[b];
+    }
+  }
+  __syncthreads();
+  float *const out = a.dw_part + blockIdx.x * int64_t(S::kV) * (dim16 * 16);
+  for (int i = tid; i < S::kV * dim16 * 16; i += kGradThreads)
+    out[i] = join[i / (dim16 * 16) * S::kX + i % (dim16 * 16)];
+  if (tid < S::kV) a.db_part[blockIdx.x * int64_t(S::kV) + tid] = join_db[tid];
+}
+
 // The workgroups' sums of dw and db: 64 elements per workgroup, 16 threads each.
 __global__ void __launch_bounds__(1024)
     few_sum_kernel(FewArgs a, int64_t blocks, int64_t classes_pad, int64_t dim_pad) {
@@ -452,12 +766,35 @@ int64_t lds_of(int64_t dim, int64_t classes, bool backward) {
   return floats_of(dim, class_blocks(classes), backward) * 4 + 256;
 }
 
+template <typename F> int32_t with_blocks(int64_t dim, int64_t classes, F &&f);
+
+// The LDS of the backward pass that gives each wave tiles of its own, 0 where it doesn't fit.
+int64_t wave_lds(int64_t dim, int64_t classes) {
+  int64_t bytes = 0;
+  if (dim % 4 != 0) return bytes;
+  with_blocks(dim, classes, [&](auto vb, auto db) {
+    using S = WaveShape<decltype(vb)::value, decltype(db)::value>;
+    if constexpr (S::kFits) bytes = S::kFloats * 4;
+    return static_cast<int32_t>(SPORDER_OK);
+  });
+  return bytes;
+}
+
+// Whether a call takes that.
+template <typename T> bool by_waves(const CeCall &c) {
+  constexpr int64_t kFar = int64_t(1) << 24; // sixteen rows apart in 32 bits
+  return wave_lds(c.dim, c.classes) && (c.dx_stride % 4 == 0 || c.rows == 1) && aligned_to(c.dx, 4 * sizeof(T)) &&
+         c.x_stride < kFar && c.dx_stride < kFar;
+}
+bool by_waves(const CeCall &c) { return c.type == SPORDER_TYPE_F32 ? by_waves<float>(c) : by_waves<f16_t>(c); }
+
 // Workgroups: as many per CU as fit, up to two (sixteen waves) or three of the forward pass's.
 int64_t grid_of(int64_t rows, int64_t dim, int64_t classes, bool backward) {
   const int64_t fit = kLds / lds_of(dim, classes, backward);
   return std::min(ceil_div64(rows, backward ? kRows : 64), 256 * std::min<int64_t>(fit, backward ? 2 : 3));
 }
 
+// f with the class and feature blocks, as types.
 template <typename F> int32_t with_blocks(int64_t dim, int64_t classes, F &&f) {
   auto classes_of = [&](auto db) {
     constexpr int DB = decltype(db)::value;
@@ -516,7 +853,7 @@ struct FewLayout {
 };
 FewLayout few_layout(int64_t rows, int64_t dim, int64_t classes, bool backward) {
   FewLayout l{};
-  l.grid = grid_of(rows, dim, classes, backward);
+  l.grid = grid_of(rows, dim, classes, backward); // at least what either backward pass takes
   const int64_t pad = class_blocks(classes) * 16;
   size_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -544,6 +881,11 @@ template <typename T> int32_t few_loss(const FewArgs &a, int64_t grid, void *str
 template <typename T> int32_t few_grad(const FewArgs &a, int64_t grid, void *stream) {
   return with_blocks(a.c.dim, a.c.classes, [&](auto vb, auto db) {
     constexpr int VB = decltype(vb)::value, DB = decltype(db)::value;
+    using S = WaveShape<VB, DB>;
+    if constexpr (S::kFits) {
+      if (by_waves(a.c))
+        return launch_lds(few_grad_wave_kernel<T, VB, DB>, grid, kGradThreads, S::kFloats * 4, stream, a);
+    }
     return launch_lds(few_grad_kernel<T, VB, DB>, grid, kGradThreads, floats_of(a.c.dim, VB, true) * 4, stream, a);
   });
 }
@@ -573,14 +915,15 @@ int32_t few_forward(const CeCall &c, void *work, void *stream) {
 int32_t few_backward(const CeCall &c, void *work, void *stream) {
   const FewLayout l = few_layout(c.rows, c.dim, c.classes, true);
   char *const base = static_cast<char *>(work);
+  const int64_t grid = by_waves(c) ? std::min<int64_t>(ceil_div64(c.rows, 16 * 8), 256) : l.grid;
   FewArgs a{c, ceil_div64(c.rows, kRows), nullptr,
             reinterpret_cast<float *>(base + l.dw), reinterpret_cast<float *>(base + l.db)};
-  const int32_t rc = c.type == SPORDER_TYPE_BF16  ? few_grad<bf16_t>(a, l.grid, stream)
-                     : c.type == SPORDER_TYPE_F16 ? few_grad<f16_t>(a, l.grid, stream)
-                                                  : few_grad<float>(a, l.grid, stream);
+  const int32_t rc = c.type == SPORDER_TYPE_BF16  ? few_grad<bf16_t>(a, grid, stream)
+                     : c.type == SPORDER_TYPE_F16 ? few_grad<f16_t>(a, grid, stream)
+                                                  : few_grad<float>(a, grid, stream);
   if (rc != SPORDER_OK) return rc;
   const int64_t pad = class_blocks(c.classes) * 16, dim_pad = ceil_div64(c.dim, 16) * 16;
-  return launch(few_sum_kernel, dim3(ceil_div64(pad * dim_pad + pad, kWave)), dim3(1024), stream, a, l.grid, pad,
+  return launch(few_sum_kernel, dim3(ceil_div64(pad * dim_pad + pad, kWave)), dim3(1024), stream, a, grid, pad,
                 dim_pad);
 }
 

@@ -473,7 +473,12 @@ template <typename F> int32_t forward_lanes(int64_t dim, F &&f) {
 }
 
 template <typename F> int32_t backward_lanes(int64_t dim, F &&f) {
-  if (dim <= 512) return forward_lanes(dim, f);
+  if (dim <= 16) return f(Const<2>{}, Const<8>{});
+  if (dim <= 32) return f(Const<4>{}, Const<8>{});
+  if (dim <= 64) return f(Const<8>{}, Const<8>{});
+  if (dim <= 128) return f(Const<16>{}, Const<8>{});
+  if (dim <= 256) return f(Const<32>{}, Const<8>{});
+  if (dim <= 512) return f(Const<64>{}, Const<8>{});
   if (dim <= 1024) return f(Const<128>{}, Const<8>{});
   if (dim <= 2048) return f(Const<256>{}, Const<8>{});
   if (dim <= 4096) return f(Const<512>{}, Const<8>{});

@@ -242,7 +242,7 @@ __global__ void __launch_bounds__(256)
 // The largest element of each column of rows of x (listed) or w: a strip of rows and 64
 // accesses' columns per workgroup, then the strips'.  (One atomic maximum per strip and
 // column instead: 206 us for 50,000 rows of 2,048 16-bit elements.)
-constexpr int kStrips = 128;
+constexpr int kStrips = 1024; // at most
 template <typename T>
 __global__ void __launch_bounds__(256)
     ce_column_most_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
@@ -789,19 +789,22 @@ template <typename T> __global__ void __launch_bounds__(256) ce_zero_kernel(CeAr
   for (int64_t c = lane_id(); c < a.dim; c += kWave) out[c] = static_cast<T>(0.0f);
 }
 
-// db of a piece: 64 classes per workgroup, four threads each.
-__global__ void __launch_bounds__(256) ce_bias_kernel(CeArgs a, int64_t v0, int tile) {
-  __shared__ float part[4][kWave];
-  const int x = threadIdx.x % kWave, y = threadIdx.x / kWave;
-  const int64_t v = blockIdx.x * int64_t(kWave) + x;
+// db of a piece: 16 classes per workgroup, 64 threads each.
+__global__ void __launch_bounds__(1024) ce_bias_kernel(CeArgs a, int64_t v0, int tile) {
+  __shared__ float part[64][17];
+  const int x = threadIdx.x % 16, y = threadIdx.x / 16;
+  const int64_t v = blockIdx.x * int64_t(16) + x;
   const int64_t chunks = ceil_div64(a.meta->count, tile) * (tile / 64);
   float s = 0.0f;
-#pragma unroll 4
-  for (int64_t c = y; c < chunks; c += 4) s += a.db_part[c * a.piece + v];
+#pragma unroll 8
+  for (int64_t c = y; c < chunks; c += 64) s += a.db_part[c * a.piece + v];
   part[y][x] = s;
   __syncthreads();
-  if (y == 0 && v0 + v < a.classes && v < a.piece)
-    store_typed(a.db, a.bias_type, v0 + v, (part[0][x] + part[1][x]) + (part[2][x] + part[3][x]));
+  for (int k = 32; k > 0; k /= 2) {
+    if (y < k) part[y][x] += part[y + k][x];
+    __syncthreads();
+  }
+  if (y == 0 && v0 + v < a.classes) store_typed(a.db, a.bias_type, v0 + v, part[0][x]);
 }
 
 // ---- host --------------------------------------------------------------------------------
@@ -885,7 +888,7 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
   }
   a.classes_pad = ceil_div64(a.classes, a.piece) * a.piece;
   p.z = cut_logits(std::min(a.piece, a.classes), a.rows);
-  if (!backward && a.rows <= 64) p.z.shape = 0;
+  if (!backward && a.rows <= 64 && p.planes == 1) p.z.shape = 0;
   const int down = p.z.shape == 2 ? Large::kM : Middle::kM; // classes of a tile
   a.chunks = ceil_div64(a.classes, down) * (p.z.shape == 0 ? Narrow::WM : 2);
   size_t at = 0;
@@ -991,7 +994,12 @@ template <typename T, typename U, int PLANES> int32_t forward(const CeArgs &a, c
                   dim3(ceil_div64(a.classes, S::kM) * ceil_div64(a.rows, S::kN)), dim3(S::kThreads),
                   stream, a);
   };
-  steps([&] { return p.z.shape == 2 ? go(Large{}) : p.z.shape == 1 ? go(Middle{}) : go(Narrow{}); });
+  steps([&] {
+    if constexpr (PLANES == 1) {
+      if (p.z.shape == 0) return go(Narrow{});
+    }
+    return p.z.shape == 2 ? go(Large{}) : go(Middle{});
+  });
   steps([&] { return launch(ce_join_kernel, dim3(ceil_div64(a.rows, 16)), dim3(256), stream, a); });
   const int64_t blocks = std::min(ceil_div64(a.rows, kSumRows), kSumBlocks);
   const int64_t per = ceil_div64(a.rows, blocks);
@@ -1015,8 +1023,9 @@ template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, 
   steps([&] { return list_rows(a, true, stream); });
   steps([&] { return pack_operands<T, U, PLANES>(a, p, stream); });
   auto columns_most = [&](const T *src, int64_t stride, int64_t rows, const int32_t *list, float *most) {
-    const int64_t strips = std::min<int64_t>(ceil_div64(rows, 32), kStrips);
-    const int32_t rc = launch(ce_column_most_kernel<T>, dim3(ceil_div64(a.dim, kWave * (16 / sizeof(T))), strips),
+    const int64_t across = ceil_div64(a.dim, kWave * (16 / sizeof(T)));
+    const int64_t strips = std::min(ceil_div64(rows, 32), std::min<int64_t>(std::max<int64_t>(512 / across, 64), kStrips));
+    const int32_t rc = launch(ce_column_most_kernel<T>, dim3(across, strips),
                               dim3(256), stream, src, stride, rows, a.dim, a.meta, list, a.most_part);
     if (rc != SPORDER_OK) return rc;
     return launch(ce_strips_most_kernel, dim3(ceil_div64(a.dim, kWave)), dim3(256), stream, a.most_part, strips,
@@ -1044,7 +1053,7 @@ template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, 
     steps([&] { return p.z.shape == 2 ? tiles(Large{}) : tiles(Middle{}); });
     if (a.db)
       steps([&] {
-        return launch(ce_bias_kernel, dim3(a.piece / 64), dim3(256), stream, a, v0,
+        return launch(ce_bias_kernel, dim3(a.piece / 16), dim3(1024), stream, a, v0,
                       p.z.shape == 2 ? Large::kN : Middle::kN);
       });
     auto gradients = [&](auto shape, auto kind) {
@@ -1109,6 +1118,7 @@ size_t sporder_linear_cross_entropy_work_bytes(int32_t type, int64_t rows, int64
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
   if (bad_sizes(a, false) || rows == 0) return 0;
   if (few_takes(dim, classes, false)) return few_work_bytes(rows, dim, classes, false);
+  if (narrow_takes(type, rows, dim, false)) return narrow_work_bytes(rows, dim, classes, false);
   return lay_out(a, false, nullptr).bytes;
 }
 
@@ -1130,6 +1140,9 @@ int32_t sporder_linear_cross_entropy(void *stream, int32_t type, int64_t rows, i
   if (few_takes(dim, classes, false))
     return work_bytes < few_work_bytes(rows, dim, classes, false) ? SPORDER_BAD_ARGUMENT
                                                                    : few_forward(a, d_work, stream);
+  if (narrow_takes(type, rows, dim, false))
+    return work_bytes < narrow_work_bytes(rows, dim, classes, false) ? SPORDER_BAD_ARGUMENT
+                                                                      : narrow_run(a, false, d_work, stream);
   const CePlan p = lay_out(a, false, d_work);
   if (work_bytes < p.bytes) return SPORDER_BAD_ARGUMENT;
   if (type == SPORDER_TYPE_BF16) return forward<bf16_t, bf16_t, 1>(a, p, stream);
@@ -1147,6 +1160,7 @@ size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows, 
   a.db = &a; // the scratch of a bias whether there is one or not
   if (bad_sizes(a, true) || rows == 0) return 0;
   if (few_takes(dim, classes, true)) return few_work_bytes(rows, dim, classes, true);
+  if (narrow_takes(type, rows, dim, true)) return narrow_work_bytes(rows, dim, classes, true);
   return lay_out(a, true, nullptr).bytes;
 }
 
@@ -1181,6 +1195,9 @@ int32_t sporder_linear_cross_entropy_grad(void *stream, int32_t type, int64_t ro
   if (few_takes(dim, classes, true))
     return work_bytes < few_work_bytes(rows, dim, classes, true) ? SPORDER_BAD_ARGUMENT
                                                                   : few_backward(a, d_work, stream);
+  if (narrow_takes(type, rows, dim, true))
+    return work_bytes < narrow_work_bytes(rows, dim, classes, true) ? SPORDER_BAD_ARGUMENT
+                                                                     : narrow_run(a, true, d_work, stream);
   const CePlan p = lay_out(a, true, d_work);
   if (work_bytes < p.bytes) return SPORDER_BAD_ARGUMENT;
   if (type == SPORDER_TYPE_BF16) return backward<bf16_t, bf16_t, 1>(a, p, stream);

@@ -1,7 +1,8 @@
-// cross_entropy.hpp -- the two forms of the linear cross entropy: tiles of
-// 16-bit products over any number of classes (cross_entropy.hip), and one pass
-// over the rows where the classes' weights fit a workgroup's LDS
-// (cross_entropy_few.hip).
+// cross_entropy.hpp -- the three forms of the linear cross entropy: tiles of
+// 16-bit products over any number of classes (cross_entropy.hip), one pass over
+// the rows where the classes' weights fit a workgroup's LDS
+// (cross_entropy_few.hip), and 32-bit products straight from memory for a few rows
+// (cross_entropy_narrow.hip).
 #pragma once
 
 #include "dense.hpp"
@@ -53,10 +54,42 @@ __device__ __forceinline__ double block_sums(double s, double n, double (&part)[
   return (p[0] + p[1]) + (p[2] + p[3]);
 }
 
+using f32x4 = float __attribute__((ext_vector_type(4)));
+
+// Four elements of a row from `col` on, or its last four where it ends before (a row has
+// four at least).
+template <typename T> __device__ __forceinline__ Words<T, 4> four(const T *row, int col, int dim) {
+  return __builtin_bit_cast(Words<T, 4>, *reinterpret_cast<const LoosePack<T, 4> *>(row + min(col, dim - 4)));
+}
+
+// As floats, zeros past the row's end.
+template <typename T> __device__ __forceinline__ f32x4 floats(const Words<T, 4> &words, int col, int dim) {
+  const auto q = __builtin_bit_cast(Pack<T, 4>, words);
+  f32x4 v;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(q.v[e]);
+  if (dim % 4 != 0) { // move the row's last elements to their places
+    const int past = col + 4 - dim;
+    if (past > 0)
+      v = past == 1   ? f32x4{v[1], v[2], v[3], 0.0f}
+          : past == 2 ? f32x4{v[2], v[3], 0.0f, 0.0f}
+          : past == 3 ? f32x4{v[3], 0.0f, 0.0f, 0.0f}
+                      : f32x4{};
+  } else if (col >= dim) {
+    v = f32x4{};
+  }
+  return v;
+}
+
 // The one-pass form.
 bool few_takes(int64_t dim, int64_t classes, bool backward);
 size_t few_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward);
 int32_t few_forward(const CeCall &a, void *work, void *stream);
 int32_t few_backward(const CeCall &a, void *work, void *stream);
+
+// The form of few rows.
+bool narrow_takes(int type, int64_t rows, int64_t dim, bool backward);
+size_t narrow_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward);
+int32_t narrow_run(const CeCall &a, bool backward, void *work, void *stream);
 
 } // namespace sporder_hip

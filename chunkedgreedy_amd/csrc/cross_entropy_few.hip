@@ -20,8 +20,6 @@ namespace sporder_hip {
 
 namespace {
 
-using f32x4 = float __attribute__((ext_vector_type(4)));
-
 constexpr int kLossThreads = 256, kGradThreads = 512;
 constexpr int kLds = 160 * 1024;
 
@@ -35,31 +33,6 @@ struct FewArgs {
 
 __device__ __forceinline__ f32x4 mfma_16x16(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
-}
-
-// Four elements of a row from `col` on, or its last four where it ends before (a row has
-// four at least).
-template <typename T> __device__ __forceinline__ Words<T, 4> four(const T *row, int col, int dim) {
-  return __builtin_bit_cast(Words<T, 4>, *reinterpret_cast<const LoosePack<T, 4> *>(row + min(col, dim - 4)));
-}
-
-// As floats, zeros past the row's end.
-template <typename T> __device__ __forceinline__ f32x4 floats(const Words<T, 4> &words, int col, int dim) {
-  const auto q = __builtin_bit_cast(Pack<T, 4>, words);
-  f32x4 v;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) v[e] = static_cast<float>(q.v[e]);
-  if (dim % 4 != 0) { // move the row's last elements to their places
-    const int past = col + 4 - dim;
-    if (past > 0)
-      v = past == 1   ? f32x4{v[1], v[2], v[3], 0.0f}
-          : past == 2 ? f32x4{v[2], v[3], 0.0f, 0.0f}
-          : past == 3 ? f32x4{v[3], 0.0f, 0.0f, 0.0f}
-                      : f32x4{};
-  } else if (col >= dim) {
-    v = f32x4{};
-  }
-  return v;
 }
 
 // Floats of a row of x or w in LDS: whole blocks of 64 features, so that rows' places are

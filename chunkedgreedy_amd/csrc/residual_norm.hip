@@ -351,6 +351,128 @@ __global__ void __launch_bounds__(norm_block(L)) block_norm_grad_kernel(BlockGra
   }
 }
 
+// Rows whose column sums and weights would not fit the registers besides: 1,024 lanes of
+// 16 elements, tensor after tensor, the weights read for each row (L2 holds them) and
+// the column sums in LDS.
+constexpr int kWideLanes = 1024, kWideDim = kWideLanes * 16;
+template <typename T, bool LOOSE, int VEC>
+__global__ void __launch_bounds__(kWideLanes) block_norm_grad_wide_kernel(BlockGradArgs a) {
+  constexpr int L = kWideLanes, C = 16 / VEC;
+  __shared__ float shared[2][1][L / kWave];
+  __shared__ __attribute__((aligned(16))) float sums[2][kWideDim];
+  RowSum<L, 1> row_sum{shared};
+  const int lane = threadIdx.x;
+  const float dim = static_cast<float>(a.dim);
+#pragma unroll
+  for (int c = 0; c < C; ++c) {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) sums[0][(c * L + lane) * VEC + i] = sums[1][(c * L + lane) * VEC + i] = 0.0f;
+  }
+  auto add = [&](int which, const float (&v)[C][VEC], const float (&w)[C][VEC]) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) sums[which][(c * L + lane) * VEC + i] += v[c][i] * w[c][i];
+    }
+  };
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float r1 = a.post_rstd[row], r2 = a.rstd[row];
+    int place = lane;
+    asm volatile("" : "+v"(place)); // else the weights' addresses fill the registers before the loop
+    Words<T, VEC> raw[C], raw_two[C];
+    float b[C][VEC], u[C][VEC], w[C][VEC];
+    fetch_row<LOOSE, VEC, L>(a.y, row, a.y_stride, a.dim, true, lane, raw);
+    fetch_row<LOOSE, VEC, L>(a.dh, row, a.dh_stride, a.dim, true, lane, raw_two);
+    load_vector<LOOSE, VEC, L>(a.w2, a.vector_type, a.dim, 1.0f, place, w);
+    to_floats<VEC>(raw, u);
+    to_floats<VEC>(raw_two, b);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        u[c][i] *= (c * L + lane) * VEC + (LOOSE ? i : 0) < a.dim ? r2 : 0.0f;
+    }
+    add(1, b, u);
+    float s[1] = {0.0f};
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        b[c][i] *= w[c][i];
+        s[0] += b[c][i] * u[c][i];
+      }
+    }
+    fetch_row<LOOSE, VEC, L>(a.dy, row, a.dy_stride, a.dim, true, lane, raw);
+    fetch_row<LOOSE, VEC, L>(a.x, row, a.x_stride, a.dim, true, lane, raw_two);
+    row_sum(s);
+    const float m1 = s[0] / dim;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) b[c][i] = (b[c][i] - u[c][i] * m1) * r2;
+    }
+    to_floats<VEC>(raw, u);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) b[c][i] += u[c][i];
+    }
+    put_row<LOOSE, VEC, L>(static_cast<T *>(a.dres) + row * a.dres_stride, a.dim, lane, b);
+    fetch_row<LOOSE, VEC, L>(a.gate, row, a.gate_stride, a.dim, true, lane, raw);
+    load_gain<LOOSE, VEC, L>(a, place, w);
+    to_floats<VEC>(raw_two, u);
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i)
+        u[c][i] *= (c * L + lane) * VEC + (LOOSE ? i : 0) < a.dim ? r1 : 0.0f;
+    }
+    if (a.gate) {
+      T *const dgate = static_cast<T *>(a.dgate) + row * a.dgate_stride;
+#pragma unroll
+      for (int c = 0; c < C; ++c) {
+        const int col = (c * L + lane) * VEC;
+        const auto gate = __builtin_bit_cast(Pack<T, VEC>, raw[c]);
+        float g[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          g[i] = b[c][i] * w[c][i] * u[c][i];
+          b[c][i] *= static_cast<float>(gate.v[i]);
+        }
+        if (col < a.dim) put<LOOSE, VEC>(dgate + col, a.dim - col, g);
+      }
+    }
+    add(0, b, u);
+    s[0] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) {
+        b[c][i] *= w[c][i];
+        s[0] += b[c][i] * u[c][i];
+      }
+    }
+    float m2 = 0.0f;
+    if (a.post) {
+      row_sum(s);
+      m2 = s[0] / dim;
+    }
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) b[c][i] = (b[c][i] - u[c][i] * m2) * r1;
+    }
+    put_row<LOOSE, VEC, L>(static_cast<T *>(a.dx) + row * a.dx_stride, a.dim, lane, b);
+  }
+  if (!a.partial) return;
+  float *const out = a.partial + static_cast<int64_t>(blockIdx.x) * 2 * a.dim;
+  __syncthreads();
+  for (int64_t i = lane; i < a.dim; i += L) {
+    out[i] = sums[0][i];
+    out[a.dim + i] = sums[1][i];
+  }
+}
+
 // Rows that no workgroup's registers hold: three passes over each, by elements;
 // the column sums stay in the workgroup's partial row.
 template <typename T>
@@ -515,14 +637,16 @@ template <typename T> int32_t block_typed(const BlockArgs &a, void *stream) {
 }
 
 template <typename T> int32_t block_grad_typed(const BlockGradArgs &a, int64_t blocks, void *stream) {
-  if (a.dim > kBlockGradMostDim)
-    return launch(block_norm_grad_long_kernel<T>, dim3(blocks), dim3(1024), stream, a);
+  if (a.dim > kWideDim) return launch(block_norm_grad_long_kernel<T>, dim3(blocks), dim3(1024), stream, a);
   constexpr int kVec = 16 / sizeof(T);
   const bool whole = row_vec(sizeof(T), a.dim,
                              {a.dy_stride, a.dh_stride, a.x_stride, a.y_stride, a.gate_stride, a.dx_stride,
                               a.dres_stride, a.dgate_stride},
                              {a.dy, a.dh, a.x, a.y, a.gate, a.gate_vector, a.w1, a.w2, a.dx, a.dres,
                               a.dgate}) == kVec;
+  if (a.dim > kBlockGradMostDim)
+    return whole ? launch(block_norm_grad_wide_kernel<T, false, kVec>, dim3(blocks), dim3(kWideLanes), stream, a)
+                 : launch(block_norm_grad_wide_kernel<T, true, kVec>, dim3(blocks), dim3(kWideLanes), stream, a);
   return backward_lanes(a.dim, [&](auto lanes, auto elements) {
     constexpr int L = decltype(lanes)::value, E = decltype(elements)::value;
     return whole ? launch(block_norm_grad_kernel<T, false, kVec, L, E / kVec>, dim3(blocks),

@@ -833,10 +833,10 @@ bool direct_rows(int type, int64_t dim, int64_t stride, const void *p, int64_t s
          span_rows * stride * 2 < (int64_t(1) << 32);
 }
 
-// A large tile (256 x 256, one to a CU) does 1.3 times the products in its time that the
-// four middle ones of its place (two to a CU) do: 8,192 x 50,000 x 2,048 1.09 and 0.83 PFLOP/s,
-// short sums nearer.
-constexpr double kMiddleTime = 0.65; // of a middle tile, two at a time, beside a large one's
+// A large tile (256 x 256, one to a CU) does four times a middle one's products, and of those
+// two run on a CU: 8,192 x 50,000 with sums of 2,048 terms take 1.09 PFLOP/s in large tiles
+// and 0.985 in middle ones, half the time of a large tile times their ratio.
+constexpr double kMiddleTime = 0.55; // of a middle tile, two at a time, beside a large one's
 
 Cut cut_logits(int64_t classes, int64_t rows) {
   const double large = static_cast<double>(ceil_div64(ceil_div64(classes, 256) * ceil_div64(rows, 256), 256));
@@ -1024,7 +1024,7 @@ template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, 
   steps([&] { return pack_operands<T, U, PLANES>(a, p, stream); });
   auto columns_most = [&](const T *src, int64_t stride, int64_t rows, const int32_t *list, float *most) {
     const int64_t across = ceil_div64(a.dim, kWave * (16 / sizeof(T)));
-    const int64_t strips = std::min(ceil_div64(rows, 32), std::min<int64_t>(std::max<int64_t>(512 / across, 64), kStrips));
+    const int64_t strips = std::min(ceil_div64(rows, 32), std::min<int64_t>(std::max<int64_t>(1024 / across, 64), kStrips));
     const int32_t rc = launch(ce_column_most_kernel<T>, dim3(across, strips),
                               dim3(256), stream, src, stride, rows, a.dim, a.meta, list, a.most_part);
     if (rc != SPORDER_OK) return rc;

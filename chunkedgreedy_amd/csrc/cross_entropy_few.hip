@@ -130,7 +130,6 @@ __device__ __forceinline__ void logits(const float *w, const float *rows, int di
                                        f32x4 (&z)[BLOCKS]) {
   constexpr int stride = few_stride(DB);
   const int lane = lane_id(), at = lane % 16 * stride + lane / 16 * 4;
-#pragma unroll 2
   for (int k = 0; k < dim16; ++k) {
     const f32x4 b = *reinterpret_cast<const f32x4 *>(rows + at + k * 16);
 #pragma unroll

@@ -25,7 +25,7 @@ With --fused-scaling the operator is one call of
 SpMM: the same values bit for bit, without the two elementwise passes); the
 default keeps the reference driver's three steps.
 
-Three more options train a richer model with this library's training operators
+More options train a richer model with this library's training operators
 (``chunkedgreedy_amd.nn``), which the reference driver has none of; without
 them the model and its results are the reference's:
 
@@ -35,6 +35,14 @@ them the model and its results are the reference's:
   --layer-norm  a layer norm on the hidden layer, before its relu
   --muon        the two weight matrices are updated along their orthogonalised
                 momentum; biases, norm and table stay with Adam
+  --blocks N    N more graph convolutions of the hidden width, each added to a
+                residual stream, with root mean square norms after it and before
+                the next (nn.residual_norm)
+  --dropout P   dropout behind the hidden layer and behind each block's
+                convolution, from a counter; it follows the rows, so that
+                orderings train with different masks
+  --fused-loss  the last product and its cross entropy in one, without the
+                logits in memory (nn.linear_cross_entropy)
 
 Usage:  python -m chunkedgreedy_amd.e2e_gcn [--nodes N] [--epochs E] ...
 prints one JSON record per ordering (ORIGIN and sporder-csg by default;
@@ -109,12 +117,15 @@ def _spmm_fn():
 
 def train(ptr, ind, X, y, *, hidden: int, classes: int, epochs: int, warmup: int = 3,
           seed: int = 0, ctx=None, fused: bool = False, tokens=None, norm: bool = False,
-          muon: bool = False) -> dict:
+          muon: bool = False, blocks: int = 0, dropout: float = 0.0,
+          fused_loss: bool = False) -> dict:
     """Train the 2-layer GCN for `epochs` timed epochs after `warmup` untimed
     ones; returns per-epoch times, SpMM time per epoch and the losses.  With
     `tokens` (a node id per row) X is the start of a learned table of node
     vectors; `norm` puts a layer norm on the hidden layer; `muon` updates the
-    weight matrices along their orthogonalised momentum."""
+    weight matrices along their orthogonalised momentum; `blocks` graph
+    convolutions with residual norms follow the hidden layer; `dropout` is the
+    probability of both kinds; `fused_loss` keeps no logits."""
     import torch
     import torch.nn.functional as F
 
@@ -128,6 +139,13 @@ def train(ptr, ind, X, y, *, hidden: int, classes: int, epochs: int, warmup: int
     W1 = torch.nn.Linear(X.shape[1], hidden).to(X.device)
     W2 = torch.nn.Linear(hidden, classes).to(X.device)
     params = list(W1.parameters()) + list(W2.parameters())
+    layers = []
+    for _ in range(blocks):
+        linear = torch.nn.Linear(hidden, hidden).to(X.device)
+        norms = [torch.nn.Parameter(torch.ones(hidden, device=X.device)) for _ in range(2)]
+        layers.append((linear, *norms))
+        params += list(linear.parameters()) + norms
+    drops = [nn.Dropout(dropout, seed + k).to(X.device) for k in range(blocks + 1)]
     opts = []
     if muon:
         opts.append(nn.Muon([p for p in params if p.dim() == 2]))
@@ -148,8 +166,20 @@ def train(ptr, ind, X, y, *, hidden: int, classes: int, epochs: int, warmup: int
         h1 = SpMMFn.apply(W1(h0), op)
         if norm:
             h1 = nn.layer_norm(h1, scale, shift)
-        z = W2(SpMMFn.apply(F.relu(h1), op))
-        loss = -F.log_softmax(z, 1).gather(1, y[:, None]).mean()
+        h1 = F.relu(h1)
+        if dropout:
+            h1 = drops[0](h1)
+        stream = h1
+        for (linear, post, pre), drop in zip(layers, drops[1:]):
+            out = SpMMFn.apply(linear(h1), op)
+            if dropout:
+                out = drop(out)
+            stream, h1 = nn.residual_norm(out, stream, post_weight=post, weight=pre)
+        h2 = SpMMFn.apply(h1, op)
+        if fused_loss:
+            loss = nn.linear_cross_entropy(h2, W2.weight, y, W2.bias)
+        else:
+            loss = -F.log_softmax(W2(h2), 1).gather(1, y[:, None]).mean()
         loss.backward()
         for opt in opts:
             opt.step()
@@ -183,7 +213,8 @@ def permute_graph(ptr, ind, X, y, order, ctx=None):
 
 def run(ptr_h, ind_h, *, features: int, hidden: int, classes: int, epochs: int,
         orders=("ORIGIN", "sporder-csg"), seed: int = 0, fused: bool = False,
-        embed: bool = False, norm: bool = False, muon: bool = False) -> list[dict]:
+        embed: bool = False, norm: bool = False, muon: bool = False, blocks: int = 0,
+        dropout: float = 0.0, fused_loss: bool = False) -> list[dict]:
     import torch
 
     from chunkedgreedy_amd import sporder
@@ -219,10 +250,12 @@ def run(ptr_h, ind_h, *, features: int, hidden: int, classes: int, epochs: int,
             perm_ms = _sync_ms(torch, t0)
         r = train(ptr_u, ind_u, X0 if embed else X, y, hidden=hidden, classes=classes,
                   epochs=epochs, seed=seed, ctx=ctx, fused=fused,
-                  tokens=order if embed else None, norm=norm, muon=muon)
+                  tokens=order if embed else None, norm=norm, muon=muon, blocks=blocks,
+                  dropout=dropout, fused_loss=fused_loss)
         total = reorder_ms + perm_ms + r["prep_ms"] + epochs * r["epoch_ms"]
-        extras = {k: True for k, on in (("embed", embed), ("layer_norm", norm), ("muon", muon))
-                  if on}
+        extras = {k: on for k, on in (("embed", embed), ("layer_norm", norm), ("muon", muon),
+                                      ("blocks", blocks), ("dropout", dropout),
+                                      ("fused_loss", fused_loss)) if on}
         rows.append({"order": name, "fused_scaling": fused, **extras, "n": n,
                      "nnz": int(ind_h.shape[0]),
                      "features": features,
@@ -267,6 +300,11 @@ def main(argv=None) -> int:
     ap.add_argument("--layer-norm", action="store_true", help="a layer norm on the hidden layer")
     ap.add_argument("--muon", action="store_true",
                     help="update the weight matrices along their orthogonalised momentum")
+    ap.add_argument("--blocks", type=int, default=0,
+                    help="graph convolutions with residual norms behind the hidden layer")
+    ap.add_argument("--dropout", type=float, default=0.0, help="probability of dropout")
+    ap.add_argument("--fused-loss", action="store_true",
+                    help="the last product and its cross entropy without the logits in memory")
     args = ap.parse_args(argv)
 
     import torch
@@ -286,7 +324,8 @@ def main(argv=None) -> int:
                    classes=args.classes, epochs=args.epochs,
                    orders=tuple(args.orders.split(",")), seed=args.seed,
                    fused=args.fused_scaling, embed=args.embed, norm=args.layer_norm,
-                   muon=args.muon):
+                   muon=args.muon, blocks=args.blocks, dropout=args.dropout,
+                   fused_loss=args.fused_loss):
         print(json.dumps(row), flush=True)
     return 0
 

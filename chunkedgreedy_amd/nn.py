@@ -94,7 +94,10 @@ def dropout(x, p, seed, *, offset=0, residual=None, training=True):
 
 class Dropout(torch.nn.Module):
     """Dropout with its own seed and a count of its calls, held on the GPU so that
-    each replay of a captured step drops other elements."""
+    each replay of a captured step drops other elements.  Modules of one model
+    have different seeds, or they drop the same elements.  A part that is run again
+    for its gradients needs ``dropout`` with an offset of its own instead: its
+    second run would count on."""
 
     def __init__(self, p=0.5, seed=0):
         super().__init__()

@@ -606,7 +606,8 @@ def linear_cross_entropy(x, weight, targets, bias=None, *, ignore_index=-100):
     Returns (loss, lse, sums): loss and lse float32 of the targets' shape (NaN
     for a target that is neither a class nor ignored), sums float32 (2,) of the
     losses' sum and the number of rows that are not ignored.  At most 2^23 - 256
-    rows, 2^25 classes and 65536 elements a row.
+    rows (more with up to 64 classes of 4 to 256 elements, or 192 of 4 to 64),
+    2^25 classes, 2^37 logits and 65536 elements a row.
 
     Sums are held in 32 bits.  float32 products have operands of 22 bits: a term
     is within 2^-21 of itself, and within some 2^-38 of the product of its rows'
@@ -642,11 +643,10 @@ def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignor
     Returns (dx, dweight, dbias), dbias None without a bias.  The logits are
     made again, a piece of the classes at a time; rows that are ignored, or
     whose target is no class, have no gradient.  g = grad (exp(z - lse) -
-    [target]) is rounded to x's type before its products with weight and x
-    (22 bits for float32), whose sums are held in 32 bits.  The same call gives
-    the same bits from run to run.
+    [target]) keeps 11 bits or more in its products with weight and x (22 for
+    float32), whose sums are held in 32 bits.  The same call gives the same bits
+    from run to run.
     """
-    x_shape = x.shape
     x, x_stride, weight, weight_stride, targets, bias = _loss_inputs(x, weight, targets, bias)
     ignore_index = _ignored(ignore_index)
     rows, (classes, dim) = targets.numel(), weight.shape
@@ -666,7 +666,7 @@ def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignor
     one = grad.numel() == 1 or all(s == 0 for s in grad.stride())
     if not one and not grad.is_contiguous():
         grad = grad.contiguous()
-    dx = x.new_empty(x_shape)
+    dx = x.new_empty((*targets.shape, dim))
     dweight = weight.new_empty(weight.shape, dtype=dtype)
     dbias = None if bias is None else torch.empty_like(bias)
     sizes = (x_stride, x.data_ptr(), weight_stride, weight.data_ptr())

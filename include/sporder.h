@@ -580,9 +580,10 @@ SPORDER_API int32_t sporder_residual_norm_grad(
  * targets of target_bits (32 or 64, signed).  A row whose target is ignore_index has loss
  * and lse 0 and is not read; one whose target is no class otherwise has NaN.  d_sums
  * receives the sum of the losses and the number of rows whose target is not ignore_index.
- * dim is at most 65536, classes 2^25, rows 2^23 - 256, rows times classes 2^37.  d_work is
- * 256-byte aligned and of the size that *_work_bytes gives for the same sizes, strides
- * and alignments.
+ * dim is at most 65536, classes 2^25, rows 2^23 - 256 and rows times classes 2^37; up to
+ * 64 classes of 4 to 256 features, or 192 of 4 to 64, rows are at most 2^37.  d_work is
+ * 256-byte aligned and of the size that *_work_bytes gives for the same sizes, strides and
+ * alignments.
  */
 SPORDER_API size_t sporder_linear_cross_entropy_work_bytes(int32_t type, int64_t rows,
                                                            int64_t dim, int64_t classes,
@@ -600,7 +601,8 @@ SPORDER_API int32_t sporder_linear_cross_entropy(
  * target is a class and 0 for the others: d_dx = g w (of `type`), d_dweight = g^T x (of
  * dweight_type: `type` or SPORDER_TYPE_F32) and, where not NULL, d_dbias = sum_t g (of
  * bias_type).  d_grad has elements grad_stride apart (0: one for all rows); d_lse is the
- * forward call's.  g is rounded to `type` before the products of 16-bit types.
+ * forward call's.  Operands of these products keep 11 bits for 16-bit types (g too) and 22
+ * for 32-bit ones; sums are held in 32 bits.
  */
 SPORDER_API size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows,
                                                                 int64_t dim, int64_t classes,

@@ -72,9 +72,8 @@ struct CeArgs : CeCall {
 
 // ---- the list of rows, and what else comes first -----------------------------------
 
-__global__ void __launch_bounds__(256) ce_prepare_kernel(CeArgs a) {
-  const int64_t i = blockIdx.x * int64_t(256) + threadIdx.x;
-  if (i == 0) *a.meta = {0, -1000};
+__device__ __forceinline__ void prepare(const CeArgs &a, int64_t block) {
+  const int64_t i = block * 256 + threadIdx.x;
   if (i < a.classes_pad) {
     float b = -INFINITY;
     if (i < a.classes) {
@@ -84,6 +83,11 @@ __global__ void __launch_bounds__(256) ce_prepare_kernel(CeArgs a) {
     a.bias32[i] = b;
   }
   if (a.w_unit && i >= a.classes && i < a.classes_pad) a.w_unit[i] = 1.0f;
+}
+
+__global__ void __launch_bounds__(256) ce_prepare_kernel(CeArgs a) {
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.meta = {0, -1000};
+  prepare(a, blockIdx.x);
 }
 
 __global__ void __launch_bounds__(256) ce_count_kernel(CeArgs a) {
@@ -114,15 +118,16 @@ __device__ __forceinline__ int wave_total(int v) {
 }
 
 // The rows' places in the list: those counted before the block, then before the
-// thread in it.
-__global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward) {
+// thread in it.  Workgroups past the list's `blocks` prepare.
+__global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, int blocks) {
   __shared__ int32_t part[4], placed[kListBlock / 256][4], most;
+  if (blockIdx.x >= blocks) return prepare(a, blockIdx.x - blocks);
   const int tid = threadIdx.x, wave = tid / kWave, lane = lane_id();
   const int64_t first = blockIdx.x * int64_t(kListBlock);
   if (tid == 0) most = -1000;
   int before = 0;
   if (a.rows <= kListDirect) {
-#pragma unroll 4
+#pragma unroll 16
     for (int64_t row = tid; row < first; row += 256)
       before += counted(a, target_of(a, row)) ? 1 : 0;
   } else {
@@ -175,8 +180,13 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward) {
   }
   if (backward) atomicMax(&most, top);
   __syncthreads();
-  if (backward && tid == 0) atomicMax(&a.meta->most, most);
-  if (blockIdx.x != gridDim.x - 1) return;
+  if (backward && tid == 0) {
+    if (blocks == 1)
+      a.meta->most = most;
+    else
+      atomicMax(&a.meta->most, most);
+  }
+  if (blockIdx.x != blocks - 1) return;
   if (tid == 0) a.meta->count = before;
   // What the last tile reads past the list.
   const int64_t at = before + tid;
@@ -198,15 +208,32 @@ template <typename U> __device__ __forceinline__ void split(float v, U &hi, U &l
   lo = static_cast<U>(v - static_cast<float>(hi));
 }
 
-// Rows of x (listed) or w, zeros up to a multiple of 64 elements: a wave per row,
-// 8 elements a lane.
+// Rows of x (listed) or of w, which one launch packs: a launch costs some 4 us of a small
+// call (64 rows of 276 over 243 classes, gradients: 67 us with a launch each).
+struct CeRows {
+  const void *src;
+  int64_t stride, rows;
+  const int32_t *list; // of x
+  char *out;
+  int64_t out_stride, plane; // bytes
+  float *unit;               // of rows (32-bit types)
+  float *most;               // of columns
+  int64_t blocks;            // workgroups that take these rows
+};
+
+// Zeros up to a multiple of 64 elements: a wave per row, 8 elements a lane.
 template <typename T, typename U, int PLANES>
 __global__ void __launch_bounds__(256)
-    ce_pack_rows_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
-                        const int32_t *list, char *out, int64_t out_stride, int64_t plane, float *unit) {
-  const int64_t row = blockIdx.x * int64_t(4) + threadIdx.x / kWave;
-  if (row >= (list ? meta->count : rows)) return;
-  const T *const from = src + (list ? list[row] : row) * stride;
+    ce_pack_rows_kernel(CeRows x, CeRows w, int64_t dim, const CeMeta *meta) {
+  const bool first = blockIdx.x < x.blocks;
+  const CeRows &a = first ? x : w;
+  const int64_t row = (blockIdx.x - (first ? 0 : x.blocks)) * int64_t(4) + threadIdx.x / kWave;
+  const int32_t *const list = a.list;
+  if (row >= (list ? meta->count : a.rows)) return;
+  const T *const from = static_cast<const T *>(a.src) + (list ? list[row] : row) * a.stride;
+  const int64_t out_stride = a.out_stride, plane = a.plane;
+  char *const out = a.out;
+  float *const unit = a.unit;
   const int lane = lane_id();
   float scale = 1.0f;
   if constexpr (PLANES == 2) {
@@ -241,20 +268,39 @@ __global__ void __launch_bounds__(256)
 
 // The largest element of each column of rows of x (listed) or w: a strip of rows and 64
 // accesses' columns per workgroup, then the strips'.  (One atomic maximum per strip and
-// column instead: 206 us for 50,000 rows of 2,048 16-bit elements.)
+// column instead: 206 us for 50,000 rows of 2,048 16-bit elements.)  Workgroups past both
+// write zeros to dx where rows are not listed, 64 rows a wave.
 constexpr int kStrips = 1024; // at most
 template <typename T>
 __global__ void __launch_bounds__(256)
-    ce_column_most_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
-                          const int32_t *list, float *most) {
+    ce_column_most_kernel(CeRows ax, CeRows aw, CeArgs c, float *most) {
   constexpr int kVec = 16 / sizeof(T), kAhead = 8;
   __shared__ float part[4][kVec][kWave];
-  const int64_t all = list ? meta->count : rows;
+  const bool first = blockIdx.y < ax.blocks;
+  const CeRows &a = first ? ax : aw;
+  const T *const src = static_cast<const T *>(a.src);
+  const int32_t *const list = a.list;
+  const int64_t all = list ? c.meta->count : a.rows, stride = a.stride, dim = c.dim;
   const int x = threadIdx.x % kWave, y = threadIdx.x / kWave;
-  const int64_t col = (blockIdx.x * int64_t(kWave) + x) * kVec, step = gridDim.y * int64_t(4);
+  if (blockIdx.y >= ax.blocks + aw.blocks) {
+    const int64_t before = ax.blocks + aw.blocks;
+    for (int64_t r0 = ((blockIdx.y - before) * 4 + y) * kWave; r0 < c.rows; r0 += (gridDim.y - before) * 4 * kWave) {
+      uint64_t rest = __ballot(r0 + x < c.rows && !counted(c, target_of(c, min(r0 + x, c.rows - 1))));
+      for (; rest; rest &= rest - 1) {
+        T *const out = static_cast<T *>(c.dx) + (r0 + __builtin_ctzll(rest)) * c.dx_stride;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          const int64_t col = (blockIdx.x * int64_t(kVec) + k) * kWave + x;
+          if (col < dim) out[col] = static_cast<T>(0.0f);
+        }
+      }
+    }
+    return;
+  }
+  const int64_t col = (blockIdx.x * int64_t(kWave) + x) * kVec, step = a.blocks * 4;
   float m[kVec] = {};
   if (col < dim) {
-    for (int64_t r0 = blockIdx.y * int64_t(4) + y; r0 < all; r0 += step * kAhead) {
+    for (int64_t r0 = (blockIdx.y - (first ? 0 : ax.blocks)) * 4 + y; r0 < all; r0 += step * kAhead) {
       Pack<T, kVec> q[kAhead];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) { // past the rows the first again
@@ -281,8 +327,11 @@ __global__ void __launch_bounds__(256)
 
 // The strips' largest: 64 columns per workgroup, four threads each.
 __global__ void __launch_bounds__(256)
-    ce_strips_most_kernel(const float *parts, int64_t strips, int64_t dim, float *most) {
+    ce_strips_most_kernel(const float *parts, CeRows ax, CeRows aw, int64_t dim) {
   __shared__ float part[4][kWave];
+  const int64_t strips = blockIdx.y ? aw.blocks : ax.blocks;
+  float *const most = blockIdx.y ? aw.most : ax.most;
+  if (blockIdx.y) parts += ax.blocks * dim;
   const int x = threadIdx.x % kWave, y = threadIdx.x / kWave;
   const int64_t col = blockIdx.x * int64_t(kWave) + x;
   float m = 0.0f;
@@ -300,12 +349,17 @@ __global__ void __launch_bounds__(256)
 // turned in LDS.  Listed rows come with 2^(their exponent - the largest).
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
-    ce_pack_columns_kernel(const T *src, int64_t stride, int64_t rows, int64_t dim, const CeMeta *meta,
-                           const int32_t *list, const int32_t *exponent, const float *most, char *out,
-                           int64_t out_stride, int64_t plane) {
+    ce_pack_columns_kernel(CeRows ax, CeRows aw, int64_t dim, const CeMeta *meta, const int32_t *exponent) {
   __shared__ float tile[64][65];
-  const int64_t all = list ? meta->count : rows;
-  const int64_t k0 = blockIdx.x * int64_t(64), j0 = blockIdx.y * int64_t(64);
+  const bool first = blockIdx.x < ax.blocks;
+  const CeRows &a = first ? ax : aw;
+  const int32_t *const list = a.list;
+  const T *const src = static_cast<const T *>(a.src);
+  const float *const most = a.most;
+  char *const out = a.out;
+  const int64_t stride = a.stride, out_stride = a.out_stride, plane = a.plane;
+  const int64_t all = list ? meta->count : a.rows;
+  const int64_t k0 = (blockIdx.x - (first ? 0 : ax.blocks)) * int64_t(64), j0 = blockIdx.y * int64_t(64);
   if (k0 >= all) return;
   constexpr int kVec = 16 / sizeof(T), kAcross = 64 / kVec, kRound = 256 / kAcross, kRounds = 64 / kRound;
   const int x = threadIdx.x % kAcross * kVec, y = threadIdx.x / kAcross;
@@ -781,14 +835,6 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(CeArgs a, int64_t v0, in
   put_four(out + (DX ? a.list[n] : v0 + n) * stride, m, a.dim, whole, v);
 }
 
-// dx of the rows that are not listed.
-template <typename T> __global__ void __launch_bounds__(256) ce_zero_kernel(CeArgs a) {
-  const int64_t row = blockIdx.x * int64_t(4) + threadIdx.x / kWave;
-  if (row >= a.rows || counted(a, target_of(a, row))) return;
-  T *const out = static_cast<T *>(a.dx) + row * a.dx_stride;
-  for (int64_t c = lane_id(); c < a.dim; c += kWave) out[c] = static_cast<T>(0.0f);
-}
-
 // db of a piece: 16 classes per workgroup, 64 threads each.
 __global__ void __launch_bounds__(1024) ce_bias_kernel(CeArgs a, int64_t v0, int tile) {
   __shared__ float part[64][17];
@@ -935,7 +981,7 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     cut_gradients(a.dim, a.rows, std::min(a.piece, a.classes), p.dx, p.dw);
     take(a.x_most, a.dim);
     take(a.w_most, a.dim);
-    take(a.most_part, kStrips * a.dim);
+    take(a.most_part, 2 * kStrips * a.dim);
     take(a.xt, a.dim * a.rows_pad * 2 * p.planes);
     take(a.wt, a.dim * a.piece * 2 * p.planes);
     take(a.g, a.rows_pad * a.piece * 2 * p.planes);
@@ -957,30 +1003,38 @@ struct Steps {
   }
 };
 
+CeRows rows_of_x(const CeArgs &a) {
+  CeRows r{};
+  r.src = a.x, r.stride = a.x_stride, r.rows = a.rows, r.list = a.list, r.most = a.x_most;
+  return r;
+}
+CeRows rows_of_w(const CeArgs &a) {
+  CeRows r{};
+  r.src = a.w, r.stride = a.w_stride, r.rows = a.classes, r.most = a.w_most;
+  return r;
+}
+
 template <typename T, typename U, int PLANES> int32_t pack_operands(const CeArgs &a, const CePlan &p, void *stream) {
-  const T *const x = static_cast<const T *>(a.x), *const w = static_cast<const T *>(a.w);
-  Steps steps;
-  if (!p.x_direct)
-    steps([&] {
-      return launch(ce_pack_rows_kernel<T, U, PLANES>, dim3(ceil_div64(a.rows, 4)), dim3(256), stream, x,
-                    a.x_stride, a.rows, a.dim, a.meta, a.list, a.xp, a.xp_stride, a.xp_plane, a.x_unit);
-    });
-  if (!p.w_direct)
-    steps([&] {
-      return launch(ce_pack_rows_kernel<T, U, PLANES>, dim3(ceil_div64(a.classes, 4)), dim3(256), stream,
-                    w, a.w_stride, a.classes, a.dim, a.meta, static_cast<const int32_t *>(nullptr), a.wp,
-                    a.wp_stride, a.wp_plane, a.w_unit);
-    });
-  return steps.rc;
+  CeRows x = rows_of_x(a), w = rows_of_w(a);
+  x.out = a.xp, x.out_stride = a.xp_stride, x.plane = a.xp_plane, x.unit = a.x_unit;
+  w.out = a.wp, w.out_stride = a.wp_stride, w.plane = a.wp_plane, w.unit = a.w_unit;
+  if (!p.x_direct) x.blocks = ceil_div64(a.rows, 4);
+  if (!p.w_direct) w.blocks = ceil_div64(a.classes, 4);
+  if (x.blocks + w.blocks == 0) return SPORDER_OK;
+  return launch(ce_pack_rows_kernel<T, U, PLANES>, dim3(x.blocks + w.blocks), dim3(256), stream, x, w, a.dim,
+                a.meta);
 }
 
 int32_t list_rows(const CeArgs &a, bool backward, void *stream) {
   Steps steps;
-  steps([&] { return launch(ce_prepare_kernel, dim3(ceil_div64(a.classes_pad, 256)), dim3(256), stream, a); });
-  const dim3 blocks(ceil_div64(a.rows, kListBlock));
+  const int64_t blocks = ceil_div64(a.rows, kListBlock), others = ceil_div64(a.classes_pad, 256);
+  const bool alone = blocks == 1; // no workgroup needs what another one prepares
+  if (!alone) steps([&] { return launch(ce_prepare_kernel, dim3(others), dim3(256), stream, a); });
   if (a.rows > kListDirect)
-    steps([&] { return launch(ce_count_kernel, blocks, dim3(256), stream, a); });
-  steps([&] { return launch(ce_list_kernel, blocks, dim3(256), stream, a, backward); });
+    steps([&] { return launch(ce_count_kernel, dim3(blocks), dim3(256), stream, a); });
+  steps([&] {
+    return launch(ce_list_kernel, dim3(blocks + (alone ? others : 0)), dim3(256), stream, a, backward, blocks);
+  });
   return steps.rc;
 }
 
@@ -1017,34 +1071,36 @@ int32_t finish(const CeArgs &a, int64_t v0, int64_t rows, int splits, void *stre
 }
 
 template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, const CePlan &p, void *stream) {
-  const T *const x = static_cast<const T *>(a.x), *const w = static_cast<const T *>(a.w);
-  const int32_t *const no_list = nullptr;
   Steps steps;
   steps([&] { return list_rows(a, true, stream); });
   steps([&] { return pack_operands<T, U, PLANES>(a, p, stream); });
-  auto columns_most = [&](const T *src, int64_t stride, int64_t rows, const int32_t *list, float *most) {
-    const int64_t across = ceil_div64(a.dim, kWave * (16 / sizeof(T)));
-    const int64_t strips = std::min(ceil_div64(rows, 32), std::min<int64_t>(std::max<int64_t>(1024 / across, 64), kStrips));
-    const int32_t rc = launch(ce_column_most_kernel<T>, dim3(across, strips),
-                              dim3(256), stream, src, stride, rows, a.dim, a.meta, list, a.most_part);
-    if (rc != SPORDER_OK) return rc;
-    return launch(ce_strips_most_kernel, dim3(ceil_div64(a.dim, kWave)), dim3(256), stream, a.most_part, strips,
-                  a.dim, most);
+  CeRows x = rows_of_x(a), w = rows_of_w(a);
+  const int64_t across = ceil_div64(a.dim, kWave * (16 / sizeof(T)));
+  auto strips = [&](int64_t rows) {
+    return std::min(ceil_div64(rows, 32), std::min<int64_t>(std::max<int64_t>(1024 / across, 64), kStrips));
   };
-  steps([&] { return columns_most(x, a.x_stride, a.rows, a.list, a.x_most); });
-  steps([&] { return columns_most(w, a.w_stride, a.classes, no_list, a.w_most); });
-  auto pack_columns = [&](const T *src, int64_t stride, int64_t rows, const int32_t *list, const float *most,
-                          char *out, int64_t out_rows) {
-    return launch(ce_pack_columns_kernel<T, PLANES>, dim3(ceil_div64(rows, 64), ceil_div64(a.dim, 64)), dim3(256),
-                  stream, src, stride, rows, a.dim, a.meta, list, a.exponent, most, out, out_rows * 2,
-                  a.dim * out_rows * 2);
-  };
-  steps([&] { return pack_columns(x, a.x_stride, a.rows, a.list, a.x_most, a.xt, a.rows_pad); });
-  steps([&] { return launch(ce_zero_kernel<T>, dim3(ceil_div64(a.rows, 4)), dim3(256), stream, a); });
+  x.blocks = strips(a.rows), w.blocks = strips(a.classes);
+  steps([&] {
+    const int64_t zeros = std::min<int64_t>(ceil_div64(a.rows, 256), kStrips);
+    return launch(ce_column_most_kernel<T>, dim3(across, x.blocks + w.blocks + zeros), dim3(256), stream, x, w, a,
+                  a.most_part);
+  });
+  steps([&] {
+    return launch(ce_strips_most_kernel, dim3(ceil_div64(a.dim, kWave), 2), dim3(256), stream, a.most_part, x,
+                  w, a.dim);
+  });
+  x.out = a.xt, x.out_stride = a.rows_pad * 2, x.plane = a.dim * x.out_stride;
+  w.out = a.wt, w.out_stride = a.piece * 2, w.plane = a.dim * w.out_stride;
+  x.blocks = ceil_div64(a.rows, 64);
   const bool one_piece = a.piece >= a.classes, dx_direct = one_piece && p.dx.splits == 1;
   for (int64_t v0 = 0; v0 < a.classes; v0 += a.piece) {
     const int64_t here = std::min(a.piece, a.classes - v0);
-    steps([&] { return pack_columns(w + v0 * a.w_stride, a.w_stride, here, no_list, a.w_most, a.wt, a.piece); });
+    w.src = static_cast<const T *>(a.w) + v0 * a.w_stride, w.rows = here, w.blocks = ceil_div64(here, 64);
+    steps([&] {
+      return launch(ce_pack_columns_kernel<T, PLANES>, dim3(x.blocks + w.blocks, ceil_div64(a.dim, 64)), dim3(256),
+                    stream, x, w, a.dim, a.meta, a.exponent);
+    });
+    x.blocks = 0; // with the first piece
     auto tiles = [&](auto shape) {
       using S = decltype(shape);
       return launch(ce_g_kernel<U, PLANES, S>, dim3(ceil_div64(here, S::kM) * ceil_div64(a.rows, S::kN)),

@@ -1,5 +1,6 @@
 // dense.hpp -- pieces shared by the training operators (layer_norm.hip,
-// embedding.hip, newton_schulz.hip): element types, vector access, sums over
+// embedding.hip, newton_schulz.hip, dropout.hip, residual_norm.hip,
+// cross_entropy*.hip): element types, vector access, sums over
 // lane groups and the status codes of their C entries.
 //
 // These entries differ from the rest of the library: they run on the caller's

@@ -1,13 +1,14 @@
 """Differentiable forms of the training operators, and the optimiser that uses
 the orthogonalisation.
 
-``embedding`` and ``layer_norm`` are ``sporder.embedding`` and
-``sporder.layer_norm`` with their gradients behind torch's autograd; ``Muon``
-updates weight matrices along the orthogonalised momentum
-(``sporder.newton_schulz``).  Their backward passes are not differentiable in
-turn, and they take neither forward-mode derivatives nor ``torch.func``'s
-transforms (RuntimeError).  The end-to-end GCN (``e2e_gcn``) trains with them
-on request.  They have no counterpart in the reference.
+``embedding``, ``layer_norm``, ``dropout``, ``residual_norm`` and
+``linear_cross_entropy`` are ``sporder``'s with their gradients behind torch's
+autograd; ``Dropout`` holds a seed and counts its calls; ``Muon`` updates weight
+matrices along the orthogonalised momentum (``sporder.newton_schulz``).  Their
+backward passes are not differentiable in turn, and they take neither
+forward-mode derivatives nor ``torch.func``'s transforms (RuntimeError).  The
+end-to-end GCN (``e2e_gcn``) trains with them on request.  They have no
+counterpart in the reference.
 """
 
 from __future__ import annotations

@@ -1,6 +1,6 @@
-"""Operators of a training step around the SpMM: row lookup, layer norm and
-the orthogonalisation of a weight's update, each with what its backward pass
-needs.  They have no counterpart in the reference.
+"""Operators of a training step around the SpMM: row lookup, layer norm, the
+orthogonalisation of a weight's update, dropout, the norms around a block and
+the cross entropy of linear logits, each with what its backward pass needs.  They have no counterpart in the reference.
 
 Unlike the rest of the package they run on torch's current stream of the
 input's device and return without waiting, so they follow and precede torch

@@ -37,9 +37,10 @@ __device__ __forceinline__ bool counted(const CeCall &a, int64_t target) {
 constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
 
-// Sums of two values over a workgroup of 256, in 64 bits and a fixed order, in its
+// Sums of two values over a workgroup of WAVES waves, in 64 bits and a fixed order, in its
 // first two threads (the first value in thread 0).
-__device__ __forceinline__ double block_sums(double s, double n, double (&part)[2][4]) {
+template <int WAVES>
+__device__ __forceinline__ double block_sums(double s, double n, double (&part)[2][WAVES]) {
 #pragma unroll
   for (int j = 1; j < kWave; j <<= 1) {
     s += __shfl_xor(s, j);
@@ -50,8 +51,10 @@ __device__ __forceinline__ double block_sums(double s, double n, double (&part)[
     part[1][threadIdx.x / kWave] = n;
   }
   __syncthreads();
-  const double *const p = part[threadIdx.x & 1];
-  return (p[0] + p[1]) + (p[2] + p[3]);
+  double all = 0.0;
+#pragma unroll
+  for (int i = 0; i < WAVES; ++i) all += part[threadIdx.x & 1][i];
+  return all;
 }
 
 using f32x4 = float __attribute__((ext_vector_type(4)));
@@ -82,7 +85,7 @@ template <typename T> __device__ __forceinline__ f32x4 floats(const Words<T, 4> 
 }
 
 // The one-pass form.
-bool few_takes(int64_t dim, int64_t classes, bool backward);
+bool few_takes(int type, int64_t dim, int64_t classes, bool backward);
 size_t few_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward);
 int32_t few_forward(const CeCall &a, void *work, void *stream);
 int32_t few_backward(const CeCall &a, void *work, void *stream);

@@ -1,13 +1,14 @@
 // cross_entropy_few.hip -- linear cross entropy where all classes' weights fit a
 // workgroup's LDS (a graph's node classes): one pass over the rows each way.
 //
-// A workgroup keeps w in LDS and takes tiles of rows.  The products are 32-bit ones
-// (16 x 16 x 4 per matrix instruction) whatever the type, so nothing is rounded on
-// the way:
+// A workgroup keeps w in LDS and takes 16 or 32 rows at a time:
 //   z^T = w x^T      classes down (a lane's registers), rows across (lanes)
 //   dx^T = w^T g^T   features down, rows across
 //   dw = g^T x       classes down, features across, in registers over all tiles
-// A matrix instruction's four steps along the sum may be any four: lane group q
+// Three kernels: the loss, whose rows never see LDS; the gradients where a wave's own tile
+// fits LDS besides w; and the gradients with tiles shared by the workgroup, in 32-bit
+// products (16 x 16 x 4 per matrix instruction) whatever the type.
+// A matrix instruction's four steps along the sum may be any four: there lane group q
 // takes elements 4 q .. 4 q + 3 of 16 (one LDS access for four instructions where
 // they lie side by side), and in the last two products rows r + 4 q, which
 // with rows 4 floats longer than a multiple of 16 lie in different banks.
@@ -142,49 +143,207 @@ __device__ __forceinline__ void logits(const float *w, const float *rows, int di
   }
 }
 
-// ---- forward: 64 rows a tile, 16 a wave ------------------------------------------------
+// ---- forward: rows straight from memory, 16 a wave ----------------------------------------
+
+// A lane's eight neighbouring features of a row are what a matrix instruction takes, so x
+// goes from memory to registers and to the products, and only w is in LDS: 16-bit types as
+// they are, 32-bit ones as two 16-bit halves of their row's unit, three products for each
+// (22 bits).  An access that would pass the row's end is the row's last one, and w's copy in
+// LDS has those features there, each once, and zeros: nothing of x is moved or masked.
+// Bound by memory: 2,449,029 rows of 128, 47 classes in 306 us (4.2 TB/s; 32-bit products from
+// tiles in LDS took 482), bfloat16 140 (4.8 TB/s; 430); 580,000 rows of 500, 80 classes, bfloat16
+// 130 us (tiles of any number of classes: 464).
+template <typename T> struct LossType {
+  using U = T;
+  static constexpr int kPlanes = 1;
+};
+template <> struct LossType<float> {
+  using U = f16_t;
+  static constexpr int kPlanes = 2;
+};
+
+__device__ __forceinline__ f32x4 mfma_sixteen(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ f32x4 mfma_sixteen(bf16x8 a, bf16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ void split_eight(const float (&v)[8], f16x8 &hi, f16x8 &lo) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const f16_t h = static_cast<f16_t>(v[e]);
+    hi[e] = h;
+    lo[e] = static_cast<f16_t>(v[e] - static_cast<float>(h));
+  }
+}
+
+template <typename T> constexpr int loss_lds(int class_blocks, int feature_blocks) {
+  return class_blocks * 16 * ((feature_blocks * 64 + 8) * 2 * LossType<T>::kPlanes + 8);
+}
+// Workgroups on a CU that registers allow.
+template <typename T> constexpr int loss_groups(int class_blocks, int feature_blocks) {
+  const int bytes = feature_blocks * sizeof(T);
+  return bytes <= 8 && class_blocks <= 6 && class_blocks * bytes <= 32 ? 2 : 1;
+}
 
 template <typename T, int VB, int DB>
-__global__ void __launch_bounds__(kLossThreads) few_loss_kernel(FewArgs a) {
+__global__ void __launch_bounds__(kGradThreads, 2 * loss_groups<T>(VB, DB)) few_loss_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
+  using U = typename LossType<T>::U;
+  using U8 = U __attribute__((ext_vector_type(8)));
+  constexpr int kPlanes = LossType<T>::kPlanes, kVec = 16 / sizeof(T), kV = VB * 16, kW = DB * 64 + 8;
+  constexpr int kParts = 8 / kVec; // accesses for eight features
+  constexpr bool kAhead = DB * sizeof(T) <= 16; // the next row's words have room in registers
   const CeCall &c = a.c;
-  constexpr int stride = few_stride(DB);
-  const int dim16 = static_cast<int>(ceil_div64(c.dim, 16));
-  float *const w = lds, *const x = w + VB * 16 * stride, *const bias = x + 64 * stride;
-  const int lane = lane_id(), wave = threadIdx.x / kWave;
-  hold_weights<T, VB, DB, kLossThreads>(c, w, bias);
+  const int dim = static_cast<int>(c.dim), tid = threadIdx.x, lane = lane_id(), q = lane / 16, l = lane % 16;
+  float *const w_unit = lds, *const bias = lds + kV;
+  U *const w = reinterpret_cast<U *>(lds + 2 * kV); // hi, then lo
+
+  // w by accesses as x's, 16 threads a row.
+  const int part = tid % 16 * 4, inside = part % kVec;
+  for (int v = tid / 16; v < kV; v += kGradThreads / 16) {
+    const T *const row = static_cast<const T *>(c.w) + min(static_cast<int64_t>(v), c.classes - 1) * c.w_stride;
+    f32x4 f[DB];
+    float most = 0.0f;
+#pragma unroll
+    for (int k = 0; k < DB; ++k) {
+      const int start = k * 64 + part - inside, from = min(start, dim - kVec) + inside;
+      const auto p = __builtin_bit_cast(Pack<T, 4>, *reinterpret_cast<const LoosePack<T, 4> *>(row + from));
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        f[k][e] = v < c.classes && from + e >= start ? static_cast<float>(p.v[e]) : 0.0f;
+        most = fmaxf(most, fabsf(f[k][e]));
+      }
+    }
+    float scale = 1.0f;
+    if constexpr (kPlanes == 2) {
+      const float u = unit_of(group_max<16>(most));
+      scale = unit_inverse(u);
+      if (part == 0) w_unit[v] = u;
+    }
+#pragma unroll
+    for (int k = 0; k < DB; ++k) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float s = f[k][e] * scale;
+        const U h = static_cast<U>(s);
+        w[v * kW + k * 64 + part + e] = h;
+        if constexpr (kPlanes == 2) w[(kV + v) * kW + k * 64 + part + e] = static_cast<U>(s - static_cast<float>(h));
+      }
+    }
+  }
+  for (int v = tid; v < kV; v += kGradThreads) {
+    float b = v < c.classes ? 0.0f : -INFINITY;
+    if (c.bias && v < c.classes) with_type(c.bias, c.bias_type, [&](auto *p) { b = static_cast<float>(p[v]); });
+    bias[v] = b;
+  }
+  __syncthreads();
+
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int64_t step = gridDim.x * int64_t(kGradThreads / kWave * 16);
+  const int64_t first = (blockIdx.x * int64_t(kGradThreads / kWave) + wave) * 16;
+  int next_at;
+  RawTarget next_target;
+  Words<T, kVec> next[DB * 2][kParts];
+  // Rows that count nothing are read as the first one, which the caches hold.
+  auto fetch_row = [&](int64_t r) {
+    next_at = class_of(c, r, next_target);
+    const T *const x = static_cast<const T *>(c.x) + (next_at >= 0 ? r : 0) * c.x_stride;
+#pragma unroll
+    for (int k = 0; k < DB * 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < kParts; ++i)
+        next[k][i] = __builtin_bit_cast(Words<T, kVec>, *reinterpret_cast<const LoosePack<T, kVec> *>(
+                                                            x + min(k * 32 + q * 8 + i * kVec, dim - kVec)));
+    }
+  };
+  next_target = fetch_target(c, first + l);
+  if constexpr (kAhead) {
+    fetch_row(first + l);
+    __builtin_amdgcn_sched_barrier(0); // loads in the loop's order, so that it waits for no later ones
+    next_target = fetch_target(c, first + l + step);
+  }
   double sum = 0.0, n = 0.0;
-  const int64_t step = gridDim.x * int64_t(64);
-  int target[4];            // of the rows on their way
-  RawTarget next_target[4]; // of those after them
-  Words<T, 4> next[4][DB];
-  int64_t row = blockIdx.x * int64_t(64) + wave * 16 + lane % 16; // of this lane
-  fetch_targets<16>(c, blockIdx.x * int64_t(64), next_target);
-  classes_of<16>(c, blockIdx.x * int64_t(64), next_target, target);
-  fetch_tile<T, 16>(c, blockIdx.x * int64_t(64), target, next);
-  __builtin_amdgcn_sched_barrier(0); // loads in the loop's order, so that it waits for no later ones
-  fetch_targets<16>(c, blockIdx.x * int64_t(64) + step, next_target);
-  RawTarget next_class = fetch_target(c, row);
-  for (int64_t tile = blockIdx.x; tile < a.tiles; tile += gridDim.x) {
-    __syncthreads(); // the tile before is done with
-    put_tile<T, 16>(c, x, target, next);
-    __syncthreads();
-    const int at = class_of(c, row, next_class);
-    classes_of<16>(c, tile * 64 + step, next_target, target);
-    fetch_tile<T, 16>(c, tile * 64 + step, target, next);
-    fetch_targets<16>(c, tile * 64 + 2 * step, next_target);
-    next_class = fetch_target(c, row + step);
+  for (int64_t r0 = first; r0 < c.rows; r0 += step) {
+    const int64_t row = r0 + l;
+    if constexpr (!kAhead) {
+      fetch_row(row);
+      next_target = fetch_target(c, row + step);
+    }
+    Words<T, kVec> x[DB * 2][kParts];
+#pragma unroll
+    for (int k = 0; k < DB * 2; ++k) {
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) x[k][i] = next[k][i];
+    }
+    const int at = next_at;
+    if constexpr (kAhead) {
+      fetch_row(row + step);
+      next_target = fetch_target(c, row + 2 * step);
+    }
+    float unit = 1.0f, inverse = 1.0f;
+    if constexpr (kPlanes == 2) {
+      float most = 0.0f;
+#pragma unroll
+      for (int k = 0; k < DB * 2; ++k) {
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          const auto p = __builtin_bit_cast(Pack<T, kVec>, x[k][i]);
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) most = fmaxf(most, fabsf(static_cast<float>(p.v[e])));
+        }
+      }
+      most = fmaxf(most, lane_xor_f32(most, 16));
+      most = fmaxf(most, lane_xor_f32(most, 32));
+      unit = unit_of(most);
+      inverse = unit_inverse(unit);
+    }
+    // Places in LDS that the compiler can't tell from the last row's, or it would keep all of
+    // w in registers.
+    uint32_t w_at = l * kW + q * 8, four_at = q * 4;
+    asm volatile("" : "+v"(w_at), "+v"(four_at));
     f32x4 z[VB] = {};
-    logits<VB, 1, DB>(w, x + wave * 16 * stride, dim16, VB, z);
+#pragma unroll
+    for (int k = 0; k < DB * 2; ++k) {
+      U8 hi, lo;
+      if constexpr (kPlanes == 2) {
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const auto p = __builtin_bit_cast(Pack<T, kVec>, x[k][i]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[i * 4 + e] = p.v[e] * inverse;
+        }
+        split_eight(v, hi, lo);
+      } else {
+        hi = __builtin_bit_cast(U8, x[k][0]);
+      }
+#pragma unroll
+      for (int b = 0; b < VB; ++b) {
+        const U *const from = w + w_at + b * 16 * kW + k * 32;
+        const U8 wh = *reinterpret_cast<const U8 *>(from);
+        z[b] = mfma_sixteen(wh, hi, z[b]);
+        if constexpr (kPlanes == 2) {
+          z[b] = mfma_sixteen(wh, lo, z[b]);
+          z[b] = mfma_sixteen(*reinterpret_cast<const U8 *>(from + kV * kW), hi, z[b]);
+        }
+      }
+    }
     float most = -INFINITY, hit = 0.0f;
+    const int mine = at - static_cast<int>(four_at);
 #pragma unroll
     for (int v = 0; v < VB; ++v) {
-      const f32x4 b = *reinterpret_cast<const f32x4 *>(bias + v * 16 + lane / 16 * 4);
+      const f32x4 b = *reinterpret_cast<const f32x4 *>(bias + four_at + v * 16);
+      if constexpr (kPlanes == 2) {
+        const f32x4 u = *reinterpret_cast<const f32x4 *>(w_unit + four_at + v * 16);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) z[v][e] = z[v][e] * unit * u[e];
+      }
       z[v] += b;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         most = fmaxf(most, z[v][e]);
-        hit += v * 16 + lane / 16 * 4 + e == at ? z[v][e] : 0.0f;
+        hit += v * 16 + e == mine ? z[v][e] : 0.0f;
       }
     }
     most = fmaxf(most, lane_xor_f32(most, 16));
@@ -208,15 +367,14 @@ __global__ void __launch_bounds__(kLossThreads) few_loss_kernel(FewArgs a) {
       sum += loss;
       n += at == -1 ? 0.0 : 1.0;
     }
-    row += step;
   }
-  __shared__ double part[2][4];
-  const double v = block_sums(sum, n, part);
-  if (threadIdx.x >= 2) return;
+  __shared__ double parts[2][kGradThreads / kWave];
+  const double v = block_sums(sum, n, parts);
+  if (tid >= 2) return;
   if (gridDim.x == 1)
-    c.sums[threadIdx.x] = static_cast<float>(v);
+    c.sums[tid] = static_cast<float>(v);
   else
-    a.sums[2 * blockIdx.x + threadIdx.x] = v;
+    a.sums[2 * blockIdx.x + tid] = v;
 }
 
 __global__ void __launch_bounds__(kLossThreads) few_total_kernel(FewArgs a, int blocks) {
@@ -382,18 +540,6 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
 // in units of x's and w's rows and w's columns, as in the tiled form), at a fifth of the
 // 32-bit products' time; dw, which sums over rows of any scale, stays with those.  Rows are
 // of whole accesses of four elements, and dx's at such addresses.
-__device__ __forceinline__ f32x4 mfma_halves(f16x8 a, f16x8 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
-}
-__device__ __forceinline__ void split_eight(const float (&v)[8], f16x8 &hi, f16x8 &lo) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const f16_t h = static_cast<f16_t>(v[e]);
-    hi[e] = h;
-    lo[e] = static_cast<f16_t>(v[e] - static_cast<float>(h));
-  }
-}
-
 template <int VB, int DB> struct WaveShape {
   static constexpr int kV = VB * 16, kV32 = (VB + 1) / 2 * 32, kD = DB * 64;
   static constexpr int kW = kD + 8, kT = kV32 + 8;   // halves of a row of w and of w^T
@@ -561,11 +707,11 @@ __global__ void __launch_bounds__(kGradThreads, 2) few_grad_wave_kernel(FewArgs 
         wl[b] = *reinterpret_cast<const f16x8 *>(from + S::kV * S::kW);
       }
 #pragma unroll
-      for (int b = 0; b < VB; ++b) z[b] = mfma_halves(wl[b], hi, z[b]);
+      for (int b = 0; b < VB; ++b) z[b] = mfma_sixteen(wl[b], hi, z[b]);
 #pragma unroll
-      for (int b = 0; b < VB; ++b) z[b] = mfma_halves(wh[b], lo, z[b]);
+      for (int b = 0; b < VB; ++b) z[b] = mfma_sixteen(wh[b], lo, z[b]);
 #pragma unroll
-      for (int b = 0; b < VB; ++b) z[b] = mfma_halves(wh[b], hi, z[b]);
+      for (int b = 0; b < VB; ++b) z[b] = mfma_sixteen(wh[b], hi, z[b]);
     }
     f16x8 gh[S::kV32 / 32], gl[S::kV32 / 32];
 #pragma unroll
@@ -624,11 +770,11 @@ __global__ void __launch_bounds__(kGradThreads, 2) few_grad_wave_kernel(FewArgs 
           tl[j] = *reinterpret_cast<const f16x8 *>(from + S::kD * S::kT);
         }
 #pragma unroll
-        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_halves(tl[j], gh[b], d[j0 + j]);
+        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_sixteen(tl[j], gh[b], d[j0 + j]);
 #pragma unroll
-        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_halves(th[j], gl[b], d[j0 + j]);
+        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_sixteen(th[j], gl[b], d[j0 + j]);
 #pragma unroll
-        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_halves(th[j], gh[b], d[j0 + j]);
+        for (int j = 0; j < kSide; ++j) d[j0 + j] = mfma_sixteen(th[j], gh[b], d[j0 + j]);
         __builtin_amdgcn_sched_barrier(0); // the next ones' operands would not fit the registers
       }
     }
@@ -729,22 +875,24 @@ int feature_blocks(int64_t dim) {
   return 0;
 }
 
-int64_t floats_of(int64_t dim, int blocks, bool backward) {
-  const int64_t stride = few_stride(feature_blocks(dim));
-  return backward ? (blocks * 16 + 2 * kRows) * stride + kRows * (blocks * 16 + 4) + blocks * 16
-                  : (blocks * 16 + 64) * stride + blocks * 16;
-}
-int64_t lds_of(int64_t dim, int64_t classes, bool backward) {
-  return floats_of(dim, class_blocks(classes), backward) * 4 + 256;
-}
+// Blocks of classes times blocks of features that kernels are built for: what LDS holds of w
+// in 32 bits, or in 16.
+constexpr int kMostBlocks = 24, kMostHalves = 48;
 
-template <typename F> int32_t with_blocks(int64_t dim, int64_t classes, F &&f);
+// Backward, with tiles shared by the workgroup.
+int64_t floats_of(int64_t dim, int blocks) {
+  const int64_t stride = few_stride(feature_blocks(dim));
+  return (blocks * 16 + 2 * kRows) * stride + kRows * (blocks * 16 + 4) + blocks * 16;
+}
+int64_t lds_of(int64_t dim, int64_t classes) { return floats_of(dim, class_blocks(classes)) * 4 + 256; }
+
+template <int MOST, typename F> int32_t with_blocks(int64_t dim, int64_t classes, F &&f);
 
 // The LDS of the backward pass that gives each wave tiles of its own, 0 where it doesn't fit.
 int64_t wave_lds(int64_t dim, int64_t classes) {
   int64_t bytes = 0;
   if (dim % 4 != 0) return bytes;
-  with_blocks(dim, classes, [&](auto vb, auto db) {
+  with_blocks<kMostBlocks>(dim, classes, [&](auto vb, auto db) {
     using S = WaveShape<decltype(vb)::value, decltype(db)::value>;
     if constexpr (S::kFits) bytes = S::kFloats * 4;
     return static_cast<int32_t>(SPORDER_OK);
@@ -760,19 +908,18 @@ template <typename T> bool by_waves(const CeCall &c) {
 }
 bool by_waves(const CeCall &c) { return c.type == SPORDER_TYPE_F32 ? by_waves<float>(c) : by_waves<f16_t>(c); }
 
-// Workgroups: as many per CU as fit, up to two (sixteen waves) or three of the forward pass's.
-int64_t grid_of(int64_t rows, int64_t dim, int64_t classes, bool backward) {
-  const int64_t fit = kLds / lds_of(dim, classes, backward);
-  return std::min(ceil_div64(rows, backward ? kRows : 64), 256 * std::min<int64_t>(fit, backward ? 2 : 3));
+// Workgroups: as many per CU as fit, up to two.
+int64_t grid_of(int64_t rows, int64_t dim, int64_t classes) {
+  return std::min(ceil_div64(rows, kRows), 256 * std::min<int64_t>(kLds / lds_of(dim, classes), 2));
 }
 
 // f with the class and feature blocks, as types.
-template <typename F> int32_t with_blocks(int64_t dim, int64_t classes, F &&f) {
+template <int MOST, typename F> int32_t with_blocks(int64_t dim, int64_t classes, F &&f) {
   auto classes_of = [&](auto db) {
     constexpr int DB = decltype(db)::value;
     const int b = class_blocks(classes);
     auto at = [&](auto vb) {
-      if constexpr (decltype(vb)::value * DB <= 24)
+      if constexpr (decltype(vb)::value * DB <= MOST)
         return f(vb, db);
       else
         return static_cast<int32_t>(SPORDER_BAD_ARGUMENT); // not reached
@@ -825,7 +972,7 @@ struct FewLayout {
 };
 FewLayout few_layout(int64_t rows, int64_t dim, int64_t classes, bool backward) {
   FewLayout l{};
-  l.grid = grid_of(rows, dim, classes, backward); // at least what either backward pass takes
+  if (backward) l.grid = grid_of(rows, dim, classes); // at least what either backward pass takes
   const int64_t pad = class_blocks(classes) * 16;
   size_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -834,7 +981,7 @@ FewLayout few_layout(int64_t rows, int64_t dim, int64_t classes, bool backward) 
     return here;
   };
   if (!backward) {
-    l.sums = take(l.grid * 16);
+    l.sums = take(2 * 256 * 16);
   } else {
     l.dw = take(l.grid * pad * ceil_div64(dim, 16) * 16 * 4);
     l.db = take(l.grid * pad * 4);
@@ -843,30 +990,39 @@ FewLayout few_layout(int64_t rows, int64_t dim, int64_t classes, bool backward) 
   return l;
 }
 
-template <typename T> int32_t few_loss(const FewArgs &a, int64_t grid, void *stream) {
-  return with_blocks(a.c.dim, a.c.classes, [&](auto vb, auto db) {
+template <typename T> int32_t few_loss(const FewArgs &a, void *stream) {
+  int64_t grid = 0;
+  constexpr int kMost = sizeof(T) == 2 ? kMostHalves : kMostBlocks;
+  const int32_t rc = with_blocks<kMost>(a.c.dim, a.c.classes, [&](auto vb, auto db) {
     constexpr int VB = decltype(vb)::value, DB = decltype(db)::value;
-    return launch_lds(few_loss_kernel<T, VB, DB>, grid, kLossThreads, floats_of(a.c.dim, VB, false) * 4, stream, a);
+    constexpr int lds = loss_lds<T>(VB, DB);
+    static_assert(lds + 256 <= kLds);
+    grid = std::min<int64_t>(ceil_div64(a.c.rows, kGradThreads / 4),
+                             256 * std::min(kLds / (lds + 256), loss_groups<T>(VB, DB)));
+    return launch_lds(few_loss_kernel<T, VB, DB>, grid, kGradThreads, lds, stream, a);
   });
+  if (rc != SPORDER_OK || grid == 1) return rc;
+  return launch(few_total_kernel, dim3(1), dim3(kLossThreads), stream, a, static_cast<int>(grid));
 }
 
 template <typename T> int32_t few_grad(const FewArgs &a, int64_t grid, void *stream) {
-  return with_blocks(a.c.dim, a.c.classes, [&](auto vb, auto db) {
+  return with_blocks<kMostBlocks>(a.c.dim, a.c.classes, [&](auto vb, auto db) {
     constexpr int VB = decltype(vb)::value, DB = decltype(db)::value;
     using S = WaveShape<VB, DB>;
     if constexpr (S::kFits) {
       if (by_waves(a.c))
         return launch_lds(few_grad_wave_kernel<T, VB, DB>, grid, kGradThreads, S::kFloats * 4, stream, a);
     }
-    return launch_lds(few_grad_kernel<T, VB, DB>, grid, kGradThreads, floats_of(a.c.dim, VB, true) * 4, stream, a);
+    return launch_lds(few_grad_kernel<T, VB, DB>, grid, kGradThreads, floats_of(a.c.dim, VB) * 4, stream, a);
   });
 }
 
 } // namespace
 
-bool few_takes(int64_t dim, int64_t classes, bool backward) {
-  const int b = class_blocks(classes), f = feature_blocks(dim);
-  return dim >= 4 && b && f && b * f <= 24 && lds_of(dim, classes, backward) <= kLds;
+bool few_takes(int type, int64_t dim, int64_t classes, bool backward) {
+  const int blocks = class_blocks(classes) * feature_blocks(dim);
+  const int most = type != SPORDER_TYPE_F32 && !backward ? kMostHalves : kMostBlocks;
+  return dim >= 8 && blocks && blocks <= most && (!backward || lds_of(dim, classes) <= kLds);
 }
 
 size_t few_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward) {
@@ -875,13 +1031,11 @@ size_t few_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward)
 
 int32_t few_forward(const CeCall &c, void *work, void *stream) {
   const FewLayout l = few_layout(c.rows, c.dim, c.classes, false);
-  FewArgs a{c, ceil_div64(c.rows, 64), reinterpret_cast<double *>(static_cast<char *>(work) + l.sums), nullptr,
+  FewArgs a{c, 0, reinterpret_cast<double *>(static_cast<char *>(work) + l.sums), nullptr,
             nullptr};
-  const int32_t rc = c.type == SPORDER_TYPE_BF16  ? few_loss<bf16_t>(a, l.grid, stream)
-                     : c.type == SPORDER_TYPE_F16 ? few_loss<f16_t>(a, l.grid, stream)
-                                                  : few_loss<float>(a, l.grid, stream);
-  if (rc != SPORDER_OK || l.grid == 1) return rc;
-  return launch(few_total_kernel, dim3(1), dim3(kLossThreads), stream, a, static_cast<int>(l.grid));
+  return c.type == SPORDER_TYPE_BF16  ? few_loss<bf16_t>(a, stream)
+         : c.type == SPORDER_TYPE_F16 ? few_loss<f16_t>(a, stream)
+                                      : few_loss<float>(a, stream);
 }
 
 int32_t few_backward(const CeCall &c, void *work, void *stream) {

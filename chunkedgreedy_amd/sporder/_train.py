@@ -621,7 +621,7 @@ def linear_cross_entropy(x, weight, targets, bias=None, *, ignore_index=-100):
     Returns (loss, lse, sums): loss and lse float32 of the targets' shape (NaN
     for a target that is neither a class nor ignored), sums float32 (2,) of the
     losses' sum and the number of rows that are not ignored.  At most 2^23 - 256
-    rows (more with up to 64 classes of 4 to 256 elements, or 192 of 4 to 64),
+    rows (more with up to 64 classes of 8 to 256 elements, or 192 of 8 to 64),
     2^25 classes, 2^37 logits and 65536 elements a row.
 
     Sums are held in 32 bits.  float32 products have operands of 22 bits: a term

@@ -581,7 +581,7 @@ SPORDER_API int32_t sporder_residual_norm_grad(
  * and lse 0 and is not read; one whose target is no class otherwise has NaN.  d_sums
  * receives the sum of the losses and the number of rows whose target is not ignore_index.
  * dim is at most 65536, classes 2^25, rows 2^23 - 256 and rows times classes 2^37; up to
- * 64 classes of 4 to 256 features, or 192 of 4 to 64, rows are at most 2^37.  d_work is
+ * 64 classes of 8 to 256 features, or 192 of 8 to 64, rows are at most 2^37.  d_work is
  * 256-byte aligned and of the size that *_work_bytes gives for the same sizes, strides and
  * alignments.
  */

@@ -454,3 +454,56 @@ def test_refusals(sporder):
     with pytest.raises(ValueError):
         wide = torch.zeros(1, 65537, device="cuda")
         sporder.linear_cross_entropy(wide, wide, t[:1])
+
+
+@pytest.mark.parametrize("dim", [8, 9, 15, 33, 64, 99, 130, 255, 257, 300, 388, 500, 512])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+def test_few_classes_by_lengths(sporder, dim, dtype):
+    """The loss's one-pass form over rows that end inside its accesses, at odd
+    places and strides, with each number of class blocks."""
+    for classes in (1, 16, 30, 47, 64, 90, 128, 172, 192):
+        for rows in (1, 17, 150):
+            x, w, t, b, _ = inputs(rows, dim + 3, classes, dtype, dtype, 0.1, seed=dim + classes)
+            xs, ws = x[:, 1:dim + 1], w[:, 2:dim + 2]
+            check_loss(sporder.linear_cross_entropy(xs, ws, t, b), xs, ws, t, b)
+
+
+@pytest.mark.parametrize("dtype, dim", [(F32, 40), (BF16, 40), (F32, 260), (F32, 500)])
+def test_few_classes_of_many_rows(sporder, dtype, dim):
+    """More rows than the workgroups' waves take at a time; rows that count nothing,
+    and a first row that counts and holds no numbers, touch no other."""
+    rows = 140_003 if dim < 100 else 70_003
+    x, w, t, b, _ = inputs(rows, dim, 12, dtype, F32, 0.3, seed=3)
+    t[0] = 1
+    want = sporder.linear_cross_entropy(x, w, t, b)
+    check_loss(want, x, w, t, b)
+    x[0] = float("nan")
+    loss, lse, sums = sporder.linear_cross_entropy(x, w, t, b)
+    assert loss[0].isnan() and lse[0].isnan() and sums[0].isnan()
+    assert torch.equal(loss[1:], want[0][1:]) and torch.equal(lse[1:], want[1][1:])
+
+
+def test_few_classes_past_the_tiles_rows(sporder):
+    """2^23 + 77 rows, which only the one-pass form takes."""
+    rows = 2**23 + 77
+    x, w, t, b, s = inputs(rows, 8, 3, BF16, F32, 0.1, seed=4)
+    loss, lse, sums = sporder.linear_cross_entropy(x, w, t, b)
+    dx, dw, db = sporder.linear_cross_entropy_grad(s, x, w, t, lse, b)
+    some = torch.cat([torch.arange(0, rows, 99_991, device="cuda"),
+                      torch.arange(rows - 90, rows, device="cuda")])
+    check_loss((loss[some], lse[some], torch.stack([loss[some].sum(), (t[some] != -100).sum().float()])),
+               x[some], w, t[some], b)
+    assert float(sums[1]) == float((t != -100).sum())
+    p = torch.softmax(x.double() @ w.double().t() + b.double(), 1)
+    on = t != -100
+    p[torch.arange(rows, device="cuda")[on], t[on]] -= 1.0
+    g = p * (s * on).double()[:, None]
+    # 2^23 terms of |g| <= |s|; the sums' parts add up to some 2^-24 of the magnitudes a step.
+    size = g.abs().sum(0)
+    assert ((db.double() - g.sum(0)).abs() <= (rows / 256 / 512 + 600) * U * size).all()
+    want = g.t().contiguous() @ x.double()
+    size = g.abs().t().contiguous() @ x.double().abs()
+    assert ((dw.double() - want).abs() <= (2.0**-8 * want.abs() + 2.0**-11 * size)).all()
+    got = dx[some].double() - (g[some] @ w.double())
+    bound = 2.0**-8 * (g[some] @ w.double()).abs() + 2.0**-11 * (g[some].abs() @ w.double().abs())
+    assert (got.abs() <= bound + 2.0**-126).all()

@@ -90,7 +90,7 @@ COMMON = [
     dict(type=3), dict(bias_type=3), dict(target_bits=16), dict(rows=-1), dict(dim=0),
     dict(dim=65537), dict(classes=0), dict(classes=2**25 + 1), dict(x_stride=-1),
     dict(weight_stride=-1), dict(rows=2**37 + 1), dict(rows=2**23 - 255, classes=1000),
-    dict(rows=2**23 - 255, dim=3), dict(rows=2**20, classes=2**18), dict(x=0), dict(weight=0),
+    dict(rows=2**23 - 255, dim=7), dict(rows=2**20, classes=2**18), dict(x=0), dict(weight=0),
     dict(targets=0), dict(work=0), dict(work=P + 128), dict(classes=50_000, size=1000)]
 
 

@@ -507,3 +507,51 @@ def test_few_classes_past_the_tiles_rows(sporder):
     got = dx[some].double() - (g[some] @ w.double())
     bound = 2.0**-8 * (g[some] @ w.double()).abs() + 2.0**-11 * (g[some].abs() @ w.double().abs())
     assert (got.abs() <= bound + 2.0**-126).all()
+
+
+@pytest.mark.parametrize("dtype, rows", [(F32, 1), (F32, 29), (F32, 64), (BF16, 20), (F16, 32)])
+def test_few_rows_that_count_nothing_are_not_read(sporder, dtype, rows):
+    """The form of few rows: NaN and infinities in ignored rows and in rows whose target is
+    no class change nothing."""
+    x, w, t, b, s = inputs(rows + 3, 200, 777, dtype, F32, 0.3, seed=rows)
+    x, t, s = x[:rows], t[:rows], s[:rows]
+    t[0] = 5
+    want, grads = both(sporder, x, w, t, b, s)
+    bad = x.clone()
+    bad[t == -100] = float("nan")
+    if (t == -100).any():
+        bad[(t == -100).nonzero()[0]] = float("inf")
+    got = sporder.linear_cross_entropy(bad, w, t, b)
+    again = sporder.linear_cross_entropy_grad(s, bad, w, t, got[1], b)
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    assert all(torch.equal(p, q) for p, q in zip(grads, again))
+    if rows > 1:
+        out = t.clone()
+        out[1] = 777
+        got = sporder.linear_cross_entropy(bad, w, out, b)
+        assert got[0][1].isnan() and got[0][0] == want[0][0]
+        dx, dw, db = sporder.linear_cross_entropy_grad(s, bad, w, out, got[1], b)
+        assert (dx[1] == 0).all() and dw.isfinite().all() and db.isfinite().all()
+
+
+def test_calls_at_once_on_two_streams(sporder):
+    """Each form on two streams at a time, each call with scratch of its own."""
+    cases = [(F32, 20, 96, 3000), (BF16, 900, 96, 3000), (F32, 5000, 96, 40), (BF16, 5000, 300, 100)]
+    for dtype, rows, dim, classes in cases:
+        sets = [inputs(rows, dim, classes, dtype, F32, 0.1, seed=k) for k in range(2)]
+        want = [both(sporder, *v) for v in sets]
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        got = [[], []]
+        for _ in range(4):
+            for k, stream in enumerate(streams):
+                x, w, t, b, s = sets[k]
+                with torch.cuda.stream(stream):
+                    loss = sporder.linear_cross_entropy(x, w, t, b)
+                    got[k].append((loss, sporder.linear_cross_entropy_grad(s, x, w, t, loss[1], b)))
+        torch.cuda.synchronize()
+        for k in range(2):
+            for loss, grads in got[k]:
+                assert all(torch.equal(p, q) for p, q in zip(loss, want[k][0]))
+                assert all(torch.equal(p, q) for p, q in zip(grads, want[k][1]))

@@ -127,21 +127,28 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, i
   if (tid == 0) most = -1000;
   int before = 0;
   if (a.rows <= kListDirect) {
-#pragma unroll 16
-    for (int64_t row = tid; row < first; row += 256)
-      before += counted(a, target_of(a, row)) ? 1 : 0;
+    constexpr int kAhead = 16;
+    for (int64_t row = tid; row < first; row += 256 * kAhead) {
+      RawTarget raw[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) raw[k] = fetch_target(a, row + k * 256);
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k)
+        before += row + k * 256 < first && class_of(a, row + k * 256, raw[k]) >= 0 ? 1 : 0;
+    }
   } else {
 #pragma unroll 4
     for (int64_t b = tid; b < blockIdx.x; b += 256) before += a.counts[b];
   }
   before = block_total(wave_total(before), part);
   constexpr int kEach = kListBlock / 256;
-  int64_t target[kEach];
+  RawTarget raw[kEach];
+  int target[kEach];
   float scale[kEach] = {}, row_lse[kEach] = {};
 #pragma unroll
   for (int k = 0; k < kEach; ++k) { // past the rows the last one
     const int64_t row = min(first + k * 256 + tid, a.rows - 1);
-    target[k] = target_of(a, row);
+    raw[k] = fetch_target(a, row);
     if (backward) {
       scale[k] = a.grad[row * a.grad_stride];
       row_lse[k] = a.given_lse[row];
@@ -150,7 +157,8 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, i
   uint64_t mask[kEach];
 #pragma unroll
   for (int k = 0; k < kEach; ++k) {
-    mask[k] = __ballot(first + k * 256 + tid < a.rows && counted(a, target[k]));
+    target[k] = class_of(a, first + k * 256 + tid, raw[k]);
+    mask[k] = __ballot(target[k] >= 0);
     if (lane == 0) placed[k][wave] = __popcll(mask[k]);
   }
   __syncthreads();
@@ -162,7 +170,7 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, i
     for (int w = 0; w < wave; ++w) at += placed[k][w];
     if (mask[k] >> lane & 1) {
       a.list[at] = static_cast<int32_t>(row);
-      a.target[at] = static_cast<int32_t>(target[k]);
+      a.target[at] = target[k];
       if (backward) {
         // |s| = m 2^e with 1 <= m < 2 (a scale below 2^-126 keeps its place in m).
         const int e = max(static_cast<int>(__builtin_bit_cast(uint32_t, scale[k]) >> 23 & 255), 1) - 127;
@@ -172,7 +180,7 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, i
         if (scale[k] != 0.0f) top = max(top, e);
       }
     } else if (row < a.rows && !backward) {
-      const float none = target[k] == a.ignore ? 0.0f : NAN;
+      const float none = target[k] == -1 ? 0.0f : NAN;
       a.loss[row] = none;
       a.lse[row] = none;
     }

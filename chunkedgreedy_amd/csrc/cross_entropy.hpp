@@ -34,6 +34,27 @@ __device__ __forceinline__ bool counted(const CeCall &a, int64_t target) {
   return target != a.ignore && target >= 0 && target < a.classes;
 }
 
+// A row's target as it lies in memory, loaded some time before it is looked at: without a
+// branch (past the rows the last one's), for a branch's end would wait for it and for
+// every load before it.
+struct RawTarget {
+  int32_t low, high;
+};
+__device__ __forceinline__ RawTarget fetch_target(const CeCall &c, int64_t row) {
+  const int words = c.target_bits / 32;
+  const int32_t *const p = static_cast<const int32_t *>(c.targets) + min(row, c.rows - 1) * words;
+  return {p[0], p[words - 1]};
+}
+
+// As a class, -1 where it counts nothing, -2 where it is no class, -3 past the rows.
+__device__ __forceinline__ int class_of(const CeCall &c, int64_t row, const RawTarget &raw) {
+  const int high = c.target_bits == 64 ? raw.high : raw.low >> 31;
+  const bool ignored = raw.low == static_cast<int>(c.ignore) && high == static_cast<int>(c.ignore >> 32);
+  const bool in = high == 0 && static_cast<uint32_t>(raw.low) < static_cast<uint32_t>(c.classes);
+  const int k = ignored ? -1 : in ? raw.low : -2;
+  return row < c.rows ? k : -3;
+}
+
 constexpr float kLog2e = 1.44269504088896340736f;
 __device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f(v * kLog2e); }
 

@@ -165,8 +165,8 @@ __device__ __forceinline__ float element_of(const void *p, int type, int64_t i) 
   return v;
 }
 
-// Rows that no workgroup's registers hold: three passes over each, by elements (256 rows of
-// 132,660 floats in 105 us, 5.2 TB/s).
+// Rows that no workgroup's registers hold: three passes over each, by elements (2,000
+// rows of 40,000 floats in 655 us, 2.0 TB/s, bfloat16 720, 0.9).
 template <typename T> __global__ void __launch_bounds__(1024) block_norm_long_kernel(BlockArgs a) {
   __shared__ float shared[2][1][1024 / kWave];
   RowSum<1024, 1> row_sum{shared};
@@ -481,8 +481,8 @@ __global__ void __launch_bounds__(kWideLanes) block_norm_grad_wide_kernel(BlockG
 }
 
 // Rows that no workgroup's registers hold: three passes over each, by elements;
-// the column sums stay in the workgroup's partial row (1,236 rows of 39,553 float16 in 199 us,
-// 2.9 TB/s).
+// the column sums stay in the workgroup's partial row (2,000 rows of 20,000 floats in 592 us,
+// 1.6 TB/s, bfloat16 757, 0.6).
 template <typename T>
 __global__ void __launch_bounds__(1024) block_norm_grad_long_kernel(BlockGradArgs a) {
   __shared__ float shared[2][1][1024 / kWave];
@@ -622,12 +622,12 @@ int64_t grad_groups(int64_t dim) {
   return norm_block(lanes) / lanes;
 }
 
-// Workgroups of the gradient, each with a partial row of 2 dim floats: at most
-// enough to fill the card, and few enough that the partial rows stay small
-// beside the rows themselves.
+// Workgroups of the gradient, each with a partial row of 2 dim floats: at most enough to fill
+// the card, few enough that the partial rows stay small beside the rows themselves (eight
+// turns of rows for each), but no fewer than the CUs while each has two turns.
 int64_t grad_blocks(int64_t rows, int64_t dim) {
-  const int64_t most = dim > 4096 ? 512 : 1024;
-  return std::max<int64_t>(1, std::min(ceil_div64(rows, 8 * grad_groups(dim)), most));
+  const int64_t most = dim > 4096 ? 512 : 1024, turns = ceil_div64(rows, grad_groups(dim));
+  return std::min(most, std::max(ceil_div64(turns, 8), std::min<int64_t>(256, ceil_div64(turns, 2))));
 }
 
 template <typename T> int32_t block_typed(const BlockArgs &a, void *stream) {

@@ -1190,7 +1190,7 @@ size_t sporder_linear_cross_entropy_work_bytes(int32_t type, int64_t rows, int64
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
   if (bad_sizes(a, false) || rows == 0) return 0;
   if (few_takes(type, dim, classes, false)) return few_work_bytes(rows, dim, classes, false);
-  if (narrow_takes(type, rows, dim, false)) return narrow_work_bytes(rows, dim, classes, false);
+  if (narrow_takes(type, rows, dim, classes, false)) return narrow_work_bytes(rows, dim, classes, false);
   return lay_out(a, false, nullptr).bytes;
 }
 
@@ -1212,7 +1212,7 @@ int32_t sporder_linear_cross_entropy(void *stream, int32_t type, int64_t rows, i
   if (few_takes(type, dim, classes, false))
     return work_bytes < few_work_bytes(rows, dim, classes, false) ? SPORDER_BAD_ARGUMENT
                                                                    : few_forward(a, d_work, stream);
-  if (narrow_takes(type, rows, dim, false))
+  if (narrow_takes(type, rows, dim, classes, false))
     return work_bytes < narrow_work_bytes(rows, dim, classes, false) ? SPORDER_BAD_ARGUMENT
                                                                       : narrow_run(a, false, d_work, stream);
   const CePlan p = lay_out(a, false, d_work);
@@ -1232,7 +1232,7 @@ size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows, 
   a.db = &a; // the scratch of a bias whether there is one or not
   if (bad_sizes(a, true) || rows == 0) return 0;
   if (few_takes(type, dim, classes, true)) return few_work_bytes(rows, dim, classes, true);
-  if (narrow_takes(type, rows, dim, true)) return narrow_work_bytes(rows, dim, classes, true);
+  if (narrow_takes(type, rows, dim, classes, true)) return narrow_work_bytes(rows, dim, classes, true);
   return lay_out(a, true, nullptr).bytes;
 }
 
@@ -1267,7 +1267,7 @@ int32_t sporder_linear_cross_entropy_grad(void *stream, int32_t type, int64_t ro
   if (few_takes(type, dim, classes, true))
     return work_bytes < few_work_bytes(rows, dim, classes, true) ? SPORDER_BAD_ARGUMENT
                                                                   : few_backward(a, d_work, stream);
-  if (narrow_takes(type, rows, dim, true))
+  if (narrow_takes(type, rows, dim, classes, true))
     return work_bytes < narrow_work_bytes(rows, dim, classes, true) ? SPORDER_BAD_ARGUMENT
                                                                      : narrow_run(a, true, d_work, stream);
   const CePlan p = lay_out(a, true, d_work);

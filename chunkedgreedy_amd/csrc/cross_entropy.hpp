@@ -112,7 +112,7 @@ int32_t few_forward(const CeCall &a, void *work, void *stream);
 int32_t few_backward(const CeCall &a, void *work, void *stream);
 
 // The form of few rows.
-bool narrow_takes(int type, int64_t rows, int64_t dim, bool backward);
+bool narrow_takes(int type, int64_t rows, int64_t dim, int64_t classes, bool backward);
 size_t narrow_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward);
 int32_t narrow_run(const CeCall &a, bool backward, void *work, void *stream);
 

@@ -368,11 +368,14 @@ template <typename T> int32_t narrow_typed(const NarrowArgs &a, bool backward, v
 
 // Measured both ways.  32-bit types: 50,000 x 4,096, one row 243 us and the tiles 648 (with the
 // gradients 668 and 1,646), 30,000 x 4,096, 64 rows 302 and 449 (791 and 1,153).  16-bit
-// types, whose w the tiles read as it is: forward 164 and 106 us for one row, 156 and 65 for 64,
-// so never; with the gradients 491 and 812, 16 rows of 50,000 x 2,048 268 and 443, but 64 rows
-// 627 and 531.
-bool narrow_takes(int type, int64_t rows, int64_t dim, bool backward) {
-  return dim >= 8 && rows <= (type == SPORDER_TYPE_F32 ? 64 : backward ? 32 : 0);
+// types, whose w the tiles read as it is: forward 164 and 106 us for one row of the first, 156
+// and 65 for 64, but 35 and 37 for up to 32 rows of 16,000 x 2,048 and 24 and 28 of 1,000 x 512
+// (three launches instead of five); with the gradients 491 and 812, 16 rows of 50,000 x 2,048
+// 268 and 443, but 64 rows 627 and 531.
+bool narrow_takes(int type, int64_t rows, int64_t dim, int64_t classes, bool backward) {
+  if (dim < 8) return false;
+  if (type == SPORDER_TYPE_F32) return rows <= 64;
+  return rows <= 32 && (backward || classes * dim <= int64_t(1) << 25);
 }
 
 size_t narrow_work_bytes(int64_t rows, int64_t dim, int64_t classes, bool backward) {

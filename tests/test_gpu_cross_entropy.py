@@ -555,3 +555,12 @@ def test_calls_at_once_on_two_streams(sporder):
             for loss, grads in got[k]:
                 assert all(torch.equal(p, q) for p, q in zip(loss, want[k][0]))
                 assert all(torch.equal(p, q) for p, q in zip(grads, want[k][1]))
+
+
+@pytest.mark.parametrize("rows", [1, 32, 50])
+@pytest.mark.parametrize("dim", [1024, 1003])
+def test_few_rows_of_large_weights(sporder, rows, dim):
+    """16-bit weights on either side of 2^25 elements, which few rows take in two forms."""
+    for classes in (34_001, 3001):
+        x, w, t, b, s = inputs(rows, dim, classes, BF16, BF16, 0.1, seed=rows + dim)
+        both(sporder, x, w, t, b, s)

@@ -275,6 +275,29 @@ __global__ void __launch_bounds__(256)
   }
 }
 
+// COUNT accesses of rows whose places are given, at column `col` or, past the rows' ends, the
+// rows' last elements: `at` is where that is.  Without a branch at each, which would make the
+// next access wait for it.
+template <int VEC, int COUNT, typename T>
+__device__ __forceinline__ void fetch_columns(const T *src, const int64_t (&place)[COUNT], int64_t stride,
+                                              int64_t dim, int64_t col, int64_t &at, Pack<T, VEC> (&q)[COUNT]) {
+  at = dim >= VEC ? min(col, dim - VEC) : col;
+  if (dim >= VEC) {
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k)
+      q[k] = __builtin_bit_cast(Pack<T, VEC>,
+                                *reinterpret_cast<const LoosePack<T, VEC> *>(src + place[k] * stride + at));
+  } else {
+#pragma unroll
+    for (int k = 0; k < COUNT; ++k) q[k] = fetch<true, VEC>(src + place[k] * stride + at, dim - at);
+  }
+}
+template <int COUNT> __device__ __forceinline__ void listed(const int32_t *list, int64_t (&place)[COUNT]) {
+  if (!list) return;
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) place[k] = list[place[k]];
+}
+
 // The largest element of each column of rows of x (listed) or w: a strip of rows and 64
 // accesses' columns per workgroup, then the strips'.  (One atomic maximum per strip and
 // column instead: 206 us for 50,000 rows of 2,048 16-bit elements.)  Workgroups past both
@@ -308,14 +331,15 @@ __global__ void __launch_bounds__(256)
   }
   const int64_t col = (blockIdx.x * int64_t(kWave) + x) * kVec, step = a.blocks * 4;
   float m[kVec] = {};
+  int64_t at = col;
   if (col < dim) {
     for (int64_t r0 = (blockIdx.y - (first ? 0 : ax.blocks)) * 4 + y; r0 < all; r0 += step * kAhead) {
-      Pack<T, kVec> q[kAhead];
+      int64_t place[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) { // past the rows the first again
-        const int64_t r = r0 + k * step < all ? r0 + k * step : r0;
-        q[k] = fetch<true, kVec>(src + (list ? list[r] : r) * stride + col, dim - col);
-      }
+      for (int k = 0; k < kAhead; ++k) place[k] = min(r0 + k * step, all - 1); // the last row again
+      listed(list, place);
+      Pack<T, kVec> q[kAhead];
+      fetch_columns<kVec>(src, place, stride, dim, col, at, q);
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) {
 #pragma unroll
@@ -323,14 +347,15 @@ __global__ void __launch_bounds__(256)
       }
     }
   }
+  if (dim >= kVec) at = min(col, dim - kVec); // also where no row was
 #pragma unroll
   for (int e = 0; e < kVec; ++e) part[y][e][x] = m[e];
   __syncthreads();
   if (y != 0) return;
 #pragma unroll
   for (int e = 0; e < kVec; ++e)
-    if (col + e < dim)
-      most[blockIdx.y * dim + col + e] =
+    if (col < dim && at + e < dim)
+      most[blockIdx.y * dim + at + e] =
           fmaxf(fmaxf(part[0][e][x], part[1][e][x]), fmaxf(part[2][e][x], part[3][e][x]));
 }
 
@@ -355,7 +380,7 @@ __global__ void __launch_bounds__(256)
 
 // Columns of rows of x (listed) or w as operand rows: out[j][k] of k-th row,
 // zeros for k past the rows up to a multiple of 64.  64 x 64 per workgroup,
-// turned in LDS (25,000 rows of 2,048 bfloat16 62 us, 3.3 TB/s).  Listed rows come with 2^(their exponent - the largest).
+// turned in LDS (25,000 rows of 2,048 bfloat16 49 us, 4.2 TB/s).  Listed rows come with 2^(their exponent - the largest).
 template <typename T, int PLANES>
 __global__ void __launch_bounds__(256)
     ce_pack_columns_kernel(CeRows ax, CeRows aw, int64_t dim, const CeMeta *meta, const int32_t *exponent) {
@@ -376,16 +401,18 @@ __global__ void __launch_bounds__(256)
   const int64_t col = j0 + x;
   Pack<T, kVec> q[kRounds];
   int power[kRounds] = {};
+  int64_t place[kRounds], at;
 #pragma unroll
-  for (int i = 0; i < kRounds; ++i) {
-    const int64_t k = min(k0 + y + i * kRound, all - 1);
-    q[i] = {};
-    if (col < dim) q[i] = fetch<true, kVec>(src + (list ? list[k] : k) * stride + col, dim - col);
-    if (list) power[i] = min(exponent[k] - top, 0); // no row has a scale: top is below all
+  for (int i = 0; i < kRounds; ++i) place[i] = min(k0 + y + i * kRound, all - 1);
+  if (list) {
+#pragma unroll
+    for (int i = 0; i < kRounds; ++i) power[i] = min(exponent[place[i]] - top, 0); // no row has a scale: top is below all
   }
+  listed(list, place);
+  fetch_columns<kVec>(src, place, stride, dim, min(col, dim - 1), at, q);
   float scale[kVec];
 #pragma unroll
-  for (int e = 0; e < kVec; ++e) scale[e] = unit_inverse(unit_of(most[min(col + e, dim - 1)]));
+  for (int e = 0; e < kVec; ++e) scale[e] = unit_inverse(unit_of(most[min(at + e, dim - 1)]));
 #pragma unroll
   for (int i = 0; i < kRounds; ++i) {
     const int r = y + i * kRound;
@@ -393,7 +420,8 @@ __global__ void __launch_bounds__(256)
     for (int e = 0; e < kVec; ++e) {
       float v = static_cast<float>(q[i].v[e]) * scale[e];
       if (list) v = ldexpf(v, power[i]);
-      tile[r][x + e] = k0 + r < all ? v : 0.0f;
+      const int64_t j = at + e - j0; // an access at the end may begin before the tile
+      if (j >= 0 && j < 64) tile[r][j] = k0 + r < all ? v : 0.0f;
     }
   }
   __syncthreads();

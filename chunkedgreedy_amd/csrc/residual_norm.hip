@@ -210,8 +210,8 @@ template <typename T> __global__ void __launch_bounds__(1024) block_norm_long_ke
 }
 
 // 2,449,029 rows of 128 floats in 1,472 us (5.1 TB/s), 16,384 of 4,096 bfloat16 with a gate by
-// row in 211 (5.1 TB/s); rows of 16-bit elements of odd length, whose accesses are loose, some
-// 3 TB/s.
+// row in 211 (5.1 TB/s); rows of 16-bit elements of odd length, whose accesses are loose, 1.8 to
+// 2.7 TB/s.
 // The gradients by element, and the workgroup's sums over its rows by column,
 // kept in registers and written as one row of partial sums at the end.  No
 // atomics: the order of every sum is fixed by the grid.

@@ -583,9 +583,8 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeArgs a) {
   const float base = most == -INFINITY ? 0.0f : most;
   sum = 0.0f;
   for (int k = 0; k < 16; ++k) sum += part[k][x].y * exp_of(part[k][x].x - base);
-  const float lse = base + logf(sum);
-  a.lse[a.list[n]] = lse;
-  a.loss[a.list[n]] = lse - a.hit[n];
+  a.lse[a.list[n]] = base + logf(sum);
+  a.loss[a.list[n]] = loss_of(base, sum, a.hit[n]);
 }
 
 // The losses' sum and the number of rows not ignored, in 64 bits and a fixed

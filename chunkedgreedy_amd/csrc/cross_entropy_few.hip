@@ -339,7 +339,7 @@ __global__ void __launch_bounds__(kGradThreads, 2 * loss_groups<T>(VB, DB)) few_
     total += lane_xor_f32(total, 32);
     hit += lane_xor_f32(hit, 32);
     if (lane < 16 && at > -3) {
-      float lse = base + logf(total), loss = lse - hit;
+      float lse = base + logf(total), loss = loss_of(base, total, hit);
       if (at < 0) loss = lse = at == -1 ? 0.0f : NAN;
       c.lse[row] = lse;
       c.loss[row] = loss;

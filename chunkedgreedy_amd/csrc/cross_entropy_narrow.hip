@@ -180,9 +180,9 @@ __global__ void __launch_bounds__(256) narrow_join_kernel(NarrowArgs a, int rows
   if (threadIdx.x != 0) return;
   for (int k = 1; k < 4; ++k) join(part[k].x, part[k].y);
   const int at = class_at(c, row);
-  const float lse = (most == -INFINITY ? 0.0f : most) + logf(sum);
-  c.lse[row] = at >= 0 ? lse : at == -1 ? 0.0f : NAN;
-  c.loss[row] = at >= 0 ? lse - a.hit[row] : at == -1 ? 0.0f : NAN;
+  const float base = most == -INFINITY ? 0.0f : most;
+  c.lse[row] = at >= 0 ? base + logf(sum) : at == -1 ? 0.0f : NAN;
+  c.loss[row] = at >= 0 ? loss_of(base, sum, a.hit[row]) : at == -1 ? 0.0f : NAN;
 }
 
 __global__ void __launch_bounds__(kWave) narrow_sums_kernel(NarrowArgs a) {

@@ -166,6 +166,9 @@ SIGNATURES = {
     "sporder_linear_cross_entropy_grad": (
         [vp, i32, i64, i64, i64, i64, vp, i64, vp, i64, vp, i32, vp, i32, vp, i64, vp, i64, vp, i32,
          i64, vp, vp, vp, sz], i32),
+    "sporder_linear_cross_entropy_grad_of_loss": (
+        [vp, i32, i64, i64, i64, i64, vp, i64, vp, i64, vp, i32, vp, i32, vp, i64, vp, vp, i64, vp,
+         i32, i64, vp, vp, vp, sz], i32),
     "sporder_hbm_stream": ([vp, i32, i32, vp, vp, ctypes.c_int64, i32, P(f32)], None),
 }
 

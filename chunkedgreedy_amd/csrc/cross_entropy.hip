@@ -51,7 +51,7 @@ struct CeArgs : CeCall {
   int32_t *counts;       // of the list's blocks, past kListDirect rows
   int32_t *list, *target; // of the listed rows
   int32_t *exponent;
-  float *mantissa, *row_lse;
+  float *mantissa, *row_lse, *miss; // miss_of
   float *bias32;      // [classes_pad], -inf past the classes
   float *hit;         // the target's logit
   float2 *partial;    // [chunks][rows_pad] largest and sum
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, i
   constexpr int kEach = kListBlock / 256;
   RawTarget raw[kEach];
   int target[kEach];
-  float scale[kEach] = {}, row_lse[kEach] = {};
+  float scale[kEach] = {}, row_lse[kEach] = {}, row_loss[kEach] = {};
 #pragma unroll
   for (int k = 0; k < kEach; ++k) { // past the rows the last one
     const int64_t row = min(first + k * 256 + tid, a.rows - 1);
@@ -152,6 +152,7 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, i
     if (backward) {
       scale[k] = a.grad[row * a.grad_stride];
       row_lse[k] = a.given_lse[row];
+      row_loss[k] = fetch_loss(a, row);
     }
   }
   uint64_t mask[kEach];
@@ -177,6 +178,7 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, i
         a.exponent[at] = e;
         a.mantissa[at] = ldexpf(scale[k], -e);
         a.row_lse[at] = row_lse[k];
+        a.miss[at] = miss_of(a, row_loss[k]);
         if (scale[k] != 0.0f) top = max(top, e);
       }
     } else if (row < a.rows && !backward) {
@@ -205,6 +207,7 @@ __global__ void __launch_bounds__(256) ce_list_kernel(CeArgs a, bool backward, i
       a.exponent[at] = 0;
       a.mantissa[at] = 0.0f;
       a.row_lse[at] = 0.0f;
+      a.miss[at] = 1.0f;
     }
   }
 }
@@ -638,7 +641,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
   const int wm = wave / S::WN, wn = wave % S::WN;
   f32x16 acc[S::MB][S::NB] = {};
   logit_tile<U, PLANES, S>(a, lds, wave, m0, n0, v0, count, acc);
-  float lse[S::NB], m[S::NB], grad[S::NB];
+  float lse[S::NB], miss[S::NB], m[S::NB], grad[S::NB];
   int target[S::NB];
 #pragma unroll
   for (int j = 0; j < S::NB; ++j) {
@@ -646,6 +649,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
     const bool on = n < count;
     target[j] = register_of<S::MB>(on ? a.target[n] - static_cast<int>(v0 + m0) - wm * S::MB * 32 : -1);
     lse[j] = on ? a.row_lse[n] : 0.0f;
+    miss[j] = on ? a.miss[n] : 1.0f;
     m[j] = on ? a.mantissa[n] * (1 << kShift) : 0.0f;
     grad[j] = on ? ldexpf(a.mantissa[n], a.exponent[n]) : 0.0f;
   }
@@ -656,7 +660,7 @@ __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0)
     for (int j = 0; j < S::NB; ++j) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        float g = exp_of(acc[i][j][r] - lse[j]) - (target[j] == i * 16 + r ? 1.0f : 0.0f);
+        float g = less_target(exp_of(acc[i][j][r] - lse[j]), target[j] == i * 16 + r, miss[j]);
         g = n0 + (wn * S::NB + j) * 32 + lane % 32 < count ? g : 0.0f; // the product is of another row
         total[r] += g * grad[j];
         acc[i][j][r] = g * m[j];
@@ -1021,6 +1025,7 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     take(a.exponent, a.rows_pad);
     take(a.mantissa, a.rows_pad);
     take(a.row_lse, a.rows_pad);
+    take(a.miss, a.rows_pad);
     cut_gradients(a.dim, a.rows, std::min(a.piece, a.classes), p.dx, p.dw);
     take(a.x_most, a.dim);
     take(a.w_most, a.dim);
@@ -1263,21 +1268,18 @@ size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows, 
   return lay_out(a, true, nullptr).bytes;
 }
 
-int32_t sporder_linear_cross_entropy_grad(void *stream, int32_t type, int64_t rows, int64_t dim,
-                                          int64_t classes, int64_t grad_stride, const float *d_grad,
-                                          int64_t x_stride, const void *d_x, int64_t weight_stride,
-                                          const void *d_weight, int32_t bias_type,
-                                          const void *d_bias, int32_t target_bits,
-                                          const void *d_targets, int64_t ignore_index,
-                                          const float *d_lse, int64_t dx_stride, void *d_dx,
-                                          int32_t dweight_type, int64_t dweight_stride,
-                                          void *d_dweight, void *d_dbias, void *d_work,
-                                          size_t work_bytes) {
+int32_t sporder_linear_cross_entropy_grad_of_loss(
+    void *stream, int32_t type, int64_t rows, int64_t dim, int64_t classes, int64_t grad_stride,
+    const float *d_grad, int64_t x_stride, const void *d_x, int64_t weight_stride, const void
+    *d_weight, int32_t bias_type, const void *d_bias, int32_t target_bits, const void *d_targets,
+    int64_t ignore_index, const float *d_lse, const float *d_loss, int64_t dx_stride, void *d_dx,
+    int32_t dweight_type, int64_t dweight_stride, void *d_dweight, void *d_dbias, void *d_work,
+    size_t work_bytes) {
   CeArgs a{};
   a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = target_bits;
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
   a.bias_type = bias_type, a.bias = d_bias, a.targets = d_targets, a.ignore = ignore_index;
-  a.grad = d_grad, a.grad_stride = grad_stride, a.given_lse = d_lse;
+  a.grad = d_grad, a.grad_stride = grad_stride, a.given_lse = d_lse, a.given_loss = d_loss;
   a.dx = d_dx, a.dx_stride = dx_stride, a.dw = d_dweight, a.dw_stride = dweight_stride;
   a.dw_type = dweight_type, a.db = d_dbias;
   if (bad_sizes(a, true) || (dweight_type != type && dweight_type != SPORDER_TYPE_F32) || grad_stride < 0 ||
@@ -1302,6 +1304,22 @@ int32_t sporder_linear_cross_entropy_grad(void *stream, int32_t type, int64_t ro
   if (type == SPORDER_TYPE_BF16) return backward<bf16_t, bf16_t, 1>(a, p, stream);
   if (type == SPORDER_TYPE_F16) return backward<f16_t, f16_t, 1>(a, p, stream);
   return backward<float, f16_t, 2>(a, p, stream);
+}
+
+int32_t sporder_linear_cross_entropy_grad(void *stream, int32_t type, int64_t rows, int64_t dim,
+                                          int64_t classes, int64_t grad_stride, const float *d_grad,
+                                          int64_t x_stride, const void *d_x, int64_t weight_stride,
+                                          const void *d_weight, int32_t bias_type,
+                                          const void *d_bias, int32_t target_bits,
+                                          const void *d_targets, int64_t ignore_index,
+                                          const float *d_lse, int64_t dx_stride, void *d_dx,
+                                          int32_t dweight_type, int64_t dweight_stride,
+                                          void *d_dweight, void *d_dbias, void *d_work,
+                                          size_t work_bytes) {
+  return sporder_linear_cross_entropy_grad_of_loss(
+      stream, type, rows, dim, classes, grad_stride, d_grad, x_stride, d_x, weight_stride, d_weight,
+      bias_type, d_bias, target_bits, d_targets, ignore_index, d_lse, nullptr, dx_stride, d_dx,
+      dweight_type, dweight_stride, d_dweight, d_dbias, d_work, work_bytes);
 }
 
 } // extern "C"

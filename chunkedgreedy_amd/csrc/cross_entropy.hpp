@@ -19,7 +19,7 @@ struct CeCall {
   // forward
   float *loss, *lse, *sums;
   // backward
-  const float *grad, *given_lse;
+  const float *grad, *given_lse, *given_loss; // the loss may be null
   int64_t grad_stride;
   void *dx, *dw, *db;
   int64_t dx_stride, dw_stride;
@@ -63,6 +63,22 @@ __device__ __forceinline__ float exp_of(float v) { return __builtin_amdgcn_exp2f
 // have half a step of lse's (60 beside a rival 12 below: 6.1e-6 would come out as 7.6e-6).
 __device__ __forceinline__ float loss_of(float base, float sum, float hit) {
   return (base - hit) + logf(sum);
+}
+
+// Backward, the target's exp(z - lse) - 1 = e^-loss - 1: made of the loss where it is given,
+// else 1 (no such value) and the caller makes it of lse, whose half step is all that a sure
+// row's has left.
+__device__ __forceinline__ float miss_of(const CeCall &c, float loss) {
+  return c.given_loss ? expm1f(-loss) : 1.0f;
+}
+// exp(z - lse) - [target] of a class.
+__device__ __forceinline__ float less_target(float p, bool is_target, float miss) {
+  const float t = miss <= 0.0f ? miss : p - 1.0f;
+  return is_target ? t : p;
+}
+// A row's given loss, or something to load in its place: without a branch.
+__device__ __forceinline__ float fetch_loss(const CeCall &c, int64_t row) {
+  return (c.given_loss ? c.given_loss : c.given_lse)[row];
 }
 
 // Sums of two values over a workgroup of WAVES waves, in 64 bits and a fixed order, in its

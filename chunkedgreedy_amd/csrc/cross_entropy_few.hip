@@ -374,8 +374,9 @@ constexpr int kRows = 32, kSplit = 4; // waves that share a block of 16 rows
 // dx of a tile goes out a tile later, by whole rows through LDS.  (Stored from the
 // accumulators, 64 bytes of 16 rows at a time, it took a third of the kernel's time; stored at
 // the tile's end, the next tile's loads waited for it.)
+// (Past four blocks of features LDS holds one workgroup a CU, which may have all registers.)
 template <typename T, int VB, int DB>
-__global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB < 8 ? 4 : 2) few_grad_kernel(FewArgs a) {
+__global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB < 6 ? 4 : 2) few_grad_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   constexpr int kMine = (VB + kSplit - 1) / kSplit;
   constexpr int kG = VB * 16 + 4;  // floats of a row of g
@@ -428,6 +429,7 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
   for (; tile < a.tiles; tile += gridDim.x) {
     __syncthreads(); // x is read no more, the last tile's dx is there
     put_tile<T, 32>(c, x, target, next);
+    const float loss = fetch_loss(c, min(row, c.rows - 1)); // before the next tile's, to wait for none of them
     __syncthreads();
     classes_of<32>(c, tile * kRows + step, next_target, target);
     fetch_tile<T, 32>(c, tile * kRows + step, target, next);
@@ -441,6 +443,7 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
     f32x4 z[kMine] = {};
     logits<kMine, kSplit, DB>(w + part * 16 * stride, x + tb * 16 * stride, dim16,
                               (VB - part + kSplit - 1) / kSplit, z);
+    const float miss = miss_of(c, loss);
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int v = (i * kSplit + part) * 16 + q * 4;
@@ -448,7 +451,7 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
       const f32x4 b = *reinterpret_cast<const f32x4 *>(bias + v);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p = exp_of(z[i][e] + b[e] - lse) - (v + e == at ? 1.0f : 0.0f);
+        const float p = less_target(exp_of(z[i][e] + b[e] - lse), v + e == at, miss);
         z[i][e] = at >= 0 ? p * s : 0.0f;
       }
       *reinterpret_cast<f32x4 *>(g + (tb * 16 + l) * kG + v) = z[i];
@@ -620,11 +623,12 @@ __global__ void __launch_bounds__(kGradThreads, 2) few_grad_wave_kernel(FewArgs 
     }
   };
   RawTarget next_class;
-  float next_lse, next_scale;
+  float next_lse, next_loss, next_scale;
   auto fetch_row = [&](int64_t r) {
     next_class = fetch_target(c, r);
     const int64_t in = min(r, c.rows - 1);
     next_lse = c.given_lse[in];
+    next_loss = fetch_loss(c, in);
     next_scale = c.grad[in * c.grad_stride];
   };
   targets_from(first);
@@ -660,7 +664,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) few_grad_wave_kernel(FewArgs 
     rows_from(r0 + step);
     targets_from(r0 + 2 * step);
     const int at = class_of(c, r0 + l, next_class);
-    const float lse = at >= 0 ? next_lse : 0.0f, scale = next_scale;
+    const float lse = at >= 0 ? next_lse : 0.0f, miss = miss_of(c, next_loss), scale = next_scale;
     fetch_row(r0 + step + l);
 
     // z, and g of them.
@@ -700,7 +704,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) few_grad_wave_kernel(FewArgs 
       f32x4 out;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float p = exp_of(z[b][e] * (unit * u[e]) + add[e] - lse) - (v + e == at ? 1.0f : 0.0f);
+        const float p = less_target(exp_of(z[b][e] * (unit * u[e]) + add[e] - lse), v + e == at, miss);
         const float held = at >= 0 ? p : 0.0f, much = held * 8192.0f;
         out[e] = at >= 0 ? held * scale : 0.0f;
         const f16_t h = static_cast<f16_t>(much);

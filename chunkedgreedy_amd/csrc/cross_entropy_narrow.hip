@@ -132,11 +132,11 @@ __global__ void __launch_bounds__(kThreads) narrow_logit_kernel(NarrowArgs a) {
       if (h == 0) a.partial[v0 / kBlock * (TB * 32) + row] = make_float2(most, sum);
     } else {
       const int64_t in = min(row, c.rows - 1);
-      const float lse = c.given_lse[in], scale = c.grad[in * c.grad_stride];
+      const float lse = c.given_lse[in], miss = miss_of(c, fetch_loss(c, in)), scale = c.grad[in * c.grad_stride];
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         const int64_t v = v0 + result_row(r);
-        const float p = exp_of(z[r] - lse) - (v == at ? 1.0f : 0.0f);
+        const float p = less_target(exp_of(z[r] - lse), v == at, miss);
         const float g = at >= 0 ? p * scale : 0.0f;
         a.g[v * (TB * 32) + row] = g;
         db[r] += g;

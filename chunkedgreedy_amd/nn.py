@@ -147,20 +147,20 @@ class _LinearCrossEntropy(torch.autograd.Function):
     def forward(ctx, x, weight, targets, bias, ignore_index, reduction):
         loss, lse, sums = sporder.linear_cross_entropy(x, weight, targets, bias,
                                                        ignore_index=ignore_index)
-        ctx.save_for_backward(x, weight, targets, bias, lse, sums)
+        ctx.save_for_backward(x, weight, targets, bias, lse, sums, loss)
         ctx.ignore_index, ctx.reduction = ignore_index, reduction
         if reduction == "none":
-            return loss
+            return loss.clone()  # the caller may write to it, and the backward pass reads this one
         return sums[0] / sums[1] if reduction == "mean" else sums[0].clone()
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad):
-        x, weight, targets, bias, lse, sums = ctx.saved_tensors
+        x, weight, targets, bias, lse, sums, loss = ctx.saved_tensors
         if ctx.reduction == "mean":
             grad = grad / sums[1]
         dx, dweight, dbias = sporder.linear_cross_entropy_grad(
-            grad, x, weight, targets, lse, bias, ignore_index=ctx.ignore_index)
+            grad, x, weight, targets, lse, bias, ignore_index=ctx.ignore_index, loss=loss)
         return dx, dweight, None, dbias, None, None
 
 

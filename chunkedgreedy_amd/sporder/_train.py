@@ -646,7 +646,7 @@ def linear_cross_entropy(x, weight, targets, bias=None, *, ignore_index=-100):
 
 
 def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignore_index=-100,
-                              dtype=None):
+                              dtype=None, loss=None):
     """Gradients of :func:`linear_cross_entropy` by x, weight and bias.
 
     Arguments:
@@ -655,23 +655,28 @@ def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignor
         x, weight, targets, bias, ignore_index: as in the forward call
         lse: as it returned it
         dtype: weight's type (default) or float32, the type of weight's gradient
+        loss: as the forward call returned it, or None; with it the target's g is
+            made of the loss rather than of lse, whose rounding is more than all
+            of it for rows that are sure of their target
 
     Returns (dx, dweight, dbias), dbias None without a bias.  The logits are
     made again, a piece of the classes at a time; rows that are ignored, or
     whose target is no class, have no gradient.  g = grad (exp(z - lse) -
     [target]) keeps 11 bits or more in its products with weight and x (22 for
-    float32), whose sums are held in 32 bits.  The same call gives the same bits
+    float32; nothing below 2^-38 of grad), whose sums are held in 32 bits.  The same call gives the same bits
     from run to run.
     """
     x, x_stride, weight, weight_stride, targets, bias = _loss_inputs(x, weight, targets, bias)
     ignore_index = _ignored(ignore_index)
     rows, (classes, dim) = targets.numel(), weight.shape
-    for t, name in ((grad, "grad"), (lse, "lse")):
+    for t, name in ((grad, "grad"), (lse, "lse"), (loss, "loss")):
+        if t is None and name == "loss":
+            continue
         if not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or not t.is_cuda:
             raise TypeError(f"{name} must be a float32 GPU tensor")
         _same_device(t, x, name)
-    if lse.shape != targets.shape:
-        raise ValueError("lse must have the targets' shape")
+        if name != "grad" and t.shape != targets.shape:
+            raise ValueError(f"{name} must have the targets' shape")
     if grad.shape != targets.shape and grad.numel() != 1:
         raise ValueError("grad must have the targets' shape or one element")
     if dtype is None:
@@ -679,6 +684,8 @@ def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignor
     elif dtype not in (weight.dtype, torch.float32):
         raise ValueError("dtype must be weight's type or float32")
     lse = lse if lse.is_contiguous() else lse.contiguous()
+    if loss is not None and not loss.is_contiguous():
+        loss = loss.contiguous()
     one = grad.numel() == 1 or all(s == 0 for s in grad.stride())
     if not one and not grad.is_contiguous():
         grad = grad.contiguous()
@@ -690,10 +697,10 @@ def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignor
                       classes, x_stride, x.data_ptr() % 16, weight_stride,
                       weight.data_ptr() % 16)
     work = x.new_empty(size, dtype=torch.uint8) if size else None
-    _call("sporder_linear_cross_entropy_grad", x, _TYPES[x.dtype], rows, dim, classes,
+    _call("sporder_linear_cross_entropy_grad_of_loss", x, _TYPES[x.dtype], rows, dim, classes,
           0 if one else 1, grad.data_ptr(), *sizes,
           _TYPES[x.dtype if bias is None else bias.dtype], _address(bias),
-          _TOKEN_BITS[targets.dtype], targets.data_ptr(), ignore_index, lse.data_ptr(), dim,
-          dx.data_ptr(), _TYPES[dtype], dim, dweight.data_ptr(), _address(dbias), _address(work),
-          size)
+          _TOKEN_BITS[targets.dtype], targets.data_ptr(), ignore_index, lse.data_ptr(),
+          _address(loss), dim, dx.data_ptr(), _TYPES[dtype], dim, dweight.data_ptr(), _address(dbias),
+          _address(work), size)
     return dx, dweight, dbias

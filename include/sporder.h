@@ -602,7 +602,7 @@ SPORDER_API int32_t sporder_linear_cross_entropy(
  * dweight_type: `type` or SPORDER_TYPE_F32) and, where not NULL, d_dbias = sum_t g (of
  * bias_type).  d_grad has elements grad_stride apart (0: one for all rows); d_lse is the
  * forward call's.  Operands of these products keep 11 bits for 16-bit types (g too) and 22
- * for 32-bit ones; sums are held in 32 bits.
+ * for 32-bit ones, g nothing below 2^-38 of its row's grad; sums are held in 32 bits.
  */
 SPORDER_API size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows,
                                                                 int64_t dim, int64_t classes,
@@ -617,6 +617,19 @@ SPORDER_API int32_t sporder_linear_cross_entropy_grad(
     const void *d_targets, int64_t ignore_index, const float *d_lse, int64_t dx_stride, void *d_dx,
     int32_t dweight_type, int64_t dweight_stride, void *d_dweight, void *d_dbias, void *d_work,
     size_t work_bytes);
+
+/*
+ * The same with the forward call's d_loss too, of which the target's exp(z - lse) - 1 is made
+ * as e^-loss - 1.  Made of lse alone it is off by the rounding of lse (up to 2^-24 |lse|),
+ * which is more than itself for rows that are sure of their target.
+ */
+SPORDER_API int32_t sporder_linear_cross_entropy_grad_of_loss(
+    void *stream, int32_t type, int64_t rows, int64_t dim, int64_t classes, int64_t grad_stride,
+    const float *d_grad, int64_t x_stride, const void *d_x, int64_t weight_stride,
+    const void *d_weight, int32_t bias_type, const void *d_bias, int32_t target_bits,
+    const void *d_targets, int64_t ignore_index, const float *d_lse, const float *d_loss,
+    int64_t dx_stride, void *d_dx, int32_t dweight_type, int64_t dweight_stride, void *d_dweight,
+    void *d_dbias, void *d_work, size_t work_bytes);
 
 #ifdef __cplusplus
 }

@@ -11,10 +11,14 @@
 // writes its tokens' largest logit and sum of exponentials over its classes, and
 // the target's logit where it meets it; a second kernel joins the pieces.
 //
-// Backward.  For a piece of the classes at a time the logits are made again and
-// become g, in 16 bits and in both orders, since both products that follow sum
-// along another side of it; the piece's rows of dw are then final and dx is
-// summed over the pieces in 32 bits.  The pieces' size bounds the scratch.
+// Backward.  For a piece of the rows and of the classes at a time the logits are made
+// again and become g, in 16 bits and in both orders, since both products that follow sum
+// along another side of it.  dx is summed over the pieces of the classes in 32 bits and final
+// with each piece of the rows; dw is final with each piece of the classes, or, where the
+// rows are cut too, summed over their pieces in 32 bits.  What the pieces hold is bounded
+// (kPieceBytes each of g in either order and of the rows and classes turned for the
+// products), so that beside them the scratch is w packed (where it is not read as it lies)
+// and, over cut rows, dw in 32 bits.
 //
 // Types.  The matrix units take 16 bits.  The logits' operands are x and w themselves
 // where those are 16 bits wide.  g is rounded to float16 before its products whatever
@@ -67,8 +71,18 @@ struct CeArgs : CeCall {
   float *dx_part;     // [splits][rows_pad][dim_pad]
   float *dw_part;     // [splits][piece][dim_pad]
   float *db_part;     // [token chunks][piece]
+  float *dw_sum, *db_sum; // of the pieces of the rows so far, [classes][dim_pad] and [classes]; or null
   int64_t rows_pad, dim_pad, classes_pad, chunks, piece;
+  // A piece of the rows: the listed ones from `skip` on, at most `rows` of them; list, target,
+  // exponent, mantissa, row_lse and miss begin there, rows_pad is the piece's.
+  int64_t skip;
+  bool last; // of the pieces
 };
+
+__device__ __forceinline__ int listed_here(const CeMeta *meta, int64_t skip, int64_t most) {
+  return static_cast<int>(min(max(meta->count - skip, int64_t(0)), most));
+}
+__device__ __forceinline__ int listed_here(const CeArgs &a) { return listed_here(a.meta, a.skip, a.rows); }
 
 // ---- the list of rows, and what else comes first -----------------------------------
 
@@ -224,7 +238,8 @@ template <typename U> __device__ __forceinline__ void split(float v, U &hi, U &l
 struct CeRows {
   const void *src;
   int64_t stride, rows;
-  const int32_t *list; // of x
+  const int32_t *list; // of x, from `skip` on
+  int64_t skip;
   char *out;
   int64_t out_stride, plane; // bytes
   float *unit;               // of rows (32-bit types)
@@ -241,7 +256,7 @@ __global__ void __launch_bounds__(256)
   const CeRows &a = first ? x : w;
   const int64_t row = (blockIdx.x - (first ? 0 : x.blocks)) * int64_t(4) + threadIdx.x / kWave;
   const int32_t *const list = a.list;
-  if (row >= (list ? meta->count : a.rows)) return;
+  if (row >= (list ? listed_here(meta, a.skip, a.rows) : a.rows)) return;
   const T *const from = static_cast<const T *>(a.src) + (list ? list[row] : row) * a.stride;
   const int64_t out_stride = a.out_stride, plane = a.plane;
   char *const out = a.out;
@@ -315,7 +330,7 @@ __global__ void __launch_bounds__(256)
   const CeRows &a = first ? ax : aw;
   const T *const src = static_cast<const T *>(a.src);
   const int32_t *const list = a.list;
-  const int64_t all = list ? c.meta->count : a.rows, stride = a.stride, dim = c.dim;
+  const int64_t all = list ? listed_here(c) : a.rows, stride = a.stride, dim = c.dim;
   const int x = threadIdx.x % kWave, y = threadIdx.x / kWave;
   if (blockIdx.y >= ax.blocks + aw.blocks) {
     const int64_t before = ax.blocks + aw.blocks;
@@ -395,7 +410,7 @@ __global__ void __launch_bounds__(256)
   const float *const most = a.most;
   char *const out = a.out;
   const int64_t stride = a.stride, out_stride = a.out_stride, plane = a.plane;
-  const int64_t all = list ? meta->count : a.rows;
+  const int64_t all = list ? listed_here(meta, a.skip, a.rows) : a.rows;
   const int64_t k0 = (blockIdx.x - (first ? 0 : ax.blocks)) * int64_t(64), j0 = blockIdx.y * int64_t(64);
   if (k0 >= all) return;
   constexpr int kVec = 16 / sizeof(T), kAcross = 64 / kVec, kRound = 256 / kAcross, kRounds = 64 / kRound;
@@ -523,7 +538,7 @@ __device__ __forceinline__ void logit_tile(const CeArgs &a, char *lds, int wave,
 template <typename U, int PLANES, typename S>
 __global__ void __launch_bounds__(S::kThreads) ce_loss_kernel(CeArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[logit_lds<S>(false)];
-  const int count = a.meta->count;
+  const int count = listed_here(a);
   int64_t ti, tj;
   place_tile(xcd_block(), ceil_div64(a.classes, S::kM), ceil_div64(a.rows, S::kN), 8, ti, tj);
   const int64_t m0 = ti * S::kM, n0 = tj * S::kN;
@@ -567,7 +582,7 @@ __global__ void __launch_bounds__(256) ce_join_kernel(CeArgs a) {
   __shared__ float2 part[16][17];
   const int x = threadIdx.x % 16, y = threadIdx.x / 16;
   const int64_t n = blockIdx.x * int64_t(16) + x;
-  const int count = a.meta->count;
+  const int count = listed_here(a);
   if (blockIdx.x * int64_t(16) >= count) return;
   float most = -INFINITY, sum = 0.0f;
   if (n < count) {
@@ -631,7 +646,7 @@ __global__ void __launch_bounds__(256) ce_total_kernel(CeArgs a, int blocks) {
 template <typename U, int PLANES, typename S>
 __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0) {
   __shared__ __attribute__((aligned(16))) char lds[logit_lds<S>(true)];
-  const int count = a.meta->count;
+  const int count = listed_here(a);
   int64_t ti, tj;
   place_tile(xcd_block(), ceil_div64(min(a.piece, a.classes - v0), S::kM), ceil_div64(a.rows, S::kN), 8,
              ti, tj);
@@ -778,7 +793,7 @@ struct CeShare {
 template <int PLANES, typename S, typename O, bool DX>
 __device__ __forceinline__ void gradient_tile(const CeArgs &a, char *lds, int64_t v0, const CeShare &share,
                                               bool direct, bool add) {
-  const int count = a.meta->count;
+  const int count = listed_here(a);
   const int64_t here = min(a.piece, a.classes - v0), across = DX ? a.rows : here;
   const int64_t at = blockIdx.x - share.first, all = share.tiles * share.splits;
   if (at >= all) return; // between two shares
@@ -859,11 +874,12 @@ __global__ void __launch_bounds__(S::kThreads)
     gradient_tile<PLANES, S, O, false>(a, lds, v0, dw, dw_direct, false);
 }
 
-// The parts' sum, four elements of a row per thread.
+// The parts' sum, four elements of a row per thread; of dw with what the pieces of the rows
+// before gave.
 template <typename O, bool DX>
 __global__ void __launch_bounds__(256) ce_finish_kernel(CeArgs a, int64_t v0, int splits) {
   const int64_t n = blockIdx.z * int64_t(gridDim.y) + blockIdx.y, m = (blockIdx.x * int64_t(256) + threadIdx.x) * 4;
-  const int64_t limit = DX ? a.meta->count : min(a.piece, a.classes - v0);
+  const int64_t limit = DX ? listed_here(a) : min(a.piece, a.classes - v0);
   if (n >= limit || m >= a.dim) return;
   const int64_t part = (DX ? a.rows_pad : a.piece) * a.dim_pad;
   const float *const from = (DX ? a.dx_part : a.dw_part) + n * a.dim_pad + m;
@@ -871,6 +887,17 @@ __global__ void __launch_bounds__(256) ce_finish_kernel(CeArgs a, int64_t v0, in
   for (int s = 0; s < splits; ++s) {
     const float4 p = *reinterpret_cast<const float4 *>(from + s * part);
     v[0] += p.x, v[1] += p.y, v[2] += p.z, v[3] += p.w;
+  }
+  if (!DX && a.dw_sum) {
+    float4 *const held = reinterpret_cast<float4 *>(a.dw_sum + (v0 + n) * a.dim_pad + m);
+    if (a.skip > 0) {
+      const float4 old = *held;
+      v[0] += old.x, v[1] += old.y, v[2] += old.z, v[3] += old.w;
+    }
+    if (!a.last) {
+      *held = make_float4(v[0], v[1], v[2], v[3]);
+      return;
+    }
   }
   const int power = (DX ? a.exponent[n] : a.meta->most) - kShift;
 #pragma unroll
@@ -887,7 +914,7 @@ __global__ void __launch_bounds__(1024) ce_bias_kernel(CeArgs a, int64_t v0, int
   __shared__ float part[64][17];
   const int x = threadIdx.x % 16, y = threadIdx.x / 16;
   const int64_t v = blockIdx.x * int64_t(16) + x;
-  const int64_t chunks = ceil_div64(a.meta->count, tile) * (tile / 64);
+  const int64_t chunks = ceil_div64(listed_here(a), tile) * (tile / 64);
   float s = 0.0f;
 #pragma unroll 8
   for (int64_t c = y; c < chunks; c += 64) s += a.db_part[c * a.piece + v];
@@ -897,13 +924,22 @@ __global__ void __launch_bounds__(1024) ce_bias_kernel(CeArgs a, int64_t v0, int
     if (y < k) part[y][x] += part[y + k][x];
     __syncthreads();
   }
-  if (y == 0 && v0 + v < a.classes) store_typed(a.db, a.bias_type, v0 + v, part[0][x]);
+  if (y != 0 || v0 + v >= a.classes) return;
+  s = part[0][x];
+  if (a.db_sum) {
+    if (a.skip > 0) s += a.db_sum[v0 + v];
+    if (!a.last) {
+      a.db_sum[v0 + v] = s;
+      return;
+    }
+  }
+  store_typed(a.db, a.bias_type, v0 + v, s);
 }
 
 // ---- host --------------------------------------------------------------------------------
 
-constexpr int64_t kPieceBytes = int64_t(512) << 20; // of g in one order, about
-constexpr int64_t kMostRows = (int64_t(1) << 23) - 256; // 256 rows of xt in 32 bits
+constexpr int64_t kPieceBytes = int64_t(512) << 20; // of g in one order, and of operands turned for it
+constexpr int64_t kMostRows = (int64_t(1) << 23) - 256;
 constexpr int64_t kMostClasses = int64_t(1) << 25;
 constexpr int64_t kMostLogits = int64_t(1) << 37; // a launch's threads in 32 bits
 constexpr int64_t kMostFeatures = 65536;
@@ -918,6 +954,7 @@ struct CePlan {
   bool x_direct, w_direct;
   int planes;
   Cut z, dx, dw;
+  int64_t row_piece;
   size_t bytes;
 };
 
@@ -969,18 +1006,23 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
   p.planes = a.type == SPORDER_TYPE_F32 ? 2 : 1;
   p.x_direct = direct_rows(a.type, a.dim, a.x_stride, a.x, a.rows);
   p.w_direct = direct_rows(a.type, a.dim, a.w_stride, a.w, 256);
-  a.rows_pad = ceil_div64(a.rows, 256) * 256;
+  const int64_t rows_pad = ceil_div64(a.rows, 256) * 256; // of all rows
+  a.rows_pad = rows_pad;
   a.dim_pad = ceil_div64(a.dim, kStageK) * kStageK;
   a.piece = ceil_div64(a.classes, 256) * 256;
-  if (backward) {
-    const int64_t most = std::max<int64_t>(1024, kPieceBytes / (a.rows_pad * 2 * p.planes) / 256 * 256);
-    if (a.piece > most) { // pieces of one size
-      const int64_t pieces = ceil_div64(a.piece, most);
-      a.piece = ceil_div64(ceil_div64(a.classes, pieces), 256) * 256;
-    }
+  if (backward) { // pieces of one size, of at least 1,024 classes (or all) and as many rows as that leaves
+    const int64_t elements = kPieceBytes / (2 * p.planes), fewest = std::min<int64_t>(1024, a.piece);
+    auto cut = [](int64_t all, int64_t most) {
+      return ceil_div64(ceil_div64(all, ceil_div64(all, most / 256 * 256)), 256) * 256;
+    };
+    a.rows_pad = cut(a.rows, elements / std::max(fewest, a.dim));
+    a.piece = cut(a.classes, std::max(fewest, elements / std::max(a.rows_pad, a.dim)));
   }
+  p.row_piece = a.rows_pad;
+  const bool cut_rows = p.row_piece < a.rows;
+  const int64_t rows_here = std::min(a.rows, p.row_piece);
   a.classes_pad = ceil_div64(a.classes, a.piece) * a.piece;
-  p.z = cut_logits(std::min(a.piece, a.classes), a.rows);
+  p.z = cut_logits(std::min(a.piece, a.classes), rows_here);
   if (!backward && a.rows <= 64 && p.planes == 1) p.z.shape = 0;
   const int down = p.z.shape == 2 ? Large::kM : Middle::kM; // classes of a tile
   a.chunks = ceil_div64(a.classes, down) * (p.z.shape == 0 ? Narrow::WM : 2);
@@ -992,8 +1034,8 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
   };
   take(a.meta, 1);
   if (a.rows > kListDirect) take(a.counts, ceil_div64(a.rows, kListBlock));
-  take(a.list, a.rows_pad);
-  take(a.target, a.rows_pad);
+  take(a.list, rows_pad);
+  take(a.target, rows_pad);
   take(a.bias32, a.classes_pad);
   if (p.planes == 2) {
     take(a.x_unit, a.rows_pad);
@@ -1006,7 +1048,7 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     a.xp_stride = a.x_stride * 2;
   } else {
     a.xp_stride = row_bytes;
-    a.xp_plane = a.rows * row_bytes;
+    a.xp_plane = rows_here * row_bytes;
     take(a.xp, a.xp_plane * p.planes);
   }
   if (p.w_direct) {
@@ -1022,11 +1064,11 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     take(a.partial, a.chunks * a.rows_pad);
     take(a.sum_parts, 2 * kSumBlocks);
   } else {
-    take(a.exponent, a.rows_pad);
-    take(a.mantissa, a.rows_pad);
-    take(a.row_lse, a.rows_pad);
-    take(a.miss, a.rows_pad);
-    cut_gradients(a.dim, a.rows, std::min(a.piece, a.classes), p.dx, p.dw);
+    take(a.exponent, rows_pad);
+    take(a.mantissa, rows_pad);
+    take(a.row_lse, rows_pad);
+    take(a.miss, rows_pad);
+    cut_gradients(a.dim, rows_here, std::min(a.piece, a.classes), p.dx, p.dw);
     take(a.x_most, a.dim);
     take(a.w_most, a.dim);
     take(a.most_part, 2 * kStrips * a.dim);
@@ -1035,9 +1077,15 @@ CePlan lay_out(CeArgs &a, bool backward, void *work) {
     take(a.g, a.rows_pad * a.piece * 2 * p.planes);
     take(a.gt, a.rows_pad * a.piece * 2 * p.planes);
     if (a.piece < a.classes || p.dx.splits > 1) take(a.dx_part, p.dx.splits * a.rows_pad * a.dim_pad);
-    if (p.dw.splits > 1) take(a.dw_part, p.dw.splits * a.piece * a.dim_pad);
+    if (p.dw.splits > 1 || cut_rows) take(a.dw_part, p.dw.splits * a.piece * a.dim_pad);
     if (a.db) take(a.db_part, a.rows_pad / 64 * a.piece);
+    if (cut_rows) {
+      take(a.dw_sum, a.classes * a.dim_pad);
+      take(a.db_sum, a.classes);
+    }
   }
+  a.rows_pad = rows_pad;
+  a.last = true;
   p.bytes = at;
   return p;
 }
@@ -1053,7 +1101,7 @@ struct Steps {
 
 CeRows rows_of_x(const CeArgs &a) {
   CeRows r{};
-  r.src = a.x, r.stride = a.x_stride, r.rows = a.rows, r.list = a.list, r.most = a.x_most;
+  r.src = a.x, r.stride = a.x_stride, r.rows = a.rows, r.list = a.list, r.skip = a.skip, r.most = a.x_most;
   return r;
 }
 CeRows rows_of_w(const CeArgs &a) {
@@ -1062,12 +1110,23 @@ CeRows rows_of_w(const CeArgs &a) {
   return r;
 }
 
+// A piece of the rows from `skip` on.
+CeArgs piece_of(CeArgs a, const CePlan &p, int64_t skip) {
+  a.last = skip + p.row_piece >= a.rows;
+  a.rows = std::min(p.row_piece, a.rows - skip);
+  a.rows_pad = p.row_piece;
+  a.skip = skip;
+  a.list += skip, a.target += skip, a.exponent += skip, a.mantissa += skip, a.row_lse += skip, a.miss += skip;
+  return a;
+}
+
+// x's rows (of a piece) and, with the first piece, w's.
 template <typename T, typename U, int PLANES> int32_t pack_operands(const CeArgs &a, const CePlan &p, void *stream) {
   CeRows x = rows_of_x(a), w = rows_of_w(a);
   x.out = a.xp, x.out_stride = a.xp_stride, x.plane = a.xp_plane, x.unit = a.x_unit;
   w.out = a.wp, w.out_stride = a.wp_stride, w.plane = a.wp_plane, w.unit = a.w_unit;
   if (!p.x_direct) x.blocks = ceil_div64(a.rows, 4);
-  if (!p.w_direct) w.blocks = ceil_div64(a.classes, 4);
+  if (!p.w_direct && a.skip == 0) w.blocks = ceil_div64(a.classes, 4);
   if (x.blocks + w.blocks == 0) return SPORDER_OK;
   return launch(ce_pack_rows_kernel<T, U, PLANES>, dim3(x.blocks + w.blocks), dim3(256), stream, x, w, a.dim,
                 a.meta);
@@ -1118,32 +1177,20 @@ int32_t finish(const CeArgs &a, int64_t v0, int64_t rows, int splits, void *stre
                 dim3(256), stream, a, v0, splits);
 }
 
-template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, const CePlan &p, void *stream) {
+// The gradients of a piece of the rows.
+template <typename T, typename U, int PLANES> int32_t backward_piece(const CeArgs &a, const CePlan &p, void *stream) {
   Steps steps;
-  steps([&] { return list_rows(a, true, stream); });
   steps([&] { return pack_operands<T, U, PLANES>(a, p, stream); });
   CeRows x = rows_of_x(a), w = rows_of_w(a);
-  const int64_t across = ceil_div64(a.dim, kWave * (16 / sizeof(T)));
-  auto strips = [&](int64_t rows) {
-    return std::min(ceil_div64(rows, 32), std::min<int64_t>(std::max<int64_t>(1024 / across, 64), kStrips));
-  };
-  x.blocks = strips(a.rows), w.blocks = strips(a.classes);
-  steps([&] {
-    const int64_t zeros = std::min<int64_t>(ceil_div64(a.rows, 256), kStrips);
-    return launch(ce_column_most_kernel<T>, dim3(across, x.blocks + w.blocks + zeros), dim3(256), stream, x, w, a,
-                  a.most_part);
-  });
-  steps([&] {
-    return launch(ce_strips_most_kernel, dim3(ceil_div64(a.dim, kWave), 2), dim3(256), stream, a.most_part, x,
-                  w, a.dim);
-  });
   x.out = a.xt, x.out_stride = a.rows_pad * 2, x.plane = a.dim * x.out_stride;
   w.out = a.wt, w.out_stride = a.piece * 2, w.plane = a.dim * w.out_stride;
   x.blocks = ceil_div64(a.rows, 64);
   const bool one_piece = a.piece >= a.classes, dx_direct = one_piece && p.dx.splits == 1;
+  const bool dw_direct = p.dw.splits == 1 && !a.dw_sum;
   for (int64_t v0 = 0; v0 < a.classes; v0 += a.piece) {
     const int64_t here = std::min(a.piece, a.classes - v0);
-    w.src = static_cast<const T *>(a.w) + v0 * a.w_stride, w.rows = here, w.blocks = ceil_div64(here, 64);
+    w.src = static_cast<const T *>(a.w) + v0 * a.w_stride, w.rows = here;
+    w.blocks = one_piece && a.skip > 0 ? 0 : ceil_div64(here, 64); // or there from the rows before
     steps([&] {
       return launch(ce_pack_columns_kernel<T, PLANES>, dim3(x.blocks + w.blocks, ceil_div64(a.dim, 64)), dim3(256),
                     stream, x, w, a.dim, a.meta, a.exponent);
@@ -1170,7 +1217,7 @@ template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, 
       CeShare &one = dx_first ? dx : dw, &two = dx_first ? dw : dx;
       two.first = ceil_div64(one.tiles * one.splits, kXcds) * kXcds;
       return launch(ce_gradients_kernel<PLANES, S, T, O>, dim3(two.first + two.tiles * two.splits),
-                    dim3(S::kThreads), stream, a, v0, dx, dw, dx_direct, v0 > 0, p.dw.splits == 1);
+                    dim3(S::kThreads), stream, a, v0, dx, dw, dx_direct, v0 > 0, dw_direct);
     };
     auto finish_dw = [&](auto kind) {
       return finish<decltype(kind), false>(a, v0, here, p.dw.splits, stream);
@@ -1180,9 +1227,32 @@ template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, 
       if (wide) return p.dx.shape == 2 ? gradients(Large{}, float{}) : gradients(Middle{}, float{});
       return p.dx.shape == 2 ? gradients(Large{}, T{}) : gradients(Middle{}, T{});
     });
-    if (p.dw.splits > 1) steps([&] { return wide ? finish_dw(float{}) : finish_dw(T{}); });
+    if (!dw_direct) steps([&] { return wide ? finish_dw(float{}) : finish_dw(T{}); });
   }
   if (!dx_direct) steps([&] { return finish<T, true>(a, 0, a.rows, p.dx.splits, stream); });
+  return steps.rc;
+}
+
+template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, const CePlan &p, void *stream) {
+  Steps steps;
+  steps([&] { return list_rows(a, true, stream); });
+  CeRows x = rows_of_x(a), w = rows_of_w(a);
+  const int64_t across = ceil_div64(a.dim, kWave * (16 / sizeof(T)));
+  auto strips = [&](int64_t rows) {
+    return std::min(ceil_div64(rows, 32), std::min<int64_t>(std::max<int64_t>(1024 / across, 64), kStrips));
+  };
+  x.blocks = strips(a.rows), w.blocks = strips(a.classes);
+  steps([&] {
+    const int64_t zeros = std::min<int64_t>(ceil_div64(a.rows, 256), kStrips);
+    return launch(ce_column_most_kernel<T>, dim3(across, x.blocks + w.blocks + zeros), dim3(256), stream, x, w, a,
+                  a.most_part);
+  });
+  steps([&] {
+    return launch(ce_strips_most_kernel, dim3(ceil_div64(a.dim, kWave), 2), dim3(256), stream, a.most_part, x,
+                  w, a.dim);
+  });
+  for (int64_t skip = 0; skip < a.rows; skip += p.row_piece)
+    steps([&] { return backward_piece<T, U, PLANES>(piece_of(a, p, skip), p, stream); });
   return steps.rc;
 }
 

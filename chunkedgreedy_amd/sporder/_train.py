@@ -660,8 +660,9 @@ def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignor
             of it for rows that are sure of their target
 
     Returns (dx, dweight, dbias), dbias None without a bias.  The logits are
-    made again, a piece of the classes at a time; rows that are ignored, or
-    whose target is no class, have no gradient.  g = grad (exp(z - lse) -
+    made again, a piece of the rows and classes at a time, so that scratch is at
+    most some 4 GB beside weight packed, its gradient in 32 bits and 40 bytes a
+    row; rows that are ignored, or whose target is no class, have no gradient.  g = grad (exp(z - lse) -
     [target]) keeps 11 bits or more in its products with weight and x (22 for
     float32; nothing below 2^-38 of grad), whose sums are held in 32 bits.  The same call gives the same bits
     from run to run.

@@ -603,6 +603,8 @@ SPORDER_API int32_t sporder_linear_cross_entropy(
  * bias_type).  d_grad has elements grad_stride apart (0: one for all rows); d_lse is the
  * forward call's.  Operands of these products keep 11 bits for 16-bit types (g too) and 22
  * for 32-bit ones, g nothing below 2^-38 of its row's grad; sums are held in 32 bits.
+ * Rows and classes are cut into pieces: whatever the sizes the scratch is at most some 4 GB
+ * beside w packed (where it is of 32 bits or unaligned), dw in 32 bits and 40 bytes a row.
  */
 SPORDER_API size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows,
                                                                 int64_t dim, int64_t classes,

@@ -26,3 +26,29 @@ def test_gradient_of_losses_refuses(lib, bad):  # noqa: F811
     assert result is ctypes.c_int32 and len(kinds) == len(OF_LOSS)
     for loss in (P, 0):
         assert call(lib, name, {**OF_LOSS, "loss": loss, **bad}) == _lib.BAD_ARGUMENT
+
+
+GB = 2**30
+F32 = _lib.TYPE_F32
+
+
+@pytest.mark.parametrize("kind, rows, dim, classes", [
+    (F32, 2_449_029, 128, 193), (F32, 2_449_029, 128, 1000), (F32, 2_449_029, 256, 172),
+    (F32, 580_000, 500, 172), (BF16, 580_000, 500, 172), (F32, 8_000_000, 100, 300),
+    (BF16, 8_000_000, 64, 1000), (BF16, 8_000_000, 65, 1000), (F32, 2**23 - 256, 16, 2**14),
+    (BF16, 2**23 - 256, 8, 2**14), (BF16, 300_000, 4096, 50_000), (F32, 300_000, 4096, 50_000),
+    (F16, 16_384, 4096, 60_000), (BF16, 256, 4096, 131_072), (F32, 100, 65_536, 100_000),
+    (BF16, 2000, 65_536, 200_000), (F32, 131_072, 300, 1000), (F32, 131_073, 300, 1000)])
+def test_scratch_of_the_gradients_is_bounded(lib, kind, rows, dim, classes):  # noqa: F811
+    """Rows and classes are cut into pieces of which g in either order, the packed rows, both
+    turned operands and dx's sums take at most half a GB each (dx's one), and column maxima
+    another half; beside them w packed, dw's sums over the pieces of the rows and some numbers a
+    row and class."""
+    entry = lib.sporder_linear_cross_entropy_grad_work_bytes
+    for at in (P, P + 2):  # 16-bit operands read where they lie, and packed
+        size = entry(kind, rows, dim, classes, dim, at, dim, at)
+        whole = (dim + 63) // 64 * 64
+        limit = 4 * GB + classes * (2 * 4 * whole + 8) + 40 * rows
+        assert 0 < size <= limit, (size / GB, limit / GB)
+        if rows >= 131_072 and classes <= 1000:  # below 2.1 GB however many rows
+            assert size <= 2.1 * GB + 40 * rows, size / GB

@@ -940,6 +940,7 @@ __global__ void __launch_bounds__(1024) ce_bias_kernel(CeArgs a, int64_t v0, int
 
 constexpr int64_t kPieceBytes = int64_t(512) << 20; // of g in one order, and of operands turned for it
 constexpr int64_t kMostRows = (int64_t(1) << 23) - 256;
+constexpr int64_t kMostListed = (int64_t(1) << 31) - 1024;
 constexpr int64_t kMostClasses = int64_t(1) << 25;
 constexpr int64_t kMostLogits = int64_t(1) << 37; // a launch's threads in 32 bits
 constexpr int64_t kMostFeatures = 65536;
@@ -1256,12 +1257,18 @@ template <typename T, typename U, int PLANES> int32_t backward(const CeArgs &a, 
   return steps.rc;
 }
 
-bool bad_sizes(const CeArgs &a, bool backward) {
+// Rows that a call may have, in both directions alike: a training step is refused by its
+// forward call or not at all.  Where the loss takes one pass and the gradients tiles, as many
+// as the list's numbers hold.
+int64_t most_rows(const CeArgs &a) {
+  if (!few_takes(a.type, a.dim, a.classes, false)) return std::min(kMostRows, kMostLogits / a.classes);
+  return few_takes(a.type, a.dim, a.classes, true) ? kMostLogits : kMostListed;
+}
+
+bool bad_sizes(const CeArgs &a) {
   return !type_known(a.type) || !type_known(a.bias_type) || (a.target_bits != 32 && a.target_bits != 64) ||
          a.rows < 0 || a.dim < 1 || a.dim > kMostFeatures || a.classes < 1 || a.classes > kMostClasses ||
-         a.rows > (few_takes(a.type, a.dim, a.classes, backward) ? kMostLogits
-                                                         : std::min(kMostRows, kMostLogits / a.classes)) ||
-         a.x_stride < 0 || a.w_stride < 0;
+         a.rows > most_rows(a) || a.x_stride < 0 || a.w_stride < 0;
 }
 
 template <typename T> __global__ void ce_nothing_kernel(CeArgs a) {
@@ -1290,7 +1297,7 @@ size_t sporder_linear_cross_entropy_work_bytes(int32_t type, int64_t rows, int64
   CeArgs a{};
   a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = 64;
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
-  if (bad_sizes(a, false) || rows == 0) return 0;
+  if (bad_sizes(a) || rows == 0) return 0;
   if (few_takes(type, dim, classes, false)) return few_work_bytes(rows, dim, classes, false);
   if (narrow_takes(type, rows, dim, classes, false)) return narrow_work_bytes(rows, dim, classes, false);
   return lay_out(a, false, nullptr).bytes;
@@ -1307,7 +1314,7 @@ int32_t sporder_linear_cross_entropy(void *stream, int32_t type, int64_t rows, i
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
   a.bias_type = bias_type, a.bias = d_bias, a.targets = d_targets, a.ignore = ignore_index;
   a.loss = d_loss, a.lse = d_lse, a.sums = d_sums;
-  if (bad_sizes(a, false) || !d_sums) return SPORDER_BAD_ARGUMENT;
+  if (bad_sizes(a) || !d_sums) return SPORDER_BAD_ARGUMENT;
   if (rows == 0) return launch(ce_no_rows_kernel, dim3(1), dim3(kWave), stream, a);
   if (!d_x || !d_weight || !d_targets || !d_loss || !d_lse || !d_work || !aligned_to(d_work, 256))
     return SPORDER_BAD_ARGUMENT;
@@ -1332,7 +1339,7 @@ size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows, 
   a.type = type, a.rows = rows, a.dim = dim, a.classes = classes, a.target_bits = 64;
   a.x_stride = x_stride, a.x = d_x, a.w_stride = weight_stride, a.w = d_weight;
   a.db = &a; // the scratch of a bias whether there is one or not
-  if (bad_sizes(a, true) || rows == 0) return 0;
+  if (bad_sizes(a) || rows == 0) return 0;
   if (few_takes(type, dim, classes, true)) return few_work_bytes(rows, dim, classes, true);
   if (narrow_takes(type, rows, dim, classes, true)) return narrow_work_bytes(rows, dim, classes, true);
   return lay_out(a, true, nullptr).bytes;
@@ -1352,7 +1359,7 @@ int32_t sporder_linear_cross_entropy_grad_of_loss(
   a.grad = d_grad, a.grad_stride = grad_stride, a.given_lse = d_lse, a.given_loss = d_loss;
   a.dx = d_dx, a.dx_stride = dx_stride, a.dw = d_dweight, a.dw_stride = dweight_stride;
   a.dw_type = dweight_type, a.db = d_dbias;
-  if (bad_sizes(a, true) || (dweight_type != type && dweight_type != SPORDER_TYPE_F32) || grad_stride < 0 ||
+  if (bad_sizes(a) || (dweight_type != type && dweight_type != SPORDER_TYPE_F32) || grad_stride < 0 ||
       dx_stride < 0 || (rows > 1 && dx_stride < dim) || dweight_stride < 0 ||
       (classes > 1 && dweight_stride < dim) || !d_dweight)
     return SPORDER_BAD_ARGUMENT;

@@ -555,6 +555,15 @@ def residual_norm_grad(grad_y, grad_h, x, y, post_rstd, rstd, gate=None, post_we
     return dx, dresidual, dgate, dpost, dweight
 
 
+def _one_pass(dtype, dim, classes):
+    """Whether the loss takes any number of rows in one pass."""
+    for most, floats, halves in ((48, 512, 512), (64, 384, 512), (96, 256, 512), (128, 192, 384),
+                                 (192, 128, 256)):
+        if classes <= most:
+            return 8 <= dim <= (floats if dtype == torch.float32 else halves)
+    return False
+
+
 def _loss_inputs(x, weight, targets, bias):
     """(x of two dimensions, its stride, weight, its stride, targets, bias)."""
     x = _floats(x, "x")
@@ -583,8 +592,10 @@ def _loss_inputs(x, weight, targets, bias):
         _same_device(bias, x, "bias")
         bias = bias if bias.is_contiguous() else bias.contiguous()
     classes, rows = weight.shape[0], targets.numel()
-    if classes > 2**25 or (classes > 192 and (rows > 2**23 - 256 or rows * classes > 2**37)):
-        raise ValueError("at most 2^25 classes, and past 192 of them 2^23 - 256 rows and 2^37 logits")
+    if classes > 2**25:
+        raise ValueError("at most 2^25 classes")
+    if (rows > 2**23 - 256 or rows * classes > 2**37) and not _one_pass(x.dtype, x.shape[-1], classes):
+        raise ValueError("at most 2^23 - 256 rows and 2^37 logits over so many classes and elements a row")
     x, _, x_stride = _rows(x)
     weight, _, weight_stride = _rows(weight)
     targets = targets if targets.is_contiguous() else targets.contiguous()
@@ -621,8 +632,10 @@ def linear_cross_entropy(x, weight, targets, bias=None, *, ignore_index=-100):
     Returns (loss, lse, sums): loss and lse float32 of the targets' shape (NaN
     for a target that is neither a class nor ignored), sums float32 (2,) of the
     losses' sum and the number of rows that are not ignored.  At most 2^23 - 256
-    rows (more with up to 64 classes of 8 to 256 elements, or 192 of 8 to 64),
-    2^25 classes, 2^37 logits and 65536 elements a row.
+    rows and 2^37 logits (more over up to 48 classes of 8 to 512 elements, 64 of
+    384, 96 of 256, 128 of 192 or 192 of 128; of 16-bit types 96 of 512, 128 of
+    384 or 192 of 256), 2^25 classes and 65536 elements a row.  The gradients
+    take the same sizes.
 
     Sums are held in 32 bits.  float32 products have operands of 22 bits: a term
     is within 2^-21 of itself, and within some 2^-38 of the product of its rows'

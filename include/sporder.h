@@ -580,8 +580,10 @@ SPORDER_API int32_t sporder_residual_norm_grad(
  * targets of target_bits (32 or 64, signed).  A row whose target is ignore_index has loss
  * and lse 0 and is not read; one whose target is no class otherwise has NaN.  d_sums
  * receives the sum of the losses and the number of rows whose target is not ignore_index.
- * dim is at most 65536, classes 2^25, rows 2^23 - 256 and rows times classes 2^37; up to
- * 64 classes of 8 to 256 features, or 192 of 8 to 64, rows are at most 2^37.  d_work is
+ * dim is at most 65536, classes 2^25, rows 2^23 - 256 and rows times classes 2^37.  From 8
+ * features on, rows may be more (2^31 - 1024 at least) over up to 48 classes of 512 features
+ * at most, 64 of 384, 96 of 256, 128 of 192 or 192 of 128; of 16-bit types 96 of 512, 128 of
+ * 384 or 192 of 256.  The gradients take the same sizes.  d_work is
  * 256-byte aligned and of the size that *_work_bytes gives for the same sizes, strides and
  * alignments.
  */
@@ -604,7 +606,8 @@ SPORDER_API int32_t sporder_linear_cross_entropy(
  * forward call's.  Operands of these products keep 11 bits for 16-bit types (g too) and 22
  * for 32-bit ones, g nothing below 2^-38 of its row's grad; sums are held in 32 bits.
  * Rows and classes are cut into pieces: whatever the sizes the scratch is at most some 4 GB
- * beside w packed (where it is of 32 bits or unaligned), dw in 32 bits and 40 bytes a row.
+ * beside w packed (where it is of 32 bits or unaligned), dw in 32 bits, 40 bytes a row and, of up
+ * to 64 rows, 256 bytes a class.
  */
 SPORDER_API size_t sporder_linear_cross_entropy_grad_work_bytes(int32_t type, int64_t rows,
                                                                 int64_t dim, int64_t classes,

@@ -6,7 +6,7 @@ import ctypes
 import pytest
 
 from chunkedgreedy_amd import _lib
-from test_more_entries import COMMON, LOSS_GRAD, P, call, lib  # noqa: F401 (a fixture)
+from test_more_entries import COMMON, LOSS, LOSS_GRAD, P, call, lib  # noqa: F401 (a fixture)
 
 BF16, F16 = _lib.TYPE_BF16, _lib.TYPE_F16
 OF_LOSS = {}
@@ -52,3 +52,32 @@ def test_scratch_of_the_gradients_is_bounded(lib, kind, rows, dim, classes):  # 
         assert 0 < size <= limit, (size / GB, limit / GB)
         if rows >= 131_072 and classes <= 1000:  # below 2.1 GB however many rows
             assert size <= 2.1 * GB + 40 * rows, size / GB
+
+
+SHAPES = [(classes, dim) for classes in (1, 16, 17, 32, 47, 48, 49, 64, 65, 90, 96, 97, 128, 129, 172, 192, 193, 1000)
+          for dim in (7, 8, 64, 100, 128, 129, 192, 193, 256, 257, 384, 385, 512, 513)]
+
+
+@pytest.mark.parametrize("kind", [F32, BF16, F16])
+def test_both_directions_take_the_same_rows(lib, kind):  # noqa: F811
+    """Every number of rows that the forward call takes its gradients take, and the
+    Python check tells which."""
+    import torch
+
+    from chunkedgreedy_amd.sporder import _train
+
+    dtype = {F32: torch.float32, BF16: torch.bfloat16, F16: torch.float16}[kind]
+    for classes, dim in SHAPES:
+        for rows in (2**23 - 256, 2**23 - 255, 10_000_000, 2**31 - 1024, 2**37 // classes, 2**37 // classes + 1):
+            taken = [entry(kind, rows, dim, classes, dim, P, dim, P) > 0 for entry in (
+                lib.sporder_linear_cross_entropy_work_bytes,
+                lib.sporder_linear_cross_entropy_grad_work_bytes)]
+            assert taken[0] == taken[1], (classes, dim, rows)
+            small = rows <= 2**23 - 256 and rows * classes <= 2**37
+            if rows <= 2**31 - 1024:
+                assert taken[0] == (small or _train._one_pass(dtype, dim, classes)), (classes, dim, rows)
+            for name, good in (("sporder_linear_cross_entropy", LOSS), ("sporder_linear_cross_entropy_grad", LOSS_GRAD)):
+                if not taken[0]:
+                    bad = dict(type=kind, rows=rows, dim=dim, classes=classes, x_stride=dim, weight_stride=dim)
+                    more = {"dweight_type": kind, "dx_stride": dim, "dweight_stride": dim} if "dx" in good else {}
+                    assert call(lib, name, {**good, **bad, **more}) == _lib.BAD_ARGUMENT

@@ -113,3 +113,24 @@ def test_pieces_of_the_rows_captured(sporder):
         torch.cuda.synchronize()
         want = run(x * (k + 1) / 2, torch.roll(t, k))
         assert all(torch.equal(p, q) for p, q in zip(out, want))
+
+
+def test_rows_that_only_the_loss_takes_in_one_pass(sporder):
+    """2^23 + 77 rows over 172 classes, whose loss is the one-pass form's and whose gradients
+    are the tiles': the forward call takes them, and so does the backward pass."""
+    rows, dim, classes = 2**23 + 77, 129, 172
+    print(f"[pieces of the rows] {rows} {dim} {classes}", flush=True)
+    x, w, t, b, s = inputs(rows, dim, classes, BF16, F32, 0.1, seed=9)
+    lse = sporder.linear_cross_entropy(x, w, t, b)[1]
+    got = sporder.linear_cross_entropy_grad(s, x, w, t, lse, b, dtype=F32)
+    check_in_blocks(got, x, w, t, b, s, lse, 200_000)
+
+
+def test_rows_refused_by_the_forward_call(sporder):
+    """More rows than the gradients take: the forward call says so."""
+    x = torch.zeros(1, 8, device="cuda").expand(2**23, 8)
+    t = torch.zeros((), device="cuda", dtype=torch.int64).expand(2**23)
+    for classes, dim in ((193, 8), (100, 7)):
+        w = torch.zeros(classes, dim, device="cuda")
+        with pytest.raises(ValueError, match="rows"):
+            sporder.linear_cross_entropy(x[:, :dim], w, t)

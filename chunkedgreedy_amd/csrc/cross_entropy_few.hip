@@ -374,9 +374,8 @@ constexpr int kRows = 32, kSplit = 4; // waves that share a block of 16 rows
 // dx of a tile goes out a tile later, by whole rows through LDS.  (Stored from the
 // accumulators, 64 bytes of 16 rows at a time, it took a third of the kernel's time; stored at
 // the tile's end, the next tile's loads waited for it.)
-// (Past four blocks of features LDS holds one workgroup a CU, which may have all registers.)
 template <typename T, int VB, int DB>
-__global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB < 6 ? 4 : 2) few_grad_kernel(FewArgs a) {
+__global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB < 8 ? 4 : 2) few_grad_kernel(FewArgs a) {
   extern __shared__ __attribute__((aligned(16))) float lds[];
   constexpr int kMine = (VB + kSplit - 1) / kSplit;
   constexpr int kG = VB * 16 + 4;  // floats of a row of g
@@ -402,16 +401,16 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
   __builtin_amdgcn_sched_barrier(0); // loads in the loop's order, so that it waits for no later ones
   fetch_targets<32>(c, first + step, next_target);
   // This lane's row: its class, scale and lse, a tile ahead too.
-  int64_t row = first + tb * 16 + l;
   RawTarget next_class;
-  float next_lse, next_scale;
+  float next_lse, next_loss, next_scale;
   auto fetch_row = [&](int64_t r) {
     next_class = fetch_target(c, r);
     const int64_t in = min(r, c.rows - 1);
     next_lse = c.given_lse[in];
+    next_loss = fetch_loss(c, in);
     next_scale = c.grad[in * c.grad_stride];
   };
-  fetch_row(row);
+  fetch_row(first + tb * 16 + l);
   auto put_dx = [&](int64_t tile) {
     const int64_t r = tile * kRows + threadIdx.x / 16;
     if (r >= c.rows) return;
@@ -429,13 +428,13 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
   for (; tile < a.tiles; tile += gridDim.x) {
     __syncthreads(); // x is read no more, the last tile's dx is there
     put_tile<T, 32>(c, x, target, next);
-    const float loss = fetch_loss(c, min(row, c.rows - 1)); // before the next tile's, to wait for none of them
     __syncthreads();
     classes_of<32>(c, tile * kRows + step, next_target, target);
     fetch_tile<T, 32>(c, tile * kRows + step, target, next);
     fetch_targets<32>(c, tile * kRows + 2 * step, next_target);
+    const int64_t row = tile * kRows + tb * 16 + l; // made anew: registers are short
     const int at = class_of(c, row, next_class);
-    const float lse = at >= 0 ? next_lse : 0.0f, s = next_scale;
+    const float lse = at >= 0 ? next_lse : 0.0f, miss = miss_of(c, next_loss), s = next_scale;
     fetch_row(row + step);
     if (tile != blockIdx.x) put_dx(tile - gridDim.x);
 
@@ -443,7 +442,6 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
     f32x4 z[kMine] = {};
     logits<kMine, kSplit, DB>(w + part * 16 * stride, x + tb * 16 * stride, dim16,
                               (VB - part + kSplit - 1) / kSplit, z);
-    const float miss = miss_of(c, loss);
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int v = (i * kSplit + part) * 16 + q * 4;
@@ -492,7 +490,6 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
         }
       }
     }
-    row += step;
   }
   __syncthreads();
   put_dx(tile - gridDim.x);

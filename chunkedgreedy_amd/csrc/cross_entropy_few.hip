@@ -467,6 +467,7 @@ __global__ void __launch_bounds__(kGradThreads, VB * ((DB + 1) / 2) <= 4 && DB <
         for (int e = 0; e < 4; ++e)
           d = mfma_16x16(w[(v * 16 + q * 4 + e) * stride + j * 16 + l], gv[e], d);
       }
+      if (at < 0) d = f32x4{}; // g is 0, but w may hold anything
       *reinterpret_cast<f32x4 *>(dx + (tb * 16 + l) * stride + j * 16 + q * 4) = d;
     }
     // dw: all classes and every eighth block of features.

@@ -105,7 +105,10 @@ class Dropout(torch.nn.Module):
         if not 0.0 <= p <= 1.0:
             raise ValueError("p must be in [0, 1]")
         self.p = p
-        self.register_buffer("state", torch.tensor([seed, 0], dtype=torch.int64))
+        if not -(2**63) <= seed < 2**64:
+            raise ValueError("seed must be in [0, 2^64)")
+        signed = seed - 2**64 if seed >= 2**63 else seed  # the same 64 bits
+        self.register_buffer("state", torch.tensor([signed, 0], dtype=torch.int64))
 
     def forward(self, x, residual=None):
         out = dropout(x, self.p, self.state, residual=residual, training=self.training)

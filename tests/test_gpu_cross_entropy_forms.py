@@ -82,3 +82,28 @@ def test_tiles_of_a_wave_keep_22_bits(sporder, dim, classes):
         left, xd = g.t().contiguous(), torch.where(on[:, None], xd, torch.zeros_like(xd))
         near(dw, left @ xd, off.t().contiguous() @ xd.abs() + (3001 + 64) * U * (left.abs() @ xd.abs()))
         near(db, g.sum(0), (off + (3001 + 64) * U * g.abs()).sum(0))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_one_scale_of_all_rows_does_not_touch_gs_bits(sporder, dtype):
+    """Tiles of 16-bit types.  Undecided rows over C classes have a g of 1 / C - 1 for their
+    target, which 11 bits hold to 2^-12, whatever the one scale of all rows is: chosen here so
+    that g times its mantissa would lie halfway between two values of 11 bits above 1, 2^-11
+    from each.  Row i's x is the i-th unit vector: column i of w's gradient is g."""
+    rows = 200
+    print(f"[forms] one scale {dtype}", flush=True)
+    x = torch.eye(rows, device="cuda").to(dtype)
+    for classes in (211, 500, 1000, 2001, 5003):
+        w = torch.zeros(classes, rows, device="cuda", dtype=dtype)
+        t = torch.arange(rows, device="cuda") * 7 % classes
+        lse = sporder.linear_cross_entropy(x, w, t)[1]
+        hit = 1.0 - 1.0 / classes
+        for power, sign in ((0, 1), (-9, 1), (5, -1)):
+            scale = sign * 2.0**power * (1.0 + 2.0**-11 - 2.0**-20) / hit
+            s = torch.full((rows,), scale, device="cuda")
+            s[3:5] *= -1  # a scale's sign is no bit of g
+            for grad in (s, torch.tensor(scale, device="cuda")):
+                dw = sporder.linear_cross_entropy_grad(grad, x, w, t, lse, dtype=F32)[1]
+                g = dw[t, torch.arange(rows, device="cuda")].double() / grad.double()
+                # Beside the 11 bits: lse's rounding and the scale's, u of 9 and of g.
+                assert ((g + hit).abs() <= 2.0**-12 + 16 * U).all()

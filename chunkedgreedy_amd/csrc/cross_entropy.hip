@@ -652,8 +652,8 @@ __global__ void __launch_bounds__(256) ce_total_kernel(CeArgs a, int blocks) {
 // ---- gradients ---------------------------------------------------------------------------
 
 // g of a tile in both orders, each turned in LDS and written by whole rows.  Half of the classes
-// above in 851 us (0.89 PFLOP/s, and 820 MB written: 144 us that no other tile's products cover,
-// for two tiles' accumulators don't fit the registers).
+// above in 860 us (0.88 PFLOP/s, and 745 MB written in the two orders: 131 us at a copy's rate that
+// no other tile's products cover, for two tiles' accumulators don't fit the registers).
 template <typename U, int PLANES, typename S>
 __global__ void __launch_bounds__(S::kThreads) ce_g_kernel(CeArgs a, int64_t v0) {
   __shared__ __attribute__((aligned(16))) char lds[logit_lds<S>(true)];

@@ -129,9 +129,10 @@ __device__ __forceinline__ void logits(const float *w, const float *rows, int di
 // they are, 32-bit ones as two 16-bit halves of their row's unit, three products for each
 // (22 bits).  An access that would pass the row's end is the row's last one, and w's copy in
 // LDS has those features there, each once, and zeros: nothing of x is moved or masked.
-// Bound by memory: 2,449,029 rows of 128, 47 classes in 306 us (4.2 TB/s; 32-bit products from
+// 2,449,029 rows of 128, 47 classes in 280 to 306 us (4.2 to 4.5 TB/s; 32-bit products from
 // tiles in LDS took 482), bfloat16 140 (4.8 TB/s; 430); 580,000 rows of 500, 80 classes, bfloat16
-// 130 us (tiles of any number of classes: 464).
+// 130 us (tiles of any number of classes: 464).  What keeps it from a copy's rate are the address
+// units, busy 81 % of the time (bfloat16 77 %): an access of a wave lies in 16 rows.
 template <typename T> struct LossType {
   using U = T;
   static constexpr int kPlanes = 1;

@@ -10,8 +10,11 @@
 // which elements those are is free as long as both operands agree, and so is the order of
 // rows.  So a lane's eight neighbouring elements serve eight instructions, and where
 // features lie across lanes, four neighbouring ones serve four blocks of 32.
-// Bound by memory for 32-bit types (50,000 x 2,048 floats of w, 16 rows), for 16-bit ones
-// by the 32-bit products.
+// Not at memory's rate: one row over 50,000 x 4,096 floats in 240 us (3.4 TB/s; a copy reaches 5.7),
+// for an access of a wave takes 64 bytes of 32 rows of w each, two to four accesses ahead; from some
+// 32 rows on, and in 16-bit types from the first, the 32-bit products take as long (64 rows over
+// 30,000 x 4,096 floats 298 us, of which the products are worth 102; one row over 50,000 x 4,096
+// bfloat16 with its gradients 479 us, its bytes 144).
 #include <algorithm>
 
 #include "cross_entropy.hpp"
@@ -371,7 +374,7 @@ template <typename T> int32_t narrow_typed(const NarrowArgs &a, bool backward, v
 // types, whose w the tiles read as it is: forward 164 and 106 us for one row of the first, 156
 // and 65 for 64, but 35 and 37 for up to 32 rows of 16,000 x 2,048 and 24 and 28 of 1,000 x 512
 // (three launches instead of five); with the gradients 491 and 812, 16 rows of 50,000 x 2,048
-// 268 and 443, but 64 rows 627 and 531.
+// 268 and 443, but 64 rows 627 and 380.
 bool narrow_takes(int type, int64_t rows, int64_t dim, int64_t classes, bool backward) {
   if (dim < 8) return false;
   if (type == SPORDER_TYPE_F32) return rows <= 64;

@@ -89,6 +89,9 @@ __device__ __forceinline__ void put_row(T *p, int64_t dim, int lane, const float
 
 // A row per L lanes, held in registers between its read and both outputs' writes: 16,384
 // rows of 4,096 bfloat16 with a residual in 99 us (5.4 TB/s), by torch operations 1,242.
+// Loose accesses of 16-bit elements: 97,560 rows of 1,025 in 258 us (3.1 TB/s) where 1,024 take 149,
+// with 85 million turns of the first-level caches for 13 million; rows of 100 and 101 in 278 and
+// 311, the address units busy 89 % of the time.
 template <typename T, bool LOOSE, int VEC, int L, int C>
 __global__ void __launch_bounds__(norm_block(L)) block_norm_kernel(BlockArgs a) {
   constexpr int kGroups = norm_block(L) / L;
@@ -211,7 +214,7 @@ template <typename T> __global__ void __launch_bounds__(1024) block_norm_long_ke
 
 // 2,449,029 rows of 128 floats in 1,472 us (5.1 TB/s), 16,384 of 4,096 bfloat16 with a gate by
 // row in 211 (5.1 TB/s); rows of 16-bit elements of odd length, whose accesses are loose, 1.8 to
-// 2.7 TB/s.
+// 3.4 TB/s (such an access takes the caches six times as many turns; below).
 // The gradients by element, and the workgroup's sums over its rows by column,
 // kept in registers and written as one row of partial sums at the end.  No
 // atomics: the order of every sum is fixed by the grid.

@@ -1,6 +1,7 @@
 """Operators of a training step around the SpMM: row lookup, layer norm, the
 orthogonalisation of a weight's update, dropout, the norms around a block and
-the cross entropy of linear logits, each with what its backward pass needs.  They have no counterpart in the reference.
+the cross entropy of linear logits, each with what its backward pass needs.
+They have no counterpart in the reference.
 
 Unlike the rest of the package they run on torch's current stream of the
 input's device and return without waiting, so they follow and precede torch
@@ -478,7 +479,10 @@ def residual_norm(x, residual=None, gate=None, post_weight=None, weight=None, *,
     Returns (y, h, post_rstd, rstd): y, the new residual stream, and h, the next
     block's input, of x's shape and type; post_rstd and rstd are float32 of
     shape x.shape[:-1], as :func:`residual_norm_grad` takes them.  Sums are held
-    in 32 bits, and h is made of y before its rounding.
+    in 32 bits, and h is made of y before its rounding.  So are squares: a row of
+    x whose elements pass some 1e19 has an infinite mean square and adds nothing
+    to y, a row of y that passes it has an h of 0; with an eps of 0 rows below some
+    1e-19 have none.
     """
     x = _floats(x, "x")
     gate, post_weight, weight, kind, by_row = _block_inputs(x, gate, post_weight, weight, post_norm)
@@ -639,7 +643,8 @@ def linear_cross_entropy(x, weight, targets, bias=None, *, ignore_index=-100):
 
     Sums are held in 32 bits.  float32 products have operands of 22 bits: a term
     is within 2^-21 of itself, and within some 2^-38 of the product of its rows'
-    largest elements; a row that holds an infinity gives NaN.
+    largest elements; a row that holds an infinity gives NaN, and elements past
+    some 1e33 may pass 32 bits on the way.
     """
     x, x_stride, weight, weight_stride, targets, bias = _loss_inputs(x, weight, targets, bias)
     ignore_index = _ignored(ignore_index)
@@ -677,7 +682,9 @@ def linear_cross_entropy_grad(grad, x, weight, targets, lse, bias=None, *, ignor
     most some 4 GB beside weight packed, its gradient in 32 bits and 40 bytes a
     row; rows that are ignored, or whose target is no class, have no gradient.  g = grad (exp(z - lse) -
     [target]) keeps 11 bits or more in its products with weight and x (22 for
-    float32; nothing below 2^-38 of grad), whose sums are held in 32 bits.  The same call gives the same bits
+    float32; nothing below 2^-38 of grad), weight's and x's elements nothing
+    below 2^-40 of their column's largest, in dweight times the largest grad;
+    sums are held in 32 bits.  The same call gives the same bits
     from run to run.
     """
     x, x_stride, weight, weight_stride, targets, bias = _loss_inputs(x, weight, targets, bias)

@@ -546,8 +546,8 @@ SPORDER_API int32_t sporder_dropout(void *stream, int32_t type, int64_t rows, in
  * for each of `rows` rows of `dim` elements of `type`; without post_norm, post_rstd is 1
  * (and there is no post_weight).  d_residual (0), d_gate, d_post_weight and d_weight (1) may
  * be NULL; the weights have dim elements of vector_type, and so has the gate, or it is of
- * `type` with rows of its own (gate_by_row).  h is made of y before its rounding.  Outputs
- * do not overlap inputs.
+ * `type` with rows of its own (gate_by_row).  h is made of y before its rounding.  Squares
+ * and sums are held in 32 bits (elements up to some 1e19).  Outputs do not overlap inputs.
  */
 SPORDER_API int32_t sporder_residual_norm(
     void *stream, int32_t type, int32_t vector_type, int64_t rows, int64_t dim, int64_t x_stride,
@@ -604,7 +604,8 @@ SPORDER_API int32_t sporder_linear_cross_entropy(
  * dweight_type: `type` or SPORDER_TYPE_F32) and, where not NULL, d_dbias = sum_t g (of
  * bias_type).  d_grad has elements grad_stride apart (0: one for all rows); d_lse is the
  * forward call's.  Operands of these products keep 11 bits for 16-bit types (g too) and 22
- * for 32-bit ones, g nothing below 2^-38 of its row's grad; sums are held in 32 bits.
+ * for 32-bit ones, g nothing below 2^-38 of its row's grad, w and x nothing below 2^-40
+ * of their column's largest element (in dw times the largest grad); sums are held in 32 bits.
  * Rows and classes are cut into pieces: whatever the sizes the scratch is at most some 4 GB
  * beside w packed (where it is of 32 bits or unaligned), dw in 32 bits, 40 bytes a row and, of up
  * to 64 rows, 256 bytes a class.
